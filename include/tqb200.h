@@ -173,6 +173,60 @@ int32_t tq_append(tq_ctx* ctx, int32_t layer, int32_t seq_begin, int32_t seq_cou
 int32_t tq_decode(tq_ctx* ctx, int32_t layer, const void* q, int32_t q_dtype, float* out,
                   void* stream);
 
+/* Queries of one token or of many per sequence, attended on the codes with the causal mask, a sliding
+ * window and first tokens that stay visible: what tq_decode is for one new token over everything stored.
+ * (The reference answers such queries on its dense getters, hf_cache.py:196-205.)
+ *
+ * Sequence s of the call holds N tokens, the newest n of which (n = q_lens[s], or n_tokens) are the queries'
+ * own: query token i < n stands at position p = N - n + i and sees the tokens j <= p with j < sinks or
+ * j > p - window.  Rows that see nothing (i >= n, p < 0, an empty sequence) become zeros. */
+typedef struct tq_attend_args {
+  const void* q;            /* device: element (s, i, head, d) at s * q_seq_stride + i * q_tok_stride +
+                             * head * q_head_stride + d (strides in elements)                        */
+  void* out;                /* device, [seq_count][n_tokens][n_q_heads][D] of q_dtype; aligned to 16   */
+  const int32_t* q_lens;    /* device, [seq_count], values below 0 and above n_tokens count as these;
+                             * null: n_tokens each                                                 */
+  void* workspace;          /* device, 256-byte aligned, as tq_attend_workspace asks for            */
+  size_t workspace_bytes;
+  int64_t q_seq_stride, q_tok_stride, q_head_stride;
+  int32_t layer, seq_begin, seq_count, n_tokens;
+  int32_t q_dtype;          /* TQ_*: of q and out                                                  */
+  int32_t window;           /* tokens a query sees, itself among them; 0: no window                 */
+  int32_t sinks;            /* first tokens that stay visible                                      */
+  int32_t reserved_;
+} tq_attend_args;
+
+/* Bytes of workspace that tq_attend wants for these arguments (pointers are not looked at), on this stream: a
+ * captured call asks for what the capacity of the sequences may need, since it may be replayed on longer
+ * ones.  A call may be given less, down to what one sequence needs; it then takes several rounds. */
+int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* args, void* stream, size_t* bytes);
+int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* args, void* stream);
+
+/* Root-mean-square norm of every query and key head and their rotation by position, in one pass: what stands
+ * between a layer's projections and tq_append / tq_attend.
+ *   y = x / sqrt(mean(x^2) + eps) * weight   where a weight is given, else x
+ *   channels i and i + rotary_dim / 2 turn by position * inv_freq[i]; those from rotary_dim on do not
+ * (rotate-half layout, as per_channel_kv.py:243-267 turns the key bias).  Angles are reduced in 64 bits, the
+ * rest is float32, rounded once.  An output may be its own input where that is contiguous. */
+typedef struct tq_rope {
+  const void *q, *k;        /* device: element (s, t, head, d), strides in elements, as in tq_append  */
+  void *q_out, *k_out;      /* device, contiguous [n_seqs][n_tokens][heads][128]                     */
+  const void *q_weight, *k_weight; /* device, [128] of weight_dtype; null: that tensor is not normed  */
+  const float* inv_freq;    /* device, [rotary_dim / 2]                                            */
+  const void* positions;    /* device, integers of pos_bits bits (32, 64)                          */
+  int64_t q_seq_stride, q_tok_stride, q_head_stride;
+  int64_t k_seq_stride, k_tok_stride, k_head_stride;
+  int64_t pos_seq_stride, pos_tok_stride;
+  int32_t n_seqs, n_tokens, n_q_heads, n_kv_heads;
+  int32_t dtype, weight_dtype, pos_bits, rotary_dim; /* rotary_dim: a multiple of 8, at most 128      */
+  float eps;
+  int32_t reserved_;
+} tq_rope;
+int32_t tq_norm_rope(const tq_rope* rope, int32_t device, void* stream);
+/* The same for tokens that are about to be appended to sequences seq_begin .. of a layer: their positions
+ * follow from the lengths on the device (rope->positions is not looked at). */
+int32_t tq_ctx_norm_rope(tq_ctx* ctx, int32_t layer, int32_t seq_begin, const tq_rope* rope, void* stream);
+
 /* Sequence-split form of tq_decode for one long sequence spread over several devices:
  * attends only cold blocks [block_begin, block_end) and, if `with_hot` is non-zero, the
  * hot window, and writes the un-normalised state (m, l, o[D]) per query head to

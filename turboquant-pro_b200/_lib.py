@@ -53,6 +53,27 @@ class TqBuffers(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in REGIONS]
 
 
+class TqAttendArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("q_lens", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t), ("q_seq_stride", C.c_int64), ("q_tok_stride", C.c_int64),
+        ("q_head_stride", C.c_int64), ("layer", C.c_int32), ("seq_begin", C.c_int32),
+        ("seq_count", C.c_int32), ("n_tokens", C.c_int32), ("q_dtype", C.c_int32),
+        ("window", C.c_int32), ("sinks", C.c_int32), ("reserved_", C.c_int32),
+    ]
+
+
+class TqRope(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_weight", "k_weight", "inv_freq",
+                                          "positions")] + [
+        (n, C.c_int64) for n in ("q_seq_stride", "q_tok_stride", "q_head_stride", "k_seq_stride",
+                                 "k_tok_stride", "k_head_stride", "pos_seq_stride",
+                                 "pos_tok_stride")] + [
+        (n, C.c_int32) for n in ("n_seqs", "n_tokens", "n_q_heads", "n_kv_heads", "dtype",
+                                 "weight_dtype", "pos_bits", "rotary_dim")] + [
+        ("eps", C.c_float), ("reserved_", C.c_int32)]
+
+
 # every exported symbol of include/tqb200.h with its signature
 SIGNATURES = {
     "tq_version": (C.c_int32, []),
@@ -70,6 +91,12 @@ SIGNATURES = {
                               C.c_void_p]),
     "tq_decode_static_scratch": (C.c_int32, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32,
                                              C.c_void_p, C.c_void_p]),
+    "tq_attend_workspace": (C.c_int32, [C.c_void_p, C.POINTER(TqAttendArgs), C.c_void_p,
+                                        C.POINTER(C.c_size_t)]),
+    "tq_attend": (C.c_int32, [C.c_void_p, C.POINTER(TqAttendArgs), C.c_void_p]),
+    "tq_norm_rope": (C.c_int32, [C.POINTER(TqRope), C.c_int32, C.c_void_p]),
+    "tq_ctx_norm_rope": (C.c_int32, [C.c_void_p, C.c_int32, C.c_int32, C.POINTER(TqRope),
+                                     C.c_void_p]),
     "tq_decode_partial": (C.c_int32, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32,
                                       C.c_int32, C.c_int32, C.c_void_p, C.c_void_p]),
     "tq_lse_combine": (C.c_int32, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,

@@ -346,13 +346,15 @@ class TurboQuantKVCache:
         return self._range(start, end, False)
 
     # --------------------------------------------------------------------- decode ----
-    def fused_decode(self, query, method: str = "warp"):
+    def fused_decode(self, query, method: str = "warp", *, window: int | None = None,
+                     sinks: int = 0):
         """One decode-step attention output over the whole cache, computed on the codes.
 
         ``query``: ``(n_q_heads, head_dim)`` or ``(1, n_q_heads, 1, head_dim)``; returns
         ``(n_q_heads, head_dim)`` float32 — a numpy array for numpy input, a CUDA tensor
         for tensor input.  Unlike the reference (``core.py:1193``) it does not require
-        ``key_bits == value_bits``.
+        ``key_bits == value_bits``.  With ``window`` only the newest ``window`` tokens and the
+        first ``sinks`` ones are attended (:meth:`KVContext.attend`).
         """
         import torch
 
@@ -364,7 +366,10 @@ class TurboQuantKVCache:
         q = q.reshape(1, hq, self.head_dim).to(self._ctx.device)
         if q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             q = q.float()
-        out = self._ctx.decode(0, q)[0]
+        if window is None:
+            out = self._ctx.decode(0, q)[0]
+        else:
+            out = self._ctx.attend(0, q[:, None].float(), window, sinks)[0, 0]
         return out.cpu().numpy() if is_np else out
 
     # ---------------------------------------------------------------------- stats ----

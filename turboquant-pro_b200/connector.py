@@ -225,10 +225,13 @@ class DeviceBlockStore:
         kv_layer[1][blk, row] = v.permute(1, 0, 2).to(kv_layer.dtype)
         return n
 
-    def attend(self, layer_name: str | int, queries: dict):
+    def attend(self, layer_name: str | int, queries: dict, window: int | None = None,
+               sinks: int = 0):
         """One decode step on the codes for several stored requests of one layer:
         ``queries`` maps request id -> ``(n_q_heads, D)`` query; returns request id ->
-        ``(n_q_heads, D)`` float32 output.  Requests the store does not hold are left out."""
+        ``(n_q_heads, D)`` float32 output.  Requests the store does not hold are left out.  With
+        ``window`` only the newest ``window`` tokens of a request and its first ``sinks`` ones
+        are attended."""
         import torch
 
         layer = self.layer_index(layer_name)
@@ -243,7 +246,8 @@ class DeviceBlockStore:
                 held[rid] = slot
         if not held:
             return {}
-        out = self.ctx.decode(layer, q)
+        out = self.ctx.decode(layer, q) if window is None else \
+            self.ctx.attend(layer, q[:, None], window, sinks)[:, 0]
         return {rid: out[slot] for rid, slot in held.items()}
 
     # ------------------------------------------------------------ eviction, hand-off ----

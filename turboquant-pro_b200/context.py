@@ -21,7 +21,7 @@ import math
 import numpy as np
 
 from . import _lib
-from ._lib import REGIONS, TqBuffers, TqGeom, TqSizes, check
+from ._lib import REGIONS, TqAttendArgs, TqBuffers, TqGeom, TqSizes, check
 
 _NO_GUARD = contextlib.nullcontext()
 
@@ -280,6 +280,95 @@ class KVContext:
         if check_status:
             self.raise_on_timeout()
         return out
+
+    def attend(self, layer: int, q, window: int | None = None, sinks: int = 0, q_lens=None,
+               seq_begin: int = 0, out=None):
+        """Attention of one or many query tokens per sequence on the codes, with the causal mask, a
+        sliding window and first tokens that stay visible.
+
+        ``q``: CUDA tensor ``[n_seqs', T, n_q_heads, D]`` (float32 / float16 / bfloat16, any strides
+        with contiguous channels) for ``n_seqs'`` consecutive sequences from ``seq_begin``; the queries
+        of a sequence belong to its newest ``T`` tokens (append those first), or to its newest
+        ``q_lens[s]`` ones, whose rows then come first (``q_lens``: int32 CUDA tensor
+        ``[n_seqs']``, values beyond ``0 .. T`` count as these).  A token at position ``p`` sees the tokens
+        ``j <= p`` with ``j > p - window`` or ``j < sinks`` (``window=None``: all of them).  Returns
+        ``[n_seqs', T, n_q_heads, D]`` of ``q``'s type; rows that see nothing (padding, queries
+        before the first token, empty sequences) are zeros.  Inference only: no gradients.
+        """
+        torch = _torch()
+        g = self.geom
+        if q.dim() != 4 or tuple(q.shape[2:]) != (g.n_q_heads, g.head_dim):
+            raise ValueError(f"expected q of shape [n_seqs, T, {g.n_q_heads}, {g.head_dim}], "
+                             f"got {tuple(q.shape)}")
+        if q.device != self.device:
+            raise ValueError(f"q lives on {q.device}, the context on {self.device}")
+        if q.dtype not in _dtype_codes():
+            raise ValueError(f"q must be float32, float16 or bfloat16, got {q.dtype}")
+        if q.requires_grad and torch.is_grad_enabled():
+            raise ValueError("attention on the codes has no backward pass: call it under torch.no_grad()")
+        if window is not None and window < 1:
+            raise ValueError(f"window must be at least 1 (or None), got {window}")
+        if sinks < 0:
+            raise ValueError(f"sinks must not be negative, got {sinks}")
+        if q_lens is not None and (q_lens.dtype != torch.int32 or q_lens.device != self.device
+                                   or tuple(q_lens.shape) != (q.shape[0],)):
+            raise ValueError(f"q_lens must be an int32 tensor of shape ({q.shape[0]},) on {self.device}")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device \
+                or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)} "
+                             f"on {self.device}, aligned to 16 bytes")
+        step = 16 // q.element_size()
+        if q.numel() and (q.stride(3) != 1 or q.data_ptr() % 16 or any(s % step for s in q.stride()[:3])):
+            q = q.contiguous() if not q.is_contiguous() else q.clone()
+        if q_lens is not None:
+            q_lens = q_lens.contiguous()
+        a = TqAttendArgs()
+        a.q, a.out = q.data_ptr(), out.data_ptr()
+        a.q_lens = q_lens.data_ptr() if q_lens is not None else None
+        a.q_seq_stride, a.q_tok_stride, a.q_head_stride = q.stride()[:3]
+        a.layer, a.seq_begin, a.seq_count, a.n_tokens = layer, seq_begin, q.shape[0], q.shape[1]
+        a.q_dtype = _dtype_code(q.dtype)
+        a.window, a.sinks = min(window or 0, 2**31 - 1), min(sinks, 2**31 - 1)
+        with self._here():
+            stream = self._stream()
+            size = C.c_size_t()
+            check(self._lib.tq_attend_workspace(self._h, C.byref(a), stream, C.byref(size)))
+            work = torch.empty(size.value, dtype=torch.uint8, device=self.device)
+            a.workspace, a.workspace_bytes = work.data_ptr(), size.value
+            check(self._lib.tq_attend(self._h, C.byref(a), stream))
+        return out
+
+    def norm_rope(self, layer: int, q, k, inv_freq, positions=None, *, q_weight=None, k_weight=None,
+                  eps: float = 1e-6, seq_begin: int = 0):
+        """:func:`~turboquant_pro_b200.norm_rope` of the tokens that sequences ``seq_begin`` .. of
+        ``layer`` get next: without ``positions`` they follow what is stored (read on the device, so
+        a captured step stays right as the sequences grow).  ``q`` ``[n_seqs', T, n_q_heads, D]``,
+        ``k`` ``[n_seqs', T, n_kv_heads, D]``."""
+        from .rotary import _norm_rope
+
+        g = self.geom
+        if q.dim() != 4 or k.dim() != 4 or q.shape[2] != g.n_q_heads or k.shape[2] != g.n_kv_heads:
+            raise ValueError(f"expected q [n_seqs, T, {g.n_q_heads}, D] and k [n_seqs, T, "
+                             f"{g.n_kv_heads}, D], got {tuple(q.shape)} and {tuple(k.shape)}")
+        if q.device != self.device:
+            raise ValueError(f"q lives on {q.device}, the context on {self.device}")
+        return _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps,
+                          (self, layer, seq_begin))
+
+    def step(self, layer: int, q, k, v, inv_freq, *, q_weight=None, k_weight=None, eps: float = 1e-6,
+             window: int | None = None, sinks: int = 0, seq_begin: int = 0):
+        """One layer's attention for new tokens, from its projections to its output: :meth:`norm_rope`
+        at the positions that follow, :meth:`append`, :meth:`attend`.  ``q`` ``[n_seqs', T, n_q_heads,
+        D]``, ``k`` / ``v`` ``[n_seqs', T, n_kv_heads, D]``; prompts, chunks of them and single
+        tokens alike."""
+        if v.dim() != 4 or v.shape != k.shape:
+            raise ValueError(f"k and v differ in shape: {tuple(k.shape)} and {tuple(v.shape)}")
+        q, k = self.norm_rope(layer, q, k, inv_freq, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                              seq_begin=seq_begin)
+        self.append(layer, k, v, seq_begin)
+        return self.attend(layer, q, window, sinks, seq_begin=seq_begin)
 
     def raise_on_timeout(self) -> int:
         """Reads the status word (synchronises); raises if a bounded wait of a kernel ran out since

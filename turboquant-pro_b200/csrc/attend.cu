@@ -1,0 +1,130 @@
+// tq_attend: checks, the choice of a form, the division of the work, the workspace.
+#include <algorithm>
+
+#include "attend.cuh"
+
+namespace {
+
+constexpr size_t AT_ONE_GO = (size_t)1 << 30;  // workspace that a call asks for at most, unless one
+                                               // sequence needs more
+
+struct Plan {
+  int ns_cold, ns_hot;
+  size_t seq_bytes;  // workspace of a sequence
+};
+
+int check_args(const tq_ctx* ctx, const tq_attend_args* r) {
+  TQ_REQUIRE(ctx != nullptr && r != nullptr, TQ_ERR_INVALID, "null argument");
+  const tq_geom& g = ctx->g;
+  TQ_REQUIRE(r->layer >= 0 && r->layer < g.n_layers, TQ_ERR_INVALID, "bad layer");
+  TQ_REQUIRE(r->seq_begin >= 0 && r->seq_count >= 0 && (int64_t)r->seq_begin + r->seq_count <= g.n_seqs,
+             TQ_ERR_INVALID, "sequence range out of bounds");
+  TQ_REQUIRE(r->n_tokens >= 0 && (int64_t)r->n_tokens * g.group <= (1 << 30), TQ_ERR_INVALID,
+             "n_tokens out of range");
+  TQ_REQUIRE(r->window >= 0 && r->sinks >= 0, TQ_ERR_INVALID, "window and sinks must not be negative");
+  TQ_REQUIRE(r->q_dtype == TQ_F32 || r->q_dtype == TQ_F16 || r->q_dtype == TQ_BF16, TQ_ERR_INVALID,
+             "bad q_dtype");
+  return TQ_OK;
+}
+
+// The most tokens a sequence of the call may hold when the kernels run: the host's lengths, or the
+// capacity where the launch is captured, since a replay may find longer sequences.
+int most_tokens(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone)
+    return ctx->g.max_tokens_per_seq;
+  int n = 0;
+  for (int s = r->seq_begin; s < r->seq_begin + r->seq_count; ++s)
+    n = std::max(n, ctx->len[(size_t)r->layer * ctx->g.n_seqs + s]);
+  return n;
+}
+
+// Splits of the tokens: enough CTAs for the GPU, of what is visible in the longest sequence, in blocks and in
+// the window (a tile of either counts the same).
+Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
+  const tq_geom& g = ctx->g;
+  const int n = most_tokens(ctx, r, st), rows = r->n_tokens * g.group;
+  const int nb = n_cold_blocks(n, g.hot_window, g.block_tokens);
+  const int64_t seen = r->window == 0 ? n : std::min<int64_t>(n, (int64_t)r->window + r->n_tokens + r->sinks + 128);
+  const int64_t hot_tokens = std::min<int64_t>(g.hot_window, n);
+  const int64_t cold = nb > 0 ? std::max<int64_t>(seen - (n - (int64_t)nb * g.block_tokens), 1) : 0;
+  const int64_t cold_tiles = (cold + 63) / 64, hot_tiles = (hot_tokens + 63) / 64;
+  const int row_tile = rows <= 16 ? 16 : 64, per_sm = rows <= 16 ? 2 : 1;
+  const int64_t ctas = (int64_t)r->seq_count * g.n_kv_heads * ((rows + row_tile - 1) / row_tile);
+  int sm_count = 148;
+  cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, ctx->device);
+  const int64_t want = std::min<int64_t>(
+      std::max<int64_t>((2 * per_sm * sm_count + ctas - 1) / std::max<int64_t>(ctas, 1), 1), 64);
+  const int64_t all = std::max<int64_t>(cold_tiles + hot_tiles, 1), each = (all + want - 1) / want;
+  Plan p;
+  p.ns_cold = (int)((cold_tiles + each - 1) / each);
+  p.ns_hot = (int)std::max<int64_t>((hot_tiles + each - 1) / each, 1);
+  // (the kernels go by the lengths on the device: blocks always have a split where there can be any)
+  if (p.ns_cold == 0 && n_cold_blocks(g.max_tokens_per_seq, g.hot_window, g.block_tokens) > 0) p.ns_cold = 1;
+  p.seq_bytes = (size_t)g.n_kv_heads * rows * (p.ns_cold + p.ns_hot) * TQ_PART_STRIDE * 4;
+  return p;
+}
+
+}  // namespace
+
+extern "C" int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* r, void* stream, size_t* bytes) {
+  const int rc = check_args(ctx, r);
+  if (rc != TQ_OK) return rc;
+  TQ_REQUIRE(bytes != nullptr, TQ_ERR_INVALID, "null argument");
+  const Plan p = make_plan(ctx, r, (cudaStream_t)stream);
+  const size_t n = std::max<size_t>(AT_ONE_GO / std::max<size_t>(p.seq_bytes, 1), 1);
+  *bytes = align_up(std::min<size_t>(n, r->seq_count) * p.seq_bytes, 256);
+  return TQ_OK;
+}
+
+extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream) {
+  int rc = check_args(ctx, r);
+  if (rc != TQ_OK) return rc;
+  if (r->seq_count == 0 || r->n_tokens == 0) return TQ_OK;
+  const tq_geom& g = ctx->g;
+  TQ_REQUIRE(r->q != nullptr && r->out != nullptr, TQ_ERR_INVALID, "q and out must be device pointers");
+  TQ_REQUIRE(r->workspace != nullptr && (uintptr_t)r->workspace % 256 == 0, TQ_ERR_INVALID,
+             "workspace must be a device pointer aligned to 256 bytes");
+  TQ_CUDA(cudaSetDevice(ctx->device));
+  cudaStream_t st = (cudaStream_t)stream;
+  const Plan p = make_plan(ctx, r, st);
+  TQ_REQUIRE(r->workspace_bytes >= p.seq_bytes, TQ_ERR_CAPACITY,
+             "workspace smaller than tq_attend_workspace asked for");
+  const int at_once = (int)std::min<size_t>(r->workspace_bytes / p.seq_bytes, r->seq_count);
+
+  AttendArgs a = {};
+  a.g = g;
+  a.pages = (const uint8_t*)ctx->b.pages;
+  a.hot_k = ctx->b.hot_k;
+  a.hot_v = ctx->b.hot_v;
+  a.pool_dec = (const uint32_t*)ctx->b.pool_dec;
+  a.pool_val = (const uint16_t*)ctx->b.pool_val;
+  a.page_meta = (const PageMeta*)ctx->b.page_meta;
+  a.seq_len = (const int32_t*)((const uint8_t*)ctx->b.state + state_len_off(g));
+  a.status = (int32_t*)((uint8_t*)ctx->b.state + state_status_off(g));
+  a.tables = (const Tables*)ctx->b.tables;
+  a.q_seq = r->q_seq_stride, a.q_tok = r->q_tok_stride, a.q_head = r->q_head_stride;
+  a.partials = (float*)r->workspace;
+  a.layer = r->layer;
+  a.n_tokens = r->n_tokens;
+  a.q_dtype = r->q_dtype;
+  a.window = r->window == 0 ? INT_MAX : r->window;
+  a.sinks = r->sinks;
+  a.ns_cold = p.ns_cold, a.ns_hot = p.ns_hot;
+  a.rows = r->n_tokens * g.group;
+  const size_t esz = elem_size(r->q_dtype);
+  ctx->last_launches = 0;
+  for (int s = 0; s < r->seq_count; s += at_once) {
+    a.seq_begin = r->seq_begin + s;
+    a.seq_count = std::min(at_once, r->seq_count - s);
+    a.q = (const uint8_t*)r->q + (int64_t)s * r->q_seq_stride * (int64_t)esz;
+    a.out = (uint8_t*)r->out + (size_t)s * r->n_tokens * g.n_q_heads * TQ_D * esz;
+    a.q_lens = r->q_lens == nullptr ? nullptr : r->q_lens + s;
+    rc = tq_launch_attend_general(a, st);
+    if (rc != TQ_OK) return rc;
+    rc = tq_launch_attend_combine(a, st);
+    if (rc != TQ_OK) return rc;
+    ctx->last_launches += 2;
+  }
+  return TQ_OK;
+}

@@ -115,9 +115,10 @@ class TurboQuantKVManager:
         k, v = self._ctx.dequant(layer_id, 0, start, end)
         return k.cpu().numpy()[None], v.cpu().numpy()[None]
 
-    def attend(self, layer_id: int, query):
+    def attend(self, layer_id: int, query, window: int | None = None, sinks: int = 0):
         """Decode-step attention output of a layer, computed on the codes: ``query``
-        ``(n_q_heads, head_dim)`` (numpy or CUDA tensor) -> same kind, float32."""
+        ``(n_q_heads, head_dim)`` (numpy or CUDA tensor) -> same kind, float32.  With ``window``
+        only the newest ``window`` tokens and the first ``sinks`` ones are attended."""
         import torch
 
         is_np = not isinstance(query, torch.Tensor)
@@ -125,7 +126,10 @@ class TurboQuantKVManager:
         q = q.reshape(1, self._ctx.n_q_heads, self._head_dim).to(self._ctx.device)
         if self.length(layer_id) == 0:
             raise RuntimeError("cache is empty")
-        out = self._ctx.decode(layer_id, q)[0]
+        if window is None:
+            out = self._ctx.decode(layer_id, q)[0]
+        else:
+            out = self._ctx.attend(layer_id, q[:, None].float(), window, sinks)[0, 0]
         return out.cpu().numpy() if is_np else out
 
     def length(self, layer_id: int = 0) -> int:
