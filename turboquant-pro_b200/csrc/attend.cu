@@ -8,7 +8,9 @@ namespace {
 constexpr size_t AT_ONE_GO = (size_t)1 << 30;  // workspace that a call asks for at most, unless one
                                                // sequence needs more
 
+enum Form { GENERAL, ROWS };
 struct Plan {
+  Form form;
   int ns_cold, ns_hot;
   size_t seq_bytes;  // workspace of a sequence
 };
@@ -40,25 +42,28 @@ int most_tokens(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
 }
 
 // Splits of the tokens: enough CTAs for the GPU, of what is visible in the longest sequence, in blocks and in
-// the window (a tile of either counts the same).
+// the window.
 Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
   const tq_geom& g = ctx->g;
+  Plan p;
   const int n = most_tokens(ctx, r, st), rows = r->n_tokens * g.group;
   const int nb = n_cold_blocks(n, g.hot_window, g.block_tokens);
-  const int64_t seen = r->window == 0 ? n : std::min<int64_t>(n, (int64_t)r->window + r->n_tokens + r->sinks + 128);
-  const int64_t hot_tokens = std::min<int64_t>(g.hot_window, n);
-  const int64_t cold = nb > 0 ? std::max<int64_t>(seen - (n - (int64_t)nb * g.block_tokens), 1) : 0;
-  const int64_t cold_tiles = (cold + 63) / 64, hot_tiles = (hot_tokens + 63) / 64;
-  const int row_tile = rows <= 16 ? 16 : 64, per_sm = rows <= 16 ? 2 : 1;
-  const int64_t ctas = (int64_t)r->seq_count * g.n_kv_heads * ((rows + row_tile - 1) / row_tile);
+  p.form = rows <= 64 && g.block_tokens == 256 && g.key_mode != TQ_KEYS_POLAR && !ctx->force_generic ? ROWS : GENERAL;
+  const int row_tile = p.form == ROWS ? tq_attend_rows_tile(rows) : rows <= 16 ? 16 : 64;
+  const int cold_size = p.form == ROWS ? 256 : 64, hot_size = p.form == ROWS ? 128 : 64;
+  // tokens in blocks that the rows of a tile can see
+  const int64_t in_blocks = (int64_t)nb * g.block_tokens;
+  const int64_t seen = r->window == 0 ? in_blocks
+                                      : std::min<int64_t>(in_blocks, (int64_t)r->window + row_tile / g.group + r->sinks + cold_size);
+  const int64_t cold = (seen + cold_size - 1) / cold_size;
+  const int64_t hot = (std::min<int64_t>(g.hot_window, n) + hot_size - 1) / hot_size;
+  const int64_t ctas = std::max<int64_t>((int64_t)r->seq_count * g.n_kv_heads * ((rows + row_tile - 1) / row_tile), 1);
   int sm_count = 148;
   cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, ctx->device);
-  const int64_t want = std::min<int64_t>(
-      std::max<int64_t>((2 * per_sm * sm_count + ctas - 1) / std::max<int64_t>(ctas, 1), 1), 64);
-  const int64_t all = std::max<int64_t>(cold_tiles + hot_tiles, 1), each = (all + want - 1) / want;
-  Plan p;
-  p.ns_cold = (int)((cold_tiles + each - 1) / each);
-  p.ns_hot = (int)std::max<int64_t>((hot_tiles + each - 1) / each, 1);
+  const int64_t want = std::min<int64_t>(std::max<int64_t>((4 * sm_count + ctas - 1) / ctas, 1), 64);
+  const int64_t each = (std::max<int64_t>(cold + hot, 1) + want - 1) / want;
+  p.ns_cold = (int)((cold + each - 1) / each);
+  p.ns_hot = (int)std::max<int64_t>((hot + each - 1) / each, 1);
   // (the kernels go by the lengths on the device: blocks always have a split where there can be any)
   if (p.ns_cold == 0 && n_cold_blocks(g.max_tokens_per_seq, g.hot_window, g.block_tokens) > 0) p.ns_cold = 1;
   p.seq_bytes = (size_t)g.n_kv_heads * rows * (p.ns_cold + p.ns_hot) * TQ_PART_STRIDE * 4;
@@ -120,7 +125,7 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
     a.q = (const uint8_t*)r->q + (int64_t)s * r->q_seq_stride * (int64_t)esz;
     a.out = (uint8_t*)r->out + (size_t)s * r->n_tokens * g.n_q_heads * TQ_D * esz;
     a.q_lens = r->q_lens == nullptr ? nullptr : r->q_lens + s;
-    rc = tq_launch_attend_general(a, st);
+    rc = p.form == ROWS ? tq_launch_attend_rows(a, st) : tq_launch_attend_general(a, st);
     if (rc != TQ_OK) return rc;
     rc = tq_launch_attend_combine(a, st);
     if (rc != TQ_OK) return rc;

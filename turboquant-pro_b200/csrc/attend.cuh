@@ -94,3 +94,6 @@ TQ_DEV float attend_ld(const void* p, size_t i, int dt) {
 
 int tq_launch_attend_general(const AttendArgs& a, cudaStream_t st);
 int tq_launch_attend_combine(const AttendArgs& a, cudaStream_t st);
+// 256-token blocks of per-channel keys only
+int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st);
+int tq_attend_rows_tile(int rows);  // query rows of a CTA
