@@ -3,13 +3,15 @@
 //   channels i and i + r/2 (i < r/2) turn by  position * inv_freq[i]
 // what a model does to q and k between their projections and the cache.
 //
-// A warp holds a head: four channels a lane, loaded and stored as one 8- or 16-byte word; the sum of squares
-// is five shuffles, the partner channels come from the lane r/8 further.  The angles of a token are the same
-// for all heads, so a CTA takes one token and forms them once: position * inv_freq / 2 pi in 64 bits, of which
-// only the fraction counts (a 32-bit angle of position 10^6 is off by 0.06), then one sincospi in float32.
-// Sums, norm and rotation are float32, rounded once.
+// A lane holds 16 bytes of a head, so a warp two heads of 16-bit elements or one of float32.  The sum of squares
+// goes over the head's lanes with shuffles; the partner channels come, still packed, from the lane half a
+// rotation further.  What a token's heads have in common is formed once per token: position * inv_freq / 2 pi in
+// 64 bits, of which only the fraction counts (a 32-bit angle of position 10^6 is off by 0.06), one sincospi in
+// float32, and the weights times cosines and sines, so that a channel costs two multiply-adds.  Sums, norm and
+// rotation are float32, rounded once.
 //
-// Bound by memory for prompts, by launch and latency for single tokens.
+// Bound by memory for prompts, by launch and latency for single tokens: there a CTA of eight warps takes one
+// token; from a few tokens per SM on four, two warps each, whose angles are one step of the CTA.
 #include "common.cuh"
 
 namespace {
@@ -21,129 +23,229 @@ struct RopeArgs {
   const int32_t* seq_len;  // positions of the tokens that follow what is stored; null: r.positions
 };
 
-// elements 4 * lane .. + 3 of a row
-template <int DT>
-TQ_DEV void nr_load(const void* row, int64_t at, bool vec, float (&x)[4]) {
-  using T = typename Elem<DT>::type;
-  const T* p = (const T*)row + at;
-  if constexpr (DT == TQ_F32) {
-    if (vec) {
-      const float4 v = *(const float4*)p;
-      x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-      return;
-    }
-  } else if (vec) {
-    const uint2 v = *(const uint2*)p;
-    const T* e = (const T*)&v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = Elem<DT>::ld(e, i);
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = Elem<DT>::ld(p, i);
-}
-TQ_DEV float nr_round(float x, float*) { return x; }
-TQ_DEV __half nr_round(float x, __half*) { return __float2half_rn(x); }
-TQ_DEV __nv_bfloat16 nr_round(float x, __nv_bfloat16*) { return __float2bfloat16_rn(x); }
-template <int DT>
-TQ_DEV void nr_store(void* row, int64_t at, const float (&x)[4]) {
-  using T = typename Elem<DT>::type;
-  struct alignas(4 * sizeof(T)) V4 { T v[4]; } v;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v.v[i] = nr_round(x[i], (T*)nullptr);
-  *(V4*)((T*)row + at) = v;
-}
 TQ_DEV float nr_weight(const void* w, int i, int dt) {
   if (dt == TQ_F32) return ((const float*)w)[i];
   if (dt == TQ_F16) return __half2float(((const __half*)w)[i]);
   return __bfloat162float(((const __nv_bfloat16*)w)[i]);
 }
-
+// the elements of a 16-byte word
 template <int DT>
-__global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(RopeArgs a, int vec) {
-  __shared__ __align__(16) float cos_s[TQ_D / 2], sin_s[TQ_D / 2];
-  const tq_rope& r = a.r;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int s = blockIdx.x / r.n_tokens, t = blockIdx.x % r.n_tokens;
-  const int half = r.rotary_dim / 2, heads = r.n_q_heads + r.n_kv_heads;
-  constexpr int N = 4;  // heads of a warp in flight
-  float x[N][4];
-  auto row_of = [&](int h, int64_t& at) -> const void* {
-    const bool is_q = h < r.n_q_heads;
-    at = is_q ? (int64_t)s * r.q_seq_stride + (int64_t)t * r.q_tok_stride + (int64_t)h * r.q_head_stride
-              : (int64_t)s * r.k_seq_stride + (int64_t)t * r.k_tok_stride +
-                    (int64_t)(h - r.n_q_heads) * r.k_head_stride;
-    at += 4 * lane;
-    return is_q ? r.q : r.k;
-  };
-  auto fetch = [&](int h0) {
+TQ_DEV void nr_unpack(const uint4& v, float* x) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int h = h0 + i * (NR_THREADS / 32);
-      if (h < heads) {
-        int64_t at;
-        const void* row = row_of(h, at);
-        nr_load<DT>(row, at, vec, x[i]);
+  for (int i = 0; i < 4; ++i) {
+    if (DT == TQ_F32) {
+      x[i] = __uint_as_float(w[i]);
+    } else if (DT == TQ_F16) {
+      const float2 f = __half22float2(*(const __half2*)&w[i]);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    } else {
+      x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+template <int DT>
+TQ_DEV uint4 nr_pack(const float* x) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (DT == TQ_F32) {
+      w[i] = __float_as_uint(x[i]);
+    } else if (DT == TQ_F16) {
+      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *(const uint32_t*)&h;
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *(const uint32_t*)&h;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// 16 bytes of a row, by elements where rows may lie anywhere
+template <int DT, bool VEC>
+TQ_DEV uint4 nr_load(const typename Elem<DT>::type* p) {
+  using T = typename Elem<DT>::type;
+  if constexpr (VEC) {
+    return *(const uint4*)p;
+  } else {
+    union { uint4 v; T e[16 / sizeof(T)]; } u;
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i) u.e[i] = p[i];
+    return u.v;
+  }
+}
+
+// A head's elements as one lane holds them: 16 bytes, with what the lane knows of them.
+template <int DT>
+struct NrLane {
+  static constexpr int E = 16 / (int)sizeof(typename Elem<DT>::type);
+  static constexpr int LPH = TQ_D / E, HPW = 32 / LPH;  // lanes of a head, heads of a warp
+  int lane, hl, ch, half, partner;
+  bool low, turned;
+  float own[E], other[E];  // y = f * (x * own + partner * other), f the norm's factor
+};
+
+// PAIRED: a lane's partner channels are all of one lane (half the rotation is a multiple of a lane's channels);
+// otherwise they come one by one.
+template <int DT, bool PAIRED>
+TQ_DEV void nr_factors(NrLane<DT>& n, const float* w, const float* cos_s, const float* sin_s) {
+  constexpr int E = NrLane<DT>::E;
+  if (PAIRED) {
+    const int pr = n.turned ? (n.low ? n.ch : n.ch - n.half) : 0, oc = n.turned ? (n.low ? n.ch + n.half : n.ch - n.half) : n.ch;
+#pragma unroll
+    for (int i = 0; i < E; i += 4) {
+      const float4 c4 = *(const float4*)(cos_s + pr + i), s4 = *(const float4*)(sin_s + pr + i);
+      const float4 w4 = *(const float4*)(w + n.ch + i), o4 = *(const float4*)(w + oc + i);
+      const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+      const float a[4] = {w4.x, w4.y, w4.z, w4.w}, o[4] = {o4.x, o4.y, o4.z, o4.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        n.own[i + j] = n.turned ? a[j] * c[j] : a[j];
+        n.other[i + j] = n.turned ? (n.low ? -s[j] : s[j]) * o[j] : 0.0f;
       }
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int c = n.ch + i;
+      const bool lo = c < n.half, in = c < 2 * n.half;
+      const int pr = in ? (lo ? c : c - n.half) : 0, oc = in ? (lo ? c + n.half : c - n.half) : c;
+      n.own[i] = in ? w[c] * cos_s[pr] : w[c];
+      n.other[i] = in ? (lo ? -sin_s[pr] : sin_s[pr]) * w[oc] : 0.0f;
+    }
+  }
+}
+template <int DT, bool PAIRED>
+TQ_DEV uint4 nr_head(const NrLane<DT>& n, const uint4& raw, bool normed, float eps) {
+  constexpr int E = NrLane<DT>::E, LPH = NrLane<DT>::LPH;
+  float x[E], z[E], y[E];
+  nr_unpack<DT>(raw, x);
+  float f = 1.0f;
+  if (normed) {
+    float ss[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < E; ++c) ss[c & 1] = fmaf(x[c], x[c], ss[c & 1]);
+    ss[0] += ss[1];
+#pragma unroll
+    for (int d = LPH / 2; d >= 1; d >>= 1) ss[0] += __shfl_xor_sync(0xffffffffu, ss[0], d);
+    f = rsqrtf(fmaf(ss[0], 1.0f / TQ_D, eps));
+  }
+  if (PAIRED) {
+    uint4 o;
+    o.x = __shfl_sync(0xffffffffu, raw.x, n.partner), o.y = __shfl_sync(0xffffffffu, raw.y, n.partner);
+    o.z = __shfl_sync(0xffffffffu, raw.z, n.partner), o.w = __shfl_sync(0xffffffffu, raw.w, n.partner);
+    if (!n.turned) o = make_uint4(0u, 0u, 0u, 0u);
+    nr_unpack<DT>(o, z);
+  } else {
+#pragma unroll
+    for (int c = 0; c < E; ++c) {
+      // the channel's partner: element (oc % E) of its lane, whichever that is
+      const int d = n.ch + c, oc = d < n.half ? d + n.half : d < 2 * n.half ? d - n.half : d;
+      z[c] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float v = __shfl_sync(0xffffffffu, x[e], n.hl * LPH + oc / E);
+        if (oc % E == e && d < 2 * n.half) z[c] = v;
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < E; ++c) y[c] = f * fmaf(x[c], n.own[c], z[c] * n.other[c]);
+  return nr_pack<DT>(y);
+}
+
+template <int DT, bool PAIRED, bool VEC>
+__global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(RopeArgs a, int64_t tokens, int per_cta) {
+  using T = typename Elem<DT>::type;
+  using Lane = NrLane<DT>;
+  constexpr int HPW = Lane::HPW;
+  constexpr int N = 4;  // query items of a warp in flight, and one of keys
+  __shared__ __align__(16) float cos_s[4][TQ_D / 2], sin_s[4][TQ_D / 2], weight_s[2][TQ_D];
+  static_assert(NR_THREADS == 2 * TQ_D, "a thread per weight");
+  const tq_rope& r = a.r;
+  const int tid = threadIdx.x, warp = tid >> 5;
+  const int wpt = NR_THREADS / 32 / per_cta;  // warps of a token
+  const int mine = warp / wpt, sub = warp % wpt;
+  const int64_t tok = (int64_t)blockIdx.x * per_cta + mine;
+  const bool active = tok < tokens;
+  const int s = active ? (int)(tok / r.n_tokens) : 0, t = active ? (int)(tok - (int64_t)s * r.n_tokens) : 0;
+  Lane n;
+  n.lane = tid & 31;
+  n.hl = n.lane / Lane::LPH, n.ch = n.lane % Lane::LPH * Lane::E, n.half = r.rotary_dim / 2;
+  n.low = n.ch < n.half, n.turned = n.ch < 2 * n.half;
+  n.partner = !PAIRED || !n.turned ? n.lane : n.low ? n.lane + n.half / Lane::E : n.lane - n.half / Lane::E;
+  // this lane's head of item 0; the items of a warp are `step` heads apart
+  const int h0 = sub * HPW + n.hl, step = wpt * HPW;
+  const T* q = (const T*)r.q + ((int64_t)s * r.q_seq_stride + (int64_t)t * r.q_tok_stride + h0 * r.q_head_stride + n.ch);
+  const T* k = (const T*)r.k + ((int64_t)s * r.k_seq_stride + (int64_t)t * r.k_tok_stride + h0 * r.k_head_stride + n.ch);
+  const int64_t q_step = step * r.q_head_stride, k_step = step * r.k_head_stride;
+
+  uint4 raw[N], raw_k = make_uint4(0u, 0u, 0u, 0u);
+  auto fetch = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      raw[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (active && h + i * step < r.n_q_heads) raw[i] = nr_load<DT, VEC>(q);
+      q += q_step;
+    }
   };
-  fetch(warp);  // (the loads are on their way while the angles are formed)
-  if (tid < half) {
+  fetch(h0);  // (on their way while the angles are formed)
+  if (active && h0 < r.n_kv_heads) raw_k = nr_load<DT, VEC>(k);
+  {
+    const void* w = tid < TQ_D ? r.q_weight : r.k_weight;
+    weight_s[tid / TQ_D][tid % TQ_D] = w == nullptr ? 1.0f : nr_weight(w, tid % TQ_D, r.weight_dtype);
+  }
+  for (int i = tid; i < per_cta * n.half; i += NR_THREADS) {
+    const int u = i / n.half, f = i - u * n.half;
+    const int64_t tk = (int64_t)blockIdx.x * per_cta + u;
+    if (tk >= tokens) break;
+    const int us = (int)(tk / r.n_tokens), ut = (int)(tk - (int64_t)us * r.n_tokens);
     int64_t p;
-    if (a.seq_len != nullptr) p = (int64_t)a.seq_len[s] + t;
+    if (a.seq_len != nullptr) p = (int64_t)a.seq_len[us] + ut;
     else {
-      const int64_t at = (int64_t)s * r.pos_seq_stride + (int64_t)t * r.pos_tok_stride;
+      const int64_t at = (int64_t)us * r.pos_seq_stride + (int64_t)ut * r.pos_tok_stride;
       p = r.pos_bits == 64 ? ((const int64_t*)r.positions)[at] : (int64_t)((const int32_t*)r.positions)[at];
     }
-    const double turns = (double)p * ((double)r.inv_freq[tid] * 0.15915494309189533577);
+    const double turns = (double)p * ((double)r.inv_freq[f] * 0.15915494309189533577);
     float sn, cs;
     sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
-    cos_s[tid] = cs;
-    sin_s[tid] = sn;
-  }
-  float wq[4], wk[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    wq[i] = r.q_weight != nullptr ? nr_weight(r.q_weight, 4 * lane + i, r.weight_dtype) : 1.0f;
-    wk[i] = r.k_weight != nullptr ? nr_weight(r.k_weight, 4 * lane + i, r.weight_dtype) : 1.0f;
+    cos_s[u][f] = cs;
+    sin_s[u][f] = sn;
   }
   __syncthreads();
-  // this lane's channels: the first ones of their pairs, the second ones, or not turned at all
-  const int ch = 4 * lane;
-  const bool low = ch < half, turns = ch < 2 * half;
-  const int pair = turns ? (low ? ch : ch - half) : 0, other = turns ? (low ? lane + half / 4 : lane - half / 4) : lane;
-  float cs[4], sn[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    cs[i] = turns ? cos_s[pair + i] : 1.0f;
-    sn[i] = turns ? (low ? -sin_s[pair + i] : sin_s[pair + i]) : 0.0f;
-  }
-  for (int h0 = warp; h0 < heads; h0 += N * (NR_THREADS / 32)) {
-    if (h0 != warp) fetch(h0);
+  if (!active) return;
+
+  T* out = (T*)r.q_out + ((tok * r.n_q_heads + h0) * TQ_D + n.ch);
+  nr_factors<DT, PAIRED>(n, weight_s[0], cos_s[mine], sin_s[mine]);
+  for (int h = h0; h - n.hl < r.n_q_heads; h += N * step) {  // (a warp's lanes stay together)
+    if (h != h0) fetch(h);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int h = h0 + i * (NR_THREADS / 32);
-      if (h >= heads) break;  // (the whole warp)
-      const bool is_q = h < r.n_q_heads;
-      if ((is_q ? r.q_weight : r.k_weight) != nullptr) {
-        float ss = (x[i][0] * x[i][0] + x[i][1] * x[i][1]) + (x[i][2] * x[i][2] + x[i][3] * x[i][3]);
-#pragma unroll
-        for (int d = 16; d >= 1; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-        const float f = 1.0f / sqrtf(ss * (1.0f / TQ_D) + r.eps);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) x[i][c] *= f * (is_q ? wq[c] : wk[c]);
-      }
-      float y[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float z = __shfl_sync(0xffffffffu, x[i][c], other);
-        y[c] = turns ? fmaf(x[i][c], cs[c], z * sn[c]) : x[i][c];
-      }
-      const int64_t tok = (int64_t)s * r.n_tokens + t;
-      if (is_q) nr_store<DT>(r.q_out, (tok * r.n_q_heads + h) * TQ_D + 4 * lane, y);
-      else nr_store<DT>(r.k_out, (tok * r.n_kv_heads + h - r.n_q_heads) * TQ_D + 4 * lane, y);
+      if (h - n.hl + i * step >= r.n_q_heads) break;
+      const uint4 y = nr_head<DT, PAIRED>(n, raw[i], r.q_weight != nullptr, r.eps);
+      if (h + i * step < r.n_q_heads) *(uint4*)out = y;
+      out += step * TQ_D;
     }
   }
+  out = (T*)r.k_out + ((tok * r.n_kv_heads + h0) * TQ_D + n.ch);
+  nr_factors<DT, PAIRED>(n, weight_s[1], cos_s[mine], sin_s[mine]);
+  for (int h = h0; h - n.hl < r.n_kv_heads; h += step) {
+    const uint4 x = raw_k;
+    k += k_step;
+    if (h + step < r.n_kv_heads) raw_k = nr_load<DT, VEC>(k);
+    const uint4 y = nr_head<DT, PAIRED>(n, x, r.k_weight != nullptr, r.eps);
+    if (h < r.n_kv_heads) *(uint4*)out = y;
+    out += step * TQ_D;
+  }
+}
+
+template <int DT, bool PAIRED>
+void start(const RopeArgs& a, int64_t tokens, bool vec, cudaStream_t st) {
+  // (four tokens a CTA as soon as these fill the SMs)
+  const int per_cta = tokens >= 512 ? 4 : 1;
+  const int grid = (int)((tokens + per_cta - 1) / per_cta);
+  if (vec) norm_rope_kernel<DT, PAIRED, true><<<grid, NR_THREADS, 0, st>>>(a, tokens, per_cta);
+  else norm_rope_kernel<DT, PAIRED, false><<<grid, NR_THREADS, 0, st>>>(a, tokens, per_cta);
 }
 
 int check_rope(const tq_rope* r, bool stored) {
@@ -165,23 +267,24 @@ int check_rope(const tq_rope* r, bool stored) {
   TQ_REQUIRE(r->rotary_dim == 0 || r->inv_freq, TQ_ERR_INVALID, "inv_freq must be a device pointer");
   TQ_REQUIRE(r->rotary_dim == 0 || stored || (r->positions && (r->pos_bits == 32 || r->pos_bits == 64)),
              TQ_ERR_INVALID, "positions must be a device pointer to 32- or 64-bit integers");
-  TQ_REQUIRE(((uintptr_t)r->q_out | (uintptr_t)r->k_out) % (4 * elem_size(r->dtype)) == 0, TQ_ERR_INVALID,
-             "q_out and k_out must be aligned to four elements");
+  TQ_REQUIRE(((uintptr_t)r->q_out | (uintptr_t)r->k_out) % 16 == 0, TQ_ERR_INVALID,
+             "q_out and k_out must be aligned to 16 bytes");
   return TQ_OK;
 }
 
 int launch(const tq_rope* r, const int32_t* seq_len, cudaStream_t st) {
   const int64_t tokens = (int64_t)r->n_seqs * r->n_tokens;
   if (tokens == 0 || r->n_q_heads + r->n_kv_heads == 0) return TQ_OK;
-  const int word = 4 * elem_size(r->dtype);
-  const bool vec = ((uintptr_t)r->q | (uintptr_t)r->k) % word == 0 &&
+  const int e = 16 / elem_size(r->dtype);
+  const bool vec = ((uintptr_t)r->q | (uintptr_t)r->k) % 16 == 0 &&
                    ((r->q_seq_stride | r->q_tok_stride | r->q_head_stride | r->k_seq_stride |
-                     r->k_tok_stride | r->k_head_stride) & 3) == 0;
+                     r->k_tok_stride | r->k_head_stride) & (e - 1)) == 0;
   RopeArgs a = {*r, seq_len};
+  const bool paired = r->rotary_dim / 2 % e == 0;
   switch (r->dtype) {
-    case TQ_F32: norm_rope_kernel<TQ_F32><<<(int)tokens, NR_THREADS, 0, st>>>(a, vec); break;
-    case TQ_F16: norm_rope_kernel<TQ_F16><<<(int)tokens, NR_THREADS, 0, st>>>(a, vec); break;
-    default: norm_rope_kernel<TQ_BF16><<<(int)tokens, NR_THREADS, 0, st>>>(a, vec); break;
+    case TQ_F32: start<TQ_F32, true>(a, tokens, vec, st); break;
+    case TQ_F16: paired ? start<TQ_F16, true>(a, tokens, vec, st) : start<TQ_F16, false>(a, tokens, vec, st); break;
+    default: paired ? start<TQ_BF16, true>(a, tokens, vec, st) : start<TQ_BF16, false>(a, tokens, vec, st);
   }
   TQ_CUDA(cudaGetLastError());
   return TQ_OK;

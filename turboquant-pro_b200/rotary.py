@@ -12,7 +12,7 @@ import ctypes as C
 
 from . import _lib
 from ._lib import TqRope, check
-from .context import _dtype_code, _dtype_codes, _raw_stream, _torch
+from .context import _NO_GUARD, _dtype_codes, _raw_stream, _torch
 
 __all__ = ["norm_rope"]
 
@@ -38,69 +38,76 @@ def norm_rope(q, k, inv_freq, positions, *, q_weight=None, k_weight=None, eps: f
     return _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, None)
 
 
-def _readable(t):
-    """``t`` with contiguous channels."""
-    return t if t.numel() == 0 or t.stride(-1) == 1 else t.contiguous()
-
-
 def _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, cache):
+    # (a decode step's call is a few microseconds on the GPU: the checks are kept short)
     torch = _torch()
-    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2]:
-        raise ValueError(f"expected q, k of shape [n_seqs, T, heads, {HEAD_DIM}], got {tuple(q.shape)} "
-                         f"and {tuple(k.shape)}")
-    if q.shape[3] != HEAD_DIM or k.shape[3] != HEAD_DIM:
+    q_shape, k_shape, dev, dtype = q.shape, k.shape, q.device, q.dtype
+    if len(q_shape) != 4 or len(k_shape) != 4 or q_shape[:2] != k_shape[:2]:
+        raise ValueError(f"expected q, k of shape [n_seqs, T, heads, {HEAD_DIM}], got {tuple(q_shape)} "
+                         f"and {tuple(k_shape)}")
+    if q_shape[3] != HEAD_DIM or k_shape[3] != HEAD_DIM:
         raise NotImplementedError(f"only head_dim {HEAD_DIM} is implemented")
-    if q.device.type != "cuda":
-        raise ValueError(f"q must be a CUDA tensor, it lives on {q.device}")
-    if q.dtype not in _dtype_codes() or k.dtype != q.dtype:
-        raise ValueError(f"q and k must share float32, float16 or bfloat16, got {q.dtype} and {k.dtype}")
-    dev = q.device
-    inputs = {"k": k, "inv_freq": inv_freq, "positions": positions, "q_weight": q_weight,
-              "k_weight": k_weight}
-    for name, t in inputs.items():
-        if t is not None and t.device != dev:
+    if dev.type != "cuda":
+        raise ValueError(f"q must be a CUDA tensor, it lives on {dev}")
+    codes = _dtype_codes()
+    if dtype not in codes or k.dtype != dtype:
+        raise ValueError(f"q and k must share float32, float16 or bfloat16, got {dtype} and {k.dtype}")
+    grad = torch.is_grad_enabled()
+    for name, t in (("q", q), ("k", k), ("inv_freq", inv_freq), ("positions", positions),
+                    ("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is None:
+            continue
+        if t.device != dev:
             raise ValueError(f"{name} lives on {t.device}, q on {dev}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (q, k, inv_freq, q_weight, k_weight)):
-        raise ValueError("norm_rope has no backward pass: call it under torch.no_grad()")
+        if grad and t.requires_grad:
+            raise ValueError("norm_rope has no backward pass: call it under torch.no_grad()")
     if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
         raise ValueError("inv_freq must be a float32 vector")
     if eps < 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    weights = [w for w in (q_weight, k_weight) if w is not None]
-    for w in weights:
-        if tuple(w.shape) != (HEAD_DIM,) or w.dtype not in _dtype_codes() or w.dtype != weights[0].dtype:
+    weight_type = 0
+    for w in (q_weight, k_weight):
+        if w is None:
+            continue
+        if w.shape != (HEAD_DIM,) or w.dtype not in codes \
+                or (k_weight is not None and w.dtype != k_weight.dtype):
             raise ValueError(f"norm weights must be [{HEAD_DIM}] and of one floating type")
-    n, t = q.shape[:2]
-    r = TqRope()
+        weight_type = codes[w.dtype]
+    n, t = q_shape[0], q_shape[1]
+    pos, pos_bits, pos_stride = None, 0, (0, 0)
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-        if tuple(positions.shape) not in ((n, t), (t,)):
+        if positions.shape == (n, t):
+            pos_stride = positions.stride()
+        elif positions.shape == (t,):
+            pos_stride = (0, positions.stride(0))
+        else:
             raise ValueError(f"positions must be [{n}, {t}] or [{t}], got {tuple(positions.shape)}")
-        positions = positions.expand(n, t)
-        r.positions, r.pos_bits = positions.data_ptr(), 8 * positions.element_size()
-        r.pos_seq_stride, r.pos_tok_stride = positions.stride()
-    q, k, inv_freq = _readable(q), _readable(k), inv_freq.contiguous()
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
+        pos, pos_bits = positions.data_ptr(), 64 if positions.dtype == torch.int64 else 32
+    qs, ks = q.stride(), k.stride()
+    if qs[3] != 1:
+        q = q.contiguous()
+        qs = q.stride()
+    if ks[3] != 1:
+        k = k.contiguous()
+        ks = k.stride()
+    inv_freq = inv_freq.contiguous()
     q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
-    r.q, r.k, r.q_out, r.k_out = q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr()
-    r.q_weight = q_weight.data_ptr() if q_weight is not None else None
-    r.k_weight = k_weight.data_ptr() if k_weight is not None else None
-    r.inv_freq = inv_freq.data_ptr()
-    r.q_seq_stride, r.q_tok_stride, r.q_head_stride = q.stride()[:3]
-    r.k_seq_stride, r.k_tok_stride, r.k_head_stride = k.stride()[:3]
-    r.n_seqs, r.n_tokens, r.n_q_heads, r.n_kv_heads = n, t, q.shape[2], k.shape[2]
-    r.dtype = _dtype_code(q.dtype)
-    r.weight_dtype = _dtype_code(weights[0].dtype) if weights else 0
-    r.rotary_dim, r.eps = 2 * inv_freq.numel(), eps
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        stream = _raw_stream()(dev.index)
+    q_out = torch.empty(q_shape, dtype=dtype, device=dev)
+    k_out = torch.empty(k_shape, dtype=dtype, device=dev)
+    r = TqRope(q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
+               None if q_weight is None else q_weight.data_ptr(),
+               None if k_weight is None else k_weight.data_ptr(), inv_freq.data_ptr(), pos,
+               qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], pos_stride[0], pos_stride[1],
+               n, t, q_shape[2], k_shape[2], codes[dtype], weight_type, pos_bits,
+               2 * inv_freq.numel(), eps)
+    lib, index = _lib.load(), dev.index
+    with _NO_GUARD if torch.cuda.current_device() == index else torch.cuda.device(dev):
+        stream = _raw_stream()(index)
         if cache is not None and positions is None:
             ctx, layer, seq_begin = cache
             check(lib.tq_ctx_norm_rope(ctx._h, layer, seq_begin, C.byref(r), stream))
         else:
-            check(lib.tq_norm_rope(C.byref(r), dev.index, stream))
+            check(lib.tq_norm_rope(C.byref(r), index, stream))
     return q_out, k_out
