@@ -8,10 +8,11 @@ namespace {
 constexpr size_t AT_ONE_GO = (size_t)1 << 30;  // workspace that a call asks for at most, unless one
                                                // sequence needs more
 
-enum Form { GENERAL, ROWS };
+enum Form { GENERAL, ROWS, TILES };
 struct Plan {
   Form form;
   int ns_cold, ns_hot;
+  int cap, splits;   // TILES: tiles that a (sequence, KV head) has room for, splits of them
   size_t seq_bytes;  // workspace of a sequence
 };
 
@@ -45,10 +46,35 @@ int most_tokens(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
 // the window.
 Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
   const tq_geom& g = ctx->g;
-  Plan p;
+  Plan p = {};
   const int n = most_tokens(ctx, r, st), rows = r->n_tokens * g.group;
   const int nb = n_cold_blocks(n, g.hot_window, g.block_tokens);
-  p.form = rows <= 64 && g.block_tokens == 256 && g.key_mode != TQ_KEYS_POLAR && !ctx->force_generic ? ROWS : GENERAL;
+  const bool channels = g.key_mode != TQ_KEYS_POLAR && !ctx->force_generic;
+  p.form = rows > 64 && channels && r->q_dtype != TQ_F32 ? TILES
+           : rows <= 64 && channels && g.block_tokens == 256 ? ROWS : GENERAL;
+  int sm_count = 148;
+  cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, ctx->device);
+  if (p.form == TILES) {
+    const int64_t all = std::max<int64_t>((n + 127) / 128, 1);
+    auto seen = [&](int64_t tokens) {  // tiles that so many neighbouring query tokens see
+      return r->window == 0 ? all : std::min<int64_t>(all, (r->window + tokens + 254) / 128 + (r->sinks + 127) / 128);
+    };
+    p.cap = (int)seen(r->n_tokens);
+    // splits of a tile of rows: as many as bring the rounds of CTAs nearest to even (with four tiles' time for
+    // what a CTA does besides)
+    const int64_t each = seen(256 / g.group + 1), ctas = (int64_t)r->seq_count * g.n_kv_heads * ((rows + 255) / 256);
+    int64_t best = INT64_MAX;
+    for (int k = 1; k <= 32 && k <= each; ++k) {
+      const int64_t time = (ctas * k + sm_count - 1) / sm_count * ((each + k - 1) / k + 4);
+      if (time < best) best = time, p.splits = k;
+    }
+    AttendArgs a = {};
+    a.g = g;
+    a.rows = rows;
+    a.q_dtype = r->q_dtype;
+    p.seq_bytes = tq_attend_tiles_bytes(a, g.n_kv_heads, p.cap, p.splits);
+    return p;
+  }
   const int row_tile = p.form == ROWS ? tq_attend_rows_tile(rows) : rows <= 16 ? 16 : 64;
   const int cold_size = p.form == ROWS ? 256 : 64, hot_size = p.form == ROWS ? 128 : 64;
   // tokens in blocks that the rows of a tile can see
@@ -58,8 +84,6 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
   const int64_t cold = (seen + cold_size - 1) / cold_size;
   const int64_t hot = (std::min<int64_t>(g.hot_window, n) + hot_size - 1) / hot_size;
   const int64_t ctas = std::max<int64_t>((int64_t)r->seq_count * g.n_kv_heads * ((rows + row_tile - 1) / row_tile), 1);
-  int sm_count = 148;
-  cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, ctx->device);
   const int64_t want = std::min<int64_t>(std::max<int64_t>((4 * sm_count + ctas - 1) / ctas, 1), 64);
   const int64_t each = (std::max<int64_t>(cold + hot, 1) + want - 1) / want;
   p.ns_cold = (int)((cold + each - 1) / each);
@@ -117,6 +141,7 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
   a.sinks = r->sinks;
   a.ns_cold = p.ns_cold, a.ns_hot = p.ns_hot;
   a.rows = r->n_tokens * g.group;
+  a.unit_stride = (int64_t)a.rows * (p.ns_cold + p.ns_hot) * TQ_PART_STRIDE;
   const size_t esz = elem_size(r->q_dtype);
   ctx->last_launches = 0;
   for (int s = 0; s < r->seq_count; s += at_once) {
@@ -125,6 +150,12 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
     a.q = (const uint8_t*)r->q + (int64_t)s * r->q_seq_stride * (int64_t)esz;
     a.out = (uint8_t*)r->out + (size_t)s * r->n_tokens * g.n_q_heads * TQ_D * esz;
     a.q_lens = r->q_lens == nullptr ? nullptr : r->q_lens + s;
+    if (p.form == TILES) {
+      rc = tq_launch_attend_tiles(a, r->workspace, p.cap, p.splits, st);
+      if (rc != TQ_OK) return rc;
+      ctx->last_launches += 4;
+      continue;
+    }
     rc = p.form == ROWS ? tq_launch_attend_rows(a, st) : tq_launch_attend_general(a, st);
     if (rc != TQ_OK) return rc;
     rc = tq_launch_attend_combine(a, st);

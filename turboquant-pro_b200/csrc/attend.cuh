@@ -31,7 +31,8 @@ struct AttendArgs {
   int64_t q_seq, q_tok, q_head;  // strides in elements
   void* out;                     // [seq_count][n_tokens][n_q_heads][D] of q_dtype
   const int32_t* q_lens;         // [seq_count] or null: n_tokens everywhere
-  float* partials;               // [unit][row][ns_cold + ns_hot][2 + D]
+  float* partials;               // per unit, unit_stride floats apart: [row][ns_cold + ns_hot][2 + D]
+  int64_t unit_stride;
   // flags of the tiled kernels per unit: not zero, the unit is left to the general kernel (null: none)
   const int32_t* left;
   int32_t layer, seq_begin, seq_count, n_tokens, q_dtype;
@@ -83,7 +84,7 @@ TQ_DEV AttendTiles attend_tiles(const AttendArgs& a, int base, int end, int size
 }
 
 TQ_DEV float* attend_partial(const AttendArgs& a, int unit, int row, int split) {
-  return a.partials + (((size_t)unit * a.rows + row) * (a.ns_cold + a.ns_hot) + split) * TQ_PART_STRIDE;
+  return a.partials + (size_t)unit * a.unit_stride + ((size_t)row * (a.ns_cold + a.ns_hot) + split) * TQ_PART_STRIDE;
 }
 
 TQ_DEV float attend_ld(const void* p, size_t i, int dt) {
@@ -97,3 +98,6 @@ int tq_launch_attend_combine(const AttendArgs& a, cudaStream_t st);
 // 256-token blocks of per-channel keys only
 int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st);
 int tq_attend_rows_tile(int rows);  // query rows of a CTA
+// 16-bit queries, per-channel keys: everything in one, the merge too; `cap` tiles of 128 tokens per unit have room
+size_t tq_attend_tiles_bytes(const AttendArgs& a, int units, int cap, int splits);
+int tq_launch_attend_tiles(const AttendArgs& a, void* workspace, int cap, int splits, cudaStream_t st);
