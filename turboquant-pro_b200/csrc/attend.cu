@@ -151,7 +151,7 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
     a.out = (uint8_t*)r->out + (size_t)s * r->n_tokens * g.n_q_heads * TQ_D * esz;
     a.q_lens = r->q_lens == nullptr ? nullptr : r->q_lens + s;
     if (p.form == TILES) {
-      rc = tq_launch_attend_tiles(a, r->workspace, p.cap, p.splits, st);
+      rc = tq_launch_attend_tiles(a, r->workspace, p.cap, p.splits, ctx->device, st);
       if (rc != TQ_OK) return rc;
       ctx->last_launches += 4;
       continue;

@@ -100,4 +100,5 @@ int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st);
 int tq_attend_rows_tile(int rows);  // query rows of a CTA
 // 16-bit queries, per-channel keys: everything in one, the merge too; `cap` tiles of 128 tokens per unit have room
 size_t tq_attend_tiles_bytes(const AttendArgs& a, int units, int cap, int splits);
-int tq_launch_attend_tiles(const AttendArgs& a, void* workspace, int cap, int splits, cudaStream_t st);
+int tq_launch_attend_tiles(const AttendArgs& a, void* workspace, int cap, int splits, int device,
+                           cudaStream_t st);

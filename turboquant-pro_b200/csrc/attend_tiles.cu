@@ -38,6 +38,7 @@ constexpr int TI_SLOTS = 5;                  // images in shared memory
 constexpr int TI_THREADS = 320;              // two softmax groups, a warp that issues, a warp that loads
 constexpr float TI_KEY = 16.0f;              // keys are divided by it
 constexpr float TI_LIFT = 7.0f, TI_GROW = 8.0f;  // probabilities reach 2^(7 + 8) at most
+constexpr int TI_POLY = 3;                   // of eight pairs of exponentials, those on the multiply-add units
 constexpr int TI_WAIT = 1 << 21;             // probes of a wait, a microsecond or two each at most
 
 struct TileArgs {
@@ -71,17 +72,38 @@ TQ_DEV uint32_t ti_rest(float a, float b, uint32_t hi) {  // what the pair's rou
 }
 
 constexpr int TS_THREADS = 256;
-constexpr int TS_VS = TQ_D + 4;  // floats per row of window values
+constexpr int TS_VS = TQ_D + 4;   // floats per row of window values
+constexpr int TS_VT = 32;         // window tokens that are rotated at a time
 template <bool SPLIT>
 struct StageShared {
-  alignas(16) uint8_t k[SPLIT ? 2 : 1][TI_IMAGE];
-  float v[TI_T][TS_VS];
+  alignas(16) uint8_t k[SPLIT ? 2 : 1][TI_IMAGE];  // afterwards rows of window values
   float center[TQ_D], grid[16], cent[16], norm[TI_T];
   float top[TS_THREADS / 32];
 };
+static_assert(TS_VT * TS_VS * 4 <= TI_IMAGE, "the window values' place");
+
+// eight neighbouring elements of a window row
+TQ_DEV void ts_ld8(const void* p, size_t at, int dt, float (&x)[8]) {
+  if (dt == TQ_F32) {
+    const float4 u = *(const float4*)((const float*)p + at), v = *(const float4*)((const float*)p + at + 4);
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+    return;
+  }
+  const uint4 u = *(const uint4*)((const uint16_t*)p + at);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (dt == TQ_F16) {
+      const float2 f = __half22float2(*(const __half2*)&w[i]);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    } else {
+      x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
 
 template <bool SPLIT>
-__global__ void __launch_bounds__(TS_THREADS) attend_stage_kernel(AttendArgs a, TileArgs ta) {
+__global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel(AttendArgs a, TileArgs ta) {
   extern __shared__ __align__(16) uint8_t ts_smem[];
   StageShared<SPLIT>& sh = *(StageShared<SPLIT>*)ts_smem;
   const tq_geom& g = a.g;
@@ -101,7 +123,10 @@ __global__ void __launch_bounds__(TS_THREADS) attend_stage_kernel(AttendArgs a, 
   const size_t uix = unit_index(g, a.layer, a.seq_begin + s, head);
   const uint8_t* const pages = a.pages + page_offset(g, a.layer, a.seq_begin + s, head, 0);
   const size_t ring = hot_offset_elems(g, a.layer, a.seq_begin + s, head);
+  const bool hot = t1 > sq.cold;  // some tokens are of the window
 
+  PageMeta first = {0, 0};  // of the tile's first block, ahead of its use
+  if (g.outlier_k > 0 && t0 < sq.cold) first = a.page_meta[uix * g.max_blocks + t0 / S];
   if (tid < 16) {
     sh.grid[tid] = a.tables->grid[tid];
     sh.cent[tid] = a.tables->centroids[tid];
@@ -115,8 +140,37 @@ __global__ void __launch_bounds__(TS_THREADS) attend_stage_kernel(AttendArgs a, 
     }
     sh.center[tid] = c;
   }
-  __syncthreads();
   bool odd = false;
+  {  // ---- norms of the values: two threads a token
+    const int row = tid >> 1, t = t0 + row;
+    float norm = 0.0f;
+    if (t < sq.cold) {
+      const int b = t / S;
+      norm = ((const float*)(pages + (size_t)b * g.page_bytes + g.norm_off))[t - b * S];
+    }
+    if (hot) {
+      float ss = 0.0f;
+      if (t >= sq.cold && t < t1) {
+        const size_t at = ring + (size_t)(t % g.hot_cap) * TQ_D + (tid & 1) * (TQ_D / 2);
+#pragma unroll 4
+        for (int i = 0; i < 8; ++i) {
+          float x[8];
+          ts_ld8(a.hot_v, at + 8 * i, g.kv_dtype, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+        }
+      }
+      ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+      if (t >= sq.cold) norm = sqrtf(ss);
+    }
+    odd |= !isfinite(norm);
+    if ((tid & 1) == 0) sh.norm[row] = norm;
+    float top = fabsf(norm);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) sh.top[warp] = top;
+  }
+  __syncthreads();
   {  // ---- keys: a thread has half a token
     const int row = tid & 127, h = tid >> 7, t = t0 + row;
     auto put = [&](int chunk, const float (&x)[8]) {
@@ -152,13 +206,18 @@ __global__ void __launch_bounds__(TS_THREADS) attend_stage_kernel(AttendArgs a, 
         put(8 * h + i, x);
       }
     } else {
-#pragma unroll
+      const size_t at = ring + (size_t)(t % g.hot_cap) * TQ_D + 64 * h;
+#pragma unroll 4
       for (int i = 0; i < 8; ++i) {
-        const int d = 64 * h + 8 * i;
         float x[8];
+        if (t < t1) {
+          ts_ld8(a.hot_k, at + 8 * i, g.kv_dtype, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          x[e] = t < t1 ? attend_ld(a.hot_k, ring + (size_t)(t % g.hot_cap) * TQ_D + d + e, g.kv_dtype) - sh.center[d + e] : 0.0f;
+          for (int e = 0; e < 8; ++e) x[e] -= sh.center[64 * h + 8 * i + e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = 0.0f;
+        }
         put(8 * h + i, x);
       }
     }
@@ -166,13 +225,15 @@ __global__ void __launch_bounds__(TS_THREADS) attend_stage_kernel(AttendArgs a, 
   __syncthreads();
   if (g.outlier_k > 0) {
     for (int b = t0 / S; b * S < min(t1, sq.cold); ++b) {
-      const PageMeta pm = a.page_meta[uix * g.max_blocks + b];
+      const PageMeta pm = b == t0 / S ? first : a.page_meta[uix * g.max_blocks + b];
       const size_t slab = uix * (size_t)g.pool_entries + pm.off;
+#pragma unroll 3
       for (uint32_t e = tid; e < pm.cnt; e += TS_THREADS) {
         const uint32_t w = a.pool_dec[slab + e];
+        const __half val = __ushort_as_half(a.pool_val[slab + e]);
         const int t = b * S + (int)(w >> 24), ch = (w >> 16) & 127;
         if (t < t0 || t >= t1) continue;
-        const float x = (__half2float(__ushort_as_half(a.pool_val[slab + e])) - sh.center[ch]) * (1.0f / TI_KEY);
+        const float x = (__half2float(val) - sh.center[ch]) * (1.0f / TI_KEY);
         odd |= !(fabsf(x) <= 65504.0f);
         const int at = (ch >> 3) * TI_LBO + (t - t0) * 16 + (ch & 7) * 2;
         const __half hi = __float2half_rn(x);
@@ -181,49 +242,16 @@ __global__ void __launch_bounds__(TS_THREADS) attend_stage_kernel(AttendArgs a, 
       }
     }
   }
-
-  // ---- values: norms, the tile's power of two
-  const bool hot = t1 > sq.cold;  // some tokens are of the window
-  if (hot) {
-    for (int i = tid; i < TI_T * (TQ_D / 4); i += TS_THREADS) {
-      const int row = i / (TQ_D / 4), d = i % (TQ_D / 4) * 4, t = t0 + row;
-      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (t >= sq.cold && t < t1) {
-        const size_t at = ring + (size_t)(t % g.hot_cap) * TQ_D + d;
-        x = make_float4(attend_ld(a.hot_v, at, g.kv_dtype), attend_ld(a.hot_v, at + 1, g.kv_dtype),
-                        attend_ld(a.hot_v, at + 2, g.kv_dtype), attend_ld(a.hot_v, at + 3, g.kv_dtype));
-      }
-      *(float4*)&sh.v[row][d] = x;
-    }
-  }
-  __syncthreads();
+  odd = __syncthreads_or(odd);
+  if (odd && tid == 0) ta.left[unit] = 1;
   uint8_t* const images = ta.images + ((size_t)unit * ta.cap + idx) * (SPLIT ? 4 : 2) * TI_IMAGE;
-  {
-    float norm = 0.0f;
-    if (tid < TI_T) {
-      const int t = t0 + tid;
-      if (t < sq.cold) {
-        const int b = t / S;
-        norm = ((const float*)(pages + (size_t)b * g.page_bytes + g.norm_off))[t - b * S];
-      } else if (t < t1) {
-        float x = 0.0f;
-        for (int d = 0; d < TQ_D; ++d) x = fmaf(sh.v[tid][d], sh.v[tid][d], x);
-        norm = sqrtf(x);
-      }
-      odd |= !isfinite(norm);
-      sh.norm[tid] = norm;
-    }
-    float top = fabsf(norm);
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) sh.top[warp] = top;
-  }
-  for (int i = tid; i < TI_IMAGE / 16; i += TS_THREADS) {  // (the keys are complete)
+#pragma unroll 4
+  for (int i = tid; i < TI_IMAGE / 16; i += TS_THREADS) {
     *(uint4*)(images + 16 * i) = *(const uint4*)(sh.k[0] + 16 * i);
     if (SPLIT) *(uint4*)(images + TI_IMAGE + 16 * i) = *(const uint4*)(sh.k[SPLIT] + 16 * i);
   }
-  odd = __syncthreads_or(odd);
-  if (odd && tid == 0) ta.left[unit] = 1;
+
+  // ---- values
   float top = 0.0f, exponent;
 #pragma unroll
   for (int w = 0; w < TS_THREADS / 32; ++w) top = fmaxf(top, sh.top[w]);
@@ -234,86 +262,95 @@ __global__ void __launch_bounds__(TS_THREADS) attend_stage_kernel(AttendArgs a, 
   if (!hot && S % TQ_GROUP_TOK == 0) {
     // a warp expands the records of a group of 16 tokens: two tokens of a channel are a word of the image
     const int t = t0 + warp * TQ_GROUP_TOK, b = t / S, slot = t - b * S, r = lane >> 2, c = lane & 3;
-    if (t < t1) {
-      const uint8_t* grp = pages + (size_t)b * g.page_bytes + g.v_off + (size_t)(slot >> 4) * v_group_bytes(vb);
-      uint32_t w[9];
-      if (vb == 4) {
-        const uint4 x = *(const uint4*)(grp + lane * 16), y = *(const uint4*)(grp + 512 + lane * 16);
-        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          const uint2 x = *(const uint2*)(grp + i * 256 + lane * 8);
-          w[2 * i] = x.x, w[2 * i + 1] = x.y;
-        }
-        w[6] = w[7] = 0u;
-      }
-      w[8] = 0u;
-      float nv[2][2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) nv[h][x] = sh.norm[warp * TQ_GROUP_TOK + 8 * h + 2 * c + x] * up;
-#pragma unroll
-      for (int p = 0; p < 32; ++p) {
-        const int h = p & 1, d = r + 8 * (p >> 1);
-        uint32_t ca, cb;
-        if (vb == 4) {
-          const uint32_t by = w[p >> 2] >> (8 * (p & 3));
-          ca = by & 15, cb = by >> 4 & 15;
-        } else {
-          const uint32_t by = __funnelshift_r(w[6 * p >> 5], w[(6 * p >> 5) + 1], (6 * p) & 31);
-          ca = by & 7, cb = by >> 3 & 7;
-        }
-        const float x = nv[h][0] * sh.cent[ca], y = nv[h][1] * sh.cent[cb];
-        const uint32_t hi = ti_pair(x, y);
-        const int at = (2 * warp + h) * TI_LBO + d * 16 + 4 * c;
-        *(uint32_t*)(v_hi + at) = hi;
-        if (SPLIT) *(uint32_t*)(v_lo + at) = ti_rest(x, y, hi);
-      }
+    const bool there = t < t1;
+    const uint8_t* grp = pages + (size_t)(there ? b : 0) * g.page_bytes + g.v_off + (size_t)(there ? slot >> 4 : 0) * v_group_bytes(vb);
+    uint32_t w[9];
+    if (vb == 4) {
+      const uint4 x = *(const uint4*)(grp + lane * 16), y = *(const uint4*)(grp + 512 + lane * 16);
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
     } else {
-#pragma unroll 4
-      for (int p = 0; p < 32; ++p) {
-        const int at = (2 * warp + (p & 1)) * TI_LBO + (r + 8 * (p >> 1)) * 16 + 4 * c;
-        *(uint32_t*)(v_hi + at) = 0u;
-        if (SPLIT) *(uint32_t*)(v_lo + at) = 0u;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const uint2 x = *(const uint2*)(grp + i * 256 + lane * 8);
+        w[2 * i] = x.x, w[2 * i + 1] = x.y;
       }
+      w[6] = w[7] = 0u;
     }
-  } else {
-    // a thread has 8 tokens x 8 channels: window tokens v @ Pi^T, tokens of blocks from their codes
-    const int ty = tid >> 4, tx = tid & 15;
-    float x[8][8];
+    w[8] = 0u;
+    float nv[2][2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
-    if (hot) {
+      for (int x = 0; x < 2; ++x) nv[h][x] = there ? sh.norm[warp * TQ_GROUP_TOK + 8 * h + 2 * c + x] * up : 0.0f;
+#pragma unroll
+    for (int p = 0; p < 32; ++p) {
+      const int h = p & 1, d = r + 8 * (p >> 1);
+      uint32_t ca, cb;
+      if (vb == 4) {
+        const uint32_t by = w[p >> 2] >> (8 * (p & 3));
+        ca = by & 15, cb = by >> 4 & 15;
+      } else {
+        const uint32_t by = __funnelshift_r(w[6 * p >> 5], w[(6 * p >> 5) + 1], (6 * p) & 31);
+        ca = by & 7, cb = by >> 3 & 7;
+      }
+      const float x = nv[h][0] * sh.cent[ca], y = nv[h][1] * sh.cent[cb];
+      const uint32_t hi = ti_pair(x, y);
+      const int at = (2 * warp + h) * TI_LBO + d * 16 + 4 * c;
+      *(uint32_t*)(v_hi + at) = hi;
+      if (SPLIT) *(uint32_t*)(v_lo + at) = ti_rest(x, y, hi);
+    }
+    return;
+  }
+  // a thread has 8 tokens x 2 channels: window tokens v @ Pi^T, tokens of blocks from their codes
+  const int tg = tid >> 6, cp = tid & 63;
+  float(*vs)[TS_VS] = (float(*)[TS_VS])sh.k[0];
+#pragma unroll 1
+  for (int c0 = 0; c0 < TI_T; c0 += TS_VT) {
+    float x[8][2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i][0] = x[i][1] = 0.0f;
+    if (t0 + c0 + TS_VT > sq.cold && t0 + c0 < t1) {
+      __syncthreads();  // (the keys, or the rows before, have been read)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = tid >> 3, d = (tid & 7) * 16 + 8 * u, t = t0 + c0 + row;
+        float v[8];
+        if (t >= sq.cold && t < t1) {
+          ts_ld8(a.hot_v, ring + (size_t)(t % g.hot_cap) * TQ_D + d, g.kv_dtype, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+        }
+        *(float4*)&vs[row][d] = make_float4(v[0], v[1], v[2], v[3]);
+        *(float4*)&vs[row][d + 4] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+      __syncthreads();
 #pragma unroll 2
-      for (int d = 0; d < TQ_D; ++d) {
-        const float4 p0 = *(const float4*)&a.tables->pi_t[d * TQ_D + 8 * tx], p1 = *(const float4*)&a.tables->pi_t[d * TQ_D + 8 * tx + 4];
+      for (int d = 0; d < TQ_D; d += 4) {
+        float2 w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = *(const float2*)&a.tables->pi_t[(d + e) * TQ_D + 2 * cp];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float v = sh.v[8 * ty + i][d];
-          x[i][0] = fmaf(v, p0.x, x[i][0]), x[i][1] = fmaf(v, p0.y, x[i][1]);
-          x[i][2] = fmaf(v, p0.z, x[i][2]), x[i][3] = fmaf(v, p0.w, x[i][3]);
-          x[i][4] = fmaf(v, p1.x, x[i][4]), x[i][5] = fmaf(v, p1.y, x[i][5]);
-          x[i][6] = fmaf(v, p1.z, x[i][6]), x[i][7] = fmaf(v, p1.w, x[i][7]);
+          const float4 v = *(const float4*)&vs[8 * tg + i][d];
+          x[i][0] = fmaf(v.x, w[0].x, fmaf(v.y, w[1].x, fmaf(v.z, w[2].x, fmaf(v.w, w[3].x, x[i][0]))));
+          x[i][1] = fmaf(v.x, w[0].y, fmaf(v.y, w[1].y, fmaf(v.z, w[2].y, fmaf(v.w, w[3].y, x[i][1]))));
         }
       }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int t = t0 + 8 * ty + i;
+      const int t = t0 + c0 + 8 * tg + i;
       if (t < sq.cold) {
         const int b = t / S, slot = t - b * S;
         const uint8_t* grp = pages + (size_t)b * g.page_bytes + g.v_off + (size_t)(slot >> 4) * v_group_bytes(vb);
-        const float norm = sh.norm[8 * ty + i];
+        const float norm = sh.norm[c0 + 8 * tg + i];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = norm * sh.cent[v_get_code(grp, vb, slot & 15, 8 * tx + e)];
+        for (int e = 0; e < 2; ++e) x[i][e] = norm * sh.cent[v_get_code(grp, vb, slot & 15, 2 * cp + e)];
       }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 2; ++e) {
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -321,7 +358,7 @@ __global__ void __launch_bounds__(TS_THREADS) attend_stage_kernel(AttendArgs a, 
         hi[i] = ti_pair(p, q);
         if (SPLIT) lo[i] = ti_rest(p, q, hi[i]);
       }
-      const int at = ty * TI_LBO + (8 * tx + e) * 16;
+      const int at = (c0 / 8 + tg) * TI_LBO + (2 * cp + e) * 16;
       *(uint4*)(v_hi + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       if (SPLIT) *(uint4*)(v_lo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
@@ -332,7 +369,7 @@ __global__ void __launch_bounds__(TS_THREADS) attend_stage_kernel(AttendArgs a, 
 struct TiShared {
   alignas(128) uint8_t q[2][TI_IMAGE];
   alignas(128) uint8_t kv[TI_SLOTS][TI_IMAGE];
-  unsigned long long full[TI_SLOTS], empty[TI_SLOTS], q_ready, s_full[2], p_full[2], o_done[2];
+  unsigned long long full[TI_SLOTS], empty[TI_SLOTS], q_ready, s_full[2], p_half[2], p_full[2], o_done[2];
   uint32_t tmem;
 };
 
@@ -367,6 +404,54 @@ TQ_DEV void ti_st32(uint32_t addr, const uint32_t* r) {
       TI_R8(r, 0), TI_R8(r, 8), TI_R8(r, 16), TI_R8(r, 24)
       : "memory");
 }
+TQ_DEV float ti_max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// pairs of floats in one register pair
+TQ_DEV uint64_t ti_u2(uint32_t a, uint32_t b) {
+  uint64_t y;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "r"(a), "r"(b));
+  return y;
+}
+TQ_DEV uint64_t ti_f2(float a, float b) { return ti_u2(__float_as_uint(a), __float_as_uint(b)); }
+TQ_DEV float2 ti_floats(uint64_t x) {
+  float2 y;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
+  return y;
+}
+TQ_DEV uint64_t ti_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t y;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+  return y;
+}
+TQ_DEV uint64_t ti_add2(uint64_t a, uint64_t b) {
+  uint64_t y;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+  return y;
+}
+// 2^x on the special-function units, which do 16 a cycle and SM; and on the multiply-add units: x = n + f with n whole
+// and |f| <= 1/2, a polynomial of degree 4 for 2^f (least largest relative error, 2.6e-6, fitted for this), n
+// added to its exponent.  Both together finish sooner than either.  The polynomial takes what is below 2^-120 for
+// that.
+TQ_DEV float2 ti_exp2_unit(uint64_t x) {
+  const float2 y = ti_floats(x);
+  return make_float2(tq_exp2(y.x), tq_exp2(y.y));
+}
+TQ_DEV float2 ti_exp2_poly(uint64_t x) {
+  const float2 y = ti_floats(x);
+  const uint64_t z = ti_f2(fmaxf(y.x, -120.0f), fmaxf(y.y, -120.0f));
+  const uint64_t n = ti_add2(z, ti_f2(12582912.0f, 12582912.0f));  // 1.5 * 2^23: whole numbers in the low bits
+  const uint64_t f = ti_fma2(ti_add2(n, ti_f2(-12582912.0f, -12582912.0f)), ti_f2(-1.0f, -1.0f), z);
+  uint64_t p = ti_fma2(ti_f2(0.009570101791435913f, 0.009570101791435913f), f, ti_f2(0.05591786030999481f, 0.05591786030999481f));
+  p = ti_fma2(p, f, ti_f2(0.24024744830820266f, 0.24024744830820266f));
+  p = ti_fma2(p, f, ti_f2(0.6931218147384395f, 0.6931218147384395f));
+  p = ti_fma2(p, f, ti_f2(0.9999992614448223f, 0.9999992614448223f));
+  const float2 m = ti_floats(n), w = ti_floats(p);
+  return make_float2(__uint_as_float(__float_as_uint(w.x) + (__float_as_uint(m.x) << 23)),
+                     __uint_as_float(__float_as_uint(w.y) + (__float_as_uint(m.y) << 23)));
+}
 TQ_DEV void ti_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 TQ_DEV void ti_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 TQ_DEV void ti_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -399,6 +484,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(enc_smem(&sh.s_full[i]), 1);
+      mbar_init(enc_smem(&sh.p_half[i]), 128);
       mbar_init(enc_smem(&sh.p_full[i]), 128);
       mbar_init(enc_smem(&sh.o_done[i]), 1);
     }
@@ -483,14 +569,17 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
         if (k + 1 < n)
           for (int i = 0; i < PARTS; ++i) landed(ck + i);
         for (int x = 0; x < groups; ++x) {
-          wait(&sh.p_full[x], k & 1);
-          ti_fence_after();
 #pragma unroll
-          for (int i = PARTS - 1; i >= 0; --i) {
-            const uint64_t b = image(cv + i);
+          for (int h = 0; h < 2; ++h) {  // the first half of the tokens while the second's probabilities are made
+            wait(h == 0 ? &sh.p_half[x] : &sh.p_full[x], k & 1);
+            ti_fence_after();
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              ti_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * j, b + j * STEP, idesc, k > 0 || i < PARTS - 1 || j > 0);
+            for (int i = PARTS - 1; i >= 0; --i) {
+              const uint64_t b = image(cv + i);
+#pragma unroll
+              for (int j = 4 * h; j < 4 * h + 4; ++j)
+                ti_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * j, b + j * STEP, idesc, k > 0 || i < PARTS - 1 || j > 0);
+            }
           }
           umma_commit(enc_smem(&sh.o_done[x]));
           if (x == groups - 1) release(cv);
@@ -564,7 +653,8 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
 #pragma unroll
       for (int i = 0; i < 4; ++i) ti_ld32(ts + 32 * i, v + 32 * i);
       ti_wait_ld();
-      if (!(whole && t0 + TI_T - 1 <= p_lo && (t0 >= w_hi || t0 + TI_T <= a.sinks))) {
+      const bool open = whole && t0 + TI_T - 1 <= p_lo && (t0 >= w_hi || t0 + TI_T <= a.sinks);
+      if (!open) {
         const int hi = min(p, sq.n - 1) - t0, lo = w - t0, sk = a.sinks - t0;
 #pragma unroll
         for (int i = 0; i < 128; ++i)
@@ -572,7 +662,8 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(v[i]));
+      for (int i = 0; i < 128; i += 2)
+        top[i / 2 & 3] = ti_max3(top[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
       const float now = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), factor, e);
       const bool grown = now > m + TI_GROW;  // (also from -inf)
       float down = 1.0f;
@@ -595,23 +686,34 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
         }
       }
       const float off = TI_LIFT + e - (m > -INFINITY ? m : 0.0f);
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const uint64_t factor2 = ti_f2(factor, factor), off2 = ti_f2(off, off);
+      uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t h[32];
+        if (open) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float y = tq_exp2(fmaf(__uint_as_float(v[64 * i + 2 * j]), factor, off));
-          const float z = tq_exp2(fmaf(__uint_as_float(v[64 * i + 2 * j + 1]), factor, off));
-          sum[j & 3] += y + z;
-          h[j] = ti_pair(y, z);
+          for (int j = 0; j < 32; ++j) {
+            const uint64_t y = ti_fma2(ti_u2(v[64 * i + 2 * j], v[64 * i + 2 * j + 1]), factor2, off2);
+            const float2 z = j % 8 < TI_POLY ? ti_exp2_poly(y) : ti_exp2_unit(y);
+            sum[j & 1] = ti_add2(sum[j & 1], ti_f2(z.x, z.y));
+            h[j] = ti_pair(z.x, z.y);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float2 z = ti_exp2_unit(ti_fma2(ti_u2(v[64 * i + 2 * j], v[64 * i + 2 * j + 1]), factor2, off2));
+            sum[j & 1] = ti_add2(sum[j & 1], ti_f2(z.x, z.y));
+            h[j] = ti_pair(z.x, z.y);
+          }
         }
         ti_st32(ts + 32 * i, h);
+        ti_wait_st();
+        ti_fence_before();
+        mbar_arrive(enc_smem(i == 0 ? &sh.p_half[x] : &sh.p_full[x]));
       }
-      ti_wait_st();
-      ti_fence_before();
-      mbar_arrive(enc_smem(&sh.p_full[x]));
-      l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), exp2f(-e), l * down);
+      const float2 s2 = ti_floats(ti_add2(sum[0], sum[1]));
+      l = fmaf(s2.x + s2.y, exp2f(-e), l * down);
     }
     // the row's state: [channel][row], neighbouring threads side by side
     const size_t part = ((size_t)unit * ta.splits + split) * ta.row_tiles + rt;
@@ -643,95 +745,137 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
 }
 
 // ---------------------------------------------------------------------------------------------------
-// 64 rows of a unit: the splits' sums in order, sum @ Pi, over the sum of the weights.
-constexpr int TC_ROWS = 64, TC_THREADS = 256, TC_S = TC_ROWS + 4;
-__global__ void __launch_bounds__(TC_THREADS) attend_tiles_combine_kernel(AttendArgs a, TileArgs ta, int tiles) {
-  __shared__ __align__(16) float c[TQ_D][TC_S];
+// The splits' sums in order, over the sum of the weights, times Pi.  CTAs take tiles of 64 rows in turn.  The
+// merged rows go to shared memory as fp16 pairs hi + lo, each row scaled by a power of two, and through mma.sync as the
+// B operand against Pi^T, whose pairs a warp keeps in registers (16 channels of the output each): hi * hi + hi * lo +
+// lo * hi, good to 2^-22.  Bound by reading the sums.
+constexpr int TC_ROWS = 64, TC_THREADS = 256, TC_PITCH = TQ_D * 2 + 16;
+
+TQ_DEV void tc_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__global__ void __launch_bounds__(TC_THREADS, 2) attend_tiles_combine_kernel(AttendArgs a, TileArgs ta, int tiles, int total) {
+  __shared__ __align__(16) uint8_t hi[TC_ROWS * TC_PITCH], lo[TC_ROWS * TC_PITCH];
+  __shared__ float top_s[4][TC_ROWS], inv_s[TC_ROWS];
   const tq_geom& g = a.g;
-  const int tid = threadIdx.x, unit = blockIdx.x / tiles, row0 = blockIdx.x % tiles * TC_ROWS;
-  const int H = g.n_kv_heads, G = g.group, s = unit / H, head = unit % H;
-  const int rows = min(TC_ROWS, a.rows - row0);
-  if (ta.left[unit] != 0) {  // the general kernel's states: blocks and window, the latter not in code space
-    for (int i = tid; i < rows * TQ_D; i += TC_THREADS) {
-      const int r = i / TQ_D, e = i % TQ_D, row = row0 + r;
-      const float* p = attend_partial(a, unit, row, 0);
-      const float* q = p + TQ_PART_STRIDE;
-      const float M = fmaxf(p[0], q[0]), by = M > -INFINITY ? M : 0.0f;
-      const float wp = p[1] == 0.0f ? 0.0f : p[0] > -INFINITY ? tq_exp2(p[0] - by) : 1.0f;
-      const float wq = q[1] == 0.0f ? 0.0f : q[0] > -INFINITY ? tq_exp2(q[0] - by) : 1.0f;
-      float x = 0.0f;
-      if (wp != 0.0f)
-        for (int d = 0; d < TQ_D; ++d) x = fmaf(p[2 + d] * wp, a.tables->pi[d * TQ_D + e], x);
-      if (wq != 0.0f) x = fmaf(q[2 + e], wq, x);
-      const float L = (wp != 0.0f ? p[1] * wp : 0.0f) + (wq != 0.0f ? q[1] * wq : 0.0f);
-      x = L == 0.0f ? 0.0f : x / L;
-      const size_t at = (((size_t)s * a.n_tokens + row / G) * g.n_q_heads + head * G + row % G) * TQ_D + e;
-      if (a.q_dtype == TQ_F16) ((__half*)a.out)[at] = __float2half_rn(x);
-      else ((__nv_bfloat16*)a.out)[at] = __float2bfloat16_rn(x);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, q = lane >> 2, c = lane & 3;
+  const int H = g.n_kv_heads, G = g.group;
+  uint32_t ph[8][4], pl[8][4];  // A: rows = output channels 16 warp .., k = input channels
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 x = *(const float2*)&a.tables->pi_t[(16 * warp + q + 8 * (i & 1)) * TQ_D + 16 * k + 2 * c + 8 * (i >> 1)];
+      ph[k][i] = ti_pair(x.x * 256.0f, x.y * 256.0f);
+      pl[k][i] = ti_rest(x.x * 256.0f, x.y * 256.0f, ph[k][i]);
     }
-    return;
-  }
-  const int rt = row0 / TI_ROWS, in = row0 % TI_ROWS;
-  {
-    const int r = tid % TC_ROWS, d0 = tid / TC_ROWS * (TQ_D * TC_ROWS / TC_THREADS);
-    float M = -INFINITY, L = 0.0f;
-    float x[TQ_D * TC_ROWS / TC_THREADS];
-    constexpr int N = TQ_D * TC_ROWS / TC_THREADS;
+  for (int item = blockIdx.x; item < total; item += gridDim.x) {
+    const int unit = item / tiles, row0 = item % tiles * TC_ROWS, s = unit / H, head = unit % H;
+    const int rows = min(TC_ROWS, a.rows - row0);
+    auto out_at = [&](int row) {
+      return (((size_t)s * a.n_tokens + row / G) * g.n_q_heads + head * G + row % G) * TQ_D;
+    };
+    if (ta.left[unit] != 0) {  // the general kernel's states: blocks and window, the latter not in code space
+      for (int i = tid; i < rows * TQ_D; i += TC_THREADS) {
+        const int e = i % TQ_D, row = row0 + i / TQ_D;
+        const float* x = attend_partial(a, unit, row, 0);
+        const float* y = x + TQ_PART_STRIDE;
+        const float M = fmaxf(x[0], y[0]), by = M > -INFINITY ? M : 0.0f;
+        const float wx = x[1] == 0.0f ? 0.0f : x[0] > -INFINITY ? tq_exp2(x[0] - by) : 1.0f;
+        const float wy = y[1] == 0.0f ? 0.0f : y[0] > -INFINITY ? tq_exp2(y[0] - by) : 1.0f;
+        float o = 0.0f;
+        if (wx != 0.0f)
+          for (int d = 0; d < TQ_D; ++d) o = fmaf(x[2 + d] * wx, a.tables->pi[d * TQ_D + e], o);
+        if (wy != 0.0f) o = fmaf(y[2 + e], wy, o);
+        const float L = (wx != 0.0f ? x[1] * wx : 0.0f) + (wy != 0.0f ? y[1] * wy : 0.0f);
+        o = L == 0.0f ? 0.0f : o / L;
+        if (a.q_dtype == TQ_F16) ((__half*)a.out)[out_at(row) + e] = __float2half_rn(o);
+        else ((__nv_bfloat16*)a.out)[out_at(row) + e] = __float2bfloat16_rn(o);
+      }
+      continue;
+    }
+    const int rt = row0 / TI_ROWS, in = row0 % TI_ROWS;
+    constexpr int N = TQ_D * TC_ROWS / TC_THREADS;  // channels of a thread
+    const int r = tid % TC_ROWS, part = tid / TC_ROWS;
+    float x[N], L = 0.0f, M = -INFINITY;
 #pragma unroll
     for (int i = 0; i < N; ++i) x[i] = 0.0f;
     if (r < rows) {
-      for (int i = 0; i < ta.splits; ++i)
-        M = fmaxf(M, ta.stats[((((size_t)unit * ta.splits + i) * ta.row_tiles + rt) * 2) * TI_ROWS + in + r]);
+      const float* stats = ta.stats + ((size_t)unit * ta.splits * ta.row_tiles + rt) * 2 * TI_ROWS + in + r;
+      const size_t step = (size_t)ta.row_tiles * 2 * TI_ROWS;
+      const float* sums = ta.sums + (size_t)unit * a.unit_stride + ((size_t)rt * TQ_D + part * N) * TI_ROWS + in + r;
+      for (int i = 0; i < ta.splits; ++i) M = fmaxf(M, stats[i * step]);
       const float by = M > -INFINITY ? M : 0.0f;
       for (int i = 0; i < ta.splits; ++i) {
-        const size_t part = ((size_t)unit * ta.splits + i) * ta.row_tiles + rt;
-        const float mi = ta.stats[part * 2 * TI_ROWS + in + r], li = ta.stats[(part * 2 + 1) * TI_ROWS + in + r];
+        const float mi = stats[i * step], li = stats[i * step + TI_ROWS];
         if (li == 0.0f) continue;
         const float w = mi > -INFINITY ? tq_exp2(mi - by) : 1.0f;
         L += li * w;
-        const float* from = ta.sums + (size_t)unit * a.unit_stride + (((size_t)i * ta.row_tiles + rt) * TQ_D + d0) * TI_ROWS + in + r;
+        const float* from = sums + (size_t)i * ta.row_tiles * TI_ROWS * TQ_D;
 #pragma unroll
         for (int k = 0; k < N; ++k) x[k] = fmaf(from[k * TI_ROWS], w, x[k]);
       }
     }
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    float top = 0.0f;
 #pragma unroll
-    for (int k = 0; k < N; ++k) c[d0 + k][r] = x[k] * inv;
-  }
-  __syncthreads();
-  // a thread has 4 rows x 8 channels
-  const int ty = tid >> 4, tx = tid & 15;
-  float y[4][8];
+    for (int k = 0; k < N; ++k) top = fmaxf(top, fabsf(x[k]));
+    __syncthreads();  // (the tile before has been read)
+    top_s[part][r] = top;
+    __syncthreads();
+    float exponent;
+    const float up = ti_lift(fmaxf(fmaxf(top_s[0][r], top_s[1][r]), fmaxf(top_s[2][r], top_s[3][r])), 13, exponent);
+    if (part == 0) inv_s[r] = L == 0.0f ? 0.0f : exp2f(exponent - 8.0f) / L;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int k = 0; k < N; k += 8) {
+      uint32_t h[4], l[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[i][e] = 0.0f;
-#pragma unroll 4
-  for (int d = 0; d < TQ_D; ++d) {
-    const float4 r4 = *(const float4*)&c[d][4 * ty];
-    const float4 p0 = *(const float4*)&a.tables->pi[d * TQ_D + 8 * tx], p1 = *(const float4*)&a.tables->pi[d * TQ_D + 8 * tx + 4];
-    const float rr[4] = {r4.x, r4.y, r4.z, r4.w}, pp[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+      for (int i = 0; i < 4; ++i) {
+        const float u = x[k + 2 * i] * up, v = x[k + 2 * i + 1] * up;
+        h[i] = ti_pair(u, v);
+        l[i] = ti_rest(u, v, h[i]);
+      }
+      const int at = r * TC_PITCH + (part * N + k) * 2;
+      *(uint4*)(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+      *(uint4*)(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+    __syncthreads();
+#pragma unroll 2
+    for (int nt = 0; nt < TC_ROWS / 8; ++nt) {
+      if (8 * nt >= rows) break;
+      float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const int at = (8 * nt + q) * TC_PITCH + 4 * c;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t h0 = *(const uint32_t*)(hi + at + 32 * k), h1 = *(const uint32_t*)(hi + at + 32 * k + 16);
+        const uint32_t l0 = *(const uint32_t*)(lo + at + 32 * k), l1 = *(const uint32_t*)(lo + at + 32 * k + 16);
+        tc_mma(d, pl[k], h0, h1);
+        tc_mma(d, ph[k], l0, l1);
+        tc_mma(d, ph[k], h0, h1);
+      }
+      // channels q, q + 8 of the warp's sixteen; rows 2 c, 2 c + 1
+      const float f0 = inv_s[8 * nt + 2 * c], f1 = inv_s[8 * nt + 2 * c + 1];
+      uint32_t w[2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[i][e] = fmaf(rr[i], pp[e], y[i][e]);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 4 * ty + i, row = row0 + r;
-    if (r >= rows) continue;
-    const size_t at = (((size_t)s * a.n_tokens + row / G) * g.n_q_heads + head * G + row % G) * TQ_D + 8 * tx;
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (a.q_dtype == TQ_F16) {
-        w[e] = ti_pair(y[i][2 * e], y[i][2 * e + 1]);
-      } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(y[i][2 * e], y[i][2 * e + 1]);
-        w[e] = *(const uint32_t*)&h;
+      for (int y = 0; y < 2; ++y) {
+        const float u = d[2 * y] * f0, v = d[2 * y + 1] * f1;
+        if (a.q_dtype == TQ_F16) {
+          w[y] = ti_pair(u, v);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(u, v);
+          w[y] = *(const uint32_t*)&h;
+        }
+        asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(w[y]) : "r"(w[y]));
+      }
+      const int row = 8 * nt + q;  // now two neighbouring channels of row q
+      if (row < rows) {
+        uint16_t* to = (uint16_t*)a.out + out_at(row0 + row) + 16 * warp + 2 * c;
+        *(uint32_t*)to = w[0];
+        *(uint32_t*)(to + 8) = w[1];
       }
     }
-    *(uint4*)((uint16_t*)a.out + at) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -780,7 +924,8 @@ size_t tq_attend_tiles_bytes(const AttendArgs& a, int units, int cap, int splits
   return layout(a, units, cap, splits).total;
 }
 
-int tq_launch_attend_tiles(const AttendArgs& base, void* workspace, int cap, int splits, cudaStream_t st) {
+int tq_launch_attend_tiles(const AttendArgs& base, void* workspace, int cap, int splits, int device,
+                           cudaStream_t st) {
   AttendArgs a = base;
   const int units = a.seq_count * a.g.n_kv_heads;
   const Layout l = layout(a, units, cap, splits);
@@ -806,7 +951,9 @@ int tq_launch_attend_tiles(const AttendArgs& base, void* workspace, int cap, int
   if (rc != TQ_OK) return rc;
   rc = tq_launch_attend_general(a, st);
   if (rc != TQ_OK) return rc;
-  attend_tiles_combine_kernel<<<units * tiles, TC_THREADS, 0, st>>>(a, ta, tiles);
+  int sm_count = 148;
+  TQ_CUDA(cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, device));
+  attend_tiles_combine_kernel<<<std::min(units * tiles, 2 * sm_count), TC_THREADS, 0, st>>>(a, ta, tiles, units * tiles);
   TQ_CUDA(cudaGetLastError());
   return TQ_OK;
 }
