@@ -38,7 +38,7 @@ constexpr int TI_SLOTS = 5;                  // images in shared memory
 constexpr int TI_THREADS = 320;              // two softmax groups, a warp that issues, a warp that loads
 constexpr float TI_KEY = 16.0f;              // keys are divided by it
 constexpr float TI_LIFT = 7.0f, TI_GROW = 8.0f;  // probabilities reach 2^(7 + 8) at most
-constexpr int TI_POLY = 3;                   // of eight pairs of exponentials, those on the multiply-add units
+constexpr int TI_POLY = 2;                   // of eight pairs of exponentials, those on the multiply-add units
 constexpr int TI_WAIT = 1 << 21;             // probes of a wait, a microsecond or two each at most
 
 struct TileArgs {
@@ -387,6 +387,16 @@ TQ_DEV void ti_mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint
       "r"(ta), "l"(db), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// (without a time to sleep: the waiting threads have little slack)
+TQ_DEV bool ti_try_wait(uint32_t bar, unsigned parity) {
+  unsigned done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 #define TI_R8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
 #define TI_W8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
 TQ_DEV void ti_ld32(uint32_t addr, uint32_t* r) {
@@ -435,9 +445,14 @@ TQ_DEV uint64_t ti_add2(uint64_t a, uint64_t b) {
 // and |f| <= 1/2, a polynomial of degree 4 for 2^f (least largest relative error, 2.6e-6, fitted for this), n
 // added to its exponent.  Both together finish sooner than either.  The polynomial takes what is below 2^-120 for
 // that.
+TQ_DEV float ti_exp2(float x) {  // (results below 2^-126 are zero: nothing next to the row's largest, and one instruction)
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 TQ_DEV float2 ti_exp2_unit(uint64_t x) {
   const float2 y = ti_floats(x);
-  return make_float2(tq_exp2(y.x), tq_exp2(y.y));
+  return make_float2(ti_exp2(y.x), ti_exp2(y.y));
 }
 TQ_DEV float2 ti_exp2_poly(uint64_t x) {
   const float2 y = ti_floats(x);
@@ -505,7 +520,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
   bool gave_up = false;
   auto wait = [&](unsigned long long* bar, unsigned parity) {
     const uint32_t at = enc_smem(bar);
-    for (int i = 0; !gave_up && !mbar_try_wait(at, parity);)
+    for (int i = 0; !gave_up && !ti_try_wait(at, parity);)
       if (++i >= limit) {
         atomicOr(a.status, TQ_STATUS_WAIT_TIMEOUT);
         gave_up = true;
