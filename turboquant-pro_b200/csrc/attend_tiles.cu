@@ -373,19 +373,23 @@ struct TiShared {
   uint32_t tmem;
 };
 
-TQ_DEV void ti_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
-      : "memory");
+// (accumulate: known where the call stands, so that no predicate has to be formed)
+template <bool ACC>
+TQ_DEV void ti_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+               "l"(da), "l"(db), "r"(idesc), "n"(ACC ? 1 : 0)
+               : "memory");
 }
-TQ_DEV void ti_mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(ta), "l"(db), "r"(idesc), "r"(accumulate)
-      : "memory");
+template <bool ACC>
+TQ_DEV void ti_mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+               "r"(ta), "l"(db), "r"(idesc), "n"(ACC ? 1 : 0)
+               : "memory");
+}
+TQ_DEV bool ti_elect() {  // one thread of the (converged) warp
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(on));
+  return on != 0;
 }
 // (without a time to sleep: the waiting threads have little slack)
 TQ_DEV bool ti_try_wait(uint32_t bar, unsigned parity) {
@@ -513,7 +517,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
   ti_fence_before();
   __syncthreads();
   ti_fence_after();
-  const uint32_t tmem = *(volatile uint32_t*)&sh.tmem;
+  constexpr uint32_t tmem = 0;  // (all 512 columns are this CTA's: they begin at the first)
 
   // Bounded waits: one that runs out sets the status bit, and the thread then waits for nothing more.
   const int limit = TI_WAIT;
@@ -554,60 +558,96 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
     }
   } else if (warp == 8) {
     // ---- products
-    if (lane == 0 && n > 0) {
+    // The whole warp runs this, one thread issues.  What the products take are constants or the same in all lanes to
+    // the compiler's knowledge (the shuffle), so that it lies in uniform registers: fetched there product by product,
+    // each took about a hundred cycles to issue, more than its execution.
+    const int n_u = __shfl_sync(0xffffffffu, n, 0), groups_u = __shfl_sync(0xffffffffu, groups, 0);
+    if (n_u > 0) {
       constexpr uint32_t idesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
       constexpr uint64_t STEP = 2 * TI_LBO >> 4;  // 16 deep
-      auto image = [&](int c) { return umma_desc_k_major(enc_smem(sh.kv[c % TI_SLOTS]), TI_LBO, TI_SBO); };
-      auto landed = [&](int c) { wait(&sh.full[c % TI_SLOTS], (c / TI_SLOTS) & 1); };
+      const uint64_t q0 = umma_desc_k_major(enc_smem(sh.q[0]), TI_LBO, TI_SBO);
+      const uint64_t kv0 = umma_desc_k_major(enc_smem(sh.kv[0]), TI_LBO, TI_SBO);
+      auto image = [&](int c) { return kv0 + (uint64_t)((uint32_t)(c % TI_SLOTS) * (TI_IMAGE >> 4)); };
+      auto wait_all = [&](unsigned long long* bar, unsigned parity) {  // (the warp stays together)
+        wait(bar, parity);
+        gave_up = __any_sync(0xffffffffu, gave_up);
+      };
+      auto landed = [&](int c) { wait_all(&sh.full[c % TI_SLOTS], (c / TI_SLOTS) & 1); };
       // scores of half x against the keys of tile k
       auto scores = [&](int x, int k) {
-        const uint64_t q = umma_desc_k_major(enc_smem(sh.q[x]), TI_LBO, TI_SBO);
+        uint64_t b[PARTS];
 #pragma unroll
-        for (int i = PARTS - 1; i >= 0; --i) {
-          const uint64_t b = image(2 * PARTS * k + i);
+        for (int i = 0; i < PARTS; ++i) b[i] = image(2 * PARTS * k + i);
+        if (ti_elect()) {
+          const uint64_t q = q0 + (uint64_t)(x * (TI_IMAGE >> 4));
+          const uint32_t d = tmem + 128 * x;
+          ti_mma<false>(d, q, b[PARTS - 1], idesc);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) ti_mma(tmem + 128 * x, q + j * STEP, b + j * STEP, idesc, i < PARTS - 1 || j > 0);
+          for (int j = 1; j < 8; ++j) ti_mma<true>(d, q + j * STEP, b[PARTS - 1] + j * STEP, idesc);
+          if (SPLIT)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ti_mma<true>(d, q + j * STEP, b[0] + j * STEP, idesc);
+          umma_commit(enc_smem(&sh.s_full[x]));
         }
-        umma_commit(enc_smem(&sh.s_full[x]));
+        __syncwarp();
       };
       auto release = [&](int c) {  // the parts of an operand, once the products issued so far are done
-        for (int i = 0; i < PARTS; ++i) umma_commit(enc_smem(&sh.empty[(c + i) % TI_SLOTS]));
+        if (ti_elect())
+#pragma unroll
+          for (int i = 0; i < PARTS; ++i) umma_commit(enc_smem(&sh.empty[(c + i) % TI_SLOTS]));
+        __syncwarp();
       };
-      wait(&sh.q_ready, 0);
+      // half h of the tokens of a tile, its values in chunk c: O += P V
+      auto values = [&](int x, int h, int c, bool fresh) {
+        uint64_t b[PARTS];
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) b[i] = image(c + i) + 4 * h * STEP;
+        if (ti_elect()) {
+          const uint32_t d = tmem + 256 + 128 * x, p = tmem + 128 * x + 32 * h;
+          if (fresh) ti_mma_ts<false>(d, p, b[PARTS - 1], idesc);
+          else ti_mma_ts<true>(d, p, b[PARTS - 1], idesc);
+#pragma unroll
+          for (int j = 1; j < 4; ++j) ti_mma_ts<true>(d, p + 8 * j, b[PARTS - 1] + j * STEP, idesc);
+          if (SPLIT)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ti_mma_ts<true>(d, p + 8 * j, b[0] + j * STEP, idesc);
+          if (h == 1) umma_commit(enc_smem(&sh.o_done[x]));
+        }
+        __syncwarp();
+      };
+      wait_all(&sh.q_ready, 0);
       for (int i = 0; i < PARTS; ++i) landed(i);
       ti_fence_after();
-      for (int x = 0; x < groups; ++x) scores(x, 0);
+      scores(0, 0);
+      if (groups_u > 1) scores(1, 0);
       release(0);
-      for (int k = 0; k < n; ++k) {
+#pragma unroll 1
+      for (int k = 0; k < n_u; ++k) {
         const int cv = 2 * PARTS * k + PARTS, ck = cv + PARTS;  // values of this tile, keys of the next
         for (int i = 0; i < PARTS; ++i) landed(cv + i);
-        if (k + 1 < n)
+        if (k + 1 < n_u)
           for (int i = 0; i < PARTS; ++i) landed(ck + i);
-        for (int x = 0; x < groups; ++x) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {  // the first half of the tokens while the second's probabilities are made
-            wait(h == 0 ? &sh.p_half[x] : &sh.p_full[x], k & 1);
-            ti_fence_after();
-#pragma unroll
-            for (int i = PARTS - 1; i >= 0; --i) {
-              const uint64_t b = image(cv + i);
-#pragma unroll
-              for (int j = 4 * h; j < 4 * h + 4; ++j)
-                ti_mma_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * j, b + j * STEP, idesc, k > 0 || i < PARTS - 1 || j > 0);
-            }
-          }
-          umma_commit(enc_smem(&sh.o_done[x]));
-          if (x == groups - 1) release(cv);
-          if (k + 1 < n) {
+        for (int x = 0; x < 2; ++x) {
+          if (x >= groups_u) break;
+          // (the first half of the tokens while the second's probabilities are made)
+          wait_all(&sh.p_half[x], k & 1);
+          ti_fence_after();
+          values(x, 0, cv, k == 0);
+          wait_all(&sh.p_full[x], k & 1);
+          ti_fence_after();
+          values(x, 1, cv, false);
+          if (x == groups_u - 1) release(cv);
+          if (k + 1 < n_u) {
             // the next scores take the place of the probabilities that these products read
-            wait(&sh.o_done[x], k & 1);
+            wait_all(&sh.o_done[x], k & 1);
             scores(x, k + 1);
           }
         }
-        if (k + 1 < n) release(ck);
+        if (k + 1 < n_u) release(ck);
       }
-      gave_up = false;  // (nor are products under way then)
-      for (int x = 0; x < groups; ++x) wait(&sh.o_done[x], (n - 1) & 1);
+      gave_up = false;  // (nor are products under way when the CTA's memory goes)
+      for (int x = 0; x < groups_u; ++x) wait_all(&sh.o_done[x], (n_u - 1) & 1);
     }
   } else if (warp < 4 * groups) {
     // ---- a thread per row
