@@ -182,7 +182,8 @@ int32_t tq_decode(tq_ctx* ctx, int32_t layer, const void* q, int32_t q_dtype, fl
  * j > p - window.  Rows that see nothing (i >= n, p < 0, an empty sequence) become zeros. */
 typedef struct tq_attend_args {
   const void* q;            /* device: element (s, i, head, d) at s * q_seq_stride + i * q_tok_stride +
-                             * head * q_head_stride + d (strides in elements)                        */
+                             * head * q_head_stride + d (strides in elements); rows aligned to 16
+                             * bytes                                                               */
   void* out;                /* device, [seq_count][n_tokens][n_q_heads][D] of q_dtype; aligned to 16   */
   const int32_t* q_lens;    /* device, [seq_count], values below 0 and above n_tokens count as these;
                              * null: n_tokens each                                                 */

@@ -13,7 +13,8 @@ struct Plan {
   Form form;
   int ns_cold, ns_hot;
   int cap, splits;   // TILES: tiles that a (sequence, KV head) has room for, splits of them
-  size_t seq_bytes;  // workspace of a sequence
+  int seqs;          // most sequences of a launch
+  size_t fixed_bytes, seq_bytes;  // workspace: of a launch, of a sequence
 };
 
 int check_args(const tq_ctx* ctx, const tq_attend_args* r) {
@@ -27,6 +28,10 @@ int check_args(const tq_ctx* ctx, const tq_attend_args* r) {
   TQ_REQUIRE(r->window >= 0 && r->sinks >= 0, TQ_ERR_INVALID, "window and sinks must not be negative");
   TQ_REQUIRE(r->q_dtype == TQ_F32 || r->q_dtype == TQ_F16 || r->q_dtype == TQ_BF16, TQ_ERR_INVALID,
              "bad q_dtype");
+  const int64_t step = 16 / elem_size(r->q_dtype);
+  TQ_REQUIRE(r->q_seq_stride % step == 0 && r->q_tok_stride % step == 0 && r->q_head_stride % step == 0 &&
+                 (uintptr_t)r->q % 16 == 0 && (uintptr_t)r->out % 16 == 0,
+             TQ_ERR_INVALID, "q, its strides and out must be aligned to 16 bytes");
   return TQ_OK;
 }
 
@@ -47,6 +52,7 @@ int most_tokens(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
 Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
   const tq_geom& g = ctx->g;
   Plan p = {};
+  p.seqs = INT_MAX;
   const int n = most_tokens(ctx, r, st), rows = r->n_tokens * g.group;
   const int nb = n_cold_blocks(n, g.hot_window, g.block_tokens);
   const bool channels = g.key_mode != TQ_KEYS_POLAR && !ctx->force_generic;
@@ -75,8 +81,24 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
     p.seq_bytes = tq_attend_tiles_bytes(a, g.n_kv_heads, p.cap, p.splits);
     return p;
   }
-  const int row_tile = p.form == ROWS ? tq_attend_rows_tile(rows) : rows <= 16 ? 16 : 64;
-  const int cold_size = p.form == ROWS ? 256 : 64, hot_size = p.form == ROWS ? 128 : 64;
+  if (p.form == ROWS) {
+    AttendArgs a = {};
+    a.g = g;
+    a.rows = rows;
+    a.seq_count = r->seq_count;
+    a.n_tokens = r->n_tokens;
+    a.window = r->window == 0 ? INT_MAX : r->window;
+    a.sinks = r->sinks;
+    a.q_dtype = r->q_dtype;
+    const AttendRowsPlan rp = tq_attend_rows_plan(a, n, sm_count);
+    p.ns_cold = rp.ns_cold, p.ns_hot = rp.ns_hot;
+    p.seqs = rp.seqs;
+    p.fixed_bytes = rp.plan_bytes;
+    p.seq_bytes = (size_t)g.n_kv_heads * rows * (p.ns_cold + p.ns_hot) * TQ_PART_STRIDE * 4;
+    return p;
+  }
+  const int row_tile = rows <= 16 ? 16 : 64;
+  constexpr int cold_size = 64, hot_size = 64;
   // tokens in blocks that the rows of a tile can see
   const int64_t in_blocks = (int64_t)nb * g.block_tokens;
   const int64_t seen = r->window == 0 ? in_blocks
@@ -102,7 +124,7 @@ extern "C" int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* r, voi
   TQ_REQUIRE(bytes != nullptr, TQ_ERR_INVALID, "null argument");
   const Plan p = make_plan(ctx, r, (cudaStream_t)stream);
   const size_t n = std::max<size_t>(AT_ONE_GO / std::max<size_t>(p.seq_bytes, 1), 1);
-  *bytes = align_up(std::min<size_t>(n, r->seq_count) * p.seq_bytes, 256);
+  *bytes = align_up(p.fixed_bytes + std::min({n, (size_t)r->seq_count, (size_t)p.seqs}) * p.seq_bytes, 256);
   return TQ_OK;
 }
 
@@ -117,9 +139,12 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
   TQ_CUDA(cudaSetDevice(ctx->device));
   cudaStream_t st = (cudaStream_t)stream;
   const Plan p = make_plan(ctx, r, st);
-  TQ_REQUIRE(r->workspace_bytes >= p.seq_bytes, TQ_ERR_CAPACITY,
+  TQ_REQUIRE(r->workspace_bytes >= p.fixed_bytes + p.seq_bytes, TQ_ERR_CAPACITY,
              "workspace smaller than tq_attend_workspace asked for");
-  const int at_once = (int)std::min<size_t>(r->workspace_bytes / p.seq_bytes, r->seq_count);
+  const int at_once =
+      (int)std::min({(r->workspace_bytes - p.fixed_bytes) / p.seq_bytes, (size_t)r->seq_count, (size_t)p.seqs});
+  int sm_count = 148;
+  cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, ctx->device);
 
   AttendArgs a = {};
   a.g = g;
@@ -133,7 +158,8 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
   a.status = (int32_t*)((uint8_t*)ctx->b.state + state_status_off(g));
   a.tables = (const Tables*)ctx->b.tables;
   a.q_seq = r->q_seq_stride, a.q_tok = r->q_tok_stride, a.q_head = r->q_head_stride;
-  a.partials = (float*)r->workspace;
+  a.plan = r->workspace;
+  a.partials = (float*)((uint8_t*)r->workspace + p.fixed_bytes);
   a.layer = r->layer;
   a.n_tokens = r->n_tokens;
   a.q_dtype = r->q_dtype;
@@ -156,7 +182,13 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
       ctx->last_launches += 4;
       continue;
     }
-    rc = p.form == ROWS ? tq_launch_attend_rows(a, st) : tq_launch_attend_general(a, st);
+    if (p.form == ROWS) {
+      rc = tq_launch_attend_rows(a, sm_count, st);
+      if (rc != TQ_OK) return rc;
+      ctx->last_launches += 2;
+      continue;
+    }
+    rc = tq_launch_attend_general(a, st);
     if (rc != TQ_OK) return rc;
     rc = tq_launch_attend_combine(a, st);
     if (rc != TQ_OK) return rc;

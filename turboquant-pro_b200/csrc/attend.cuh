@@ -33,6 +33,7 @@ struct AttendArgs {
   const int32_t* q_lens;         // [seq_count] or null: n_tokens everywhere
   float* partials;               // per unit, unit_stride floats apart: [row][ns_cold + ns_hot][2 + D]
   int64_t unit_stride;
+  void* plan;                    // the rows form's
   // flags of the tiled kernels per unit: not zero, the unit is left to the general kernel (null: none)
   const int32_t* left;
   int32_t layer, seq_begin, seq_count, n_tokens, q_dtype;
@@ -95,9 +96,14 @@ TQ_DEV float attend_ld(const void* p, size_t i, int dt) {
 
 int tq_launch_attend_general(const AttendArgs& a, cudaStream_t st);
 int tq_launch_attend_combine(const AttendArgs& a, cudaStream_t st);
-// 256-token blocks of per-channel keys only
-int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st);
-int tq_attend_rows_tile(int rows);  // query rows of a CTA
+// Few rows, 256-token blocks of per-channel keys, queries on 16-byte boundaries; the merge too.
+struct AttendRowsPlan {
+  int ns_cold, ns_hot;  // slots of a row's states
+  int seqs;             // most sequences of a launch
+  size_t plan_bytes;    // at a.plan
+};
+AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens, int sm_count);
+int tq_launch_attend_rows(const AttendArgs& a, int sm_count, cudaStream_t st);
 // 16-bit queries, per-channel keys: everything in one, the merge too; `cap` tiles of 128 tokens per unit have room
 size_t tq_attend_tiles_bytes(const AttendArgs& a, int units, int cap, int splits);
 int tq_launch_attend_tiles(const AttendArgs& a, void* workspace, int cap, int splits, int device,
