@@ -2,31 +2,33 @@
 // 256-token blocks with per-channel keys; the products on mma.sync (m16n8k16) with the codes as the A operand,
 // straight from a table into registers, and NT tiles of eight query rows as the B operand.
 //
-// Persistent CTAs of eight warps.  The pages that the rows of each (sequence, KV head, row tile) see, first tokens,
-// then the window, and after them its tiles of the uncompressed window, form one list that is cut into shares of
-// equal cost, one per CTA, so ragged batches and every number of heads balance; where a share enters or leaves a
-// row tile, or goes from pages to the window, the CTA writes a state, and the merge sums these.  Items come
-// in whole with cp.async, the next one while this one is attended.  Of a page's 256 tokens a warp attends 32:
-//   weights  w = q * scale, scaled by a power of two per row, as an fp16 pair hi + lo in the layout of the
-//            B operand, and the zero-points' part of the score, q . mean: once per page, a row per warp;
+// Persistent CTAs, one an SM; every warp works alone, without barriers.  The 64-token strips of pages that the rows
+// of each (sequence, KV head, row tile) see, first tokens, then the window, and after them the 16-token tiles of the
+// uncompressed window, form one list that is cut into shares of equal cost, one per warp, so ragged batches and every
+// number of heads balance; where a share leaves a row tile, or goes from pages to the window, the warp writes a
+// state, and the merge sums these.  What a warp needs of a strip comes with cp.async into its own piece of shared
+// memory, the key half of the next one while the values of this one are summed and the other way round:
+//   weights  w = q * scale, scaled by a power of two per row, as fp16 pairs hi + lo in the registers of the B
+//            operand, and the zero-points' part of the score, q . mean: once per page;
 //   scores   a byte of key codes (two channels) is one look-up; hi * w and lo * w accumulate apart;
 //   mask     by position, where a row of the tile does not see the whole strip;
-//   softmax  running maximum and sum per row and warp, in units of log 2;
+//   softmax  running maximum and sum per row, in units of log 2, once per strip;
 //   values   probability * norm, scaled by a power of two per row and strip, transposed in registers into the
 //            B operand; two tokens' codes of a channel are one look-up.  The sums of a strip start from zero and are
 //            added in float32.
+// (With eight warps on a page, its weights in shared memory and a CTA per pair of heads it took twice as long: a
+// page cost five barriers and twice the instructions.)
 //
 // SPLIT (float32 and float16 queries): the table's entries are hi + lo pairs too, hi * hi of 16 channels is added
 // up in float32 registers, and outliers count with their exact stored value: as exact as float32 arithmetic.
 // bfloat16 queries leave the table's lo part out (2^-12 of a level; their own step is 2^-8), and take the outliers
 // from the page's list by token, which holds their distance from the grid in fp16.
 //
-// The uncompressed window, 64 tokens at a time: 16-bit rows are the A operand as they are, in their own type
-// (ldmatrix), so that only the other operand is split: the query is exact in one part for 16-bit queries of that type
-// or of bfloat16 in fp16, and has as many as it needs otherwise; probabilities have one part in fp16 (two with SPLIT)
-// and two in bfloat16 (three).  float32 rows, 32 at a time, are split into fp16 pairs as they are read.  A tile that
-// holds an infinity or a NaN is attended term by term instead (products with masked tokens and with low parts would
-// spread it), and so is one of float32 keys beyond fp16's range.
+// The uncompressed window: 16-bit rows are the A operand as they are, in their own type (ldmatrix), so that only the
+// other operand is split: a query that is exact in that type has one part, others as many as they need;
+// probabilities have two parts in fp16 and in bfloat16 (three there with SPLIT).  float32 rows are split into fp16 pairs
+// as they are read.  A tile that holds an infinity or a NaN is attended term by term instead (products with masked
+// tokens and with low parts would spread it), and so is one of float32 keys beyond fp16's range.
 //
 // Bound by the issue slots of look-ups and products; at one row tile the codes are read once.
 #include <algorithm>
@@ -35,51 +37,51 @@
 
 namespace {
 
-constexpr int AR_THREADS = 256, AR_WARPS = 8;
 constexpr int AR_S = 256;          // tokens of a page
-constexpr int AR_STRIP = 32;       // of them, a warp's
-constexpr int AR_HOT = 64, AR_HOT32 = 32;  // window tokens of a tile: 16-bit rows, float32 rows
-constexpr int AR_PITCH = TQ_D * 2 + 16, AR_PITCH32 = TQ_D * 4 + 16;  // bytes of a window row in shared memory
-constexpr int AR_COST = 4;         // a page takes the time of so many tiles of the window
+constexpr int AR_STRIP = 64;       // of them, in an item of the list
+constexpr int AR_HOT = 16;         // window tokens of an item
+constexpr int AR_PITCH = TQ_D * 2 + 16;  // bytes of a window row in shared memory
+constexpr int AR_COST = 4;         // a strip takes the time of so many tiles of the window
 constexpr int AR_SEQS = 64;        // sequences of a launch
-constexpr int AR_LIST = 1024;      // outliers of a page that are copied ahead (640 is usual)
+constexpr int AR_LIST = 256;       // outliers of a strip that are copied ahead (160 is usual)
 
 template <int NT, bool SPLIT, int VB>
 struct ArShape {
   static constexpr int N = 8 * NT;                     // query rows
   static constexpr int NV = VB == 4 ? 256 : 64;
-  // copies of a table side by side: 16 pairs fill a half warp's banks; of single words as many as leave
-  // room for two CTAs on an SM
-  static constexpr int REP = SPLIT ? 16 : (VB == 4 ? 8 : 16);
-  static constexpr int ENTRY = REP * (SPLIT ? 8 : 4);  // bytes of an entry, copies and all
+  static constexpr int WARPS = SPLIT ? (NT == 1 ? 8 : 6) : (NT == 1 ? 12 : 8);  // as many as have room
+  // sixteen copies of a table side by side: pairs fill a half warp's banks
+  static constexpr int ENTRY = 16 * (SPLIT ? 8 : 4);   // bytes of an entry, copies and all
   static constexpr int LUTK = 256 * ENTRY, LUTV = NV * ENTRY;
-  static constexpr int PAGE = AR_S * TQ_D / 2 + AR_S * TQ_D * VB / 8 + AR_S * 4 + 2 * TQ_D * 4 + TQ_TAIL_BYTES;
-  static constexpr int LIST = SPLIT ? AR_LIST * 6 : 0;
-  static constexpr int STAGE = PAGE + LIST;            // a page, or a tile of the window
-  static constexpr int WROW = 33 * 16;                 // bytes of a k-step's B fragments, padded
-  static constexpr int QROW = TQ_D * (SPLIT ? 4 : 2);  // bytes of a query as it comes, at most
 };
-static_assert(2 * AR_HOT * AR_PITCH <= ArShape<1, false, 3>::PAGE && 2 * AR_HOT32 * AR_PITCH32 <= ArShape<1, false, 3>::PAGE,
-              "a tile of the window in a page's place");
-static_assert(AR_WARPS * 8 * TQ_D * 4 <= ArShape<1, false, 3>::PAGE, "the warps' sums of eight rows in a page's place");
+
+// A warp's strip of a page, or a tile of the window (two rows of AR_PITCH bytes a token) in its place.
+template <int NT, bool SPLIT, int VB>
+struct alignas(16) ArWarp {
+  uint8_t keys[AR_STRIP * TQ_D / 2];
+  uint16_t delta[TQ_ELL_SLOTS][AR_STRIP];
+  uint8_t col[TQ_ELL_SLOTS][AR_STRIP];
+  float scale[4][36], mean[4][36];  // 32 channels a row (the pad spreads a lane's rows over the banks)
+  PageHeader hdr;
+  uint32_t ovf[TQ_OVF_CAP];
+  uint8_t values[AR_STRIP * TQ_D * VB / 8];
+  float norms[AR_STRIP];
+  uint32_t dec[SPLIT ? AR_LIST : 4];
+  uint16_t val[SPLIT ? AR_LIST : 8];
+  float corr[32][8 * NT];           // outliers' part of the scores of 32 tokens
+  uint8_t q[TQ_D][8 * NT * (SPLIT ? 4 : 2)];  // row q_row(d): channel d
+};
+static_assert(2 * AR_HOT * AR_PITCH <= 6528 + 64 * TQ_D * 3 / 8 + 256, "a tile of the window in a strip's place");
 
 template <int NT, bool SPLIT, int VB>
 struct ArShared {
   using Sh = ArShape<NT, SPLIT, VB>;
   alignas(128) uint8_t lut[Sh::LUTK + Sh::LUTV];
-  alignas(128) uint8_t stage[2][Sh::STAGE];
-  alignas(16) uint8_t q_raw[Sh::N * Sh::QROW];  // the next rows' queries
-  alignas(16) uint8_t w[NT][8][Sh::WROW];       // [tile][k-step][lane] {b0 hi, b1 hi, b0 lo, b1 lo}
-  alignas(16) uint2 w3[SPLIT ? NT : 1][SPLIT ? 8 : 1][32];  // third parts (bfloat16 windows)
-  alignas(16) float corr[AR_S][Sh::N];          // outliers' part of the scores
-  alignas(16) float q[TQ_D][Sh::N];             // row q_row(d): channel d
-  float bias[Sh::N], inv[Sh::N];
-  float m[AR_WARPS][Sh::N], l[AR_WARPS][Sh::N];
-  int pos[Sh::N], win[Sh::N];
-  float grid[16], cent[16], top[AR_WARPS];
-  int most[2];                                  // pages and window tiles of the longest row
+  ArWarp<NT, SPLIT, VB> warp[Sh::WARPS];
+  float grid[16], cent[16];
   int2 seq[AR_SEQS];                            // tokens, query tokens
-  int cum[AR_SEQS + 1];                         // work before each sequence, per row
+  int64_t cum[AR_SEQS + 1];                     // the cost of the sequences before
+  int most[2];                                  // strips and window tiles of the longest row
 };
 
 TQ_DEV void ar_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
@@ -152,6 +154,13 @@ TQ_DEV uint2 ar_lut2(uint32_t addr) {
   asm("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
   return v;
 }
+TQ_DEV int64_t ar_div(int64_t x, int64_t y) {  // (mostly of numbers that fit 32 bits)
+  return (x | y) >> 32 == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+}
+template <int N>
+struct ArTiles {
+  static constexpr int value = N;
+};
 template <bool TRANS>
 TQ_DEV void ar_ldm(uint32_t (&a)[4], uint32_t addr) {
   if (TRANS)
@@ -166,49 +175,44 @@ TQ_DEV void ar_ldm(uint32_t (&a)[4], uint32_t addr) {
                  : "memory");
 }
 
-// A sequence's work in a launch: its pages (first tokens, then the window), then its tiles of the uncompressed
+// A sequence's work in a launch: its strips of pages (first tokens, then the window), then its tiles of the uncompressed
 // window; the same for all of its heads and row tiles.
 struct ArWork {
-  AttendTiles page, hot;
+  AttendTiles strip, hot;
   int cold;  // tokens in blocks
-  TQ_DEV int items() const { return page.count() + hot.count(); }
-  TQ_DEV int cost() const { return AR_COST * page.count() + hot.count(); }
+  TQ_DEV int items() const { return strip.count() + hot.count(); }
+  TQ_DEV int cost() const { return AR_COST * strip.count() + hot.count(); }
 };
 TQ_DEV ArWork ar_work(const AttendArgs& a, int n, int q_n) {
   ArWork w;
   w.cold = n_cold_blocks(n, a.g.hot_window, AR_S) * AR_S;
   const int p_lo = n - q_n, p_hi = q_n > 0 ? n - 1 : -1;
-  w.page = attend_tiles(a, 0, w.cold, AR_S, p_lo, p_hi);
-  w.hot = attend_tiles(a, w.cold, n, a.g.kv_dtype == TQ_F32 ? AR_HOT32 : AR_HOT, p_lo, p_hi);
+  w.strip = attend_tiles(a, 0, w.cold, AR_STRIP, p_lo, p_hi);
+  w.hot = attend_tiles(a, w.cold, n, AR_HOT, p_lo, p_hi);
   return w;
 }
+// row tiles of a sequence that have query tokens
+TQ_DEV int ar_tiles(const AttendArgs& a, int q_n, int n) { return (q_n * a.g.group + n - 1) / n; }
 
 // How a launch divides its work; the first CTA leaves it for the merge.
 struct ArPlan {
   int64_t share;
-  int cum[AR_SEQS + 1];
-};
-
-// An item of the list.
-struct ArItem {
-  int s, row, it;  // sequence, row (head * row tiles + tile), item of the row
-  int64_t at;      // the cost of what is before it
+  int64_t cum[AR_SEQS + 1];
 };
 
 template <int NT, bool SPLIT, int VB>
-__global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
-    attend_rows_kernel(AttendArgs a, int row_tiles) {
+__global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_rows_kernel(AttendArgs a) {
   using Sh = ArShape<NT, SPLIT, VB>;
-  constexpr int N = Sh::N;
+  constexpr int N = Sh::N, WARPS = Sh::WARPS, THREADS = 32 * WARPS;
   constexpr int VGB = TQ_GROUP_TOK * TQ_D * VB / 8;
   extern __shared__ __align__(128) uint8_t ar_shared[];
   ArShared<NT, SPLIT, VB>& sh = *(ArShared<NT, SPLIT, VB>*)ar_shared;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const tq_geom& g = a.g;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
-  const int H = g.n_kv_heads, G = g.group, rows_per_seq = H * row_tiles;
+  const int H = g.n_kv_heads, G = g.group;
   const bool q32 = a.q_dtype == TQ_F32, hot32 = g.kv_dtype == TQ_F32;
-  const int hot_size = hot32 ? AR_HOT32 : AR_HOT;
+  ArWarp<NT, SPLIT, VB>& my = sh.warp[warp];
 
   // ---- the work before every sequence
   if (tid < 16) {
@@ -217,7 +221,8 @@ __global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
   }
   if (warp == 0) {
     constexpr int PER = AR_SEQS / 32;
-    int sum = 0, most_page = 0, most_hot = 0, cost[PER];
+    int most_strip = 0, most_hot = 0;
+    int64_t cost[PER], sum = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int s = lane * PER + i;
@@ -226,16 +231,16 @@ __global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
         const AttendSeq sq = attend_seq(a, s);
         sh.seq[s] = make_int2(sq.n, sq.q_n);
         const ArWork w = ar_work(a, sq.n, sq.q_n);
-        cost[i] = w.cost();
-        most_page = max(most_page, w.page.count());
+        cost[i] = (int64_t)w.cost() * (H * ar_tiles(a, sq.q_n, N));
+        most_strip = max(most_strip, w.strip.count());
         most_hot = max(most_hot, w.hot.count());
       }
       sum += cost[i];
     }
-    int before = sum;
+    int64_t before = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, before, o);
+      const int64_t v = __shfl_up_sync(0xffffffffu, before, o);
       if (lane >= o) before += v;
     }
     if (lane == 31) sh.cum[AR_SEQS] = before;
@@ -245,126 +250,27 @@ __global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
       sh.cum[lane * PER + i] = before;
       before += cost[i];
     }
-    most_page = __reduce_max_sync(0xffffffffu, most_page);
+    most_strip = __reduce_max_sync(0xffffffffu, most_strip);
     most_hot = __reduce_max_sync(0xffffffffu, most_hot);
-    if (lane == 0) sh.most[0] = most_page, sh.most[1] = most_hot;
+    if (lane == 0) sh.most[0] = most_strip, sh.most[1] = most_hot;
   }
   __syncthreads();
-  // Shares of equal cost: what starts in [k share, (k + 1) share) is CTA k's.  A row's pages then meet at most
-  // AR_COST * (pages - 1) / share + 2 CTAs, its window tiles (tiles - 1) / share + 2, which have to fit their slots.
-  const int64_t total = (int64_t)sh.cum[AR_SEQS] * rows_per_seq;
-  // (at least a page's cost: otherwise CTAs between two pages would have slots, but nothing to put there)
-  int64_t share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)AR_COST);
+  // Shares of equal cost: what starts in [k share, (k + 1) share) is warp k's.  A row's strips then meet at most
+  // AR_COST * (strips - 1) / share + 2 warps, its window tiles (tiles - 1) / share + 2, which have to fit their slots; and
+  // no share is smaller than a strip's cost, so that every warp between a row's first and last has a part.
+  const int workers = gridDim.x * WARPS;
+  const int64_t total = sh.cum[AR_SEQS];
+  int64_t share = max((total + workers - 1) / workers, (int64_t)AR_COST);
   share = max(share, (int64_t)((AR_COST * sh.most[0] + a.ns_cold - 3) / (a.ns_cold - 2)));
   share = max(share, (int64_t)((sh.most[1] + a.ns_hot - 3) / (a.ns_hot - 2)));
   if (blockIdx.x == 0) {
     ArPlan* plan = (ArPlan*)a.plan;
     if (tid == 0) plan->share = share;
-    for (int i = tid; i <= AR_SEQS; i += AR_THREADS) plan->cum[i] = sh.cum[i];
+    for (int i = tid; i <= AR_SEQS; i += THREADS) plan->cum[i] = sh.cum[i];
   }
-  const int64_t lo = share * blockIdx.x, hi = min(lo + share, total);
-  if (lo >= total) return;
-
-  auto work_of = [&](int s) { return ar_work(a, sh.seq[s].x, sh.seq[s].y); };
-  ArItem cur;
-  {  // the first item that starts at lo or after it
-    int x = 0, y = a.seq_count - 1;
-    while (x < y) {  // the last sequence that starts at lo or before it
-      const int mid = (x + y + 1) >> 1;
-      if ((int64_t)sh.cum[mid] * rows_per_seq <= lo) x = mid;
-      else y = mid - 1;
-    }
-    const ArWork w = work_of(x);
-    const int64_t in = lo - (int64_t)sh.cum[x] * rows_per_seq;
-    const int cost = w.cost(), off = (int)(in % cost), pages = AR_COST * w.page.count();
-    cur.s = x;
-    cur.row = (int)(in / cost);
-    cur.it = off < pages ? (off + AR_COST - 1) / AR_COST : w.page.count() + off - pages;
-    cur.at = lo - off + (off < pages ? AR_COST * cur.it : off);
-    if (cur.it == w.items()) {  // (off lies in the last page of a row without a window)
-      cur.it = 0;
-      ++cur.row;
-    }
-  }
-  auto settle = [&](ArItem& i) {  // rows past the sequence's last: the next sequence that has any work
-    while (i.row >= rows_per_seq) {
-      i.row = 0;
-      do ++i.s;
-      while (i.s < a.seq_count && sh.cum[i.s + 1] == sh.cum[i.s]);
-      if (i.s >= a.seq_count) break;
-    }
-  };
-  auto after = [&](const ArItem& i) {
-    const ArWork w = work_of(i.s);
-    ArItem n = i;
-    n.at += i.it < w.page.count() ? AR_COST : 1;
-    if (++n.it >= w.items()) {
-      n.it = 0;
-      ++n.row;
-      settle(n);
-    }
-    return n;
-  };
-  settle(cur);
-  if (cur.at >= hi) return;
-
-  // ---- copies
-  auto unit_of = [&](const ArItem& i) {
-    return unit_index(g, a.layer, a.seq_begin + i.s, i.row / row_tiles);
-  };
-  auto meta_of = [&](const ArItem& i) -> PageMeta {
-    PageMeta pm = {0, 0};
-    if (SPLIT && g.outlier_k > 0 && i.at < hi) {
-      const ArWork w = work_of(i.s);
-      if (i.it < w.page.count()) pm = a.page_meta[unit_of(i) * g.max_blocks + w.page.at(i.it)];
-    }
-    return pm;
-  };
-  auto listed = [&](const PageMeta& pm) { return pm.cnt <= (uint32_t)AR_LIST && (pm.off & 3u) == 0u; };
-  auto fetch = [&](const ArItem& i, const PageMeta& pm, uint8_t* to) {
-    const ArWork w = work_of(i.s);
-    const size_t u = unit_of(i);
-    if (i.it < w.page.count()) {
-      const uint8_t* from = a.pages + (u * g.max_blocks + w.page.at(i.it)) * (size_t)g.page_bytes;
-      for (int k = tid; k < Sh::PAGE / 16; k += AR_THREADS) ar_cp16(to + 16 * k, from + 16 * k);
-      if (SPLIT && listed(pm)) {
-        const size_t slab = u * (size_t)g.pool_entries + pm.off;
-        const int n4 = (int)(pm.cnt + 3) / 4;  // (slices are whole fours, and slabs whole sixty-fours, of entries)
-        for (int k = tid; k < n4; k += AR_THREADS) {
-          ar_cp16(to + Sh::PAGE + 16 * k, a.pool_dec + slab + 4 * k);
-          ar_cp8(to + Sh::PAGE + 4 * AR_LIST + 8 * k, a.pool_val + slab + 4 * k);
-        }
-      }
-    } else {
-      const int t0 = w.cold + w.hot.at(i.it - w.page.count()) * hot_size, n = sh.seq[i.s].x;
-      const size_t ring = u * (size_t)g.hot_cap * TQ_D;
-      const int pieces = hot32 ? 32 : 16, pitch = hot32 ? AR_PITCH32 : AR_PITCH, esz = hot32 ? 4 : 2;
-      for (int k = tid; k < hot_size * pieces; k += AR_THREADS) {
-        const int row = k / pieces, at = (k - row * pieces) * 16, t = t0 + row;
-        const size_t from = (ring + (size_t)(t % g.hot_cap) * TQ_D) * esz + at;
-        ar_cp16_or_zero(to + row * pitch + at, (const uint8_t*)a.hot_k + from, t < n);
-        ar_cp16_or_zero(to + (hot_size + row) * pitch + at, (const uint8_t*)a.hot_v + from, t < n);
-      }
-    }
-  };
-  auto fetch_q = [&](const ArItem& i) {
-    const int head = i.row / row_tiles, row0 = i.row % row_tiles * N, pieces = q32 ? 32 : 16, esz = q32 ? 4 : 2;
-    for (int k = tid; k < N * pieces; k += AR_THREADS) {
-      const int n = k / pieces, at = (k - n * pieces) * 16, row = row0 + n;
-      const bool there = row < a.rows;
-      const int64_t from = there ? (int64_t)i.s * a.q_seq + (int64_t)(row / G) * a.q_tok +
-                                       (int64_t)(head * G + row % G) * a.q_head
-                                 : 0;
-      ar_cp16_or_zero(sh.q_raw + n * Sh::QROW + at, (const uint8_t*)a.q + from * esz + at, there);
-    }
-  };
-  int st = 0;
-  PageMeta pm = meta_of(cur);
-  fetch(cur, pm, sh.stage[0]);
-  fetch_q(cur);
-  ar_commit();
-  ArItem nxt = after(cur);
-  PageMeta pm_next = meta_of(nxt);
+  // (neighbouring shares go to different SMs: where there are few, each has one to itself)
+  const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;
+  if (share * blockIdx.x >= total) return;  // (the whole CTA)
 
   // ---- tables of pairs
   float inv_k, inv_v;
@@ -376,27 +282,131 @@ __global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
       max_v = fmaxf(max_v, fabsf(sh.cent[i]));
     }
     const float up_k = ar_lift(max_k, 7, inv_k), up_v = ar_lift(max_v, 7, inv_v);
-    for (int e = tid; e < 256 + Sh::NV; e += AR_THREADS) {
-      uint32_t hi2, lo2;
+    for (int e = tid; e < 256 + Sh::NV; e += THREADS) {
+      uint32_t hi, lo;
       uint4* to;
       if (e < 256) {
-        ar_split(sh.grid[e & 15], up_k, sh.grid[e >> 4], up_k, hi2, lo2);
+        ar_split(sh.grid[e & 15], up_k, sh.grid[e >> 4], up_k, hi, lo);
         to = (uint4*)(sh.lut + e * Sh::ENTRY);
       } else {
         const int b = e - 256;
-        ar_split(sh.cent[b & ((1 << VB) - 1)], up_v, sh.cent[b >> VB], up_v, hi2, lo2);
+        ar_split(sh.cent[b & ((1 << VB) - 1)], up_v, sh.cent[b >> VB], up_v, hi, lo);
         to = (uint4*)(sh.lut + Sh::LUTK + b * Sh::ENTRY);
       }
 #pragma unroll
       for (int i = 0; i < Sh::ENTRY / 16; ++i)
-        to[(i + lane) % (Sh::ENTRY / 16)] = SPLIT ? make_uint4(hi2, lo2, hi2, lo2) : make_uint4(hi2, hi2, hi2, hi2);
+        to[(i + lane) % (Sh::ENTRY / 16)] = SPLIT ? make_uint4(hi, lo, hi, lo) : make_uint4(hi, hi, hi, hi);
     }
   }
+  __syncthreads();  // (the last one)
+  int64_t at = share * me;
+  const int64_t stop = min(at + share, total);
+  if (at >= total) return;
 
-  // rows 8 t + 2 c + x are this lane's columns
-  float qv[NT][4];  // rows warp, warp + 8, ...: channels 4 lane .. + 3, times the scores' unit
+  // ---- where the share begins: sequence, head, row tile, item
+  int s, head, rt, it, row_items, row_strips, row_tiles;
+  ArWork w;
+  auto enter_seq = [&]() {
+    w = ar_work(a, sh.seq[s].x, sh.seq[s].y);
+    row_strips = w.strip.count();
+    row_items = w.items();
+    row_tiles = ar_tiles(a, sh.seq[s].y, N);
+  };
+  int64_t begin;  // the cost of what is before this row
+  {
+    int x = 0, y = a.seq_count - 1;
+    while (x < y) {  // the last sequence that starts here or before
+      const int mid = (x + y + 1) >> 1;
+      if (sh.cum[mid] <= at) x = mid;
+      else y = mid - 1;
+    }
+    s = x;
+    enter_seq();
+    const uint32_t cost = (uint32_t)w.cost();
+    // (a sequence's cost may pass 32 bits, a row's does not)
+    const int64_t in = at - sh.cum[s];
+    const int row = in >> 31 == 0 ? (int)((uint32_t)in / cost) : (int)(in / cost);
+    const int off = (int)(in - (int64_t)row * cost), strips = AR_COST * row_strips;
+    begin = at - off;
+    head = row / row_tiles, rt = row - head * row_tiles;
+    it = off < strips ? (off + AR_COST - 1) / AR_COST : row_strips + off - strips;
+    at = begin + (off < strips ? AR_COST * it : off);
+  }
+  auto next_row = [&]() {  // false: there is none
+    begin += AR_COST * row_strips + (row_items - row_strips);
+    it = 0;
+    if (++rt < row_tiles) return true;
+    rt = 0;
+    if (++head < H) return true;
+    head = 0;
+    do ++s;
+    while (s < a.seq_count && sh.cum[s + 1] == sh.cum[s]);
+    if (s >= a.seq_count) return false;
+    enter_seq();
+    return true;
+  };
+  if (it == row_items && !next_row()) return;  // (it began within the last strip of a row without a window)
+  if (at >= stop) return;
+
+  // ---- copies
+  size_t uix = 0;
+  uint32_t list_at = 0, list_end = 0;  // SPLIT: the strip's first entry of the page's list, the list's end
+  const uint8_t* page = nullptr;
+  auto page_of = [&](int i) { return a.pages + (uix * g.max_blocks + (w.strip.at(i) >> 2)) * (size_t)g.page_bytes; };
+  auto copy_keys = [&](const uint8_t* from, int t0, uint32_t first) {  // t0: of the strip in its page
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      ar_cp16(my.keys + (32 * i + lane) * 16, from + t0 * (TQ_D / 2) + (32 * i + lane) * 16);
+    ar_cp16(&my.scale[lane >> 3][(lane & 7) * 4], from + g.scale_off + lane * 16);
+    ar_cp16(&my.mean[lane >> 3][(lane & 7) * 4], from + g.mean_off + lane * 16);
+    if (SPLIT) {
+      // (the list's slice is whole fours of entries, and its slab whole sixty-fours: pieces of four)
+      const uint32_t base = first & ~3u;
+      const size_t slab = uix * (size_t)g.pool_entries;
+#pragma unroll
+      for (int i = 0; i < AR_LIST / 128; ++i) {
+        const uint32_t e = base + 4 * (32 * i + lane);
+        if (e < list_end) {
+          ar_cp16(my.dec + 4 * (32 * i + lane), a.pool_dec + slab + e);
+          ar_cp8(my.val + 4 * (32 * i + lane), a.pool_val + slab + e);
+        }
+      }
+    } else {
+      const uint8_t* ed = from + g.hdr_off + TQ_ELL_OFF;      // 8 pieces a slot
+      const uint8_t* ec = from + g.hdr_off + TQ_ELL_COL_OFF;  // 4 pieces a slot
+      ar_cp16((uint8_t*)my.delta + lane * 16, ed + (lane >> 3) * (AR_S * 2) + t0 * 2 + (lane & 7) * 16);
+      if (lane < 16) ar_cp16((uint8_t*)my.col + lane * 16, ec + (lane >> 2) * AR_S + t0 + (lane & 3) * 16);
+      if (lane < 4) ar_cp16((uint8_t*)&my.hdr + lane * 16, from + g.hdr_off + lane * 16);
+      else ar_cp16(my.ovf + (lane - 4) * 4, from + g.hdr_off + TQ_OVF_OFF + (lane - 4) * 16);
+    }
+  };
+  auto copy_values = [&](const uint8_t* from, int t0) {
+    const uint8_t* src = from + g.v_off + (size_t)(t0 / TQ_GROUP_TOK) * VGB;
+#pragma unroll
+    for (int i = 0; i < 4 * VGB / 512; ++i) ar_cp16(my.values + (32 * i + lane) * 16, src + (32 * i + lane) * 16);
+    if (lane < 16) ar_cp16(my.norms + lane * 4, from + g.norm_off + t0 * 4 + lane * 16);
+  };
+  static_assert(sizeof(PageHeader) == 64 && TQ_OVF_CAP * 4 == 28 * 16, "pieces of the tail");
+  // SPLIT: the list of the page of item i, and its first entry of token t0 or a later one
+  auto open_list = [&](int i, int t0) {
+    if (!SPLIT || g.outlier_k == 0) return;
+    const PageMeta pm = a.page_meta[uix * g.max_blocks + (w.strip.at(i) >> 2)];
+    list_end = pm.off + pm.cnt;
+    uint32_t lo = pm.off, hi = list_end;
+    const uint32_t* dec = a.pool_dec + uix * (size_t)g.pool_entries;
+    if (t0 > 0)
+      while (lo < hi) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if ((int)(dec[mid] >> 24) < t0) lo = mid + 1;
+        else hi = mid;
+      }
+    list_at = lo;
+  };
+
+  // ---- rows 8 t + 2 c + x are this lane's columns
   float acc[NT][8][4], m_run[NT][2], l_run[NT][2];
-  int first_pos = 0, last_win = 0, p_lo = 0, p_hi = 0;  // of the row tile: see `start_row`
+  int pos[NT][2], win[NT][2];
+  int first_pos = 0, last_win = 0, p_lo = 0, p_hi = 0, row0 = 0;
   auto reset = [&]() {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -408,83 +418,88 @@ __global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
       for (int x = 0; x < 2; ++x) m_run[t][x] = -INFINITY, l_run[t][x] = 0.0f;
     }
   };
-  // four channels of a row of q_raw
-  auto raw_q = [&](int n, float (&x)[4]) {
-    const uint8_t* p = sh.q_raw + n * Sh::QROW + 4 * lane * (q32 ? 4 : 2);
+  // four neighbouring channels of a query row (rows that are not there: zeros)
+  auto load_q = [&](int row, int d, float (&x)[4]) {
+    x[0] = x[1] = x[2] = x[3] = 0.0f;
+    if (row >= a.rows) return;
+    const int64_t from = (int64_t)s * a.q_seq + (int64_t)(row / G) * a.q_tok + (int64_t)(head * G + row % G) * a.q_head + d;
     if (SPLIT && q32) {
-      const float4 v = *(const float4*)p;
+      const float4 v = *(const float4*)((const float*)a.q + from);
       x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
     } else {
-      const uint2 v = *(const uint2*)p;
+      const uint2 v = *(const uint2*)((const uint16_t*)a.q + from);
       if (SPLIT) {
-        const float2 u = __half22float2(*(const __half2*)&v.x), w = __half22float2(*(const __half2*)&v.y);
-        x[0] = u.x, x[1] = u.y, x[2] = w.x, x[3] = w.y;
+        const float2 u = __half22float2(*(const __half2*)&v.x), f = __half22float2(*(const __half2*)&v.y);
+        x[0] = u.x, x[1] = u.y, x[2] = f.x, x[3] = f.y;
       } else {
         x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
         x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
       }
     }
   };
-  // (between two barriers of an item; what it writes is read after the second)
-  auto start_row = [&](const ArItem& i) {
-    AttendSeq sq;
-    sq.n = sh.seq[i.s].x, sq.q_n = sh.seq[i.s].y;
-    sq.first = sq.n - sq.q_n;
-    sq.cold = 0;
-    const int row0 = i.row % row_tiles * N, last = min(min(row0 + N, a.rows), sq.q_n * G) - 1;
-    p_lo = sq.first + row0 / G;
-    p_hi = last >= row0 ? sq.first + last / G : -1;
-    // whether a tile of tokens is seen by all rows of the tile: from the earliest row, and the latest window
+  // the rows' queries in shared memory as they are; float32 ones are asked for as scores' units where they are used
+  auto q_at = [&](int qrow, int n) -> float {
+    if (SPLIT) return ((const float*)my.q[qrow])[n];
+    return __uint_as_float((uint32_t)((const uint16_t*)my.q[qrow])[n] << 16);
+  };
+  auto start_row = [&]() {
+    uix = unit_index(g, a.layer, a.seq_begin + s, head);
+    row0 = rt * N;
+    const int n = sh.seq[s].x, q_n = sh.seq[s].y, first = n - q_n;
+    const int last = min(min(row0 + N, a.rows), q_n * G) - 1;
+    p_lo = first + row0 / G;
+    p_hi = last >= row0 ? first + last / G : -1;
+    // whether tokens are seen by all rows of the tile goes by its earliest row and its latest window
     first_pos = min(row0 + N, a.rows) - 1 <= last ? p_lo : -1;
     last_win = attend_window(a, max(p_hi, 0));
-    if (tid < N) {
-      sh.pos[tid] = row0 + tid < a.rows ? attend_position(a, sq, row0 + tid) : -1;
-      sh.win[tid] = attend_window(a, sh.pos[tid]);
-    }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      raw_q(8 * t + warp, qv[t]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        qv[t][k] = tq_scaled<true>(qv[t][k]);
-        sh.q[q_row(4 * lane + k)][8 * t + warp] = qv[t][k];
-      }
-    }
-  };
-  auto row_max = [&](const float (&w)[4]) -> float {
-    float mx = fmaxf(fmaxf(fabsf(w[0]), fabsf(w[1])), fmaxf(fabsf(w[2]), fabsf(w[3])));
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    return mx;
-  };
-  // whether tokens t0 .. t1 - 1 are seen by every row of the tile, and by none
-  auto open_to_all = [&](int t0, int t1) { return t1 - 1 <= first_pos && (t0 >= last_win || t1 <= a.sinks); };
-  auto open_to_none = [&](int t0, int t1) {
-    return t0 > p_hi || (t1 <= attend_window(a, max(p_lo, 0)) && t0 >= a.sinks);
-  };
-
-  // From the scores of `tiles` times 16 tokens from `t0` on to their probabilities: maximum and sum go on, the
-  // probability stays in `sc`, times a power of two that takes the row's largest probability * nv below 2^14.
-  auto softmax = [&](float (&sc)[2][NT][4], int t0, int t_end, int tiles, const float (&nv)[2][2], float (&inv_n)[NT][2]) {
-    const bool open = t0 + 16 * tiles <= t_end && open_to_all(t0, t0 + 16 * tiles);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        uint32_t hidden = tiles == 1 ? 0xcu : 0u;  // (only one tile of 16)
-        if (!open) {
-          const int p = sh.pos[8 * t + 2 * c + x], w = sh.win[8 * t + 2 * c + x];
+        const int row = row0 + 8 * t + 2 * c + x;
+        pos[t][x] = row <= last ? max(first + row / G, -1) : -1;
+        win[t][x] = attend_window(a, pos[t][x]);
+      }
+    __syncwarp();
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+    for (int i = 0; i < N; ++i) {
+      float x[4];
+      load_q(row0 + i, 4 * lane, x);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (SPLIT) ((float*)my.q[q_row(4 * lane + k)])[i] = x[k];
+        else ((uint16_t*)my.q[q_row(4 * lane + k)])[i] = (uint16_t)(__float_as_uint(x[k]) >> 16);
+      }
+    }
+    __syncwarp();
+  };
+  auto open_to_all = [&](int t0, int t1) { return t1 - 1 <= first_pos && (t0 >= last_win || t1 <= a.sinks); };
+  auto open_to_none = [&](int t0, int t1) {
+    return t0 > p_hi || (t1 <= attend_window(a, max(p_lo, 0)) && t0 >= a.sinks);
+  };
+  const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  // From the scores of TILES times 16 tokens from `t0` on to their probabilities: maximum and sum go on, the
+  // probability stays in `sc`, times a power of two that takes the row's largest probability * nv below 2^14.
+  auto softmax = [&](auto& sc, int t0, int t_end, auto tiles, const auto& nv, float (&inv_n)[NT][2]) {
+    constexpr int TILES = decltype(tiles)::value;
+    const bool open = t0 + 16 * TILES <= t_end && open_to_all(t0, t0 + 16 * TILES);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint32_t hidden = 0u;
+        if (!open) {
+#pragma unroll
+          for (int h = 0; h < TILES; ++h)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               const int j = t0 + 16 * h + 8 * y + r;
-              if (j >= t_end || j > p || (j < w && j >= a.sinks)) hidden |= 1u << (2 * h + y);
+              if (j >= t_end || j > pos[t][x] || (j < win[t][x] && j >= a.sinks)) hidden |= 1u << (2 * h + y);
             }
         }
         float top = -INFINITY;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < TILES; ++h)
 #pragma unroll
           for (int y = 0; y < 2; ++y)
             if (!(hidden >> (2 * h + y) & 1u)) top = fmaxf(top, sc[h][t][2 * y + x]);
@@ -495,7 +510,7 @@ __global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
         const float by = top > -INFINITY ? top : 0.0f, down = tq_exp2(m_run[t][x] - by);
         float sum = 0.0f, most = 0.0f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < TILES; ++h)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             const float e = hidden >> (2 * h + y) & 1u ? 0.0f : tq_exp2(sc[h][t][2 * y + x] - by);
@@ -514,203 +529,224 @@ __global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
           acc[t][mt][2 + x] *= down;
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < TILES; ++h)
 #pragma unroll
           for (int y = 0; y < 2; ++y) sc[h][t][2 * y + x] *= up;
       }
   };
-  auto scaled_add = [&](float (&to)[4], const float (&d)[4], const float (&inv)[2], float by) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) to[i] = fmaf(d[i], inv[i & 1] * by, to[i]);
-  };
-  const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 
-  // ---- a page: weights and corrections, then, past a barrier, this warp's 32 tokens
-  const uint32_t lutk = ar_smem(sh.lut) + (lane % Sh::REP) * (SPLIT ? 8 : 4);
-  const uint32_t lutv = lutk + Sh::LUTK;
-  auto page_prepare = [&](const uint8_t* page, const PageMeta& pm, size_t u) {
-    {  // weights: k-step j of lane group c takes channels 32 c + 4 j .. + 3
-      const float4 s4 = *(const float4*)(page + g.scale_off + 16 * lane);
-      const float4 m4 = *(const float4*)(page + g.mean_off + 16 * lane);
-      const float sc[4] = {s4.x, s4.y, s4.z, s4.w}, mu[4] = {m4.x, m4.y, m4.z, m4.w};
+  // ---- a strip of a page
+  const uint32_t lutk = ar_smem(sh.lut) + (lane & 15) * (SPLIT ? 8 : 4), lutv = lutk + Sh::LUTK;
+  uint32_t bh[NT][8][2], bl[NT][8][2];  // weights: k-step j takes channels 32 c + 4 j .. + 3, column r is row 8 t + r
+  float bias[NT][2], inv[NT][2];
+  auto weights = [&]() {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float w[4], b = 0.0f, inv;
+    for (int t = 0; t < NT; ++t) {
+      float mx = 0.0f;
+      float4 b4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[i] = qv[t][i] * sc[i];
-          b = fmaf(qv[t][i], mu[i], b);
-        }
-        const float up = ar_lift(row_max(w), 13, inv);
+      for (int j = 0; j < 8; ++j) {
+        const float4 s4 = *(const float4*)&my.scale[c][4 * j], m4 = *(const float4*)&my.mean[c][4 * j];
+        const int d = 32 * c + 4 * j, n = 8 * t + r;
+        const float q0 = q_at(q_row(d), n), q1 = q_at(q_row(d + 1), n), q2 = q_at(q_row(d + 2), n), q3 = q_at(q_row(d + 3), n);
+        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(q0 * s4.x), fabsf(q1 * s4.y)), fmaxf(fabsf(q2 * s4.z), fabsf(q3 * s4.w))));
+        b4.x = fmaf(q0, m4.x, b4.x), b4.y = fmaf(q1, m4.y, b4.y);
+        b4.z = fmaf(q2, m4.z, b4.z), b4.w = fmaf(q3, m4.w, b4.w);
+      }
+      float b = (b4.x + b4.y) + (b4.z + b4.w);
+      b += __shfl_xor_sync(0xffffffffu, b, 1);
+      b += __shfl_xor_sync(0xffffffffu, b, 2);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      float i0;
+      const float up = ar_lift(mx, 13, i0);
+      i0 *= inv_k;
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) b += __shfl_xor_sync(0xffffffffu, b, o);
-        uint4 f;
-        ar_split(qv[t][0] * up, sc[0], qv[t][1] * up, sc[1], f.x, f.z);
-        ar_split(qv[t][2] * up, sc[2], qv[t][3] * up, sc[3], f.y, f.w);
-        *(uint4*)(sh.w[t][lane & 7] + (4 * warp + (lane >> 3)) * 16) = f;
-        if (lane == 0) {
-          sh.bias[8 * t + warp] = b;
-          sh.inv[8 * t + warp] = inv * inv_k;
-        }
+      for (int x = 0; x < 2; ++x) {  // of rows 2 c + x
+        bias[t][x] = __shfl_sync(0xffffffffu, b, 8 * c + 4 * x);
+        inv[t][x] = __shfl_sync(0xffffffffu, i0, 8 * c + 4 * x);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 s4 = *(const float4*)&my.scale[c][4 * j];
+        const int d = 32 * c + 4 * j, n = 8 * t + r;
+        ar_split(q_at(q_row(d), n) * up, s4.x, q_at(q_row(d + 1), n) * up, s4.y, bh[t][j][0], bl[t][j][0]);
+        ar_split(q_at(q_row(d + 2), n) * up, s4.z, q_at(q_row(d + 3), n) * up, s4.w, bh[t][j][1], bl[t][j][1]);
       }
     }
-    if (g.outlier_k == 0) return;
-    const PageHeader* hdr = (const PageHeader*)(page + g.hdr_off);
-    auto add_corr = [&](float (&e)[N], float delta, int qrow) {
+  };
+  auto add_corr = [&](float (&e)[N], float delta, int qrow) {
 #pragma unroll
-      for (int x = 0; x < N; x += 4) {
-        const float4 q4 = *(const float4*)&sh.q[qrow][x];
+    for (int x = 0; x < N; x += 4) {
+      if (SPLIT) {
+        const float4 q4 = *(const float4*)((const float*)my.q[qrow] + x);
         e[x] = fmaf(q4.x, delta, e[x]), e[x + 1] = fmaf(q4.y, delta, e[x + 1]);
         e[x + 2] = fmaf(q4.z, delta, e[x + 2]), e[x + 3] = fmaf(q4.w, delta, e[x + 3]);
+      } else {
+        const uint2 q4 = *(const uint2*)((const uint16_t*)my.q[qrow] + x);
+        e[x] = fmaf(__uint_as_float(q4.x << 16), delta, e[x]);
+        e[x + 1] = fmaf(__uint_as_float(q4.x & 0xffff0000u), delta, e[x + 1]);
+        e[x + 2] = fmaf(__uint_as_float(q4.y << 16), delta, e[x + 2]);
+        e[x + 3] = fmaf(__uint_as_float(q4.y & 0xffff0000u), delta, e[x + 3]);
       }
-    };
-    // (columns of a token's row in an order that spreads eight tokens over the banks)
-    auto put_corr = [&](int tok, const float (&e)[N]) {
+    }
+  };
+  // (columns of a token's row in an order that spreads eight tokens over the banks)
+  auto put_corr = [&](int tok, const float (&e)[N]) {
 #pragma unroll
-      for (int x = 0; x < N; x += 4)
-        *(float4*)&sh.corr[tok][x ^ (4 * (tok >> 2 & 1))] = make_float4(e[x], e[x + 1], e[x + 2], e[x + 3]);
-    };
+    for (int x = 0; x < N; x += 4)
+      *(float4*)&my.corr[tok][x ^ (4 * (tok >> 2 & 1))] = make_float4(e[x], e[x + 1], e[x + 2], e[x + 3]);
+  };
+  // the outliers' part of the scores of tokens 32 half .. + 31 of the strip, which begins at token ts of its page
+  uint32_t list_next = 0;
+  auto corrections = [&](int half, int ts) {
     float e[N];
 #pragma unroll
     for (int x = 0; x < N; ++x) e[x] = 0.0f;
+    __syncwarp();  // (those before have been read)
     if (SPLIT) {
-      // the pool's list, ordered by token: the thread that holds a token's first entry adds up all of them
-      put_corr(tid, e);
-      __syncthreads();
-      const uint32_t* dec;
-      const uint16_t* val;
-      if (listed(pm)) {
-        dec = (const uint32_t*)(page + Sh::PAGE);
-        val = (const uint16_t*)(page + Sh::PAGE + 4 * AR_LIST);
-      } else {
-        dec = a.pool_dec + u * (size_t)g.pool_entries + pm.off;
-        val = a.pool_val + u * (size_t)g.pool_entries + pm.off;
-      }
-      for (uint32_t i = tid; i < pm.cnt; i += AR_THREADS) {
-        const int tok = (int)(dec[i] >> 24);
-        if (i > 0 && (int)(dec[i - 1] >> 24) == tok) continue;
+      // the pool's list, ordered by token: the lane that holds a token's first entry adds up all of them
+      put_corr(lane, e);
+      __syncwarp();
+      const uint32_t base = list_at & ~3u;  // of what has been copied
+      const size_t slab = uix * (size_t)g.pool_entries;
+      auto dec_at = [&](uint32_t i) { return i - base < (uint32_t)AR_LIST ? my.dec[i - base] : a.pool_dec[slab + i]; };
+      auto val_at = [&](uint32_t i) { return i - base < (uint32_t)AR_LIST ? my.val[i - base] : a.pool_val[slab + i]; };
+      const int t0 = ts + 32 * half;
+      const uint32_t first = half == 0 ? list_at : list_next;
+      bool go = true;
+      for (uint32_t i = first; go; i += 32) {
+        const uint32_t k = i + lane;
+        const int tok = k < list_end ? (int)(dec_at(k) >> 24) - t0 : 32;
+        const uint32_t in = __ballot_sync(0xffffffffu, tok < 32);
+        go = in == 0xffffffffu;
+        if (!go) list_next = i + __popc(in);
+        if (tok >= 32 || (k > first && (int)(dec_at(k - 1) >> 24) - t0 == tok)) continue;
 #pragma unroll
         for (int x = 0; x < N; ++x) e[x] = 0.0f;
-        for (uint32_t j = i; j < pm.cnt && (int)(dec[j] >> 24) == tok; ++j) {
-          const int ch = (dec[j] >> 16) & 127;
-          const float on_grid = sh.grid[page[tok * (TQ_D / 2) + (ch >> 1)] >> (4 * (ch & 1)) & 15];
-          const float sc = ((const float*)(page + g.scale_off))[ch], mu = ((const float*)(page + g.mean_off))[ch];
+        for (uint32_t j = k; j < list_end; ++j) {
+          const uint32_t u = dec_at(j);
+          if ((int)(u >> 24) - t0 != tok) break;
+          const int ch = (u >> 16) & 127;
+          const float on_grid = sh.grid[my.keys[(tok + 32 * half) * (TQ_D / 2) + (ch >> 1)] >> (4 * (ch & 1)) & 15];
           // what the weights' part gives is taken off, and the value itself put in
-          add_corr(e, fmaf(-sc, on_grid, __half2float(__ushort_as_half(val[j])) - mu), q_row(ch));
+          add_corr(e, fmaf(-my.scale[ch >> 5][ch & 31], on_grid, __half2float(__ushort_as_half(val_at(j))) - my.mean[ch >> 5][ch & 31]),
+                   q_row(ch));
         }
         put_corr(tok, e);
       }
-    } else {
-      const uint8_t* col = page + g.hdr_off + TQ_ELL_COL_OFF;
-      const uint16_t* delta = (const uint16_t*)(page + g.hdr_off + TQ_ELL_OFF);
-      const bool spilled = (hdr->flags & TQ_PAGE_SPILLED) != 0;
-      if (!spilled) {
-#pragma unroll
-        for (int j = 0; j < TQ_ELL_SLOTS; ++j)
-          add_corr(e, __half2float(__ushort_as_half(delta[j * AR_S + tid])), col[j * AR_S + tid]);
-      }
-      put_corr(tid, e);
       __syncwarp();
-      // the rest of the list, ordered by token, as above
-      const uint32_t* list = (const uint32_t*)(page + g.hdr_off + TQ_OVF_OFF);
-      int e0 = hdr->ovf_start[warp >> 1], e1 = hdr->ovf_start[(warp >> 1) + 1];
-      if (spilled) {
-        list = a.pool_dec + u * (size_t)g.pool_entries + hdr->off;
-        e0 = 0, e1 = (int)hdr->cnt;
-      }
-      for (int i = e0 + lane; i < e1; i += 32) {
-        uint32_t v = list[i];
-        const int tok = (int)(v >> 24);
-        if (tok >> 5 != warp || (i > e0 && (int)(list[i - 1] >> 24) == tok)) continue;
+      return;
+    }
+    const bool spilled = (my.hdr.flags & TQ_PAGE_SPILLED) != 0;
+    const int tok = 32 * half + lane;
+    if (!spilled) {
 #pragma unroll
-        for (int x = 0; x < N; ++x) e[x] = sh.corr[tok][x ^ (4 * (tok >> 2 & 1))];
-        for (int j = i;;) {
-          add_corr(e, __half2float(__ushort_as_half((unsigned short)(v & 0xffffu))), q_row((v >> 16) & 127));
-          if (++j >= e1) break;
-          v = list[j];
-          if ((int)(v >> 24) != tok) break;
+      for (int j = 0; j < TQ_ELL_SLOTS; ++j) add_corr(e, __half2float(__ushort_as_half(my.delta[j][tok])), my.col[j][tok]);
+    }
+    put_corr(lane, e);
+    __syncwarp();
+    // the rest of the list, ordered by token, as above
+    const uint32_t* list = my.ovf;
+    int e0 = my.hdr.ovf_start[ts >> 6], e1 = my.hdr.ovf_start[(ts >> 6) + 1];
+    if (spilled) {
+      list = a.pool_dec + uix * (size_t)g.pool_entries + my.hdr.off;
+      e0 = 0, e1 = (int)my.hdr.cnt;
+    }
+    for (int i = e0 + lane; i < e1; i += 32) {
+      uint32_t v = list[i];
+      const int tk = (int)(v >> 24);
+      if (tk >> 5 != (ts >> 5) + half || (i > e0 && (int)(list[i - 1] >> 24) == tk)) continue;
+#pragma unroll
+      for (int x = 0; x < N; ++x) e[x] = my.corr[tk & 31][x ^ (4 * (tk >> 2 & 1))];
+      for (int j = i;;) {
+        add_corr(e, __half2float(__ushort_as_half((unsigned short)(v & 0xffffu))), q_row((v >> 16) & 127));
+        if (++j >= e1) break;
+        v = list[j];
+        if ((int)(v >> 24) != tk) break;
+      }
+      put_corr(tk & 31, e);
+    }
+    __syncwarp();
+  };
+  // scores of the strip's four tiles
+  auto strip_scores = [&](float (&sc)[4][NT][4], int ts) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (g.outlier_k > 0) corrections(half, ts);
+#pragma unroll
+      for (int h2 = 0; h2 < 2; ++h2) {
+        const int h = 2 * half + h2;
+        uint32_t kw[2][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint4 v = *(const uint4*)(my.keys + (16 * h + 8 * x + r) * (TQ_D / 2) + c * 16);
+          kw[x][0] = v.x, kw[x][1] = v.y, kw[x][2] = v.z, kw[x][3] = v.w;
         }
-        put_corr(tok, e);
+        float sum[NT][4], low[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[t][i] = low[t][i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t ah[4], al[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {  // tokens r, r + 8; bytes 2 j, 2 j + 1
+            const uint32_t b = __byte_perm(kw[x & 1][j >> 1], 0, 0x4440 + 2 * (j & 1) + (x >> 1));
+            if (SPLIT) {
+              const uint2 v = ar_lut2(lutk + b * Sh::ENTRY);
+              ah[x] = v.x, al[x] = v.y;
+            } else {
+              ah[x] = ar_lut1(lutk + b * Sh::ENTRY);
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if (SPLIT) {
+              float d[4];
+              ar_mma(d, ah, bh[t][j][0], bh[t][j][1], zero);
+              ar_mma(low[t], al, bh[t][j][0], bh[t][j][1], low[t]);
+              ar_mma(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sum[t][i] += d[i];
+            } else {
+              ar_mma(sum[t], ah, bh[t][j][0], bh[t][j][1], sum[t]);
+              ar_mma(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
+            }
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int n = 8 * t + 2 * c + (i & 1), tok = 16 * h2 + 8 * (i >> 1) + r;
+            float x = fmaf(sum[t][i] + low[t][i], inv[t][i & 1], bias[t][i & 1]);
+            if (g.outlier_k > 0) x += my.corr[tok][n ^ (4 * (tok >> 2 & 1))];
+            sc[h][t][i] = tq_scaled<true>(x);
+          }
       }
     }
   };
-  auto page_attend = [&](const uint8_t* page, int first, int cold) {
-    const int ts = AR_STRIP * warp, t0 = first + ts;
-    if (open_to_none(t0, t0 + AR_STRIP)) return;
-    float sc[2][NT][4];
+  auto strip_values = [&](float (&sc)[4][NT][4], const float (&nv)[4][2], const float (&inv_n)[NT][2]) {
+    float f[NT][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t kw[2][4];
+    for (int t = 0; t < NT; ++t) f[t][0] = inv_n[t][0] * inv_v, f[t][1] = inv_n[t][1] * inv_v;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const uint4 v = *(const uint4*)(page + (ts + 16 * h + 8 * x + r) * (TQ_D / 2) + c * 16);
-        kw[x][0] = v.x, kw[x][1] = v.y, kw[x][2] = v.z, kw[x][3] = v.w;
-      }
-      float sum[NT][4], low[NT][4];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[t][i] = low[t][i] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t ah[4], al[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {  // tokens r, r + 8; bytes 2 j, 2 j + 1
-          const uint32_t b = __byte_perm(kw[x & 1][j >> 1], 0, 0x4440 + 2 * (j & 1) + (x >> 1));
-          if (SPLIT) {
-            const uint2 v = ar_lut2(lutk + b * Sh::ENTRY);
-            ah[x] = v.x, al[x] = v.y;
-          } else {
-            ah[x] = ar_lut1(lutk + b * Sh::ENTRY);
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const uint4 w = *(const uint4*)(sh.w[t][j] + lane * 16);
-          if (SPLIT) {
-            float d[4];
-            ar_mma(d, ah, w.x, w.y, zero);
-            ar_mma(low[t], al, w.x, w.y, low[t]);
-            ar_mma(low[t], ah, w.z, w.w, low[t]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[t][i] += d[i];
-          } else {
-            ar_mma(sum[t], ah, w.x, w.y, sum[t]);
-            ar_mma(low[t], ah, w.z, w.w, low[t]);
-          }
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int n = 8 * t + 2 * c + (i & 1), tok = ts + 16 * h + 8 * (i >> 1) + r;
-          float x = fmaf(sum[t][i] + low[t][i], sh.inv[n], sh.bias[n]);
-          if (g.outlier_k > 0) x += sh.corr[tok][n ^ (4 * (tok >> 2 & 1))];
-          sc[h][t][i] = x;
-        }
-    }
-    float nv[2][2], inv_n[NT][2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) nv[h][y] = ((const float*)(page + g.norm_off))[ts + 16 * h + 8 * y + r];
-    softmax(sc, t0, cold, 2, nv, inv_n);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 4; ++h) {
       uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          uint32_t hi2, lo2;
+          uint32_t hi, lo;
           // (a hidden token's norm may be anything)
           const float n0 = sc[h][t][2 * y] == 0.0f ? 0.0f : nv[h][y], n1 = sc[h][t][2 * y + 1] == 0.0f ? 0.0f : nv[h][y];
-          ar_split(sc[h][t][2 * y], n0, sc[h][t][2 * y + 1], n1, hi2, lo2);
-          ph[t][y] = ar_transpose(hi2);
-          if (SPLIT) pl[t][y] = ar_transpose(lo2);
+          ar_split(sc[h][t][2 * y], n0, sc[h][t][2 * y + 1], n1, hi, lo);
+          ph[t][y] = ar_transpose(hi);
+          if (SPLIT) pl[t][y] = ar_transpose(lo);
         }
-      const uint8_t* grp = page + g.v_off + (2 * warp + h) * VGB;
+      const uint8_t* grp = my.values + h * VGB;
       uint32_t rec[9];
       if (VB == 4) {
         const uint4 x = *(const uint4*)(grp + lane * 16), y = *(const uint4*)(grp + 512 + lane * 16);
@@ -731,14 +767,23 @@ __global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
         for (int x = 0; x < 4; ++x) {
           // channels r, r + 8; tokens 0-7, 8-15: pairs 4 mt, 4 mt + 2, 4 mt + 1, 4 mt + 3 of the record
           const int pr = 4 * mt + 2 * (x & 1) + (x >> 1);
-          uint32_t b;
-          if (VB == 4) b = __byte_perm(rec[pr >> 2], 0, 0x4440 + (pr & 3));
-          else b = __funnelshift_r(rec[6 * pr >> 5], rec[(6 * pr >> 5) + 1], (6 * pr) & 31) & 63u;
+          uint32_t off;
+          if (VB == 4) {
+            off = __byte_perm(rec[pr >> 2], 0, 0x4440 + (pr & 3)) * Sh::ENTRY;
+          } else {  // the 6-bit field at bit 6 pr, moved to where it is the entry's offset
+            constexpr int UP = SPLIT ? 7 : 6;
+            static_assert(VB == 4 || Sh::ENTRY == 1 << UP, "an entry's size");
+            const int bit = 6 * pr, wd = bit >> 5, b = bit & 31;
+            const uint32_t v = b < UP         ? rec[wd] << (UP - b)
+                               : b > 26       ? __funnelshift_r(rec[wd], rec[wd + 1], b - UP)
+                                              : rec[wd] >> (b - UP);
+            off = v & (63u << UP);
+          }
           if (SPLIT) {
-            const uint2 v = ar_lut2(lutv + b * Sh::ENTRY);
+            const uint2 v = ar_lut2(lutv + off);
             ah[x] = v.x, al[x] = v.y;
           } else {
-            ah[x] = ar_lut1(lutv + b * Sh::ENTRY);
+            ah[x] = ar_lut1(lutv + off);
           }
         }
 #pragma unroll
@@ -751,84 +796,61 @@ __global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
           } else {
             ar_mma(d, ah, ph[t][0], ph[t][1], zero);
           }
-          scaled_add(acc[t][mt], d, inv_n[t], inv_v);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][mt][i] = fmaf(d[i], f[t][i & 1], acc[t][mt][i]);
         }
       }
     }
   };
 
-  // ---- a tile of the uncompressed window
+  // ---- a tile of the uncompressed window: 16 tokens
+  uint32_t b3[SPLIT ? NT : 1][SPLIT ? 8 : 1][2];  // third parts of the queries (bfloat16 windows)
   // the raw queries as B operand, in natural order of channels: k-step j takes channels 16 j ..
   auto hot_weights = [&]() {
+    const bool bf = g.kv_dtype == TQ_BF16;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      float x[4], inv = 1.0f;
-      raw_q(8 * t + warp, x);
-      const bool bf = g.kv_dtype == TQ_BF16;
-      const float up = bf ? 1.0f : ar_lift(row_max(x), 13, inv);
+      float mx = 0.0f, i0 = 1.0f, up = 1.0f;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint32_t w[3] = {0u, 0u, 0u};
-        if (bf) ar_split_bf<SPLIT ? 3 : 1>(x[2 * k], x[2 * k + 1], w);
-        else ar_split(x[2 * k], up, x[2 * k + 1], up, w[0], w[1]);
-        const int d = (4 * lane + 2 * k) & 15;  // channels d, d + 1 of the step: word d / 8 of lane (d % 8) / 2
-        uint32_t* to = (uint32_t*)(sh.w[t][lane >> 2] + (4 * warp + (d & 7) / 2) * 16) + (d >> 3);
-        to[0] = w[0], to[2] = w[1];
-        if (SPLIT) ((uint32_t*)&sh.w3[t][lane >> 2][4 * warp + (d & 7) / 2])[d >> 3] = w[2];
-      }
-      if (lane == 0) sh.inv[8 * t + warp] = inv;
-    }
-  };
-  // Whether the tile has to go term by term, and (float32) the power of two for its values.  Has a barrier.
-  auto hot_check = [&](const uint8_t* tile, float& v_up, float& v_inv) -> bool {
-    bool odd = false;
-    v_up = v_inv = 1.0f;
-    if (hot32) {
-      float top = 0.0f, top_k = 0.0f;
-      for (int k = tid; k < AR_HOT32 * 32; k += AR_THREADS) {
-        const int at = k / 32 * AR_PITCH32 + k % 32 * 16;
-        const float4 x = *(const float4*)(tile + at), y = *(const float4*)(tile + AR_HOT32 * AR_PITCH32 + at);
-        top_k = fmaxf(top_k, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-        top = fmaxf(top, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
-        odd |= !(fabsf(x.x) + fabsf(x.y) + fabsf(x.z) + fabsf(x.w) + fabsf(y.x) + fabsf(y.y) + fabsf(y.z) + fabsf(y.w) < INFINITY);
-      }
-      odd |= top_k > 65504.0f;
+      for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (lane == 0) sh.top[warp] = top;
-      odd = __syncthreads_or(odd);
+        for (int k = 0; k < 4; ++k)
+          mx = fmaxf(mx, fabsf(q_at(q_row(16 * j + 2 * c + (k & 1) + 8 * (k >> 1)), 8 * t + r)));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      if (!bf) up = ar_lift(mx, 13, i0);
 #pragma unroll
-      for (int w = 0; w < AR_WARPS; ++w) top = fmaxf(top, sh.top[w]);
-      v_up = ar_lift(top, 13, v_inv);
-    } else {
-      const uint32_t ones = g.kv_dtype == TQ_F16 ? 0x7c007c00u : 0x7f807f80u;
-      for (int k = tid; k < AR_HOT * 16; k += AR_THREADS) {
-        const uint4 x = *(const uint4*)(tile + (AR_HOT + k / 16) * AR_PITCH + k % 16 * 16);
-        // (an exponent of ones in either half)
+      for (int x = 0; x < 2; ++x) inv[t][x] = __shfl_sync(0xffffffffu, i0, 8 * c + 4 * x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t w = (i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w) & ones;
-          odd |= (w & 0xffffu) == (ones & 0xffffu) || w >> 16 == ones >> 16;
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int d = 16 * j + 2 * c + 8 * k;
+          const float x = q_at(q_row(d), 8 * t + r), y = q_at(q_row(d + 1), 8 * t + r);
+          if (bf) {
+            uint32_t p[3] = {0u, 0u, 0u};
+            ar_split_bf<SPLIT ? 3 : 1>(x, y, p);
+            bh[t][j][k] = p[0], bl[t][j][k] = p[1];
+            if (SPLIT) b3[t][j][k] = p[2];
+          } else {
+            ar_split(x, up, y, up, bh[t][j][k], bl[t][j][k]);
+          }
         }
-      }
-      odd = __syncthreads_or(odd);
     }
-    return odd;
   };
-  auto hot_terms = [&](int t0, int n, size_t ring) {  // this warp's tokens of the tile, term by term
-    const int per = hot_size / AR_WARPS;
-    for (int j = 0; j < per; ++j) {
-      const int tok = t0 + per * warp + j;
-      if (tok >= n) break;
-      const size_t at = ring + (size_t)(tok % g.hot_cap) * TQ_D;
+  auto hot_row = [&](int t) { return (uix * (size_t)g.hot_cap + (size_t)(t % g.hot_cap)) * TQ_D; };  // elements
+  auto hot_terms = [&](int t0, int n) {  // term by term
+#pragma unroll 1
+    for (int tok = t0; tok < min(t0 + AR_HOT, n); ++tok) {
+      const size_t from = hot_row(tok);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const int row = 8 * t + 2 * c + x;
-          if (tok > sh.pos[row] || (tok < sh.win[row] && tok >= a.sinks)) continue;
+          if (tok > pos[t][x] || (tok < win[t][x] && tok >= a.sinks)) continue;
           float dot = 0.0f;
-          for (int d = 0; d < TQ_D; ++d) dot = fmaf(sh.q[q_row(d)][row], attend_ld(a.hot_k, at + d, g.kv_dtype), dot);
+          for (int d = 0; d < TQ_D; ++d) dot = fmaf(q_at(q_row(d), 8 * t + 2 * c + x), attend_ld(a.hot_k, from + d, g.kv_dtype), dot);
+          dot = tq_scaled<true>(dot);
           const float top = fmaxf(m_run[t][x], dot), by = top > -INFINITY ? top : 0.0f;
           const float down = tq_exp2(m_run[t][x] - by), e = tq_exp2(dot - by);
           m_run[t][x] = top;
@@ -837,68 +859,100 @@ __global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
           for (int mt = 0; mt < 8; ++mt)
 #pragma unroll
             for (int y = 0; y < 2; ++y)
-              acc[t][mt][2 * y + x] = fmaf(e, attend_ld(a.hot_v, at + 16 * mt + 8 * y + r, g.kv_dtype),
+              acc[t][mt][2 * y + x] = fmaf(e, attend_ld(a.hot_v, from + 16 * mt + 8 * y + r, g.kv_dtype),
                                            acc[t][mt][2 * y + x] * down);
         }
     }
   };
-  auto hot_attend = [&](const uint8_t* tile, int first, int n, float v_up, float v_inv) {
-    const int ts = 16 * warp, t0 = first + ts;
-    if (ts >= hot_size || t0 >= n || open_to_none(t0, t0 + 16)) return;
+  auto hot_fetch = [&](int t0, int n) {  // 16-bit rows: keys, then values
+    uint8_t* to = my.keys;
+#pragma unroll
+    for (int i = 0; i < 2 * AR_HOT * 16 / 32; ++i) {
+      const int row = (2 * i + (lane >> 4)) % AR_HOT, t = t0 + row;
+      const void* src = i < AR_HOT / 2 ? a.hot_k : a.hot_v;
+      ar_cp16_or_zero(to + (2 * i + (lane >> 4)) * AR_PITCH + (lane & 15) * 16,
+                      (const uint16_t*)src + hot_row(t) + (lane & 15) * 8, t < n);
+    }
+  };
+  auto hot_attend = [&](int t0, int n) {
     const bool bf = g.kv_dtype == TQ_BF16;
-    float sc[2][NT][4], sum[NT][4], low[NT][4];
+    const uint8_t* rows = my.keys;
+    float v_up = 1.0f, v_inv = 1.0f;
+    bool odd = false;
+    if (hot32) {
+      float top = 0.0f, top_k = 0.0f;
+#pragma unroll 4
+      for (int i = 0; i < AR_HOT; ++i) {
+        if (t0 + i >= n) break;
+        const float4 x = *(const float4*)((const float*)a.hot_k + hot_row(t0 + i) + 4 * lane);
+        const float4 y = *(const float4*)((const float*)a.hot_v + hot_row(t0 + i) + 4 * lane);
+        top_k = fmaxf(top_k, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+        odd |= !(fabsf(x.x) + fabsf(x.y) + fabsf(x.z) + fabsf(x.w) + fabsf(y.x) + fabsf(y.y) + fabsf(y.z) + fabsf(y.w) < INFINITY);
+      }
+      odd |= top_k > 65504.0f;
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      v_up = ar_lift(top, 13, v_inv);
+    } else {
+      const uint32_t ones = g.kv_dtype == TQ_F16 ? 0x7c007c00u : 0x7f807f80u;  // (an exponent of ones in either half)
+#pragma unroll
+      for (int i = 0; i < AR_HOT / 2; ++i) {
+        const uint4 x = *(const uint4*)(rows + (AR_HOT + 2 * i + (lane >> 4)) * AR_PITCH + (lane & 15) * 16);
+        const uint32_t y[4] = {x.x & ones, x.y & ones, x.z & ones, x.w & ones};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) odd |= (y[k] & 0xffffu) == (ones & 0xffffu) || y[k] >> 16 == ones >> 16;
+      }
+    }
+    if (__any_sync(0xffffffffu, odd)) {
+      hot_terms(t0, n);
+      return;
+    }
+    // an element of a float32 row (past the last token: zero)
+    auto at32 = [&](const void* p, int t, int d) { return t < n ? ((const float*)p)[hot_row(t) + d] : 0.0f; };
+    float sc[1][NT][4], sum[NT][4], low[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[t][i] = low[t][i] = sc[1][t][i] = 0.0f;
-    const uint32_t k_at = ar_smem(tile) + (ts + (lane & 15)) * AR_PITCH + (lane >> 4) * 16;
+      for (int i = 0; i < 4; ++i) sum[t][i] = low[t][i] = 0.0f;
+    const uint32_t k_at = ar_smem(rows) + (lane & 15) * AR_PITCH + (lane >> 4) * 16;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       uint32_t ah[4], al[4] = {0u, 0u, 0u, 0u};
       if (hot32) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const float2 f = *(const float2*)(tile + (ts + r + 8 * (x & 1)) * AR_PITCH32 + (16 * j + 2 * c + 8 * (x >> 1)) * 4);
-          ar_split(f.x, 1.0f, f.y, 1.0f, ah[x], al[x]);
+          const int t = t0 + r + 8 * (x & 1), d = 16 * j + 2 * c + 8 * (x >> 1);
+          ar_split(at32(a.hot_k, t, d), 1.0f, at32(a.hot_k, t, d + 1), 1.0f, ah[x], al[x]);
         }
       } else {
         ar_ldm<false>(ah, k_at + 32 * j);
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const uint4 w = *(const uint4*)(sh.w[t][j] + lane * 16);
+        float d[4];
         if (bf) {
+          ar_mma_bf(d, ah, bh[t][j][0], bh[t][j][1], zero);
           if (SPLIT) {
-            const uint2 w3 = sh.w3[t][j][lane];
-            float d[4];
-            ar_mma_bf(d, ah, w.x, w.y, zero);
-            ar_mma_bf(low[t], ah, w.z, w.w, low[t]);
-            ar_mma_bf(low[t], ah, w3.x, w3.y, low[t]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[t][i] += d[i];
-          } else {
-            ar_mma_bf(sum[t], ah, w.x, w.y, sum[t]);
+            ar_mma_bf(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
+            ar_mma_bf(low[t], ah, b3[t][j][0], b3[t][j][1], low[t]);
           }
         } else {
-          float d[4];
-          ar_mma(d, ah, w.x, w.y, zero);
-          if (SPLIT || hot32) {
-            ar_mma(low[t], ah, w.z, w.w, low[t]);
-            if (hot32) ar_mma(low[t], al, w.x, w.y, low[t]);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum[t][i] += d[i];
+          ar_mma(d, ah, bh[t][j][0], bh[t][j][1], zero);
+          if (SPLIT || hot32) ar_mma(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
+          if (hot32) ar_mma(low[t], al, bh[t][j][0], bh[t][j][1], low[t]);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[t][i] += d[i];
       }
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sc[0][t][i] = tq_scaled<true>((sum[t][i] + low[t][i]) * sh.inv[8 * t + 2 * c + (i & 1)]);
+      for (int i = 0; i < 4; ++i) sc[0][t][i] = tq_scaled<true>((sum[t][i] + low[t][i]) * inv[t][i & 1]);
     float inv_n[NT][2];
-    const float nv[2][2] = {{1.0f, 1.0f}, {0.0f, 0.0f}};
-    softmax(sc, t0, n, 1, nv, inv_n);
+    const float nv[1][2] = {{1.0f, 1.0f}};
+    softmax(sc, t0, n, ArTiles<1>(), nv, inv_n);
     uint32_t p[NT][2][3] = {};
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -909,16 +963,15 @@ __global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
 #pragma unroll
         for (int k = 0; k < (SPLIT ? 3 : 2); ++k) p[t][y][k] = ar_transpose(p[t][y][k]);
       }
-    const uint8_t* v = tile + hot_size * (hot32 ? AR_PITCH32 : AR_PITCH);
-    const uint32_t v_at = ar_smem(v) + (ts + (lane & 7) + (lane >> 4) * 8) * AR_PITCH + (lane >> 3 & 1) * 16;
+    const uint32_t v_at = ar_smem(rows) + (AR_HOT + (lane & 7) + (lane >> 4) * 8) * AR_PITCH + (lane >> 3 & 1) * 16;
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) {
       uint32_t ah[4], al[4] = {0u, 0u, 0u, 0u};
       if (hot32) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {  // channels r, r + 8; tokens 2 c, 2 c + 1, and 8 further
-          const float* f = (const float*)(v + (ts + 2 * c + 8 * (x >> 1)) * AR_PITCH32) + 16 * mt + r + 8 * (x & 1);
-          ar_split(f[0], v_up, f[AR_PITCH32 / 4], v_up, ah[x], al[x]);
+          const int t = t0 + 2 * c + 8 * (x >> 1), d = 16 * mt + r + 8 * (x & 1);
+          ar_split(at32(a.hot_v, t, d), v_up, at32(a.hot_v, t + 1, d), v_up, ah[x], al[x]);
         }
       } else {
         ar_ldm<true>(ah, v_at + 32 * mt);
@@ -939,134 +992,132 @@ __global__ void __launch_bounds__(AR_THREADS, !SPLIT&& NT == 1 ? 2 : 1)
           if (hot32) ar_mma(d, al, p[t][0][0], p[t][1][0], d);
           ar_mma(d, ah, p[t][0][0], p[t][1][0], d);
         }
-        scaled_add(acc[t][mt], d, inv_n[t], v_inv);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][mt][i] = fmaf(d[i], inv_n[t][i & 1] * v_inv, acc[t][mt][i]);
       }
     }
   };
 
-  // ---- the warps' states become one: `work` has room for the sums of eight rows of every warp
-  auto flush = [&](const ArItem& i, const ArWork& w, bool hot, uint8_t* room) {
-    const int head = i.row / row_tiles, row0 = i.row % row_tiles * N, unit = i.s * H + head;
-    const int64_t begin = (int64_t)sh.cum[i.s] * rows_per_seq + (int64_t)i.row * w.cost();
-    const int slot = hot ? a.ns_cold + (int)(blockIdx.x - (begin + AR_COST * w.page.count()) / share)
-                         : (int)(blockIdx.x - begin / share);
+  // ---- a state
+  auto flush = [&](bool hot) {
+    const int64_t from = hot ? begin + AR_COST * row_strips : begin;
+    const int slot = (hot ? a.ns_cold : 0) + (int)(me - ar_div(from, share));
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
 #pragma unroll
         for (int o = 4; o <= 16; o <<= 1) l_run[t][x] += __shfl_xor_sync(0xffffffffu, l_run[t][x], o);
-        if (r == 0) {
-          sh.m[warp][8 * t + 2 * c + x] = m_run[t][x];
-          sh.l[warp][8 * t + 2 * c + x] = l_run[t][x];
-        }
-      }
-    float* const sums = (float*)room;  // [warp][8 rows][128], two bits of the channel by the row
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      __syncthreads();  // (the item, or the eight rows before, have been read)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int n = 8 * t + 2 * c + x;
-        float M = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < AR_WARPS; ++k) M = fmaxf(M, sh.m[k][n]);
-        const float by = M > -INFINITY ? M : 0.0f;
-        const float f = l_run[t][x] == 0.0f ? 0.0f : m_run[t][x] > -INFINITY ? tq_exp2(m_run[t][x] - by) : 1.0f;
+        const int row = row0 + 8 * t + 2 * c + x;
+        if (row >= a.rows) continue;
+        float* to = attend_partial(a, s * H + head, row, slot);
+        if (r == 0) *(float2*)to = make_float2(m_run[t][x], l_run[t][x]);
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt)
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
-            sums[(warp * 8 + 2 * c + x) * TQ_D + ((16 * mt + 8 * y + r) ^ (8 * c))] =
-                l_run[t][x] == 0.0f ? 0.0f : acc[t][mt][2 * y + x] * f;
+          for (int y = 0; y < 2; ++y) to[2 + 16 * mt + 8 * y + r] = acc[t][mt][2 * y + x];
       }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < 8 * TQ_D / AR_THREADS; ++k) {
-        const int n = k * (AR_THREADS / TQ_D) + tid / TQ_D, d = tid % TQ_D;
-        if (row0 + 8 * t + n >= a.rows) break;
-        float x = 0.0f;
-#pragma unroll
-        for (int u = 0; u < AR_WARPS; ++u) x += sums[(u * 8 + n) * TQ_D + (d ^ (8 * (n >> 1)))];
-        float* to = attend_partial(a, unit, row0 + 8 * t + n, slot);
-        to[2 + d] = x;
-        if (d == 0) {
-          float M = -INFINITY, L = 0.0f;
-#pragma unroll
-          for (int u = 0; u < AR_WARPS; ++u) M = fmaxf(M, sh.m[u][8 * t + n]);
-          const float by = M > -INFINITY ? M : 0.0f;
-#pragma unroll
-          for (int u = 0; u < AR_WARPS; ++u)
-            if (sh.l[u][8 * t + n] != 0.0f)
-              L += sh.m[u][8 * t + n] > -INFINITY ? sh.l[u][8 * t + n] * tq_exp2(sh.m[u][8 * t + n] - by) : sh.l[u][8 * t + n];
-          to[0] = M;
-          to[1] = L;
-        }
-      }
-    }
   };
 
   // ---- the share, item by item
-  bool new_row = true, new_kind = true;
-  for (;;) {
-    uint8_t* const item = sh.stage[st];
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();  // the item has landed; the one before it, and what was made for it, has been read
-    const ArWork w = work_of(cur.s);
-    const bool hot = cur.it >= w.page.count(), more = nxt.at < hi;
-    if (more) {
-      fetch(nxt, pm_next, sh.stage[st ^ 1]);
+  bool more = true;
+  while (more) {
+    // a row tile's strips, then its tiles of the window, as far as the share goes
+    start_row();
+    if (it < row_strips) {
+      reset();
+      int strip = w.strip.at(it), ts = (strip & 3) * AR_STRIP;
+      page = page_of(it);
+      open_list(it, ts);
+      copy_keys(page, ts, list_at);
       ar_commit();
-    }
-    if (new_row) {
-      start_row(cur);
-      if (!hot) __syncthreads();  // (the corrections of a page read the queries before its barrier)
-    }
-    if (new_kind) reset();
-    const size_t u = unit_of(cur);
-    const int first = hot ? w.cold + w.hot.at(cur.it - w.page.count()) * hot_size : w.page.at(cur.it) * AR_S;
-    float v_up = 1.0f, v_inv = 1.0f;
-    bool odd = false;
-    if (hot) {
-      if (new_kind) hot_weights();
-      odd = hot_check(item, v_up, v_inv);
-    } else {
-      page_prepare(item, pm, u);
-      __syncthreads();
-    }
-    const ArItem nn = more ? after(nxt) : nxt;
-    const PageMeta pm_nn = more ? meta_of(nn) : pm_next;
-    const bool row_ends = !more || nxt.row != cur.row || nxt.s != cur.s;
-    if (more && row_ends) {
-      fetch_q(nxt);
+      copy_values(page, ts);
       ar_commit();
+      bool new_page = true;
+      for (;;) {
+        at += AR_COST;
+        const int i1 = it + 1;
+        const bool last = i1 >= row_strips || at >= stop;
+        const int next = last ? strip : w.strip.at(i1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");  // the key half has landed
+        __syncwarp();
+        const int t0 = strip * AR_STRIP;
+        const bool seen = !open_to_none(t0, t0 + AR_STRIP);
+        float sc[4][NT][4];
+        if (new_page) weights();
+        if (seen) strip_scores(sc, ts);
+        else if (SPLIT) list_next = 0xffffffffu;
+        __syncwarp();  // the key half has been read
+        const bool turn = next >> 2 != strip >> 2;  // the next strip is of another page
+        if (!last) {
+          if (turn) {
+            page = page_of(i1);
+            open_list(i1, (next & 3) * AR_STRIP);
+          } else if (SPLIT) {
+            if (next == strip + 1 && list_next != 0xffffffffu) list_at = list_next;
+            else open_list(i1, (next & 3) * AR_STRIP);
+          }
+          copy_keys(page, (next & 3) * AR_STRIP, list_at);
+        }
+        ar_commit();
+        asm volatile("cp.async.wait_group 1;" ::: "memory");  // the value half has landed
+        __syncwarp();
+        if (seen) {
+          float nv[4][2], inv_n[NT][2];
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) nv[h][y] = my.norms[16 * h + 8 * y + r];
+          softmax(sc, t0, w.cold, ArTiles<4>(), nv, inv_n);
+          strip_values(sc, nv, inv_n);
+        }
+        __syncwarp();  // the value half has been read
+        if (!last) copy_values(page, (next & 3) * AR_STRIP);
+        ar_commit();
+        it = i1;
+        if (last) break;
+        strip = next, ts = (next & 3) * AR_STRIP;
+        new_page = turn;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      flush(false);
+      more = at < stop;
     }
-    if (hot) {
-      if (odd) hot_terms(first, sh.seq[cur.s].x, u * (size_t)g.hot_cap * TQ_D);
-      else hot_attend(item, first, sh.seq[cur.s].x, v_up, v_inv);
-    } else {
-      page_attend(item, first, w.cold);
+    if (more && it < row_items) {
+      reset();
+      hot_weights();
+      const int n = sh.seq[s].x;
+      for (; it < row_items && at < stop; ++it, ++at) {
+        const int t0 = w.cold + w.hot.at(it - row_strips) * AR_HOT;
+        if (open_to_none(t0, min(t0 + AR_HOT, n))) continue;
+        if (!hot32) {
+          hot_fetch(t0, n);
+          ar_commit();
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          __syncwarp();
+        }
+        hot_attend(t0, n);
+        __syncwarp();  // the rows have been read
+      }
+      flush(true);
+      more = at < stop;
     }
-    const bool kind_ends = row_ends || (!hot && nxt.it >= w.page.count());
-    if (kind_ends) flush(cur, w, hot, item);
-    if (!more) break;
-    new_row = row_ends;
-    new_kind = kind_ends;
-    cur = nxt, nxt = nn;
-    pm = pm_next, pm_next = pm_nn;
-    st ^= 1;
+    if (more) more = next_row();
   }
 }
 
 // ---------------------------------------------------------------------------------------------------
-// Merge of the states: four rows at a time, a group of 128 threads each, which sums the row's slots in order; then all
-// 512 threads rotate the four sums of pages, a quarter of the input channels each, whose rows of Pi they hold
-// in registers from before the states were there.
+// Merge of the states: a row's slots are summed in order by groups of 128 threads, a thread per channel; the pages' sum is
+// then rotated by all 512 threads, a quarter of the input channels each, whose rows of Pi they hold in registers
+// from before the states were there.  ROWS = 4: a group per row, four rows at a time; ROWS = 1 (few rows, which
+// then have many slots): every group takes a fourth of the row's slots.
 // ---------------------------------------------------------------------------------------------------
 constexpr int AC_THREADS = 512;
 
-__global__ void __launch_bounds__(AC_THREADS) attend_rows_combine_kernel(AttendArgs a, int row_tiles, int tile, int total) {
-  __shared__ __align__(16) float cs[TQ_D][4], ys[4][4][TQ_D];
+template <int ROWS>
+__global__ void __launch_bounds__(AC_THREADS) attend_rows_combine_kernel(AttendArgs a, int tile, int total) {
+  __shared__ __align__(16) float cs[TQ_D][4], ys[4][ROWS][TQ_D], hs[4][TQ_D], ls[4][TQ_D];
   const tq_geom& g = a.g;
   const int tid = threadIdx.x, e = tid % TQ_D, h = tid / TQ_D;
   const int H = g.n_kv_heads, G = g.group;
@@ -1076,8 +1127,8 @@ __global__ void __launch_bounds__(AC_THREADS) attend_rows_combine_kernel(AttendA
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const ArPlan* plan = (const ArPlan*)a.plan;
   const int64_t share = plan->share;
-  for (int r0 = blockIdx.x * 4; r0 < total; r0 += gridDim.x * 4) {
-    const int at = r0 + h;
+  for (int r0 = blockIdx.x * ROWS; r0 < total; r0 += gridDim.x * ROWS) {
+    const int at = r0 + (ROWS == 4 ? h : 0);
     float hot = 0.0f, L = 0.0f, x = 0.0f;
     int s = 0, head = 0, row = 0;
     if (at < total) {
@@ -1085,49 +1136,65 @@ __global__ void __launch_bounds__(AC_THREADS) attend_rows_combine_kernel(AttendA
       const int unit = at / a.rows;
       s = unit / H, head = unit - s * H;
       const AttendSeq sq = attend_seq(a, s);
-      const ArWork w = ar_work(a, sq.n, sq.q_n);
-      const int64_t begin = (int64_t)plan->cum[s] * H * row_tiles + (int64_t)(head * row_tiles + row / tile) * w.cost();
-      const int pages = w.page.count(), hots = w.hot.count();
-      const int64_t middle = begin + AR_COST * pages;
-      const int nc = pages > 0 ? (int)((middle - AR_COST) / share - begin / share) + 1 : 0;
-      const int nh = hots > 0 ? (int)((middle + hots - 1) / share - middle / share) + 1 : 0;
-      const float* base = attend_partial(a, unit, row, 0);
-      auto slot = [&](int i) { return base + (size_t)(i < nc ? i : a.ns_cold + i - nc) * TQ_PART_STRIDE; };
-      float M = -INFINITY;
+      const int tiles = ar_tiles(a, sq.q_n, tile);
+      if (row / tile < tiles) {
+        const ArWork w = ar_work(a, sq.n, sq.q_n);
+        const int64_t begin = plan->cum[s] + (int64_t)(head * tiles + row / tile) * w.cost();
+        const int strips = w.strip.count(), hots = w.hot.count();
+        const int64_t middle = begin + AR_COST * strips;
+        const int nc = strips > 0 ? (int)(ar_div(middle - AR_COST, share) - ar_div(begin, share)) + 1 : 0;
+        const int nh = hots > 0 ? (int)(ar_div(middle + hots - 1, share) - ar_div(middle, share)) + 1 : 0;
+        const float* base = attend_partial(a, unit, row, 0);
+        auto slot = [&](int i) { return base + (size_t)(i < nc ? i : a.ns_cold + i - nc) * TQ_PART_STRIDE; };
+        float M = -INFINITY;
 #pragma unroll 8
-      for (int i = 0; i < nc + nh; ++i) M = fmaxf(M, slot(i)[0]);
-      const float by = M > -INFINITY ? M : 0.0f;
+        for (int i = 0; i < nc + nh; ++i) M = fmaxf(M, slot(i)[0]);
+        const float by = M > -INFINITY ? M : 0.0f;
 #pragma unroll 8
-      for (int i = 0; i < nc + nh; ++i) {
-        const float* p = slot(i);
-        const float mi = p[0], li = p[1], v = p[2 + e];
-        const float f = li == 0.0f ? 0.0f : mi > -INFINITY ? tq_exp2(mi - by) : 1.0f;
-        if (f == 0.0f && li == 0.0f) continue;
-        L += li * f;
-        if (i < nc) x += v * f;
-        else hot += v * f;
+        for (int i = ROWS == 4 ? 0 : h; i < nc + nh; i += ROWS == 4 ? 1 : 4) {
+          const float* p = slot(i);
+          const float mi = p[0], li = p[1], v = p[2 + e];
+          if (li == 0.0f) continue;
+          const float f = mi > -INFINITY ? tq_exp2(mi - by) : 1.0f;
+          L = fmaf(li, f, L);
+          if (i < nc) x = fmaf(v, f, x);
+          else hot = fmaf(v, f, hot);
+        }
       }
     }
     cs[e][h] = x;
+    if (ROWS == 1) hs[h][e] = hot, ls[h][e] = L;
     __syncthreads();
-    float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float y[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) y[k] = 0.0f;
 #pragma unroll
     for (int d = 0; d < TQ_D / 4; ++d) {
       const float4 v = *(const float4*)cs[32 * h + d];
-      y[0] = fmaf(v.x, pi[d], y[0]), y[1] = fmaf(v.y, pi[d], y[1]);
-      y[2] = fmaf(v.z, pi[d], y[2]), y[3] = fmaf(v.w, pi[d], y[3]);
+      if constexpr (ROWS == 4) {
+        y[0] = fmaf(v.x, pi[d], y[0]), y[1] = fmaf(v.y, pi[d], y[1]);
+        y[2] = fmaf(v.z, pi[d], y[2]), y[3] = fmaf(v.w, pi[d], y[3]);
+      } else {
+        y[0] = fmaf((v.x + v.y) + (v.z + v.w), pi[d], y[0]);
+      }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) ys[h][k][e] = y[k];
+    for (int k = 0; k < ROWS; ++k) ys[h][k][e] = y[k];
     __syncthreads();
-    if (at < total) {
-      const float o = (ys[0][h][e] + ys[1][h][e]) + (ys[2][h][e] + ys[3][h][e]) + hot;
+    if (at < total && (ROWS == 4 || h == 0)) {
+      if (ROWS == 1) {
+        hot = (hs[0][e] + hs[1][e]) + (hs[2][e] + hs[3][e]);
+        L = (ls[0][e] + ls[1][e]) + (ls[2][e] + ls[3][e]);
+      }
+      const int k = ROWS == 4 ? h : 0;
+      const float o = (ys[0][k][e] + ys[1][k][e]) + (ys[2][k][e] + ys[3][k][e]) + hot;
       const float v = L == 0.0f ? 0.0f : o / L;
       const size_t to = (((size_t)s * a.n_tokens + row / G) * g.n_q_heads + head * G + row % G) * TQ_D + e;
       if (a.q_dtype == TQ_F32) ((float*)a.out)[to] = v;
       else if (a.q_dtype == TQ_F16) ((__half*)a.out)[to] = __float2half_rn(v);
       else ((__nv_bfloat16*)a.out)[to] = __float2bfloat16_rn(v);
     }
+    if (ROWS == 1) __syncthreads();  // (the sums have been read)
   }
 }
 
@@ -1135,26 +1202,24 @@ template <int NT, bool SPLIT, int VB>
 int launch_rows(const AttendArgs& a, int sm_count, cudaStream_t st) {
   using Shared = ArShared<NT, SPLIT, VB>;
   static_assert(sizeof(Shared) <= 227 * 1024, "shared memory of one CTA");
-  static_assert(SPLIT || NT > 1 || sizeof(Shared) <= 113 * 1024, "two CTAs on an SM");
-  constexpr int PER_SM = !SPLIT && NT == 1 ? 2 : 1;
-  const int row_tiles = (a.rows + 8 * NT - 1) / (8 * NT);
   const int64_t all = (int64_t)a.seq_count * a.g.n_kv_heads * a.rows;
   TQ_REQUIRE(all <= INT_MAX - 4 * AC_THREADS, TQ_ERR_UNSUPPORTED, "too many query rows in a call");
-  TQ_REQUIRE((ArShape<NT, SPLIT, VB>::PAGE <= a.g.page_bytes), TQ_ERR_INVALID, "page size");
   TQ_CUDA(cudaFuncSetAttribute(attend_rows_kernel<NT, SPLIT, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                (int)sizeof(Shared)));
-  attend_rows_kernel<NT, SPLIT, VB><<<PER_SM * sm_count, AR_THREADS, sizeof(Shared), st>>>(a, row_tiles);
+  attend_rows_kernel<NT, SPLIT, VB><<<sm_count, 32 * ArShape<NT, SPLIT, VB>::WARPS, sizeof(Shared), st>>>(a);
   TQ_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)std::min<int64_t>((all + 3) / 4, 2 * sm_count));
+  const bool few = all <= 4 * sm_count;
+  cfg.gridDim = dim3((unsigned)(few ? all : std::min<int64_t>((all + 3) / 4, 2 * sm_count)));
   cfg.blockDim = dim3(AC_THREADS);
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  TQ_CUDA(cudaLaunchKernelEx(&cfg, attend_rows_combine_kernel, a, row_tiles, 8 * NT, (int)all));
+  if (few) TQ_CUDA(cudaLaunchKernelEx(&cfg, attend_rows_combine_kernel<1>, a, 8 * NT, (int)all));
+  else TQ_CUDA(cudaLaunchKernelEx(&cfg, attend_rows_combine_kernel<4>, a, 8 * NT, (int)all));
   return TQ_OK;
 }
 
@@ -1171,19 +1236,17 @@ AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens, int sm_count
   const int nt = a.rows <= 8 ? 1 : 2;
   p.seqs = AR_SEQS;
   p.plan_bytes = align_up(sizeof(ArPlan), 256);
-  // Slots for the states of a row: what its work meets at the shares of this call, and a few more (the kernel
-  // makes the shares larger where they would not do).
-  const int nb = n_cold_blocks(tokens, g.hot_window, AR_S);
-  const int64_t pages = a.window == INT_MAX
-                            ? nb
-                            : std::min<int64_t>(nb, ((int64_t)a.window + a.n_tokens + 510) / 256 + (a.sinks + 255) / 256);
-  const int64_t size = g.kv_dtype == TQ_F32 ? AR_HOT32 : AR_HOT;
-  const int64_t hot = (std::min(tokens, g.hot_window) + size - 1) / size;
+  // Slots for the states of a row: what its work meets at the shares of this call where the other sequences are
+  // half as long, and a few more (the kernel makes the shares larger where they would not do).
+  const int64_t in_blocks = (int64_t)n_cold_blocks(tokens, g.hot_window, AR_S) * AR_S;
+  const int64_t seen = a.window == INT_MAX ? in_blocks : std::min<int64_t>(in_blocks, (int64_t)a.window + a.n_tokens + 128);
+  const int64_t strips = (seen + AR_STRIP - 1) / AR_STRIP + (std::min<int64_t>(a.sinks, in_blocks) + AR_STRIP - 1) / AR_STRIP;
+  const int64_t hot = (std::min(tokens, g.hot_window) + AR_HOT - 1) / AR_HOT;
   const int64_t rows = (int64_t)std::min(a.seq_count, AR_SEQS) * g.n_kv_heads * ((a.rows + 8 * nt - 1) / (8 * nt));
-  const int64_t ctas = (int64_t)sm_count * (a.q_dtype == TQ_BF16 && nt == 1 ? 2 : 1);
-  const int64_t share = std::max<int64_t>((AR_COST * pages + hot) * rows / 2 / ctas, AR_COST);  // (others may be shorter)
-  p.ns_cold = (int)std::min<int64_t>(AR_COST * pages / share + 3, 64);
-  p.ns_hot = (int)std::min<int64_t>(hot / share + 3, 32);
+  const int64_t workers = (int64_t)sm_count * (a.q_dtype == TQ_BF16 ? (nt == 1 ? 12 : 8) : (nt == 1 ? 8 : 6));
+  const int64_t share = std::max<int64_t>((AR_COST * strips + hot) * ((rows + 1) / 2) / workers, AR_COST);
+  p.ns_cold = (int)std::min<int64_t>(AR_COST * strips / share + 3, 1024);
+  p.ns_hot = (int)std::min<int64_t>(hot / share + 3, 64);
   return p;
 }
 
