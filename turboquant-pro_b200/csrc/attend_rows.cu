@@ -3,7 +3,7 @@
 // straight from a table into registers, and NT tiles of eight query rows as the B operand.
 //
 // Persistent CTAs, one an SM; every warp works alone, without barriers.  The 64-token strips of pages that the rows
-// of each (sequence, KV head, row tile) see, first tokens, then the window, and after them the 16-token tiles of the
+// of each (sequence, KV head, row tile) see, first tokens, then the window, and after them the 32-token tiles of the
 // uncompressed window, form one list that is cut into shares of equal cost, one per warp, so ragged batches and every
 // number of heads balance; where a share leaves a row tile, or goes from pages to the window, the warp writes a
 // state, and the merge sums these.  What a warp needs of a strip comes with cp.async into its own piece of shared
@@ -39,9 +39,9 @@ namespace {
 
 constexpr int AR_S = 256;          // tokens of a page
 constexpr int AR_STRIP = 64;       // of them, in an item of the list
-constexpr int AR_HOT = 16;         // window tokens of an item
+constexpr int AR_HOT = 32;         // window tokens of an item
 constexpr int AR_PITCH = TQ_D * 2 + 16;  // bytes of a window row in shared memory
-constexpr int AR_COST = 4;         // a strip takes the time of so many tiles of the window
+constexpr int AR_COST = 2;         // a strip takes the time of so many tiles of the window
 constexpr int AR_SEQS = 64;        // sequences of a launch
 constexpr int AR_LIST = 256;       // outliers of a strip that are copied ahead (160 is usual)
 
@@ -55,7 +55,7 @@ struct ArShape {
   static constexpr int LUTK = 256 * ENTRY, LUTV = NV * ENTRY;
 };
 
-// A warp's strip of a page, or a tile of the window (two rows of AR_PITCH bytes a token) in its place.
+// A warp's strip of a page, or the values of a tile of the window in its place.
 template <int NT, bool SPLIT, int VB>
 struct alignas(16) ArWarp {
   uint8_t keys[AR_STRIP * TQ_D / 2];
@@ -71,7 +71,7 @@ struct alignas(16) ArWarp {
   float corr[32][8 * NT];           // outliers' part of the scores of 32 tokens
   uint8_t q[TQ_D][8 * NT * (SPLIT ? 4 : 2)];  // row q_row(d): channel d
 };
-static_assert(2 * AR_HOT * AR_PITCH <= 6528 + 64 * TQ_D * 3 / 8 + 256, "a tile of the window in a strip's place");
+static_assert(AR_HOT * AR_PITCH <= 6528 + 64 * TQ_D * 3 / 8 + 256, "a tile of the window in a strip's place");
 
 template <int NT, bool SPLIT, int VB>
 struct ArShared {
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
   const tq_geom& g = a.g;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
   const int H = g.n_kv_heads, G = g.group;
-  const bool q32 = a.q_dtype == TQ_F32, hot32 = g.kv_dtype == TQ_F32;
+  const bool q32 = a.q_dtype == TQ_F32;
   ArWarp<NT, SPLIT, VB>& my = sh.warp[warp];
 
   // ---- the work before every sequence
@@ -272,39 +272,12 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
   const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;
   if (share * blockIdx.x >= total) return;  // (the whole CTA)
 
-  // ---- tables of pairs
-  float inv_k, inv_v;
-  {
-    float max_k = 0.0f, max_v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      max_k = fmaxf(max_k, fabsf(sh.grid[i]));
-      max_v = fmaxf(max_v, fabsf(sh.cent[i]));
-    }
-    const float up_k = ar_lift(max_k, 7, inv_k), up_v = ar_lift(max_v, 7, inv_v);
-    for (int e = tid; e < 256 + Sh::NV; e += THREADS) {
-      uint32_t hi, lo;
-      uint4* to;
-      if (e < 256) {
-        ar_split(sh.grid[e & 15], up_k, sh.grid[e >> 4], up_k, hi, lo);
-        to = (uint4*)(sh.lut + e * Sh::ENTRY);
-      } else {
-        const int b = e - 256;
-        ar_split(sh.cent[b & ((1 << VB) - 1)], up_v, sh.cent[b >> VB], up_v, hi, lo);
-        to = (uint4*)(sh.lut + Sh::LUTK + b * Sh::ENTRY);
-      }
-#pragma unroll
-      for (int i = 0; i < Sh::ENTRY / 16; ++i)
-        to[(i + lane) % (Sh::ENTRY / 16)] = SPLIT ? make_uint4(hi, lo, hi, lo) : make_uint4(hi, hi, hi, hi);
-    }
-  }
-  __syncthreads();  // (the last one)
-  int64_t at = share * me;
-  const int64_t stop = min(at + share, total);
-  if (at >= total) return;
 
   // ---- where the share begins: sequence, head, row tile, item
-  int s, head, rt, it, row_items, row_strips, row_tiles;
+  int64_t at = share * me;
+  const int64_t stop = min(at + share, total);
+  bool more = at < total;
+  int s = 0, head = 0, rt = 0, it = 0, row_items = 0, row_strips = 0, row_tiles = 1;
   ArWork w;
   auto enter_seq = [&]() {
     w = ar_work(a, sh.seq[s].x, sh.seq[s].y);
@@ -312,8 +285,8 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
     row_items = w.items();
     row_tiles = ar_tiles(a, sh.seq[s].y, N);
   };
-  int64_t begin;  // the cost of what is before this row
-  {
+  int64_t begin = 0;  // the cost of what is before this row
+  if (more) {
     int x = 0, y = a.seq_count - 1;
     while (x < y) {  // the last sequence that starts here or before
       const int mid = (x + y + 1) >> 1;
@@ -345,8 +318,8 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
     enter_seq();
     return true;
   };
-  if (it == row_items && !next_row()) return;  // (it began within the last strip of a row without a window)
-  if (at >= stop) return;
+  if (more && it == row_items) more = next_row();  // (it began within the last strip of a row without a window)
+  more = more && at < stop;
 
   // ---- copies
   size_t uix = 0;
@@ -418,33 +391,29 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
       for (int x = 0; x < 2; ++x) m_run[t][x] = -INFINITY, l_run[t][x] = 0.0f;
     }
   };
-  // four neighbouring channels of a query row (rows that are not there: zeros)
-  auto load_q = [&](int row, int d, float (&x)[4]) {
-    x[0] = x[1] = x[2] = x[3] = 0.0f;
-    if (row >= a.rows) return;
-    const int64_t from = (int64_t)s * a.q_seq + (int64_t)(row / G) * a.q_tok + (int64_t)(head * G + row % G) * a.q_head + d;
-    if (SPLIT && q32) {
-      const float4 v = *(const float4*)((const float*)a.q + from);
-      x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-    } else {
-      const uint2 v = *(const uint2*)((const uint16_t*)a.q + from);
-      if (SPLIT) {
-        const float2 u = __half22float2(*(const __half2*)&v.x), f = __half22float2(*(const __half2*)&v.y);
-        x[0] = u.x, x[1] = u.y, x[2] = f.x, x[3] = f.y;
-      } else {
-        x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
-        x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
-      }
-    }
-  };
   // the rows' queries in shared memory as they are; float32 ones are asked for as scores' units where they are used
   auto q_at = [&](int qrow, int n) -> float {
     if (SPLIT) return ((const float*)my.q[qrow])[n];
     return __uint_as_float((uint32_t)((const uint16_t*)my.q[qrow])[n] << 16);
   };
-  auto start_row = [&]() {
+  // A row tile's queries and positions; in two parts, so that other work can go on while the queries come.
+  float4 q_raw[N * (SPLIT ? 1 : 0) + 1];
+  uint2 q_half[N];
+  auto fetch_row = [&]() {
     uix = unit_index(g, a.layer, a.seq_begin + s, head);
     row0 = rt * N;
+    int i = row0 / G, k = row0 - i * G;  // query token and head of the group
+    const int64_t from = (int64_t)s * a.q_seq + (int64_t)(head * G) * a.q_head + 4 * lane;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int64_t e = from + (int64_t)i * a.q_tok + (int64_t)k * a.q_head;
+      const bool there = row0 + n < a.rows;
+      if (SPLIT && q32) q_raw[n] = there ? *(const float4*)((const float*)a.q + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      else q_half[n] = there ? *(const uint2*)((const uint16_t*)a.q + e) : make_uint2(0u, 0u);
+      if (++k == G) k = 0, ++i;
+    }
+  };
+  auto start_row = [&]() {
     const int n = sh.seq[s].x, q_n = sh.seq[s].y, first = n - q_n;
     const int last = min(min(row0 + N, a.rows), q_n * G) - 1;
     p_lo = first + row0 / G;
@@ -462,13 +431,19 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
       }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float x[4];
-      load_q(row0 + i, 4 * lane, x);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (SPLIT) ((float*)my.q[q_row(4 * lane + k)])[i] = x[k];
-        else ((uint16_t*)my.q[q_row(4 * lane + k)])[i] = (uint16_t)(__float_as_uint(x[k]) >> 16);
+    for (int k = 0; k < N; ++k) {
+      if (SPLIT) {
+        float4 x = q_raw[k];
+        if (!q32) {
+          const float2 u = __half22float2(*(const __half2*)&q_half[k].x), f = __half22float2(*(const __half2*)&q_half[k].y);
+          x = make_float4(u.x, u.y, f.x, f.y);
+        }
+        ((float*)my.q[q_row(4 * lane)])[k] = x.x, ((float*)my.q[q_row(4 * lane + 1)])[k] = x.y;
+        ((float*)my.q[q_row(4 * lane + 2)])[k] = x.z, ((float*)my.q[q_row(4 * lane + 3)])[k] = x.w;
+      } else {
+        const uint2 x = q_half[k];
+        ((uint16_t*)my.q[q_row(4 * lane)])[k] = (uint16_t)x.x, ((uint16_t*)my.q[q_row(4 * lane + 1)])[k] = (uint16_t)(x.x >> 16);
+        ((uint16_t*)my.q[q_row(4 * lane + 2)])[k] = (uint16_t)x.y, ((uint16_t*)my.q[q_row(4 * lane + 3)])[k] = (uint16_t)(x.y >> 16);
       }
     }
     __syncwarp();
@@ -536,6 +511,7 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
   };
 
   // ---- a strip of a page
+  float inv_k, inv_v;  // of the tables
   const uint32_t lutk = ar_smem(sh.lut) + (lane & 15) * (SPLIT ? 8 : 4), lutv = lutk + Sh::LUTK;
   uint32_t bh[NT][8][2], bl[NT][8][2];  // weights: k-step j takes channels 32 c + 4 j .. + 3, column r is row 8 t + r
   float bias[NT][2], inv[NT][2];
@@ -669,71 +645,67 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
     }
     __syncwarp();
   };
-  // scores of the strip's four tiles
-  auto strip_scores = [&](float (&sc)[4][NT][4], int ts) {
+  // scores of tokens 32 half .. + 31 of the strip
+  auto strip_scores = [&](float (&sc)[2][NT][4], int half, int ts) {
+    if (g.outlier_k > 0) corrections(half, ts);
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (g.outlier_k > 0) corrections(half, ts);
+    for (int h = 0; h < 2; ++h) {
+      uint32_t kw[2][4];
 #pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
-        const int h = 2 * half + h2;
-        uint32_t kw[2][4];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const uint4 v = *(const uint4*)(my.keys + (16 * h + 8 * x + r) * (TQ_D / 2) + c * 16);
-          kw[x][0] = v.x, kw[x][1] = v.y, kw[x][2] = v.z, kw[x][3] = v.w;
-        }
-        float sum[NT][4], low[NT][4];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum[t][i] = low[t][i] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint32_t ah[4], al[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {  // tokens r, r + 8; bytes 2 j, 2 j + 1
-            const uint32_t b = __byte_perm(kw[x & 1][j >> 1], 0, 0x4440 + 2 * (j & 1) + (x >> 1));
-            if (SPLIT) {
-              const uint2 v = ar_lut2(lutk + b * Sh::ENTRY);
-              ah[x] = v.x, al[x] = v.y;
-            } else {
-              ah[x] = ar_lut1(lutk + b * Sh::ENTRY);
-            }
-          }
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if (SPLIT) {
-              float d[4];
-              ar_mma(d, ah, bh[t][j][0], bh[t][j][1], zero);
-              ar_mma(low[t], al, bh[t][j][0], bh[t][j][1], low[t]);
-              ar_mma(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) sum[t][i] += d[i];
-            } else {
-              ar_mma(sum[t], ah, bh[t][j][0], bh[t][j][1], sum[t]);
-              ar_mma(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
-            }
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int n = 8 * t + 2 * c + (i & 1), tok = 16 * h2 + 8 * (i >> 1) + r;
-            float x = fmaf(sum[t][i] + low[t][i], inv[t][i & 1], bias[t][i & 1]);
-            if (g.outlier_k > 0) x += my.corr[tok][n ^ (4 * (tok >> 2 & 1))];
-            sc[h][t][i] = tq_scaled<true>(x);
-          }
+      for (int x = 0; x < 2; ++x) {
+        const uint4 v = *(const uint4*)(my.keys + (32 * half + 16 * h + 8 * x + r) * (TQ_D / 2) + c * 16);
+        kw[x][0] = v.x, kw[x][1] = v.y, kw[x][2] = v.z, kw[x][3] = v.w;
       }
+      float sum[NT][4], low[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[t][i] = low[t][i] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t ah[4], al[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {  // tokens r, r + 8; bytes 2 j, 2 j + 1
+          const uint32_t b = __byte_perm(kw[x & 1][j >> 1], 0, 0x4440 + 2 * (j & 1) + (x >> 1));
+          if (SPLIT) {
+            const uint2 v = ar_lut2(lutk + b * Sh::ENTRY);
+            ah[x] = v.x, al[x] = v.y;
+          } else {
+            ah[x] = ar_lut1(lutk + b * Sh::ENTRY);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (SPLIT) {
+            float d[4];
+            ar_mma(d, ah, bh[t][j][0], bh[t][j][1], zero);
+            ar_mma(low[t], al, bh[t][j][0], bh[t][j][1], low[t]);
+            ar_mma(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[t][i] += d[i];
+          } else {
+            ar_mma(sum[t], ah, bh[t][j][0], bh[t][j][1], sum[t]);
+            ar_mma(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = 8 * t + 2 * c + (i & 1), tok = 16 * h + 8 * (i >> 1) + r;
+          float x = fmaf(sum[t][i] + low[t][i], inv[t][i & 1], bias[t][i & 1]);
+          if (g.outlier_k > 0) x += my.corr[tok][n ^ (4 * (tok >> 2 & 1))];
+          sc[h][t][i] = tq_scaled<true>(x);
+        }
     }
   };
-  auto strip_values = [&](float (&sc)[4][NT][4], const float (&nv)[4][2], const float (&inv_n)[NT][2]) {
+  auto strip_values = [&](float (&sc)[2][NT][4], int half, const float (&nv)[2][2], const float (&inv_n)[NT][2]) {
     float f[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) f[t][0] = inv_n[t][0] * inv_v, f[t][1] = inv_n[t][1] * inv_v;
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
+    for (int h = 0; h < 2; ++h) {
       uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -746,7 +718,7 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
           ph[t][y] = ar_transpose(hi);
           if (SPLIT) pl[t][y] = ar_transpose(lo);
         }
-      const uint8_t* grp = my.values + h * VGB;
+      const uint8_t* grp = my.values + (2 * half + h) * VGB;
       uint32_t rec[9];
       if (VB == 4) {
         const uint4 x = *(const uint4*)(grp + lane * 16), y = *(const uint4*)(grp + 512 + lane * 16);
@@ -803,19 +775,16 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
     }
   };
 
-  // ---- a tile of the uncompressed window: 16 tokens
+  // ---- a tile of the uncompressed window: 32 tokens.  KIND: TQ_F16, TQ_BF16, TQ_F32.
   uint32_t b3[SPLIT ? NT : 1][SPLIT ? 8 : 1][2];  // third parts of the queries (bfloat16 windows)
-  // the raw queries as B operand, in natural order of channels: k-step j takes channels 16 j ..
+  // the queries as B operand, channels in the order of the weights
   auto hot_weights = [&]() {
     const bool bf = g.kv_dtype == TQ_BF16;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float mx = 0.0f, i0 = 1.0f, up = 1.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mx = fmaxf(mx, fabsf(q_at(q_row(16 * j + 2 * c + (k & 1) + 8 * (k >> 1)), 8 * t + r)));
+      for (int k = 0; k < 32; ++k) mx = fmaxf(mx, fabsf(q_at(q_row(32 * c + k), 8 * t + r)));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
       if (!bf) up = ar_lift(mx, 13, i0);
@@ -825,7 +794,7 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
       for (int j = 0; j < 8; ++j)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int d = 16 * j + 2 * c + 8 * k;
+          const int d = 32 * c + 4 * j + 2 * k;
           const float x = q_at(q_row(d), 8 * t + r), y = q_at(q_row(d + 1), 8 * t + r);
           if (bf) {
             uint32_t p[3] = {0u, 0u, 0u};
@@ -849,6 +818,7 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
         for (int x = 0; x < 2; ++x) {
           if (tok > pos[t][x] || (tok < win[t][x] && tok >= a.sinks)) continue;
           float dot = 0.0f;
+#pragma unroll 1
           for (int d = 0; d < TQ_D; ++d) dot = fmaf(q_at(q_row(d), 8 * t + 2 * c + x), attend_ld(a.hot_k, from + d, g.kv_dtype), dot);
           dot = tq_scaled<true>(dot);
           const float top = fmaxf(m_run[t][x], dot), by = top > -INFINITY ? top : 0.0f;
@@ -864,22 +834,21 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
         }
     }
   };
-  auto hot_fetch = [&](int t0, int n) {  // 16-bit rows: keys, then values
-    uint8_t* to = my.keys;
+  auto hot_attend = [&](int t0, int n, auto kind) {
+    constexpr int KIND = decltype(kind)::value;
+    constexpr bool BF = KIND == TQ_BF16, F32 = KIND == TQ_F32;
+    uint8_t* const rows = my.keys;
+    if (!F32) {  // values on their way
 #pragma unroll
-    for (int i = 0; i < 2 * AR_HOT * 16 / 32; ++i) {
-      const int row = (2 * i + (lane >> 4)) % AR_HOT, t = t0 + row;
-      const void* src = i < AR_HOT / 2 ? a.hot_k : a.hot_v;
-      ar_cp16_or_zero(to + (2 * i + (lane >> 4)) * AR_PITCH + (lane & 15) * 16,
-                      (const uint16_t*)src + hot_row(t) + (lane & 15) * 8, t < n);
+      for (int i = 0; i < AR_HOT / 2; ++i) {
+        const int row = 2 * i + (lane >> 4), t = t0 + row;
+        ar_cp16_or_zero(rows + row * AR_PITCH + (lane & 15) * 16, (const uint16_t*)a.hot_v + hot_row(t) + (lane & 15) * 8, t < n);
+      }
+      ar_commit();
     }
-  };
-  auto hot_attend = [&](int t0, int n) {
-    const bool bf = g.kv_dtype == TQ_BF16;
-    const uint8_t* rows = my.keys;
     float v_up = 1.0f, v_inv = 1.0f;
     bool odd = false;
-    if (hot32) {
+    if (F32) {
       float top = 0.0f, top_k = 0.0f;
 #pragma unroll 4
       for (int i = 0; i < AR_HOT; ++i) {
@@ -894,106 +863,135 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
 #pragma unroll
       for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       v_up = ar_lift(top, 13, v_inv);
-    } else {
-      const uint32_t ones = g.kv_dtype == TQ_F16 ? 0x7c007c00u : 0x7f807f80u;  // (an exponent of ones in either half)
+    }
+    float sc[2][NT][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // a lane's keys are channels 32 c .. + 31 of tokens r and r + 8
+      float sum[NT][4], low[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[t][i] = low[t][i] = 0.0f;
+      uint32_t kw[2][F32 ? 1 : 16];
+      const void* row[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int t = min(t0 + 16 * h + 8 * x + r, n - 1);  // (one past the end is hidden whatever its key)
+        row[x] = F32 ? (const void*)((const float*)a.hot_k + hot_row(t) + 32 * c) : (const void*)((const uint16_t*)a.hot_k + hot_row(t) + 32 * c);
+        if (!F32)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint4 v = ((const uint4*)row[x])[k];
+            kw[x][4 * k] = v.x, kw[x][4 * k + 1] = v.y, kw[x][4 * k + 2] = v.z, kw[x][4 * k + 3] = v.w;
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t ah[4], al[4] = {0u, 0u, 0u, 0u};
+        if (F32) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float4 v = ((const float4*)row[x])[j];
+            ar_split(v.x, 1.0f, v.y, 1.0f, ah[x], al[x]);
+            ar_split(v.z, 1.0f, v.w, 1.0f, ah[2 + x], al[2 + x]);
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) ah[x] = kw[x & 1][F32 ? 0 : 2 * j + (x >> 1)];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float d[4];
+          if (BF) {
+            ar_mma_bf(d, ah, bh[t][j][0], bh[t][j][1], zero);
+            if (SPLIT) {
+              ar_mma_bf(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
+              ar_mma_bf(low[t], ah, b3[t][j][0], b3[t][j][1], low[t]);
+            }
+          } else {
+            ar_mma(d, ah, bh[t][j][0], bh[t][j][1], zero);
+            if (SPLIT || F32) ar_mma(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
+            if (F32) ar_mma(low[t], al, bh[t][j][0], bh[t][j][1], low[t]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[t][i] += d[i];
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[h][t][i] = tq_scaled<true>((sum[t][i] + low[t][i]) * inv[t][i & 1]);
+    }
+    if (!F32) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      // an exponent of ones in either half of a word carries into the sign's place
+      constexpr uint32_t ONE = KIND == TQ_F16 ? 0x04000400u : 0x00800080u;
+      uint32_t carry = 0u;
 #pragma unroll
       for (int i = 0; i < AR_HOT / 2; ++i) {
-        const uint4 x = *(const uint4*)(rows + (AR_HOT + 2 * i + (lane >> 4)) * AR_PITCH + (lane & 15) * 16);
-        const uint32_t y[4] = {x.x & ones, x.y & ones, x.z & ones, x.w & ones};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) odd |= (y[k] & 0xffffu) == (ones & 0xffffu) || y[k] >> 16 == ones >> 16;
+        const uint4 x = *(const uint4*)(rows + (2 * i + (lane >> 4)) * AR_PITCH + (lane & 15) * 16);
+        carry |= ((x.x & 0x7fff7fffu) + ONE) | ((x.y & 0x7fff7fffu) + ONE) | ((x.z & 0x7fff7fffu) + ONE) | ((x.w & 0x7fff7fffu) + ONE);
       }
+      odd = (carry & 0x80008000u) != 0u;
     }
     if (__any_sync(0xffffffffu, odd)) {
       hot_terms(t0, n);
       return;
     }
-    // an element of a float32 row (past the last token: zero)
-    auto at32 = [&](const void* p, int t, int d) { return t < n ? ((const float*)p)[hot_row(t) + d] : 0.0f; };
-    float sc[1][NT][4], sum[NT][4], low[NT][4];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum[t][i] = low[t][i] = 0.0f;
-    const uint32_t k_at = ar_smem(rows) + (lane & 15) * AR_PITCH + (lane >> 4) * 16;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t ah[4], al[4] = {0u, 0u, 0u, 0u};
-      if (hot32) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int t = t0 + r + 8 * (x & 1), d = 16 * j + 2 * c + 8 * (x >> 1);
-          ar_split(at32(a.hot_k, t, d), 1.0f, at32(a.hot_k, t, d + 1), 1.0f, ah[x], al[x]);
-        }
-      } else {
-        ar_ldm<false>(ah, k_at + 32 * j);
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float d[4];
-        if (bf) {
-          ar_mma_bf(d, ah, bh[t][j][0], bh[t][j][1], zero);
-          if (SPLIT) {
-            ar_mma_bf(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
-            ar_mma_bf(low[t], ah, b3[t][j][0], b3[t][j][1], low[t]);
-          }
-        } else {
-          ar_mma(d, ah, bh[t][j][0], bh[t][j][1], zero);
-          if (SPLIT || hot32) ar_mma(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
-          if (hot32) ar_mma(low[t], al, bh[t][j][0], bh[t][j][1], low[t]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[t][i] += d[i];
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sc[0][t][i] = tq_scaled<true>((sum[t][i] + low[t][i]) * inv[t][i & 1]);
     float inv_n[NT][2];
-    const float nv[1][2] = {{1.0f, 1.0f}};
-    softmax(sc, t0, n, ArTiles<1>(), nv, inv_n);
-    uint32_t p[NT][2][3] = {};
+    const float nv[2][2] = {{1.0f, 1.0f}, {1.0f, 1.0f}};
+    softmax(sc, t0, n, ArTiles<2>(), nv, inv_n);
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int t = 0; t < NT; ++t) inv_n[t][0] *= v_inv, inv_n[t][1] *= v_inv;
+    auto at32 = [&](int t, int d) { return t < n ? ((const float*)a.hot_v)[hot_row(t) + d] : 0.0f; };
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        if (bf) ar_split_bf<SPLIT ? 3 : 2>(sc[0][t][2 * y], sc[0][t][2 * y + 1], p[t][y]);
-        else ar_split(sc[0][t][2 * y], 1.0f, sc[0][t][2 * y + 1], 1.0f, p[t][y][0], p[t][y][1]);
+    for (int h = 0; h < 2; ++h) {
+      uint32_t p[NT][2][3] = {};
 #pragma unroll
-        for (int k = 0; k < (SPLIT ? 3 : 2); ++k) p[t][y][k] = ar_transpose(p[t][y][k]);
-      }
-    const uint32_t v_at = ar_smem(rows) + (AR_HOT + (lane & 7) + (lane >> 4) * 8) * AR_PITCH + (lane >> 3 & 1) * 16;
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int mt = 0; mt < 8; ++mt) {
-      uint32_t ah[4], al[4] = {0u, 0u, 0u, 0u};
-      if (hot32) {
+        for (int y = 0; y < 2; ++y) {
+          if (BF) ar_split_bf<SPLIT ? 3 : 2>(sc[h][t][2 * y], sc[h][t][2 * y + 1], p[t][y]);
+          else ar_split(sc[h][t][2 * y], 1.0f, sc[h][t][2 * y + 1], 1.0f, p[t][y][0], p[t][y][1]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {  // channels r, r + 8; tokens 2 c, 2 c + 1, and 8 further
-          const int t = t0 + 2 * c + 8 * (x >> 1), d = 16 * mt + r + 8 * (x & 1);
-          ar_split(at32(a.hot_v, t, d), v_up, at32(a.hot_v, t + 1, d), v_up, ah[x], al[x]);
+          for (int k = 0; k < (BF && SPLIT ? 3 : 2); ++k) p[t][y][k] = ar_transpose(p[t][y][k]);
         }
-      } else {
-        ar_ldm<true>(ah, v_at + 32 * mt);
-      }
+      const uint32_t v_at = ar_smem(rows) + (16 * h + (lane & 7) + (lane >> 4) * 8) * AR_PITCH + (lane >> 3 & 1) * 16;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float d[4];
-        if (bf) {
-          if (SPLIT) {
-            ar_mma_bf(d, ah, p[t][0][2], p[t][1][2], zero);
-            ar_mma_bf(d, ah, p[t][0][1], p[t][1][1], d);
-          } else {
-            ar_mma_bf(d, ah, p[t][0][1], p[t][1][1], zero);
+      for (int mt = 0; mt < 8; ++mt) {
+        uint32_t ah[4], al[4] = {0u, 0u, 0u, 0u};
+        if (F32) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {  // channels r, r + 8; tokens 2 c, 2 c + 1, and 8 further
+            const int t = t0 + 16 * h + 2 * c + 8 * (x >> 1), d = 16 * mt + r + 8 * (x & 1);
+            ar_split(at32(t, d), v_up, at32(t + 1, d), v_up, ah[x], al[x]);
           }
-          ar_mma_bf(d, ah, p[t][0][0], p[t][1][0], d);
         } else {
-          ar_mma(d, ah, p[t][0][1], p[t][1][1], zero);
-          if (hot32) ar_mma(d, al, p[t][0][0], p[t][1][0], d);
-          ar_mma(d, ah, p[t][0][0], p[t][1][0], d);
+          ar_ldm<true>(ah, v_at + 32 * mt);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][mt][i] = fmaf(d[i], inv_n[t][i & 1] * v_inv, acc[t][mt][i]);
+        for (int t = 0; t < NT; ++t) {
+          float d[4];
+          if (BF) {
+            if (SPLIT) {
+              ar_mma_bf(d, ah, p[t][0][2], p[t][1][2], zero);
+              ar_mma_bf(d, ah, p[t][0][1], p[t][1][1], d);
+            } else {
+              ar_mma_bf(d, ah, p[t][0][1], p[t][1][1], zero);
+            }
+            ar_mma_bf(d, ah, p[t][0][0], p[t][1][0], d);
+          } else if (SPLIT || F32) {
+            ar_mma(d, ah, p[t][0][1], p[t][1][1], zero);
+            if (F32) ar_mma(d, al, p[t][0][0], p[t][1][0], d);
+            ar_mma(d, ah, p[t][0][0], p[t][1][0], d);
+          } else {
+            ar_mma(d, ah, p[t][0][0], p[t][1][0], zero);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][mt][i] = fmaf(d[i], inv_n[t][i & 1], acc[t][mt][i]);
+        }
       }
     }
   };
@@ -1020,19 +1018,56 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
   };
 
   // ---- the share, item by item
-  bool more = true;
+  int strip = 0, ts = 0;  // a strip of the row, its first token in its page
+  auto open_strips = [&]() {
+    strip = w.strip.at(it), ts = (strip & 3) * AR_STRIP;
+    page = page_of(it);
+    open_list(it, ts);
+    copy_keys(page, ts, list_at);
+    ar_commit();
+    copy_values(page, ts);
+    ar_commit();
+  };
+  if (more) {  // (on their way while the tables are made)
+    fetch_row();
+    if (it < row_strips) open_strips();
+  }
+  {  // tables of pairs
+    float max_k = 0.0f, max_v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      max_k = fmaxf(max_k, fabsf(sh.grid[i]));
+      max_v = fmaxf(max_v, fabsf(sh.cent[i]));
+    }
+    const float up_k = ar_lift(max_k, 7, inv_k), up_v = ar_lift(max_v, 7, inv_v);
+    for (int e = tid; e < 256 + Sh::NV; e += THREADS) {
+      uint32_t hi, lo;
+      uint4* to;
+      if (e < 256) {
+        ar_split(sh.grid[e & 15], up_k, sh.grid[e >> 4], up_k, hi, lo);
+        to = (uint4*)(sh.lut + e * Sh::ENTRY);
+      } else {
+        const int b = e - 256;
+        ar_split(sh.cent[b & ((1 << VB) - 1)], up_v, sh.cent[b >> VB], up_v, hi, lo);
+        to = (uint4*)(sh.lut + Sh::LUTK + b * Sh::ENTRY);
+      }
+#pragma unroll
+      for (int i = 0; i < Sh::ENTRY / 16; ++i)
+        to[(i + lane) % (Sh::ENTRY / 16)] = SPLIT ? make_uint4(hi, lo, hi, lo) : make_uint4(hi, hi, hi, hi);
+    }
+  }
+  __syncthreads();  // (the last one)
+  bool opened = true;
   while (more) {
     // a row tile's strips, then its tiles of the window, as far as the share goes
+    if (!opened) {
+      fetch_row();
+      if (it < row_strips) open_strips();
+    }
+    opened = false;
     start_row();
     if (it < row_strips) {
       reset();
-      int strip = w.strip.at(it), ts = (strip & 3) * AR_STRIP;
-      page = page_of(it);
-      open_list(it, ts);
-      copy_keys(page, ts, list_at);
-      ar_commit();
-      copy_values(page, ts);
-      ar_commit();
       bool new_page = true;
       for (;;) {
         at += AR_COST;
@@ -1041,43 +1076,49 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
         const int next = last ? strip : w.strip.at(i1);
         asm volatile("cp.async.wait_group 1;" ::: "memory");  // the key half has landed
         __syncwarp();
-        const int t0 = strip * AR_STRIP;
-        const bool seen = !open_to_none(t0, t0 + AR_STRIP);
-        float sc[4][NT][4];
         if (new_page) weights();
-        if (seen) strip_scores(sc, ts);
-        else if (SPLIT) list_next = 0xffffffffu;
-        __syncwarp();  // the key half has been read
-        const bool turn = next >> 2 != strip >> 2;  // the next strip is of another page
-        if (!last) {
-          if (turn) {
-            page = page_of(i1);
-            open_list(i1, (next & 3) * AR_STRIP);
-          } else if (SPLIT) {
-            if (next == strip + 1 && list_next != 0xffffffffu) list_at = list_next;
-            else open_list(i1, (next & 3) * AR_STRIP);
+        if (SPLIT) list_next = 0xffffffffu;
+        // (32 tokens at a time: a loop of 64 did not fit the instruction caches)
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          const int t0 = strip * AR_STRIP + 32 * half;
+          const bool seen = !open_to_none(t0, t0 + 32);
+          float sc[2][NT][4];
+          if (seen || (SPLIT && half == 0)) strip_scores(sc, half, ts);  // (SPLIT: the second half's list begins where the first's ends)
+          if (half == 1) {
+            __syncwarp();  // the key half has been read
+            if (!last) {
+              const int nt = (next & 3) * AR_STRIP;
+              const bool turn = next >> 2 != strip >> 2;  // another page
+              const bool follows = !turn && next == strip + 1 && list_next != 0xffffffffu && seen;
+              if (turn) page = page_of(i1);
+              if (follows) list_at = list_next;
+              else open_list(i1, nt);
+              copy_keys(page, nt, list_at);
+            }
+            ar_commit();
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+          } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");  // the value half has landed
           }
-          copy_keys(page, (next & 3) * AR_STRIP, list_at);
-        }
-        ar_commit();
-        asm volatile("cp.async.wait_group 1;" ::: "memory");  // the value half has landed
-        __syncwarp();
-        if (seen) {
-          float nv[4][2], inv_n[NT][2];
+          __syncwarp();
+          if (seen) {
+            float nv[2][2], inv_n[NT][2];
 #pragma unroll
-          for (int h = 0; h < 4; ++h)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int y = 0; y < 2; ++y) nv[h][y] = my.norms[16 * h + 8 * y + r];
-          softmax(sc, t0, w.cold, ArTiles<4>(), nv, inv_n);
-          strip_values(sc, nv, inv_n);
+              for (int y = 0; y < 2; ++y) nv[h][y] = my.norms[32 * half + 16 * h + 8 * y + r];
+            softmax(sc, t0, w.cold, ArTiles<2>(), nv, inv_n);
+            strip_values(sc, half, nv, inv_n);
+          }
         }
         __syncwarp();  // the value half has been read
         if (!last) copy_values(page, (next & 3) * AR_STRIP);
         ar_commit();
         it = i1;
         if (last) break;
+        new_page = next >> 2 != strip >> 2;
         strip = next, ts = (next & 3) * AR_STRIP;
-        new_page = turn;
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
@@ -1088,16 +1129,13 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
       reset();
       hot_weights();
       const int n = sh.seq[s].x;
+#pragma unroll 1
       for (; it < row_items && at < stop; ++it, ++at) {
         const int t0 = w.cold + w.hot.at(it - row_strips) * AR_HOT;
         if (open_to_none(t0, min(t0 + AR_HOT, n))) continue;
-        if (!hot32) {
-          hot_fetch(t0, n);
-          ar_commit();
-          asm volatile("cp.async.wait_all;" ::: "memory");
-          __syncwarp();
-        }
-        hot_attend(t0, n);
+        if (g.kv_dtype == TQ_BF16) hot_attend(t0, n, ArTiles<TQ_BF16>());
+        else if (g.kv_dtype == TQ_F16) hot_attend(t0, n, ArTiles<TQ_F16>());
+        else hot_attend(t0, n, ArTiles<TQ_F32>());
         __syncwarp();  // the rows have been read
       }
       flush(true);
