@@ -295,49 +295,49 @@ class KVContext:
         ``[n_seqs', T, n_q_heads, D]`` of ``q``'s type; rows that see nothing (padding, queries
         before the first token, empty sequences) are zeros.  Inference only: no gradients.
         """
+        # (a decode step's call is some microseconds on the GPU: the checks are kept short)
         torch = _torch()
-        g = self.geom
-        if q.dim() != 4 or tuple(q.shape[2:]) != (g.n_q_heads, g.head_dim):
+        g, dev, codes = self.geom, self.device, _dtype_codes()
+        shape, dtype = q.shape, q.dtype
+        if len(shape) != 4 or shape[2] != g.n_q_heads or shape[3] != g.head_dim:
             raise ValueError(f"expected q of shape [n_seqs, T, {g.n_q_heads}, {g.head_dim}], "
-                             f"got {tuple(q.shape)}")
-        if q.device != self.device:
-            raise ValueError(f"q lives on {q.device}, the context on {self.device}")
-        if q.dtype not in _dtype_codes():
-            raise ValueError(f"q must be float32, float16 or bfloat16, got {q.dtype}")
+                             f"got {tuple(shape)}")
+        if q.device != dev:
+            raise ValueError(f"q lives on {q.device}, the context on {dev}")
+        if dtype not in codes:
+            raise ValueError(f"q must be float32, float16 or bfloat16, got {dtype}")
         if q.requires_grad and torch.is_grad_enabled():
             raise ValueError("attention on the codes has no backward pass: call it under torch.no_grad()")
         if window is not None and window < 1:
             raise ValueError(f"window must be at least 1 (or None), got {window}")
         if sinks < 0:
             raise ValueError(f"sinks must not be negative, got {sinks}")
-        if q_lens is not None and (q_lens.dtype != torch.int32 or q_lens.device != self.device
-                                   or tuple(q_lens.shape) != (q.shape[0],)):
-            raise ValueError(f"q_lens must be an int32 tensor of shape ({q.shape[0]},) on {self.device}")
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device \
-                or not out.is_contiguous() or out.data_ptr() % 16:
-            raise ValueError(f"out must be a contiguous {q.dtype} tensor of shape {tuple(q.shape)} "
-                             f"on {self.device}, aligned to 16 bytes")
-        step = 16 // q.element_size()
-        if q.numel() and (q.stride(3) != 1 or q.data_ptr() % 16 or any(s % step for s in q.stride()[:3])):
-            q = q.contiguous() if not q.is_contiguous() else q.clone()
+        lens = None
         if q_lens is not None:
+            if q_lens.dtype != torch.int32 or q_lens.device != dev or q_lens.shape != (shape[0],):
+                raise ValueError(f"q_lens must be an int32 tensor of shape ({shape[0]},) on {dev}")
             q_lens = q_lens.contiguous()
-        a = TqAttendArgs()
-        a.q, a.out = q.data_ptr(), out.data_ptr()
-        a.q_lens = q_lens.data_ptr() if q_lens is not None else None
-        a.q_seq_stride, a.q_tok_stride, a.q_head_stride = q.stride()[:3]
-        a.layer, a.seq_begin, a.seq_count, a.n_tokens = layer, seq_begin, q.shape[0], q.shape[1]
-        a.q_dtype = _dtype_code(q.dtype)
-        a.window, a.sinks = min(window or 0, 2**31 - 1), min(sinks, 2**31 - 1)
+            lens = q_lens.data_ptr()
+        if out is None:
+            out = torch.empty(shape, dtype=dtype, device=dev)
+        elif out.shape != shape or out.dtype != dtype or out.device != dev or not out.is_contiguous() \
+                or out.data_ptr() % 16:
+            raise ValueError(f"out must be a contiguous {dtype} tensor of shape {tuple(shape)} "
+                             f"on {dev}, aligned to 16 bytes")
+        step = 16 // q.element_size()
+        s0, s1, s2, s3 = q.stride()
+        if (s3 != 1 or q.data_ptr() % 16 or s0 % step or s1 % step or s2 % step) and q.numel():
+            q = q.clone() if q.is_contiguous() else q.contiguous()
+            s0, s1, s2, s3 = q.stride()
+        a = TqAttendArgs(q.data_ptr(), out.data_ptr(), lens, None, 0, s0, s1, s2, layer, seq_begin,
+                         shape[0], shape[1], codes[dtype], min(window or 0, 2**31 - 1),
+                         min(sinks, 2**31 - 1))
         with self._here():
-            stream = self._stream()
-            size = C.c_size_t()
-            check(self._lib.tq_attend_workspace(self._h, C.byref(a), stream, C.byref(size)))
-            work = torch.empty(size.value, dtype=torch.uint8, device=self.device)
+            stream, ref, size = self._stream(), C.byref(a), C.c_size_t()
+            check(self._lib.tq_attend_workspace(self._h, ref, stream, C.byref(size)))
+            work = torch.empty(size.value, dtype=torch.uint8, device=dev)
             a.workspace, a.workspace_bytes = work.data_ptr(), size.value
-            check(self._lib.tq_attend(self._h, C.byref(a), stream))
+            check(self._lib.tq_attend(self._h, ref, stream))
         return out
 
     def norm_rope(self, layer: int, q, k, inv_freq, positions=None, *, q_weight=None, k_weight=None,

@@ -17,7 +17,7 @@ struct Plan {
   size_t fixed_bytes, seq_bytes;  // workspace: of a launch, of a sequence
 };
 
-int check_args(const tq_ctx* ctx, const tq_attend_args* r) {
+int check_args(tq_ctx* ctx, const tq_attend_args* r) {
   TQ_REQUIRE(ctx != nullptr && r != nullptr, TQ_ERR_INVALID, "null argument");
   const tq_geom& g = ctx->g;
   TQ_REQUIRE(r->layer >= 0 && r->layer < g.n_layers, TQ_ERR_INVALID, "bad layer");
@@ -32,6 +32,8 @@ int check_args(const tq_ctx* ctx, const tq_attend_args* r) {
   TQ_REQUIRE(r->q_seq_stride % step == 0 && r->q_tok_stride % step == 0 && r->q_head_stride % step == 0 &&
                  (uintptr_t)r->q % 16 == 0 && (uintptr_t)r->out % 16 == 0,
              TQ_ERR_INVALID, "q, its strides and out must be aligned to 16 bytes");
+  if (ctx->sm_count == 0)
+    TQ_CUDA(cudaDeviceGetAttribute(&ctx->sm_count, cudaDevAttrMultiProcessorCount, ctx->device));
   return TQ_OK;
 }
 
@@ -58,8 +60,7 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
   const bool channels = g.key_mode != TQ_KEYS_POLAR && !ctx->force_generic;
   p.form = rows > 64 && channels && r->q_dtype != TQ_F32 ? TILES
            : rows <= 64 && channels && g.block_tokens == 256 ? ROWS : GENERAL;
-  int sm_count = 148;
-  cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, ctx->device);
+  const int sm_count = ctx->sm_count;
   if (p.form == TILES) {
     const int64_t all = std::max<int64_t>((n + 127) / 128, 1);
     auto seen = [&](int64_t tokens) {  // tiles that so many neighbouring query tokens see
@@ -90,7 +91,8 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
     a.window = r->window == 0 ? INT_MAX : r->window;
     a.sinks = r->sinks;
     a.q_dtype = r->q_dtype;
-    const AttendRowsPlan rp = tq_attend_rows_plan(a, n, sm_count);
+    a.sm_count = sm_count;
+    const AttendRowsPlan rp = tq_attend_rows_plan(a, n);
     p.ns_cold = rp.ns_cold, p.ns_hot = rp.ns_hot;
     p.seqs = rp.seqs;
     p.fixed_bytes = rp.plan_bytes;
@@ -143,8 +145,6 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
              "workspace smaller than tq_attend_workspace asked for");
   const int at_once =
       (int)std::min({(r->workspace_bytes - p.fixed_bytes) / p.seq_bytes, (size_t)r->seq_count, (size_t)p.seqs});
-  int sm_count = 148;
-  cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, ctx->device);
 
   AttendArgs a = {};
   a.g = g;
@@ -167,6 +167,7 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
   a.sinks = r->sinks;
   a.ns_cold = p.ns_cold, a.ns_hot = p.ns_hot;
   a.rows = r->n_tokens * g.group;
+  a.device = ctx->device, a.sm_count = ctx->sm_count;
   a.unit_stride = (int64_t)a.rows * (p.ns_cold + p.ns_hot) * TQ_PART_STRIDE;
   const size_t esz = elem_size(r->q_dtype);
   ctx->last_launches = 0;
@@ -177,13 +178,13 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
     a.out = (uint8_t*)r->out + (size_t)s * r->n_tokens * g.n_q_heads * TQ_D * esz;
     a.q_lens = r->q_lens == nullptr ? nullptr : r->q_lens + s;
     if (p.form == TILES) {
-      rc = tq_launch_attend_tiles(a, r->workspace, p.cap, p.splits, ctx->device, st);
+      rc = tq_launch_attend_tiles(a, r->workspace, p.cap, p.splits, st);
       if (rc != TQ_OK) return rc;
       ctx->last_launches += 4;
       continue;
     }
     if (p.form == ROWS) {
-      rc = tq_launch_attend_rows(a, sm_count, st);
+      rc = tq_launch_attend_rows(a, st);
       if (rc != TQ_OK) return rc;
       ctx->last_launches += 2;
       continue;

@@ -40,6 +40,7 @@ struct AttendArgs {
   int32_t window, sinks;  // window: INT_MAX without one
   int32_t ns_cold, ns_hot;
   int32_t rows;  // of a unit: n_tokens * group
+  int32_t device, sm_count;
 };
 
 // What a sequence holds and where its queries stand.
@@ -94,6 +95,15 @@ TQ_DEV float attend_ld(const void* p, size_t i, int dt) {
   return __bfloat162float(((const __nv_bfloat16*)p)[i]);
 }
 
+// Sets a kernel's dynamic shared memory once per device (again by a second thread at worst).
+template <class K>
+int attend_shared(K kernel, size_t bytes, int device, bool (&done)[64]) {
+  if (device >= 0 && device < 64 && done[device]) return TQ_OK;
+  TQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  if (device >= 0 && device < 64) done[device] = true;
+  return TQ_OK;
+}
+
 int tq_launch_attend_general(const AttendArgs& a, cudaStream_t st);
 int tq_launch_attend_combine(const AttendArgs& a, cudaStream_t st);
 // Few rows, 256-token blocks of per-channel keys, queries on 16-byte boundaries; the merge too.
@@ -102,9 +112,8 @@ struct AttendRowsPlan {
   int seqs;             // most sequences of a launch
   size_t plan_bytes;    // at a.plan
 };
-AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens, int sm_count);
-int tq_launch_attend_rows(const AttendArgs& a, int sm_count, cudaStream_t st);
+AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens);
+int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st);
 // 16-bit queries, per-channel keys: everything in one, the merge too; `cap` tiles of 128 tokens per unit have room
 size_t tq_attend_tiles_bytes(const AttendArgs& a, int units, int cap, int splits);
-int tq_launch_attend_tiles(const AttendArgs& a, void* workspace, int cap, int splits, int device,
-                           cudaStream_t st);
+int tq_launch_attend_tiles(const AttendArgs& a, void* workspace, int cap, int splits, cudaStream_t st);

@@ -371,8 +371,9 @@ int launch_general(const AttendArgs& a, cudaStream_t st) {
   const int row_tiles = (a.rows + 16 * RPT - 1) / (16 * RPT);
   const int64_t grid = (int64_t)a.seq_count * a.g.n_kv_heads * row_tiles * (a.ns_cold + a.ns_hot);
   TQ_REQUIRE(grid <= INT_MAX, TQ_ERR_UNSUPPORTED, "too many (sequence, head, query row) tiles in a call");
-  TQ_CUDA(cudaFuncSetAttribute(attend_general_kernel<RPT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)sizeof(AgShared<RPT>)));
+  static bool done[64];
+  const int rc = attend_shared(attend_general_kernel<RPT>, sizeof(AgShared<RPT>), a.device, done);
+  if (rc != TQ_OK) return rc;
   attend_general_kernel<RPT><<<(int)grid, AG_THREADS, sizeof(AgShared<RPT>), st>>>(a, row_tiles);
   TQ_CUDA(cudaGetLastError());
   return TQ_OK;

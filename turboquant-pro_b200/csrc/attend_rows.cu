@@ -40,7 +40,7 @@ namespace {
 constexpr int AR_S = 256;          // tokens of a page
 constexpr int AR_STRIP = 64;       // of them, in an item of the list
 constexpr int AR_HOT = 32;         // window tokens of an item
-constexpr int AR_PITCH = TQ_D * 2 + 16;  // bytes of a window row in shared memory
+constexpr int AR_PITCH = TQ_D * 2 + 16, AR_PITCH32 = TQ_D * 4 + 16;  // bytes of a window row in shared memory
 constexpr int AR_COST = 2;         // a strip takes the time of so many tiles of the window
 constexpr int AR_SEQS = 64;        // sequences of a launch
 constexpr int AR_LIST = 256;       // outliers of a strip that are copied ahead (160 is usual)
@@ -71,7 +71,7 @@ struct alignas(16) ArWarp {
   float corr[32][8 * NT];           // outliers' part of the scores of 32 tokens
   uint8_t q[TQ_D][8 * NT * (SPLIT ? 4 : 2)];  // row q_row(d): channel d
 };
-static_assert(AR_HOT * AR_PITCH <= 6528 + 64 * TQ_D * 3 / 8 + 256, "a tile of the window in a strip's place");
+static_assert(AR_HOT * AR_PITCH <= 6528 + 64 * TQ_D * 3 / 8 + 256 && 16 * AR_PITCH32 <= 6528 + 64 * TQ_D * 3 / 8 + 256, "a tile of the window in a strip's place");
 
 template <int NT, bool SPLIT, int VB>
 struct ArShared {
@@ -198,6 +198,7 @@ TQ_DEV int ar_tiles(const AttendArgs& a, int q_n, int n) { return (q_n * a.g.gro
 struct ArPlan {
   int64_t share;
   int64_t cum[AR_SEQS + 1];
+  int4 seq[AR_SEQS];  // strips, window tiles and row tiles of a sequence
 };
 
 template <int NT, bool SPLIT, int VB>
@@ -267,6 +268,10 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
     ArPlan* plan = (ArPlan*)a.plan;
     if (tid == 0) plan->share = share;
     for (int i = tid; i <= AR_SEQS; i += THREADS) plan->cum[i] = sh.cum[i];
+    for (int i = tid; i < a.seq_count; i += THREADS) {
+      const ArWork w = ar_work(a, sh.seq[i].x, sh.seq[i].y);
+      plan->seq[i] = make_int4(w.strip.count(), w.hot.count(), ar_tiles(a, sh.seq[i].y, N), 0);
+    }
   }
   // (neighbouring shares go to different SMs: where there are few, each has one to itself)
   const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;
@@ -807,11 +812,16 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
         }
     }
   };
-  auto hot_row = [&](int t) { return (uix * (size_t)g.hot_cap + (size_t)(t % g.hot_cap)) * TQ_D; };  // elements
+  size_t ring = 0;   // elements before the row of slot 0
+  int slot0 = 0;     // slot of the tile's first token
+  auto hot_row = [&](int i) {  // elements before the row of the tile's token i
+    const int k = slot0 + i;
+    return ring + (size_t)((k >= g.hot_cap ? k - g.hot_cap : k) * TQ_D);
+  };
   auto hot_terms = [&](int t0, int n) {  // term by term
 #pragma unroll 1
     for (int tok = t0; tok < min(t0 + AR_HOT, n); ++tok) {
-      const size_t from = hot_row(tok);
+      const size_t from = hot_row(tok - t0);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -838,23 +848,28 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
     constexpr int KIND = decltype(kind)::value;
     constexpr bool BF = KIND == TQ_BF16, F32 = KIND == TQ_F32;
     uint8_t* const rows = my.keys;
-    if (!F32) {  // values on their way
+    // values on their way: all 32 tokens, or the first 16 of float32
+    auto fetch_values = [&](int h) {
 #pragma unroll
-      for (int i = 0; i < AR_HOT / 2; ++i) {
-        const int row = 2 * i + (lane >> 4), t = t0 + row;
-        ar_cp16_or_zero(rows + row * AR_PITCH + (lane & 15) * 16, (const uint16_t*)a.hot_v + hot_row(t) + (lane & 15) * 8, t < n);
+      for (int i = 0; i < 16; ++i) {
+        const int row = F32 ? 16 * h + i : 2 * i + (lane >> 4);
+        if (F32)
+          ar_cp16_or_zero(rows + i * AR_PITCH32 + lane * 16, (const float*)a.hot_v + hot_row(row) + lane * 4, t0 + row < n);
+        else
+          ar_cp16_or_zero(rows + row * AR_PITCH + (lane & 15) * 16, (const uint16_t*)a.hot_v + hot_row(row) + (lane & 15) * 8,
+                          t0 + row < n);
       }
       ar_commit();
-    }
+    };
+    fetch_values(0);
     float v_up = 1.0f, v_inv = 1.0f;
     bool odd = false;
     if (F32) {
       float top = 0.0f, top_k = 0.0f;
 #pragma unroll 4
-      for (int i = 0; i < AR_HOT; ++i) {
-        if (t0 + i >= n) break;
-        const float4 x = *(const float4*)((const float*)a.hot_k + hot_row(t0 + i) + 4 * lane);
-        const float4 y = *(const float4*)((const float*)a.hot_v + hot_row(t0 + i) + 4 * lane);
+      for (int i = 0; i < min(AR_HOT, n - t0); ++i) {
+        const float4 x = *(const float4*)((const float*)a.hot_k + hot_row(i) + 4 * lane);
+        const float4 y = *(const float4*)((const float*)a.hot_v + hot_row(i) + 4 * lane);
         top_k = fmaxf(top_k, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
         top = fmaxf(top, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
         odd |= !(fabsf(x.x) + fabsf(x.y) + fabsf(x.z) + fabsf(x.w) + fabsf(y.x) + fabsf(y.y) + fabsf(y.z) + fabsf(y.w) < INFINITY);
@@ -877,8 +892,8 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
       const void* row[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int t = min(t0 + 16 * h + 8 * x + r, n - 1);  // (one past the end is hidden whatever its key)
-        row[x] = F32 ? (const void*)((const float*)a.hot_k + hot_row(t) + 32 * c) : (const void*)((const uint16_t*)a.hot_k + hot_row(t) + 32 * c);
+        const size_t from = hot_row(min(16 * h + 8 * x + r, n - 1 - t0)) + 32 * c;  // (past the end: hidden whatever its key)
+        row[x] = F32 ? (const void*)((const float*)a.hot_k + from) : (const void*)((const uint16_t*)a.hot_k + from);
         if (!F32)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -937,6 +952,7 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
       odd = (carry & 0x80008000u) != 0u;
     }
     if (__any_sync(0xffffffffu, odd)) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
       hot_terms(t0, n);
       return;
     }
@@ -945,9 +961,16 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
     softmax(sc, t0, n, ArTiles<2>(), nv, inv_n);
 #pragma unroll
     for (int t = 0; t < NT; ++t) inv_n[t][0] *= v_inv, inv_n[t][1] *= v_inv;
-    auto at32 = [&](int t, int d) { return t < n ? ((const float*)a.hot_v)[hot_row(t) + d] : 0.0f; };
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      if (F32) {
+        if (h == 1) {
+          __syncwarp();  // (the first 16 have been read)
+          fetch_values(1);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+      }
       uint32_t p[NT][2][3] = {};
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -965,8 +988,8 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
         if (F32) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {  // channels r, r + 8; tokens 2 c, 2 c + 1, and 8 further
-            const int t = t0 + 16 * h + 2 * c + 8 * (x >> 1), d = 16 * mt + r + 8 * (x & 1);
-            ar_split(at32(t, d), v_up, at32(t + 1, d), v_up, ah[x], al[x]);
+            const float* f = (const float*)(rows + (2 * c + 8 * (x >> 1)) * AR_PITCH32) + 16 * mt + r + 8 * (x & 1);
+            ar_split(f[0], v_up, f[AR_PITCH32 / 4], v_up, ah[x], al[x]);
           }
         } else {
           ar_ldm<true>(ah, v_at + 32 * mt);
@@ -1129,9 +1152,11 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
       reset();
       hot_weights();
       const int n = sh.seq[s].x;
+      ring = uix * (size_t)g.hot_cap * TQ_D;
 #pragma unroll 1
       for (; it < row_items && at < stop; ++it, ++at) {
         const int t0 = w.cold + w.hot.at(it - row_strips) * AR_HOT;
+        slot0 = t0 % g.hot_cap;
         if (open_to_none(t0, min(t0 + AR_HOT, n))) continue;
         if (g.kv_dtype == TQ_BF16) hot_attend(t0, n, ArTiles<TQ_BF16>());
         else if (g.kv_dtype == TQ_F16) hot_attend(t0, n, ArTiles<TQ_F16>());
@@ -1154,8 +1179,8 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
 constexpr int AC_THREADS = 512;
 
 template <int ROWS>
-__global__ void __launch_bounds__(AC_THREADS) attend_rows_combine_kernel(AttendArgs a, int tile, int total) {
-  __shared__ __align__(16) float cs[TQ_D][4], ys[4][ROWS][TQ_D], hs[4][TQ_D], ls[4][TQ_D];
+__global__ void __launch_bounds__(AC_THREADS, 2) attend_rows_combine_kernel(AttendArgs a, int tile, int total) {
+  __shared__ __align__(16) float cs[TQ_D][4], ys[4][ROWS][TQ_D], hs[4][TQ_D], ls[4][TQ_D], ms[4];
   const tq_geom& g = a.g;
   const int tid = threadIdx.x, e = tid % TQ_D, h = tid / TQ_D;
   const int H = g.n_kv_heads, G = g.group;
@@ -1173,30 +1198,48 @@ __global__ void __launch_bounds__(AC_THREADS) attend_rows_combine_kernel(AttendA
       row = at % a.rows;
       const int unit = at / a.rows;
       s = unit / H, head = unit - s * H;
-      const AttendSeq sq = attend_seq(a, s);
-      const int tiles = ar_tiles(a, sq.q_n, tile);
-      if (row / tile < tiles) {
-        const ArWork w = ar_work(a, sq.n, sq.q_n);
-        const int64_t begin = plan->cum[s] + (int64_t)(head * tiles + row / tile) * w.cost();
-        const int strips = w.strip.count(), hots = w.hot.count();
-        const int64_t middle = begin + AR_COST * strips;
-        const int nc = strips > 0 ? (int)(ar_div(middle - AR_COST, share) - ar_div(begin, share)) + 1 : 0;
-        const int nh = hots > 0 ? (int)(ar_div(middle + hots - 1, share) - ar_div(middle, share)) + 1 : 0;
+      const int4 seq = plan->seq[s];
+      const int64_t before = plan->cum[s];
+      if (row / tile < seq.z) {
+        const int64_t begin = before + (int64_t)(head * seq.z + row / tile) * (AR_COST * seq.x + seq.y);
+        const int64_t middle = begin + AR_COST * seq.x;
+        const int nc = seq.x > 0 ? (int)(ar_div(middle - AR_COST, share) - ar_div(begin, share)) + 1 : 0;
+        const int nh = seq.y > 0 ? (int)(ar_div(middle + seq.y - 1, share) - ar_div(middle, share)) + 1 : 0;
         const float* base = attend_partial(a, unit, row, 0);
-        auto slot = [&](int i) { return base + (size_t)(i < nc ? i : a.ns_cold + i - nc) * TQ_PART_STRIDE; };
         float M = -INFINITY;
-#pragma unroll 8
-        for (int i = 0; i < nc + nh; ++i) M = fmaxf(M, slot(i)[0]);
-        const float by = M > -INFINITY ? M : 0.0f;
-#pragma unroll 8
-        for (int i = ROWS == 4 ? 0 : h; i < nc + nh; i += ROWS == 4 ? 1 : 4) {
-          const float* p = slot(i);
-          const float mi = p[0], li = p[1], v = p[2 + e];
-          if (li == 0.0f) continue;
-          const float f = mi > -INFINITY ? tq_exp2(mi - by) : 1.0f;
-          L = fmaf(li, f, L);
-          if (i < nc) x = fmaf(v, f, x);
-          else hot = fmaf(v, f, hot);
+        constexpr int BATCH = 4, STEP = ROWS == 4 ? 1 : 4;
+        for (int i0 = ROWS == 4 ? 0 : h; i0 < nc + nh; i0 += BATCH * STEP) {
+          float m[BATCH], l[BATCH], v[BATCH];
+          float top = M;
+#pragma unroll
+          for (int k = 0; k < BATCH; ++k) {
+            const int i = i0 + k * STEP;
+            m[k] = -INFINITY, l[k] = v[k] = 0.0f;
+            if (i < nc + nh) {
+              const float* p = base + (size_t)(i < nc ? i : a.ns_cold + i - nc) * TQ_PART_STRIDE;
+              m[k] = p[0], l[k] = p[1], v[k] = p[2 + e];
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < BATCH; ++k) top = fmaxf(top, m[k]);
+          const float by = top > -INFINITY ? top : 0.0f, down = M > -INFINITY ? tq_exp2(M - by) : 1.0f;
+          L *= down, x *= down, hot *= down;
+          M = top;
+#pragma unroll
+          for (int k = 0; k < BATCH; ++k) {
+            if (l[k] == 0.0f) continue;
+            const float f = m[k] > -INFINITY ? tq_exp2(m[k] - by) : 1.0f;
+            L = fmaf(l[k], f, L);
+            if (i0 + k * STEP < nc) x = fmaf(v[k], f, x);
+            else hot = fmaf(v[k], f, hot);
+          }
+        }
+        if (ROWS == 1) {  // the four groups to one maximum
+          if (e == 0) ms[h] = M;
+          __syncthreads();
+          const float top = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), by = top > -INFINITY ? top : 0.0f;
+          const float down = M > -INFINITY ? tq_exp2(M - by) : 1.0f;
+          L *= down, x *= down, hot *= down;
         }
       }
     }
@@ -1237,21 +1280,22 @@ __global__ void __launch_bounds__(AC_THREADS) attend_rows_combine_kernel(AttendA
 }
 
 template <int NT, bool SPLIT, int VB>
-int launch_rows(const AttendArgs& a, int sm_count, cudaStream_t st) {
+int launch_rows(const AttendArgs& a, cudaStream_t st) {
   using Shared = ArShared<NT, SPLIT, VB>;
   static_assert(sizeof(Shared) <= 227 * 1024, "shared memory of one CTA");
   const int64_t all = (int64_t)a.seq_count * a.g.n_kv_heads * a.rows;
   TQ_REQUIRE(all <= INT_MAX - 4 * AC_THREADS, TQ_ERR_UNSUPPORTED, "too many query rows in a call");
-  TQ_CUDA(cudaFuncSetAttribute(attend_rows_kernel<NT, SPLIT, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)sizeof(Shared)));
-  attend_rows_kernel<NT, SPLIT, VB><<<sm_count, 32 * ArShape<NT, SPLIT, VB>::WARPS, sizeof(Shared), st>>>(a);
+  static bool done[64];
+  const int rc = attend_shared(attend_rows_kernel<NT, SPLIT, VB>, sizeof(Shared), a.device, done);
+  if (rc != TQ_OK) return rc;
+  attend_rows_kernel<NT, SPLIT, VB><<<a.sm_count, 32 * ArShape<NT, SPLIT, VB>::WARPS, sizeof(Shared), st>>>(a);
   TQ_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
-  const bool few = all <= 4 * sm_count;
-  cfg.gridDim = dim3((unsigned)(few ? all : std::min<int64_t>((all + 3) / 4, 2 * sm_count)));
+  const bool few = all <= 2 * a.sm_count;
+  cfg.gridDim = dim3((unsigned)(few ? all : std::min<int64_t>((all + 3) / 4, 2 * a.sm_count)));
   cfg.blockDim = dim3(AC_THREADS);
   cfg.stream = st;
   cfg.attrs = &attr;
@@ -1262,13 +1306,13 @@ int launch_rows(const AttendArgs& a, int sm_count, cudaStream_t st) {
 }
 
 template <int NT, bool SPLIT>
-int launch_rows(const AttendArgs& a, int sm_count, cudaStream_t st) {
-  return a.g.value_bits == 4 ? launch_rows<NT, SPLIT, 4>(a, sm_count, st) : launch_rows<NT, SPLIT, 3>(a, sm_count, st);
+int launch_rows(const AttendArgs& a, cudaStream_t st) {
+  return a.g.value_bits == 4 ? launch_rows<NT, SPLIT, 4>(a, st) : launch_rows<NT, SPLIT, 3>(a, st);
 }
 
 }  // namespace
 
-AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens, int sm_count) {
+AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens) {
   const tq_geom& g = a.g;
   AttendRowsPlan p;
   const int nt = a.rows <= 8 ? 1 : 2;
@@ -1281,15 +1325,15 @@ AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens, int sm_count
   const int64_t strips = (seen + AR_STRIP - 1) / AR_STRIP + (std::min<int64_t>(a.sinks, in_blocks) + AR_STRIP - 1) / AR_STRIP;
   const int64_t hot = (std::min(tokens, g.hot_window) + AR_HOT - 1) / AR_HOT;
   const int64_t rows = (int64_t)std::min(a.seq_count, AR_SEQS) * g.n_kv_heads * ((a.rows + 8 * nt - 1) / (8 * nt));
-  const int64_t workers = (int64_t)sm_count * (a.q_dtype == TQ_BF16 ? (nt == 1 ? 12 : 8) : (nt == 1 ? 8 : 6));
+  const int64_t workers = (int64_t)a.sm_count * (a.q_dtype == TQ_BF16 ? (nt == 1 ? 12 : 8) : (nt == 1 ? 8 : 6));
   const int64_t share = std::max<int64_t>((AR_COST * strips + hot) * ((rows + 1) / 2) / workers, AR_COST);
   p.ns_cold = (int)std::min<int64_t>(AR_COST * strips / share + 3, 1024);
   p.ns_hot = (int)std::min<int64_t>(hot / share + 3, 64);
   return p;
 }
 
-int tq_launch_attend_rows(const AttendArgs& a, int sm_count, cudaStream_t st) {
+int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st) {
   if (a.q_dtype == TQ_BF16)
-    return a.rows <= 8 ? launch_rows<1, false>(a, sm_count, st) : launch_rows<2, false>(a, sm_count, st);
-  return a.rows <= 8 ? launch_rows<1, true>(a, sm_count, st) : launch_rows<2, true>(a, sm_count, st);
+    return a.rows <= 8 ? launch_rows<1, false>(a, st) : launch_rows<2, false>(a, st);
+  return a.rows <= 8 ? launch_rows<1, true>(a, st) : launch_rows<2, true>(a, st);
 }

@@ -961,10 +961,10 @@ Layout layout(const AttendArgs& a, int units, int cap, int splits) {
 
 template <bool SPLIT>
 int launch(const AttendArgs& a, const TileArgs& ta, int units, cudaStream_t st) {
-  TQ_CUDA(cudaFuncSetAttribute(attend_stage_kernel<SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)sizeof(StageShared<SPLIT>)));
-  TQ_CUDA(cudaFuncSetAttribute(attend_tiles_kernel<SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)sizeof(TiShared)));
+  static bool stage_done[64], tiles_done[64];
+  int rc = attend_shared(attend_stage_kernel<SPLIT>, sizeof(StageShared<SPLIT>), a.device, stage_done);
+  if (rc == TQ_OK) rc = attend_shared(attend_tiles_kernel<SPLIT>, sizeof(TiShared), a.device, tiles_done);
+  if (rc != TQ_OK) return rc;
   TQ_CUDA(cudaMemsetAsync(ta.left, 0, (size_t)units * 4, st));
   attend_stage_kernel<SPLIT><<<units * ta.cap, TS_THREADS, sizeof(StageShared<SPLIT>), st>>>(a, ta);
   TQ_CUDA(cudaGetLastError());
@@ -979,8 +979,7 @@ size_t tq_attend_tiles_bytes(const AttendArgs& a, int units, int cap, int splits
   return layout(a, units, cap, splits).total;
 }
 
-int tq_launch_attend_tiles(const AttendArgs& base, void* workspace, int cap, int splits, int device,
-                           cudaStream_t st) {
+int tq_launch_attend_tiles(const AttendArgs& base, void* workspace, int cap, int splits, cudaStream_t st) {
   AttendArgs a = base;
   const int units = a.seq_count * a.g.n_kv_heads;
   const Layout l = layout(a, units, cap, splits);
@@ -1006,9 +1005,7 @@ int tq_launch_attend_tiles(const AttendArgs& base, void* workspace, int cap, int
   if (rc != TQ_OK) return rc;
   rc = tq_launch_attend_general(a, st);
   if (rc != TQ_OK) return rc;
-  int sm_count = 148;
-  TQ_CUDA(cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, device));
-  attend_tiles_combine_kernel<<<std::min(units * tiles, 2 * sm_count), TC_THREADS, 0, st>>>(a, ta, tiles, units * tiles);
+  attend_tiles_combine_kernel<<<std::min(units * tiles, 2 * a.sm_count), TC_THREADS, 0, st>>>(a, ta, tiles, units * tiles);
   TQ_CUDA(cudaGetLastError());
   return TQ_OK;
 }

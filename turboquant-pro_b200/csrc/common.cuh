@@ -141,6 +141,7 @@ struct tq_ctx {
   bool bias_means = false;   // key zero-points come from the table behind the Tables struct
   alignas(64) unsigned char tmap_hot[2][128];
   int tmap_state = 0;
+  int sm_count = 0;  // of the device, once asked for (tq_attend)
 };
 
 TQ_HD size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
