@@ -38,25 +38,28 @@
 namespace {
 
 constexpr int AR_S = 256;          // tokens of a page
+// Tiles of eight query rows that a warp takes at once: with two it takes twice the registers, eight warps an SM
+// instead of twelve, and as long per row (18 000 cycles a strip against 13 000: 2 250 and 1 080 an SM).
+constexpr int NT = 1;
 constexpr int AR_STRIP = 64;       // of them, in an item of the list
 constexpr int AR_HOT = 32;         // window tokens of an item
 constexpr int AR_PITCH = TQ_D * 2 + 16, AR_PITCH32 = TQ_D * 4 + 16;  // bytes of a window row in shared memory
-constexpr int AR_COST = 2;         // a strip takes the time of so many tiles of the window
+constexpr int AR_COST = 4, AR_HOT_COST = 3;  // how long a strip takes, and a tile of the window
 constexpr int AR_SEQS = 64;        // sequences of a launch
 constexpr int AR_LIST = 256;       // outliers of a strip that are copied ahead (160 is usual)
 
-template <int NT, bool SPLIT, int VB>
+template <bool SPLIT, int VB>
 struct ArShape {
   static constexpr int N = 8 * NT;                     // query rows
   static constexpr int NV = VB == 4 ? 256 : 64;
-  static constexpr int WARPS = SPLIT ? (NT == 1 ? 8 : 6) : (NT == 1 ? 12 : 8);  // as many as have room
+  static constexpr int WARPS = SPLIT ? 8 : 12;         // as many as have room
   // sixteen copies of a table side by side: pairs fill a half warp's banks
   static constexpr int ENTRY = 16 * (SPLIT ? 8 : 4);   // bytes of an entry, copies and all
   static constexpr int LUTK = 256 * ENTRY, LUTV = NV * ENTRY;
 };
 
 // A warp's strip of a page, or the values of a tile of the window in its place.
-template <int NT, bool SPLIT, int VB>
+template <bool SPLIT, int VB>
 struct alignas(16) ArWarp {
   uint8_t keys[AR_STRIP * TQ_D / 2];
   uint16_t delta[TQ_ELL_SLOTS][AR_STRIP];
@@ -73,11 +76,11 @@ struct alignas(16) ArWarp {
 };
 static_assert(AR_HOT * AR_PITCH <= 6528 + 64 * TQ_D * 3 / 8 + 256 && 16 * AR_PITCH32 <= 6528 + 64 * TQ_D * 3 / 8 + 256, "a tile of the window in a strip's place");
 
-template <int NT, bool SPLIT, int VB>
+template <bool SPLIT, int VB>
 struct ArShared {
-  using Sh = ArShape<NT, SPLIT, VB>;
+  using Sh = ArShape<SPLIT, VB>;
   alignas(128) uint8_t lut[Sh::LUTK + Sh::LUTV];
-  ArWarp<NT, SPLIT, VB> warp[Sh::WARPS];
+  ArWarp<SPLIT, VB> warp[Sh::WARPS];
   float grid[16], cent[16];
   int2 seq[AR_SEQS];                            // tokens, query tokens
   int64_t cum[AR_SEQS + 1];                     // the cost of the sequences before
@@ -181,7 +184,7 @@ struct ArWork {
   AttendTiles strip, hot;
   int cold;  // tokens in blocks
   TQ_DEV int items() const { return strip.count() + hot.count(); }
-  TQ_DEV int cost() const { return AR_COST * strip.count() + hot.count(); }
+  TQ_DEV int cost() const { return AR_COST * strip.count() + AR_HOT_COST * hot.count(); }
 };
 TQ_DEV ArWork ar_work(const AttendArgs& a, int n, int q_n) {
   ArWork w;
@@ -201,19 +204,19 @@ struct ArPlan {
   int4 seq[AR_SEQS];  // strips, window tiles and row tiles of a sequence
 };
 
-template <int NT, bool SPLIT, int VB>
-__global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_rows_kernel(AttendArgs a) {
-  using Sh = ArShape<NT, SPLIT, VB>;
+template <bool SPLIT, int VB>
+__global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows_kernel(AttendArgs a) {
+  using Sh = ArShape<SPLIT, VB>;
   constexpr int N = Sh::N, WARPS = Sh::WARPS, THREADS = 32 * WARPS;
   constexpr int VGB = TQ_GROUP_TOK * TQ_D * VB / 8;
   extern __shared__ __align__(128) uint8_t ar_shared[];
-  ArShared<NT, SPLIT, VB>& sh = *(ArShared<NT, SPLIT, VB>*)ar_shared;
+  ArShared<SPLIT, VB>& sh = *(ArShared<SPLIT, VB>*)ar_shared;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const tq_geom& g = a.g;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
   const int H = g.n_kv_heads, G = g.group;
   const bool q32 = a.q_dtype == TQ_F32;
-  ArWarp<NT, SPLIT, VB>& my = sh.warp[warp];
+  ArWarp<SPLIT, VB>& my = sh.warp[warp];
 
   // ---- the work before every sequence
   if (tid < 16) {
@@ -257,13 +260,13 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
   }
   __syncthreads();
   // Shares of equal cost: what starts in [k share, (k + 1) share) is warp k's.  A row's strips then meet at most
-  // AR_COST * (strips - 1) / share + 2 warps, its window tiles (tiles - 1) / share + 2, which have to fit their slots; and
+  // AR_COST * (strips - 1) / share + 2 warps, its window tiles likewise, which have to fit their slots; and
   // no share is smaller than a strip's cost, so that every warp between a row's first and last has a part.
   const int workers = gridDim.x * WARPS;
   const int64_t total = sh.cum[AR_SEQS];
   int64_t share = max((total + workers - 1) / workers, (int64_t)AR_COST);
   share = max(share, (int64_t)((AR_COST * sh.most[0] + a.ns_cold - 3) / (a.ns_cold - 2)));
-  share = max(share, (int64_t)((sh.most[1] + a.ns_hot - 3) / (a.ns_hot - 2)));
+  share = max(share, (int64_t)((AR_HOT_COST * sh.most[1] + a.ns_hot - 3) / (a.ns_hot - 2)));
   if (blockIdx.x == 0) {
     ArPlan* plan = (ArPlan*)a.plan;
     if (tid == 0) plan->share = share;
@@ -307,11 +310,18 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
     const int off = (int)(in - (int64_t)row * cost), strips = AR_COST * row_strips;
     begin = at - off;
     head = row / row_tiles, rt = row - head * row_tiles;
-    it = off < strips ? (off + AR_COST - 1) / AR_COST : row_strips + off - strips;
-    at = begin + (off < strips ? AR_COST * it : off);
+    if (off < strips) {
+      it = (off + AR_COST - 1) / AR_COST;
+      at = begin + AR_COST * it;
+    } else {
+      const int k = (off - strips + AR_HOT_COST - 1) / AR_HOT_COST;
+      it = row_strips + k;
+      at = begin + strips + AR_HOT_COST * k;
+    }
   }
   auto next_row = [&]() {  // false: there is none
-    begin += AR_COST * row_strips + (row_items - row_strips);
+    begin += w.cost();
+    at = begin;
     it = 0;
     if (++rt < row_tiles) return true;
     rt = 0;
@@ -323,7 +333,7 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
     enter_seq();
     return true;
   };
-  if (more && it == row_items) more = next_row();  // (it began within the last strip of a row without a window)
+  if (more && it == row_items) more = next_row();  // (it began within the last item of a row)
   more = more && at < stop;
 
   // ---- copies
@@ -1154,7 +1164,7 @@ __global__ void __launch_bounds__(32 * ArShape<NT, SPLIT, VB>::WARPS, 1) attend_
       const int n = sh.seq[s].x;
       ring = uix * (size_t)g.hot_cap * TQ_D;
 #pragma unroll 1
-      for (; it < row_items && at < stop; ++it, ++at) {
+      for (; it < row_items && at < stop; ++it, at += AR_HOT_COST) {
         const int t0 = w.cold + w.hot.at(it - row_strips) * AR_HOT;
         slot0 = t0 % g.hot_cap;
         if (open_to_none(t0, min(t0 + AR_HOT, n))) continue;
@@ -1201,10 +1211,10 @@ __global__ void __launch_bounds__(AC_THREADS, 2) attend_rows_combine_kernel(Atte
       const int4 seq = plan->seq[s];
       const int64_t before = plan->cum[s];
       if (row / tile < seq.z) {
-        const int64_t begin = before + (int64_t)(head * seq.z + row / tile) * (AR_COST * seq.x + seq.y);
+        const int64_t begin = before + (int64_t)(head * seq.z + row / tile) * (AR_COST * seq.x + AR_HOT_COST * seq.y);
         const int64_t middle = begin + AR_COST * seq.x;
         const int nc = seq.x > 0 ? (int)(ar_div(middle - AR_COST, share) - ar_div(begin, share)) + 1 : 0;
-        const int nh = seq.y > 0 ? (int)(ar_div(middle + seq.y - 1, share) - ar_div(middle, share)) + 1 : 0;
+        const int nh = seq.y > 0 ? (int)(ar_div(middle + AR_HOT_COST * (seq.y - 1), share) - ar_div(middle, share)) + 1 : 0;
         const float* base = attend_partial(a, unit, row, 0);
         float M = -INFINITY;
         constexpr int BATCH = 4, STEP = ROWS == 4 ? 1 : 4;
@@ -1279,16 +1289,16 @@ __global__ void __launch_bounds__(AC_THREADS, 2) attend_rows_combine_kernel(Atte
   }
 }
 
-template <int NT, bool SPLIT, int VB>
+template <bool SPLIT, int VB>
 int launch_rows(const AttendArgs& a, cudaStream_t st) {
-  using Shared = ArShared<NT, SPLIT, VB>;
+  using Shared = ArShared<SPLIT, VB>;
   static_assert(sizeof(Shared) <= 227 * 1024, "shared memory of one CTA");
   const int64_t all = (int64_t)a.seq_count * a.g.n_kv_heads * a.rows;
   TQ_REQUIRE(all <= INT_MAX - 4 * AC_THREADS, TQ_ERR_UNSUPPORTED, "too many query rows in a call");
   static bool done[64];
-  const int rc = attend_shared(attend_rows_kernel<NT, SPLIT, VB>, sizeof(Shared), a.device, done);
+  const int rc = attend_shared(attend_rows_kernel<SPLIT, VB>, sizeof(Shared), a.device, done);
   if (rc != TQ_OK) return rc;
-  attend_rows_kernel<NT, SPLIT, VB><<<a.sm_count, 32 * ArShape<NT, SPLIT, VB>::WARPS, sizeof(Shared), st>>>(a);
+  attend_rows_kernel<SPLIT, VB><<<a.sm_count, 32 * ArShape<SPLIT, VB>::WARPS, sizeof(Shared), st>>>(a);
   TQ_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr = {};
@@ -1305,17 +1315,11 @@ int launch_rows(const AttendArgs& a, cudaStream_t st) {
   return TQ_OK;
 }
 
-template <int NT, bool SPLIT>
-int launch_rows(const AttendArgs& a, cudaStream_t st) {
-  return a.g.value_bits == 4 ? launch_rows<NT, SPLIT, 4>(a, st) : launch_rows<NT, SPLIT, 3>(a, st);
-}
-
 }  // namespace
 
 AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens) {
   const tq_geom& g = a.g;
   AttendRowsPlan p;
-  const int nt = a.rows <= 8 ? 1 : 2;
   p.seqs = AR_SEQS;
   p.plan_bytes = align_up(sizeof(ArPlan), 256);
   // Slots for the states of a row: what its work meets at the shares of this call where the other sequences are
@@ -1324,16 +1328,15 @@ AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens) {
   const int64_t seen = a.window == INT_MAX ? in_blocks : std::min<int64_t>(in_blocks, (int64_t)a.window + a.n_tokens + 128);
   const int64_t strips = (seen + AR_STRIP - 1) / AR_STRIP + (std::min<int64_t>(a.sinks, in_blocks) + AR_STRIP - 1) / AR_STRIP;
   const int64_t hot = (std::min(tokens, g.hot_window) + AR_HOT - 1) / AR_HOT;
-  const int64_t rows = (int64_t)std::min(a.seq_count, AR_SEQS) * g.n_kv_heads * ((a.rows + 8 * nt - 1) / (8 * nt));
-  const int64_t workers = (int64_t)a.sm_count * (a.q_dtype == TQ_BF16 ? (nt == 1 ? 12 : 8) : (nt == 1 ? 8 : 6));
-  const int64_t share = std::max<int64_t>((AR_COST * strips + hot) * ((rows + 1) / 2) / workers, AR_COST);
+  const int64_t rows = (int64_t)std::min(a.seq_count, AR_SEQS) * g.n_kv_heads * ((a.rows + 8 * NT - 1) / (8 * NT));
+  const int64_t workers = (int64_t)a.sm_count * (a.q_dtype == TQ_BF16 ? ArShape<false, 3>::WARPS : ArShape<true, 3>::WARPS);
+  const int64_t share = std::max<int64_t>((AR_COST * strips + AR_HOT_COST * hot) * ((rows + 1) / 2) / workers, AR_COST);
   p.ns_cold = (int)std::min<int64_t>(AR_COST * strips / share + 3, 1024);
-  p.ns_hot = (int)std::min<int64_t>(hot / share + 3, 64);
+  p.ns_hot = (int)std::min<int64_t>(AR_HOT_COST * hot / share + 3, 64);
   return p;
 }
 
 int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st) {
-  if (a.q_dtype == TQ_BF16)
-    return a.rows <= 8 ? launch_rows<1, false>(a, st) : launch_rows<2, false>(a, st);
-  return a.rows <= 8 ? launch_rows<1, true>(a, st) : launch_rows<2, true>(a, st);
+  if (a.q_dtype == TQ_BF16) return a.g.value_bits == 4 ? launch_rows<false, 4>(a, st) : launch_rows<false, 3>(a, st);
+  return a.g.value_bits == 4 ? launch_rows<true, 4>(a, st) : launch_rows<true, 3>(a, st);
 }
