@@ -71,16 +71,28 @@ TQ_DEV uint32_t ti_rest(float a, float b, uint32_t hi) {  // what the pair's rou
   return ti_pair(a - f.x, b - f.y);
 }
 
+TQ_DEV void tc_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// (a NaN stays)
+TQ_DEV float ti_max3_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 constexpr int TS_THREADS = 256;
-constexpr int TS_VS = TQ_D + 4;   // floats per row of window values
+constexpr int TS_PITCH = TQ_D * 2 + 16;  // bytes per row of window values
 constexpr int TS_VT = 32;         // window tokens that are rotated at a time
 template <bool SPLIT>
 struct StageShared {
-  alignas(16) uint8_t k[SPLIT ? 2 : 1][TI_IMAGE];  // afterwards rows of window values
-  float center[TQ_D], grid[16], cent[16], norm[TI_T];
+  alignas(16) uint8_t k[SPLIT ? 2 : 1][TI_IMAGE];  // afterwards rows of window values, as pairs hi + lo
+  alignas(16) float center[TQ_D];
+  float grid[16], cent[16], norm[TI_T];
   float top[TS_THREADS / 32];
 };
-static_assert(TS_VT * TS_VS * 4 <= TI_IMAGE, "the window values' place");
+static_assert(2 * TS_VT * TS_PITCH <= TI_IMAGE, "the window values' place");
 
 // eight neighbouring elements of a window row
 TQ_DEV void ts_ld8(const void* p, size_t at, int dt, float (&x)[8]) {
@@ -125,10 +137,18 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
   const size_t ring = hot_offset_elems(g, a.layer, a.seq_begin + s, head);
   const bool hot = t1 > sq.cold;  // some tokens are of the window
 
-  PageMeta first = {0, 0};  // of the tile's first block, ahead of its use
+  // what is used later, on its way: the tile's first block's list, this thread's half of a token's codes
+  PageMeta first = {0, 0};
   if (g.outlier_k > 0 && t0 < sq.cold) first = a.page_meta[uix * g.max_blocks + t0 / S];
+  const int kt = t0 + (tid & 127), kh = tid >> 7, kb = kt / S, kslot = kt - kb * S;
+  const uint8_t* const kpage = pages + (size_t)kb * g.page_bytes;
+  uint4 c0 = {0u, 0u, 0u, 0u}, c1 = c0;
+  if (kt < sq.cold) {
+    c0 = *(const uint4*)(kpage + kslot * (TQ_D / 2) + 32 * kh);
+    c1 = *(const uint4*)(kpage + kslot * (TQ_D / 2) + 32 * kh + 16);
+  }
   if (tid < 16) {
-    sh.grid[tid] = a.tables->grid[tid];
+    sh.grid[tid] = a.tables->grid[tid] * (1.0f / TI_KEY);
     sh.cent[tid] = a.tables->centroids[tid];
   }
   if (tid < TQ_D) {  // uniform grids count from their zero-point on: their middle
@@ -172,26 +192,22 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
   }
   __syncthreads();
   {  // ---- keys: a thread has half a token
-    const int row = tid & 127, h = tid >> 7, t = t0 + row;
-    auto put = [&](int chunk, const float (&x)[8]) {
+    const int row = tid & 127, h = kh, t = kt;
+    float most = 0.0f;
+    auto put = [&](int chunk, const float (&x)[8]) {  // (already divided by TI_KEY)
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = x[2 * i] * (1.0f / TI_KEY), q = x[2 * i + 1] * (1.0f / TI_KEY);
-        odd |= !(fabsf(p) <= 65504.0f) || !(fabsf(q) <= 65504.0f);
-        hi[i] = ti_pair(p, q);
-        if (SPLIT) lo[i] = ti_rest(p, q, hi[i]);
+        most = ti_max3_nan(most, fabsf(x[2 * i]), fabsf(x[2 * i + 1]));
+        hi[i] = ti_pair(x[2 * i], x[2 * i + 1]);
+        if (SPLIT) lo[i] = ti_rest(x[2 * i], x[2 * i + 1], hi[i]);
       }
       *(uint4*)(sh.k[0] + chunk * TI_LBO + row * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       if (SPLIT) *(uint4*)(sh.k[SPLIT] + chunk * TI_LBO + row * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     };
     if (t < sq.cold) {
-      const int b = t / S, slot = t - b * S;
-      const uint8_t* page = pages + (size_t)b * g.page_bytes;
-      const float* sc = (const float*)(page + g.scale_off);
-      const float* mu = (const float*)(page + g.mean_off);
-      const uint4 c0 = *(const uint4*)(page + slot * (TQ_D / 2) + 32 * h);
-      const uint4 c1 = *(const uint4*)(page + slot * (TQ_D / 2) + 32 * h + 16);
+      const float* sc = (const float*)(kpage + g.scale_off);
+      const float* mu = (const float*)(kpage + g.mean_off);
       const uint32_t w[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -200,9 +216,11 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         const float4 m0 = *(const float4*)(mu + d), m1 = *(const float4*)(mu + d + 4);
         const float ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
         const float mm[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
+        const float4 z0 = *(const float4*)&sh.center[d], z1 = *(const float4*)&sh.center[d + 4];
+        const float zz[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fmaf(ss[e], sh.grid[w[i] >> (4 * e) & 15], mm[e] - sh.center[d + e]);
+        for (int e = 0; e < 8; ++e) x[e] = fmaf(ss[e], sh.grid[w[i] >> (4 * e) & 15], (mm[e] - zz[e]) * (1.0f / TI_KEY));
         put(8 * h + i, x);
       }
     } else {
@@ -213,7 +231,7 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         if (t < t1) {
           ts_ld8(a.hot_k, at + 8 * i, g.kv_dtype, x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] -= sh.center[64 * h + 8 * i + e];
+          for (int e = 0; e < 8; ++e) x[e] = (x[e] - sh.center[64 * h + 8 * i + e]) * (1.0f / TI_KEY);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = 0.0f;
@@ -221,6 +239,7 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         put(8 * h + i, x);
       }
     }
+    odd |= !(most <= 65504.0f);
   }
   __syncthreads();
   if (g.outlier_k > 0) {
@@ -301,67 +320,81 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
     }
     return;
   }
-  // a thread has 8 tokens x 2 channels: window tokens v @ Pi^T, tokens of blocks from their codes
-  const int tg = tid >> 6, cp = tid & 63;
-  float(*vs)[TS_VS] = (float(*)[TS_VS])sh.k[0];
+  // Window tokens are rotated, v @ Pi^T, on mma.sync: 32 tokens at a time as pairs hi + lo are the B operand, a warp's 16
+  // output channels, whose rows of Pi are pairs too, the A operand.  Tokens of blocks in the same tile come
+  // from their codes one by one.
+  uint8_t* const vs = sh.k[0];
+  const int q = lane >> 2, c = lane & 3;
 #pragma unroll 1
-  for (int c0 = 0; c0 < TI_T; c0 += TS_VT) {
-    float x[8][2];
+  for (int n0 = 0; n0 < TI_T; n0 += TS_VT) {
+    float d[TS_VT / 8][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i][0] = x[i][1] = 0.0f;
-    if (t0 + c0 + TS_VT > sq.cold && t0 + c0 < t1) {
+    for (int nt = 0; nt < TS_VT / 8; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[nt][i] = 0.0f;
+    if (t0 + n0 + TS_VT > sq.cold && t0 + n0 < t1) {
       __syncthreads();  // (the keys, or the rows before, have been read)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int row = tid >> 3, d = (tid & 7) * 16 + 8 * u, t = t0 + c0 + row;
+        const int row = tid >> 3, ch = (tid & 7) * 16 + 8 * u, t = t0 + n0 + row;
         float v[8];
         if (t >= sq.cold && t < t1) {
-          ts_ld8(a.hot_v, ring + (size_t)(t % g.hot_cap) * TQ_D + d, g.kv_dtype, v);
+          ts_ld8(a.hot_v, ring + (size_t)(t % g.hot_cap) * TQ_D + ch, g.kv_dtype, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = 0.0f;
         }
-        *(float4*)&vs[row][d] = make_float4(v[0], v[1], v[2], v[3]);
-        *(float4*)&vs[row][d + 4] = make_float4(v[4], v[5], v[6], v[7]);
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          hi[i] = ti_pair(v[2 * i] * up, v[2 * i + 1] * up);
+          lo[i] = ti_rest(v[2 * i] * up, v[2 * i + 1] * up, hi[i]);
+        }
+        *(uint4*)(vs + row * TS_PITCH + 2 * ch) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *(uint4*)(vs + (TS_VT + row) * TS_PITCH + 2 * ch) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
       __syncthreads();
-#pragma unroll 2
-      for (int d = 0; d < TQ_D; d += 4) {
-        float2 w[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = *(const float2*)&a.tables->pi_t[(d + e) * TQ_D + 2 * cp];
+      for (int k = 0; k < 8; ++k) {
+        uint32_t ph[4], pl[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 v = *(const float4*)&vs[8 * tg + i][d];
-          x[i][0] = fmaf(v.x, w[0].x, fmaf(v.y, w[1].x, fmaf(v.z, w[2].x, fmaf(v.w, w[3].x, x[i][0]))));
-          x[i][1] = fmaf(v.x, w[0].y, fmaf(v.y, w[1].y, fmaf(v.z, w[2].y, fmaf(v.w, w[3].y, x[i][1]))));
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = *(const float2*)&a.tables->pi[(16 * warp + q + 8 * (i & 1)) * TQ_D + 16 * k + 2 * c + 8 * (i >> 1)];
+          ph[i] = ti_pair(x.x * 256.0f, x.y * 256.0f);
+          pl[i] = ti_rest(x.x * 256.0f, x.y * 256.0f, ph[i]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < TS_VT / 8; ++nt) {
+          const uint8_t* at = vs + (8 * nt + q) * TS_PITCH + 32 * k + 4 * c;
+          const uint32_t h0 = *(const uint32_t*)at, h1 = *(const uint32_t*)(at + 16);
+          const uint32_t l0 = *(const uint32_t*)(at + TS_VT * TS_PITCH), l1 = *(const uint32_t*)(at + TS_VT * TS_PITCH + 16);
+          tc_mma(d[nt], pl, h0, h1);
+          tc_mma(d[nt], ph, l0, l1);
+          tc_mma(d[nt], ph, h0, h1);
         }
       }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int t = t0 + c0 + 8 * tg + i;
-      if (t < sq.cold) {
-        const int b = t / S, slot = t - b * S;
-        const uint8_t* grp = pages + (size_t)b * g.page_bytes + g.v_off + (size_t)(slot >> 4) * v_group_bytes(vb);
-        const float norm = sh.norm[c0 + 8 * tg + i];
+    for (int nt = 0; nt < TS_VT / 8; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) x[i][e] = norm * sh.cent[v_get_code(grp, vb, slot & 15, 2 * cp + e)];
+      for (int y = 0; y < 2; ++y) {  // channels q, q + 8 of the warp's sixteen; tokens 2 c, 2 c + 1
+        const int ch = 16 * warp + q + 8 * y, n = n0 + 8 * nt + 2 * c;
+        float x[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int t = t0 + n + e;
+          x[e] = d[nt][2 * y + e] * (1.0f / 256.0f);
+          if (t < sq.cold) {
+            const int b = t / S, slot = t - b * S;
+            const uint8_t* grp = pages + (size_t)b * g.page_bytes + g.v_off + (size_t)(slot >> 4) * v_group_bytes(vb);
+            x[e] = sh.norm[n + e] * up * sh.cent[v_get_code(grp, vb, slot & 15, ch)];
+          }
+        }
+        const uint32_t hi = ti_pair(x[0], x[1]);
+        const int at = (n >> 3) * TI_LBO + ch * 16 + (n & 7) * 2;
+        *(uint32_t*)(v_hi + at) = hi;
+        if (SPLIT) *(uint32_t*)(v_lo + at) = ti_rest(x[0], x[1], hi);
       }
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = x[2 * i][e] * up, q = x[2 * i + 1][e] * up;
-        hi[i] = ti_pair(p, q);
-        if (SPLIT) lo[i] = ti_rest(p, q, hi[i]);
-      }
-      const int at = (c0 / 8 + tg) * TI_LBO + (2 * cp + e) * 16;
-      *(uint4*)(v_hi + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      if (SPLIT) *(uint4*)(v_lo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
   }
 }
 
@@ -806,11 +839,6 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
 // lo * hi, good to 2^-22.  Bound by reading the sums.
 constexpr int TC_ROWS = 64, TC_THREADS = 256, TC_PITCH = TQ_D * 2 + 16;
 
-TQ_DEV void tc_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 
 __global__ void __launch_bounds__(TC_THREADS, 2) attend_tiles_combine_kernel(AttendArgs a, TileArgs ta, int tiles, int total) {
   __shared__ __align__(16) uint8_t hi[TC_ROWS * TC_PITCH], lo[TC_ROWS * TC_PITCH];
