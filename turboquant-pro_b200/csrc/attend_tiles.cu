@@ -13,9 +13,10 @@
 //     What is not a number, or too large even so, sets the flag of its (sequence, KV head), which the general kernel
 //     then does.
 // attend_tiles_kernel   256 rows of a (sequence, KV head) per CTA against a split of these tiles.  S = Q K^T into tensor
-//     memory; two groups of 128 threads, a thread per row, make the probabilities and put them back over S as fp16;
+//     memory; two groups of 256 threads, two threads per row, make the probabilities and put them back over S as fp16;
 //     O += P V with P as the operand in tensor memory.  The groups work on different halves of the rows, so that the
-//     tensor cores have one's products while the other's softmax runs.  A tile's exponent is added to its scores, so
+//     tensor cores have one's products while the other's softmax runs; a softmax is a chain that nothing else of its half
+//     overlaps, so its latency counts (one thread per row: 2 100 cycles of 4 050 a tile).  A tile's exponent is added to its scores, so
 //     that the running maximum is that of probability * value and fp16 holds what counts.  The maximum is only
 //     renewed (and O rescaled) when it has grown by 2^8 since.
 // attend_tiles_combine_kernel   merges the splits, rotates the sums back (sum @ Pi), rounds.
@@ -35,7 +36,8 @@ constexpr int TI_ROWS = 256;                 // rows of a CTA
 constexpr int TI_IMAGE = TI_T * TQ_D * 2;    // bytes of an operand image
 constexpr int TI_LBO = TI_T * 16, TI_SBO = 128;
 constexpr int TI_SLOTS = 5;                  // images in shared memory
-constexpr int TI_THREADS = 320;              // two softmax groups, a warp that issues, a warp that loads
+constexpr int TI_SOFTMAX = 512;              // softmax threads: two a row
+constexpr int TI_THREADS = TI_SOFTMAX + 64;  // and a warp that issues, a warp that loads
 constexpr float TI_KEY = 16.0f;              // keys are divided by it
 constexpr float TI_LIFT = 7.0f, TI_GROW = 8.0f;  // probabilities reach 2^(7 + 8) at most
 constexpr int TI_POLY = 2;                   // of eight pairs of exponentials, those on the multiply-add units
@@ -402,9 +404,11 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
 struct TiShared {
   alignas(128) uint8_t q[2][TI_IMAGE];
   alignas(128) uint8_t kv[TI_SLOTS][TI_IMAGE];
-  unsigned long long full[TI_SLOTS], empty[TI_SLOTS], q_ready, s_full[2], p_half[2], p_full[2], o_done[2];
+  unsigned long long full[TI_SLOTS], empty[TI_SLOTS], q_ready, s_full[2], p_full[2], o_done[2];
   uint32_t tmem;
+  float pair[2][2][128];  // what the two threads of a row tell each other
 };
+static_assert(sizeof(TiShared) <= 227 * 1024, "shared memory of one CTA");
 
 // (accumulate: known where the call stands, so that no predicate has to be formed)
 template <bool ACC>
@@ -450,6 +454,17 @@ TQ_DEV void ti_st32(uint32_t addr, const uint32_t* r) {
       "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
       TI_R8(r, 0), TI_R8(r, 8), TI_R8(r, 16), TI_R8(r, 24)
       : "memory");
+}
+TQ_DEV void ti_ld16(uint32_t addr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : TI_W8(r, 0), TI_W8(r, 8)
+               : "r"(addr)
+               : "memory");
+}
+TQ_DEV void ti_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+               TI_R8(r, 0), TI_R8(r, 8)
+               : "memory");
 }
 TQ_DEV float ti_max3(float a, float b, float c) {
   float y;
@@ -536,14 +551,13 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(enc_smem(&sh.s_full[i]), 1);
-      mbar_init(enc_smem(&sh.p_half[i]), 128);
-      mbar_init(enc_smem(&sh.p_full[i]), 128);
+      mbar_init(enc_smem(&sh.p_full[i]), 256);
       mbar_init(enc_smem(&sh.o_done[i]), 1);
     }
-    mbar_init(q_bar, 128 * groups);
+    mbar_init(q_bar, 256 * groups);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
+  if (warp == TI_SOFTMAX / 32) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(enc_smem(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -564,7 +578,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       }
   };
 
-  if (warp == 9) {
+  if (warp == TI_SOFTMAX / 32 + 1) {
     // ---- loads: K V of tile after tile through the ring
     if (lane == 0) {
       const uint8_t* images = ta.images + (size_t)unit * ta.cap * 2 * PARTS * TI_IMAGE;
@@ -589,7 +603,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       gave_up = false;
       for (int i = max(c - TI_SLOTS, 0); i < c; ++i) wait(&sh.full[i % TI_SLOTS], (i / TI_SLOTS) & 1);
     }
-  } else if (warp == 8) {
+  } else if (warp == TI_SOFTMAX / 32) {
     // ---- products
     // The whole warp runs this, one thread issues.  What the products take are constants or the same in all lanes to
     // the compiler's knowledge (the shuffle), so that it lies in uniform registers: fetched there product by product,
@@ -630,21 +644,21 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
           for (int i = 0; i < PARTS; ++i) umma_commit(enc_smem(&sh.empty[(c + i) % TI_SLOTS]));
         __syncwarp();
       };
-      // half h of the tokens of a tile, its values in chunk c: O += P V
-      auto values = [&](int x, int h, int c, bool fresh) {
+      // O += P V, the tile's values in chunk c
+      auto values = [&](int x, int c, bool fresh) {
         uint64_t b[PARTS];
 #pragma unroll
-        for (int i = 0; i < PARTS; ++i) b[i] = image(c + i) + 4 * h * STEP;
+        for (int i = 0; i < PARTS; ++i) b[i] = image(c + i);
         if (ti_elect()) {
-          const uint32_t d = tmem + 256 + 128 * x, p = tmem + 128 * x + 32 * h;
+          const uint32_t d = tmem + 256 + 128 * x, p = tmem + 128 * x;
           if (fresh) ti_mma_ts<false>(d, p, b[PARTS - 1], idesc);
           else ti_mma_ts<true>(d, p, b[PARTS - 1], idesc);
 #pragma unroll
-          for (int j = 1; j < 4; ++j) ti_mma_ts<true>(d, p + 8 * j, b[PARTS - 1] + j * STEP, idesc);
+          for (int j = 1; j < 8; ++j) ti_mma_ts<true>(d, p + 8 * j, b[PARTS - 1] + j * STEP, idesc);
           if (SPLIT)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) ti_mma_ts<true>(d, p + 8 * j, b[0] + j * STEP, idesc);
-          if (h == 1) umma_commit(enc_smem(&sh.o_done[x]));
+            for (int j = 0; j < 8; ++j) ti_mma_ts<true>(d, p + 8 * j, b[0] + j * STEP, idesc);
+          umma_commit(enc_smem(&sh.o_done[x]));
         }
         __syncwarp();
       };
@@ -663,13 +677,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           if (x >= groups_u) break;
-          // (the first half of the tokens while the second's probabilities are made)
-          wait_all(&sh.p_half[x], k & 1);
-          ti_fence_after();
-          values(x, 0, cv, k == 0);
           wait_all(&sh.p_full[x], k & 1);
           ti_fence_after();
-          values(x, 1, cv, false);
+          values(x, cv, k == 0);
           if (x == groups_u - 1) release(cv);
           if (k + 1 < n_u) {
             // the next scores take the place of the probabilities that these products read
@@ -682,26 +692,35 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       gave_up = false;  // (nor are products under way when the CTA's memory goes)
       for (int x = 0; x < groups_u; ++x) wait_all(&sh.o_done[x], (n_u - 1) & 1);
     }
-  } else if (warp < 4 * groups) {
-    // ---- a thread per row
-    const int x = warp >> 2, r = tid & 127, row = row0 + tid;
+  } else if (warp < 8 * groups) {
+    // ---- two threads per row: 64 tokens of a tile, and 64 channels of the sums, each
+    const int x = warp >> 3, part = warp >> 2 & 1, r = tid & 127, row = row0 + 128 * x + r;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t ts = tmem + 128 * x + lanes, to = tmem + 256 + 128 * x + lanes;
+    const uint32_t ts = tmem + 128 * x + lanes + 64 * part, tp = tmem + 128 * x + lanes + 32 * part;
+    const uint32_t to = tmem + 256 + 128 * x + lanes + 64 * part;
+    // the larger of the two threads' values (NaN: the other's)
+    auto of_both = [&](float v) {
+      sh.pair[x][part][r] = v;
+      ti_fence_before();
+      asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");
+      ti_fence_after();
+      return fmaxf(v, sh.pair[x][part ^ 1][r]);
+    };
     float factor;
     {
-      uint4 raw[16];
+      uint4 raw[8];
       const bool there = row < a.rows;
       const uint16_t* q = (const uint16_t*)a.q + ((int64_t)s * a.q_seq + (int64_t)(row / G) * a.q_tok +
-                                                  (int64_t)(head * G + row % G) * a.q_head);
+                                                  (int64_t)(head * G + row % G) * a.q_head) + 64 * part;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) raw[i] = there ? *(const uint4*)(q + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < 8; ++i) raw[i] = there ? *(const uint4*)(q + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
       auto pair = [&](uint32_t w) -> float2 {
-        if (a.q_dtype == TQ_F16) return __half22float2(*(const __half2*)&w);
+        if (SPLIT) return __half22float2(*(const __half2*)&w);
         return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
       };
       float top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -710,10 +729,10 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
         }
       }
       float exponent;
-      const float up = ti_lift(top, 13, exponent);
+      const float up = ti_lift(of_both(top), 13, exponent);
       factor = tq_scaled<true>(TI_KEY * exp2f(exponent));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
         uint32_t h[4];
 #pragma unroll
@@ -721,13 +740,14 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
           const float2 f = pair(w[j]);
           h[j] = ti_pair(f.x * up, f.y * up);
         }
-        *(uint4*)(sh.q[x] + i * TI_LBO + r * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+        *(uint4*)(sh.q[x] + (8 * part + i) * TI_LBO + r * 16) = make_uint4(h[0], h[1], h[2], h[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(q_bar);
+      asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");  // (the pairs have been read)
     }
     const int p = row < a.rows ? attend_position(a, sq, row) : -1, w = attend_window(a, p);
-    // rows of this CTA: the earliest one that sees anything, the latest window
+    // whether all rows of this CTA see a tile goes by their earliest position and latest window
     const bool whole = row0 + TI_ROWS <= a.rows && i_lo < sq.q_n && (row0 + TI_ROWS - 1) / G < sq.q_n && p_lo >= 0;
     const int w_hi = attend_window(a, max(p_hi, 0));
     float m = -INFINITY, l = 0.0f;
@@ -737,22 +757,22 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       wait(&sh.s_full[x], k & 1);
       gave_up = __any_sync(0xffffffffu, gave_up);
       ti_fence_after();
-      uint32_t v[128];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ti_ld32(ts + 32 * i, v + 32 * i);
+      uint32_t v[64];
+      ti_ld32(ts, v);
+      ti_ld32(ts + 32, v + 32);
       ti_wait_ld();
       const bool open = whole && t0 + TI_T - 1 <= p_lo && (t0 >= w_hi || t0 + TI_T <= a.sinks);
       if (!open) {
-        const int hi = min(p, sq.n - 1) - t0, lo = w - t0, sk = a.sinks - t0;
+        const int c0 = t0 + 64 * part, hi = min(p, sq.n - 1) - c0, lo = w - c0, sk = a.sinks - c0;
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
+        for (int i = 0; i < 64; ++i)
           if (i > hi || (i < lo && i >= sk)) v[i] = 0xff800000u;
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 128; i += 2)
+      for (int i = 0; i < 64; i += 2)
         top[i / 2 & 3] = ti_max3(top[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-      const float now = fmaf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), factor, e);
+      const float now = fmaf(of_both(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), factor, e);
       const bool grown = now > m + TI_GROW;  // (also from -inf)
       float down = 1.0f;
       if (grown) {
@@ -765,56 +785,61 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
         ti_fence_after();
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {
-          uint32_t o[32];
-          ti_ld32(to + 32 * i, o);
+          uint32_t o[16];
+          ti_ld16(to + 16 * i, o);
           ti_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * down);
-          ti_st32(to + 32 * i, o);
+          for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * down);
+          ti_st16(to + 16 * i, o);
         }
       }
       const float off = TI_LIFT + e - (m > -INFINITY ? m : 0.0f);
       const uint64_t factor2 = ti_f2(factor, factor), off2 = ti_f2(off, off);
       uint64_t sum[2] = {0ull, 0ull};
+      uint32_t h[32];
+      if (open) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t h[32];
-        if (open) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const uint64_t y = ti_fma2(ti_u2(v[64 * i + 2 * j], v[64 * i + 2 * j + 1]), factor2, off2);
-            const float2 z = j % 8 < TI_POLY ? ti_exp2_poly(y) : ti_exp2_unit(y);
-            sum[j & 1] = ti_add2(sum[j & 1], ti_f2(z.x, z.y));
-            h[j] = ti_pair(z.x, z.y);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float2 z = ti_exp2_unit(ti_fma2(ti_u2(v[64 * i + 2 * j], v[64 * i + 2 * j + 1]), factor2, off2));
-            sum[j & 1] = ti_add2(sum[j & 1], ti_f2(z.x, z.y));
-            h[j] = ti_pair(z.x, z.y);
-          }
+        for (int j = 0; j < 32; ++j) {
+          const uint64_t y = ti_fma2(ti_u2(v[2 * j], v[2 * j + 1]), factor2, off2);
+          const float2 z = j % 8 < TI_POLY ? ti_exp2_poly(y) : ti_exp2_unit(y);
+          sum[j & 1] = ti_add2(sum[j & 1], ti_f2(z.x, z.y));
+          h[j] = ti_pair(z.x, z.y);
         }
-        ti_st32(ts + 32 * i, h);
-        ti_wait_st();
-        ti_fence_before();
-        mbar_arrive(enc_smem(i == 0 ? &sh.p_half[x] : &sh.p_full[x]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const float2 z = ti_exp2_unit(ti_fma2(ti_u2(v[2 * j], v[2 * j + 1]), factor2, off2));
+          sum[j & 1] = ti_add2(sum[j & 1], ti_f2(z.x, z.y));
+          h[j] = ti_pair(z.x, z.y);
+        }
       }
+      // (the probabilities go over the first half of the scores' columns, which the other thread of the row may still
+      // be reading: its loads are over when it has told its maximum)
+      ti_st32(tp, h);
+      ti_wait_st();
+      ti_fence_before();
+      mbar_arrive(enc_smem(&sh.p_full[x]));
       const float2 s2 = ti_floats(ti_add2(sum[0], sum[1]));
       l = fmaf(s2.x + s2.y, exp2f(-e), l * down);
     }
     // the row's state: [channel][row], neighbouring threads side by side
-    const size_t part = ((size_t)unit * ta.splits + split) * ta.row_tiles + rt;
-    float* stats = ta.stats + part * 2 * TI_ROWS + tid;
-    stats[0] = n > 0 ? m - TI_LIFT : -INFINITY;
-    stats[TI_ROWS] = l;
+    const size_t at = ((size_t)unit * ta.splits + split) * ta.row_tiles + rt;
+    asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");  // (the last maxima have been read)
+    sh.pair[x][part][r] = l;
+    asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");
+    if (part == 0) {
+      float* stats = ta.stats + at * 2 * TI_ROWS + 128 * x + r;
+      stats[0] = n > 0 ? m - TI_LIFT : -INFINITY;
+      stats[TI_ROWS] = sh.pair[x][0][r] + sh.pair[x][1][r];
+    }
     if (n > 0) {
       wait(&sh.o_done[x], (n - 1) & 1);
       gave_up = __any_sync(0xffffffffu, gave_up);
       ti_fence_after();
-      float* sums = ta.sums + (size_t)unit * a.unit_stride + ((size_t)split * ta.row_tiles + rt) * TI_ROWS * TQ_D + tid;
+      float* sums = ta.sums + (size_t)unit * a.unit_stride +
+                    (((size_t)split * ta.row_tiles + rt) * TQ_D + 64 * part) * TI_ROWS + 128 * x + r;
 #pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2; ++i) {
         uint32_t o[32];
         ti_ld32(to + 32 * i, o);
         ti_wait_ld();
@@ -826,7 +851,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
   __syncwarp();
   ti_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == TI_SOFTMAX / 32) {
     ti_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
