@@ -62,9 +62,10 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
            : rows <= 64 && channels && g.block_tokens == 256 ? ROWS : GENERAL;
   const int sm_count = ctx->sm_count;
   if (p.form == TILES) {
-    const int64_t all = std::max<int64_t>((n + 127) / 128, 1);
+    constexpr int TILE = TQ_ATTEND_TILE;
+    const int64_t all = std::max<int64_t>((n + TILE - 1) / TILE, 1);
     auto seen = [&](int64_t tokens) {  // tiles that so many neighbouring query tokens see
-      return r->window == 0 ? all : std::min<int64_t>(all, (r->window + tokens + 254) / 128 + (r->sinks + 127) / 128);
+      return r->window == 0 ? all : std::min<int64_t>(all, (r->window + tokens + 2 * TILE - 2) / TILE + (r->sinks + TILE - 1) / TILE);
     };
     p.cap = (int)seen(r->n_tokens);
     // splits of a tile of rows: as many as bring the rounds of CTAs nearest to even (with four tiles' time for

@@ -114,6 +114,7 @@ struct AttendRowsPlan {
 };
 AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens);
 int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st);
-// 16-bit queries, per-channel keys: everything in one, the merge too; `cap` tiles of 128 tokens per unit have room
+// 16-bit queries, per-channel keys: everything in one, the merge too; `cap` tiles of tokens per unit have room
+constexpr int TQ_ATTEND_TILE = 80;  // tokens of a tile
 size_t tq_attend_tiles_bytes(const AttendArgs& a, int units, int cap, int splits);
 int tq_launch_attend_tiles(const AttendArgs& a, void* workspace, int cap, int splits, cudaStream_t st);

@@ -1,7 +1,7 @@
 // Attention of many query rows per KV head on the codes: prompt chunks.  The products run on tcgen05 with the
 // accumulators in tensor memory.  Three kernels:
 //
-// attend_stage_kernel   the tokens that any row sees, 128 at a time, from codes to the two shared-memory images
+// attend_stage_kernel   the tokens that any row sees, 80 at a time, from codes to the two shared-memory images
 //     that tcgen05 takes as operands (fp16, K-major core matrices of 8 rows x 16 bytes), written to the workspace
 //     once instead of once per tile of rows:
 //       keys    (mean + scale * grid[code] - c) / 16, outliers put over it.  c is one vector per (sequence, KV head),
@@ -12,13 +12,15 @@
 //               the power of two that takes the tile's largest norm below 2^15, whose exponent is kept.
 //     What is not a number, or too large even so, sets the flag of its (sequence, KV head), which the general kernel
 //     then does.
-// attend_tiles_kernel   256 rows of a (sequence, KV head) per CTA against a split of these tiles.  S = Q K^T into tensor
-//     memory; two groups of 256 threads, two threads per row, make the probabilities and put them back over S as fp16;
-//     O += P V with P as the operand in tensor memory.  The groups work on different halves of the rows, so that the
-//     tensor cores have one's products while the other's softmax runs; a softmax is a chain that nothing else of its half
-//     overlaps, so its latency counts (one thread per row: 2 100 cycles of 4 050 a tile).  A tile's exponent is added to its scores, so
-//     that the running maximum is that of probability * value and fp16 holds what counts.  The maximum is only
-//     renewed (and O rescaled) when it has grown by 2^8 since.
+// attend_tiles_kernel   256 rows of a (sequence, KV head) per CTA against a split of these tiles, in two halves of 128 rows.
+//     S = Q K^T into tensor memory; a group of 256 threads per half, two threads per row, makes the probabilities and
+//     puts them back as fp16; O += P V with P as the operand in tensor memory.  Of its 512 columns a half has
+//     80 for scores, 40 for probabilities and 128 for the sums: that is what sets the tile.  (With 128 tokens the
+//     probabilities had to go over the scores, so that the next scores waited for the product that read them: a chain of
+//     3 800 cycles a tile, in which neither the tensor cores nor the softmax were busy for more than half.)  As it is
+//     the next scores are formed while the exponentials of these are.  A warp per half issues, one loads.
+//     A tile's exponent is added to its scores, so that the running maximum is that of probability * value and fp16
+//     holds what counts.  The maximum is only renewed (and O rescaled) when it has grown by 2^8 since.
 // attend_tiles_combine_kernel   merges the splits, rotates the sums back (sum @ Pi), rounds.
 //
 // Queries are fp16 in shared memory, each row scaled by a power of two, which is exact for both 16-bit types.
@@ -31,17 +33,20 @@
 
 namespace {
 
-constexpr int TI_T = 128;                    // tokens of a tile
+constexpr int TI_T = TQ_ATTEND_TILE;         // tokens of a tile
 constexpr int TI_ROWS = 256;                 // rows of a CTA
-constexpr int TI_IMAGE = TI_T * TQ_D * 2;    // bytes of an operand image
-constexpr int TI_LBO = TI_T * 16, TI_SBO = 128;
-constexpr int TI_SLOTS = 5;                  // images in shared memory
+constexpr int TI_IMAGE = TI_T * TQ_D * 2;    // bytes of an operand image of keys or values
+constexpr int TI_QIMAGE = 128 * TQ_D * 2;    // and of a half's queries
+constexpr int TI_KLBO = TI_T * 16, TI_LBO = TQ_D * 16, TI_SBO = 128;  // from eight K to the next: keys; queries, values
+constexpr int TI_SLOTS = 8;                  // images in shared memory
 constexpr int TI_SOFTMAX = 512;              // softmax threads: two a row
-constexpr int TI_THREADS = TI_SOFTMAX + 64;  // and a warp that issues, a warp that loads
+constexpr int TI_THREADS = TI_SOFTMAX + 96;  // and two warps that issue, a warp that loads
+constexpr int TI_S = 0, TI_P = TI_T, TI_HALF = 128, TI_O = 256;  // columns: scores, probabilities of a half, sums
 constexpr float TI_KEY = 16.0f;              // keys are divided by it
 constexpr float TI_LIFT = 7.0f, TI_GROW = 8.0f;  // probabilities reach 2^(7 + 8) at most
 constexpr int TI_POLY = 2;                   // of eight pairs of exponentials, those on the multiply-add units
-constexpr int TI_WAIT = 1 << 21;             // probes of a wait, a microsecond or two each at most
+constexpr int TI_WAIT = 1 << 21;             // probes of a wait
+static_assert(TI_P + TI_T / 2 <= TI_HALF && 2 * TI_HALF <= TI_O && TI_T % 16 == 0, "tensor memory's columns");
 
 struct TileArgs {
   uint8_t* images;    // [unit][cap][K hi, (K lo,) V hi, (V lo)]
@@ -84,9 +89,9 @@ TQ_DEV float ti_max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
-constexpr int TS_THREADS = 256;
+constexpr int TS_THREADS = 4 * TI_T;  // four a token; two warps per 16 tokens of values
 constexpr int TS_PITCH = TQ_D * 2 + 16;  // bytes per row of window values
-constexpr int TS_VT = 32;         // window tokens that are rotated at a time
+constexpr int TS_VT = 16;         // window tokens that are rotated at a time
 template <bool SPLIT>
 struct StageShared {
   alignas(16) uint8_t k[SPLIT ? 2 : 1][TI_IMAGE];  // afterwards rows of window values, as pairs hi + lo
@@ -139,16 +144,13 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
   const size_t ring = hot_offset_elems(g, a.layer, a.seq_begin + s, head);
   const bool hot = t1 > sq.cold;  // some tokens are of the window
 
-  // what is used later, on its way: the tile's first block's list, this thread's half of a token's codes
+  // what is used later, on its way: the tile's first block's list, this thread's quarter of a token's codes
   PageMeta first = {0, 0};
   if (g.outlier_k > 0 && t0 < sq.cold) first = a.page_meta[uix * g.max_blocks + t0 / S];
-  const int kt = t0 + (tid & 127), kh = tid >> 7, kb = kt / S, kslot = kt - kb * S;
+  const int krow = tid % TI_T, kq = tid / TI_T, kt = t0 + krow, kb = kt / S, kslot = kt - kb * S;
   const uint8_t* const kpage = pages + (size_t)kb * g.page_bytes;
-  uint4 c0 = {0u, 0u, 0u, 0u}, c1 = c0;
-  if (kt < sq.cold) {
-    c0 = *(const uint4*)(kpage + kslot * (TQ_D / 2) + 32 * kh);
-    c1 = *(const uint4*)(kpage + kslot * (TQ_D / 2) + 32 * kh + 16);
-  }
+  uint4 codes = {0u, 0u, 0u, 0u};
+  if (kt < sq.cold) codes = *(const uint4*)(kpage + kslot * (TQ_D / 2) + 16 * kq);
   if (tid < 16) {
     sh.grid[tid] = a.tables->grid[tid] * (1.0f / TI_KEY);
     sh.cent[tid] = a.tables->centroids[tid];
@@ -163,8 +165,8 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
     sh.center[tid] = c;
   }
   bool odd = false;
-  {  // ---- norms of the values: two threads a token
-    const int row = tid >> 1, t = t0 + row;
+  {  // ---- norms of the values: four threads a token
+    const int row = tid >> 2, t = t0 + row;
     float norm = 0.0f;
     if (t < sq.cold) {
       const int b = t / S;
@@ -173,9 +175,9 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
     if (hot) {
       float ss = 0.0f;
       if (t >= sq.cold && t < t1) {
-        const size_t at = ring + (size_t)(t % g.hot_cap) * TQ_D + (tid & 1) * (TQ_D / 2);
-#pragma unroll 4
-        for (int i = 0; i < 8; ++i) {
+        const size_t at = ring + (size_t)(t % g.hot_cap) * TQ_D + (tid & 3) * (TQ_D / 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
           float x[8];
           ts_ld8(a.hot_v, at + 8 * i, g.kv_dtype, x);
 #pragma unroll
@@ -183,18 +185,18 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         }
       }
       ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+      ss += __shfl_xor_sync(0xffffffffu, ss, 2);
       if (t >= sq.cold) norm = sqrtf(ss);
     }
     odd |= !isfinite(norm);
-    if ((tid & 1) == 0) sh.norm[row] = norm;
+    if ((tid & 3) == 0) sh.norm[row] = norm;
     float top = fabsf(norm);
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (lane == 0) sh.top[warp] = top;
   }
   __syncthreads();
-  {  // ---- keys: a thread has half a token
-    const int row = tid & 127, h = kh, t = kt;
+  {  // ---- keys: a thread has a quarter of a token
     float most = 0.0f;
     auto put = [&](int chunk, const float (&x)[8]) {  // (already divided by TI_KEY)
       uint32_t hi[4], lo[4];
@@ -204,16 +206,16 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         hi[i] = ti_pair(x[2 * i], x[2 * i + 1]);
         if (SPLIT) lo[i] = ti_rest(x[2 * i], x[2 * i + 1], hi[i]);
       }
-      *(uint4*)(sh.k[0] + chunk * TI_LBO + row * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      if (SPLIT) *(uint4*)(sh.k[SPLIT] + chunk * TI_LBO + row * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      *(uint4*)(sh.k[0] + chunk * TI_KLBO + krow * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      if (SPLIT) *(uint4*)(sh.k[SPLIT] + chunk * TI_KLBO + krow * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     };
-    if (t < sq.cold) {
+    if (kt < sq.cold) {
       const float* sc = (const float*)(kpage + g.scale_off);
       const float* mu = (const float*)(kpage + g.mean_off);
-      const uint32_t w[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+      const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int d = 64 * h + 8 * i;
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * kq + 8 * i;
         const float4 s0 = *(const float4*)(sc + d), s1 = *(const float4*)(sc + d + 4);
         const float4 m0 = *(const float4*)(mu + d), m1 = *(const float4*)(mu + d + 4);
         const float ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
@@ -223,22 +225,22 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = fmaf(ss[e], sh.grid[w[i] >> (4 * e) & 15], (mm[e] - zz[e]) * (1.0f / TI_KEY));
-        put(8 * h + i, x);
+        put(4 * kq + i, x);
       }
     } else {
-      const size_t at = ring + (size_t)(t % g.hot_cap) * TQ_D + 64 * h;
-#pragma unroll 4
-      for (int i = 0; i < 8; ++i) {
+      const size_t at = ring + (size_t)(kt % g.hot_cap) * TQ_D + 32 * kq;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
         float x[8];
-        if (t < t1) {
+        if (kt < t1) {
           ts_ld8(a.hot_k, at + 8 * i, g.kv_dtype, x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = (x[e] - sh.center[64 * h + 8 * i + e]) * (1.0f / TI_KEY);
+          for (int e = 0; e < 8; ++e) x[e] = (x[e] - sh.center[32 * kq + 8 * i + e]) * (1.0f / TI_KEY);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = 0.0f;
         }
-        put(8 * h + i, x);
+        put(4 * kq + i, x);
       }
     }
     odd |= !(most <= 65504.0f);
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         if (t < t0 || t >= t1) continue;
         const float x = (__half2float(val) - sh.center[ch]) * (1.0f / TI_KEY);
         odd |= !(fabsf(x) <= 65504.0f);
-        const int at = (ch >> 3) * TI_LBO + (t - t0) * 16 + (ch & 7) * 2;
+        const int at = (ch >> 3) * TI_KLBO + (t - t0) * 16 + (ch & 7) * 2;
         const __half hi = __float2half_rn(x);
         *(__half*)(sh.k[0] + at) = hi;
         if (SPLIT) *(__half*)(sh.k[SPLIT] + at) = __float2half_rn(x - __half2float(hi));
@@ -281,31 +283,28 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
   uint8_t* const v_hi = images + (SPLIT ? 2 : 1) * TI_IMAGE;
   uint8_t* const v_lo = v_hi + TI_IMAGE;
   if (!hot && S % TQ_GROUP_TOK == 0) {
-    // a warp expands the records of a group of 16 tokens: two tokens of a channel are a word of the image
-    const int t = t0 + warp * TQ_GROUP_TOK, b = t / S, slot = t - b * S, r = lane >> 2, c = lane & 3;
+    // two warps expand the records of a group of 16 tokens: two tokens of a channel are a word of the image
+    const int grp_i = warp >> 1, part = warp & 1, t = t0 + grp_i * TQ_GROUP_TOK, b = t / S, slot = t - b * S;
+    const int r = lane >> 2, c = lane & 3;
     const bool there = t < t1;
     const uint8_t* grp = pages + (size_t)(there ? b : 0) * g.page_bytes + g.v_off + (size_t)(there ? slot >> 4 : 0) * v_group_bytes(vb);
-    uint32_t w[9];
+    uint32_t w[4];  // pairs 16 part .. + 15
     if (vb == 4) {
-      const uint4 x = *(const uint4*)(grp + lane * 16), y = *(const uint4*)(grp + 512 + lane * 16);
-      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w, w[4] = y.x, w[5] = y.y, w[6] = y.z, w[7] = y.w;
+      const uint4 x = *(const uint4*)(grp + part * 512 + lane * 16);
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
     } else {
-#pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        const uint2 x = *(const uint2*)(grp + i * 256 + lane * 8);
-        w[2 * i] = x.x, w[2 * i + 1] = x.y;
-      }
-      w[6] = w[7] = 0u;
+      // the record's 24 bytes; these pairs are words 3 part .. + 2
+      const uint2 r0 = *(const uint2*)(grp + lane * 8), r1 = *(const uint2*)(grp + 256 + lane * 8), r2 = *(const uint2*)(grp + 512 + lane * 8);
+      w[0] = part ? r1.y : r0.x, w[1] = part ? r2.x : r0.y, w[2] = part ? r2.y : r1.x, w[3] = 0u;
     }
-    w[8] = 0u;
     float nv[2][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) nv[h][x] = there ? sh.norm[warp * TQ_GROUP_TOK + 8 * h + 2 * c + x] * up : 0.0f;
+      for (int x = 0; x < 2; ++x) nv[h][x] = there ? sh.norm[grp_i * TQ_GROUP_TOK + 8 * h + 2 * c + x] * up : 0.0f;
 #pragma unroll
-    for (int p = 0; p < 32; ++p) {
-      const int h = p & 1, d = r + 8 * (p >> 1);
+    for (int p = 0; p < 16; ++p) {
+      const int h = p & 1, d = r + 8 * (8 * part + (p >> 1));
       uint32_t ca, cb;
       if (vb == 4) {
         const uint32_t by = w[p >> 2] >> (8 * (p & 3));
@@ -316,13 +315,13 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
       }
       const float x = nv[h][0] * sh.cent[ca], y = nv[h][1] * sh.cent[cb];
       const uint32_t hi = ti_pair(x, y);
-      const int at = (2 * warp + h) * TI_LBO + d * 16 + 4 * c;
+      const int at = (2 * grp_i + h) * TI_LBO + d * 16 + 4 * c;
       *(uint32_t*)(v_hi + at) = hi;
       if (SPLIT) *(uint32_t*)(v_lo + at) = ti_rest(x, y, hi);
     }
     return;
   }
-  // Window tokens are rotated, v @ Pi^T, on mma.sync: 32 tokens at a time as pairs hi + lo are the B operand, a warp's 16
+  // Window tokens are rotated, v @ Pi^T, on mma.sync: 16 tokens at a time as pairs hi + lo are the B operand, a warp's 16
   // output channels, whose rows of Pi are pairs too, the A operand.  Tokens of blocks in the same tile come
   // from their codes one by one.
   uint8_t* const vs = sh.k[0];
@@ -336,9 +335,8 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
       for (int i = 0; i < 4; ++i) d[nt][i] = 0.0f;
     if (t0 + n0 + TS_VT > sq.cold && t0 + n0 < t1) {
       __syncthreads();  // (the keys, or the rows before, have been read)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int row = tid >> 3, ch = (tid & 7) * 16 + 8 * u, t = t0 + n0 + row;
+      if (tid < TS_VT * 16) {
+        const int row = tid >> 4, ch = (tid & 15) * 8, t = t0 + n0 + row;
         float v[8];
         if (t >= sq.cold && t < t1) {
           ts_ld8(a.hot_v, ring + (size_t)(t % g.hot_cap) * TQ_D + ch, g.kv_dtype, v);
@@ -356,6 +354,7 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         *(uint4*)(vs + (TS_VT + row) * TS_PITCH + 2 * ch) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
       __syncthreads();
+      if (warp < 8)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         uint32_t ph[4], pl[4];
@@ -376,6 +375,7 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         }
       }
     }
+    if (warp >= 8) continue;
 #pragma unroll
     for (int nt = 0; nt < TS_VT / 8; ++nt)
 #pragma unroll
@@ -402,9 +402,9 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
 
 // ---------------------------------------------------------------------------------------------------
 struct TiShared {
-  alignas(128) uint8_t q[2][TI_IMAGE];
+  alignas(128) uint8_t q[2][TI_QIMAGE];
   alignas(128) uint8_t kv[TI_SLOTS][TI_IMAGE];
-  unsigned long long full[TI_SLOTS], empty[TI_SLOTS], q_ready, s_full[2], p_full[2], o_done[2];
+  unsigned long long full[TI_SLOTS], empty[TI_SLOTS], q_ready[2], s_full[2], s_read[2], p_full[2], o_done[2];
   uint32_t tmem;
   float pair[2][2][128];  // what the two threads of a row tell each other
 };
@@ -448,13 +448,6 @@ TQ_DEV void ti_ld32(uint32_t addr, uint32_t* r) {
       : "r"(addr)
       : "memory");
 }
-TQ_DEV void ti_st32(uint32_t addr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-      TI_R8(r, 0), TI_R8(r, 8), TI_R8(r, 16), TI_R8(r, 24)
-      : "memory");
-}
 TQ_DEV void ti_ld16(uint32_t addr, uint32_t* r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                : TI_W8(r, 0), TI_W8(r, 8)
@@ -464,6 +457,13 @@ TQ_DEV void ti_ld16(uint32_t addr, uint32_t* r) {
 TQ_DEV void ti_st16(uint32_t addr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
                TI_R8(r, 0), TI_R8(r, 8)
+               : "memory");
+}
+TQ_DEV void ti_ld8(uint32_t addr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : TI_W8(r, 0) : "r"(addr) : "memory");
+}
+TQ_DEV void ti_st4(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
                : "memory");
 }
 TQ_DEV float ti_max3(float a, float b, float c) {
@@ -543,18 +543,18 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
   const int k_lo = (int)((long)tl.count() * split / ta.splits), n = (int)((long)tl.count() * (split + 1) / ta.splits) - k_lo;
   const int groups = a.rows - row0 > 128 ? 2 : 1;  // halves of the rows that there are
 
-  const uint32_t q_bar = enc_smem(&sh.q_ready);
   if (tid == 0) {
     for (int i = 0; i < TI_SLOTS; ++i) {
       mbar_init(enc_smem(&sh.full[i]), 1);
-      mbar_init(enc_smem(&sh.empty[i]), 1);
+      mbar_init(enc_smem(&sh.empty[i]), groups);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(enc_smem(&sh.s_full[i]), 1);
+      mbar_init(enc_smem(&sh.q_ready[i]), 256);
+      mbar_init(enc_smem(&sh.s_read[i]), 256);
       mbar_init(enc_smem(&sh.p_full[i]), 256);
       mbar_init(enc_smem(&sh.o_done[i]), 1);
     }
-    mbar_init(q_bar, 256 * groups);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == TI_SOFTMAX / 32) {
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       }
   };
 
-  if (warp == TI_SOFTMAX / 32 + 1) {
+  if (warp == TI_SOFTMAX / 32 + 2) {
     // ---- loads: K V of tile after tile through the ring
     if (lane == 0) {
       const uint8_t* images = ta.images + (size_t)unit * ta.cap * 2 * PARTS * TI_IMAGE;
@@ -603,101 +603,94 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       gave_up = false;
       for (int i = max(c - TI_SLOTS, 0); i < c; ++i) wait(&sh.full[i % TI_SLOTS], (i / TI_SLOTS) & 1);
     }
-  } else if (warp == TI_SOFTMAX / 32) {
-    // ---- products
+  } else if (warp >= TI_SOFTMAX / 32) {
+    // ---- products of half x
     // The whole warp runs this, one thread issues.  What the products take are constants or the same in all lanes to
     // the compiler's knowledge (the shuffle), so that it lies in uniform registers: fetched there product by product,
     // each took about a hundred cycles to issue, more than its execution.
-    const int n_u = __shfl_sync(0xffffffffu, n, 0), groups_u = __shfl_sync(0xffffffffu, groups, 0);
+    const int x = warp - TI_SOFTMAX / 32, n_u = __shfl_sync(0xffffffffu, x < groups ? n : 0, 0);
     if (n_u > 0) {
-      constexpr uint32_t idesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-      constexpr uint64_t STEP = 2 * TI_LBO >> 4;  // 16 deep
-      const uint64_t q0 = umma_desc_k_major(enc_smem(sh.q[0]), TI_LBO, TI_SBO);
-      const uint64_t kv0 = umma_desc_k_major(enc_smem(sh.kv[0]), TI_LBO, TI_SBO);
-      auto image = [&](int c) { return kv0 + (uint64_t)((uint32_t)(c % TI_SLOTS) * (TI_IMAGE >> 4)); };
+      constexpr uint32_t s_desc = (1u << 4) | ((uint32_t)(TI_T >> 3) << 17) | ((128u >> 4) << 24);
+      constexpr uint32_t o_desc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+      constexpr uint64_t KSTEP = 2 * TI_KLBO >> 4, STEP = 2 * TI_LBO >> 4;  // 16 deep
+      const uint64_t q = umma_desc_k_major(enc_smem(sh.q[0]), TI_LBO, TI_SBO) + (uint64_t)(x * (TI_QIMAGE >> 4));
+      const uint64_t k0 = umma_desc_k_major(enc_smem(sh.kv[0]), TI_KLBO, TI_SBO);
+      const uint64_t v0 = umma_desc_k_major(enc_smem(sh.kv[0]), TI_LBO, TI_SBO);
+      const uint32_t ds = tmem + TI_S + TI_HALF * x, dp = tmem + TI_P + TI_HALF * x, d_o = tmem + TI_O + 128 * x;
+      auto image = [&](int c) { return (uint64_t)((uint32_t)(c % TI_SLOTS) * (TI_IMAGE >> 4)); };
       auto wait_all = [&](unsigned long long* bar, unsigned parity) {  // (the warp stays together)
         wait(bar, parity);
         gave_up = __any_sync(0xffffffffu, gave_up);
       };
       auto landed = [&](int c) { wait_all(&sh.full[c % TI_SLOTS], (c / TI_SLOTS) & 1); };
-      // scores of half x against the keys of tile k
-      auto scores = [&](int x, int k) {
+      auto release = [&](int c) {  // an operand's parts, once the products issued so far are done (the issuing thread)
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) umma_commit(enc_smem(&sh.empty[(c + i) % TI_SLOTS]));
+      };
+      // scores against the keys of tile k
+      auto scores = [&](int k) {
+        const int c = 2 * PARTS * k;
         uint64_t b[PARTS];
 #pragma unroll
-        for (int i = 0; i < PARTS; ++i) b[i] = image(2 * PARTS * k + i);
+        for (int i = 0; i < PARTS; ++i) b[i] = k0 + image(c + i);
         if (ti_elect()) {
-          const uint64_t q = q0 + (uint64_t)(x * (TI_IMAGE >> 4));
-          const uint32_t d = tmem + 128 * x;
-          ti_mma<false>(d, q, b[PARTS - 1], idesc);
+          ti_mma<false>(ds, q, b[PARTS - 1], s_desc);
 #pragma unroll
-          for (int j = 1; j < 8; ++j) ti_mma<true>(d, q + j * STEP, b[PARTS - 1] + j * STEP, idesc);
+          for (int j = 1; j < 8; ++j) ti_mma<true>(ds, q + j * STEP, b[PARTS - 1] + j * KSTEP, s_desc);
           if (SPLIT)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ti_mma<true>(d, q + j * STEP, b[0] + j * STEP, idesc);
+            for (int j = 0; j < 8; ++j) ti_mma<true>(ds, q + j * STEP, b[0] + j * KSTEP, s_desc);
           umma_commit(enc_smem(&sh.s_full[x]));
+          release(c);
         }
         __syncwarp();
       };
-      auto release = [&](int c) {  // the parts of an operand, once the products issued so far are done
-        if (ti_elect())
-#pragma unroll
-          for (int i = 0; i < PARTS; ++i) umma_commit(enc_smem(&sh.empty[(c + i) % TI_SLOTS]));
-        __syncwarp();
-      };
-      // O += P V, the tile's values in chunk c
-      auto values = [&](int x, int c, bool fresh) {
+      // O += P V
+      auto values = [&](int k) {
+        const int c = 2 * PARTS * k + PARTS;
         uint64_t b[PARTS];
 #pragma unroll
-        for (int i = 0; i < PARTS; ++i) b[i] = image(c + i);
+        for (int i = 0; i < PARTS; ++i) b[i] = v0 + image(c + i);
         if (ti_elect()) {
-          const uint32_t d = tmem + 256 + 128 * x, p = tmem + 128 * x;
-          if (fresh) ti_mma_ts<false>(d, p, b[PARTS - 1], idesc);
-          else ti_mma_ts<true>(d, p, b[PARTS - 1], idesc);
+          if (k == 0) ti_mma_ts<false>(d_o, dp, b[PARTS - 1], o_desc);
+          else ti_mma_ts<true>(d_o, dp, b[PARTS - 1], o_desc);
 #pragma unroll
-          for (int j = 1; j < 8; ++j) ti_mma_ts<true>(d, p + 8 * j, b[PARTS - 1] + j * STEP, idesc);
+          for (int j = 1; j < TI_T / 16; ++j) ti_mma_ts<true>(d_o, dp + 8 * j, b[PARTS - 1] + j * STEP, o_desc);
           if (SPLIT)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ti_mma_ts<true>(d, p + 8 * j, b[0] + j * STEP, idesc);
+            for (int j = 0; j < TI_T / 16; ++j) ti_mma_ts<true>(d_o, dp + 8 * j, b[0] + j * STEP, o_desc);
           umma_commit(enc_smem(&sh.o_done[x]));
+          release(c);
         }
         __syncwarp();
       };
-      wait_all(&sh.q_ready, 0);
+      wait_all(&sh.q_ready[x], 0);
       for (int i = 0; i < PARTS; ++i) landed(i);
       ti_fence_after();
-      scores(0, 0);
-      if (groups_u > 1) scores(1, 0);
-      release(0);
+      scores(0);
 #pragma unroll 1
       for (int k = 0; k < n_u; ++k) {
-        const int cv = 2 * PARTS * k + PARTS, ck = cv + PARTS;  // values of this tile, keys of the next
-        for (int i = 0; i < PARTS; ++i) landed(cv + i);
-        if (k + 1 < n_u)
-          for (int i = 0; i < PARTS; ++i) landed(ck + i);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (x >= groups_u) break;
-          wait_all(&sh.p_full[x], k & 1);
+        if (k + 1 < n_u) {
+          for (int i = 0; i < PARTS; ++i) landed(2 * PARTS * (k + 1) + i);
+          wait_all(&sh.s_read[x], k & 1);  // (this tile's scores are in registers)
           ti_fence_after();
-          values(x, cv, k == 0);
-          if (x == groups_u - 1) release(cv);
-          if (k + 1 < n_u) {
-            // the next scores take the place of the probabilities that these products read
-            wait_all(&sh.o_done[x], k & 1);
-            scores(x, k + 1);
-          }
+          scores(k + 1);
         }
-        if (k + 1 < n_u) release(ck);
+        for (int i = 0; i < PARTS; ++i) landed(2 * PARTS * k + PARTS + i);
+        wait_all(&sh.p_full[x], k & 1);
+        ti_fence_after();
+        values(k);
       }
       gave_up = false;  // (nor are products under way when the CTA's memory goes)
-      for (int x = 0; x < groups_u; ++x) wait_all(&sh.o_done[x], (n_u - 1) & 1);
+      wait_all(&sh.o_done[x], (n_u - 1) & 1);
     }
   } else if (warp < 8 * groups) {
-    // ---- two threads per row: 64 tokens of a tile, and 64 channels of the sums, each
+    // ---- two threads per row: 40 tokens of a tile, and 64 channels of the sums, each
     const int x = warp >> 3, part = warp >> 2 & 1, r = tid & 127, row = row0 + 128 * x + r;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    const uint32_t ts = tmem + 128 * x + lanes + 64 * part, tp = tmem + 128 * x + lanes + 32 * part;
-    const uint32_t to = tmem + 256 + 128 * x + lanes + 64 * part;
+    constexpr int HT = TI_T / 2;  // a thread's tokens of a tile
+    const uint32_t ts = tmem + TI_S + TI_HALF * x + lanes + HT * part, tp = tmem + TI_P + TI_HALF * x + lanes + HT / 2 * part;
+    const uint32_t to = tmem + TI_O + 128 * x + lanes + 64 * part;
     // the larger of the two threads' values (NaN: the other's)
     auto of_both = [&](float v) {
       sh.pair[x][part][r] = v;
@@ -743,7 +736,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
         *(uint4*)(sh.q[x] + (8 * part + i) * TI_LBO + r * 16) = make_uint4(h[0], h[1], h[2], h[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(q_bar);
+      mbar_arrive(enc_smem(&sh.q_ready[x]));
       asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");  // (the pairs have been read)
     }
     const int p = row < a.rows ? attend_position(a, sq, row) : -1, w = attend_window(a, p);
@@ -757,20 +750,22 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       wait(&sh.s_full[x], k & 1);
       gave_up = __any_sync(0xffffffffu, gave_up);
       ti_fence_after();
-      uint32_t v[64];
+      uint32_t v[HT];
       ti_ld32(ts, v);
-      ti_ld32(ts + 32, v + 32);
+      ti_ld8(ts + 32, v + 32);
       ti_wait_ld();
+      ti_fence_before();
+      mbar_arrive(enc_smem(&sh.s_read[x]));
       const bool open = whole && t0 + TI_T - 1 <= p_lo && (t0 >= w_hi || t0 + TI_T <= a.sinks);
       if (!open) {
-        const int c0 = t0 + 64 * part, hi = min(p, sq.n - 1) - c0, lo = w - c0, sk = a.sinks - c0;
+        const int c0 = t0 + HT * part, hi = min(p, sq.n - 1) - c0, lo = w - c0, sk = a.sinks - c0;
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
+        for (int i = 0; i < HT; ++i)
           if (i > hi || (i < lo && i >= sk)) v[i] = 0xff800000u;
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < 64; i += 2)
+      for (int i = 0; i < HT; i += 2)
         top[i / 2 & 3] = ti_max3(top[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
       const float now = fmaf(of_both(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), factor, e);
       const bool grown = now > m + TI_GROW;  // (also from -inf)
@@ -779,7 +774,8 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
         down = tq_exp2(m - now);
         m = now;
       }
-      if (k > 0 && __any_sync(0xffffffffu, grown)) {
+      const bool rescaled = k > 0 && __any_sync(0xffffffffu, grown);
+      if (rescaled) {
         wait(&sh.o_done[x], (k - 1) & 1);
         gave_up = __any_sync(0xffffffffu, gave_up);
         ti_fence_after();
@@ -796,10 +792,10 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       const float off = TI_LIFT + e - (m > -INFINITY ? m : 0.0f);
       const uint64_t factor2 = ti_f2(factor, factor), off2 = ti_f2(off, off);
       uint64_t sum[2] = {0ull, 0ull};
-      uint32_t h[32];
+      uint32_t h[HT / 2];
       if (open) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < HT / 2; ++j) {
           const uint64_t y = ti_fma2(ti_u2(v[2 * j], v[2 * j + 1]), factor2, off2);
           const float2 z = j % 8 < TI_POLY ? ti_exp2_poly(y) : ti_exp2_unit(y);
           sum[j & 1] = ti_add2(sum[j & 1], ti_f2(z.x, z.y));
@@ -807,15 +803,19 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int j = 0; j < HT / 2; ++j) {
           const float2 z = ti_exp2_unit(ti_fma2(ti_u2(v[2 * j], v[2 * j + 1]), factor2, off2));
           sum[j & 1] = ti_add2(sum[j & 1], ti_f2(z.x, z.y));
           h[j] = ti_pair(z.x, z.y);
         }
       }
-      // (the probabilities go over the first half of the scores' columns, which the other thread of the row may still
-      // be reading: its loads are over when it has told its maximum)
-      ti_st32(tp, h);
+      if (k > 0 && !rescaled) {  // (the probabilities before have been used)
+        wait(&sh.o_done[x], (k - 1) & 1);
+        gave_up = __any_sync(0xffffffffu, gave_up);
+        ti_fence_after();
+      }
+      ti_st16(tp, h);
+      ti_st4(tp + 16, h + 16);
       ti_wait_st();
       ti_fence_before();
       mbar_arrive(enc_smem(&sh.p_full[x]));
