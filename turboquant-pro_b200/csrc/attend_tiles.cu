@@ -13,7 +13,7 @@
 //     What is not a number, or too large even so, sets the flag of its (sequence, KV head), which the general kernel
 //     then does.
 // attend_tiles_kernel   256 rows of a (sequence, KV head) per CTA against a split of these tiles, in two halves of 128 rows.
-//     S = Q K^T into tensor memory; a group of 256 threads per half, two threads per row, makes the probabilities and
+//     S = Q K^T into tensor memory; a group of 128 threads per half, a thread per row, makes the probabilities and
 //     puts them back as fp16; O += P V with P as the operand in tensor memory.  Of its 512 columns a half has
 //     80 for scores, 40 for probabilities and 128 for the sums: that is what sets the tile.  (With 128 tokens the
 //     probabilities had to go over the scores, so that the next scores waited for the product that read them: a chain of
@@ -39,7 +39,7 @@ constexpr int TI_IMAGE = TI_T * TQ_D * 2;    // bytes of an operand image of key
 constexpr int TI_QIMAGE = 128 * TQ_D * 2;    // and of a half's queries
 constexpr int TI_KLBO = TI_T * 16, TI_LBO = TQ_D * 16, TI_SBO = 128;  // from eight K to the next: keys; queries, values
 constexpr int TI_SLOTS = 8;                  // images in shared memory
-constexpr int TI_SOFTMAX = 512;              // softmax threads: two a row
+constexpr int TI_SOFTMAX = 256;              // softmax threads: one a row
 constexpr int TI_THREADS = TI_SOFTMAX + 96;  // and two warps that issue, a warp that loads
 constexpr int TI_S = 0, TI_P = TI_T, TI_HALF = 128, TI_O = 256;  // columns: scores, probabilities of a half, sums
 constexpr float TI_KEY = 16.0f;              // keys are divided by it
@@ -406,7 +406,6 @@ struct TiShared {
   alignas(128) uint8_t kv[TI_SLOTS][TI_IMAGE];
   unsigned long long full[TI_SLOTS], empty[TI_SLOTS], q_ready[2], s_full[2], s_read[2], p_full[2], o_done[2];
   uint32_t tmem;
-  float pair[2][2][128];  // what the two threads of a row tell each other
 };
 static_assert(sizeof(TiShared) <= 227 * 1024, "shared memory of one CTA");
 
@@ -454,17 +453,15 @@ TQ_DEV void ti_ld16(uint32_t addr, uint32_t* r) {
                : "r"(addr)
                : "memory");
 }
-TQ_DEV void ti_st16(uint32_t addr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
-               TI_R8(r, 0), TI_R8(r, 8)
-               : "memory");
+TQ_DEV void ti_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      TI_R8(r, 0), TI_R8(r, 8), TI_R8(r, 16), TI_R8(r, 24)
+      : "memory");
 }
-TQ_DEV void ti_ld8(uint32_t addr, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : TI_W8(r, 0) : "r"(addr) : "memory");
-}
-TQ_DEV void ti_st4(uint32_t addr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
-               : "memory");
+TQ_DEV void ti_st8(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), TI_R8(r, 0) : "memory");
 }
 TQ_DEV float ti_max3(float a, float b, float c) {
   float y;
@@ -550,9 +547,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(enc_smem(&sh.s_full[i]), 1);
-      mbar_init(enc_smem(&sh.q_ready[i]), 256);
-      mbar_init(enc_smem(&sh.s_read[i]), 256);
-      mbar_init(enc_smem(&sh.p_full[i]), 256);
+      mbar_init(enc_smem(&sh.q_ready[i]), 128);
+      mbar_init(enc_smem(&sh.s_read[i]), 128);
+      mbar_init(enc_smem(&sh.p_full[i]), 128);
       mbar_init(enc_smem(&sh.o_done[i]), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -684,36 +681,32 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       gave_up = false;  // (nor are products under way when the CTA's memory goes)
       wait_all(&sh.o_done[x], (n_u - 1) & 1);
     }
-  } else if (warp < 8 * groups) {
-    // ---- two threads per row: 40 tokens of a tile, and 64 channels of the sums, each
-    const int x = warp >> 3, part = warp >> 2 & 1, r = tid & 127, row = row0 + 128 * x + r;
+  } else if (warp < 4 * groups) {
+    // ---- a thread per row
+    const int x = warp >> 2, r = tid & 127, row = row0 + 128 * x + r;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-    constexpr int HT = TI_T / 2;  // a thread's tokens of a tile
-    const uint32_t ts = tmem + TI_S + TI_HALF * x + lanes + HT * part, tp = tmem + TI_P + TI_HALF * x + lanes + HT / 2 * part;
-    const uint32_t to = tmem + TI_O + 128 * x + lanes + 64 * part;
-    // the larger of the two threads' values (NaN: the other's)
-    auto of_both = [&](float v) {
-      sh.pair[x][part][r] = v;
-      ti_fence_before();
-      asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");
+    const uint32_t ts = tmem + TI_S + TI_HALF * x + lanes, tp = tmem + TI_P + TI_HALF * x + lanes;
+    const uint32_t to = tmem + TI_O + 128 * x + lanes;
+    auto settled = [&](unsigned long long* bar, unsigned parity) {
+      wait(bar, parity);
+      __syncwarp();
       ti_fence_after();
-      return fmaxf(v, sh.pair[x][part ^ 1][r]);
     };
     float factor;
     {
-      uint4 raw[8];
+      uint4 raw[16];
       const bool there = row < a.rows;
       const uint16_t* q = (const uint16_t*)a.q + ((int64_t)s * a.q_seq + (int64_t)(row / G) * a.q_tok +
-                                                  (int64_t)(head * G + row % G) * a.q_head) + 64 * part;
+                                                  (int64_t)(head * G + row % G) * a.q_head);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) raw[i] = there ? *(const uint4*)(q + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
+      for (int i = 0; i < 16; ++i) raw[i] = there ? *(const uint4*)(q + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
       auto pair = [&](uint32_t w) -> float2 {
         if (SPLIT) return __half22float2(*(const __half2*)&w);
         return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
       };
       float top = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 16; ++i) {
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -722,10 +715,10 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
         }
       }
       float exponent;
-      const float up = ti_lift(of_both(top), 13, exponent);
+      const float up = ti_lift(top, 13, exponent);
       factor = tq_scaled<true>(TI_KEY * exp2f(exponent));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 16; ++i) {
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
         uint32_t h[4];
 #pragma unroll
@@ -733,41 +726,52 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
           const float2 f = pair(w[j]);
           h[j] = ti_pair(f.x * up, f.y * up);
         }
-        *(uint4*)(sh.q[x] + (8 * part + i) * TI_LBO + r * 16) = make_uint4(h[0], h[1], h[2], h[3]);
+        *(uint4*)(sh.q[x] + i * TI_LBO + r * 16) = make_uint4(h[0], h[1], h[2], h[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(enc_smem(&sh.q_ready[x]));
-      asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");  // (the pairs have been read)
     }
     const int p = row < a.rows ? attend_position(a, sq, row) : -1, w = attend_window(a, p);
     // whether all rows of this CTA see a tile goes by their earliest position and latest window
     const bool whole = row0 + TI_ROWS <= a.rows && i_lo < sq.q_n && (row0 + TI_ROWS - 1) / G < sq.q_n && p_lo >= 0;
     const int w_hi = attend_window(a, max(p_hi, 0));
+    const float* const exponents = ta.exponent + (size_t)unit * ta.cap;
+    auto tile_of = [&](int k) { return tl.at(k_lo + min(k, n - 1)); };
+    auto exponent_of = [&](int t) { return exponents[t < ul.head ? t : ul.head + t - ul.first]; };
     float m = -INFINITY, l = 0.0f;
+    int t = n > 0 ? tile_of(0) : 0;
+    float e = n > 0 ? exponent_of(t) : 0.0f;
+    if (groups == 2 && x == 1 && n > 0) asm volatile("bar.arrive 1, 256;" ::: "memory");
     for (int k = 0; k < n; ++k) {
-      const int t = tl.at(k_lo + k), t0 = t * TI_T;
-      const float e = ta.exponent[(size_t)unit * ta.cap + (t < ul.head ? t : ul.head + t - ul.first)];
-      wait(&sh.s_full[x], k & 1);
-      gave_up = __any_sync(0xffffffffu, gave_up);
-      ti_fence_after();
-      uint32_t v[HT];
+      const int t0 = t * TI_T;
+      // (the next tile's exponent, on its way from memory while this one is done)
+      const int t_next = tile_of(k + 1);
+      const float e_next = exponent_of(t_next);
+      settled(&sh.s_full[x], k & 1);
+      uint32_t v[TI_T];
       ti_ld32(ts, v);
-      ti_ld8(ts + 32, v + 32);
+      ti_ld32(ts + 32, v + 32);
+      ti_ld16(ts + 64, v + 64);
       ti_wait_ld();
       ti_fence_before();
       mbar_arrive(enc_smem(&sh.s_read[x]));
       const bool open = whole && t0 + TI_T - 1 <= p_lo && (t0 >= w_hi || t0 + TI_T <= a.sinks);
       if (!open) {
-        const int c0 = t0 + HT * part, hi = min(p, sq.n - 1) - c0, lo = w - c0, sk = a.sinks - c0;
+        const int hi = min(p, sq.n - 1) - t0, lo = w - t0, sk = a.sinks - t0;
 #pragma unroll
-        for (int i = 0; i < HT; ++i)
+        for (int i = 0; i < TI_T; ++i)
           if (i > hi || (i < lo && i >= sk)) v[i] = 0xff800000u;
       }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float top[8];
 #pragma unroll
-      for (int i = 0; i < HT; i += 2)
-        top[i / 2 & 3] = ti_max3(top[i / 2 & 3], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-      const float now = fmaf(of_both(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), factor, e);
+      for (int i = 0; i < 8; ++i) top[i] = fmaxf(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+#pragma unroll
+      for (int i = 16; i < TI_T; i += 2)
+        top[i / 2 & 7] = ti_max3(top[i / 2 & 7], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+      top[0] = ti_max3(top[0], top[1], top[2]);
+      top[3] = ti_max3(top[3], top[4], top[5]);
+      top[0] = ti_max3(ti_max3(top[0], top[3], top[6]), top[7], -INFINITY);
+      const float now = fmaf(top[0], factor, e);
       const bool grown = now > m + TI_GROW;  // (also from -inf)
       float down = 1.0f;
       if (grown) {
@@ -776,26 +780,29 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       }
       const bool rescaled = k > 0 && __any_sync(0xffffffffu, grown);
       if (rescaled) {
-        wait(&sh.o_done[x], (k - 1) & 1);
-        gave_up = __any_sync(0xffffffffu, gave_up);
-        ti_fence_after();
+        settled(&sh.o_done[x], (k - 1) & 1);
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {
-          uint32_t o[16];
-          ti_ld16(to + 16 * i, o);
+          uint32_t o[32];
+          ti_ld32(to + 32 * i, o);
           ti_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * down);
-          ti_st16(to + 16 * i, o);
+          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * down);
+          ti_st32(to + 32 * i, o);
         }
       }
+      if (k > 0 && !rescaled) settled(&sh.o_done[x], (k - 1) & 1);  // (the probabilities before have been used)
+      // The halves take turns at their exponentials, which fill the unit for them (16 a cycle and SM): while one is at
+      // them, the other waits for its scores, fetches them and finds their largest.  Left to themselves both did the
+      // same at the same time (950 us for 2048 tokens on 32768; with turns 907).
+      if (groups == 2) asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");
       const float off = TI_LIFT + e - (m > -INFINITY ? m : 0.0f);
       const uint64_t factor2 = ti_f2(factor, factor), off2 = ti_f2(off, off);
       uint64_t sum[2] = {0ull, 0ull};
-      uint32_t h[HT / 2];
+      uint32_t h[TI_T / 2];
       if (open) {
 #pragma unroll
-        for (int j = 0; j < HT / 2; ++j) {
+        for (int j = 0; j < TI_T / 2; ++j) {
           const uint64_t y = ti_fma2(ti_u2(v[2 * j], v[2 * j + 1]), factor2, off2);
           const float2 z = j % 8 < TI_POLY ? ti_exp2_poly(y) : ti_exp2_unit(y);
           sum[j & 1] = ti_add2(sum[j & 1], ti_f2(z.x, z.y));
@@ -803,43 +810,32 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < HT / 2; ++j) {
+        for (int j = 0; j < TI_T / 2; ++j) {
           const float2 z = ti_exp2_unit(ti_fma2(ti_u2(v[2 * j], v[2 * j + 1]), factor2, off2));
           sum[j & 1] = ti_add2(sum[j & 1], ti_f2(z.x, z.y));
           h[j] = ti_pair(z.x, z.y);
         }
       }
-      if (k > 0 && !rescaled) {  // (the probabilities before have been used)
-        wait(&sh.o_done[x], (k - 1) & 1);
-        gave_up = __any_sync(0xffffffffu, gave_up);
-        ti_fence_after();
-      }
-      ti_st16(tp, h);
-      ti_st4(tp + 16, h + 16);
+      ti_st32(tp, h);
+      ti_st8(tp + 32, h + 32);
+      if (groups == 2 && (x == 0 || k + 1 < n)) asm volatile("bar.arrive %0, 256;" ::"r"(2 - x) : "memory");
       ti_wait_st();
       ti_fence_before();
       mbar_arrive(enc_smem(&sh.p_full[x]));
       const float2 s2 = ti_floats(ti_add2(sum[0], sum[1]));
       l = fmaf(s2.x + s2.y, exp2f(-e), l * down);
+      t = t_next, e = e_next;
     }
     // the row's state: [channel][row], neighbouring threads side by side
     const size_t at = ((size_t)unit * ta.splits + split) * ta.row_tiles + rt;
-    asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");  // (the last maxima have been read)
-    sh.pair[x][part][r] = l;
-    asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");
-    if (part == 0) {
-      float* stats = ta.stats + at * 2 * TI_ROWS + 128 * x + r;
-      stats[0] = n > 0 ? m - TI_LIFT : -INFINITY;
-      stats[TI_ROWS] = sh.pair[x][0][r] + sh.pair[x][1][r];
-    }
+    float* stats = ta.stats + at * 2 * TI_ROWS + 128 * x + r;
+    stats[0] = n > 0 ? m - TI_LIFT : -INFINITY;
+    stats[TI_ROWS] = l;
     if (n > 0) {
-      wait(&sh.o_done[x], (n - 1) & 1);
-      gave_up = __any_sync(0xffffffffu, gave_up);
-      ti_fence_after();
-      float* sums = ta.sums + (size_t)unit * a.unit_stride +
-                    (((size_t)split * ta.row_tiles + rt) * TQ_D + 64 * part) * TI_ROWS + 128 * x + r;
+      settled(&sh.o_done[x], (n - 1) & 1);
+      float* sums = ta.sums + (size_t)unit * a.unit_stride + ((size_t)split * ta.row_tiles + rt) * TQ_D * TI_ROWS + 128 * x + r;
 #pragma unroll 1
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 4; ++i) {
         uint32_t o[32];
         ti_ld32(to + 32 * i, o);
         ti_wait_ld();
