@@ -856,26 +856,38 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
 // ---------------------------------------------------------------------------------------------------
 // The splits' sums in order, over the sum of the weights, times Pi.  CTAs take tiles of 64 rows in turn.  The
 // merged rows go to shared memory as fp16 pairs hi + lo, each row scaled by a power of two, and through mma.sync as the
-// B operand against Pi^T, whose pairs a warp keeps in registers (16 channels of the output each): hi * hi + hi * lo +
-// lo * hi, good to 2^-22.  Bound by reading the sums.
-constexpr int TC_ROWS = 64, TC_THREADS = 256, TC_PITCH = TQ_D * 2 + 16;
-
-
+// B operand against Pi^T, whose pairs lie there too, a warp taking 16 channels of the output: hi * hi + hi * lo +
+// lo * hi, good to 2^-22, with an accumulator each.
+constexpr int TC_ROWS = 64, TC_THREADS = 256;
+struct CombineShared {
+  alignas(128) uint8_t ph[TQ_D * 256], pl[TQ_D * 256], hi[TC_ROWS * 256], lo[TC_ROWS * 256];
+  float top[TC_THREADS / 32][TC_ROWS], inv[TC_ROWS];
+};
+// Byte of eight neighbouring columns of a row: neither eight rows in a row nor every fourth of 32 share a bank.
+TQ_DEV int tc_at(int row, int c8) { return row * 256 + ((c8 ^ (row >> 2 & 7) ^ (row & 3) << 1) << 4); }
+TQ_DEV void tc_ldmatrix(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
 __global__ void __launch_bounds__(TC_THREADS, 2) attend_tiles_combine_kernel(AttendArgs a, TileArgs ta, int tiles, int total) {
-  __shared__ __align__(16) uint8_t hi[TC_ROWS * TC_PITCH], lo[TC_ROWS * TC_PITCH];
-  __shared__ float top_s[4][TC_ROWS], inv_s[TC_ROWS];
+  extern __shared__ __align__(128) uint8_t tc_smem[];
+  CombineShared& sh = *(CombineShared*)tc_smem;
   const tq_geom& g = a.g;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, q = lane >> 2, c = lane & 3;
   const int H = g.n_kv_heads, G = g.group;
-  uint32_t ph[8][4], pl[8][4];  // A: rows = output channels 16 warp .., k = input channels
+  for (int i = tid; i < TQ_D * 16; i += TC_THREADS) {  // (read behind the tile's first barrier)
+    const int row = i >> 4, c8 = i & 15;
+    const float4 u = *(const float4*)&a.tables->pi_t[row * TQ_D + 8 * c8], v = *(const float4*)&a.tables->pi_t[row * TQ_D + 8 * c8 + 4];
+    const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    uint32_t h[4], l[4];
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 x = *(const float2*)&a.tables->pi_t[(16 * warp + q + 8 * (i & 1)) * TQ_D + 16 * k + 2 * c + 8 * (i >> 1)];
-      ph[k][i] = ti_pair(x.x * 256.0f, x.y * 256.0f);
-      pl[k][i] = ti_rest(x.x * 256.0f, x.y * 256.0f, ph[k][i]);
+    for (int k = 0; k < 4; ++k) {
+      h[k] = ti_pair(x[2 * k] * 256.0f, x[2 * k + 1] * 256.0f);
+      l[k] = ti_rest(x[2 * k] * 256.0f, x[2 * k + 1] * 256.0f, h[k]);
     }
+    *(uint4*)(sh.ph + tc_at(row, c8)) = make_uint4(h[0], h[1], h[2], h[3]);
+    *(uint4*)(sh.pl + tc_at(row, c8)) = make_uint4(l[0], l[1], l[2], l[3]);
+  }
   for (int item = blockIdx.x; item < total; item += gridDim.x) {
     const int unit = item / tiles, row0 = item % tiles * TC_ROWS, s = unit / H, head = unit % H;
     const int rows = min(TC_ROWS, a.rows - row0);
@@ -901,66 +913,97 @@ __global__ void __launch_bounds__(TC_THREADS, 2) attend_tiles_combine_kernel(Att
       }
       continue;
     }
-    const int rt = row0 / TI_ROWS, in = row0 % TI_ROWS;
-    constexpr int N = TQ_D * TC_ROWS / TC_THREADS;  // channels of a thread
-    const int r = tid % TC_ROWS, part = tid / TC_ROWS;
-    float x[N], L = 0.0f, M = -INFINITY;
+    // a thread: eight channels of four rows
+    const int rt = row0 / TI_ROWS, in = row0 % TI_ROWS, r4 = tid % 16 * 4, c8 = tid / 16;
+    float x[4][8], L[4] = {0.0f, 0.0f, 0.0f, 0.0f}, M[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = 0.0f;
-    if (r < rows) {
-      const float* stats = ta.stats + ((size_t)unit * ta.splits * ta.row_tiles + rt) * 2 * TI_ROWS + in + r;
-      const size_t step = (size_t)ta.row_tiles * 2 * TI_ROWS;
-      const float* sums = ta.sums + (size_t)unit * a.unit_stride + ((size_t)rt * TQ_D + part * N) * TI_ROWS + in + r;
-      for (int i = 0; i < ta.splits; ++i) M = fmaxf(M, stats[i * step]);
-      const float by = M > -INFINITY ? M : 0.0f;
-      for (int i = 0; i < ta.splits; ++i) {
-        const float mi = stats[i * step], li = stats[i * step + TI_ROWS];
-        if (li == 0.0f) continue;
-        const float w = mi > -INFINITY ? tq_exp2(mi - by) : 1.0f;
-        L += li * w;
-        const float* from = sums + (size_t)i * ta.row_tiles * TI_ROWS * TQ_D;
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int k = 0; k < N; ++k) x[k] = fmaf(from[k * TI_ROWS], w, x[k]);
+      for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
+    const float* stats = ta.stats + ((size_t)unit * ta.splits * ta.row_tiles + rt) * 2 * TI_ROWS + in + r4;
+    const size_t step = (size_t)ta.row_tiles * 2 * TI_ROWS;
+    const float* sums = ta.sums + (size_t)unit * a.unit_stride + ((size_t)rt * TQ_D + c8 * 8) * TI_ROWS + in + r4;
+    for (int i = 0; i < ta.splits; ++i) {
+      const float4 m = *(const float4*)(stats + i * step);
+      M[0] = fmaxf(M[0], m.x), M[1] = fmaxf(M[1], m.y), M[2] = fmaxf(M[2], m.z), M[3] = fmaxf(M[3], m.w);
+    }
+#pragma unroll 2
+    for (int i = 0; i < ta.splits; ++i) {
+      const float4 m4 = *(const float4*)(stats + i * step), l4 = *(const float4*)(stats + i * step + TI_ROWS);
+      const float* from = sums + (size_t)i * ta.row_tiles * TI_ROWS * TQ_D;
+      float4 f[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = *(const float4*)(from + k * TI_ROWS);
+      const float m[4] = {m4.x, m4.y, m4.z, m4.w}, l[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // (a split that saw nothing of the row may not have written its sums)
+        if (l[j] == 0.0f) continue;
+        const float w = m[j] > -INFINITY ? tq_exp2(m[j] - (M[j] > -INFINITY ? M[j] : 0.0f)) : 1.0f;
+        L[j] += l[j] * w;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[j][k] = fmaf(j == 0 ? f[k].x : j == 1 ? f[k].y : j == 2 ? f[k].z : f[k].w, w, x[j][k]);
       }
     }
-    float top = 0.0f;
+    float top[4];
 #pragma unroll
-    for (int k = 0; k < N; ++k) top = fmaxf(top, fabsf(x[k]));
+    for (int j = 0; j < 4; ++j) {
+      top[j] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top[j] = fmaxf(top[j], fabsf(x[j][k]));
+      top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 16));
+    }
     __syncthreads();  // (the tile before has been read)
-    top_s[part][r] = top;
-    __syncthreads();
-    float exponent;
-    const float up = ti_lift(fmaxf(fmaxf(top_s[0][r], top_s[1][r]), fmaxf(top_s[2][r], top_s[3][r])), 13, exponent);
-    if (part == 0) inv_s[r] = L == 0.0f ? 0.0f : exp2f(exponent - 8.0f) / L;
+    if (lane < 16)
 #pragma unroll
-    for (int k = 0; k < N; k += 8) {
+      for (int j = 0; j < 4; ++j) sh.top[warp][r4 + j] = top[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float t = 0.0f, exponent;
+#pragma unroll
+      for (int i = 0; i < TC_THREADS / 32; ++i) t = fmaxf(t, sh.top[i][r4 + j]);
+      const float up = ti_lift(t, 13, exponent);
+      if (c8 == 0) sh.inv[r4 + j] = L[j] == 0.0f ? 0.0f : exp2f(exponent - 8.0f) / L[j];
       uint32_t h[4], l[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float u = x[k + 2 * i] * up, v = x[k + 2 * i + 1] * up;
+        const float u = x[j][2 * i] * up, v = x[j][2 * i + 1] * up;
         h[i] = ti_pair(u, v);
         l[i] = ti_rest(u, v, h[i]);
       }
-      const int at = r * TC_PITCH + (part * N + k) * 2;
-      *(uint4*)(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-      *(uint4*)(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+      *(uint4*)(sh.hi + tc_at(r4 + j, c8)) = make_uint4(h[0], h[1], h[2], h[3]);
+      *(uint4*)(sh.lo + tc_at(r4 + j, c8)) = make_uint4(l[0], l[1], l[2], l[3]);
     }
     __syncthreads();
+    uint32_t ph[8][4], pl[8][4];  // A: rows = output channels 16 warp .., k = input channels
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int at = tc_at(16 * warp + (lane & 15), 2 * k + (lane >> 4));
+      tc_ldmatrix(ph[k], enc_smem(sh.ph + at));
+      tc_ldmatrix(pl[k], enc_smem(sh.pl + at));
+    }
 #pragma unroll 2
     for (int nt = 0; nt < TC_ROWS / 8; ++nt) {
       if (8 * nt >= rows) break;
-      float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      const int at = (8 * nt + q) * TC_PITCH + 4 * c;
+      float d[4] = {0.0f, 0.0f, 0.0f, 0.0f}, d1[4] = {0.0f, 0.0f, 0.0f, 0.0f}, d2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t h0 = *(const uint32_t*)(hi + at + 32 * k), h1 = *(const uint32_t*)(hi + at + 32 * k + 16);
-        const uint32_t l0 = *(const uint32_t*)(lo + at + 32 * k), l1 = *(const uint32_t*)(lo + at + 32 * k + 16);
-        tc_mma(d, pl[k], h0, h1);
-        tc_mma(d, ph[k], l0, l1);
-        tc_mma(d, ph[k], h0, h1);
+      for (int k = 0; k < 8; k += 2) {
+        uint32_t h[4], l[4];
+        const int at = tc_at(8 * nt + (lane & 7), 2 * k + (lane >> 3));
+        tc_ldmatrix(h, enc_smem(sh.hi + at));
+        tc_ldmatrix(l, enc_smem(sh.lo + at));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          tc_mma(d1, pl[k + i], h[2 * i], h[2 * i + 1]);
+          tc_mma(d2, ph[k + i], l[2 * i], l[2 * i + 1]);
+          tc_mma(d, ph[k + i], h[2 * i], h[2 * i + 1]);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] += d1[i] + d2[i];
       // channels q, q + 8 of the warp's sixteen; rows 2 c, 2 c + 1
-      const float f0 = inv_s[8 * nt + 2 * c], f1 = inv_s[8 * nt + 2 * c + 1];
+      const float f0 = sh.inv[8 * nt + 2 * c], f1 = sh.inv[8 * nt + 2 * c + 1];
       uint32_t w[2];
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
@@ -1054,7 +1097,10 @@ int tq_launch_attend_tiles(const AttendArgs& base, void* workspace, int cap, int
   if (rc != TQ_OK) return rc;
   rc = tq_launch_attend_general(a, st);
   if (rc != TQ_OK) return rc;
-  attend_tiles_combine_kernel<<<std::min(units * tiles, 2 * a.sm_count), TC_THREADS, 0, st>>>(a, ta, tiles, units * tiles);
+  static bool combine_done[64];
+  rc = attend_shared(attend_tiles_combine_kernel, sizeof(CombineShared), a.device, combine_done);
+  if (rc != TQ_OK) return rc;
+  attend_tiles_combine_kernel<<<std::min(units * tiles, 2 * a.sm_count), TC_THREADS, sizeof(CombineShared), st>>>(a, ta, tiles, units * tiles);
   TQ_CUDA(cudaGetLastError());
   return TQ_OK;
 }
