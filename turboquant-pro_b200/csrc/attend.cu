@@ -49,6 +49,30 @@ int most_tokens(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
   return n;
 }
 
+// The form that does a call soonest.  16-bit queries: few rows do best where their keys and values are decoded row
+// tile by row tile (ROWS), many where they are decoded once into the operands of tcgen05 products (TILES); between
+// them goes what was measured over 600 to 32768 tokens, 1 to 32 sequences and 4 to 32 KV heads.  With W tokens
+// seen, times sequences and KV heads, in thousands, and tiles of eight rows, in microseconds (bfloat16 | float16):
+//   ROWS 25 + (0.085 | 0.165) W tiles        TILES 50 + (0.42 | 0.64) W
+// e.g. one sequence of 8192, 8 KV heads, bfloat16: 64 rows 68 against 76, 128 rows 108 against 77; of 32768: 32 rows
+// 100 against 149, 64 rows 177 against 150; 8 of 8192: 204 against 264, 393 against 266.  ROWS is written for blocks of
+// 256 tokens: with others TILES (50 to 920 us by the general form for 4 to 64 rows of 1000 to 64000 tokens, 51 to 250
+// with tiles).  float32 queries, which TILES would round: ROWS up to 64 rows, GENERAL above (one
+// sequence of 8000: 64 rows 130 against 177, 512 rows 813 against 763; 8 of 2000: 354 against 388, 1295 against 1071
+// at 256).
+Form choose(const tq_ctx* ctx, const tq_attend_args* r, int n) {
+  const tq_geom& g = ctx->g;
+  const int rows = r->n_tokens * g.group;
+  const bool channels = g.key_mode != TQ_KEYS_POLAR && !ctx->force_generic, blocks = g.block_tokens == 256;
+  if (!channels) return GENERAL;
+  if (r->q_dtype == TQ_F32) return blocks && rows <= 64 ? ROWS : GENERAL;
+  if (!blocks) return TILES;
+  const double seen = r->window == 0 ? n : std::min((double)n, (double)r->window + r->n_tokens + r->sinks);
+  const double w = seen * r->seq_count * g.n_kv_heads / 1000.0;
+  const bool f16 = r->q_dtype == TQ_F16;
+  return 25.0 + (f16 ? 0.165 : 0.085) * w * ((rows + 7) / 8) <= 50.0 + (f16 ? 0.64 : 0.42) * w ? ROWS : TILES;
+}
+
 // Splits of the tokens: enough CTAs for the GPU, of what is visible in the longest sequence, in blocks and in
 // the window.
 Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
@@ -57,9 +81,7 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
   p.seqs = INT_MAX;
   const int n = most_tokens(ctx, r, st), rows = r->n_tokens * g.group;
   const int nb = n_cold_blocks(n, g.hot_window, g.block_tokens);
-  const bool channels = g.key_mode != TQ_KEYS_POLAR && !ctx->force_generic;
-  p.form = rows > 64 && channels && r->q_dtype != TQ_F32 ? TILES
-           : rows <= 64 && channels && g.block_tokens == 256 ? ROWS : GENERAL;
+  p.form = choose(ctx, r, n);
   const int sm_count = ctx->sm_count;
   if (p.form == TILES) {
     constexpr int TILE = TQ_ATTEND_TILE;
