@@ -214,18 +214,31 @@ __global__ void __launch_bounds__(AG_THREADS) attend_general_kernel(AttendArgs a
     for (int r = 0; r < RPT; ++r)
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[r][j] = 0.0f;
-#pragma unroll 4
-    for (int d = 0; d < TQ_D; d += 4) {
-      float4 kk[4];
+    // (sixteen channels at a time: a sum over all 128 in a row would be rounded at its full size 128 times)
+#pragma unroll 1
+    for (int d0 = 0; d0 < TQ_D; d0 += 16) {
+      float y[RPT][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) kk[j] = *(const float4*)&sh.k[tx + 16 * j][d];
+      for (int r = 0; r < RPT; ++r)
 #pragma unroll
-      for (int r = 0; r < RPT; ++r) {
-        const float4 qq = *(const float4*)&sh.q[ty * RPT + r][d];
+        for (int j = 0; j < 4; ++j) y[r][j] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          x[r][j] = fmaf(qq.x, kk[j].x, fmaf(qq.y, kk[j].y, fmaf(qq.z, kk[j].z, fmaf(qq.w, kk[j].w, x[r][j]))));
+      for (int d = d0; d < d0 + 16; d += 4) {
+        float4 kk[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kk[j] = *(const float4*)&sh.k[tx + 16 * j][d];
+#pragma unroll
+        for (int r = 0; r < RPT; ++r) {
+          const float4 qq = *(const float4*)&sh.q[ty * RPT + r][d];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            y[r][j] = fmaf(qq.x, kk[j].x, fmaf(qq.y, kk[j].y, fmaf(qq.z, kk[j].z, fmaf(qq.w, kk[j].w, y[r][j]))));
+        }
       }
+#pragma unroll
+      for (int r = 0; r < RPT; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[r][j] += y[r][j];
     }
 #pragma unroll
     for (int r = 0; r < RPT; ++r) {
