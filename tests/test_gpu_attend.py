@@ -397,3 +397,57 @@ def test_the_classes_above_it_take_a_window(torch):
     for ctx, out in outs:
         slot = ctx.n_seqs - 1 if ctx is store.ctx and ctx.lengths(0, 0)[0] == 0 else 0
         _check(torch, ctx, torch.from_numpy(out)[None, None].cuda(), qt, 90, 2, seq_begin=slot)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("t", [1, 2, 63, 127, 128, 129, 255, 256, 257, 520])
+def test_edges_of_the_tiles(torch, dtype, t):
+    """Lengths and rows next to the tiles' sizes (80 tokens, 128 and 256 rows), blocks of 150 tokens; queries before
+    the first token, which see nothing."""
+    gen = torch.Generator(device="cuda").manual_seed(100 + t)
+    lens = [79, 80, 81, 160, 161, 449, 450, 600, 641, 1]
+    ctx = _ctx(n_seqs=len(lens), n_kv_heads=1, n_q_heads=1, kv_dtype=dtype, hot_window=300)
+    _fill(torch, ctx, lens, gen)
+    q = torch.randn(len(lens), t, 1, 128, generator=gen, device="cuda").to(getattr(torch, dtype))
+    for window, sinks in ((None, 0), (1, 0), (80, 0), (81, 80), (200, 161)):
+        got = ctx.attend(0, q, window=window, sinks=sinks)
+        _check(torch, ctx, got, q, window, sinks)
+    assert ctx.status() == 0
+
+
+@pytest.mark.parametrize("kv", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("rows", [1, 11, 31, 90])
+def test_types_of_queries_and_cache(torch, kv, dtype, rows):
+    gen = torch.Generator(device="cuda").manual_seed(31)
+    ctx = _ctx(n_seqs=3, n_kv_heads=2, n_q_heads=6, kv_dtype=kv, outlier_frac=0.12)
+    _fill(torch, ctx, [1100, 0, 530], gen)
+    q = torch.randn(3, rows, 6, 128, generator=gen, device="cuda").to(getattr(torch, dtype))
+    for window, sinks in ((None, 0), (300, 5)):
+        _check(torch, ctx, ctx.attend(0, q, window=window, sinks=sinks), q, window, sinks)
+    assert ctx.status() == 0
+
+
+@pytest.mark.parametrize("hot", [512, 128])
+def test_many_sequences(torch, hot):
+    """More of them than one launch of the form for few rows divides."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    lens = [(i * 37) % 700 for i in range(150)]
+    ctx = _ctx(n_seqs=150, n_kv_heads=1, n_q_heads=4, kv_dtype="bfloat16", hot_window=hot, max_tokens_per_seq=1024)
+    _fill(torch, ctx, lens, gen)
+    q = torch.randn(149, 2, 4, 128, generator=gen, device="cuda").bfloat16()
+    _check(torch, ctx, ctx.attend(0, q, seq_begin=1), q, seq_begin=1)
+    _check(torch, ctx, ctx.attend(0, q, seq_begin=1, window=90, sinks=3), q, 90, 3, seq_begin=1)
+
+
+@pytest.mark.parametrize("hot", [512, 200])
+def test_long_sequence(torch, hot):
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    n = 70001
+    ctx = _ctx(n_seqs=1, n_kv_heads=1, n_q_heads=2, kv_dtype="bfloat16", hot_window=hot, max_tokens_per_seq=n)
+    _fill(torch, ctx, [n], gen)
+    for t in (1, 3, 150):
+        q = torch.randn(1, t, 2, 128, generator=gen, device="cuda").bfloat16()
+        for window, sinks in ((None, 0), (60000, 100)):
+            _check(torch, ctx, ctx.attend(0, q, window=window, sinks=sinks), q, window, sinks)
+    assert ctx.status() == 0
