@@ -10,8 +10,10 @@
 // float32, and the weights times cosines and sines, so that a channel costs two multiply-adds.  Sums, norm and
 // rotation are float32, rounded once.
 //
-// Bound by memory for prompts, by launch and latency for single tokens: there a CTA of eight warps takes one
-// token; from a few tokens per SM on four, two warps each, whose angles are one step of the CTA.
+// A CTA of eight warps takes one token of few, or up to eight, a warp each, whose angles are one step of the CTA.
+// Bound by launch and latency for single tokens (4 us); for prompts by reading and writing q and k, at 68 to 80 % of
+// a plain copy's rate (8 x 2048 tokens of 32 + 8 heads, bfloat16: 75 us, 4.5 TB/s), and the unpacking, shuffles and
+// packing between them.
 #include "common.cuh"
 
 namespace {
@@ -27,6 +29,22 @@ TQ_DEV float nr_weight(const void* w, int i, int dt) {
   if (dt == TQ_F32) return ((const float*)w)[i];
   if (dt == TQ_F16) return __half2float(((const __half*)w)[i]);
   return __bfloat162float(((const __nv_bfloat16*)w)[i]);
+}
+// two float32 at once
+TQ_DEV uint64_t nr_f2(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+TQ_DEV uint64_t nr_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+TQ_DEV uint64_t nr_mul2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
 }
 // the elements of a 16-byte word
 template <int DT>
@@ -122,13 +140,13 @@ TQ_DEV uint4 nr_head(const NrLane<DT>& n, const uint4& raw, bool normed, float e
   nr_unpack<DT>(raw, x);
   float f = 1.0f;
   if (normed) {
-    float ss[2] = {0.0f, 0.0f};
+    uint64_t sq = 0ull;
 #pragma unroll
-    for (int c = 0; c < E; ++c) ss[c & 1] = fmaf(x[c], x[c], ss[c & 1]);
-    ss[0] += ss[1];
+    for (int c = 0; c < E; c += 2) sq = nr_fma2(nr_f2(x[c], x[c + 1]), nr_f2(x[c], x[c + 1]), sq);
+    float ss = __uint_as_float((uint32_t)sq) + __uint_as_float((uint32_t)(sq >> 32));
 #pragma unroll
-    for (int d = LPH / 2; d >= 1; d >>= 1) ss[0] += __shfl_xor_sync(0xffffffffu, ss[0], d);
-    f = rsqrtf(fmaf(ss[0], 1.0f / TQ_D, eps));
+    for (int d = LPH / 2; d >= 1; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+    f = rsqrtf(fmaf(ss, 1.0f / TQ_D, eps));
   }
   if (PAIRED) {
     uint4 o;
@@ -150,25 +168,29 @@ TQ_DEV uint4 nr_head(const NrLane<DT>& n, const uint4& raw, bool normed, float e
     }
   }
 #pragma unroll
-  for (int c = 0; c < E; ++c) y[c] = f * fmaf(x[c], n.own[c], z[c] * n.other[c]);
+  for (int c = 0; c < E; c += 2) {
+    const uint64_t v = nr_mul2(nr_f2(f, f), nr_fma2(nr_f2(x[c], x[c + 1]), nr_f2(n.own[c], n.own[c + 1]),
+                                                    nr_mul2(nr_f2(z[c], z[c + 1]), nr_f2(n.other[c], n.other[c + 1]))));
+    y[c] = __uint_as_float((uint32_t)v), y[c + 1] = __uint_as_float((uint32_t)(v >> 32));
+  }
   return nr_pack<DT>(y);
 }
 
 template <int DT, bool PAIRED, bool VEC>
-__global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(RopeArgs a, int64_t tokens, int per_cta) {
+__global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(RopeArgs a, int tokens, int per_cta) {
   using T = typename Elem<DT>::type;
   using Lane = NrLane<DT>;
   constexpr int HPW = Lane::HPW;
   constexpr int N = 4;  // query items of a warp in flight, and one of keys
-  __shared__ __align__(16) float cos_s[4][TQ_D / 2], sin_s[4][TQ_D / 2], weight_s[2][TQ_D];
+  __shared__ __align__(16) float cos_s[8][TQ_D / 2], sin_s[8][TQ_D / 2], weight_s[2][TQ_D];
   static_assert(NR_THREADS == 2 * TQ_D, "a thread per weight");
   const tq_rope& r = a.r;
   const int tid = threadIdx.x, warp = tid >> 5;
   const int wpt = NR_THREADS / 32 / per_cta;  // warps of a token
   const int mine = warp / wpt, sub = warp % wpt;
-  const int64_t tok = (int64_t)blockIdx.x * per_cta + mine;
-  const bool active = tok < tokens;
-  const int s = active ? (int)(tok / r.n_tokens) : 0, t = active ? (int)(tok - (int64_t)s * r.n_tokens) : 0;
+  const uint32_t tok = blockIdx.x * (uint32_t)per_cta + mine;  // (at most 2^31 + 7)
+  const bool active = tok < (uint32_t)tokens;
+  const uint32_t s = active ? tok / (uint32_t)r.n_tokens : 0u, t = active ? tok - s * (uint32_t)r.n_tokens : 0u;
   Lane n;
   n.lane = tid & 31;
   n.hl = n.lane / Lane::LPH, n.ch = n.lane % Lane::LPH * Lane::E, n.half = r.rotary_dim / 2;
@@ -197,9 +219,9 @@ __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(RopeArgs a, in
   }
   for (int i = tid; i < per_cta * n.half; i += NR_THREADS) {
     const int u = i / n.half, f = i - u * n.half;
-    const int64_t tk = (int64_t)blockIdx.x * per_cta + u;
-    if (tk >= tokens) break;
-    const int us = (int)(tk / r.n_tokens), ut = (int)(tk - (int64_t)us * r.n_tokens);
+    const uint32_t tk = blockIdx.x * (uint32_t)per_cta + u;
+    if (tk >= (uint32_t)tokens) break;
+    const uint32_t us = tk / (uint32_t)r.n_tokens, ut = tk - us * (uint32_t)r.n_tokens;
     int64_t p;
     if (a.seq_len != nullptr) p = (int64_t)a.seq_len[us] + ut;
     else {
@@ -215,7 +237,7 @@ __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(RopeArgs a, in
   __syncthreads();
   if (!active) return;
 
-  T* out = (T*)r.q_out + ((tok * r.n_q_heads + h0) * TQ_D + n.ch);
+  T* out = (T*)r.q_out + (((int64_t)tok * r.n_q_heads + h0) * TQ_D + n.ch);
   nr_factors<DT, PAIRED>(n, weight_s[0], cos_s[mine], sin_s[mine]);
   for (int h = h0; h - n.hl < r.n_q_heads; h += N * step) {  // (a warp's lanes stay together)
     if (h != h0) fetch(h);
@@ -227,7 +249,7 @@ __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(RopeArgs a, in
       out += step * TQ_D;
     }
   }
-  out = (T*)r.k_out + ((tok * r.n_kv_heads + h0) * TQ_D + n.ch);
+  out = (T*)r.k_out + (((int64_t)tok * r.n_kv_heads + h0) * TQ_D + n.ch);
   nr_factors<DT, PAIRED>(n, weight_s[1], cos_s[mine], sin_s[mine]);
   for (int h = h0; h - n.hl < r.n_kv_heads; h += step) {
     const uint4 x = raw_k;
@@ -240,10 +262,15 @@ __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(RopeArgs a, in
 }
 
 template <int DT, bool PAIRED>
-void start(const RopeArgs& a, int64_t tokens, bool vec, cudaStream_t st) {
-  // (four tokens a CTA as soon as these fill the SMs)
-  const int per_cta = tokens >= 512 ? 4 : 1;
-  const int grid = (int)((tokens + per_cta - 1) / per_cta);
+void start(const RopeArgs& a, int tokens, bool vec, cudaStream_t st) {
+  // The fewest tokens a CTA with which all are resident at once, three an SM: another round of them costs more than a
+  // warp's longer work, and that more than the angles of more tokens a thread.  us for 1 | 2 | 4 | 8 tokens a CTA (32 + 8
+  // heads, bfloat16): 64 tokens 3.7 | 4.2 | 5.5 | 8.5, 600: 8.3 |
+  // 6.3 | 6.9 | 8.6, 1700: 17.1 | 11.6 | 9.1 | 11.1, 6000: 62 | 41 | 34 | 32.
+  constexpr int RESIDENT = 3 * 148;
+  int per_cta = 1;
+  while (per_cta < NR_THREADS / 32 && tokens > per_cta * RESIDENT) per_cta *= 2;
+  const int grid = (int)(((int64_t)tokens + per_cta - 1) / per_cta);
   if (vec) norm_rope_kernel<DT, PAIRED, true><<<grid, NR_THREADS, 0, st>>>(a, tokens, per_cta);
   else norm_rope_kernel<DT, PAIRED, false><<<grid, NR_THREADS, 0, st>>>(a, tokens, per_cta);
 }
@@ -273,7 +300,7 @@ int check_rope(const tq_rope* r, bool stored) {
 }
 
 int launch(const tq_rope* r, const int32_t* seq_len, cudaStream_t st) {
-  const int64_t tokens = (int64_t)r->n_seqs * r->n_tokens;
+  const int tokens = r->n_seqs * r->n_tokens;
   if (tokens == 0 || r->n_q_heads + r->n_kv_heads == 0) return TQ_OK;
   const int e = 16 / elem_size(r->dtype);
   const bool vec = ((uintptr_t)r->q | (uintptr_t)r->k) % 16 == 0 &&
