@@ -38,6 +38,12 @@ def norm_rope(q, k, inv_freq, positions, *, q_weight=None, k_weight=None, eps: f
     return _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, None)
 
 
+def _weight(w, codes, other):
+    if w.shape != (HEAD_DIM,) or w.dtype not in codes or (other is not None and w.dtype != other):
+        raise ValueError(f"norm weights must be [{HEAD_DIM}] and of one floating type")
+    return w.contiguous(), codes[w.dtype]
+
+
 def _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, cache):
     # (a decode step's call is a few microseconds on the GPU: the checks are kept short)
     torch = _torch()
@@ -52,39 +58,42 @@ def _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, cache):
     codes = _dtype_codes()
     if dtype not in codes or k.dtype != dtype:
         raise ValueError(f"q and k must share float32, float16 or bfloat16, got {dtype} and {k.dtype}")
-    grad = torch.is_grad_enabled()
-    for name, t in (("q", q), ("k", k), ("inv_freq", inv_freq), ("positions", positions),
-                    ("q_weight", q_weight), ("k_weight", k_weight)):
-        if t is None:
-            continue
-        if t.device != dev:
-            raise ValueError(f"{name} lives on {t.device}, q on {dev}")
-        if grad and t.requires_grad:
-            raise ValueError("norm_rope has no backward pass: call it under torch.no_grad()")
+    if k.device != dev or inv_freq.device != dev or (positions is not None and positions.device != dev) \
+            or (q_weight is not None and q_weight.device != dev) \
+            or (k_weight is not None and k_weight.device != dev):
+        raise ValueError(f"k, inv_freq, positions and weights must live where q does, on {dev}")
+    if torch.is_grad_enabled() and (
+            q.requires_grad or k.requires_grad or inv_freq.requires_grad
+            or (q_weight is not None and q_weight.requires_grad)
+            or (k_weight is not None and k_weight.requires_grad)):
+        raise ValueError("norm_rope has no backward pass: call it under torch.no_grad()")
     if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
         raise ValueError("inv_freq must be a float32 vector")
     if eps < 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    weight_type = 0
-    for w in (q_weight, k_weight):
-        if w is None:
-            continue
-        if w.shape != (HEAD_DIM,) or w.dtype not in codes \
-                or (k_weight is not None and w.dtype != k_weight.dtype):
-            raise ValueError(f"norm weights must be [{HEAD_DIM}] and of one floating type")
-        weight_type = codes[w.dtype]
+    weight_type, qw, kw = 0, None, None
+    if q_weight is not None:
+        q_weight, weight_type = _weight(q_weight, codes, None if k_weight is None else k_weight.dtype)
+        qw = q_weight.data_ptr()
+    if k_weight is not None:
+        k_weight, weight_type = _weight(k_weight, codes, None)
+        kw = k_weight.data_ptr()
     n, t = q_shape[0], q_shape[1]
-    pos, pos_bits, pos_stride = None, 0, (0, 0)
+    pos, pos_bits, ps, pt = None, 0, 0, 0
     if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64):
+        if positions.dtype == torch.int64:
+            pos_bits = 64
+        elif positions.dtype == torch.int32:
+            pos_bits = 32
+        else:
             raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
         if positions.shape == (n, t):
-            pos_stride = positions.stride()
+            ps, pt = positions.stride()
         elif positions.shape == (t,):
-            pos_stride = (0, positions.stride(0))
+            pt = positions.stride(0)
         else:
             raise ValueError(f"positions must be [{n}, {t}] or [{t}], got {tuple(positions.shape)}")
-        pos, pos_bits = positions.data_ptr(), 64 if positions.dtype == torch.int64 else 32
+        pos = positions.data_ptr()
     qs, ks = q.stride(), k.stride()
     if qs[3] != 1:
         q = q.contiguous()
@@ -93,15 +102,12 @@ def _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, cache):
         k = k.contiguous()
         ks = k.stride()
     inv_freq = inv_freq.contiguous()
-    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
-    q_out = torch.empty(q_shape, dtype=dtype, device=dev)
-    k_out = torch.empty(k_shape, dtype=dtype, device=dev)
-    r = TqRope(q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(),
-               None if q_weight is None else q_weight.data_ptr(),
-               None if k_weight is None else k_weight.data_ptr(), inv_freq.data_ptr(), pos,
-               qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], pos_stride[0], pos_stride[1],
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    r = TqRope(q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), qw, kw, inv_freq.data_ptr(), pos,
+               qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], ps, pt,
                n, t, q_shape[2], k_shape[2], codes[dtype], weight_type, pos_bits,
-               2 * inv_freq.numel(), eps)
+               2 * inv_freq.shape[0], eps)
     lib, index = _lib.load(), dev.index
     with _NO_GUARD if torch.cuda.current_device() == index else torch.cuda.device(dev):
         stream = _raw_stream()(index)
