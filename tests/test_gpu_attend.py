@@ -175,11 +175,12 @@ def test_orders_and_alignments_of_the_queries(torch, dtype):
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("rows", [1, 40, 300])
-def test_what_is_masked_may_hold_anything(torch, dtype, rows):
+@pytest.mark.parametrize("hot", [512, 200])
+def test_what_is_masked_may_hold_anything(torch, dtype, rows, hot):
     """Infinities and NaN in hidden tokens of the window reach nothing; in visible ones, only those that see them."""
     dt = getattr(torch, dtype)
     gen = torch.Generator(device="cuda").manual_seed(9)
-    ctx = _ctx(n_seqs=1, n_kv_heads=1, n_q_heads=4, kv_dtype=dtype)
+    ctx = _ctx(n_seqs=1, n_kv_heads=1, n_q_heads=4, kv_dtype=dtype, hot_window=hot)
     n = 600
     k = torch.randn(1, n, 1, 128, generator=gen, device="cuda").to(dt)
     v = torch.randn(1, n, 1, 128, generator=gen, device="cuda").to(dt)
@@ -205,12 +206,13 @@ def test_what_is_masked_may_hold_anything(torch, dtype, rows):
     assert bool((off <= 2.0**-9 * 6 + torch.finfo(dt).eps * want[0, ~sees].double().abs()).all())
 
 
-def test_value_that_is_no_number_stays_in_its_channels(torch):
+@pytest.mark.parametrize("hot, at, many", [(512, 450, 200), (200, 650, 45)])  # (all rows see the token)
+def test_value_that_is_no_number_stays_in_its_channels(torch, hot, at, many):
     gen = torch.Generator(device="cuda").manual_seed(2)
-    for rows in (1, 200):
-        ctx = _ctx(n_seqs=1, n_kv_heads=1, n_q_heads=2, kv_dtype="bfloat16")
+    for rows in (1, many):
+        ctx = _ctx(n_seqs=1, n_kv_heads=1, n_q_heads=2, kv_dtype="bfloat16", hot_window=hot)
         k, v = (torch.randn(1, 700, 1, 128, generator=gen, device="cuda").bfloat16() for _ in range(2))
-        v[0, 450, 0, 9] = float("nan")
+        v[0, at, 0, 9] = float("nan")
         ctx.append(0, k, v)
         got = ctx.attend(0, torch.randn(1, rows, 2, 128, generator=gen, device="cuda").bfloat16())
         assert bool(got[..., 9].isnan().all()) and int(got.isnan().sum()) == 2 * rows
@@ -218,11 +220,12 @@ def test_value_that_is_no_number_stays_in_its_channels(torch):
 
 @pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
 @pytest.mark.parametrize("rows", [1, 8, 300])
-def test_a_token_with_a_small_value_may_dominate(torch, dtype, rows):
+@pytest.mark.parametrize("hot", [512, 300])
+def test_a_token_with_a_small_value_may_dominate(torch, dtype, rows, hot):
     """The softmax all on a token whose value is 2^-9 of the others': the output keeps its digits."""
     dt = getattr(torch, dtype)
     gen = torch.Generator(device="cuda").manual_seed(21)
-    ctx = _ctx(n_seqs=1, n_kv_heads=1, n_q_heads=1, kv_dtype=dtype, outlier_frac=0.0)
+    ctx = _ctx(n_seqs=1, n_kv_heads=1, n_q_heads=1, kv_dtype=dtype, outlier_frac=0.0, hot_window=hot)
     n = 1100
     k = 0.1 * torch.randn(1, n, 1, 128, generator=gen, device="cuda")
     v = torch.randn(1, n, 1, 128, generator=gen, device="cuda")
@@ -450,4 +453,37 @@ def test_long_sequence(torch, hot):
         q = torch.randn(1, t, 2, 128, generator=gen, device="cuda").bfloat16()
         for window, sinks in ((None, 0), (60000, 100)):
             _check(torch, ctx, ctx.attend(0, q, window=window, sinks=sinks), q, window, sinks)
+    assert ctx.status() == 0
+
+
+def test_one_unit_of_many_is_left_to_the_general_form(torch):
+    """Keys beyond half precision's range in one KV head of one sequence, many rows; the others stay as they are."""
+    gen = torch.Generator(device="cuda").manual_seed(41)
+    ctx = _ctx(n_seqs=3, n_kv_heads=2, n_q_heads=4, kv_dtype="bfloat16", hot_window=200)
+    k, v = (torch.randn(3, 900, 2, 128, generator=gen, device="cuda").bfloat16() for _ in range(2))
+    k[1, 850, 1, 3] = 2.0**30
+    ctx.append(0, k, v)
+    q = torch.randn(3, 300, 4, 128, generator=gen, device="cuda").bfloat16()
+    q[..., 3] = -q[..., 3].abs()  # (that key gets no weight, so that the bound means something)
+    got = ctx.attend(0, q, window=400, sinks=5)
+    ctx.clear(0)
+    k[1, 850, 1, 3] = 0.0
+    ctx.append(0, k, v)
+    # token 850 aside, the same attention: 64 bits without it
+    for s in range(3):
+        n, h = 900, 1
+        kk, vv = (x.double() for x in ctx.dequant(0, s, 0, n))
+        p = n - 300 + torch.arange(300, device="cuda")
+        j = torch.arange(n, device="cuda")
+        sees = (j <= p[:, None]) & ((j > p[:, None] - 400) | (j < 5))
+        for hq in range(4):
+            see = sees & ((j != 850)[None] if s == 1 and hq // 2 == 1 else True)
+            qk = q[s, :, hq].double()
+            pr = torch.softmax((qk @ kk[hq // 2].t() / math.sqrt(128)).masked_fill(~see, -math.inf), 1)
+            want = pr @ vv[hq // 2]
+            a = (qk.abs() @ kk[hq // 2].abs().t() / math.sqrt(128)).masked_fill(~see, 0.0).amax(1)
+            top = vv[hq // 2].abs().amax(1)[None].masked_fill(~see, 0.0).amax(1)
+            limit = ((2 * a + 4) * 2.0**-11 * top)[:, None] + torch.finfo(q.dtype).eps / 2 * want.abs()
+            off = (got[s, :, hq].double() - want).abs()
+            assert bool((off <= limit).all()), (s, hq, float((off / limit).max()))
     assert ctx.status() == 0
