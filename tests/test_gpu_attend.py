@@ -487,3 +487,37 @@ def test_one_unit_of_many_is_left_to_the_general_form(torch):
             off = (got[s, :, hq].double() - want).abs()
             assert bool((off <= limit).all()), (s, hq, float((off / limit).max()))
     assert ctx.status() == 0
+
+
+@pytest.mark.parametrize("window", [None, 90])
+def test_hf_layers_attend_chunks_and_windows(torch, window):
+    """The adapter's attention function on stored history: one and several tokens, with and without a window."""
+    from types import SimpleNamespace
+
+    from turboquant_pro_b200 import hf_cache
+
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    cache = hf_cache.TurboQuantCache(n_layers=1, n_q_heads=4, max_tokens=2048, attend=True)
+    module = SimpleNamespace(layer_idx=0, is_causal=True, sliding_window=window, num_key_value_groups=2, training=False)
+    n = 0
+    for t in (600, 1, 70, 5, 300):
+        q = torch.randn(2, 4, t, 128, generator=gen, device="cuda").bfloat16()
+        k, v = (torch.randn(2, 2, t, 128, generator=gen, device="cuda").bfloat16() for _ in range(2))
+        kk, vv = cache.layers[0].update(k, v)
+        n += t
+        if n == t:
+            continue
+        p, j = torch.arange(n - t, n, device="cuda")[:, None], torch.arange(n, device="cuda")
+        sees = (j <= p) & (j > p - window) if window else j <= p
+        outs = [hf_cache.turboquant_attention_forward(module, q, kk, vv, m, scaling=128**-0.5)[0]
+                for m in (None, torch.ones(2, n, dtype=torch.int64, device="cuda"), sees[None, None].expand(2, 1, t, n))]
+        if t > 1 or window:  # (a single token without a window is decoded, as without the option)
+            _check(torch, cache.context, outs[0], q.transpose(1, 2), window)
+            assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    # a mask of another kind is attended densely
+    other = sees.clone()
+    other[:, 3] = False
+    got = hf_cache.turboquant_attention_forward(module, q, kk, vv, other[None, None], scaling=128**-0.5)[0]
+    kd, vd = cache.layers[0].full()
+    want = torch.nn.functional.scaled_dot_product_attention(q, kd, vd, other[None, None], enable_gqa=True)
+    assert torch.allclose(got, want.transpose(1, 2), rtol=2e-2, atol=2e-2)

@@ -22,6 +22,9 @@ Differences from the reference adapter, all forced by the paged device format:
   dense getters (``dense=True`` forces that path for every decode step: it is how the
   reference's adapter works, and this adapter's own cross-check);
 * capacity (``max_tokens``) is fixed when the context is created.
+
+``attend=True`` puts two of these cases on the codes as well, through ``KVContext.attend``: queries of
+several tokens on stored history (chunks of a prompt, drafts to verify), and layers with a sliding window.
 """
 
 from __future__ import annotations
@@ -73,6 +76,20 @@ def _mask_is_open(mask) -> bool:
     return is_open
 
 
+def _mask_is_causal(mask, t: int, n: int, window) -> bool:
+    """Whether ``mask`` is what ``KVContext.attend`` applies to the newest ``t`` of ``n`` tokens: none (the
+    layer's own rule), a padding mask that hides nothing, or exactly the causal mask with the window."""
+    if mask is None:
+        return True
+    if mask.dim() == 2:
+        return _mask_is_open(mask if mask.dtype == torch.bool else mask != 0)
+    if tuple(mask.shape[-2:]) != (t, n):
+        return False
+    p, j = torch.arange(n - t, n, device=mask.device)[:, None], torch.arange(n, device=mask.device)
+    sees = j <= p if window is None else (j <= p) & (j > p - window)
+    return bool(((mask if mask.dtype == torch.bool else mask >= 0) == sees).all())
+
+
 class _SharedContext:
     """The one KVContext behind all layers of a TurboQuantCache, created at the first
     update (when batch size, KV-head count, head_dim, dtype and device are known)."""
@@ -104,8 +121,10 @@ class TurboQuantLayer(CacheLayerMixin):
     is_compileable = False
     is_sliding = False
 
-    def __init__(self, shared: _SharedContext, layer_idx: int, dense: bool = False) -> None:
+    def __init__(self, shared: _SharedContext, layer_idx: int, dense: bool = False,
+                 attend: bool = False) -> None:
         super().__init__()
+        self.attend = bool(attend)
         self._shared = shared
         self.layer_idx = int(layer_idx)
         self.dense = bool(dense)
@@ -206,12 +225,14 @@ class TurboQuantCache(Cache):
             ``TurboQuantCache`` (``hf_cache.py:283-300``).
         max_tokens: capacity per sequence.
         dense: hand the model dense K/V on every step instead of attending on the codes.
+        attend: attend on the codes too where a query has several tokens on stored history, or the layer a
+            sliding window.
     """
 
     def __init__(self, config=None, hot_window: int = 512, key_bits: int = 4,
                  value_bits: int = 4, outlier_frac: float = 0.02, seed: int = 0,
                  max_tokens: int = 8192, dense: bool = False, n_layers: int | None = None,
-                 n_q_heads: int | None = None) -> None:
+                 n_q_heads: int | None = None, attend: bool = False) -> None:
         if not _HAS_TRANSFORMERS:
             raise ImportError("TurboQuantCache requires transformers v5+")
         if config is not None:
@@ -224,7 +245,7 @@ class TurboQuantCache(Cache):
         self.outlier_frac, self.seed, self.dense = outlier_frac, seed, dense
         self._shared = _SharedContext(n_layers, n_q_heads, hot_window, key_bits, value_bits,
                                       outlier_frac, seed, max_tokens)
-        super().__init__(layers=[TurboQuantLayer(self._shared, i, dense) for i in range(n_layers)])
+        super().__init__(layers=[TurboQuantLayer(self._shared, i, dense, attend) for i in range(n_layers)])
 
     @property
     def context(self) -> KVContext | None:
@@ -263,6 +284,16 @@ def turboquant_attention_forward(module, query, key, value, attention_mask, drop
     if fused:
         out = layer.ctx.decode(layer.layer_idx, query[:, :, 0, :])  # [B, Hq, D] float32
         return out.to(query.dtype)[:, None, :, :], None
+    if layer is not None and layer.attend and not layer.dense and key.shape[2] == query.shape[2]:
+        n, t = layer.get_seq_length(), query.shape[2]
+        window = kwargs.get("sliding_window") or getattr(module, "sliding_window", None)
+        if (n > t and not dropout and not kwargs.get("softcap")
+                and (scaling is None or abs(scaling * query.shape[-1] ** 0.5 - 1.0) <= 1e-3)
+                and (window is not None or not getattr(module, "is_sliding", False))
+                and is_causal is not False and getattr(module, "is_causal", True)
+                and not (query.requires_grad and torch.is_grad_enabled())
+                and _mask_is_causal(attention_mask, t, n, window)):
+            return layer.ctx.attend(layer.layer_idx, query.transpose(1, 2), window=window), None
     if layer is not None and key.shape[2] != layer.get_seq_length():
         # a multi-token query on top of stored history, a masked batch, a windowed or capped
         # layer: the dense history
