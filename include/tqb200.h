@@ -199,7 +199,8 @@ typedef struct tq_attend_args {
 
 /* Bytes of workspace that tq_attend wants for these arguments (pointers are not looked at), on this stream: a
  * captured call asks for what the capacity of the sequences may need, since it may be replayed on longer
- * ones.  A call may be given less, down to what one sequence needs; it then takes several rounds. */
+ * ones.  A call may be given less, down to what one sequence needs; it then takes several rounds.  tq_attend writes
+ * only to its workspace and out, so calls of one context with a workspace each may overlap on the device. */
 int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* args, void* stream, size_t* bytes);
 int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* args, void* stream);
 
@@ -391,6 +392,7 @@ int32_t tq_clear(tq_ctx* ctx, int32_t layer, int32_t seq, void* stream);
  *   bit 1 (2): a bounded wait ran out and the kernel returned, so the device stays usable:
  *              - in the tensor-core decode kernel (a tile copy did not arrive within the limit):
  *                the `out` / `mlo` of that call is undefined;
+ *              - in tq_attend's form for many rows: the `out` of that call is undefined;
  *              - in an encoder, on tq_append: a block was stored that does not hold its tokens (the
  *                key encoder for 256-token blocks stores an empty key block: keys of zero), so the
  *                sequence has to be cleared and appended again.

@@ -376,7 +376,7 @@ class KVContext:
         flags = self.status()
         if flags & 2:
             raise _lib.TqError(-3, "a bounded wait inside a kernel ran out: the output of that decode "
-                                   "is undefined, or that append stored a block without its tokens")
+                                   "or attention is undefined, or that append stored a block without its tokens")
         return flags
 
     def decode_static_scratch(self, layer: int, q, out=None):
@@ -767,7 +767,7 @@ class KVContext:
 
     def status(self) -> int:
         """Device status flags (bit 0: an outlier pool overflowed; bit 1: a bounded wait ran out:
-        in the tensor-core decode kernel, and that call's output is undefined, or in an append,
+        in the tensor-core decode kernel or :meth:`attend`, and that call's output is undefined, or in an append,
         which then stored a block without its tokens: clear the sequence; bit 2:
         :meth:`dequant_into_pages` met a page outside the tensor); clears them."""
         f = C.c_int32()

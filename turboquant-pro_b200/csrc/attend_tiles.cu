@@ -23,6 +23,14 @@
 //     holds what counts.  The maximum is only renewed (and O rescaled) when it has grown by 2^8 since.
 // attend_tiles_combine_kernel   merges the splits, rotates the sums back (sum @ Pi), rounds.
 //
+// Measured, 8 KV heads of 4 query heads, bfloat16: 2048 tokens on 32768 1 066 us, of which stage 79, tiles 907 (72 % of
+// the rate of a large library product of as many operations, 4.3 GB/ms of operands from L2), merge 68; 512 tokens on 16384
+// 204 us: 49, 137, 16.  What bounds the tiles: exponentials (16 a cycle and SM: 1 280 cycles a tile, of which a
+// quarter goes over the multiply-add units) and tcgen05 products (1 280 cycles) take as long, and a half's chain of
+// waits, fetch, maximum and exponentials, 2 000 cycles, is covered by the other half alone.  Shares of exponentials on the
+// multiply-add units of 1, 2, 3, 4, 5 eighths: 899, 907, 923, 958, 994 us at 2048 tokens and 66.9, 64.7, 66.1, 67.0,
+// 68.1 for 777 float16 ones.
+//
 // Queries are fp16 in shared memory, each row scaled by a power of two, which is exact for both 16-bit types.
 // SPLIT (float16 queries): keys and values as pairs hi + lo, so that only the probabilities are rounded to fp16 and the
 // result is off by about its own rounding; bfloat16 queries take the hi parts alone (2^-12 against 2^-9).
