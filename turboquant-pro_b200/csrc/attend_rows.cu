@@ -1307,6 +1307,9 @@ int launch_rows(const AttendArgs& a, cudaStream_t st) {
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
+  // A CTA per row while these are two an SM at most, else groups of threads with four rows at a time, in turn.  Whole
+  // calls, 4000 tokens: 32 rows 29 us against 47, 256 rows 36 against 50; 8 x 1000 tokens: 256 rows 25 against 30, 512
+  // rows 30 and 30, 1024 rows 44 against 35.
   const bool few = all <= 2 * a.sm_count;
   cfg.gridDim = dim3((unsigned)(few ? all : std::min<int64_t>((all + 3) / 4, 2 * a.sm_count)));
   cfg.blockDim = dim3(AC_THREADS);
