@@ -138,6 +138,12 @@ TQ_DEV float ar_lift(float x, int top, float& inverse) {
   inverse = __int_as_float((e - top) << 23);
   return __int_as_float((254 + top - e) << 23);
 }
+// tq_scaled of a score, less `by`, without a rounding at the score's full size
+TQ_DEV float ar_exponent(float x, float by) {
+  constexpr TqFactor f{TQ_SCORE_LOG2};
+  constexpr float hi = f.hi, lo = f.lo;
+  return fmaf(x, lo, fmaf(x, hi, -by));
+}
 TQ_DEV uint32_t ar_smem(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 TQ_DEV void ar_cp16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ar_smem(dst)), "l"(src) : "memory");
@@ -471,8 +477,9 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
     return t0 > p_hi || (t1 <= attend_window(a, max(p_lo, 0)) && t0 >= a.sinks);
   };
   const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  // From the scores of TILES times 16 tokens from `t0` on to their probabilities: maximum and sum go on, the
-  // probability stays in `sc`, times a power of two that takes the row's largest probability * nv below 2^14.
+  // From the scores (q . k as it is) of TILES times 16 tokens from `t0` on to their probabilities: maximum and sum go
+  // on, in units of log 2 (taken to the exponent in one multiply-add: a score in these units would be rounded once
+  // more at its full size), the probability stays in `sc`, times a power of two that takes the row's largest probability * nv below 2^14.
   auto softmax = [&](auto& sc, int t0, int t_end, auto tiles, const auto& nv, float (&inv_n)[NT][2]) {
     constexpr int TILES = decltype(tiles)::value;
     const bool open = t0 + 16 * TILES <= t_end && open_to_all(t0, t0 + 16 * TILES);
@@ -498,7 +505,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
             if (!(hidden >> (2 * h + y) & 1u)) top = fmaxf(top, sc[h][t][2 * y + x]);
 #pragma unroll
         for (int o = 4; o <= 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        top = fmaxf(m_run[t][x], top);
+        top = fmaxf(m_run[t][x], tq_scaled<true>(top));
         // (-inf: nothing seen yet, or scores that are no numbers, which stay so)
         const float by = top > -INFINITY ? top : 0.0f, down = tq_exp2(m_run[t][x] - by);
         float sum = 0.0f, most = 0.0f;
@@ -506,7 +513,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
         for (int h = 0; h < TILES; ++h)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const float e = hidden >> (2 * h + y) & 1u ? 0.0f : tq_exp2(sc[h][t][2 * y + x] - by);
+            const float e = hidden >> (2 * h + y) & 1u ? 0.0f : tq_exp2(ar_exponent(sc[h][t][2 * y + x], by));
             sum += e;
             sc[h][t][2 * y + x] = e;
             most = fmaxf(most, fabsf(e * nv[h][y]));
@@ -674,7 +681,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
         const uint4 v = *(const uint4*)(my.keys + (32 * half + 16 * h + 8 * x + r) * (TQ_D / 2) + c * 16);
         kw[x][0] = v.x, kw[x][1] = v.y, kw[x][2] = v.z, kw[x][3] = v.w;
       }
-      float sum[NT][4], low[NT][4];
+      float sum[NT][4], low[NT][4], pair[NT][4];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -700,7 +707,10 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
             ar_mma(low[t], al, bh[t][j][0], bh[t][j][1], low[t]);
             ar_mma(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[t][i] += d[i];
+            for (int i = 0; i < 4; ++i) {  // (32 channels at a time)
+              if (j & 1) sum[t][i] += pair[t][i] + d[i];
+              else pair[t][i] = d[i];
+            }
           } else {
             ar_mma(sum[t], ah, bh[t][j][0], bh[t][j][1], sum[t]);
             ar_mma(low[t], ah, bl[t][j][0], bl[t][j][1], low[t]);
@@ -712,9 +722,10 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int n = 8 * t + 2 * c + (i & 1), tok = 16 * h + 8 * (i >> 1) + r;
-          float x = fmaf(sum[t][i] + low[t][i], inv[t][i & 1], bias[t][i & 1]);
+          // (small parts first)
+          float x = bias[t][i & 1];
           if (g.outlier_k > 0) x += my.corr[tok][n ^ (4 * (tok >> 2 & 1))];
-          sc[h][t][i] = tq_scaled<true>(x);
+          sc[h][t][i] = fmaf(sum[t][i], inv[t][i & 1], fmaf(low[t][i], inv[t][i & 1], x));
         }
     }
   };
@@ -896,7 +907,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       // a lane's keys are channels 32 c .. + 31 of tokens r and r + 8
-      float sum[NT][4], low[NT][4];
+      float sum[NT][4], low[NT][4], pair[NT][4];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -943,13 +954,16 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
             if (F32) ar_mma(low[t], al, bh[t][j][0], bh[t][j][1], low[t]);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sum[t][i] += d[i];
+          for (int i = 0; i < 4; ++i) {
+            if (j & 1) sum[t][i] += pair[t][i] + d[i];
+            else pair[t][i] = d[i];
+          }
         }
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[h][t][i] = tq_scaled<true>((sum[t][i] + low[t][i]) * inv[t][i & 1]);
+        for (int i = 0; i < 4; ++i) sc[h][t][i] = (sum[t][i] + low[t][i]) * inv[t][i & 1];
     }
     if (!F32) {
       asm volatile("cp.async.wait_all;" ::: "memory");
