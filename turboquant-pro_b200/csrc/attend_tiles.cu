@@ -27,7 +27,9 @@
 // the rate of a large library product of as many operations, 4.3 GB/ms of operands from L2), merge 68; 512 tokens on 16384
 // 204 us: 49, 137, 16.  What bounds the tiles: exponentials (16 a cycle and SM: 1 280 cycles a tile, of which a
 // quarter goes over the multiply-add units) and tcgen05 products (1 280 cycles) take as long, and a half's chain of
-// waits, fetch, maximum and exponentials, 2 000 cycles, is covered by the other half alone.  Shares of exponentials on the
+// waits, fetch, maximum and exponentials, 2 000 cycles, is covered by the other half alone.  (An even division over the
+// SMs, whose parts went on through a CTA's tiles of rows, took as long for 512 tokens on 148 SMs as this does on 128: the
+// clock, 1.65 GHz, gives way.)  Shares of exponentials on the
 // multiply-add units of 1, 2, 3, 4, 5 eighths: 899, 907, 923, 958, 994 us at 2048 tokens and 66.9, 64.7, 66.1, 67.0,
 // 68.1 for 777 float16 ones.
 //
