@@ -673,7 +673,8 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   // scores of tokens 32 half .. + 31 of the strip
   auto strip_scores = [&](float (&sc)[2][NT][4], int half, int ts) {
     if (g.outlier_k > 0) corrections(half, ts);
-#pragma unroll
+    // (a loop, here and of the values: unrolled, the code did not fit the instruction caches)
+#pragma unroll 1
     for (int h = 0; h < 2; ++h) {
       uint32_t kw[2][4];
 #pragma unroll
@@ -725,7 +726,8 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
           // (small parts first)
           float x = bias[t][i & 1];
           if (g.outlier_k > 0) x += my.corr[tok][n ^ (4 * (tok >> 2 & 1))];
-          sc[h][t][i] = fmaf(sum[t][i], inv[t][i & 1], fmaf(low[t][i], inv[t][i & 1], x));
+          sc[0][t][i] = sc[1][t][i];
+          sc[1][t][i] = fmaf(sum[t][i], inv[t][i & 1], fmaf(low[t][i], inv[t][i & 1], x));
         }
     }
   };
@@ -733,7 +735,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
     float f[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) f[t][0] = inv_n[t][0] * inv_v, f[t][1] = inv_n[t][1] * inv_v;
-#pragma unroll
+#pragma unroll 1
     for (int h = 0; h < 2; ++h) {
       uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
@@ -742,8 +744,10 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
         for (int y = 0; y < 2; ++y) {
           uint32_t hi, lo;
           // (a hidden token's norm may be anything)
-          const float n0 = sc[h][t][2 * y] == 0.0f ? 0.0f : nv[h][y], n1 = sc[h][t][2 * y + 1] == 0.0f ? 0.0f : nv[h][y];
-          ar_split(sc[h][t][2 * y], n0, sc[h][t][2 * y + 1], n1, hi, lo);
+          const float v = h == 0 ? nv[0][y] : nv[1][y];
+          const float n0 = sc[0][t][2 * y] == 0.0f ? 0.0f : v, n1 = sc[0][t][2 * y + 1] == 0.0f ? 0.0f : v;
+          ar_split(sc[0][t][2 * y], n0, sc[0][t][2 * y + 1], n1, hi, lo);
+          sc[0][t][2 * y] = sc[1][t][2 * y], sc[0][t][2 * y + 1] = sc[1][t][2 * y + 1];
           ph[t][y] = ar_transpose(hi);
           if (SPLIT) pl[t][y] = ar_transpose(lo);
         }
@@ -1133,7 +1137,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
         for (int half = 0; half < 2; ++half) {
           const int t0 = strip * AR_STRIP + 32 * half;
           const bool seen = !open_to_none(t0, t0 + 32);
-          float sc[2][NT][4];
+          float sc[2][NT][4] = {};
           if (seen || (SPLIT && half == 0)) strip_scores(sc, half, ts);  // (SPLIT: the second half's list begins where the first's ends)
           if (half == 1) {
             __syncwarp();  // the key half has been read
