@@ -34,6 +34,7 @@ struct AttendArgs {
   float* partials;               // per unit, unit_stride floats apart: [row][ns_cold + ns_hot][2 + D]
   int64_t unit_stride;
   void* plan;                    // the rows form's
+  int32_t hot_cost;              // and its division of work: of a window tile
   // flags of the tiled kernels per unit: not zero, the unit is left to the general kernel (null: none)
   const int32_t* left;
   int32_t layer, seq_begin, seq_count, n_tokens, q_dtype;

@@ -47,7 +47,12 @@ constexpr int NT = 1;
 constexpr int AR_STRIP = 64;       // of them, in an item of the list
 constexpr int AR_HOT = 32;         // window tokens of an item
 constexpr int AR_PITCH = TQ_D * 2 + 16, AR_PITCH32 = TQ_D * 4 + 16;  // bytes of a window row in shared memory
-constexpr int AR_COST = 4, AR_HOT_COST = 3;  // how long a strip takes, and a tile of the window
+// How long a strip takes, by whether operands are pairs, and a tile of the window beside it.  Measured, tile to strip:
+// bfloat16 queries, 16 x 8192 tokens 2:4 76 us, 3:4 72, 4:4 79; 8 x 8000 and five tokens 100, 99, 108; float16 ones on a
+// float16 window, 24 ragged sequences, 3:8 68, 4:8 73, 5:8 74, 6:8 75; float32 ones on a float32 window, 32 heads of
+// 2500 tokens, 3:8 44, 4:8 37, 5:8 37, 6:8 41.
+TQ_HD constexpr int ar_cost(bool split) { return split ? 8 : 4; }
+inline int ar_hot_cost(int q_dtype, int kv_dtype) { return q_dtype != TQ_BF16 && kv_dtype == TQ_F32 ? 4 : 3; }
 constexpr int AR_SEQS = 64;        // sequences of a launch
 constexpr int AR_LIST = 256;       // outliers of a strip that are copied ahead (160 is usual)
 
@@ -193,7 +198,7 @@ struct ArWork {
   AttendTiles strip, hot;
   int cold;  // tokens in blocks
   TQ_DEV int items() const { return strip.count() + hot.count(); }
-  TQ_DEV int cost() const { return AR_COST * strip.count() + AR_HOT_COST * hot.count(); }
+  TQ_DEV int cost(int of_strip, int of_hot) const { return of_strip * strip.count() + of_hot * hot.count(); }
 };
 TQ_DEV ArWork ar_work(const AttendArgs& a, int n, int q_n) {
   ArWork w;
@@ -216,7 +221,7 @@ struct ArPlan {
 template <bool SPLIT, int VB>
 __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows_kernel(AttendArgs a) {
   using Sh = ArShape<SPLIT, VB>;
-  constexpr int N = Sh::N, WARPS = Sh::WARPS, THREADS = 32 * WARPS;
+  constexpr int N = Sh::N, WARPS = Sh::WARPS, THREADS = 32 * WARPS, COST = ar_cost(SPLIT);
   constexpr int VGB = TQ_GROUP_TOK * TQ_D * VB / 8;
   extern __shared__ __align__(128) uint8_t ar_shared[];
   ArShared<SPLIT, VB>& sh = *(ArShared<SPLIT, VB>*)ar_shared;
@@ -244,7 +249,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
         const AttendSeq sq = attend_seq(a, s);
         sh.seq[s] = make_int2(sq.n, sq.q_n);
         const ArWork w = ar_work(a, sq.n, sq.q_n);
-        cost[i] = (int64_t)w.cost() * (H * ar_tiles(a, sq.q_n, N));
+        cost[i] = (int64_t)w.cost(COST, a.hot_cost) * (H * ar_tiles(a, sq.q_n, N));
         most_strip = max(most_strip, w.strip.count());
         most_hot = max(most_hot, w.hot.count());
       }
@@ -269,13 +274,13 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   }
   __syncthreads();
   // Shares of equal cost: what starts in [k share, (k + 1) share) is warp k's.  A row's strips then meet at most
-  // AR_COST * (strips - 1) / share + 2 warps, its window tiles likewise, which have to fit their slots; and
+  // COST * (strips - 1) / share + 2 warps, its window tiles likewise, which have to fit their slots; and
   // no share is smaller than a strip's cost, so that every warp between a row's first and last has a part.
   const int workers = gridDim.x * WARPS;
   const int64_t total = sh.cum[AR_SEQS];
-  int64_t share = max((total + workers - 1) / workers, (int64_t)AR_COST);
-  share = max(share, (int64_t)((AR_COST * sh.most[0] + a.ns_cold - 3) / (a.ns_cold - 2)));
-  share = max(share, (int64_t)((AR_HOT_COST * sh.most[1] + a.ns_hot - 3) / (a.ns_hot - 2)));
+  int64_t share = max((total + workers - 1) / workers, (int64_t)COST);
+  share = max(share, (int64_t)((COST * sh.most[0] + a.ns_cold - 3) / (a.ns_cold - 2)));
+  share = max(share, (int64_t)((a.hot_cost * sh.most[1] + a.ns_hot - 3) / (a.ns_hot - 2)));
   if (blockIdx.x == 0) {
     ArPlan* plan = (ArPlan*)a.plan;
     if (tid == 0) plan->share = share;
@@ -312,24 +317,24 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
     }
     s = x;
     enter_seq();
-    const uint32_t cost = (uint32_t)w.cost();
+    const uint32_t cost = (uint32_t)w.cost(COST, a.hot_cost);
     // (a sequence's cost may pass 32 bits, a row's does not)
     const int64_t in = at - sh.cum[s];
     const int row = in >> 31 == 0 ? (int)((uint32_t)in / cost) : (int)(in / cost);
-    const int off = (int)(in - (int64_t)row * cost), strips = AR_COST * row_strips;
+    const int off = (int)(in - (int64_t)row * cost), strips = COST * row_strips;
     begin = at - off;
     head = row / row_tiles, rt = row - head * row_tiles;
     if (off < strips) {
-      it = (off + AR_COST - 1) / AR_COST;
-      at = begin + AR_COST * it;
+      it = (off + COST - 1) / COST;
+      at = begin + COST * it;
     } else {
-      const int k = (off - strips + AR_HOT_COST - 1) / AR_HOT_COST;
+      const int k = (off - strips + a.hot_cost - 1) / a.hot_cost;
       it = row_strips + k;
-      at = begin + strips + AR_HOT_COST * k;
+      at = begin + strips + a.hot_cost * k;
     }
   }
   auto next_row = [&]() {  // false: there is none
-    begin += w.cost();
+    begin += w.cost(COST, a.hot_cost);
     at = begin;
     it = 0;
     if (++rt < row_tiles) return true;
@@ -1052,7 +1057,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
 
   // ---- a state
   auto flush = [&](bool hot) {
-    const int64_t from = hot ? begin + AR_COST * row_strips : begin;
+    const int64_t from = hot ? begin + COST * row_strips : begin;
     const int slot = (hot ? a.ns_cold : 0) + (int)(me - ar_div(from, share));
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -1124,7 +1129,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
       reset();
       bool new_page = true;
       for (;;) {
-        at += AR_COST;
+        at += COST;
         const int i1 = it + 1;
         const bool last = i1 >= row_strips || at >= stop;
         const int next = last ? strip : w.strip.at(i1);
@@ -1185,7 +1190,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
       const int n = sh.seq[s].x;
       ring = uix * (size_t)g.hot_cap * TQ_D;
 #pragma unroll 1
-      for (; it < row_items && at < stop; ++it, at += AR_HOT_COST) {
+      for (; it < row_items && at < stop; ++it, at += a.hot_cost) {
         const int t0 = w.cold + w.hot.at(it - row_strips) * AR_HOT;
         slot0 = t0 % g.hot_cap;
         if (open_to_none(t0, min(t0 + AR_HOT, n))) continue;
@@ -1214,7 +1219,7 @@ __global__ void __launch_bounds__(AC_THREADS, 2) attend_rows_combine_kernel(Atte
   __shared__ __align__(16) float cs[TQ_D][4], ys[4][ROWS][TQ_D], hs[4][TQ_D], ls[4][TQ_D], ms[4];
   const tq_geom& g = a.g;
   const int tid = threadIdx.x, e = tid % TQ_D, h = tid / TQ_D;
-  const int H = g.n_kv_heads, G = g.group;
+  const int H = g.n_kv_heads, G = g.group, cost = ar_cost(a.q_dtype != TQ_BF16);
   float pi[TQ_D / 4];
 #pragma unroll
   for (int d = 0; d < TQ_D / 4; ++d) pi[d] = a.tables->pi[(32 * h + d) * TQ_D + e];
@@ -1232,10 +1237,10 @@ __global__ void __launch_bounds__(AC_THREADS, 2) attend_rows_combine_kernel(Atte
       const int4 seq = plan->seq[s];
       const int64_t before = plan->cum[s];
       if (row / tile < seq.z) {
-        const int64_t begin = before + (int64_t)(head * seq.z + row / tile) * (AR_COST * seq.x + AR_HOT_COST * seq.y);
-        const int64_t middle = begin + AR_COST * seq.x;
-        const int nc = seq.x > 0 ? (int)(ar_div(middle - AR_COST, share) - ar_div(begin, share)) + 1 : 0;
-        const int nh = seq.y > 0 ? (int)(ar_div(middle + AR_HOT_COST * (seq.y - 1), share) - ar_div(middle, share)) + 1 : 0;
+        const int64_t begin = before + (int64_t)(head * seq.z + row / tile) * (cost * seq.x + a.hot_cost * seq.y);
+        const int64_t middle = begin + cost * seq.x;
+        const int nc = seq.x > 0 ? (int)(ar_div(middle - cost, share) - ar_div(begin, share)) + 1 : 0;
+        const int nh = seq.y > 0 ? (int)(ar_div(middle + a.hot_cost * (seq.y - 1), share) - ar_div(middle, share)) + 1 : 0;
         const float* base = attend_partial(a, unit, row, 0);
         float M = -INFINITY;
         constexpr int BATCH = 4, STEP = ROWS == 4 ? 1 : 4;
@@ -1354,13 +1359,16 @@ AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens) {
   const int64_t hot = (std::min(tokens, g.hot_window) + AR_HOT - 1) / AR_HOT;
   const int64_t rows = (int64_t)std::min(a.seq_count, AR_SEQS) * g.n_kv_heads * ((a.rows + 8 * NT - 1) / (8 * NT));
   const int64_t workers = (int64_t)a.sm_count * (a.q_dtype == TQ_BF16 ? ArShape<false, 3>::WARPS : ArShape<true, 3>::WARPS);
-  const int64_t share = std::max<int64_t>((AR_COST * strips + AR_HOT_COST * hot) * ((rows + 1) / 2) / workers, AR_COST);
-  p.ns_cold = (int)std::min<int64_t>(AR_COST * strips / share + 3, 1024);
-  p.ns_hot = (int)std::min<int64_t>(AR_HOT_COST * hot / share + 3, 64);
+  const int cost = ar_cost(a.q_dtype != TQ_BF16), hot_cost = ar_hot_cost(a.q_dtype, g.kv_dtype);
+  const int64_t share = std::max<int64_t>((cost * strips + hot_cost * hot) * ((rows + 1) / 2) / workers, cost);
+  p.ns_cold = (int)std::min<int64_t>(cost * strips / share + 3, 1024);
+  p.ns_hot = (int)std::min<int64_t>(hot_cost * hot / share + 3, 64);
   return p;
 }
 
-int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st) {
+int tq_launch_attend_rows(const AttendArgs& base, cudaStream_t st) {
+  AttendArgs a = base;
+  a.hot_cost = ar_hot_cost(a.q_dtype, a.g.kv_dtype);
   if (a.q_dtype == TQ_BF16) return a.g.value_bits == 4 ? launch_rows<false, 4>(a, st) : launch_rows<false, 3>(a, st);
   return a.g.value_bits == 4 ? launch_rows<true, 4>(a, st) : launch_rows<true, 3>(a, st);
 }
