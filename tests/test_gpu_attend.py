@@ -353,6 +353,17 @@ def test_empty_calls_and_refusals(torch):
             ctx.attend(args.pop("layer"), args.pop("q"), **args)
 
 
+def test_a_refused_step_appends_nothing(torch):
+    ctx = _ctx(n_seqs=1, n_kv_heads=2, n_q_heads=4, kv_dtype="bfloat16")
+    q, k, v = (torch.zeros(1, 3, h, 128, dtype=torch.bfloat16, device="cuda") for h in (4, 2, 2))
+    f = torch.ones(64, device="cuda")
+    for bad in (dict(window=0), dict(sinks=-1), dict(eps=-1.0), dict(layer=1), dict(v=v[:, :2]), dict(seq_begin=1)):
+        args = {"layer": 0, "q": q, "k": k, "v": v, "inv_freq": f, **bad}
+        with pytest.raises(ValueError):
+            ctx.step(**args)
+    assert ctx.lengths(0, 0)[0] == 0
+
+
 @pytest.mark.parametrize("dtype, chunks", [("bfloat16", [700, 1, 1, 40, 1, 300]), ("float32", [30, 1, 600, 5])])
 def test_a_layer_from_projections_to_output(torch, dtype, chunks):
     """step: norm and rotation, append, attention; the keys that the cache holds are the rotated ones."""
@@ -505,7 +516,16 @@ def test_hf_layers_attend_chunks_and_windows(torch, window):
         k, v = (torch.randn(2, 2, t, 128, generator=gen, device="cuda").bfloat16() for _ in range(2))
         kk, vv = cache.layers[0].update(k, v)
         n += t
-        if n == t:
+        if n == t:  # a prompt, on its own keys and values
+            got = hf_cache.turboquant_attention_forward(module, q, kk, vv, None, scaling=128**-0.5)[0]
+            j = torch.arange(t, device="cuda")
+            sees = (j <= j[:, None]) & (j > j[:, None] - (window or t))
+            qk = (q.double().view(2, 2, 2, t, 128) @ k.double()[:, :, None].transpose(3, 4)) / math.sqrt(128)
+            pr = torch.softmax(qk.masked_fill(~sees, -math.inf), 4)
+            want = (pr @ v.double()[:, :, None]).view(2, 4, t, 128).transpose(1, 2)
+            # (bfloat16 probabilities and values in that product at worst: a step of each, and the output's)
+            top = v.double().abs().amax()
+            assert bool(((got.double() - want).abs() <= 2.0**-8 * 2 * top + 2.0**-8 * want.abs()).all())
             continue
         p, j = torch.arange(n - t, n, device="cuda")[:, None], torch.arange(n, device="cuda")
         sees = (j <= p) & (j > p - window) if window else j <= p

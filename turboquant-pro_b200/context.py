@@ -365,6 +365,8 @@ class KVContext:
         tokens alike."""
         if v.dim() != 4 or v.shape != k.shape:
             raise ValueError(f"k and v differ in shape: {tuple(k.shape)} and {tuple(v.shape)}")
+        if (window is not None and window < 1) or sinks < 0:  # (before anything is appended)
+            raise ValueError(f"window must be at least 1 (or None) and sinks not negative, got {window}, {sinks}")
         q, k = self.norm_rope(layer, q, k, inv_freq, q_weight=q_weight, k_weight=k_weight, eps=eps,
                               seq_begin=seq_begin)
         self.append(layer, k, v, seq_begin)

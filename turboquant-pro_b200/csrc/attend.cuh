@@ -6,9 +6,10 @@
 // (sequence, KV head) unit are numbered i * G + g: neighbouring rows see nearly the same tokens, so a tile
 // of rows reads the codes once for all query heads of the group.
 //
-// Every kernel leaves states (m, l, o[D]) per (unit, row, split): m in units of log 2, o un-normalised; of
-// the first ns_cold splits in the values' code space, of the others in the original basis.  A combine
-// kernel merges them in split order, applies the inverse rotation once and rounds to the output's type.
+// The kernels for few rows and the general ones leave states (m, l, o[D]) per (unit, row, split): m in units of
+// log 2, o un-normalised; of the first ns_cold splits in the values' code space, of the others in the original basis.  A
+// combine kernel merges them in split order, applies the inverse rotation once and rounds to the output's type.
+// (Those for many rows have states of their own, all in code space.)
 #pragma once
 
 #include <limits.h>
@@ -35,7 +36,7 @@ struct AttendArgs {
   int64_t unit_stride;
   void* plan;                    // the rows form's
   int32_t hot_cost;              // and its division of work: of a window tile
-  // flags of the tiled kernels per unit: not zero, the unit is left to the general kernel (null: none)
+  // flags of the kernels for many rows, per unit: not zero, the unit is left to the general form (null: none)
   const int32_t* left;
   int32_t layer, seq_begin, seq_count, n_tokens, q_dtype;
   int32_t window, sinks;  // window: INT_MAX without one

@@ -85,9 +85,13 @@ def _mask_is_causal(mask, t: int, n: int, window) -> bool:
         return _mask_is_open(mask if mask.dtype == torch.bool else mask != 0)
     if tuple(mask.shape[-2:]) != (t, n):
         return False
-    p, j = torch.arange(n - t, n, device=mask.device)[:, None], torch.arange(n, device=mask.device)
-    sees = j <= p if window is None else (j <= p) & (j > p - window)
-    return bool(((mask if mask.dtype == torch.bool else mask >= 0) == sees).all())
+    return bool(((mask if mask.dtype == torch.bool else mask >= 0) == _causal(t, n, window, mask.device)).all())
+
+
+def _causal(t: int, n: int, window, device):
+    """What the newest ``t`` of ``n`` tokens see, as booleans ``[t, n]``."""
+    p, j = torch.arange(n - t, n, device=device)[:, None], torch.arange(n, device=device)
+    return j <= p if window is None else (j <= p) & (j > p - window)
 
 
 class _SharedContext:
@@ -294,6 +298,10 @@ def turboquant_attention_forward(module, query, key, value, attention_mask, drop
                 and not (query.requires_grad and torch.is_grad_enabled())
                 and _mask_is_causal(attention_mask, t, n, window)):
             return layer.ctx.attend(layer.layer_idx, query.transpose(1, 2), window=window), None
+        if n == t and window is not None and n > window and attention_mask is None \
+                and is_causal is not False and getattr(module, "is_causal", True):
+            # a prompt on its own K/V: the window that no mask brings along
+            attention_mask = _causal(t, n, window, query.device)[None, None]
     if layer is not None and key.shape[2] != layer.get_seq_length():
         # a multi-token query on top of stored history, a masked batch, a windowed or capped
         # layer: the dense history
