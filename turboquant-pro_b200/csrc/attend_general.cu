@@ -28,6 +28,35 @@ struct AgFixed {
   float v[AG_T][AG_KS];
   float grid[16], cent[16];
 };
+// 32 channels of a window row, 16 bytes at a time; whether all are numbers and finite
+TQ_DEV bool ag_row(const void* rows, size_t at, int dt, float* to) {
+  bool ok = true;
+  if (dt == TQ_F32) {
+    const float4* from = (const float4*)((const float*)rows + at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 x = from[i];
+      *(float4*)(to + 4 * i) = x;
+      ok &= isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w);
+    }
+    return ok;
+  }
+  const uint4* from = (const uint4*)((const uint16_t*)rows + at);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 u = from[i];
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float2 f;
+      if (dt == TQ_F16) f = __half22float2(*(const __half2*)&w[j]);
+      else f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+      *(float2*)(to + 8 * i + 2 * j) = f;
+      ok &= isfinite(f.x) && isfinite(f.y);
+    }
+  }
+  return ok;
+}
 template <int RPT>
 struct AgShared : AgFixed {
   float q[16 * RPT][AG_KS];
@@ -155,12 +184,8 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
       } else if (!is_cold) {
         const size_t at = hot_offset_elems(g, a.layer, a.seq_begin + s, head) +
                           (size_t)(t % g.hot_cap) * TQ_D + d0;
-#pragma unroll 8
-        for (int i = 0; i < 32; ++i) {
-          kr[i] = attend_ld(a.hot_k, at + i, g.kv_dtype);
-          vr[i] = attend_ld(a.hot_v, at + i, g.kv_dtype);
-          odd |= !isfinite(vr[i]);
-        }
+        ag_row(a.hot_k, at, g.kv_dtype, kr);
+        odd |= !ag_row(a.hot_v, at, g.kv_dtype, vr);
       } else {
         const int b = t / S, slot = t - b * S;
         const uint8_t* page = a.pages + page_offset(g, a.layer, a.seq_begin + s, head, b);
@@ -196,10 +221,13 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
     }
     odd = __syncthreads_or(odd);
     if (is_cold && g.outlier_k > 0) {
-      for (int b = t0 / S; b * S < t1; ++b) {
+      // (a block at a time by all, or, where a tile has several, by a warp each: their lists' places are loads that
+      // depend on one another)
+      const bool many = S < AG_T;
+      for (int b = t0 / S + (many ? warp : 0); b * S < t1; b += many ? AG_THREADS / 32 : 1) {
         const PageMeta pm = a.page_meta[uix * g.max_blocks + b];
         const size_t slab = uix * (size_t)g.pool_entries + pm.off;
-        for (uint32_t e = tid; e < pm.cnt; e += AG_THREADS) {
+        for (uint32_t e = many ? lane : tid; e < pm.cnt; e += many ? 32 : AG_THREADS) {
           const uint32_t w = a.pool_dec[slab + e];
           const int t = b * S + (int)(w >> 24);
           if (t >= t0 && t < t1)
