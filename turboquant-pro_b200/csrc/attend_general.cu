@@ -24,7 +24,7 @@ constexpr int AG_KS = TQ_D + 4;     // floats per row of keys, values and querie
 constexpr int AG_PS = AG_T + 4;     // floats per row of probabilities
 
 struct AgFixed {
-  float k[AG_T][AG_KS];
+  float k[AG_T][AG_KS];  // and, when the scores have been formed, the probabilities: two CTAs an SM have room then
   float v[AG_T][AG_KS];
   float grid[16], cent[16];
 };
@@ -33,7 +33,7 @@ TQ_DEV bool ag_row(const void* rows, size_t at, int dt, float* to) {
   bool ok = true;
   if (dt == TQ_F32) {
     const float4* from = (const float4*)((const float*)rows + at);
-#pragma unroll
+#pragma unroll 4
     for (int i = 0; i < 8; ++i) {
       const float4 x = from[i];
       *(float4*)(to + 4 * i) = x;
@@ -42,7 +42,7 @@ TQ_DEV bool ag_row(const void* rows, size_t at, int dt, float* to) {
     return ok;
   }
   const uint4* from = (const uint4*)((const uint16_t*)rows + at);
-#pragma unroll
+#pragma unroll 2
   for (int i = 0; i < 4; ++i) {
     const uint4 u = from[i];
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -60,8 +60,8 @@ TQ_DEV bool ag_row(const void* rows, size_t at, int dt, float* to) {
 template <int RPT>
 struct AgShared : AgFixed {
   float q[16 * RPT][AG_KS];
-  float p[16 * RPT][AG_PS];
 };
+static_assert(64 * AG_PS <= AG_T * AG_KS, "the probabilities' place");
 
 // The value-layout codes of token `t` of a block, channels d0 .. d0 + 31, times `f`.
 TQ_DEV void ag_codes(const uint8_t* codes, int bits, int t, int d0, const float* cent, float f, float* to) {
@@ -196,7 +196,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
           const uint32_t w[4] = {cw.x, cw.y, cw.z, cw.w};
           const float* sc = (const float*)(page + g.scale_off) + d0;
           const float* mu = (const float*)(page + g.mean_off) + d0;
-#pragma unroll
+#pragma unroll 4
           for (int i = 0; i < 32; i += 4) {
             const float4 x = *(const float4*)(sc + i), y = *(const float4*)(mu + i);
             const uint32_t c = w[i >> 3] >> (4 * (i & 7));
@@ -237,6 +237,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
       __syncthreads();
     }
 
+    float (*const prob)[AG_PS] = (float (*)[AG_PS])&sh.k[0][0];
     // ---- scores: rows ty * RPT .., tokens tx + 16 j
     float x[RPT][4];
 #pragma unroll
@@ -269,6 +270,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[r][j] += y[r][j];
     }
+    __syncthreads();  // (the keys have been read)
 #pragma unroll
     for (int r = 0; r < RPT; ++r) {
       bool sees[4];
@@ -293,7 +295,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
       for (int j = 0; j < 4; ++j) {
         const float p = sees[j] ? tq_exp2(x[r][j] - by) : 0.0f;
         l[r] += p;
-        sh.p[ty * RPT + r][tx + 16 * j] = odd && !sees[j] ? -1.0f : p;
+        prob[ty * RPT + r][tx + 16 * j] = odd && !sees[j] ? -1.0f : p;
       }
     }
     __syncwarp();  // (a row's sixteen threads are in one warp)
@@ -304,7 +306,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
       for (int t = 0; t < AG_T; t += 4) {
         float4 pp[RPT];
 #pragma unroll
-        for (int r = 0; r < RPT; ++r) pp[r] = *(const float4*)&sh.p[ty * RPT + r][t];
+        for (int r = 0; r < RPT; ++r) pp[r] = *(const float4*)&prob[ty * RPT + r][t];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const float4 va = *(const float4*)&sh.v[t + u][4 * tx], vc = *(const float4*)&sh.v[t + u][64 + 4 * tx];
@@ -322,7 +324,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
       for (int t = 0; t < AG_T; ++t)
 #pragma unroll
         for (int r = 0; r < RPT; ++r) {
-          const float p = sh.p[ty * RPT + r][t];
+          const float p = prob[ty * RPT + r][t];
           if (p < 0.0f) continue;
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -346,7 +348,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
 }
 
 template <int RPT>
-__global__ void __launch_bounds__(AG_THREADS) attend_general_kernel(AttendArgs a, int row_tiles) {
+__global__ void __launch_bounds__(AG_THREADS, 2) attend_general_kernel(AttendArgs a, int row_tiles) {
   extern __shared__ __align__(16) uint8_t ag_smem[];
   ag_item(a, row_tiles, (int)blockIdx.x, *(AgShared<RPT>*)ag_smem);
 }
