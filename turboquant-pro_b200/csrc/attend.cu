@@ -56,21 +56,25 @@ int most_tokens(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
 //   ROWS 25 + (0.085 | 0.165) W tiles        TILES 50 + (0.42 | 0.64) W
 // e.g. one sequence of 8192, 8 KV heads, bfloat16: 64 rows 68 against 76, 128 rows 108 against 77; of 32768: 32 rows
 // 100 against 149, 64 rows 177 against 150; 8 of 8192: 204 against 264, 393 against 266.  ROWS is written for blocks of
-// 256 tokens: with others TILES (50 to 920 us by the general form for 4 to 64 rows of 1000 to 64000 tokens, 51 to 250
-// with tiles).  float32 queries, which TILES would round: ROWS up to 64 rows, GENERAL above (one
-// sequence of 8000: 64 rows 130 against 177, 512 rows 813 against 763; 8 of 2000: 354 against 388, 1295 against 1071
-// at 256).
+// 256 tokens.  With others it is between TILES and, up to 64 rows, GENERAL:
+//   GENERAL up to 16 rows 26 + 0.9 W, above 40 + 1.7 W
+// (8 KV heads, bfloat16, GENERAL against TILES: one sequence, a window of 100: 4 rows 17 and 38, 64 rows 32 and 41; one
+// of 1000: 4 rows 37 and 52, 32 rows 57 and 53, 64 rows 66 and 55; one of 4000: 61 and 58, 89 and 60, 98 and 61.)
+// float32 queries, which TILES would round: ROWS up to 48 rows, GENERAL above (ROWS against GENERAL, four
+// sequences of 8000, 8 KV heads: 32 rows 222 and 344, 48: 311 and 351, 64: 394 and 361, 128: 740 and 693; eight of 2000, 32
+// KV heads: 32 rows 527 and 666, 64: 1100 and 729).
 Form choose(const tq_ctx* ctx, const tq_attend_args* r, int n) {
   const tq_geom& g = ctx->g;
   const int rows = r->n_tokens * g.group;
   const bool channels = g.key_mode != TQ_KEYS_POLAR && !ctx->force_generic, blocks = g.block_tokens == 256;
   if (!channels) return GENERAL;
-  if (r->q_dtype == TQ_F32) return blocks && rows <= 64 ? ROWS : GENERAL;
-  if (!blocks) return TILES;
+  if (r->q_dtype == TQ_F32) return blocks && rows <= 48 ? ROWS : GENERAL;
   const double seen = r->window == 0 ? n : std::min((double)n, (double)r->window + r->n_tokens + r->sinks);
   const double w = seen * r->seq_count * g.n_kv_heads / 1000.0;
   const bool f16 = r->q_dtype == TQ_F16;
-  return 25.0 + (f16 ? 0.165 : 0.085) * w * ((rows + 7) / 8) <= 50.0 + (f16 ? 0.64 : 0.42) * w ? ROWS : TILES;
+  const double tiles = 50.0 + (f16 ? 0.64 : 0.42) * w;
+  if (!blocks) return rows <= 64 && (rows <= 16 ? 26.0 + 0.9 * w : 40.0 + 1.7 * w) <= tiles ? GENERAL : TILES;
+  return 25.0 + (f16 ? 0.165 : 0.085) * w * ((rows + 7) / 8) <= tiles ? ROWS : TILES;
 }
 
 // Splits of the tokens: enough CTAs for the GPU, of what is visible in the longest sequence, in blocks and in
