@@ -11,7 +11,8 @@
 // A value that is not finite must not reach rows that do not see its token (0 * inf): a tile that holds
 // one is summed with the masked products left out one by one.
 //
-// Bound by the FP32 pipe (large calls) and by the dequantisation into shared memory (few rows).
+// Bound by the FP32 pipe and the loads that feed it at two CTAs an SM (large calls: 200 tokens of 28 query heads on 3 x
+// 6850, float32, 1.49 ms), and by the chain of loads of the dequantisation into shared memory (few rows).
 #include <algorithm>
 
 #include "attend.cuh"
@@ -369,8 +370,8 @@ __global__ void __launch_bounds__(AG_THREADS) attend_left_kernel(AttendArgs a, i
 // ---------------------------------------------------------------------------------------
 // Merge of a row's states, a CTA per row and a thread per channel.  The splits are visited in order, so the result
 // depends on nothing else; a state without a sum takes no part, one whose sum is not a number does.  (Sixteen rows
-// a CTA, which read Pi once for all, took longer at every number of rows: 218 us against 61 for 128 rows of
-// 4000 tokens, 665 against 655 for 51200 rows with a window of 64.)
+// a CTA, which read Pi once for all, took longer at every number of rows: by 157 us for 128 rows of 4000
+// tokens, by 10 us for 51200 rows with a window of 64.)
 // ---------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(TQ_D) attend_combine_kernel(AttendArgs a) {
   const tq_geom& g = a.g;
@@ -429,8 +430,8 @@ int launch_general(const AttendArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-// Tiles of 16 rows, or of 64 with a fourth of the loads per product: 4 to 16 rows 59 to 62 us against 92 to 96 (4000 tokens,
-// 8 KV heads), 32 rows 100 against 99, 64 rows 162 against 108.
+// Tiles of 16 rows, or of 64 with a fourth of the loads per product: 4 to 16 rows 54 to 56 us against 69 to 71 (4000
+// float32 tokens, 8 KV heads), 32 rows 94 against 73, 64 rows 160 against 77.
 int tq_launch_attend_general(const AttendArgs& a, cudaStream_t st) {
   return a.rows <= 16 ? launch_general<1>(a, st) : launch_general<4>(a, st);
 }

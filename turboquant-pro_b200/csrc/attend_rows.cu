@@ -33,7 +33,7 @@
 // Bound by look-ups, products and their latencies at twelve warps an SM: 43 % of the issue slots, a seventh of the
 // waiting for instructions (the code of all formats is long); at one row tile the codes are read once.  Measured, 8 KV
 // heads, one token: 16 sequences of 8192 with a window of 4096 72 us, of these the merge's tail 10; 8 sequences of
-// 8000 and five tokens, three row tiles, 99 us; one sequence, window 1024, 18.6 us, a chain of latencies.
+// 8000 and five tokens, three row tiles, 99 us; one sequence, window 1024, 19 us, a chain of latencies.
 #include <algorithm>
 
 #include "attend.cuh"
