@@ -1,0 +1,36 @@
+"""KVContext.attend at the ends of its arguments' ranges, in all of its forms: against attention in 64 bits over
+the dequantised keys and values, within the bounds that ``test_gpu_attend.py`` derives."""
+
+from __future__ import annotations
+
+import pytest
+
+from test_gpu_attend import _check, _ctx, _fill
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+
+    if not torch.cuda.is_available():
+        pytest.fail("CUDA device required for -m gpu tests")
+    return torch
+
+
+# rows of one KV head and tokens of the window that take each form: few rows, many, general
+FORMS = [(2, 512), (300, 512), (300, 200), (2, 200)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("rows, hot", FORMS)
+def test_largest_windows_and_sinks(torch, dtype, rows, hot):
+    gen = torch.Generator(device="cuda").manual_seed(51)
+    ctx = _ctx(n_seqs=2, n_kv_heads=1, n_q_heads=2, kv_dtype=dtype, hot_window=hot)
+    _fill(torch, ctx, [1300, 600], gen)
+    q = torch.randn(2, rows, 2, 128, generator=gen, device="cuda").to(getattr(torch, dtype))
+    for window, sinks in ((7, 2**31 - 1), (2**31 - 1, 0), (2**31 - 1, 2**31 - 1), (2**40, 2**40), (1, 2**31 - 80)):
+        got = ctx.attend(0, q, window=window, sinks=sinks)
+        _check(torch, ctx, got, q, window, sinks)
+    assert ctx.status() == 0

@@ -91,7 +91,9 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
     constexpr int TILE = TQ_ATTEND_TILE;
     const int64_t all = std::max<int64_t>((n + TILE - 1) / TILE, 1);
     auto seen = [&](int64_t tokens) {  // tiles that so many neighbouring query tokens see
-      return r->window == 0 ? all : std::min<int64_t>(all, (r->window + tokens + 2 * TILE - 2) / TILE + (r->sinks + TILE - 1) / TILE);
+      return r->window == 0 ? all
+                            : std::min<int64_t>(all, ((int64_t)r->window + tokens + 2 * TILE - 2) / TILE +
+                                                         ((int64_t)r->sinks + TILE - 1) / TILE);
     };
     p.cap = (int)seen(r->n_tokens);
     // splits of a tile of rows: as many as bring the rounds of CTAs nearest to even (with four tiles' time for
