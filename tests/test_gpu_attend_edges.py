@@ -34,3 +34,28 @@ def test_largest_windows_and_sinks(torch, dtype, rows, hot):
         got = ctx.attend(0, q, window=window, sinks=sinks)
         _check(torch, ctx, got, q, window, sinks)
     assert ctx.status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("rows", [60, 129, 700])
+@pytest.mark.parametrize("image", [0, 1, 5, 24])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(torch, dtype, rows, image):
+    """Many rows: the test hook withholds the copy of one operand image (keys or values, of the first tile or a
+    later one) and shortens the probe limit; the call returns, the status word has bit 1, and nothing of it is left."""
+    from turboquant_pro_b200._lib import TqError
+
+    gen = torch.Generator(device="cuda").manual_seed(52)
+    # (enough units that a CTA has a dozen tiles)
+    ctx = _ctx(n_seqs=2, n_kv_heads=37, n_q_heads=74, kv_dtype=dtype, hot_window=300)
+    _fill(torch, ctx, [2500, 2500], gen)
+    q = torch.randn(2, rows, 74, 128, generator=gen, device="cuda").to(getattr(torch, dtype))
+    good = ctx.attend(0, q, window=2200)
+    assert ctx.status() == 0 and ctx.last_launches() == 4
+    ctx.debug_wait(wait_limit=64, withhold_tile=image)
+    ctx.attend(0, q, window=2200)
+    with pytest.raises(TqError, match="wait"):
+        ctx.raise_on_timeout()
+    assert ctx.status() == 0
+    ctx.debug_wait()
+    assert torch.equal(ctx.attend(0, q, window=2200), good)
+    assert ctx.status() == 0

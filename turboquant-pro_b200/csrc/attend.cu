@@ -197,6 +197,7 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
   a.ns_cold = p.ns_cold, a.ns_hot = p.ns_hot;
   a.rows = r->n_tokens * g.group;
   a.device = ctx->device, a.sm_count = ctx->sm_count;
+  a.wait_limit = ctx->wait_limit, a.withhold = ctx->withhold_tile;
   a.unit_stride = (int64_t)a.rows * (p.ns_cold + p.ns_hot) * TQ_PART_STRIDE;
   const size_t esz = elem_size(r->q_dtype);
   ctx->last_launches = 0;

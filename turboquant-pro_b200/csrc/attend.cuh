@@ -43,6 +43,7 @@ struct AttendArgs {
   int32_t ns_cold, ns_hot;
   int32_t rows;  // of a unit: n_tokens * group
   int32_t device, sm_count;
+  int32_t wait_limit, withhold;  // test hook of the form for many rows (tq_debug_wait); 0 and -1 otherwise
 };
 
 // What a sequence holds and where its queries stand.

@@ -414,7 +414,8 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
 struct TiShared {
   alignas(128) uint8_t q[2][TI_QIMAGE];
   alignas(128) uint8_t kv[TI_SLOTS][TI_IMAGE];
-  unsigned long long full[TI_SLOTS], empty[TI_SLOTS], q_ready[2], s_full[2], s_read[2], p_full[2], o_done[2];
+  unsigned long long full[TI_SLOTS], empty[TI_SLOTS], q_ready[2], s_full[2], s_read[2], p_full[2], o_done[2],
+      drained[2];
   uint32_t tmem;
 };
 static_assert(sizeof(TiShared) <= 227 * 1024, "shared memory of one CTA");
@@ -561,6 +562,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       mbar_init(enc_smem(&sh.s_read[i]), 128);
       mbar_init(enc_smem(&sh.p_full[i]), 128);
       mbar_init(enc_smem(&sh.o_done[i]), 1);
+      mbar_init(enc_smem(&sh.drained[i]), 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -573,30 +575,34 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
   ti_fence_after();
   constexpr uint32_t tmem = 0;  // (all 512 columns are this CTA's: they begin at the first)
 
-  // Bounded waits: one that runs out sets the status bit, and the thread then waits for nothing more.
-  const int limit = TI_WAIT;
+  // Bounded waits: one that runs out sets the status bit, and the thread then waits for nothing more and starts no
+  // copies or products; those under way are waited for (with the full limit) before the CTA's memory goes.
+  const int limit = a.wait_limit > 0 ? a.wait_limit : TI_WAIT;
   bool gave_up = false;
-  auto wait = [&](unsigned long long* bar, unsigned parity) {
+  auto wait_for = [&](unsigned long long* bar, unsigned parity, int most) {
     const uint32_t at = enc_smem(bar);
     for (int i = 0; !gave_up && !ti_try_wait(at, parity);)
-      if (++i >= limit) {
+      if (++i >= most) {
         atomicOr(a.status, TQ_STATUS_WAIT_TIMEOUT);
         gave_up = true;
       }
   };
+  auto wait = [&](unsigned long long* bar, unsigned parity) { wait_for(bar, parity, limit); };
 
   if (warp == TI_SOFTMAX / 32 + 2) {
     // ---- loads: K V of tile after tile through the ring
     if (lane == 0) {
       const uint8_t* images = ta.images + (size_t)unit * ta.cap * 2 * PARTS * TI_IMAGE;
+      const int held = blockIdx.x == 0 ? a.withhold : -1;  // test hook: an image that is never copied
       int c = 0;
-      for (int k = 0; k < n; ++k) {
+      for (int k = 0; k < n && !gave_up; ++k) {
         const int t = tl.at(k_lo + k), slot_of = t < ul.head ? t : ul.head + t - ul.first;
         const uint8_t* from = images + (size_t)slot_of * 2 * PARTS * TI_IMAGE;
         for (int i = 0; i < 2 * PARTS; ++i, ++c) {
           const int slot = c % TI_SLOTS;
           if (c >= TI_SLOTS) wait(&sh.empty[slot], (c / TI_SLOTS - 1) & 1);
           if (gave_up) break;
+          if (c == held) continue;
           const uint32_t bar = enc_smem(&sh.full[slot]);
           asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(TI_IMAGE) : "memory");
           asm volatile(
@@ -608,7 +614,8 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       }
       // (the copies have all landed before the CTA's memory goes)
       gave_up = false;
-      for (int i = max(c - TI_SLOTS, 0); i < c; ++i) wait(&sh.full[i % TI_SLOTS], (i / TI_SLOTS) & 1);
+      for (int i = max(c - TI_SLOTS, 0); i < c; ++i)
+        if (i != held) wait_for(&sh.full[i % TI_SLOTS], (i / TI_SLOTS) & 1, TI_WAIT);
     }
   } else if (warp >= TI_SOFTMAX / 32) {
     // ---- products of half x
@@ -674,22 +681,28 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       wait_all(&sh.q_ready[x], 0);
       for (int i = 0; i < PARTS; ++i) landed(i);
       ti_fence_after();
-      scores(0);
+      if (!gave_up) scores(0);
 #pragma unroll 1
-      for (int k = 0; k < n_u; ++k) {
+      for (int k = 0; k < n_u && !gave_up; ++k) {
         if (k + 1 < n_u) {
           for (int i = 0; i < PARTS; ++i) landed(2 * PARTS * (k + 1) + i);
           wait_all(&sh.s_read[x], k & 1);  // (this tile's scores are in registers)
+          if (gave_up) break;
           ti_fence_after();
           scores(k + 1);
         }
         for (int i = 0; i < PARTS; ++i) landed(2 * PARTS * k + PARTS + i);
         wait_all(&sh.p_full[x], k & 1);
+        if (gave_up) break;
         ti_fence_after();
         values(k);
       }
-      gave_up = false;  // (nor are products under way when the CTA's memory goes)
-      wait_all(&sh.o_done[x], (n_u - 1) & 1);
+      // (nor are products under way when the CTA's memory goes: a barrier of one phase tells, however many of the
+      // others' there have been)
+      if (ti_elect()) umma_commit(enc_smem(&sh.drained[x]));
+      __syncwarp();
+      gave_up = false;
+      wait_for(&sh.drained[x], 0, TI_WAIT);
     }
   } else if (warp < 4 * groups) {
     // ---- a thread per row

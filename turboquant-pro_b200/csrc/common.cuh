@@ -125,7 +125,7 @@ struct tq_ctx {
   int last_q_dtype = TQ_F32;   // query element type of the most recent decode (byte accounting)
   bool force_generic = false;  // route every decode through the general-shape kernel
   bool trace_on = false;       // the tensor-core decode kernel stamps its pipeline phases
-  int wait_limit = 0;          // probes per bounded wait of the decode kernel and the encoders; 0 = default
+  int wait_limit = 0;          // probes per bounded wait of decode, attend and the encoders; 0 = default
   int withhold_tile = -1;      // test hook: the copy of this tile (key encoder: row) of CTA 0 is never started
   // optional per-kernel timing: event triples (before attention, after it, after combine)
   bool prof_on = false;
