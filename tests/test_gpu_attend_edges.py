@@ -59,3 +59,27 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(torch, dtyp
     ctx.debug_wait()
     assert torch.equal(ctx.attend(0, q, window=2200), good)
     assert ctx.status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("n, t, heads", [(1, 1, 4), (2, 1, 4), (1, 3, 4), (1, 1, 1), (3, 1, 1), (1, 5, 1), (2, 6, 1)])
+def test_views_of_odd_rows_with_sizes_of_one(torch, dtype, n, t, heads):
+    """Any strides: views of rows that are no multiple of 16 bytes, begun on and off a 16-byte boundary, where torch
+    takes tensors with sizes of one for contiguous whatever their strides."""
+    dt = getattr(torch, dtype)
+    gen = torch.Generator(device="cuda").manual_seed(53)
+    ctx = _ctx(n_seqs=n, n_kv_heads=1, n_q_heads=heads, kv_dtype=dtype)
+    _fill(torch, ctx, [700] * n, gen)
+    q = torch.randn(n, t, heads, 128, generator=gen, device="cuda").to(dt)
+    want = ctx.attend(0, q, window=90, sinks=2)
+    _check(torch, ctx, want, q, 90, 2)
+    for off in (0, 3, 8):
+        for row in (heads * 128 + 1, heads * 128 + 24):
+            flat = torch.zeros(n * t * row + 16, dtype=dt, device="cuda")
+            for strides in ((t * row, row, 128, 1), (row, n * row, 128, 1)):
+                view = flat.as_strided(q.shape, strides, off)
+                view.copy_(q)
+                assert torch.equal(ctx.attend(0, view, window=90, sinks=2), want), (off, strides)
+        wide = torch.zeros(n, t, heads, 131, dtype=dt, device="cuda")
+        wide[..., off // 3:off // 3 + 128] = q
+        assert torch.equal(ctx.attend(0, wide[..., off // 3:off // 3 + 128], window=90, sinks=2), want)

@@ -326,8 +326,15 @@ class KVContext:
                              f"on {dev}, aligned to 16 bytes")
         step = 16 // q.element_size()
         s0, s1, s2, s3 = q.stride()
+        if shape[0] == 1:  # (what a size of one strides does not count)
+            s0 = 0
+        if shape[1] == 1:
+            s1 = 0
+        if shape[2] == 1:
+            s2 = 0
         if (s3 != 1 or q.data_ptr() % 16 or s0 % step or s1 % step or s2 % step) and q.numel():
-            q = q.clone() if q.is_contiguous() else q.contiguous()
+            # (not contiguous(), which gives back a tensor that begins off a 16-byte boundary as it is)
+            q = torch.empty(shape, dtype=dtype, device=dev).copy_(q)
             s0, s1, s2, s3 = q.stride()
         a = TqAttendArgs(q.data_ptr(), out.data_ptr(), lens, None, 0, s0, s1, s2, layer, seq_begin,
                          shape[0], shape[1], codes[dtype], min(window or 0, 2**31 - 1),
