@@ -83,3 +83,42 @@ def test_views_of_odd_rows_with_sizes_of_one(torch, dtype, n, t, heads):
         wide = torch.zeros(n, t, heads, 131, dtype=dt, device="cuda")
         wide[..., off // 3:off // 3 + 128] = q
         assert torch.equal(ctx.attend(0, wide[..., off // 3:off // 3 + 128], window=90, sinks=2), want)
+
+
+def _scaled(torch, n, heads, gen, k_by, v_by=1.0):
+    k = k_by * torch.randn(1, n, heads, 128, generator=gen, device="cuda")
+    v = v_by * torch.randn(1, n, heads, 128, generator=gen, device="cuda")
+    return k, v
+
+
+@pytest.mark.parametrize("t", [1, 9])
+@pytest.mark.parametrize("by", [2.0**-20, 2.0**-13, 2.0**-6, 2.0**8, 2.0**20])
+def test_float32_digits_do_not_depend_on_the_size_of_keys_and_values(torch, t, by):
+    """Few rows: small (large) keys against large (small) queries are the same scores."""
+    gen = torch.Generator(device="cuda").manual_seed(54)
+    # (outliers are stored in half precision, which ends at 65504: keys of 2^20 have none)
+    ctx = _ctx(n_seqs=1, n_kv_heads=2, n_q_heads=4, kv_dtype="float32", outlier_frac=0.02 if by < 2.0**10 else 0.0)
+    ctx.append(0, *_scaled(torch, 1200, 2, gen, by, 1.0 / by))
+    q = torch.randn(1, t, 4, 128, generator=gen, device="cuda") / by
+    for window, sinks in ((None, 0), (300, 3)):
+        _check(torch, ctx, ctx.attend(0, q, window=window, sinks=sinks), q, window, sinks)
+
+
+@pytest.mark.parametrize("t", [1, 9])
+@pytest.mark.parametrize("by", [2.0**30, 2.0**-30])
+def test_float32_digits_do_not_depend_on_the_neighbours(torch, t, by):
+    """Few rows: every third token's keys and values are 2^30 times (a 2^30th of) the others'; where they are larger
+    a window hides them, so that the others are all there is."""
+    gen = torch.Generator(device="cuda").manual_seed(55)
+    ctx = _ctx(n_seqs=1, n_kv_heads=1, n_q_heads=4, kv_dtype="float32", outlier_frac=0.0)
+    k, v = _scaled(torch, 512, 1, gen, 1.0)
+    if by > 1.0:
+        k[0, :500:3] *= by
+        v[0, :500:3] *= by
+    else:
+        k[0, ::3] *= by
+        v[0, ::3] *= by
+    ctx.append(0, k, v)
+    q = torch.randn(1, t, 4, 128, generator=gen, device="cuda")
+    window = 14 - t if by > 1.0 else None  # (of the newest twelve and fewer, none is a larger one)
+    _check(torch, ctx, ctx.attend(0, q, window=window), q, window)

@@ -27,8 +27,8 @@
 // The uncompressed window: 16-bit rows are the A operand as they are, in their own type (ldmatrix), so that only the
 // other operand is split: a query that is exact in that type has one part, others as many as they need;
 // probabilities have two parts in fp16 and in bfloat16 (three there with SPLIT).  float32 rows are split into fp16 pairs
-// as they are read.  A tile that holds an infinity or a NaN is attended term by term instead (products with masked
-// tokens and with low parts would spread it), and so is one of float32 keys beyond fp16's range.
+// as they are read, each times a power of two of its own.  A tile that holds an infinity or a NaN is
+// attended term by term instead (products with masked tokens and with low parts would spread it).
 //
 // Bound by look-ups, products and their latencies at twelve warps an SM: 43 % of the issue slots, a seventh of the
 // waiting for instructions (the code of all formats is long); at one row tile the codes are read once.  Measured, 8 KV
@@ -895,23 +895,22 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
       ar_commit();
     };
     fetch_values(0);
-    float v_up = 1.0f, v_inv = 1.0f;
     bool odd = false;
-    if (F32) {
-      float top = 0.0f, top_k = 0.0f;
-#pragma unroll 4
-      for (int i = 0; i < min(AR_HOT, n - t0); ++i) {
-        const float4 x = *(const float4*)((const float*)a.hot_k + hot_row(i) + 4 * lane);
-        const float4 y = *(const float4*)((const float*)a.hot_v + hot_row(i) + 4 * lane);
-        top_k = fmaxf(top_k, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-        top = fmaxf(top, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
-        odd |= !(fabsf(x.x) + fabsf(x.y) + fabsf(x.z) + fabsf(x.w) + fabsf(y.x) + fabsf(y.y) + fabsf(y.z) + fabsf(y.w) < INFINITY);
-      }
-      odd |= top_k > 65504.0f;
+    // float32 rows: a power of two per token (and its inverse), so that the pairs' digits depend neither on its size nor on
+    // that of the others, hidden ones among them
+    auto row_lift = [&](const float* from, float& inverse) {  // of 32 channels, this lane's
+      float top = 0.0f;
 #pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      v_up = ar_lift(top, 13, v_inv);
-    }
+      for (int j = 0; j < 8; ++j) {
+        const float4 v = ((const float4*)from)[j];
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        odd |= !(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY);
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      return ar_lift(top, 13, inverse);
+    };
+    float nv[2][2] = {{1.0f, 1.0f}, {1.0f, 1.0f}}, v_up[2][2];  // values of tokens 16 h + 8 y + r
     float sc[2][NT][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -934,6 +933,14 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
             kw[x][4 * k] = v.x, kw[x][4 * k + 1] = v.y, kw[x][4 * k + 2] = v.z, kw[x][4 * k + 3] = v.w;
           }
       }
+      float k_up[2] = {1.0f, 1.0f}, k_inv[2] = {1.0f, 1.0f};
+      if (F32)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const size_t from = hot_row(min(16 * h + 8 * x + r, n - 1 - t0)) + 32 * c;
+          k_up[x] = row_lift((const float*)a.hot_k + from, k_inv[x]);
+          v_up[h][x] = row_lift((const float*)a.hot_v + from, nv[h][x]);
+        }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         uint32_t ah[4], al[4] = {0u, 0u, 0u, 0u};
@@ -941,8 +948,8 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const float4 v = ((const float4*)row[x])[j];
-            ar_split(v.x, 1.0f, v.y, 1.0f, ah[x], al[x]);
-            ar_split(v.z, 1.0f, v.w, 1.0f, ah[2 + x], al[2 + x]);
+            ar_split(v.x, k_up[x], v.y, k_up[x], ah[x], al[x]);
+            ar_split(v.z, k_up[x], v.w, k_up[x], ah[2 + x], al[2 + x]);
           }
         } else {
 #pragma unroll
@@ -972,7 +979,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[h][t][i] = (sum[t][i] + low[t][i]) * inv[t][i & 1];
+        for (int i = 0; i < 4; ++i) sc[h][t][i] = (sum[t][i] + low[t][i]) * inv[t][i & 1] * (F32 ? k_inv[i >> 1] : 1.0f);
     }
     if (!F32) {
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -993,10 +1000,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
       return;
     }
     float inv_n[NT][2];
-    const float nv[2][2] = {{1.0f, 1.0f}, {1.0f, 1.0f}};
     softmax(sc, t0, n, ArTiles<2>(), nv, inv_n);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) inv_n[t][0] *= v_inv, inv_n[t][1] *= v_inv;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       if (F32) {
@@ -1013,10 +1017,16 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           if (BF) ar_split_bf<SPLIT ? 3 : 2>(sc[h][t][2 * y], sc[h][t][2 * y + 1], p[t][y]);
-          else ar_split(sc[h][t][2 * y], 1.0f, sc[h][t][2 * y + 1], 1.0f, p[t][y][0], p[t][y][1]);
+          else ar_split(sc[h][t][2 * y], nv[h][y], sc[h][t][2 * y + 1], nv[h][y], p[t][y][0], p[t][y][1]);
 #pragma unroll
           for (int k = 0; k < (BF && SPLIT ? 3 : 2); ++k) p[t][y][k] = ar_transpose(p[t][y][k]);
         }
+      float up[2][2] = {};  // of tokens 2 c, 2 c + 1, and 8 further
+      if (F32)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) up[y][k] = __shfl_sync(0xffffffffu, v_up[h][y], 8 * c + 4 * k);
       const uint32_t v_at = ar_smem(rows) + (16 * h + (lane & 7) + (lane >> 4) * 8) * AR_PITCH + (lane >> 3 & 1) * 16;
 #pragma unroll
       for (int mt = 0; mt < 8; ++mt) {
@@ -1025,7 +1035,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
 #pragma unroll
           for (int x = 0; x < 4; ++x) {  // channels r, r + 8; tokens 2 c, 2 c + 1, and 8 further
             const float* f = (const float*)(rows + (2 * c + 8 * (x >> 1)) * AR_PITCH32) + 16 * mt + r + 8 * (x & 1);
-            ar_split(f[0], v_up, f[AR_PITCH32 / 4], v_up, ah[x], al[x]);
+            ar_split(f[0], up[x >> 1][0], f[AR_PITCH32 / 4], up[x >> 1][1], ah[x], al[x]);
           }
         } else {
           ar_ldm<true>(ah, v_at + 32 * mt);
