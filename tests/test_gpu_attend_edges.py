@@ -122,3 +122,48 @@ def test_float32_digits_do_not_depend_on_the_neighbours(torch, t, by):
     q = torch.randn(1, t, 4, 128, generator=gen, device="cuda")
     window = 14 - t if by > 1.0 else None  # (of the newest twelve and fewer, none is a larger one)
     _check(torch, ctx, ctx.attend(0, q, window=window), q, window)
+
+
+@pytest.mark.parametrize("kv", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("rows, hot", [(1, 512), (9, 512), (300, 512), (5, 200), (300, 200)])
+def test_an_infinite_key_may_take_all_weight_from_its_token(torch, kv, dtype, rows, hot):
+    """A visible key of -inf where the queries are positive: its score is -inf, its weight zero, and the output that
+    of the other tokens."""
+    gen = torch.Generator(device="cuda").manual_seed(56)
+    ctx = _ctx(n_seqs=1, n_kv_heads=1, n_q_heads=2, kv_dtype=kv, hot_window=hot)
+    k, v = (x.to(ctx.kv_dtype) for x in _scaled(torch, 700, 1, gen, 1.0))
+    q = torch.randn(1, rows, 2, 128, generator=gen, device="cuda").to(getattr(torch, dtype))
+    q[..., 17] = q[..., 17].abs() + 1.0
+    k[0, 640, 0, 17] = -float("inf")  # in the uncompressed window
+    ctx.append(0, k, v)
+    kk, vv = (x[0].double() for x in ctx.dequant(0, 0, 0, 700))
+    u = 2.0**-22 if dtype == "float32" else 2.0**-11
+    p, j = torch.arange(700 - rows, 700, device="cuda")[:, None], torch.arange(700, device="cuda")
+    for window, sinks in ((None, 0), (100, 2)):
+        got = ctx.attend(0, q, window=window, sinks=sinks)[0].double()
+        sees = (j <= p) & (j != 640)  # (without the token)
+        if window is not None:
+            sees &= (j > p - window) | (j < sinks)
+        for h in range(2):
+            x = q[0, :, h].double()
+            kf = kk.masked_fill(kk.isinf(), 0.0)
+            want = torch.softmax((x @ kf.t() / 128**0.5).masked_fill(~sees, -float("inf")), 1) @ vv
+            a = (x.abs() @ kf.abs().t() / 128**0.5).masked_fill(~sees, 0.0).amax(1, keepdim=True)
+            limit = (2 * a + 4) * u * vv.abs().max() + torch.finfo(q.dtype).eps / 2 * want.abs()
+            assert bool(((got[:, h] - want).abs() <= limit).all()), (window, h)
+
+
+def test_padding_that_is_no_number_slows_nothing_down_and_stays_out(torch):
+    """Rows of a padded batch hold NaN: zeros for them, the others as without."""
+    gen = torch.Generator(device="cuda").manual_seed(57)
+    for dtype in ("float16", "bfloat16", "float32"):
+        ctx = _ctx(n_seqs=2, n_kv_heads=1, n_q_heads=2, kv_dtype=dtype)
+        _fill(torch, ctx, [900, 700], gen)
+        for rows in (9, 300):
+            q = torch.randn(2, rows, 2, 128, generator=gen, device="cuda").to(getattr(torch, dtype))
+            lens = torch.tensor([rows // 2, rows], dtype=torch.int32, device="cuda")
+            want = ctx.attend(0, q, q_lens=lens)
+            _check(torch, ctx, want, q, q_lens=lens)
+            q[0, rows // 2:] = float("nan")
+            assert torch.equal(ctx.attend(0, q, q_lens=lens), want)

@@ -28,7 +28,8 @@
 // other operand is split: a query that is exact in that type has one part, others as many as they need;
 // probabilities have two parts in fp16 and in bfloat16 (three there with SPLIT).  float32 rows are split into fp16 pairs
 // as they are read, each times a power of two of its own.  A tile that holds an infinity or a NaN is
-// attended term by term instead (products with masked tokens and with low parts would spread it).
+// attended term by term instead (products with masked tokens and with low parts would spread it); of 16-bit keys, one
+// whose scores are no numbers.
 //
 // Bound by look-ups, products and their latencies at twelve warps an SM: 43 % of the issue slots, a seventh of the
 // waiting for instructions (the code of all formats is long); at one row tile the codes are read once.  Measured, 8 KV
@@ -979,7 +980,13 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[h][t][i] = (sum[t][i] + low[t][i]) * inv[t][i & 1] * (F32 ? k_inv[i >> 1] : 1.0f);
+        for (int i = 0; i < 4; ++i) {
+          const float x = (sum[t][i] + low[t][i]) * inv[t][i & 1] * (F32 ? k_inv[i >> 1] : 1.0f);
+          sc[h][t][i] = x;
+          // An infinite key is no number next to a part that is zero, where the score may be -inf, a weight of zero.
+          // (Rows of padding may hold anything: they do not count.)
+          if (!F32) odd |= !(x == x) && pos[t][i & 1] >= 0;
+        }
     }
     if (!F32) {
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -992,7 +999,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
         const uint4 x = *(const uint4*)(rows + (2 * i + (lane >> 4)) * AR_PITCH + (lane & 15) * 16);
         carry |= ((x.x & 0x7fff7fffu) + ONE) | ((x.y & 0x7fff7fffu) + ONE) | ((x.z & 0x7fff7fffu) + ONE) | ((x.w & 0x7fff7fffu) + ONE);
       }
-      odd = (carry & 0x80008000u) != 0u;
+      odd |= (carry & 0x80008000u) != 0u;
     }
     if (__any_sync(0xffffffffu, odd)) {
       asm volatile("cp.async.wait_all;" ::: "memory");
