@@ -167,3 +167,47 @@ def test_padding_that_is_no_number_slows_nothing_down_and_stays_out(torch):
             _check(torch, ctx, want, q, q_lens=lens)
             q[0, rows // 2:] = float("nan")
             assert torch.equal(ctx.attend(0, q, q_lens=lens), want)
+
+
+def _relative(torch, ctx, got, q, window=None, sinks=0, q_lens=None, seq_begin=0):
+    """The largest relative error (2-norms over a query head's rows) against 64 bits."""
+    from test_gpu_attend import _want
+
+    worst = 0.0
+    for s in range(q.shape[0]):
+        q_n = q.shape[1] if q_lens is None else int(q_lens[s])
+        want, _ = _want(torch, ctx, 0, seq_begin + s, q[s], q_n, window, sinks)
+        off = (got[s].double() - want).norm(dim=(0, 2)) / want.norm(dim=(0, 2)).clamp_min(1e-300)
+        worst = max(worst, float(off.max()))
+    return worst
+
+
+def _step(torch, dtype):
+    """What ``_relative`` may give for scores of standard deviation one.  16-bit queries: half a step of the output's
+    type; its rounding alone is 0.42 of that in the mean square, operands and probabilities of half precision (2^-12 each, and a
+    score's by its error of 2^-12) less than 0.3 of it.  float32: 2^-20, four parts of 2^-22 (the pairs of queries, keys,
+    probabilities and values); float32 sums of 128 products are below that."""
+    return 2.0**-20 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+
+
+@pytest.mark.parametrize("kv", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("rows, hot", FORMS)
+def test_digits_do_not_depend_on_the_size_of_the_keys(torch, kv, dtype, rows, hot):
+    """Small (large) keys against large (small) queries are the same scores."""
+    dt = getattr(torch, dtype)
+    gen = torch.Generator(device="cuda").manual_seed(58)
+    for by in (2.0**-8, 1.0, 2.0**8) if "float16" in (kv, dtype) else \
+            (2.0**-28, 2.0**-20, 2.0**-13, 2.0**-6, 2.0**9):
+        # (Outliers are stored in half precision, and beside it as their distance from the grid, in half precision too:
+        # below 2^-14 both have a step of 2^-24, so that of keys of 2^-28, step 2^-24 / 2^-28 = 16, nothing is left of them
+        # in the cache itself.  Such keys have none here.)
+        ctx = _ctx(n_seqs=1, n_kv_heads=1, n_q_heads=2, kv_dtype=kv, hot_window=hot,
+                   outlier_frac=0.02 if by >= 2.0**-8 else 0.0)
+        ctx.append(0, *(x.to(ctx.kv_dtype) for x in _scaled(torch, 1300, 1, gen, by)))
+        q = (torch.randn(1, rows, 2, 128, generator=gen, device="cuda") / by).to(dt)
+        for window, sinks in ((None, 0), (700, 20)):
+            got = ctx.attend(0, q, window=window, sinks=sinks)
+            rel = _relative(torch, ctx, got, q, window, sinks)
+            assert rel <= _step(torch, dt), (by, window, rel)
+        assert ctx.status() == 0

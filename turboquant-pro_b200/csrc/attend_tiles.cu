@@ -4,13 +4,14 @@
 // attend_stage_kernel   the tokens that any row sees, 80 at a time, from codes to the two shared-memory images
 //     that tcgen05 takes as operands (fp16, K-major core matrices of 8 rows x 16 bytes), written to the workspace
 //     once instead of once per tile of rows:
-//       keys    (mean + scale * grid[code] - c) / 16, outliers put over it.  c is one vector per (sequence, KV head),
+//       keys    mean + scale * grid[code] - c, outliers put over it.  c is one vector per (sequence, KV head),
 //               the zero-point of its first block: it moves all scores of a row alike, so the softmax does not
-//               see it, and large constant channels do not eat the half-precision digits.  The 16 keeps keys to 10^6
-//               in fp16's range.
+//               see it, and large constant channels do not eat the half-precision digits.  All times the power of
+//               two that takes the tile's largest below 2^15; its inverse is kept, for the scores.
 //       values  transposed, in code space: norm * centroid[code], window tokens rotated into that space; all times
 //               the power of two that takes the tile's largest norm below 2^15, whose exponent is kept.
-//     What is not a number, or too large even so, sets the flag of its (sequence, KV head), which the general kernel
+//     What is not a number, keys beyond 2^20, and a token whose keys or values lie below 2^-20 of the tile's largest (zeros
+//     aside: its digits would fall out of fp16) set the flag of their (sequence, KV head), which the general kernel
 //     then does.
 // attend_tiles_kernel   256 rows of a (sequence, KV head) per CTA against a split of these tiles, in two halves of 128 rows.
 //     S = Q K^T into tensor memory; a group of 128 threads per half, a thread per row, makes the probabilities and
@@ -52,7 +53,7 @@ constexpr int TI_SLOTS = 8;                  // images in shared memory
 constexpr int TI_SOFTMAX = 256;              // softmax threads: one a row
 constexpr int TI_THREADS = TI_SOFTMAX + 96;  // and two warps that issue, a warp that loads
 constexpr int TI_S = 0, TI_P = TI_T, TI_HALF = 128, TI_O = 256;  // columns: scores, probabilities of a half, sums
-constexpr float TI_KEY = 16.0f;              // keys are divided by it
+constexpr float TI_KEY_MOST = 0x1p20f, TI_LEAST = 0x1p-20f;  // largest key; least part of a tile's largest
 constexpr float TI_LIFT = 7.0f, TI_GROW = 8.0f;  // probabilities reach 2^(7 + 8) at most
 constexpr int TI_POLY = 2;                   // of eight pairs of exponentials, those on the multiply-add units
 constexpr int TI_WAIT = 1 << 21;             // probes of a wait
@@ -60,7 +61,7 @@ static_assert(TI_P + TI_T / 2 <= TI_HALF && 2 * TI_HALF <= TI_O && TI_T % 16 == 
 
 struct TileArgs {
   uint8_t* images;    // [unit][cap][K hi, (K lo,) V hi, (V lo)]
-  float* exponent;    // [unit][cap]
+  float2* exponent;   // [unit][cap]: of the values; the keys' factor
   int32_t* left;      // [unit]
   float* sums;        // per unit, unit_stride floats apart: [split][row tile][channel][256]
   float* stats;       // [unit][split][row tile][2][256]
@@ -73,8 +74,9 @@ TQ_DEV AttendTiles unit_tiles(const AttendArgs& a, const AttendSeq& sq) {
   return attend_tiles(a, 0, sq.n, TI_T, sq.first, sq.q_n > 0 ? sq.n - 1 : -1);
 }
 
-TQ_DEV float ti_lift(float x, int top, float& exponent) {  // 2^(top - floor(log2 x)), and the exponent of its inverse
-  const int e = min(max((int)(__float_as_uint(x) >> 23 & 255u), 64), 254);
+// 2^(top - floor(log2 x)), and the exponent of its inverse; what is below 2^-63, or 2^(least - 127), counts as that
+TQ_DEV float ti_lift(float x, int top, float& exponent, int least = 64) {
+  const int e = min(max((int)(__float_as_uint(x) >> 23 & 255u), least), 254);
   exponent = (float)(e - 127 - top);
   return __int_as_float((254 + top - e) << 23);
 }
@@ -102,14 +104,13 @@ TQ_DEV float ti_max3_nan(float a, float b, float c) {
 constexpr int TS_THREADS = 4 * TI_T;  // four a token; two warps per 16 tokens of values
 constexpr int TS_PITCH = TQ_D * 2 + 16;  // bytes per row of window values
 constexpr int TS_VT = 16;         // window tokens that are rotated at a time
-template <bool SPLIT>
 struct StageShared {
-  alignas(16) uint8_t k[SPLIT ? 2 : 1][TI_IMAGE];  // afterwards rows of window values, as pairs hi + lo
+  alignas(16) float k[TQ_D / 4][TI_T][4];  // four channels a plane; afterwards rows of window values, as pairs hi + lo
   alignas(16) float center[TQ_D];
   float grid[16], cent[16], norm[TI_T];
-  float top[TS_THREADS / 32];
+  float top[TS_THREADS / 32], k_top[TS_THREADS / 32], part_top[4][TI_T];
 };
-static_assert(2 * TS_VT * TS_PITCH <= TI_IMAGE, "the window values' place");
+static_assert(2 * TS_VT * TS_PITCH <= 2 * TI_IMAGE, "the window values' place");
 
 // eight neighbouring elements of a window row
 TQ_DEV void ts_ld8(const void* p, size_t at, int dt, float (&x)[8]) {
@@ -134,7 +135,7 @@ TQ_DEV void ts_ld8(const void* p, size_t at, int dt, float (&x)[8]) {
 template <bool SPLIT>
 __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel(AttendArgs a, TileArgs ta) {
   extern __shared__ __align__(16) uint8_t ts_smem[];
-  StageShared<SPLIT>& sh = *(StageShared<SPLIT>*)ts_smem;
+  StageShared& sh = *(StageShared*)ts_smem;
   const tq_geom& g = a.g;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // (the last tiles first: the window's take longest)
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
   uint4 codes = {0u, 0u, 0u, 0u};
   if (kt < sq.cold) codes = *(const uint4*)(kpage + kslot * (TQ_D / 2) + 16 * kq);
   if (tid < 16) {
-    sh.grid[tid] = a.tables->grid[tid] * (1.0f / TI_KEY);
+    sh.grid[tid] = a.tables->grid[tid];
     sh.cent[tid] = a.tables->centroids[tid];
   }
   if (tid < TQ_D) {  // uniform grids count from their zero-point on: their middle
@@ -206,18 +207,13 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
     if (lane == 0) sh.top[warp] = top;
   }
   __syncthreads();
+  float most = 0.0f;
   {  // ---- keys: a thread has a quarter of a token
-    float most = 0.0f;
-    auto put = [&](int chunk, const float (&x)[8]) {  // (already divided by TI_KEY)
-      uint32_t hi[4], lo[4];
+    auto put = [&](int chunk, const float (&x)[8]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        most = ti_max3_nan(most, fabsf(x[2 * i]), fabsf(x[2 * i + 1]));
-        hi[i] = ti_pair(x[2 * i], x[2 * i + 1]);
-        if (SPLIT) lo[i] = ti_rest(x[2 * i], x[2 * i + 1], hi[i]);
-      }
-      *(uint4*)(sh.k[0] + chunk * TI_KLBO + krow * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      if (SPLIT) *(uint4*)(sh.k[SPLIT] + chunk * TI_KLBO + krow * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      for (int i = 0; i < 4; ++i) most = ti_max3_nan(most, fabsf(x[2 * i]), fabsf(x[2 * i + 1]));
+      *(float4*)sh.k[2 * chunk][krow] = make_float4(x[0], x[1], x[2], x[3]);
+      *(float4*)sh.k[2 * chunk + 1][krow] = make_float4(x[4], x[5], x[6], x[7]);
     };
     if (kt < sq.cold) {
       const float* sc = (const float*)(kpage + g.scale_off);
@@ -234,7 +230,7 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         const float zz[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fmaf(ss[e], sh.grid[w[i] >> (4 * e) & 15], (mm[e] - zz[e]) * (1.0f / TI_KEY));
+        for (int e = 0; e < 8; ++e) x[e] = fmaf(ss[e], sh.grid[w[i] >> (4 * e) & 15], mm[e] - zz[e]);
         put(4 * kq + i, x);
       }
     } else {
@@ -245,7 +241,7 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         if (kt < t1) {
           ts_ld8(a.hot_k, at + 8 * i, g.kv_dtype, x);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = (x[e] - sh.center[32 * kq + 8 * i + e]) * (1.0f / TI_KEY);
+          for (int e = 0; e < 8; ++e) x[e] -= sh.center[32 * kq + 8 * i + e];
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = 0.0f;
@@ -253,9 +249,12 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         put(4 * kq + i, x);
       }
     }
-    odd |= !(most <= 65504.0f);
+    odd |= !(most < TI_KEY_MOST);
+    sh.part_top[kq][krow] = most;
   }
   __syncthreads();
+  const float token_top =
+      tid < TI_T ? fmaxf(fmaxf(sh.part_top[0][tid], sh.part_top[1][tid]), fmaxf(sh.part_top[2][tid], sh.part_top[3][tid])) : 0.0f;
   if (g.outlier_k > 0) {
     for (int b = t0 / S; b * S < min(t1, sq.cold); ++b) {
       const PageMeta pm = b == t0 / S ? first : a.page_meta[uix * g.max_blocks + b];
@@ -266,22 +265,36 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
         const __half val = __ushort_as_half(a.pool_val[slab + e]);
         const int t = b * S + (int)(w >> 24), ch = (w >> 16) & 127;
         if (t < t0 || t >= t1) continue;
-        const float x = (__half2float(val) - sh.center[ch]) * (1.0f / TI_KEY);
-        odd |= !(fabsf(x) <= 65504.0f);
-        const int at = (ch >> 3) * TI_KLBO + (t - t0) * 16 + (ch & 7) * 2;
-        const __half hi = __float2half_rn(x);
-        *(__half*)(sh.k[0] + at) = hi;
-        if (SPLIT) *(__half*)(sh.k[SPLIT] + at) = __float2half_rn(x - __half2float(hi));
+        const float x = __half2float(val) - sh.center[ch];
+        odd |= !(fabsf(x) < TI_KEY_MOST);
+        most = fmaxf(most, fabsf(x));
+        sh.k[ch >> 2][t - t0][ch & 3] = x;
       }
     }
   }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if (lane == 0) sh.k_top[warp] = most;
   odd = __syncthreads_or(odd);
   if (odd && tid == 0) ta.left[unit] = 1;
+#pragma unroll
+  for (int w = 0; w < TS_THREADS / 32; ++w) most = fmaxf(most, sh.k_top[w]);
+  if (token_top > 0.0f && token_top < most * TI_LEAST) ta.left[unit] = 1;
+  // (from 2^-30 on: the factor times a row's own stays a number above zero)
+  float k_exponent;
+  const float k_up = ti_lift(most, 14, k_exponent, 97);
   uint8_t* const images = ta.images + ((size_t)unit * ta.cap + idx) * (SPLIT ? 4 : 2) * TI_IMAGE;
-#pragma unroll 4
-  for (int i = tid; i < TI_IMAGE / 16; i += TS_THREADS) {
-    *(uint4*)(images + 16 * i) = *(const uint4*)(sh.k[0] + 16 * i);
-    if (SPLIT) *(uint4*)(images + TI_IMAGE + 16 * i) = *(const uint4*)(sh.k[SPLIT] + 16 * i);
+#pragma unroll
+  for (int i = tid; i < TI_IMAGE / 16; i += TS_THREADS) {  // eight channels of a token
+    const int chunk = i / TI_T, row = i - chunk * TI_T;
+    const float4 x = *(const float4*)sh.k[2 * chunk][row], y = *(const float4*)sh.k[2 * chunk + 1][row];
+    const uint4 hi = {ti_pair(x.x * k_up, x.y * k_up), ti_pair(x.z * k_up, x.w * k_up), ti_pair(y.x * k_up, y.y * k_up),
+                      ti_pair(y.z * k_up, y.w * k_up)};
+    *(uint4*)(images + 16 * i) = hi;
+    if (SPLIT)
+      *(uint4*)(images + TI_IMAGE + 16 * i) =
+          make_uint4(ti_rest(x.x * k_up, x.y * k_up, hi.x), ti_rest(x.z * k_up, x.w * k_up, hi.y),
+                     ti_rest(y.x * k_up, y.y * k_up, hi.z), ti_rest(y.z * k_up, y.w * k_up, hi.w));
   }
 
   // ---- values
@@ -289,7 +302,7 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
 #pragma unroll
   for (int w = 0; w < TS_THREADS / 32; ++w) top = fmaxf(top, sh.top[w]);
   const float up = ti_lift(top, 14, exponent);
-  if (tid == 0) ta.exponent[(size_t)unit * ta.cap + idx] = exponent;
+  if (tid == 0) ta.exponent[(size_t)unit * ta.cap + idx] = make_float2(exponent, exp2f(k_exponent));
   uint8_t* const v_hi = images + (SPLIT ? 2 : 1) * TI_IMAGE;
   uint8_t* const v_lo = v_hi + TI_IMAGE;
   if (!hot && S % TQ_GROUP_TOK == 0) {
@@ -334,7 +347,7 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
   // Window tokens are rotated, v @ Pi^T, on mma.sync: 16 tokens at a time as pairs hi + lo are the B operand, a warp's 16
   // output channels, whose rows of Pi are pairs too, the A operand.  Tokens of blocks in the same tile come
   // from their codes one by one.
-  uint8_t* const vs = sh.k[0];
+  uint8_t* const vs = (uint8_t*)sh.k;
   const int q = lane >> 2, c = lane & 3;
 #pragma unroll 1
   for (int n0 = 0; n0 < TI_T; n0 += TS_VT) {
@@ -739,7 +752,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       }
       float exponent;
       const float up = ti_lift(top, 13, exponent);
-      factor = tq_scaled<true>(TI_KEY * exp2f(exponent));
+      factor = tq_scaled<true>(exp2f(exponent));
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -758,18 +771,19 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
     // whether all rows of this CTA see a tile goes by their earliest position and latest window
     const bool whole = row0 + TI_ROWS <= a.rows && i_lo < sq.q_n && (row0 + TI_ROWS - 1) / G < sq.q_n && p_lo >= 0;
     const int w_hi = attend_window(a, max(p_hi, 0));
-    const float* const exponents = ta.exponent + (size_t)unit * ta.cap;
+    const float2* const exponents = ta.exponent + (size_t)unit * ta.cap;
     auto tile_of = [&](int k) { return tl.at(k_lo + min(k, n - 1)); };
     auto exponent_of = [&](int t) { return exponents[t < ul.head ? t : ul.head + t - ul.first]; };
     float m = -INFINITY, l = 0.0f;
     int t = n > 0 ? tile_of(0) : 0;
-    float e = n > 0 ? exponent_of(t) : 0.0f;
+    float2 of_tile = n > 0 ? exponent_of(t) : make_float2(0.0f, 0.0f);
     if (groups == 2 && x == 1 && n > 0) asm volatile("bar.arrive 1, 256;" ::: "memory");
     for (int k = 0; k < n; ++k) {
       const int t0 = t * TI_T;
-      // (the next tile's exponent, on its way from memory while this one is done)
+      // (the next tile's exponent and factor, on their way from memory while this one is done)
       const int t_next = tile_of(k + 1);
-      const float e_next = exponent_of(t_next);
+      const float2 next = exponent_of(t_next);
+      const float e = of_tile.x, by = factor * of_tile.y;
       settled(&sh.s_full[x], k & 1);
       uint32_t v[TI_T];
       ti_ld32(ts, v);
@@ -794,7 +808,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       top[0] = ti_max3(top[0], top[1], top[2]);
       top[3] = ti_max3(top[3], top[4], top[5]);
       top[0] = ti_max3(ti_max3(top[0], top[3], top[6]), top[7], -INFINITY);
-      const float now = fmaf(top[0], factor, e);
+      const float now = fmaf(top[0], by, e);
       const bool grown = now > m + TI_GROW;  // (also from -inf)
       float down = 1.0f;
       if (grown) {
@@ -820,7 +834,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       // same at the same time (950 us for 2048 tokens on 32768; with turns 907).
       if (groups == 2) asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");
       const float off = TI_LIFT + e - (m > -INFINITY ? m : 0.0f);
-      const uint64_t factor2 = ti_f2(factor, factor), off2 = ti_f2(off, off);
+      const uint64_t factor2 = ti_f2(by, by), off2 = ti_f2(off, off);
       uint64_t sum[2] = {0ull, 0ull};
       uint32_t h[TI_T / 2];
       if (open) {
@@ -847,7 +861,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       mbar_arrive(enc_smem(&sh.p_full[x]));
       const float2 s2 = ti_floats(ti_add2(sum[0], sum[1]));
       l = fmaf(s2.x + s2.y, exp2f(-e), l * down);
-      t = t_next, e = e_next;
+      t = t_next, of_tile = next;
     }
     // the row's state: [channel][row], neighbouring threads side by side
     const size_t at = ((size_t)unit * ta.splits + split) * ta.row_tiles + rt;
@@ -1064,7 +1078,7 @@ Layout layout(const AttendArgs& a, int units, int cap, int splits) {
     return x;
   };
   l.images = take((size_t)units * cap * (pairs ? 4 : 2) * TI_IMAGE);
-  l.exponent = take((size_t)units * cap * 4);
+  l.exponent = take((size_t)units * cap * 8);
   l.left = take((size_t)units * 4);
   l.stats = take((size_t)units * splits * row_tiles * TI_ROWS * 2 * 4);
   // a unit's sums, or, if it is left to the general kernel, two states a row
@@ -1077,11 +1091,11 @@ Layout layout(const AttendArgs& a, int units, int cap, int splits) {
 template <bool SPLIT>
 int launch(const AttendArgs& a, const TileArgs& ta, int units, cudaStream_t st) {
   static bool stage_done[64], tiles_done[64];
-  int rc = attend_shared(attend_stage_kernel<SPLIT>, sizeof(StageShared<SPLIT>), a.device, stage_done);
+  int rc = attend_shared(attend_stage_kernel<SPLIT>, sizeof(StageShared), a.device, stage_done);
   if (rc == TQ_OK) rc = attend_shared(attend_tiles_kernel<SPLIT>, sizeof(TiShared), a.device, tiles_done);
   if (rc != TQ_OK) return rc;
   TQ_CUDA(cudaMemsetAsync(ta.left, 0, (size_t)units * 4, st));
-  attend_stage_kernel<SPLIT><<<units * ta.cap, TS_THREADS, sizeof(StageShared<SPLIT>), st>>>(a, ta);
+  attend_stage_kernel<SPLIT><<<units * ta.cap, TS_THREADS, sizeof(StageShared), st>>>(a, ta);
   TQ_CUDA(cudaGetLastError());
   attend_tiles_kernel<SPLIT><<<units * ta.splits * ta.row_tiles, TI_THREADS, sizeof(TiShared), st>>>(a, ta);
   TQ_CUDA(cudaGetLastError());
@@ -1101,7 +1115,7 @@ int tq_launch_attend_tiles(const AttendArgs& base, void* workspace, int cap, int
   uint8_t* w = (uint8_t*)workspace;
   TileArgs ta;
   ta.images = w + l.images;
-  ta.exponent = (float*)(w + l.exponent);
+  ta.exponent = (float2*)(w + l.exponent);
   ta.left = (int32_t*)(w + l.left);
   ta.sums = (float*)(w + l.sums);
   ta.stats = (float*)(w + l.stats);
