@@ -211,3 +211,31 @@ def test_digits_do_not_depend_on_the_size_of_the_keys(torch, kv, dtype, rows, ho
             rel = _relative(torch, ctx, got, q, window, sinks)
             assert rel <= _step(torch, dt), (by, window, rel)
         assert ctx.status() == 0
+
+
+@pytest.mark.parametrize("kv", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("rows, hot", FORMS)
+@pytest.mark.parametrize("part", ["keys", "values"])
+def test_large_tokens_that_a_window_hides_take_no_digits(torch, kv, dtype, rows, hot, part):
+    """Tokens 2^40 times the others stand next to those that are seen, in the uncompressed window or in blocks."""
+    dt = getattr(torch, dtype)
+    gen = torch.Generator(device="cuda").manual_seed(59)
+    for n in (500, 1300):
+        ctx = _ctx(n_seqs=1, n_kv_heads=2, n_q_heads=4, kv_dtype=kv, hot_window=hot, outlier_frac=0.0)
+        k, v = _scaled(torch, n, 2, gen, 1.0)
+        first = n - rows - 100  # of the tokens that are seen
+        at = slice(first - 7, first)
+        if part == "keys":
+            # (a block's channels have one scale for all of its tokens: large keys stay in the uncompressed window)
+            if at.start < ctx.cold_blocks(n) * ctx.block_tokens:
+                continue
+            k[0, at, 1] *= 2.0**40
+        else:
+            v[0, at, 1] *= 2.0**40
+        ctx.append(0, k.to(ctx.kv_dtype), v.to(ctx.kv_dtype))
+        q = torch.randn(1, rows, 4, 128, generator=gen, device="cuda").to(dt)
+        got = ctx.attend(0, q, window=101)
+        rel = _relative(torch, ctx, got, q, 101)
+        assert rel <= _step(torch, dt), (n, rel)
+        assert ctx.status() == 0

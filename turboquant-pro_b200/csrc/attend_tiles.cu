@@ -302,6 +302,7 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
 #pragma unroll
   for (int w = 0; w < TS_THREADS / 32; ++w) top = fmaxf(top, sh.top[w]);
   const float up = ti_lift(top, 14, exponent);
+  if (tid < TI_T && sh.norm[tid] != 0.0f && fabsf(sh.norm[tid]) < top * TI_LEAST) ta.left[unit] = 1;
   if (tid == 0) ta.exponent[(size_t)unit * ta.cap + idx] = make_float2(exponent, exp2f(k_exponent));
   uint8_t* const v_hi = images + (SPLIT ? 2 : 1) * TI_IMAGE;
   uint8_t* const v_lo = v_hi + TI_IMAGE;
