@@ -199,8 +199,10 @@ typedef struct tq_attend_args {
 
 /* Bytes of workspace that tq_attend wants for these arguments (pointers are not looked at), on this stream: a
  * captured call asks for what the capacity of the sequences may need, since it may be replayed on longer
- * ones.  A call may be given less, down to what one sequence needs; it then takes several rounds.  tq_attend writes
- * only to its workspace and out, so calls of one context with a workspace each may overlap on the device. */
+ * ones.  It asks for 1 GB at most, unless one sequence needs more.  A call may be given less, down to the most
+ * that any one of its sequences is told by itself (seq_count 1); it then takes several rounds, perhaps in other
+ * forms.  tq_attend writes only to its workspace and out, so calls of one context with a workspace each may overlap
+ * on the device. */
 int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* args, void* stream, size_t* bytes);
 int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* args, void* stream);
 

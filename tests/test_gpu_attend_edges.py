@@ -239,3 +239,42 @@ def test_large_tokens_that_a_window_hides_take_no_digits(torch, kv, dtype, rows,
         rel = _relative(torch, ctx, got, q, 101)
         assert rel <= _step(torch, dt), (n, rel)
         assert ctx.status() == 0
+
+
+def _told(torch, ctx, q, seq_begin, seq_count):
+    """What tq_attend_workspace asks for."""
+    import ctypes as C
+
+    from turboquant_pro_b200 import _lib
+
+    a = _lib.TqAttendArgs(q=q.data_ptr(), out=q.data_ptr(), q_seq_stride=q.stride(0), q_tok_stride=q.stride(1),
+                          q_head_stride=q.stride(2), seq_begin=seq_begin, seq_count=seq_count, n_tokens=q.shape[1],
+                          q_dtype={torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[q.dtype])
+    size, stream = C.c_size_t(), torch.cuda.current_stream().cuda_stream
+    assert ctx._lib.tq_attend_workspace(ctx._h, C.byref(a), stream, C.byref(size)) == 0
+    return size.value
+
+
+@pytest.mark.parametrize("dtype, t, lens, hot", [
+    # one sequence takes the form for few rows, all of them that for many, whose share of a sequence is larger
+    ("bfloat16", 16, [8192] * 8, 512), ("bfloat16", 16, [8192, 300, 0, 5000, 8000, 1, 700, 8192], 512),
+    ("float16", 9, [6000] * 7, 512), ("float16", 5, [4000, 20, 3999] * 3, 200), ("float32", 30, [3000, 2000], 512)])
+def test_workspace_of_what_one_sequence_needs_will_do(torch, dtype, t, lens, hot):
+    from turboquant_pro_b200._lib import TqError
+
+    gen = torch.Generator(device="cuda").manual_seed(60)
+    ctx = _ctx(n_seqs=len(lens), n_kv_heads=8, n_q_heads=32, kv_dtype=dtype, hot_window=hot, max_tokens_per_seq=8192)
+    _fill(torch, ctx, lens, gen)
+    q = torch.randn(len(lens), t, 32, 128, generator=gen, device="cuda").to(getattr(torch, dtype))
+    q_lens = torch.tensor([(5 * i + 3) % (t + 1) for i in range(len(lens))], dtype=torch.int32, device="cuda")
+    least = max(_told(torch, ctx, q, s, 1) for s in range(len(lens)))
+    for lens_of in (None, q_lens):
+        got = ctx.attend(0, q, q_lens=lens_of, max_workspace=least)
+        _check(torch, ctx, got, q, q_lens=lens_of)
+    out = torch.full_like(q, 3.0)
+    with pytest.raises(TqError, match="workspace"):
+        ctx.attend(0, q, max_workspace=256, out=out)
+    with pytest.raises((TqError, ValueError)):
+        ctx.attend(0, q, max_workspace=0, out=out)
+    torch.cuda.synchronize()
+    assert bool((out == 3.0).all())

@@ -282,7 +282,7 @@ class KVContext:
         return out
 
     def attend(self, layer: int, q, window: int | None = None, sinks: int = 0, q_lens=None,
-               seq_begin: int = 0, out=None):
+               seq_begin: int = 0, out=None, max_workspace: int | None = None):
         """Attention of one or many query tokens per sequence on the codes, with the causal mask, a
         sliding window and first tokens that stay visible.
 
@@ -294,6 +294,12 @@ class KVContext:
         ``j <= p`` with ``j > p - window`` or ``j < sinks`` (``window=None``: all of them).  Returns
         ``[n_seqs', T, n_q_heads, D]`` of ``q``'s type; rows that see nothing (padding, queries
         before the first token, empty sequences) are zeros.  Inference only: no gradients.
+
+        Scores are ``q . k / sqrt(D)``: for another scale multiply ``q`` by ``scale * sqrt(D)``; there is
+        no capping.  A call takes workspace from torch's allocator: few rows some MB; many rows 512 bytes
+        (float16 queries: 1024) per visible token and KV head, up to 1 GB, or what one sequence needs if that is
+        more.  With ``max_workspace`` it takes at most so many bytes and goes in several rounds; a
+        :class:`TqError` says that they do not do for one sequence.
         """
         # (a decode step's call is some microseconds on the GPU: the checks are kept short)
         torch = _torch()
@@ -342,8 +348,9 @@ class KVContext:
         with self._here():
             stream, ref, size = self._stream(), C.byref(a), C.c_size_t()
             check(self._lib.tq_attend_workspace(self._h, ref, stream, C.byref(size)))
-            work = torch.empty(size.value, dtype=torch.uint8, device=dev)
-            a.workspace, a.workspace_bytes = work.data_ptr(), size.value
+            n = size.value if max_workspace is None else min(size.value, max(max_workspace, 0))
+            work = torch.empty(n, dtype=torch.uint8, device=dev)
+            a.workspace, a.workspace_bytes = work.data_ptr(), n
             check(self._lib.tq_attend(self._h, ref, stream))
         return out
 

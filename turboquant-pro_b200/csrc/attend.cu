@@ -147,34 +147,13 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
   return p;
 }
 
-}  // namespace
+size_t least_bytes(const Plan& p) { return p.fixed_bytes + p.seq_bytes; }
 
-extern "C" int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* r, void* stream, size_t* bytes) {
-  const int rc = check_args(ctx, r);
-  if (rc != TQ_OK) return rc;
-  TQ_REQUIRE(bytes != nullptr, TQ_ERR_INVALID, "null argument");
-  const Plan p = make_plan(ctx, r, (cudaStream_t)stream);
-  const size_t n = std::max<size_t>(AT_ONE_GO / std::max<size_t>(p.seq_bytes, 1), 1);
-  *bytes = align_up(p.fixed_bytes + std::min({n, (size_t)r->seq_count, (size_t)p.seqs}) * p.seq_bytes, 256);
-  return TQ_OK;
-}
-
-extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream) {
-  int rc = check_args(ctx, r);
-  if (rc != TQ_OK) return rc;
-  if (r->seq_count == 0 || r->n_tokens == 0) return TQ_OK;
+// The sequences of `r` by a plan that its workspace has room for, as many at once as it has.
+int run(tq_ctx* ctx, const tq_attend_args* r, const Plan& p, cudaStream_t st) {
   const tq_geom& g = ctx->g;
-  TQ_REQUIRE(r->q != nullptr && r->out != nullptr, TQ_ERR_INVALID, "q and out must be device pointers");
-  TQ_REQUIRE(r->workspace != nullptr && (uintptr_t)r->workspace % 256 == 0, TQ_ERR_INVALID,
-             "workspace must be a device pointer aligned to 256 bytes");
-  TQ_CUDA(cudaSetDevice(ctx->device));
-  cudaStream_t st = (cudaStream_t)stream;
-  const Plan p = make_plan(ctx, r, st);
-  TQ_REQUIRE(r->workspace_bytes >= p.fixed_bytes + p.seq_bytes, TQ_ERR_CAPACITY,
-             "workspace smaller than tq_attend_workspace asked for");
   const int at_once =
       (int)std::min({(r->workspace_bytes - p.fixed_bytes) / p.seq_bytes, (size_t)r->seq_count, (size_t)p.seqs});
-
   AttendArgs a = {};
   a.g = g;
   a.pages = (const uint8_t*)ctx->b.pages;
@@ -200,7 +179,6 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
   a.wait_limit = ctx->wait_limit, a.withhold = ctx->withhold_tile;
   a.unit_stride = (int64_t)a.rows * (p.ns_cold + p.ns_hot) * TQ_PART_STRIDE;
   const size_t esz = elem_size(r->q_dtype);
-  ctx->last_launches = 0;
   for (int s = 0; s < r->seq_count; s += at_once) {
     a.seq_begin = r->seq_begin + s;
     a.seq_count = std::min(at_once, r->seq_count - s);
@@ -208,22 +186,75 @@ extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream)
     a.out = (uint8_t*)r->out + (size_t)s * r->n_tokens * g.n_q_heads * TQ_D * esz;
     a.q_lens = r->q_lens == nullptr ? nullptr : r->q_lens + s;
     if (p.form == TILES) {
-      rc = tq_launch_attend_tiles(a, r->workspace, p.cap, p.splits, st);
+      const int rc = tq_launch_attend_tiles(a, r->workspace, p.cap, p.splits, st);
       if (rc != TQ_OK) return rc;
       ctx->last_launches += 4;
       continue;
     }
     if (p.form == ROWS) {
-      rc = tq_launch_attend_rows(a, st);
+      const int rc = tq_launch_attend_rows(a, st);
       if (rc != TQ_OK) return rc;
       ctx->last_launches += 2;
       continue;
     }
-    rc = tq_launch_attend_general(a, st);
+    int rc = tq_launch_attend_general(a, st);
     if (rc != TQ_OK) return rc;
     rc = tq_launch_attend_combine(a, st);
     if (rc != TQ_OK) return rc;
     ctx->last_launches += 2;
+  }
+  return TQ_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* r, void* stream, size_t* bytes) {
+  const int rc = check_args(ctx, r);
+  if (rc != TQ_OK) return rc;
+  TQ_REQUIRE(bytes != nullptr, TQ_ERR_INVALID, "null argument");
+  const Plan p = make_plan(ctx, r, (cudaStream_t)stream);
+  const size_t n = std::max<size_t>(AT_ONE_GO / std::max<size_t>(p.seq_bytes, 1), 1);
+  *bytes = align_up(p.fixed_bytes + std::min({n, (size_t)r->seq_count, (size_t)p.seqs}) * p.seq_bytes, 256);
+  return TQ_OK;
+}
+
+extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream) {
+  const int rc = check_args(ctx, r);
+  if (rc != TQ_OK) return rc;
+  if (r->seq_count == 0 || r->n_tokens == 0) return TQ_OK;
+  TQ_REQUIRE(r->q != nullptr && r->out != nullptr, TQ_ERR_INVALID, "q and out must be device pointers");
+  TQ_REQUIRE(r->workspace != nullptr && (uintptr_t)r->workspace % 256 == 0, TQ_ERR_INVALID,
+             "workspace must be a device pointer aligned to 256 bytes");
+  TQ_CUDA(cudaSetDevice(ctx->device));
+  cudaStream_t st = (cudaStream_t)stream;
+  const Plan all = make_plan(ctx, r, st);
+  if (r->workspace_bytes >= least_bytes(all)) {
+    ctx->last_launches = 0;
+    return run(ctx, r, all, st);
+  }
+  // Even one sequence needs more in the form that suits all of them: half as many, planned by themselves, and so on
+  // (another form may suit them).  Looked through before anything is launched.
+  for (const bool launch : {false, true}) {
+    if (launch) ctx->last_launches = 0;
+    for (int s = 0, n = 0; s < r->seq_count; s += n) {
+      tq_attend_args part = *r;
+      part.seq_begin = r->seq_begin + s;
+      part.q = (const uint8_t*)r->q + (int64_t)s * r->q_seq_stride * (int64_t)elem_size(r->q_dtype);
+      part.out = (uint8_t*)r->out + (size_t)s * r->n_tokens * ctx->g.n_q_heads * TQ_D * elem_size(r->q_dtype);
+      part.q_lens = r->q_lens == nullptr ? nullptr : r->q_lens + s;
+      n = r->seq_count - s;
+      Plan p;
+      for (;;) {
+        part.seq_count = n;
+        p = make_plan(ctx, &part, st);
+        if (r->workspace_bytes >= least_bytes(p)) break;
+        TQ_REQUIRE(n > 1, TQ_ERR_CAPACITY, "workspace smaller than tq_attend_workspace asks for one sequence");
+        n = (n + 1) / 2;
+      }
+      if (!launch) continue;
+      const int rc2 = run(ctx, &part, p, st);
+      if (rc2 != TQ_OK) return rc2;
+    }
   }
   return TQ_OK;
 }
