@@ -57,23 +57,29 @@ __all__ = ["TurboQuantCache", "TurboQuantLayer", "enable_turboquant_cache",
 # caches or two models in one process cannot reach each other's history.
 _STAMP = "_turboquant_layer"
 
-# decision "this mask hides nothing" for the mask object of the current forward: every layer
-# of a step receives the same tensor, so the device is asked once per step, not per layer
-_MASK_MEMO: list = [None, False]
+# decisions on the masks of the current forward ("hides nothing", "is the causal one"): the layers
+# of a step receive the same tensor, or one for each of two kinds, so the device is asked once per
+# step and kind, not per layer
+_MASK_MEMO: list = []
+
+
+def _remembered(mask, question, ask) -> bool:
+    for ref, of, answer in _MASK_MEMO:
+        if ref() is mask and of == question:
+            return answer
+    answer = bool(ask())
+    _MASK_MEMO.insert(0, (weakref.ref(mask), question, answer))
+    del _MASK_MEMO[4:]
+    return answer
 
 
 def _mask_is_open(mask) -> bool:
+    """Whether ``mask`` hides and shifts nothing: booleans (a padding mask's ones) that are all set, or zeros
+    to add."""
     if mask is None:
         return True
-    ref = _MASK_MEMO[0]
-    if ref is not None and ref() is mask:
-        return _MASK_MEMO[1]
-    if mask.dtype == torch.bool:
-        is_open = bool(mask.all())
-    else:
-        is_open = not bool((mask < 0).any())
-    _MASK_MEMO[0], _MASK_MEMO[1] = weakref.ref(mask), is_open
-    return is_open
+    keeps = mask.dtype == torch.bool or mask.dim() == 2
+    return _remembered(mask, "open", lambda: (mask != 0).all() if keeps else ~(mask != 0).any())
 
 
 def _mask_is_causal(mask, t: int, n: int, window) -> bool:
@@ -82,10 +88,17 @@ def _mask_is_causal(mask, t: int, n: int, window) -> bool:
     if mask is None:
         return True
     if mask.dim() == 2:
-        return _mask_is_open(mask if mask.dtype == torch.bool else mask != 0)
+        return _mask_is_open(mask)
     if tuple(mask.shape[-2:]) != (t, n):
         return False
-    return bool(((mask if mask.dtype == torch.bool else mask >= 0) == _causal(t, n, window, mask.device)).all())
+
+    def ask():
+        sees = _causal(t, n, window, mask.device)
+        if mask.dtype == torch.bool:
+            return (mask == sees).all()
+        return torch.where(sees, mask == 0, mask <= torch.finfo(mask.dtype).min).all()
+
+    return _remembered(mask, (t, n, window), ask)
 
 
 def _causal(t: int, n: int, window, device):
