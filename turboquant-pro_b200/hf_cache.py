@@ -18,9 +18,9 @@ Differences from the reference adapter, all forced by the paged device format:
 * cold blocks follow the core cache's rule (oldest half of an over-full window, i.e. 256
   tokens at ``hot_window`` 512), not the adapter's "whole overflow as one block";
 * a query of more than one token against a non-empty cache (chunked prefill, assisted
-  decoding), attention masks with padding, ``crop`` / beam reordering fall back to the
-  dense getters (``dense=True`` forces that path for every decode step: it is how the
-  reference's adapter works, and this adapter's own cross-check);
+  decoding), attention masks with padding, layers with a sliding window, score capping or a scale of
+  their own, ``crop`` / beam reordering fall back to the dense getters (``dense=True`` forces that path
+  for every decode step: it is how the reference's adapter works, and this adapter's own cross-check);
 * capacity (``max_tokens``) is fixed when the context is created.
 
 ``attend=True`` puts two of these cases on the codes as well, through ``KVContext.attend``: queries of
@@ -275,8 +275,8 @@ def turboquant_attention_forward(module, query, key, value, attention_mask, drop
                                  **kwargs):
     """Attention function for ``AttentionInterface``: single-token queries are attended on
     the compressed cache's codes; everything else goes to the stock SDPA implementation on
-    the K/V it is given (with a :class:`TurboQuantCache` in its default mode that is only
-    right for a prompt into an empty cache; other cases switch the layer to dense K/V)."""
+    the K/V it is given, which is right for a prompt into an empty cache; in other cases on the
+    layer's dense K/V (capped scores by a dense form of their own)."""
     from transformers.integrations.sdpa_attention import sdpa_attention_forward
 
     # the key tensor is the one TurboQuantLayer.update returned in this forward, or the call
@@ -286,49 +286,68 @@ def turboquant_attention_forward(module, query, key, value, attention_mask, drop
     if layer is not None and (layer.get_seq_length() != stamp[1]
                               or layer.layer_idx != getattr(module, "layer_idx", layer.layer_idx)):
         layer = None  # a stale tensor: the cache has moved on since it was stamped
-    # what the codes-only kernel does not implement goes to the dense path: windows, score
-    # capping, any scale other than 1/sqrt(head_dim)
-    plain = (not kwargs.get("sliding_window") and not kwargs.get("softcap")
-             and not getattr(module, "sliding_window", None)
-             and not getattr(module, "is_sliding", False))
-    fused = (layer is not None and not layer.dense and plain and query.shape[2] == 1
-             and key.shape[2] == 1 and layer.get_seq_length() > 1)
-    if fused:
-        d = query.shape[-1]
-        if scaling is not None and abs(scaling * d ** 0.5 - 1.0) > 1e-3:
-            raise NotImplementedError("the decode kernel uses the 1/sqrt(head_dim) scale")
-        fused = _mask_is_open(attention_mask)
-    if fused:
-        out = layer.ctx.decode(layer.layer_idx, query[:, :, 0, :])  # [B, Hq, D] float32
-        return out.to(query.dtype)[:, None, :, :], None
-    if layer is not None and layer.attend and not layer.dense and key.shape[2] == query.shape[2]:
-        n, t = layer.get_seq_length(), query.shape[2]
-        window = kwargs.get("sliding_window") or getattr(module, "sliding_window", None)
-        if (n > t and not dropout and not kwargs.get("softcap")
-                and (scaling is None or abs(scaling * query.shape[-1] ** 0.5 - 1.0) <= 1e-3)
-                and (window is not None or not getattr(module, "is_sliding", False))
-                and is_causal is not False and getattr(module, "is_causal", True)
+    # what the codes-only kernels do not implement goes to the dense path: score capping, any scale
+    # other than 1/sqrt(head_dim)
+    t, d = query.shape[2], query.shape[-1]
+    window = kwargs.get("sliding_window") or getattr(module, "sliding_window", None) or None
+    softcap = kwargs.get("softcap") or None
+    causal = is_causal is not False and getattr(module, "is_causal", True)
+    usual = softcap is None and (scaling is None or abs(scaling * d ** 0.5 - 1.0) <= 1e-3)
+    if layer is not None and not layer.dense and key.shape[2] == t and usual:
+        n = layer.get_seq_length()
+        if t == 1 and n > 1 and window is None and not getattr(module, "is_sliding", False) \
+                and _mask_is_open(attention_mask):
+            out = layer.ctx.decode(layer.layer_idx, query[:, :, 0, :])  # [B, Hq, D] float32
+            return out.to(query.dtype)[:, None, :, :], None
+        if (layer.attend and n > t and not dropout
+                and (window is not None or not getattr(module, "is_sliding", False)) and causal
                 and not (query.requires_grad and torch.is_grad_enabled())
                 and _mask_is_causal(attention_mask, t, n, window)):
             return layer.ctx.attend(layer.layer_idx, query.transpose(1, 2), window=window), None
-        if n == t and window is not None and n > window and attention_mask is None \
-                and is_causal is not False and getattr(module, "is_causal", True):
-            # a prompt on its own K/V: the window that no mask brings along
-            attention_mask = _causal(t, n, window, query.device)[None, None]
     if layer is not None and key.shape[2] != layer.get_seq_length():
         # a multi-token query on top of stored history, a masked batch, a windowed or capped
         # layer: the dense history
         key, value = layer.full()
+    n = key.shape[2]
+    if attention_mask is None:
+        # no mask stands for the causal one; the stock implementation takes it from the upper left, which is
+        # right for a prompt alone, and does not know windows
+        if causal and t <= n and (1 < t < n or (window is not None and n > window) or (softcap is not None and t > 1)):
+            attention_mask = _causal(t, n, window, query.device)[None, None]
+    elif attention_mask.dim() == 2 and attention_mask.shape[-1] == n:  # what is padding, as [batch, tokens]
+        attention_mask = (attention_mask != 0)[:, None, None, :]
+        if causal and t <= n:
+            attention_mask = attention_mask & _causal(t, n, window, query.device)
+    if softcap is not None:
+        return _capped_attention(query, key, value, attention_mask, dropout if module.training else 0.0,
+                                 d ** -0.5 if scaling is None else scaling, softcap), None
     return sdpa_attention_forward(module, query, key, value, attention_mask, dropout=dropout,
                                   scaling=scaling, is_causal=is_causal, **kwargs)
+
+
+def _capped_attention(query, key, value, mask, dropout, scaling, softcap):
+    """Dense attention with scores ``softcap * tanh(score / softcap)``, which the stock implementation leaves out:
+    ``[B, Hq, T, D]`` queries to ``[B, T, Hq, D]``."""
+    groups = query.shape[1] // key.shape[1]
+    key, value = key.repeat_interleave(groups, 1), value.repeat_interleave(groups, 1)
+    scores = torch.tanh((query.float() @ key.float().transpose(2, 3)) * (scaling / softcap)) * softcap
+    if mask is not None:
+        mask = mask[..., :key.shape[2]]
+        # (the type's lowest value: a row that sees nothing, a padding query's, stays finite)
+        scores = scores.masked_fill(~mask, torch.finfo(scores.dtype).min) if mask.dtype == torch.bool else scores + mask
+    weights = torch.nn.functional.dropout(torch.softmax(scores, -1).to(value.dtype), dropout, dropout > 0.0)
+    return (weights @ value).transpose(1, 2).contiguous()
 
 
 def enable_turboquant_cache(model, **cache_kwargs) -> TurboQuantCache:
     """Registers the attention function, switches ``model`` to it and returns a fresh
     :class:`TurboQuantCache` for ``model.generate(..., past_key_values=cache)``
     (the reference's helper of the same name: ``hf_cache.py``)."""
-    from transformers import AttentionInterface
+    from transformers import AttentionInterface, AttentionMaskInterface
+    from transformers.masking_utils import sdpa_mask
 
     AttentionInterface.register("turboquant", turboquant_attention_forward)
+    # without a mask function of its own an attention function is given no masks: padding and windows would be lost
+    AttentionMaskInterface.register("turboquant", sdpa_mask)
     model.config._attn_implementation = "turboquant"
     return TurboQuantCache(model.config, **cache_kwargs)
