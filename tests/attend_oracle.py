@@ -83,6 +83,6 @@ def check(got, want):
 
 
 # float16 queries with scores of standard deviation four: the output's rounding and, at worst, that of the probabilities
-# are 0.42 of eps / 2 each in the mean square, 0.6 together; keys of half precision without a low part would add
-# 0.42 * 4 = 1.7 to that.
+# are 0.42 of eps / 2 each in the mean square, 0.6 together.  Keys of half precision without a low part would move scores by
+# 0.42 * 4 = 1.7, less what a row's heaviest tokens, which then have most of its weight, have in common.
 PAIRS = 0.75 * torch.finfo(torch.float16).eps / 2

@@ -45,4 +45,4 @@ def test_the_measure_of_pairs_sees_keys_without_low_parts():
     q = (4.0 * torch.randn(64, 2, 128, generator=gen)).half()
     want = attention(k, v, q, 64, None, 0)
     assert measures(want.half(), want)[0] <= 0.6 * PAIRS
-    assert measures(attention(k.half(), v, q, 64, None, 0).half(), want)[0] > 1.5 * PAIRS
+    assert measures(attention(k.half(), v, q, 64, None, 0).half(), want)[0] > 1.25 * PAIRS
