@@ -14,6 +14,8 @@
 // Bound by launch and latency for single tokens (4 us); for prompts by reading and writing q and k, at 68 to 80 % of
 // a plain copy's rate (8 x 2048 tokens of 32 + 8 heads, bfloat16: 75 us, 4.5 TB/s), and the unpacking, shuffles and
 // packing between them.
+#include <atomic>
+
 #include "common.cuh"
 
 namespace {
@@ -262,14 +264,14 @@ __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(RopeArgs a, in
 }
 
 template <int DT, bool PAIRED>
-void start(const RopeArgs& a, int tokens, bool vec, cudaStream_t st) {
+void start(const RopeArgs& a, int tokens, int sm_count, bool vec, cudaStream_t st) {
   // The fewest tokens a CTA with which all are resident at once, three an SM: another round of them costs more than a
   // warp's longer work, and that more than the angles of more tokens a thread.  us for 1 | 2 | 4 | 8 tokens a CTA (32 + 8
   // heads, bfloat16): 64 tokens 3.7 | 4.2 | 5.5 | 8.5, 600: 8.3 |
   // 6.3 | 6.9 | 8.6, 1700: 17.1 | 11.6 | 9.1 | 11.1, 6000: 62 | 41 | 34 | 32.
-  constexpr int RESIDENT = 3 * 148;
+  const int resident = 3 * sm_count;
   int per_cta = 1;
-  while (per_cta < NR_THREADS / 32 && tokens > per_cta * RESIDENT) per_cta *= 2;
+  while (per_cta < NR_THREADS / 32 && tokens > per_cta * resident) per_cta *= 2;
   const int grid = (int)(((int64_t)tokens + per_cta - 1) / per_cta);
   if (vec) norm_rope_kernel<DT, PAIRED, true><<<grid, NR_THREADS, 0, st>>>(a, tokens, per_cta);
   else norm_rope_kernel<DT, PAIRED, false><<<grid, NR_THREADS, 0, st>>>(a, tokens, per_cta);
@@ -299,9 +301,15 @@ int check_rope(const tq_rope* r, bool stored) {
   return TQ_OK;
 }
 
-int launch(const tq_rope* r, const int32_t* seq_len, cudaStream_t st) {
+int launch(const tq_rope* r, const int32_t* seq_len, int device, cudaStream_t st) {
   const int tokens = r->n_seqs * r->n_tokens;
   if (tokens == 0 || r->n_q_heads + r->n_kv_heads == 0) return TQ_OK;
+  static std::atomic<int> counts[64];  // (asked for once per device)
+  int sms = device >= 0 && device < 64 ? counts[device].load(std::memory_order_relaxed) : 0;
+  if (sms == 0) {
+    TQ_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    if (device >= 0 && device < 64) counts[device].store(sms, std::memory_order_relaxed);
+  }
   const int e = 16 / elem_size(r->dtype);
   const bool vec = ((uintptr_t)r->q | (uintptr_t)r->k) % 16 == 0 &&
                    ((r->q_seq_stride | r->q_tok_stride | r->q_head_stride | r->k_seq_stride |
@@ -309,9 +317,9 @@ int launch(const tq_rope* r, const int32_t* seq_len, cudaStream_t st) {
   RopeArgs a = {*r, seq_len};
   const bool paired = r->rotary_dim / 2 % e == 0;
   switch (r->dtype) {
-    case TQ_F32: start<TQ_F32, true>(a, tokens, vec, st); break;
-    case TQ_F16: paired ? start<TQ_F16, true>(a, tokens, vec, st) : start<TQ_F16, false>(a, tokens, vec, st); break;
-    default: paired ? start<TQ_BF16, true>(a, tokens, vec, st) : start<TQ_BF16, false>(a, tokens, vec, st);
+    case TQ_F32: start<TQ_F32, true>(a, tokens, sms, vec, st); break;
+    case TQ_F16: paired ? start<TQ_F16, true>(a, tokens, sms, vec, st) : start<TQ_F16, false>(a, tokens, sms, vec, st); break;
+    default: paired ? start<TQ_BF16, true>(a, tokens, sms, vec, st) : start<TQ_BF16, false>(a, tokens, sms, vec, st);
   }
   TQ_CUDA(cudaGetLastError());
   return TQ_OK;
@@ -323,7 +331,7 @@ extern "C" int32_t tq_norm_rope(const tq_rope* r, int32_t device, void* stream) 
   const int rc = check_rope(r, false);
   if (rc != TQ_OK) return rc;
   TQ_CUDA(cudaSetDevice(device));
-  return launch(r, nullptr, (cudaStream_t)stream);
+  return launch(r, nullptr, device, (cudaStream_t)stream);
 }
 
 extern "C" int32_t tq_ctx_norm_rope(tq_ctx* ctx, int32_t layer, int32_t seq_begin, const tq_rope* r,
@@ -339,5 +347,5 @@ extern "C" int32_t tq_ctx_norm_rope(tq_ctx* ctx, int32_t layer, int32_t seq_begi
   TQ_CUDA(cudaSetDevice(ctx->device));
   const int32_t* len = (const int32_t*)((const uint8_t*)ctx->b.state + state_len_off(g)) +
                        (size_t)layer * g.n_seqs + seq_begin;
-  return launch(r, len, (cudaStream_t)stream);
+  return launch(r, len, ctx->device, (cudaStream_t)stream);
 }
