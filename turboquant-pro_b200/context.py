@@ -673,6 +673,54 @@ class KVContext:
                 self._h, layer, seq, block, n, base, base + n * size, base + at_val,
                 base + at_first, base + at_first + 4 * (n * h + 1), self._stream()))
 
+    def import_blocks(self, layer: int, seq: int, block: int, containers: dict) -> None:
+        """:meth:`import_block` of consecutive blocks from ``block`` on whose containers are tensors, on this
+        context's device or not: the arrays of :meth:`export_block`, a block each along the first
+        dimension (``key_indices``, ``nf4_scale``, ``nf4_mean``, ``value_indices``, ``value_norms``, and
+        ``outlier_idx`` / ``outlier_val``: ``[n_blocks, n]``, lists where the blocks differ, or ``None``).  What is on the device already does not
+        travel; one kernel writes the pages.  :meth:`restore_hot` then sets the length."""
+        torch = _torch()
+        g, dev = self.geom, self.device
+        h, s, d, vb = g.n_kv_heads, g.block_tokens, g.head_dim, g.value_bits
+        key, scale, mean, val, norm, size = self._wire_parts()
+        n = len(containers["key_indices"])
+        if n == 0:
+            return
+        # (offset in a block's part of the staging buffer, elements, type)
+        parts = {"key_indices": (key, h * s * d // 2, torch.uint8), "nf4_scale": (scale, h * d, torch.float32),
+                 "nf4_mean": (mean, h * d, torch.float32), "value_indices": (val, h * s * d * vb // 8, torch.uint8),
+                 "value_norms": (norm, h * s, torch.float32)}
+        idx, words = containers.get("outlier_idx"), containers.get("outlier_val")
+        with self._here():
+            staging = torch.empty((n, size), dtype=torch.uint8, device=dev)
+            for name, (at, count, dtype) in parts.items():
+                x = torch.as_tensor(containers[name]).to(device=dev, dtype=dtype)
+                if x.numel() != n * count or len(x) != n:
+                    raise ValueError(f"{name} does not match {n} blocks of this context's shape "
+                                     f"(H={h}, S={s}, D={d}, value_bits={vb})")
+                staging.view(dtype)[:, at // x.element_size():][:, :count] = x.reshape(n, count)
+            if idx is None:
+                idx, words = [torch.empty(0, dtype=torch.int32)] * n, [torch.empty(0, dtype=torch.int16)] * n
+            if len(idx) != n or len(words) != n or [len(i) for i in idx] != [len(w) for w in words]:
+                raise ValueError(f"outlier_idx and outlier_val must be of {n} blocks, as many values as indices each")
+            counts = torch.tensor([len(i) for i in idx], dtype=torch.int64, device=dev)
+            idx, words = (torch.cat([torch.as_tensor(x).reshape(-1) for x in xs]).to(dev)
+                          for xs in (idx, words))
+            if idx.dtype not in (torch.int32, torch.int64) \
+                    or words.dtype not in (torch.float16, torch.int16, torch.uint16):
+                raise ValueError(f"expected integers and float16 values (or their words) of outliers, got {idx.dtype} and "
+                                 f"{words.dtype}")
+            # the indices through all blocks: where those of every (block, head) begin, and behind that the flag
+            flat = torch.arange(n, device=dev).repeat_interleave(counts) * (h * s * d) + idx
+            if idx.numel() and not bool((idx >= 0).all() & (idx < h * s * d).all() & (flat[1:] > flat[:-1]).all()):
+                raise ValueError("outlier indices must ascend inside the (H, S, D) block")
+            first = torch.zeros(n * h + 2, dtype=torch.int32, device=dev)
+            first[:-1] = torch.searchsorted(flat, torch.arange(0, n * h + 1, device=dev) * (s * d))
+            idx = idx.int()
+            check(self._lib.tq_import_blocks(
+                self._h, layer, seq, block, n, staging.data_ptr(), idx.data_ptr(), words.data_ptr(),
+                first.data_ptr(), first.data_ptr() + 4 * (n * h + 1), self._stream()))
+
     def restore_hot(self, layer: int, seq: int, n_tokens: int, hot_k, hot_v) -> None:
         """Completes a restore: the cache holds ``n_tokens`` tokens, its cold blocks were
         imported, and ``hot_k`` / ``hot_v`` (tensors ``[tokens, n_kv_heads, D]``) are the tokens after the last cold block."""
