@@ -265,25 +265,6 @@ def _inputs_attend(case, seed):
     return state
 
 
-def _stored(state, seq, n_blocks, n_hot):
-    """One sequence as ``KVContext.import_state`` takes it."""
-    from turboquant_pro_b200.kv_blob import block_to_blob
-
-    case = state["case"]
-    h, s, vb = case["heads"], (case["hot"] + 1) // 2, case["value_bits"]
-    host = {k: state[k][seq, :n_blocks].cpu().numpy() for k in (
-        "key_indices", "nf4_scale", "nf4_mean", "outlier_idx", "outlier_val", "value_indices", "value_norms")}
-    blobs = [block_to_blob({"key_indices": host["key_indices"][b].reshape(-1), "nf4_scale": host["nf4_scale"][b][None],
-                            "nf4_mean": host["nf4_mean"][b][None], "outlier_idx": host["outlier_idx"][b],
-                            "outlier_val": host["outlier_val"][b], "value_indices": host["value_indices"][b].reshape(-1),
-                            "value_norms": host["value_norms"][b][None], "shape": (1, h, s, D), "key_bits": 4,
-                            "value_bits": vb}, key_mode=case["keys"], position_start=b * s) for b in range(n_blocks)]
-    word = torch.int32 if case["dtype"] == "float32" else torch.int16
-    raw = [state[k][seq, :n_hot].contiguous().view(word).cpu().numpy() for k in ("hot_k", "hot_v")]
-    return {"n_tokens": n_blocks * s + n_hot, "blocks": blobs, "hot_k": raw[0], "hot_v": raw[1],
-            "kv_dtype": case["dtype"], "geom": (h, s, D, vb), "key_mode": case["keys"]}
-
-
 def prepare(case, seed):
     if case["kind"] == "rope":
         return dict(_prepare_rope(case, seed), case=case)
@@ -297,8 +278,10 @@ def prepare(case, seed):
             value_bits=case["value_bits"], hot_window=case["hot"], outlier_frac=OUTLIER_FRAC,
             max_tokens_per_seq=max(lens), kv_dtype=case["dtype"], pi=state["pi"].cpu().numpy(),
             key_mode=case["keys"])
+        names = ("key_indices", "nf4_scale", "nf4_mean", "outlier_idx", "outlier_val", "value_indices", "value_norms")
         for seq, (n, b) in enumerate(zip(lens, blocks)):
-            state["ctx"].import_state(0, seq, _stored(state, seq, b, n - b * s))
+            state["ctx"].import_blocks(0, seq, 0, {name: state[name][seq, :b] for name in names})
+            state["ctx"].restore_hot(0, seq, n, state["hot_k"][seq, :n - b * s], state["hot_v"][seq, :n - b * s])
     return state
 
 
