@@ -12,6 +12,7 @@ enum Form { GENERAL, ROWS, TILES };
 struct Plan {
   Form form;
   int ns_cold, ns_hot;
+  int hot_cost;      // ROWS: of a window tile, in the division of the work
   int cap, splits;   // TILES: tiles that a (sequence, KV head) has room for, splits of them
   int seqs;          // most sequences of a launch
   size_t fixed_bytes, seq_bytes;  // workspace: of a launch, of a sequence
@@ -122,7 +123,7 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
     a.q_dtype = r->q_dtype;
     a.sm_count = sm_count;
     const AttendRowsPlan rp = tq_attend_rows_plan(a, n);
-    p.ns_cold = rp.ns_cold, p.ns_hot = rp.ns_hot;
+    p.ns_cold = rp.ns_cold, p.ns_hot = rp.ns_hot, p.hot_cost = rp.hot_cost;
     p.seqs = rp.seqs;
     p.fixed_bytes = rp.plan_bytes;
     p.seq_bytes = (size_t)g.n_kv_heads * rows * (p.ns_cold + p.ns_hot) * TQ_PART_STRIDE * 4;
@@ -173,7 +174,7 @@ int run(tq_ctx* ctx, const tq_attend_args* r, const Plan& p, cudaStream_t st) {
   a.q_dtype = r->q_dtype;
   a.window = r->window == 0 ? INT_MAX : r->window;
   a.sinks = r->sinks;
-  a.ns_cold = p.ns_cold, a.ns_hot = p.ns_hot;
+  a.ns_cold = p.ns_cold, a.ns_hot = p.ns_hot, a.hot_cost = p.hot_cost;
   a.rows = r->n_tokens * g.group;
   a.device = ctx->device, a.sm_count = ctx->sm_count;
   a.wait_limit = ctx->wait_limit, a.withhold = ctx->withhold_tile;

@@ -113,6 +113,7 @@ int tq_launch_attend_combine(const AttendArgs& a, cudaStream_t st);
 struct AttendRowsPlan {
   int ns_cold, ns_hot;  // slots of a row's states
   int seqs;             // most sequences of a launch
+  int hot_cost;         // of a window tile, for AttendArgs
   size_t plan_bytes;    // at a.plan
 };
 AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens);

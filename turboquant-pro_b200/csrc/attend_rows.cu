@@ -48,12 +48,20 @@ constexpr int NT = 1;
 constexpr int AR_STRIP = 64;       // of them, in an item of the list
 constexpr int AR_HOT = 32;         // window tokens of an item
 constexpr int AR_PITCH = TQ_D * 2 + 16, AR_PITCH32 = TQ_D * 4 + 16;  // bytes of a window row in shared memory
-// How long a strip takes, by whether operands are pairs, and a tile of the window beside it.  Measured, tile to strip:
-// bfloat16 queries, 16 x 8192 tokens 2:4 76 us, 3:4 72, 4:4 79; 8 x 8000 and five tokens 100, 99, 108; float16 ones on a
-// float16 window, 24 ragged sequences, 3:8 68, 4:8 73, 5:8 74, 6:8 75; float32 ones on a float32 window, 32 heads of
-// 2500 tokens, 3:8 44, 4:8 37, 5:8 37, 6:8 41.
+// How long a strip takes, by whether operands are pairs, and a tile of the window beside it.  Measured, tile to strip, us
+// (8 KV heads of 4 query heads, one token, unless said):
+//   bfloat16 on 16-bit windows   2:4, 3:4, 4:4: 16 x 8192 tokens 76, 72, 79; 8 x 8000 and five tokens 100, 99, 108; 8 x
+//     3000 of 32 KV heads of one 73, 70, 76; 64 x 1500, window 700, 79, 82, 88; 32 x 700 39, 36, 35; 1 x 600 23, 23, 18
+//   float16 and float32 on 16-bit windows   2:8, 3:8, 4:8, 6:8: 8 x 8192 83, 79, 79, 80; 64 x 700 73, 80, 82, 87; 16 x 3000
+//     float32 on bfloat16 75, 71, 72, 72
+//   bfloat16 on float32 windows   3:4, 4:4, 5:4, 6:4: 16 x 2000 of 4 x 7, two tokens, 63, 55, 59, 58; 32 x 700 -, 65, 69, 72
+//   float16 and float32 on float32 windows   4:8, 6:8, 8:8, 10:8: 8 x 3000 of 32 x 1 177, 155, 148, 153; 4 x 20000, two
+//     tokens, 106, 90, 85, 84; 16 x 3000 float16 98, 88, 82, 89; 32 x 700 76, 70, 72, 80; 1 x 600 35, 35, 24, 24.  Half of
+//     that (HALF_HOT) where every warp then has one share of a strip's length, and would not otherwise: 1 x 2500 of 32 x 1,
+//     window 2000, 39, 43, 44, -.  (The kernel cannot choose: that took 1.5 to 4 us of its prologue.)
 TQ_HD constexpr int ar_cost(bool split) { return split ? 8 : 4; }
-inline int ar_hot_cost(int q_dtype, int kv_dtype) { return q_dtype != TQ_BF16 && kv_dtype == TQ_F32 ? 4 : 3; }
+inline int ar_hot_cost(int q_dtype, int kv_dtype) { return kv_dtype != TQ_F32 ? 3 : q_dtype == TQ_BF16 ? 4 : 8; }
+constexpr int HALF_HOT = 4;
 constexpr int AR_SEQS = 64;        // sequences of a launch
 constexpr int AR_LIST = 256;       // outliers of a strip that are copied ahead (160 is usual)
 
@@ -1376,16 +1384,24 @@ AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens) {
   const int64_t hot = (std::min(tokens, g.hot_window) + AR_HOT - 1) / AR_HOT;
   const int64_t rows = (int64_t)std::min(a.seq_count, AR_SEQS) * g.n_kv_heads * ((a.rows + 8 * NT - 1) / (8 * NT));
   const int64_t workers = (int64_t)a.sm_count * (a.q_dtype == TQ_BF16 ? ArShape<false, 3>::WARPS : ArShape<true, 3>::WARPS);
-  const int cost = ar_cost(a.q_dtype != TQ_BF16), hot_cost = ar_hot_cost(a.q_dtype, g.kv_dtype);
+  const int cost = ar_cost(a.q_dtype != TQ_BF16);
+  int hot_cost = ar_hot_cost(a.q_dtype, g.kv_dtype);
+  if (hot_cost > HALF_HOT) {  // (by what the longest sequence's rows see, as ar_work has it)
+    const int64_t room = workers * cost;
+    const int64_t w = a.window == INT_MAX ? 0 : std::max<int64_t>((int64_t)tokens - a.n_tokens - a.window + 1, 0), first = w / AR_STRIP;
+    const int64_t n_strips = std::max<int64_t>(in_blocks / AR_STRIP - first, 0) +
+                             std::min<int64_t>((std::min<int64_t>(a.sinks, in_blocks) + AR_STRIP - 1) / AR_STRIP, first);
+    const int64_t n_hot = (tokens - in_blocks + AR_HOT - 1) / AR_HOT - std::max<int64_t>(w - in_blocks, 0) / AR_HOT;
+    if (rows * (cost * n_strips + hot_cost * n_hot) > room && rows * (cost * n_strips + HALF_HOT * n_hot) <= room) hot_cost = HALF_HOT;
+  }
+  p.hot_cost = hot_cost;
   const int64_t share = std::max<int64_t>((cost * strips + hot_cost * hot) * ((rows + 1) / 2) / workers, cost);
   p.ns_cold = (int)std::min<int64_t>(cost * strips / share + 3, 1024);
   p.ns_hot = (int)std::min<int64_t>(hot_cost * hot / share + 3, 64);
   return p;
 }
 
-int tq_launch_attend_rows(const AttendArgs& base, cudaStream_t st) {
-  AttendArgs a = base;
-  a.hot_cost = ar_hot_cost(a.q_dtype, a.g.kv_dtype);
+int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st) {
   if (a.q_dtype == TQ_BF16) return a.g.value_bits == 4 ? launch_rows<false, 4>(a, st) : launch_rows<false, 3>(a, st);
   return a.g.value_bits == 4 ? launch_rows<true, 4>(a, st) : launch_rows<true, 3>(a, st);
 }
