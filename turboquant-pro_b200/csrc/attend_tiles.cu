@@ -516,7 +516,7 @@ TQ_DEV uint64_t ti_add2(uint64_t a, uint64_t b) {
   return y;
 }
 // 2^x on the special-function units, which do 16 a cycle and SM; and on the multiply-add units: x = n + f with n whole
-// and |f| <= 1/2, a polynomial of degree 4 for 2^f (least largest relative error, 2.6e-6, fitted for this), n
+// and |f| <= 1/2, a polynomial of degree 4 for 2^f (Remez exchange on the relative error: 2.6e-6 at all six extrema), n
 // added to its exponent.  Both together finish sooner than either.  The polynomial takes what is below 2^-120 for
 // that.
 TQ_DEV float ti_exp2(float x) {  // (results below 2^-126 are zero: nothing next to the row's largest, and one instruction)
