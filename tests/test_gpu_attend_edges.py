@@ -278,3 +278,15 @@ def test_workspace_of_what_one_sequence_needs_will_do(torch, dtype, t, lens, hot
         ctx.attend(0, q, max_workspace=0, out=out)
     torch.cuda.synchronize()
     assert bool((out == 3.0).all())
+
+
+def test_a_step_with_arguments_of_another_type_appends_nothing(torch):
+    ctx = _ctx(n_seqs=1, n_kv_heads=2, n_q_heads=4, kv_dtype="bfloat16")
+    q, k, v = (torch.zeros(1, 3, h, 128, dtype=torch.bfloat16, device="cuda") for h in (4, 2, 2))
+    f = torch.ones(64, device="cuda")
+    for bad in (dict(window=2.5), dict(window="2"), dict(sinks=1.0), dict(sinks=None)):
+        with pytest.raises(TypeError):
+            ctx.step(0, q, k, v, f, **bad)
+    assert ctx.lengths(0, 0)[0] == 0
+    ctx.step(0, q, k, v, f, window=torch.tensor(2), sinks=True)
+    assert ctx.lengths(0, 0)[0] == 3

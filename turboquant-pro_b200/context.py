@@ -17,6 +17,7 @@ import contextlib
 import ctypes as C
 import functools
 import math
+import operator
 
 import numpy as np
 
@@ -379,7 +380,9 @@ class KVContext:
         tokens alike."""
         if v.dim() != 4 or v.shape != k.shape:
             raise ValueError(f"k and v differ in shape: {tuple(k.shape)} and {tuple(v.shape)}")
-        if (window is not None and window < 1) or sinks < 0:  # (before anything is appended)
+        # (what attend refuses is refused before anything is appended)
+        window, sinks = None if window is None else operator.index(window), operator.index(sinks)
+        if (window is not None and window < 1) or sinks < 0:
             raise ValueError(f"window must be at least 1 (or None) and sinks not negative, got {window}, {sinks}")
         q, k = self.norm_rope(layer, q, k, inv_freq, q_weight=q_weight, k_weight=k_weight, eps=eps,
                               seq_begin=seq_begin)
