@@ -8,12 +8,12 @@ of 50 / n: a hundredth of the output at n = 10^6, more where n is less.
 
 Measures.  ``by_head``: the 2-norm of the error over all rows and channels of a query head, relative to the output's.  For 16-bit
 types half a step of the type, eps / 2: the output's own rounding has 0.42 of that in the mean square (an error even over half a
-step, relative to a mantissa even over [1, 2)); probabilities, values and keys as half-precision numbers are off by 2^-12 each at
-worst, 0.29 of that in the mean square, a score by the root of 128 such products / sqrt(128): together less than 0.3 of eps / 2 for
-bfloat16, and with pairs for keys and values (float16) less than 0.6, 0.73 in all.  float32: 2^-20, four pairs of half-precision
-parts (2^-22 each) at worst.
-``by_row``: the same of every row by itself, within eps / 2 + 2^-11 + 2^-11 (each rounding at its worst, all of one sign, no
-score's error beyond 2^-11); float32: 2^-19.
+step, relative to a mantissa even over [1, 2)).  Bfloat16 (2^-8) meets probabilities, values and keys as half-precision numbers
+(2^-11 at worst, 0.42 of that in the mean square; a score is off by the root of 128 such products / sqrt(128), that is by as much): three
+times 0.42 / 8, added as squares, 0.1 of eps / 2.  Float16 (2^-11) meets keys and values as pairs, and its probabilities are rounded once:
+0.6 with the output's.  float32: 2^-20, four pairs of half-precision parts (2^-22 each) at worst.
+``by_row``: the same of every row by itself, within eps / 2 + 2^-10: the output's rounding, a probability's and a value's at their worst
+and of one sign; float32: 2^-19.
 """
 
 from __future__ import annotations

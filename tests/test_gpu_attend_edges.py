@@ -184,8 +184,8 @@ def _relative(torch, ctx, got, q, window=None, sinks=0, q_lens=None, seq_begin=0
 
 def _step(torch, dtype):
     """What ``_relative`` may give for scores of standard deviation one.  16-bit queries: half a step of the output's
-    type; its rounding alone is 0.42 of that in the mean square, operands and probabilities of half precision (2^-12 each, and a
-    score's by its error of 2^-12) less than 0.3 of it.  float32: 2^-20, four parts of 2^-22 (the pairs of queries, keys,
+    type; its rounding alone is 0.42 of that in the mean square, and half-precision probabilities, values and keys (2^-11 at worst) add
+    less than 0.6 in all (``attend_oracle.py``).  float32: 2^-20, four parts of 2^-22 (the pairs of queries, keys,
     probabilities and values); float32 sums of 128 products are below that."""
     return 2.0**-20 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
 

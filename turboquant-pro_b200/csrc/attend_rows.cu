@@ -21,8 +21,9 @@
 //
 // SPLIT (float32 and float16 queries): the table's entries are hi + lo pairs too, hi * hi of 16 channels is added
 // up in float32 registers, and outliers count with their exact stored value: as exact as float32 arithmetic.
-// bfloat16 queries leave the table's lo part out (2^-12 of a level; their own step is 2^-8), and take the outliers
-// from the page's list by token, which holds their distance from the grid in fp16.
+// bfloat16 queries leave the table's lo part out (2^-11 of a level at worst, against the half step of their own type, 2^-8),
+// and take the outliers from the page's list by token, which holds their distance from the grid in fp16: 1.7 to 1.8e-3 off
+// (2-norms, 64 bits), where rounding the exact result gives 1.65e-3.
 //
 // The uncompressed window: 16-bit rows are the A operand as they are, in their own type (ldmatrix), so that only the
 // other operand is split: a query that is exact in that type has one part, others as many as they need;
@@ -31,10 +32,11 @@
 // attended term by term instead (products with masked tokens and with low parts would spread it); of 16-bit keys, one
 // whose scores are no numbers.
 //
-// Bound by look-ups, products and their latencies at twelve warps an SM: 43 % of the issue slots, a seventh of the
-// waiting for instructions (the code of all formats is long); at one row tile the codes are read once.  Measured, 8 KV
-// heads, one token: 16 sequences of 8192 with a window of 4096 72 us, of these the merge's tail 10; 8 sequences of
-// 8000 and five tokens, three row tiles, 99 us; one sequence, window 1024, 19 us, a chain of latencies.
+// Bound by look-ups, products and their latencies at twelve warps an SM: 44 % of the issue slots (29 % and 22 % with pairs, at
+// eight warps), a tenth of the waiting for instructions (a fifth for float32 windows: the code of all formats is
+// long); at one row tile the codes are read once.  Measured, 8 KV
+// heads, one token: 16 sequences of 8192 with a window of 4096 72.5 us, of these the merge's tail 10; 8 sequences of
+// 8000 and five tokens, three row tiles, 100 us; one sequence, window 1024, 19 us, a chain of latencies.
 #include <algorithm>
 
 #include "attend.cuh"

@@ -24,19 +24,23 @@
 //     holds what counts.  The maximum is only renewed (and O rescaled) when it has grown by 2^8 since.
 // attend_tiles_combine_kernel   merges the splits, rotates the sums back (sum @ Pi), rounds.
 //
-// Measured, 8 KV heads of 4 query heads, bfloat16: 2048 tokens on 32768 1 066 us, of which stage 79, tiles 907 (72 % of
-// the rate of a large library product of as many operations, 4.3 GB/ms of operands from L2), merge 68; 512 tokens on 16384
-// 204 us: 49, 137, 16.  What bounds the tiles: exponentials (16 a cycle and SM: 1 280 cycles a tile, of which a
-// quarter goes over the multiply-add units) and tcgen05 products (1 280 cycles) take as long, and a half's chain of
-// waits, fetch, maximum and exponentials, 2 000 cycles, is covered by the other half alone.  (An even division over the
-// SMs, whose parts went on through a CTA's tiles of rows, took as long for 512 tokens on 148 SMs as this does on 128: the
-// clock, 1.65 GHz, gives way.)  Shares of exponentials on the
-// multiply-add units of 1, 2, 3, 4, 5 eighths: 899, 907, 923, 958, 994 us at 2048 tokens and 66.9, 64.7, 66.1, 67.0,
-// 68.1 for 777 float16 ones.
+// Measured, 8 KV heads of 4 query heads, bfloat16, with the clock of two boxes: 2048 tokens on 32768 1 103 to 1 130 us, of
+// which stage 83, tiles 914 to 935 (70 to 71 % of the rate of a large library product of as many operations, 4.3 GB/ms of
+// operands from L2), merge 66; 512 tokens on 16384 210 us: 52, 141, 16; 777 float16 ones with a window of 2000 106 us: 18, 63,
+// 22.  What bounds the tiles: a half's chain of waits, fetch, maximum and exponentials, 2 000 cycles of a period of 2 200, is
+// covered by the other half alone.  Products (1 280 cycles a tile) have the tensor pipe busy for 56 % and exponentials (16 a
+// cycle and SM: as long, but for the quarter that goes over the multiply-add units) the special-function units for 43 %:
+// neither is full.  (An even division over the SMs, whose parts went on through a CTA's tiles of rows, took as long for 512
+// tokens on 148 SMs as this does on 128, at 1.65 GHz.)  Shares of exponentials on the multiply-add units of 1, 2, 3, 4, 5
+// eighths, before the keys had a power of two per tile: 899, 907, 923, 958, 994 us at 2048 tokens and 66.9, 64.7, 66.1,
+// 67.0, 68.1 for 777 float16 ones.
 //
-// Queries are fp16 in shared memory, each row scaled by a power of two, which is exact for both 16-bit types.
-// SPLIT (float16 queries): keys and values as pairs hi + lo, so that only the probabilities are rounded to fp16 and the
-// result is off by about its own rounding; bfloat16 queries take the hi parts alone (2^-12 against 2^-9).
+// Queries are fp16 in shared memory, each row scaled by a power of two, which is exact for both 16-bit types (from 2^-27
+// of a row's largest on).  SPLIT (float16 queries): keys and values as pairs hi + lo, so that only the probabilities
+// are rounded to fp16 and the result is off by about its own rounding (2.4e-4 in 2-norms against 64 bits, where rounding the
+// exact result gives 2.1e-4).  Bfloat16 queries take the hi parts alone, 2^-11 at worst against the half step of their type,
+// 2^-8: scores of a deviation of five, with channels 20 times the others, are then off by 1e-3, and the result by 2.0 to
+// 2.2e-3 instead of 1.65e-3; pairs would double the products.
 #include <algorithm>
 
 #include "attend.cuh"
@@ -832,7 +836,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       if (k > 0 && !rescaled) settled(&sh.o_done[x], (k - 1) & 1);  // (the probabilities before have been used)
       // The halves take turns at their exponentials, which fill the unit for them (16 a cycle and SM): while one is at
       // them, the other waits for its scores, fetches them and finds their largest.  Left to themselves both did the
-      // same at the same time (950 us for 2048 tokens on 32768; with turns 907).
+      // same at the same time (950 us for 2048 tokens on 32768; with turns 907, both before the keys' power of two).
       if (groups == 2) asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");
       const float off = TI_LIFT + e - (m > -INFINITY ? m : 0.0f);
       const uint64_t factor2 = ti_f2(by, by), off2 = ti_f2(off, off);
