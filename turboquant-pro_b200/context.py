@@ -680,8 +680,9 @@ class KVContext:
         """:meth:`import_block` of consecutive blocks from ``block`` on whose containers are tensors, on this
         context's device or not: the arrays of :meth:`export_block`, a block each along the first
         dimension (``key_indices``, ``nf4_scale``, ``nf4_mean``, ``value_indices``, ``value_norms``, and
-        ``outlier_idx`` / ``outlier_val``: ``[n_blocks, n]``, lists where the blocks differ, or ``None``).  What is on the device already does not
-        travel; one kernel writes the pages.  :meth:`restore_hot` then sets the length."""
+        ``outlier_idx`` / ``outlier_val``: ``[n_blocks, n]``, lists where the blocks differ, or ``None``).
+        What is on the device already does not travel; one kernel writes the pages.  :meth:`restore_hot` then
+        sets the length."""
         torch = _torch()
         g, dev = self.geom, self.device
         h, s, d, vb = g.n_kv_heads, g.block_tokens, g.head_dim, g.value_bits

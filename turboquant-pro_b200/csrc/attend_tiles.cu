@@ -24,7 +24,7 @@
 //     holds what counts.  The maximum is only renewed (and O rescaled) when it has grown by 2^8 since.
 // attend_tiles_combine_kernel   merges the splits, rotates the sums back (sum @ Pi), rounds.
 //
-// Measured, 8 KV heads of 4 query heads, bfloat16, with the clock of two boxes: 2048 tokens on 32768 1 103 to 1 130 us, of
+// Measured, 8 KV heads of 4 query heads, bfloat16, by the clock that the power cap leaves: 2048 tokens on 32768 1 103 to 1 130 us, of
 // which stage 83, tiles 914 to 935 (70 to 71 % of the rate of a large library product of as many operations, 4.3 GB/ms of
 // operands from L2), merge 66; 512 tokens on 16384 210 us: 52, 141, 16; 777 float16 ones with a window of 2000 106 us: 18, 63,
 // 22.  What bounds the tiles: a half's chain of waits, fetch, maximum and exponentials, 2 000 cycles of a period of 2 200, is
