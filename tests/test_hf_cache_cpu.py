@@ -156,6 +156,11 @@ def test_the_device_is_asked_once_per_mask():
         for i, m in enumerate(masks):
             hf_cache._remembered(m, (3, 7, None), lambda i=i: asked.append(i) or torch.tensor(True))
     assert asked == [0, 1, 2]
+    masks[1][0, 0, 0, 0] = False  # written again
+    assert not hf_cache._remembered(masks[1], (3, 7, None), masks[1].all)
+    with torch.inference_mode():
+        mask = torch.ones(1, 1, 1, 7, dtype=torch.bool)
+        assert hf_cache._mask_is_open(mask) and hf_cache._mask_is_causal(mask, 1, 7, None)
 
 
 @pytest.mark.parametrize("window", [None, 2])

@@ -64,6 +64,8 @@ _MASK_MEMO: list = []
 
 
 def _remembered(mask, question, ask) -> bool:
+    # (a mask that is written again, as a step's buffer may be, is another one)
+    question = question, None if mask.is_inference() else mask._version
     for ref, of, answer in _MASK_MEMO:
         if ref() is mask and of == question:
             return answer
