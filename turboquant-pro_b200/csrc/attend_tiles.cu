@@ -24,16 +24,16 @@
 //     holds what counts.  The maximum is only renewed (and O rescaled) when it has grown by 2^8 since.
 // attend_tiles_combine_kernel   merges the splits, rotates the sums back (sum @ Pi), rounds.
 //
-// Measured, 8 KV heads of 4 query heads, bfloat16, by the clock that the power cap leaves: 2048 tokens on 32768 1 103 to 1 130 us, of
-// which stage 83, tiles 914 to 935 (70 to 71 % of the rate of a large library product of as many operations, 4.3 GB/ms of
-// operands from L2), merge 66; 512 tokens on 16384 210 us: 52, 141, 16; 777 float16 ones with a window of 2000 106 us: 18, 63,
-// 22.  What bounds the tiles: a half's chain of waits, fetch, maximum and exponentials, 2 000 cycles of a period of 2 200, is
-// covered by the other half alone.  Products (1 280 cycles a tile) have the tensor pipe busy for 56 % and exponentials (16 a
-// cycle and SM: as long, but for the quarter that goes over the multiply-add units) the special-function units for 43 %:
-// neither is full.  (An even division over the SMs, whose parts went on through a CTA's tiles of rows, took as long for 512
-// tokens on 148 SMs as this does on 128, at 1.65 GHz.)  Shares of exponentials on the multiply-add units of 1, 2, 3, 4, 5
-// eighths, before the keys had a power of two per tile: 899, 907, 923, 958, 994 us at 2048 tokens and 66.9, 64.7, 66.1,
-// 67.0, 68.1 for 777 float16 ones.
+// Measured, 8 KV heads of 4 query heads, bfloat16, by the clock that the power cap leaves: 2048 tokens on 32768 1 103 to
+// 1 130 us, of which stage 83, tiles 914 to 935 (70 to 71 % of the rate of a large library product of as many
+// operations, 4.3 GB/ms of operands from L2), merge 66; 512 tokens on 16384 210 us: 52, 141, 16; 777 float16 ones with a
+// window of 2000 106 us: 18, 63, 22.  What bounds the tiles: a half's chain of waits, fetch, maximum and exponentials, 2
+// 000 cycles of a period of 2 200, is covered by the other half alone.  Products (1 280 cycles a tile) have the tensor
+// pipe busy for 56 % and exponentials (16 a cycle and SM: as long, but for the quarter that goes over the multiply-add
+// units) the special-function units for 43 %: neither is full.  (An even division over the SMs, whose parts went on
+// through a CTA's tiles of rows, took as long for 512 tokens on 148 SMs as this does on 128, at 1.65 GHz.)  Shares of
+// exponentials on the multiply-add units of 1, 2, 3, 4, 5 eighths, before the keys had a power of two per tile: 899,
+// 907, 923, 958, 994 us at 2048 tokens and 66.9, 64.7, 66.1, 67.0, 68.1 for 777 float16 ones.
 //
 // Queries are fp16 in shared memory, each row scaled by a power of two, which is exact for both 16-bit types (from 2^-27
 // of a row's largest on).  SPLIT (float16 queries): keys and values as pairs hi + lo, so that only the probabilities
