@@ -705,11 +705,14 @@ class KVContext:
                 staging.view(dtype)[:, at // x.element_size():][:, :count] = x.reshape(n, count)
             if idx is None:
                 idx, words = [torch.empty(0, dtype=torch.int32)] * n, [torch.empty(0, dtype=torch.int16)] * n
-            if len(idx) != n or len(words) != n or [len(i) for i in idx] != [len(w) for w in words]:
+            # (of the tensors' rows nothing is asked one by one: short blocks are thousands)
+            of = [[x.shape[1]] * len(x) if isinstance(x, torch.Tensor) and x.dim() == 2 else [len(i) for i in x]
+                  for x in (idx, words)]
+            if len(of[0]) != n or of[0] != of[1]:
                 raise ValueError(f"outlier_idx and outlier_val must be of {n} blocks, as many values as indices each")
-            counts = torch.tensor([len(i) for i in idx], dtype=torch.int64, device=dev)
-            idx, words = (torch.cat([torch.as_tensor(x).reshape(-1) for x in xs]).to(dev)
-                          for xs in (idx, words))
+            counts = torch.tensor(of[0], dtype=torch.int64, device=dev)
+            idx, words = ((x.reshape(-1) if isinstance(x, torch.Tensor) else
+                           torch.cat([torch.as_tensor(i).reshape(-1) for i in x])).to(dev) for x in (idx, words))
             if idx.dtype not in (torch.int32, torch.int64) \
                     or words.dtype not in (torch.float16, torch.int16, torch.uint16):
                 raise ValueError(f"expected integers and float16 values (or their words) of outliers, got {idx.dtype} and "
