@@ -206,6 +206,28 @@ typedef struct tq_attend_args {
 int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* args, void* stream, size_t* bytes);
 int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* args, void* stream);
 
+/* The blocks of a sequence that are worth attending for a query token, per KV head, by a cheap score: the sum over the
+ * group's query heads of the largest q . k that the block's grid allows, outliers aside - a key's channel lies between
+ * mean + lo * scale and mean + hi * scale (NF4: -1 and 1, uniform: 0 and 15).  Query token i of sequence s stands at a
+ * position p as in tq_attend; the blocks that begin at p or before are ranked.  The first `first` blocks and the one
+ * that the token itself stands in come before all others; equal scores: the lowest index; what is no number comes last.
+ * `out` gets the n_blocks best, ascending, and -1 behind them where there are fewer (all -1 for rows that have
+ * no position).  Keys of TQ_KEYS_POLAR have no grid: TQ_ERR_UNSUPPORTED. */
+typedef struct tq_select_args {
+  const void* q;            /* device, as in tq_attend_args; any alignment of whole elements         */
+  int32_t* out;             /* device, [seq_count][n_tokens][n_kv_heads][n_blocks]                   */
+  const int32_t* q_lens;    /* device, [seq_count], as in tq_attend_args; null: n_tokens each        */
+  void* workspace;          /* device, 256-byte aligned, as tq_select_blocks_workspace asks for; null if that is none */
+  size_t workspace_bytes;
+  int64_t q_seq_stride, q_tok_stride, q_head_stride;
+  int32_t layer, seq_begin, seq_count, n_tokens;
+  int32_t q_dtype;
+  int32_t n_blocks, first;
+  int32_t reserved_;
+} tq_select_args;
+int32_t tq_select_blocks_workspace(tq_ctx* ctx, const tq_select_args* args, void* stream, size_t* bytes);
+int32_t tq_select_blocks(tq_ctx* ctx, const tq_select_args* args, void* stream);
+
 /* Root-mean-square norm of every query and key head and their rotation by position, in one pass: what stands
  * between a layer's projections and tq_append / tq_attend.
  *   y = x / sqrt(mean(x^2) + eps) * weight   where a weight is given, else x
@@ -230,6 +252,20 @@ int32_t tq_norm_rope(const tq_rope* rope, int32_t device, void* stream);
 /* The same for tokens that are about to be appended to sequences seq_begin .. of a layer: their positions
  * follow from the lengths on the device (rope->positions is not looked at). */
 int32_t tq_ctx_norm_rope(tq_ctx* ctx, int32_t layer, int32_t seq_begin, const tq_rope* rope, void* stream);
+/* The same where the sequences go on from sequence `prefix` of the layer: its length is added to their positions (see
+ * tq_attend_prefix; -1: none). */
+int32_t tq_ctx_norm_rope_after(tq_ctx* ctx, int32_t layer, int32_t seq_begin, int32_t prefix, const tq_rope* rope,
+                               void* stream);
+/* tq_norm_rope with positions of several axes (the time, height and width of images and video): frequency i turns by
+ * the position of axis axes[i], which is pos_axis_stride elements behind that of the axis before.  A null `axes`
+ * argument: one axis. */
+typedef struct tq_rope_axes {
+  const uint8_t* axes;      /* device, [rotary_dim / 2]; numbers from n_axes on count as n_axes - 1    */
+  int64_t pos_axis_stride;
+  int32_t n_axes;
+  int32_t reserved_;
+} tq_rope_axes;
+int32_t tq_norm_rope_axes(const tq_rope* rope, const tq_rope_axes* axes, int32_t device, void* stream);
 
 /* Sequence-split form of tq_decode for one long sequence spread over several devices:
  * attends only cold blocks [block_begin, block_end) and, if `with_hot` is non-zero, the

@@ -63,6 +63,16 @@ class TqAttendArgs(C.Structure):
     ]
 
 
+class TqSelectArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("q_lens", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t), ("q_seq_stride", C.c_int64), ("q_tok_stride", C.c_int64),
+        ("q_head_stride", C.c_int64), ("layer", C.c_int32), ("seq_begin", C.c_int32),
+        ("seq_count", C.c_int32), ("n_tokens", C.c_int32), ("q_dtype", C.c_int32),
+        ("n_blocks", C.c_int32), ("first", C.c_int32), ("reserved_", C.c_int32),
+    ]
+
+
 class TqRope(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out", "q_weight", "k_weight", "inv_freq",
                                           "positions")] + [
@@ -72,6 +82,11 @@ class TqRope(C.Structure):
         (n, C.c_int32) for n in ("n_seqs", "n_tokens", "n_q_heads", "n_kv_heads", "dtype",
                                  "weight_dtype", "pos_bits", "rotary_dim")] + [
         ("eps", C.c_float), ("reserved_", C.c_int32)]
+
+
+class TqRopeAxes(C.Structure):
+    _fields_ = [("axes", C.c_void_p), ("pos_axis_stride", C.c_int64), ("n_axes", C.c_int32),
+                ("reserved_", C.c_int32)]
 
 
 # every exported symbol of include/tqb200.h with its signature
@@ -94,7 +109,13 @@ SIGNATURES = {
     "tq_attend_workspace": (C.c_int32, [C.c_void_p, C.POINTER(TqAttendArgs), C.c_void_p,
                                         C.POINTER(C.c_size_t)]),
     "tq_attend": (C.c_int32, [C.c_void_p, C.POINTER(TqAttendArgs), C.c_void_p]),
+    "tq_select_blocks_workspace": (C.c_int32, [C.c_void_p, C.POINTER(TqSelectArgs), C.c_void_p,
+                                               C.POINTER(C.c_size_t)]),
+    "tq_select_blocks": (C.c_int32, [C.c_void_p, C.POINTER(TqSelectArgs), C.c_void_p]),
     "tq_norm_rope": (C.c_int32, [C.POINTER(TqRope), C.c_int32, C.c_void_p]),
+    "tq_norm_rope_axes": (C.c_int32, [C.POINTER(TqRope), C.POINTER(TqRopeAxes), C.c_int32, C.c_void_p]),
+    "tq_ctx_norm_rope_after": (C.c_int32, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.POINTER(TqRope),
+                                           C.c_void_p]),
     "tq_ctx_norm_rope": (C.c_int32, [C.c_void_p, C.c_int32, C.c_int32, C.POINTER(TqRope),
                                      C.c_void_p]),
     "tq_decode_partial": (C.c_int32, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32,

@@ -22,7 +22,7 @@ import operator
 import numpy as np
 
 from . import _lib
-from ._lib import REGIONS, TqAttendArgs, TqBuffers, TqGeom, TqSizes, check
+from ._lib import REGIONS, TqAttendArgs, TqBuffers, TqGeom, TqSelectArgs, TqSizes, check
 
 _NO_GUARD = contextlib.nullcontext()
 
@@ -321,9 +321,7 @@ class KVContext:
             raise ValueError(f"sinks must not be negative, got {sinks}")
         lens = None
         if q_lens is not None:
-            if q_lens.dtype != torch.int32 or q_lens.device != dev or q_lens.shape != (shape[0],):
-                raise ValueError(f"q_lens must be an int32 tensor of shape ({shape[0]},) on {dev}")
-            q_lens = q_lens.contiguous()
+            q_lens = self._check_q_lens(q_lens, shape[0])
             lens = q_lens.data_ptr()
         if out is None:
             out = torch.empty(shape, dtype=dtype, device=dev)
@@ -355,12 +353,65 @@ class KVContext:
             check(self._lib.tq_attend(self._h, ref, stream))
         return out
 
+    def select_blocks(self, layer: int, q, n: int, *, first: int = 1, q_lens=None, seq_begin: int = 0, out=None):
+        """The ``n`` blocks (of ``block_tokens`` tokens) that are worth attending for each query token and KV head, for
+        ``blocks`` of :meth:`attend`: int32 ``[n_seqs', T, n_kv_heads, n]``, ascending, ``-1`` behind them
+        where there are fewer.
+
+        The score of a block is the sum over the group's query heads of the largest ``q . k`` that its grid allows,
+        outliers aside: what a page holds per channel, its zero-points and scales, is all that is read, 1 kB of some 35.
+        ``q`` and ``q_lens`` are those of :meth:`attend`.  Blocks that begin behind the token are no candidates;
+        the ``first`` first ones, and the one that the token itself stands in (a chunk may be longer than
+        the window), come before all others.  Equal scores go by the lower index, what is no number comes last.
+        """
+        torch = _torch()
+        g, dev, codes = self.geom, self.device, _dtype_codes()
+        shape, dtype = q.shape, q.dtype
+        if len(shape) != 4 or shape[2] != g.n_q_heads or shape[3] != g.head_dim:
+            raise ValueError(f"expected q of shape [n_seqs, T, {g.n_q_heads}, {g.head_dim}], "
+                             f"got {tuple(shape)}")
+        if q.device != dev:
+            raise ValueError(f"q lives on {q.device}, the context on {dev}")
+        if dtype not in codes:
+            raise ValueError(f"q must be float32, float16 or bfloat16, got {dtype}")
+        n, first = operator.index(n), operator.index(first)
+        if not 1 <= n < 2**31 or not 0 <= first < 2**31:
+            raise ValueError(f"n must be at least 1 and first not negative, got {n} and {first}")
+        lens = None
+        if q_lens is not None:
+            q_lens = self._check_q_lens(q_lens, shape[0])
+            lens = q_lens.data_ptr()
+        shape = (shape[0], shape[1], g.n_kv_heads, n)
+        if out is None:
+            out = torch.empty(shape, dtype=torch.int32, device=dev)
+        elif out.shape != shape or out.dtype != torch.int32 or out.device != dev or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous int32 tensor of shape {shape} on {dev}")
+        q = q.detach()
+        if q.stride(3) != 1:
+            q = q.contiguous()
+        s0, s1, s2, _ = q.stride()
+        a = TqSelectArgs(q.data_ptr(), out.data_ptr(), lens, None, 0, s0, s1, s2, layer, seq_begin,
+                         shape[0], shape[1], codes[dtype], n, first)
+        with self._here():
+            stream, ref, size = self._stream(), C.byref(a), C.c_size_t()
+            check(self._lib.tq_select_blocks_workspace(self._h, ref, stream, C.byref(size)))
+            if size.value:
+                work = torch.empty(size.value, dtype=torch.uint8, device=dev)
+                a.workspace, a.workspace_bytes = work.data_ptr(), size.value
+            check(self._lib.tq_select_blocks(self._h, ref, stream))
+        return out
+
+    def _check_q_lens(self, q_lens, n_seqs: int):
+        if q_lens.dtype != _torch().int32 or q_lens.device != self.device or q_lens.shape != (n_seqs,):
+            raise ValueError(f"q_lens must be an int32 tensor of shape ({n_seqs},) on {self.device}")
+        return q_lens.contiguous()
+
     def norm_rope(self, layer: int, q, k, inv_freq, positions=None, *, q_weight=None, k_weight=None,
-                  eps: float = 1e-6, seq_begin: int = 0):
+                  eps: float = 1e-6, seq_begin: int = 0, axes=None, prefix: int | None = None):
         """:func:`~turboquant_pro_b200.norm_rope` of the tokens that sequences ``seq_begin`` .. of
         ``layer`` get next: without ``positions`` they follow what is stored (read on the device, so
-        a captured step stays right as the sequences grow).  ``q`` ``[n_seqs', T, n_q_heads, D]``,
-        ``k`` ``[n_seqs', T, n_kv_heads, D]``."""
+        a captured step stays right as the sequences grow), behind the tokens of sequence ``prefix`` if there is one
+        (see :meth:`attend`).  ``q`` ``[n_seqs', T, n_q_heads, D]``, ``k`` ``[n_seqs', T, n_kv_heads, D]``."""
         from .rotary import _norm_rope
 
         g = self.geom
@@ -369,8 +420,19 @@ class KVContext:
                              f"{g.n_kv_heads}, D], got {tuple(q.shape)} and {tuple(k.shape)}")
         if q.device != self.device:
             raise ValueError(f"q lives on {q.device}, the context on {self.device}")
-        return _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps,
-                          (self, layer, seq_begin))
+        if prefix is not None:
+            if positions is not None:
+                raise ValueError("positions are given: they count the prefix's tokens already")
+            prefix = self._check_prefix(prefix, seq_begin, q.shape[0])
+        return _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, axes,
+                          (self, layer, seq_begin, -1 if prefix is None else prefix))
+
+    def _check_prefix(self, prefix: int, seq_begin: int, n_seqs: int) -> int:
+        prefix = operator.index(prefix)
+        if not 0 <= prefix < self.n_seqs or seq_begin <= prefix < seq_begin + n_seqs:
+            raise ValueError(f"prefix must be a sequence of the context outside the call's own {seq_begin} .. "
+                             f"{seq_begin + n_seqs - 1}, got {prefix}")
+        return prefix
 
     def step(self, layer: int, q, k, v, inv_freq, *, q_weight=None, k_weight=None, eps: float = 1e-6,
              window: int | None = None, sinks: int = 0, seq_begin: int = 0):

@@ -3,6 +3,18 @@
 
 #include "attend.cuh"
 
+// The most tokens a sequence of the call may hold when the kernels run: the host's lengths, or the
+// capacity where the launch is captured, since a replay may find longer sequences.
+int tq_most_tokens(const tq_ctx* ctx, int layer, int seq_begin, int seq_count, cudaStream_t st) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone)
+    return ctx->g.max_tokens_per_seq;
+  int n = 0;
+  for (int s = seq_begin; s < seq_begin + seq_count; ++s)
+    n = std::max(n, ctx->len[(size_t)layer * ctx->g.n_seqs + s]);
+  return n;
+}
+
 namespace {
 
 constexpr size_t AT_ONE_GO = (size_t)1 << 30;  // workspace that a call asks for at most, unless one
@@ -36,18 +48,6 @@ int check_args(tq_ctx* ctx, const tq_attend_args* r) {
   if (ctx->sm_count == 0)
     TQ_CUDA(cudaDeviceGetAttribute(&ctx->sm_count, cudaDevAttrMultiProcessorCount, ctx->device));
   return TQ_OK;
-}
-
-// The most tokens a sequence of the call may hold when the kernels run: the host's lengths, or the
-// capacity where the launch is captured, since a replay may find longer sequences.
-int most_tokens(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
-  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(st, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone)
-    return ctx->g.max_tokens_per_seq;
-  int n = 0;
-  for (int s = r->seq_begin; s < r->seq_begin + r->seq_count; ++s)
-    n = std::max(n, ctx->len[(size_t)r->layer * ctx->g.n_seqs + s]);
-  return n;
 }
 
 // The form that does a call soonest.  16-bit queries: few rows do best where their keys and values are decoded row
@@ -84,7 +84,7 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
   const tq_geom& g = ctx->g;
   Plan p = {};
   p.seqs = INT_MAX;
-  const int n = most_tokens(ctx, r, st), rows = r->n_tokens * g.group;
+  const int n = tq_most_tokens(ctx, r->layer, r->seq_begin, r->seq_count, st), rows = r->n_tokens * g.group;
   const int nb = n_cold_blocks(n, g.hot_window, g.block_tokens);
   p.form = choose(ctx, r, n);
   const int sm_count = ctx->sm_count;

@@ -107,6 +107,8 @@ int attend_shared(K kernel, size_t bytes, int device, bool (&done)[64]) {
   return TQ_OK;
 }
 
+// The most tokens that one of these sequences may hold when a call's kernels run
+int tq_most_tokens(const tq_ctx* ctx, int layer, int seq_begin, int seq_count, cudaStream_t st);
 int tq_launch_attend_general(const AttendArgs& a, cudaStream_t st);
 int tq_launch_attend_combine(const AttendArgs& a, cudaStream_t st);
 // Few rows, 256-token blocks of per-channel keys, queries on 16-byte boundaries; the merge too.

@@ -10,6 +10,9 @@
 // float32, and the weights times cosines and sines, so that a channel costs two multiply-adds.  Sums, norm and
 // rotation are float32, rounded once.
 //
+// Positions of several axes (time, height, width): every frequency has the number of the axis whose position it goes
+// by, one more load per angle.
+//
 // A CTA of eight warps takes one token of few, or up to eight, a warp each, whose angles are one step of the CTA.
 // Bound by launch and latency for single tokens (4 us); for prompts by reading and writing q and k, at 68 to 80 % of
 // a plain copy's rate (8 x 2048 tokens of 32 + 8 heads, bfloat16: 75 us, 4.5 TB/s), and the unpacking, shuffles and
@@ -25,6 +28,8 @@ constexpr int NR_THREADS = 256;
 struct RopeArgs {
   tq_rope r;
   const int32_t* seq_len;  // positions of the tokens that follow what is stored; null: r.positions
+  const int32_t* before;   // and behind so many tokens of a prefix (null: none)
+  tq_rope_axes x;          // x.axes null: a position each
 };
 
 TQ_DEV float nr_weight(const void* w, int i, int dt) {
@@ -225,9 +230,12 @@ __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(RopeArgs a, in
     if (tk >= (uint32_t)tokens) break;
     const uint32_t us = tk / (uint32_t)r.n_tokens, ut = tk - us * (uint32_t)r.n_tokens;
     int64_t p;
-    if (a.seq_len != nullptr) p = (int64_t)a.seq_len[us] + ut;
-    else {
-      const int64_t at = (int64_t)us * r.pos_seq_stride + (int64_t)ut * r.pos_tok_stride;
+    if (a.seq_len != nullptr) {
+      p = (int64_t)a.seq_len[us] + ut;
+      if (a.before != nullptr) p += *a.before;
+    } else {
+      int64_t at = (int64_t)us * r.pos_seq_stride + (int64_t)ut * r.pos_tok_stride;
+      if (a.x.axes != nullptr) at += min((int)a.x.axes[f], a.x.n_axes - 1) * a.x.pos_axis_stride;
       p = r.pos_bits == 64 ? ((const int64_t*)r.positions)[at] : (int64_t)((const int32_t*)r.positions)[at];
     }
     const double turns = (double)p * ((double)r.inv_freq[f] * 0.15915494309189533577);
@@ -301,7 +309,8 @@ int check_rope(const tq_rope* r, bool stored) {
   return TQ_OK;
 }
 
-int launch(const tq_rope* r, const int32_t* seq_len, int device, cudaStream_t st) {
+int launch(const tq_rope* r, const int32_t* seq_len, const int32_t* before, const tq_rope_axes& x, int device,
+           cudaStream_t st) {
   const int tokens = r->n_seqs * r->n_tokens;
   if (tokens == 0 || r->n_q_heads + r->n_kv_heads == 0) return TQ_OK;
   static std::atomic<int> counts[64];  // (asked for once per device)
@@ -314,7 +323,7 @@ int launch(const tq_rope* r, const int32_t* seq_len, int device, cudaStream_t st
   const bool vec = ((uintptr_t)r->q | (uintptr_t)r->k) % 16 == 0 &&
                    ((r->q_seq_stride | r->q_tok_stride | r->q_head_stride | r->k_seq_stride |
                      r->k_tok_stride | r->k_head_stride) & (e - 1)) == 0;
-  RopeArgs a = {*r, seq_len};
+  RopeArgs a = {*r, seq_len, before, x};
   const bool paired = r->rotary_dim / 2 % e == 0;
   switch (r->dtype) {
     case TQ_F32: start<TQ_F32, true>(a, tokens, sms, vec, st); break;
@@ -328,14 +337,24 @@ int launch(const tq_rope* r, const int32_t* seq_len, int device, cudaStream_t st
 }  // namespace
 
 extern "C" int32_t tq_norm_rope(const tq_rope* r, int32_t device, void* stream) {
-  const int rc = check_rope(r, false);
-  if (rc != TQ_OK) return rc;
-  TQ_CUDA(cudaSetDevice(device));
-  return launch(r, nullptr, device, (cudaStream_t)stream);
+  return tq_norm_rope_axes(r, nullptr, device, stream);
 }
 
-extern "C" int32_t tq_ctx_norm_rope(tq_ctx* ctx, int32_t layer, int32_t seq_begin, const tq_rope* r,
-                                    void* stream) {
+extern "C" int32_t tq_norm_rope_axes(const tq_rope* r, const tq_rope_axes* x, int32_t device, void* stream) {
+  const int rc = check_rope(r, false);
+  if (rc != TQ_OK) return rc;
+  TQ_REQUIRE(x == nullptr || ((x->axes != nullptr || r->rotary_dim == 0) && x->n_axes >= 1), TQ_ERR_INVALID,
+             "axes must be a device pointer, and n_axes at least 1");
+  TQ_CUDA(cudaSetDevice(device));
+  return launch(r, nullptr, nullptr, x == nullptr ? tq_rope_axes{} : *x, device, (cudaStream_t)stream);
+}
+
+extern "C" int32_t tq_ctx_norm_rope(tq_ctx* ctx, int32_t layer, int32_t seq_begin, const tq_rope* r, void* stream) {
+  return tq_ctx_norm_rope_after(ctx, layer, seq_begin, -1, r, stream);
+}
+
+extern "C" int32_t tq_ctx_norm_rope_after(tq_ctx* ctx, int32_t layer, int32_t seq_begin, int32_t prefix,
+                                          const tq_rope* r, void* stream) {
   TQ_REQUIRE(ctx != nullptr && layer >= 0 && layer < ctx->g.n_layers, TQ_ERR_INVALID, "bad context or layer");
   const int rc = check_rope(r, true);
   if (rc != TQ_OK) return rc;
@@ -344,8 +363,9 @@ extern "C" int32_t tq_ctx_norm_rope(tq_ctx* ctx, int32_t layer, int32_t seq_begi
              "head counts do not match the context");
   TQ_REQUIRE(seq_begin >= 0 && r->n_seqs >= 0 && (int64_t)seq_begin + r->n_seqs <= g.n_seqs, TQ_ERR_INVALID,
              "sequence range out of bounds");
+  TQ_REQUIRE(prefix >= -1 && prefix < g.n_seqs, TQ_ERR_INVALID, "prefix is no sequence of the context");
   TQ_CUDA(cudaSetDevice(ctx->device));
-  const int32_t* len = (const int32_t*)((const uint8_t*)ctx->b.state + state_len_off(g)) +
-                       (size_t)layer * g.n_seqs + seq_begin;
-  return launch(r, len, ctx->device, (cudaStream_t)stream);
+  const int32_t* len = (const int32_t*)((const uint8_t*)ctx->b.state + state_len_off(g)) + (size_t)layer * g.n_seqs;
+  return launch(r, len + seq_begin, prefix < 0 ? nullptr : len + prefix, tq_rope_axes{}, ctx->device,
+                (cudaStream_t)stream);
 }

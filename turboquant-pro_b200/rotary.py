@@ -11,7 +11,7 @@ from __future__ import annotations
 import ctypes as C
 
 from . import _lib
-from ._lib import TqRope, check
+from ._lib import TqRope, TqRopeAxes, check
 from .context import _NO_GUARD, _dtype_codes, _raw_stream, _torch
 
 __all__ = ["norm_rope"]
@@ -19,7 +19,7 @@ __all__ = ["norm_rope"]
 HEAD_DIM = 128
 
 
-def norm_rope(q, k, inv_freq, positions, *, q_weight=None, k_weight=None, eps: float = 1e-6):
+def norm_rope(q, k, inv_freq, positions, *, q_weight=None, k_weight=None, eps: float = 1e-6, axes=None):
     """Root-mean-square norm of every query and key head and their rotation by position, in one pass.
 
     ``q`` ``[n_seqs, T, n_q_heads, 128]``, ``k`` ``[n_seqs, T, n_kv_heads, 128]``: CUDA tensors of one
@@ -30,12 +30,16 @@ def norm_rope(q, k, inv_freq, positions, *, q_weight=None, k_weight=None, eps: f
     after it are not turned).  ``positions``: int32 or int64, ``[n_seqs, T]`` or ``[T]``; angles
     are reduced in 64 bits, so far positions keep their precision.
 
+    ``axes``: positions with several axes, as the time, height and width of images and video have them.  A uint8 CUDA tensor
+    ``[rotary_dim / 2]`` with the axis that each frequency goes by (one after the other, or in turn);
+    ``positions`` is then ``[n_axes, n_seqs, T]`` or ``[n_axes, T]``.  Numbers beyond the axes count as the last one.
+
     Returns new contiguous tensors ``(q, k)``, float32 arithmetic rounded once.  Inference only: no
     gradients.
     """
     if positions is None:
         raise ValueError("positions are needed (KVContext.norm_rope knows those of a cache)")
-    return _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, None)
+    return _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, axes, None)
 
 
 def _weight(w, codes, other):
@@ -44,7 +48,7 @@ def _weight(w, codes, other):
     return w.contiguous(), codes[w.dtype]
 
 
-def _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, cache):
+def _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, axes, cache):
     # (a decode step's call is a few microseconds on the GPU: the checks are kept short)
     torch = _torch()
     q_shape, k_shape, dev, dtype = q.shape, k.shape, q.device, q.dtype
@@ -60,8 +64,8 @@ def _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, cache):
         raise ValueError(f"q and k must share float32, float16 or bfloat16, got {dtype} and {k.dtype}")
     if k.device != dev or inv_freq.device != dev or (positions is not None and positions.device != dev) \
             or (q_weight is not None and q_weight.device != dev) \
-            or (k_weight is not None and k_weight.device != dev):
-        raise ValueError(f"k, inv_freq, positions and weights must live where q does, on {dev}")
+            or (k_weight is not None and k_weight.device != dev) or (axes is not None and axes.device != dev):
+        raise ValueError(f"k, inv_freq, positions, axes and weights must live where q does, on {dev}")
     if torch.is_grad_enabled() and (
             q.requires_grad or k.requires_grad or inv_freq.requires_grad
             or (q_weight is not None and q_weight.requires_grad)
@@ -79,7 +83,18 @@ def _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, cache):
         k_weight, weight_type = _weight(k_weight, codes, None)
         kw = k_weight.data_ptr()
     n, t = q_shape[0], q_shape[1]
-    pos, pos_bits, ps, pt = None, 0, 0, 0
+    pos, pos_bits, ps, pt, several = None, 0, 0, 0, None
+    if axes is not None:
+        if positions is None:
+            raise ValueError("axes need positions")
+        if axes.dtype != torch.uint8 or axes.shape != inv_freq.shape:
+            raise ValueError(f"axes must be uint8, one for each of the {inv_freq.shape[0]} frequencies, got {axes.dtype} "
+                             f"{tuple(axes.shape)}")
+        if positions.dim() < 2 or positions.shape[0] < 1 or positions.shape[1:] not in ((n, t), (t,)):
+            raise ValueError(f"positions must be [n_axes, {n}, {t}] or [n_axes, {t}], got {tuple(positions.shape)}")
+        axes = axes.contiguous()
+        several = TqRopeAxes(axes.data_ptr(), positions.stride(0), positions.shape[0])
+        positions = positions[0]
     if positions is not None:
         if positions.dtype == torch.int64:
             pos_bits = 64
@@ -112,8 +127,10 @@ def _norm_rope(q, k, inv_freq, positions, q_weight, k_weight, eps, cache):
     with _NO_GUARD if torch.cuda.current_device() == index else torch.cuda.device(dev):
         stream = _raw_stream()(index)
         if cache is not None and positions is None:
-            ctx, layer, seq_begin = cache
-            check(lib.tq_ctx_norm_rope(ctx._h, layer, seq_begin, C.byref(r), stream))
+            ctx, layer, seq_begin, prefix = cache
+            check(lib.tq_ctx_norm_rope_after(ctx._h, layer, seq_begin, prefix, C.byref(r), stream))
+        elif several is not None:
+            check(lib.tq_norm_rope_axes(C.byref(r), C.byref(several), index, stream))
         else:
             check(lib.tq_norm_rope(C.byref(r), index, stream))
     return q_out, k_out
