@@ -228,6 +228,13 @@ typedef struct tq_select_args {
 int32_t tq_select_blocks_workspace(tq_ctx* ctx, const tq_select_args* args, void* stream, size_t* bytes);
 int32_t tq_select_blocks(tq_ctx* ctx, const tq_select_args* args, void* stream);
 
+/* tq_attend on listed blocks: of the tokens in blocks a query token's KV head sees only those of the blocks that `blocks`
+ * (device, [seq_count][n_tokens][n_kv_heads][n_blocks], as tq_select_blocks gives them) names, of them and of the
+ * uncompressed window those up to its position.  A list ascends; it ends at the first entry that is not above the one
+ * before, or no block of the sequence.  `window` and `sinks` must be 0. */
+int32_t tq_attend_blocks_workspace(tq_ctx* ctx, const tq_attend_args* args, int32_t n_blocks, void* stream, size_t* bytes);
+int32_t tq_attend_blocks(tq_ctx* ctx, const tq_attend_args* args, const int32_t* blocks, int32_t n_blocks, void* stream);
+
 /* Root-mean-square norm of every query and key head and their rotation by position, in one pass: what stands
  * between a layer's projections and tq_append / tq_attend.
  *   y = x / sqrt(mean(x^2) + eps) * weight   where a weight is given, else x

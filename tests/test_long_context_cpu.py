@@ -43,12 +43,14 @@ def test_norm_rope_axes_refuses(lib, rope, axes):
 
 
 def test_null_arguments(lib):
-    from turboquant_pro_b200._lib import TqSelectArgs
+    from turboquant_pro_b200._lib import TqAttendArgs, TqSelectArgs
 
     size = C.c_size_t()
     assert lib.tq_norm_rope_axes(None, None, 0, None) == -1
     assert lib.tq_ctx_norm_rope_after(None, 0, 0, -1, C.byref(_rope()), None) == -1
     assert lib.tq_select_blocks(None, C.byref(TqSelectArgs()), None) == -1
+    assert lib.tq_attend_blocks(None, C.byref(TqAttendArgs()), None, 1, None) == -1
+    assert lib.tq_attend_blocks_workspace(None, C.byref(TqAttendArgs()), 1, None, C.byref(size)) == -1
     assert lib.tq_select_blocks_workspace(None, C.byref(TqSelectArgs()), None, C.byref(size)) == -1
 
 

@@ -283,7 +283,7 @@ class KVContext:
         return out
 
     def attend(self, layer: int, q, window: int | None = None, sinks: int = 0, q_lens=None,
-               seq_begin: int = 0, out=None, max_workspace: int | None = None):
+               seq_begin: int = 0, out=None, max_workspace: int | None = None, blocks=None):
         """Attention of one or many query tokens per sequence on the codes, with the causal mask, a
         sliding window and first tokens that stay visible.
 
@@ -301,6 +301,11 @@ class KVContext:
         (float16 queries: 1024) per visible token and KV head, up to 1 GB, or what one sequence needs if that is
         more.  With ``max_workspace`` it takes at most so many bytes and goes in several rounds; a
         :class:`TqError` says that they do not do for one sequence.
+
+        ``blocks``: int32 CUDA tensor ``[n_seqs', T, n_kv_heads, n]``, as :meth:`select_blocks` gives it.  Of the tokens in
+        blocks a query token then sees, for each KV head, those of the listed ones up to its own position, and the
+        uncompressed window as ever.  A list ascends; it ends at the first entry that is not above the one before it, or
+        no block of the sequence (``-1``).  It takes the place of ``window`` and ``sinks``.
         """
         # (a decode step's call is some microseconds on the GPU: the checks are kept short)
         torch = _torch()
@@ -319,6 +324,14 @@ class KVContext:
             raise ValueError(f"window must be at least 1 (or None), got {window}")
         if sinks < 0:
             raise ValueError(f"sinks must not be negative, got {sinks}")
+        if blocks is not None:
+            if window is not None or sinks:
+                raise ValueError("blocks take the place of a window: window and sinks must be left out")
+            if blocks.dtype != torch.int32 or blocks.device != dev or blocks.dim() != 4 \
+                    or blocks.shape[:3] != (shape[0], shape[1], g.n_kv_heads):
+                raise ValueError(f"blocks must be an int32 tensor of shape ({shape[0]}, {shape[1]}, {g.n_kv_heads}, n) on "
+                                 f"{dev}")
+            blocks = blocks.contiguous()
         lens = None
         if q_lens is not None:
             q_lens = self._check_q_lens(q_lens, shape[0])
@@ -346,11 +359,17 @@ class KVContext:
                          min(sinks, 2**31 - 1))
         with self._here():
             stream, ref, size = self._stream(), C.byref(a), C.c_size_t()
-            check(self._lib.tq_attend_workspace(self._h, ref, stream, C.byref(size)))
+            if blocks is None:
+                check(self._lib.tq_attend_workspace(self._h, ref, stream, C.byref(size)))
+            else:
+                check(self._lib.tq_attend_blocks_workspace(self._h, ref, blocks.shape[3], stream, C.byref(size)))
             n = size.value if max_workspace is None else min(size.value, max(max_workspace, 0))
             work = torch.empty(n, dtype=torch.uint8, device=dev)
             a.workspace, a.workspace_bytes = work.data_ptr(), n
-            check(self._lib.tq_attend(self._h, ref, stream))
+            if blocks is None:
+                check(self._lib.tq_attend(self._h, ref, stream))
+            else:
+                check(self._lib.tq_attend_blocks(self._h, ref, blocks.data_ptr(), blocks.shape[3], stream))
         return out
 
     def select_blocks(self, layer: int, q, n: int, *, first: int = 1, q_lens=None, seq_begin: int = 0, out=None):

@@ -30,6 +30,31 @@ struct Plan {
   size_t fixed_bytes, seq_bytes;  // workspace: of a launch, of a sequence
 };
 
+// A call: the caller's arguments, and the blocks on its lists (listed).
+struct Call : tq_attend_args {
+  const int32_t* list;
+  int32_t n_list;
+  bool listed;
+};
+Call plain_call(const tq_attend_args* r) {
+  Call c = {};
+  (tq_attend_args&)c = *r;
+  return c;
+}
+// The sequences from `s` on, `n` of them.
+Call part_of(const tq_ctx* ctx, const Call& r, int s, int n) {
+  const tq_geom& g = ctx->g;
+  const size_t esz = elem_size(r.q_dtype);
+  Call part = r;
+  part.seq_begin = r.seq_begin + s;
+  part.seq_count = n;
+  part.q = (const uint8_t*)r.q + (int64_t)s * r.q_seq_stride * (int64_t)esz;
+  part.out = (uint8_t*)r.out + (size_t)s * r.n_tokens * g.n_q_heads * TQ_D * esz;
+  part.q_lens = r.q_lens == nullptr ? nullptr : r.q_lens + s;
+  part.list = r.list == nullptr ? nullptr : r.list + (size_t)s * r.n_tokens * g.n_kv_heads * r.n_list;
+  return part;
+}
+
 int check_args(tq_ctx* ctx, const tq_attend_args* r) {
   TQ_REQUIRE(ctx != nullptr && r != nullptr, TQ_ERR_INVALID, "null argument");
   const tq_geom& g = ctx->g;
@@ -64,11 +89,13 @@ int check_args(tq_ctx* ctx, const tq_attend_args* r) {
 // float32 queries, which TILES would round: ROWS up to 48 rows, GENERAL above (ROWS against GENERAL, four
 // sequences of 8000, 8 KV heads: 32 rows 222 and 344, 48: 311 and 351, 64: 394 and 361, 128: 740 and 693; eight of 2000, 32
 // KV heads: 32 rows 527 and 666, 64: 1100 and 729).
-Form choose(const tq_ctx* ctx, const tq_attend_args* r, int n) {
+// Listed blocks differ from token to token: what is written for few rows, where the blocks are those it is written for.
+Form choose(const tq_ctx* ctx, const Call* r, int n) {
   const tq_geom& g = ctx->g;
   const int rows = r->n_tokens * g.group;
   const bool channels = g.key_mode != TQ_KEYS_POLAR && !ctx->force_generic, blocks = g.block_tokens == 256;
   if (!channels) return GENERAL;
+  if (r->listed) return blocks ? ROWS : GENERAL;
   if (r->q_dtype == TQ_F32) return blocks && rows <= 48 ? ROWS : GENERAL;
   const double seen = r->window == 0 ? n : std::min((double)n, (double)r->window + r->n_tokens + r->sinks);
   const double w = seen * r->seq_count * g.n_kv_heads / 1000.0;
@@ -80,7 +107,7 @@ Form choose(const tq_ctx* ctx, const tq_attend_args* r, int n) {
 
 // Splits of the tokens: enough CTAs for the GPU, of what is visible in the longest sequence, in blocks and in
 // the window.
-Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
+Plan make_plan(const tq_ctx* ctx, const Call* r, cudaStream_t st) {
   const tq_geom& g = ctx->g;
   Plan p = {};
   p.seqs = INT_MAX;
@@ -122,6 +149,7 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
     a.sinks = r->sinks;
     a.q_dtype = r->q_dtype;
     a.sm_count = sm_count;
+    a.n_list = r->n_list, a.listed = r->listed;
     const AttendRowsPlan rp = tq_attend_rows_plan(a, n);
     p.ns_cold = rp.ns_cold, p.ns_hot = rp.ns_hot, p.hot_cost = rp.hot_cost;
     p.seqs = rp.seqs;
@@ -129,15 +157,17 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
     p.seq_bytes = (size_t)g.n_kv_heads * rows * (p.ns_cold + p.ns_hot) * TQ_PART_STRIDE * 4;
     return p;
   }
-  const int row_tile = rows <= 16 ? 16 : 64;
+  const int row_tile = rows <= 16 || r->listed ? 16 : 64;
   constexpr int cold_size = 64, hot_size = 64;
   // tokens in blocks that the rows of a tile can see
   const int64_t in_blocks = (int64_t)nb * g.block_tokens;
-  const int64_t seen = r->window == 0 ? in_blocks
-                                      : std::min<int64_t>(in_blocks, (int64_t)r->window + row_tile / g.group + r->sinks + cold_size);
+  const int64_t seen = r->listed         ? std::min<int64_t>(in_blocks, (int64_t)r->n_list * g.block_tokens)
+                       : r->window == 0 ? in_blocks
+                                        : std::min<int64_t>(in_blocks, (int64_t)r->window + row_tile / g.group + r->sinks + cold_size);
   const int64_t cold = (seen + cold_size - 1) / cold_size;
   const int64_t hot = (std::min<int64_t>(g.hot_window, n) + hot_size - 1) / hot_size;
-  const int64_t ctas = std::max<int64_t>((int64_t)r->seq_count * g.n_kv_heads * ((rows + row_tile - 1) / row_tile), 1);
+  const int64_t tiles = r->listed ? r->n_tokens : (rows + row_tile - 1) / row_tile;
+  const int64_t ctas = std::max<int64_t>((int64_t)r->seq_count * g.n_kv_heads * tiles, 1);
   const int64_t want = std::min<int64_t>(std::max<int64_t>((4 * sm_count + ctas - 1) / ctas, 1), 64);
   const int64_t each = (std::max<int64_t>(cold + hot, 1) + want - 1) / want;
   p.ns_cold = (int)((cold + each - 1) / each);
@@ -151,7 +181,7 @@ Plan make_plan(const tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st) {
 size_t least_bytes(const Plan& p) { return p.fixed_bytes + p.seq_bytes; }
 
 // The sequences of `r` by a plan that its workspace has room for, as many at once as it has.
-int run(tq_ctx* ctx, const tq_attend_args* r, const Plan& p, cudaStream_t st) {
+int run(tq_ctx* ctx, const Call* r, const Plan& p, cudaStream_t st) {
   const tq_geom& g = ctx->g;
   const int at_once =
       (int)std::min({(r->workspace_bytes - p.fixed_bytes) / p.seq_bytes, (size_t)r->seq_count, (size_t)p.seqs});
@@ -179,13 +209,11 @@ int run(tq_ctx* ctx, const tq_attend_args* r, const Plan& p, cudaStream_t st) {
   a.device = ctx->device, a.sm_count = ctx->sm_count;
   a.wait_limit = ctx->wait_limit, a.withhold = ctx->withhold_tile;
   a.unit_stride = (int64_t)a.rows * (p.ns_cold + p.ns_hot) * TQ_PART_STRIDE;
-  const size_t esz = elem_size(r->q_dtype);
+  a.n_list = r->n_list, a.listed = r->listed;
   for (int s = 0; s < r->seq_count; s += at_once) {
-    a.seq_begin = r->seq_begin + s;
-    a.seq_count = std::min(at_once, r->seq_count - s);
-    a.q = (const uint8_t*)r->q + (int64_t)s * r->q_seq_stride * (int64_t)esz;
-    a.out = (uint8_t*)r->out + (size_t)s * r->n_tokens * g.n_q_heads * TQ_D * esz;
-    a.q_lens = r->q_lens == nullptr ? nullptr : r->q_lens + s;
+    const Call part = part_of(ctx, *r, s, std::min(at_once, r->seq_count - s));
+    a.seq_begin = part.seq_begin, a.seq_count = part.seq_count;
+    a.q = part.q, a.out = part.out, a.q_lens = part.q_lens, a.list = part.list;
     if (p.form == TILES) {
       const int rc = tq_launch_attend_tiles(a, r->workspace, p.cap, p.splits, st);
       if (rc != TQ_OK) return rc;
@@ -207,55 +235,85 @@ int run(tq_ctx* ctx, const tq_attend_args* r, const Plan& p, cudaStream_t st) {
   return TQ_OK;
 }
 
-}  // namespace
-
-extern "C" int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* r, void* stream, size_t* bytes) {
-  const int rc = check_args(ctx, r);
-  if (rc != TQ_OK) return rc;
+int workspace_of(tq_ctx* ctx, const Call& r, void* stream, size_t* bytes) {
   TQ_REQUIRE(bytes != nullptr, TQ_ERR_INVALID, "null argument");
-  const Plan p = make_plan(ctx, r, (cudaStream_t)stream);
+  const Plan p = make_plan(ctx, &r, (cudaStream_t)stream);
   const size_t n = std::max<size_t>(AT_ONE_GO / std::max<size_t>(p.seq_bytes, 1), 1);
-  *bytes = align_up(p.fixed_bytes + std::min({n, (size_t)r->seq_count, (size_t)p.seqs}) * p.seq_bytes, 256);
+  *bytes = align_up(p.fixed_bytes + std::min({n, (size_t)r.seq_count, (size_t)p.seqs}) * p.seq_bytes, 256);
   return TQ_OK;
 }
 
-extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream) {
-  const int rc = check_args(ctx, r);
-  if (rc != TQ_OK) return rc;
-  if (r->seq_count == 0 || r->n_tokens == 0) return TQ_OK;
-  TQ_REQUIRE(r->q != nullptr && r->out != nullptr, TQ_ERR_INVALID, "q and out must be device pointers");
-  TQ_REQUIRE(r->workspace != nullptr && (uintptr_t)r->workspace % 256 == 0, TQ_ERR_INVALID,
+int attend(tq_ctx* ctx, const Call& r, void* stream) {
+  if (r.seq_count == 0 || r.n_tokens == 0) return TQ_OK;
+  TQ_REQUIRE(r.q != nullptr && r.out != nullptr, TQ_ERR_INVALID, "q and out must be device pointers");
+  TQ_REQUIRE(r.workspace != nullptr && (uintptr_t)r.workspace % 256 == 0, TQ_ERR_INVALID,
              "workspace must be a device pointer aligned to 256 bytes");
   TQ_CUDA(cudaSetDevice(ctx->device));
   cudaStream_t st = (cudaStream_t)stream;
-  const Plan all = make_plan(ctx, r, st);
-  if (r->workspace_bytes >= least_bytes(all)) {
+  const Plan all = make_plan(ctx, &r, st);
+  if (r.workspace_bytes >= least_bytes(all)) {
     ctx->last_launches = 0;
-    return run(ctx, r, all, st);
+    return run(ctx, &r, all, st);
   }
   // Even one sequence needs more in the form that suits all of them: half as many, planned by themselves, and so on
   // (another form may suit them).  Looked through before anything is launched.
   for (const bool launch : {false, true}) {
     if (launch) ctx->last_launches = 0;
-    for (int s = 0, n = 0; s < r->seq_count; s += n) {
-      tq_attend_args part = *r;
-      part.seq_begin = r->seq_begin + s;
-      part.q = (const uint8_t*)r->q + (int64_t)s * r->q_seq_stride * (int64_t)elem_size(r->q_dtype);
-      part.out = (uint8_t*)r->out + (size_t)s * r->n_tokens * ctx->g.n_q_heads * TQ_D * elem_size(r->q_dtype);
-      part.q_lens = r->q_lens == nullptr ? nullptr : r->q_lens + s;
-      n = r->seq_count - s;
+    for (int s = 0, n = 0; s < r.seq_count; s += n) {
+      n = r.seq_count - s;
       Plan p;
       for (;;) {
-        part.seq_count = n;
+        const Call part = part_of(ctx, r, s, n);
         p = make_plan(ctx, &part, st);
-        if (r->workspace_bytes >= least_bytes(p)) break;
+        if (r.workspace_bytes >= least_bytes(p)) break;
         TQ_REQUIRE(n > 1, TQ_ERR_CAPACITY, "workspace smaller than tq_attend_workspace asks for one sequence");
         n = (n + 1) / 2;
       }
       if (!launch) continue;
-      const int rc2 = run(ctx, &part, p, st);
-      if (rc2 != TQ_OK) return rc2;
+      const Call part = part_of(ctx, r, s, n);
+      const int rc = run(ctx, &part, p, st);
+      if (rc != TQ_OK) return rc;
     }
   }
   return TQ_OK;
+}
+
+int check_listed(const tq_attend_args* r, const int32_t* blocks, int32_t n_blocks) {
+  TQ_REQUIRE(r->window == 0 && r->sinks == 0, TQ_ERR_INVALID, "listed blocks take the place of a window");
+  TQ_REQUIRE(n_blocks >= 0, TQ_ERR_INVALID, "n_blocks must not be negative");
+  TQ_REQUIRE(blocks != nullptr || n_blocks == 0 || r->seq_count == 0 || r->n_tokens == 0, TQ_ERR_INVALID,
+             "blocks must be a device pointer");
+  return TQ_OK;
+}
+
+Call listed_call(const tq_attend_args* r, const int32_t* blocks, int32_t n_blocks) {
+  Call c = plain_call(r);
+  c.list = blocks, c.n_list = n_blocks, c.listed = true;
+  return c;
+}
+
+}  // namespace
+
+extern "C" int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* r, void* stream, size_t* bytes) {
+  const int rc = check_args(ctx, r);
+  return rc != TQ_OK ? rc : workspace_of(ctx, plain_call(r), stream, bytes);
+}
+
+extern "C" int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* r, void* stream) {
+  const int rc = check_args(ctx, r);
+  return rc != TQ_OK ? rc : attend(ctx, plain_call(r), stream);
+}
+
+extern "C" int32_t tq_attend_blocks_workspace(tq_ctx* ctx, const tq_attend_args* r, int32_t n_blocks, void* stream,
+                                              size_t* bytes) {
+  int rc = check_args(ctx, r);
+  if (rc == TQ_OK) rc = check_listed(r, (const int32_t*)r, n_blocks);  // (pointers are not looked at)
+  return rc != TQ_OK ? rc : workspace_of(ctx, listed_call(r, nullptr, n_blocks), stream, bytes);
+}
+
+extern "C" int32_t tq_attend_blocks(tq_ctx* ctx, const tq_attend_args* r, const int32_t* blocks, int32_t n_blocks,
+                                    void* stream) {
+  int rc = check_args(ctx, r);
+  if (rc == TQ_OK) rc = check_listed(r, blocks, n_blocks);
+  return rc != TQ_OK ? rc : attend(ctx, listed_call(r, blocks, n_blocks), stream);
 }

@@ -43,6 +43,9 @@ struct AttendArgs {
   int32_t ns_cold, ns_hot;
   int32_t rows;  // of a unit: n_tokens * group
   int32_t device, sm_count;
+  // listed: of the blocks a query token sees those on its list alone, [seq_count][n_tokens][n_kv_heads][n_list]
+  const int32_t* list;
+  int32_t n_list, listed;
   int32_t wait_limit, withhold;  // test hook of the form for many rows (tq_debug_wait); 0 and -1 otherwise
 };
 
@@ -86,6 +89,23 @@ TQ_DEV AttendTiles attend_tiles(const AttendArgs& a, int base, int end, int size
   const int sink = min(a.sinks, last + 1) - base;
   t.head = sink > 0 ? min((sink + size - 1) / size, t.first) : 0;
   return t;
+}
+
+// ---- attention of listed blocks: every query token and KV head has a list of its own
+TQ_DEV const int32_t* attend_list(const AttendArgs& a, int s, int i, int head) {
+  return a.list + (((size_t)s * a.n_tokens + i) * a.g.n_kv_heads + head) * a.n_list;
+}
+// Entries of a list that count: a list ends at the first one that is not above the one before, or no block of the sequence
+// (by a whole warp).
+TQ_DEV int attend_listed(const AttendArgs& a, const int32_t* list, int blocks) {
+  const int lane = threadIdx.x & 31;
+  for (int k0 = 0; k0 < a.n_list; k0 += 32) {
+    const int k = k0 + lane;
+    const int v = k < a.n_list ? list[k] : -1, before = k > 0 && k < a.n_list ? list[k - 1] : -1;
+    const uint32_t in = __ballot_sync(0xffffffffu, v > before && v < blocks);
+    if (in != 0xffffffffu) return k0 + __ffs(~in) - 1;
+  }
+  return a.n_list;
 }
 
 TQ_DEV float* attend_partial(const AttendArgs& a, int unit, int row, int split) {

@@ -104,8 +104,9 @@ TQ_DEV void ag_group(const uint8_t* grp, int bits, int lane, const float* cent, 
   }
 }
 
-// A tile of rows and a split of its tokens.
-template <int RPT>
+// A tile of rows and a split of its tokens.  LIST: the rows are those of one query token, and what is counted through in tiles
+// of 64 are the tokens of the blocks on its list, one block after the other.
+template <int RPT, bool LIST>
 TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>& sh) {
   constexpr int RT = 16 * RPT;
   const tq_geom& g = a.g;
@@ -114,7 +115,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
   const int split = item % ns, rt = item / ns % row_tiles, unit = item / ns / row_tiles;
   if (a.left != nullptr && a.left[unit] == 0) return;
   const int H = g.n_kv_heads, G = g.group, S = g.block_tokens, vb = g.value_bits;
-  const int s = unit / H, head = unit % H, row0 = rt * RT;
+  const int s = unit / H, head = unit % H, row0 = rt * (LIST ? G : RT), rows = LIST ? row0 + G : a.rows;
   const AttendSeq sq = attend_seq(a, s);
   const bool polar = g.key_mode == TQ_KEYS_POLAR, is_cold = split < a.ns_cold;
   const size_t uix = unit_index(g, a.layer, a.seq_begin + s, head);
@@ -127,7 +128,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
   for (int i = tid; i < RT * TQ_D; i += AG_THREADS) {
     const int r = i / TQ_D, d = i % TQ_D, row = row0 + r;
     float x = 0.0f;
-    if (row < a.rows)
+    if (row < rows)
       x = attend_ld(a.q, (size_t)((int64_t)s * a.q_seq + (int64_t)(row / G) * a.q_tok +
                                   (int64_t)(head * G + row % G) * a.q_head + d), a.q_dtype);
     sh.q[r][d] = tq_scaled<true>(x);
@@ -152,10 +153,14 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
   }
 
   // ---- the token tiles of this split
-  const int i_lo = row0 / G, i_hi = min(min(row0 + RT, a.rows) - 1, sq.q_n * G - 1) / G;
+  const int i_lo = row0 / G, i_hi = min(min(row0 + RT, rows) - 1, sq.q_n * G - 1) / G;
   const int p_lo = sq.first + i_lo, p_hi = i_lo < sq.q_n ? sq.first + i_hi : -1;
-  const int base = is_cold ? 0 : sq.cold, end = is_cold ? sq.cold : sq.n;
-  const AttendTiles tl = attend_tiles(a, base, end, AG_T, p_lo, p_hi);
+  const bool listed = LIST && is_cold;
+  const int32_t* const list = listed ? attend_list(a, s, rt, head) : nullptr;
+  const int base = is_cold ? 0 : sq.cold;
+  const int end = listed ? (p_hi < 0 ? 0 : attend_listed(a, list, sq.cold / S) * S) : is_cold ? sq.cold : sq.n;
+  const AttendTiles tl = listed ? AttendTiles{0, 0, (end + AG_T - 1) / AG_T} : attend_tiles(a, base, end, AG_T, p_lo, p_hi);
+  auto block_of = [&](int b) { return listed ? list[b] : b; };
   const int part = is_cold ? split : split - a.ns_cold, parts = is_cold ? a.ns_cold : a.ns_hot;
   const int k_lo = (int)((long)tl.count() * part / parts), k_hi = (int)((long)tl.count() * (part + 1) / parts);
 
@@ -164,7 +169,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
 #pragma unroll
   for (int r = 0; r < RPT; ++r) {
     const int row = row0 + ty * RPT + r;
-    pos[r] = row < a.rows ? attend_position(a, sq, row) : -1;
+    pos[r] = row < rows ? attend_position(a, sq, row) : -1;
     win[r] = attend_window(a, pos[r]);
     m[r] = -INFINITY;
     l[r] = 0.0f;
@@ -190,7 +195,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
         odd |= !ag_row(a.hot_v, at, g.kv_dtype, vr);
       } else {
         const int b = t / S, slot = t - b * S;
-        const uint8_t* page = a.pages + page_offset(g, a.layer, a.seq_begin + s, head, b);
+        const uint8_t* page = a.pages + page_offset(g, a.layer, a.seq_begin + s, head, block_of(b));
         if (polar) {
           ag_codes(page, vb, slot, d0, sh.cent, ((const float*)(page + g.scale_off))[slot], kr);
         } else {
@@ -216,7 +221,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
     if (is_cold && S % TQ_GROUP_TOK == 0 && warp < AG_T / TQ_GROUP_TOK) {
       const int t = t0 + warp * TQ_GROUP_TOK, b = t / S, slot = t - b * S;
       if (t < t1) {  // (blocks are whole groups, and so is what is in blocks)
-        const uint8_t* page = a.pages + page_offset(g, a.layer, a.seq_begin + s, head, b);
+        const uint8_t* page = a.pages + page_offset(g, a.layer, a.seq_begin + s, head, block_of(b));
         ag_group(page + g.v_off + (size_t)(slot >> 4) * v_group_bytes(vb), vb, lane, sh.cent,
                  (const float*)(page + g.norm_off) + slot, &sh.v[warp * TQ_GROUP_TOK]);
       }
@@ -227,7 +232,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
       // depend on one another)
       const bool many = S < AG_T;
       for (int b = t0 / S + (many ? warp : 0); b * S < t1; b += many ? AG_THREADS / 32 : 1) {
-        const PageMeta pm = a.page_meta[uix * g.max_blocks + b];
+        const PageMeta pm = a.page_meta[uix * g.max_blocks + block_of(b)];
         const size_t slab = uix * (size_t)g.pool_entries + pm.off;
         for (uint32_t e = many ? lane : tid; e < pm.cnt; e += many ? 32 : AG_THREADS) {
           const uint32_t w = a.pool_dec[slab + e];
@@ -273,14 +278,19 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
         for (int j = 0; j < 4; ++j) x[r][j] += y[r][j];
     }
     __syncthreads();  // (the keys have been read)
+    int at[4];  // tokens of the sequence
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int t = t0 + tx + 16 * j;
+      at[j] = t < t1 ? (listed ? list[t / S] * S + t % S : t) : INT_MAX;
+    }
 #pragma unroll
     for (int r = 0; r < RPT; ++r) {
       bool sees[4];
       float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int t = t0 + tx + 16 * j;
-        sees[j] = t < t1 && t <= pos[r] && (t >= win[r] || t < a.sinks);
+        sees[j] = at[j] <= pos[r] && (at[j] >= win[r] || at[j] < a.sinks);
         if (sees[j]) top = fmaxf(top, x[r][j]);
       }
 #pragma unroll
@@ -340,7 +350,7 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
     const int row = row0 + ty * RPT + r;
 #pragma unroll
     for (int d = 8; d >= 1; d >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
-    if (row >= a.rows) continue;
+    if (row >= rows) continue;
     float* to = attend_partial(a, unit, row, split);
     if (tx == 0) *(float2*)to = make_float2(m[r], l[r]);
 #pragma unroll
@@ -349,10 +359,10 @@ TQ_DEV void ag_item(const AttendArgs& a, int row_tiles, int item, AgShared<RPT>&
   }
 }
 
-template <int RPT>
+template <int RPT, bool LIST>
 __global__ void __launch_bounds__(AG_THREADS, 2) attend_general_kernel(AttendArgs a, int row_tiles) {
   extern __shared__ __align__(16) uint8_t ag_smem[];
-  ag_item(a, row_tiles, (int)blockIdx.x, *(AgShared<RPT>*)ag_smem);
+  ag_item<RPT, LIST>(a, row_tiles, (int)blockIdx.x, *(AgShared<RPT>*)ag_smem);
 }
 // Only the (sequence, KV head) units that the form for many rows has left: hardly ever one, so that a CTA per SM looks
 // through the flags first (a CTA per item, that finds its own unset, took 7.5 us for 2048 tokens of 8 KV heads).
@@ -363,7 +373,7 @@ __global__ void __launch_bounds__(AG_THREADS) attend_left_kernel(AttendArgs a, i
   for (int i = threadIdx.x; i < a.seq_count * a.g.n_kv_heads; i += AG_THREADS) any |= a.left[i] != 0;
   if (!__syncthreads_or(any)) return;
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    ag_item(a, row_tiles, (int)item, *(AgShared<RPT>*)ag_smem);
+    ag_item<RPT, false>(a, row_tiles, (int)item, *(AgShared<RPT>*)ag_smem);
     __syncthreads();
   }
 }
@@ -408,9 +418,10 @@ __global__ void __launch_bounds__(TQ_D) attend_combine_kernel(AttendArgs a) {
   else ((__nv_bfloat16*)a.out)[at] = __float2bfloat16_rn(x);
 }
 
-template <int RPT>
+template <int RPT, bool LIST = false>
 int launch_general(const AttendArgs& a, cudaStream_t st) {
-  const int row_tiles = (a.rows + 16 * RPT - 1) / (16 * RPT);
+  static_assert(!LIST || 16 * RPT >= TQ_MAX_G, "a query token's rows in one tile");
+  const int row_tiles = LIST ? a.n_tokens : (a.rows + 16 * RPT - 1) / (16 * RPT);
   const int64_t grid = (int64_t)a.seq_count * a.g.n_kv_heads * row_tiles * (a.ns_cold + a.ns_hot);
   TQ_REQUIRE(grid <= INT_MAX, TQ_ERR_UNSUPPORTED, "too many (sequence, head, query row) tiles in a call");
   static bool done[64], left_done[64];
@@ -422,9 +433,9 @@ int launch_general(const AttendArgs& a, cudaStream_t st) {
     TQ_CUDA(cudaGetLastError());
     return TQ_OK;
   }
-  const int rc = attend_shared(attend_general_kernel<RPT>, sizeof(AgShared<RPT>), a.device, done);
+  const int rc = attend_shared(attend_general_kernel<RPT, LIST>, sizeof(AgShared<RPT>), a.device, done);
   if (rc != TQ_OK) return rc;
-  attend_general_kernel<RPT><<<(int)grid, AG_THREADS, sizeof(AgShared<RPT>), st>>>(a, row_tiles);
+  attend_general_kernel<RPT, LIST><<<(int)grid, AG_THREADS, sizeof(AgShared<RPT>), st>>>(a, row_tiles);
   TQ_CUDA(cudaGetLastError());
   return TQ_OK;
 }
@@ -434,6 +445,7 @@ int launch_general(const AttendArgs& a, cudaStream_t st) {
 // Tiles of 16 rows, or of 64 with a fourth of the loads per product: 4 to 16 rows 54 to 56 us against 69 to 71 (4000
 // float32 tokens, 8 KV heads), 32 rows 94 against 73, 64 rows 160 against 77.
 int tq_launch_attend_general(const AttendArgs& a, cudaStream_t st) {
+  if (a.listed) return launch_general<1, true>(a, st);
   return a.rows <= 16 ? launch_general<1>(a, st) : launch_general<4>(a, st);
 }
 

@@ -211,16 +211,23 @@ struct ArWork {
   TQ_DEV int items() const { return strip.count() + hot.count(); }
   TQ_DEV int cost(int of_strip, int of_hot) const { return of_strip * strip.count() + of_hot * hot.count(); }
 };
+// LIST: as many strips as a list can have, whether it has them or not, for every query token and head alike.
+template <bool LIST>
 TQ_DEV ArWork ar_work(const AttendArgs& a, int n, int q_n) {
   ArWork w;
   w.cold = n_cold_blocks(n, a.g.hot_window, AR_S) * AR_S;
   const int p_lo = n - q_n, p_hi = q_n > 0 ? n - 1 : -1;
-  w.strip = attend_tiles(a, 0, w.cold, AR_STRIP, p_lo, p_hi);
+  w.strip = LIST ? AttendTiles{0, 0, p_hi >= 0 ? min(a.n_list, w.cold / AR_S) * (AR_S / AR_STRIP) : 0}
+                 : attend_tiles(a, 0, w.cold, AR_STRIP, p_lo, p_hi);
   w.hot = attend_tiles(a, w.cold, n, AR_HOT, p_lo, p_hi);
   return w;
 }
 // row tiles of a sequence that have query tokens
-TQ_DEV int ar_tiles(const AttendArgs& a, int q_n, int n) { return (q_n * a.g.group + n - 1) / n; }
+// (LIST: a tile has rows of one query token alone)
+template <bool LIST>
+TQ_DEV int ar_tiles(const AttendArgs& a, int q_n, int n) {
+  return LIST ? q_n * ((a.g.group + n - 1) / n) : (q_n * a.g.group + n - 1) / n;
+}
 
 // How a launch divides its work; the first CTA leaves it for the merge.
 struct ArPlan {
@@ -229,7 +236,7 @@ struct ArPlan {
   int4 seq[AR_SEQS];  // strips, window tiles and row tiles of a sequence
 };
 
-template <bool SPLIT, int VB>
+template <bool SPLIT, int VB, bool LIST>
 __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows_kernel(AttendArgs a) {
   using Sh = ArShape<SPLIT, VB>;
   constexpr int N = Sh::N, WARPS = Sh::WARPS, THREADS = 32 * WARPS, COST = ar_cost(SPLIT);
@@ -259,8 +266,8 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
       if (s < a.seq_count) {
         const AttendSeq sq = attend_seq(a, s);
         sh.seq[s] = make_int2(sq.n, sq.q_n);
-        const ArWork w = ar_work(a, sq.n, sq.q_n);
-        cost[i] = (int64_t)w.cost(COST, a.hot_cost) * (H * ar_tiles(a, sq.q_n, N));
+        const ArWork w = ar_work<LIST>(a, sq.n, sq.q_n);
+        cost[i] = (int64_t)w.cost(COST, a.hot_cost) * (H * ar_tiles<LIST>(a, sq.q_n, N));
         most_strip = max(most_strip, w.strip.count());
         most_hot = max(most_hot, w.hot.count());
       }
@@ -297,8 +304,8 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
     if (tid == 0) plan->share = share;
     for (int i = tid; i <= AR_SEQS; i += THREADS) plan->cum[i] = sh.cum[i];
     for (int i = tid; i < a.seq_count; i += THREADS) {
-      const ArWork w = ar_work(a, sh.seq[i].x, sh.seq[i].y);
-      plan->seq[i] = make_int4(w.strip.count(), w.hot.count(), ar_tiles(a, sh.seq[i].y, N), 0);
+      const ArWork w = ar_work<LIST>(a, sh.seq[i].x, sh.seq[i].y);
+      plan->seq[i] = make_int4(w.strip.count(), w.hot.count(), ar_tiles<LIST>(a, sh.seq[i].y, N), 0);
     }
   }
   // (neighbouring shares go to different SMs: where there are few, each has one to itself)
@@ -313,10 +320,10 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   int s = 0, head = 0, rt = 0, it = 0, row_items = 0, row_strips = 0, row_tiles = 1;
   ArWork w;
   auto enter_seq = [&]() {
-    w = ar_work(a, sh.seq[s].x, sh.seq[s].y);
+    w = ar_work<LIST>(a, sh.seq[s].x, sh.seq[s].y);
     row_strips = w.strip.count();
     row_items = w.items();
-    row_tiles = ar_tiles(a, sh.seq[s].y, N);
+    row_tiles = ar_tiles<LIST>(a, sh.seq[s].y, N);
   };
   int64_t begin = 0;  // the cost of what is before this row
   if (more) {
@@ -365,7 +372,10 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   size_t uix = 0;
   uint32_t list_at = 0, list_end = 0;  // SPLIT: the strip's first entry of the page's list, the list's end
   const uint8_t* page = nullptr;
-  auto page_of = [&](int i) { return a.pages + (uix * g.max_blocks + (w.strip.at(i) >> 2)) * (size_t)g.page_bytes; };
+  const int32_t* list = nullptr;  // LIST: the row tile's blocks
+  int row_valid = 0;              // and strips of these
+  auto strip_at = [&](int i) { return LIST ? 4 * list[i >> 2] + (i & 3) : w.strip.at(i); };
+  auto page_of = [&](int i) { return a.pages + (uix * g.max_blocks + (strip_at(i) >> 2)) * (size_t)g.page_bytes; };
   auto copy_keys = [&](const uint8_t* from, int t0, uint32_t first) {  // t0: of the strip in its page
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -403,7 +413,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   // SPLIT: the list of the page of item i, and its first entry of token t0 or a later one
   auto open_list = [&](int i, int t0) {
     if (!SPLIT || g.outlier_k == 0) return;
-    const PageMeta pm = a.page_meta[uix * g.max_blocks + (w.strip.at(i) >> 2)];
+    const PageMeta pm = a.page_meta[uix * g.max_blocks + (strip_at(i) >> 2)];
     list_end = pm.off + pm.cnt;
     uint32_t lo = pm.off, hi = list_end;
     const uint32_t* dec = a.pool_dec + uix * (size_t)g.pool_entries;
@@ -420,6 +430,8 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   float acc[NT][8][4], m_run[NT][2], l_run[NT][2];
   int pos[NT][2], win[NT][2];
   int first_pos = 0, last_win = 0, p_lo = 0, p_hi = 0, row0 = 0;
+  int token_end = 0;  // LIST: the row behind those of the tile's query token
+  auto rows_end = [&]() { return LIST ? token_end : a.rows; };
   auto reset = [&]() {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -442,12 +454,18 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   auto fetch_row = [&]() {
     uix = unit_index(g, a.layer, a.seq_begin + s, head);
     row0 = rt * N;
+    if (LIST) {
+      const int per = (G + N - 1) / N, token = rt / per;
+      row0 = token * G + (rt - token * per) * N, token_end = (token + 1) * G;
+      list = attend_list(a, s, token, head);
+      row_valid = (AR_S / AR_STRIP) * attend_listed(a, list, w.cold / AR_S);
+    }
     int i = row0 / G, k = row0 - i * G;  // query token and head of the group
     const int64_t from = (int64_t)s * a.q_seq + (int64_t)(head * G) * a.q_head + 4 * lane;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int64_t e = from + (int64_t)i * a.q_tok + (int64_t)k * a.q_head;
-      const bool there = row0 + n < a.rows;
+      const bool there = row0 + n < rows_end();
       if (SPLIT && q32) q_raw[n] = there ? *(const float4*)((const float*)a.q + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       else q_half[n] = there ? *(const uint2*)((const uint16_t*)a.q + e) : make_uint2(0u, 0u);
       if (++k == G) k = 0, ++i;
@@ -455,11 +473,11 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   };
   auto start_row = [&]() {
     const int n = sh.seq[s].x, q_n = sh.seq[s].y, first = n - q_n;
-    const int last = min(min(row0 + N, a.rows), q_n * G) - 1;
+    const int last = min(min(row0 + N, rows_end()), q_n * G) - 1;
     p_lo = first + row0 / G;
     p_hi = last >= row0 ? first + last / G : -1;
     // whether tokens are seen by all rows of the tile goes by its earliest row and its latest window
-    first_pos = min(row0 + N, a.rows) - 1 <= last ? p_lo : -1;
+    first_pos = min(row0 + N, rows_end()) - 1 <= last ? p_lo : -1;
     last_win = attend_window(a, max(p_hi, 0));
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -1093,7 +1111,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
 #pragma unroll
         for (int o = 4; o <= 16; o <<= 1) l_run[t][x] += __shfl_xor_sync(0xffffffffu, l_run[t][x], o);
         const int row = row0 + 8 * t + 2 * c + x;
-        if (row >= a.rows) continue;
+        if (row >= rows_end()) continue;
         float* to = attend_partial(a, s * H + head, row, slot);
         if (r == 0) *(float2*)to = make_float2(m_run[t][x], l_run[t][x]);
 #pragma unroll
@@ -1106,7 +1124,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   // ---- the share, item by item
   int strip = 0, ts = 0;  // a strip of the row, its first token in its page
   auto open_strips = [&]() {
-    strip = w.strip.at(it), ts = (strip & 3) * AR_STRIP;
+    strip = strip_at(it), ts = (strip & 3) * AR_STRIP;
     page = page_of(it);
     open_list(it, ts);
     copy_keys(page, ts, list_at);
@@ -1116,7 +1134,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   };
   if (more) {  // (on their way while the tables are made)
     fetch_row();
-    if (it < row_strips) open_strips();
+    if (it < (LIST ? row_valid : row_strips)) open_strips();
   }
   {  // tables of pairs
     float max_k = 0.0f, max_v = 0.0f;
@@ -1148,18 +1166,18 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
     // a row tile's strips, then its tiles of the window, as far as the share goes
     if (!opened) {
       fetch_row();
-      if (it < row_strips) open_strips();
+      if (it < (LIST ? row_valid : row_strips)) open_strips();
     }
     opened = false;
     start_row();
     if (it < row_strips) {
       reset();
       bool new_page = true;
-      for (;;) {
+      while (!LIST || it < row_valid) {
         at += COST;
         const int i1 = it + 1;
-        const bool last = i1 >= row_strips || at >= stop;
-        const int next = last ? strip : w.strip.at(i1);
+        const bool last = i1 >= (LIST ? row_valid : row_strips) || at >= stop;
+        const int next = last ? strip : strip_at(i1);
         asm volatile("cp.async.wait_group 1;" ::: "memory");  // the key half has landed
         __syncwarp();
         if (new_page) weights();
@@ -1208,6 +1226,10 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
+      if (LIST && it < row_strips && at < stop) {  // (what the list does not have)
+        const int64_t left = min((stop - at + COST - 1) / COST, (int64_t)(row_strips - it));
+        it += (int)left, at += COST * left;
+      }
       flush(false);
       more = at < stop;
     }
@@ -1263,8 +1285,9 @@ __global__ void __launch_bounds__(AC_THREADS, 2) attend_rows_combine_kernel(Atte
       s = unit / H, head = unit - s * H;
       const int4 seq = plan->seq[s];
       const int64_t before = plan->cum[s];
-      if (row / tile < seq.z) {
-        const int64_t begin = before + (int64_t)(head * seq.z + row / tile) * (cost * seq.x + a.hot_cost * seq.y);
+      const int rt = a.listed ? row / G * ((G + tile - 1) / tile) + row % G / tile : row / tile;
+      if (rt < seq.z) {
+        const int64_t begin = before + (int64_t)(head * seq.z + rt) * (cost * seq.x + a.hot_cost * seq.y);
         const int64_t middle = begin + cost * seq.x;
         const int nc = seq.x > 0 ? (int)(ar_div(middle - cost, share) - ar_div(begin, share)) + 1 : 0;
         const int nh = seq.y > 0 ? (int)(ar_div(middle + a.hot_cost * (seq.y - 1), share) - ar_div(middle, share)) + 1 : 0;
@@ -1342,16 +1365,16 @@ __global__ void __launch_bounds__(AC_THREADS, 2) attend_rows_combine_kernel(Atte
   }
 }
 
-template <bool SPLIT, int VB>
+template <bool SPLIT, int VB, bool LIST>
 int launch_rows(const AttendArgs& a, cudaStream_t st) {
   using Shared = ArShared<SPLIT, VB>;
   static_assert(sizeof(Shared) <= 227 * 1024, "shared memory of one CTA");
   const int64_t all = (int64_t)a.seq_count * a.g.n_kv_heads * a.rows;
   TQ_REQUIRE(all <= INT_MAX - 4 * AC_THREADS, TQ_ERR_UNSUPPORTED, "too many query rows in a call");
   static bool done[64];
-  const int rc = attend_shared(attend_rows_kernel<SPLIT, VB>, sizeof(Shared), a.device, done);
+  const int rc = attend_shared(attend_rows_kernel<SPLIT, VB, LIST>, sizeof(Shared), a.device, done);
   if (rc != TQ_OK) return rc;
-  attend_rows_kernel<SPLIT, VB><<<a.sm_count, 32 * ArShape<SPLIT, VB>::WARPS, sizeof(Shared), st>>>(a);
+  attend_rows_kernel<SPLIT, VB, LIST><<<a.sm_count, 32 * ArShape<SPLIT, VB>::WARPS, sizeof(Shared), st>>>(a);
   TQ_CUDA(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr = {};
@@ -1382,16 +1405,18 @@ AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens) {
   // half as long, and a few more (the kernel makes the shares larger where they would not do).
   const int64_t in_blocks = (int64_t)n_cold_blocks(tokens, g.hot_window, AR_S) * AR_S;
   const int64_t seen = a.window == INT_MAX ? in_blocks : std::min<int64_t>(in_blocks, (int64_t)a.window + a.n_tokens + 128);
-  const int64_t strips = (seen + AR_STRIP - 1) / AR_STRIP + (std::min<int64_t>(a.sinks, in_blocks) + AR_STRIP - 1) / AR_STRIP;
+  const int64_t strips = a.listed ? std::min<int64_t>(a.n_list, in_blocks / AR_S) * (AR_S / AR_STRIP)
+                                  : (seen + AR_STRIP - 1) / AR_STRIP + (std::min<int64_t>(a.sinks, in_blocks) + AR_STRIP - 1) / AR_STRIP;
   const int64_t hot = (std::min(tokens, g.hot_window) + AR_HOT - 1) / AR_HOT;
-  const int64_t rows = (int64_t)std::min(a.seq_count, AR_SEQS) * g.n_kv_heads * ((a.rows + 8 * NT - 1) / (8 * NT));
+  const int64_t tiles = a.listed ? (int64_t)a.n_tokens * ((g.group + 8 * NT - 1) / (8 * NT)) : (a.rows + 8 * NT - 1) / (8 * NT);
+  const int64_t rows = (int64_t)std::min(a.seq_count, AR_SEQS) * g.n_kv_heads * tiles;
   const int64_t workers = (int64_t)a.sm_count * (a.q_dtype == TQ_BF16 ? ArShape<false, 3>::WARPS : ArShape<true, 3>::WARPS);
   const int cost = ar_cost(a.q_dtype != TQ_BF16);
   int hot_cost = ar_hot_cost(a.q_dtype, g.kv_dtype);
   if (hot_cost > HALF_HOT) {  // (by what the longest sequence's rows see, as ar_work has it)
     const int64_t room = workers * cost;
     const int64_t w = a.window == INT_MAX ? 0 : std::max<int64_t>((int64_t)tokens - a.n_tokens - a.window + 1, 0), first = w / AR_STRIP;
-    const int64_t n_strips = std::max<int64_t>(in_blocks / AR_STRIP - first, 0) +
+    const int64_t n_strips = a.listed ? strips : std::max<int64_t>(in_blocks / AR_STRIP - first, 0) +
                              std::min<int64_t>((std::min<int64_t>(a.sinks, in_blocks) + AR_STRIP - 1) / AR_STRIP, first);
     const int64_t n_hot = (tokens - in_blocks + AR_HOT - 1) / AR_HOT - std::max<int64_t>(w - in_blocks, 0) / AR_HOT;
     if (rows * (cost * n_strips + hot_cost * n_hot) > room && rows * (cost * n_strips + HALF_HOT * n_hot) <= room) hot_cost = HALF_HOT;
@@ -1403,7 +1428,12 @@ AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens) {
   return p;
 }
 
+template <bool LIST>
+static int launch_form(const AttendArgs& a, cudaStream_t st) {
+  if (a.q_dtype == TQ_BF16) return a.g.value_bits == 4 ? launch_rows<false, 4, LIST>(a, st) : launch_rows<false, 3, LIST>(a, st);
+  return a.g.value_bits == 4 ? launch_rows<true, 4, LIST>(a, st) : launch_rows<true, 3, LIST>(a, st);
+}
+
 int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st) {
-  if (a.q_dtype == TQ_BF16) return a.g.value_bits == 4 ? launch_rows<false, 4>(a, st) : launch_rows<false, 3>(a, st);
-  return a.g.value_bits == 4 ? launch_rows<true, 4>(a, st) : launch_rows<true, 3>(a, st);
+  return a.listed ? launch_form<true>(a, st) : launch_form<false>(a, st);
 }
