@@ -206,6 +206,14 @@ typedef struct tq_attend_args {
 int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* args, void* stream, size_t* bytes);
 int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* args, void* stream);
 
+/* tq_attend for sequences that go on from a shared beginning: the tokens of sequence `prefix` of the layer, none of the
+ * call's own, stand before those of each of them and are seen by all of their query tokens (the newest n of each
+ * sequence's own tokens, as in tq_attend; rows that have no token of their sequence stay zeros).  They are read once for all
+ * sequences.  `window` and `sinks` must be 0; with several sequences of several tokens q_seq_stride must be n_tokens *
+ * q_tok_stride.  Positions for the rotation: tq_ctx_norm_rope_after. */
+int32_t tq_attend_prefix_workspace(tq_ctx* ctx, const tq_attend_args* args, int32_t prefix, void* stream, size_t* bytes);
+int32_t tq_attend_prefix(tq_ctx* ctx, const tq_attend_args* args, int32_t prefix, void* stream);
+
 /* The blocks of a sequence that are worth attending for a query token, per KV head, by a cheap score: the sum over the
  * group's query heads of the largest q . k that the block's grid allows, outliers aside - a key's channel lies between
  * mean + lo * scale and mean + hi * scale (NF4: -1 and 1, uniform: 0 and 15).  Query token i of sequence s stands at a

@@ -1,0 +1,298 @@
+"""KVContext.attend with a shared beginning against attention in 64 bits over the dequantised keys and values of the prefix and of
+each sequence, with the data and the limits of attend_oracle."""
+
+from __future__ import annotations
+
+import pytest
+
+import attend_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+
+    if not torch.cuda.is_available():
+        pytest.fail("CUDA device required for -m gpu tests")
+    return torch
+
+
+def _ctx(**kw):
+    from turboquant_pro_b200 import KVContext
+
+    return KVContext(**{"n_layers": 1, "seed": 3, "max_tokens_per_seq": 4096, **kw})
+
+
+def _fill(torch, ctx, lens, gen, layer=0):
+    h, s = ctx.n_kv_heads, ctx.block_tokens
+    for seq, n in enumerate(lens):
+        if n:
+            cold = ctx.cold_blocks(n) * s
+            # tokens at what a tile of a kernel may begin or end with
+            borders = {0, n - 1, cold - 1, cold} | {c * b + d for c in (64, 80, 128, 256) for b in range(0, n // c + 1, 5) for d in (-1, 0)}
+            k = torch.randn(1, n, h, 128, generator=gen, device="cuda")
+            v = oracle.values(n, h, gen, "cuda", borders)
+            ctx.append(layer, k.to(ctx.kv_dtype), v[None].to(ctx.kv_dtype), seq_begin=seq)
+
+
+def _check(torch, ctx, got, q, prefix, q_lens=None, seq_begin=0, layer=0):
+    assert got.shape == q.shape and got.dtype == q.dtype
+    m = ctx.lengths(layer, prefix)[0]
+    pk, pv = ctx.dequant(layer, prefix, 0, m)
+    t = q.shape[1]
+    for s in range(q.shape[0]):
+        q_n = t if q_lens is None else min(max(int(q_lens[s]), 0), t)
+        n = ctx.lengths(layer, seq_begin + s)[0]
+        k, v = ctx.dequant(layer, seq_begin + s, 0, n)
+        k, v = torch.cat((pk, k), 1), torch.cat((pv, v), 1)
+        # (rows before a sequence's first token see nothing)
+        skip = max(q_n - n, 0)
+        assert not bool(got[s, :skip].any()) and not bool(got[s, q_n:].any())
+        if q_n > skip:
+            want = oracle.attention(k, v, q[s, skip:q_n], q_n - skip, None, 0)
+            oracle.check(got[s, skip:q_n], want)
+
+
+CASES = [
+    # lens of the sequences, prefix, T, Hkv, Hq, kv dtype, q dtype, hot, keys, value bits
+    ([100, 700], 2000, 1, 2, 8, "bfloat16", "bfloat16", 512, "nf4_asym", 3),
+    ([5, 1, 600, 1200, 33], 1300, 1, 2, 2, "float16", "float16", 512, "nf4_asym", 4),
+    ([900] * 40, 3000, 1, 1, 8, "bfloat16", "bfloat16", 512, "uniform", 3),
+    ([20] * 33, 4000, 1, 2, 8, "bfloat16", "bfloat16", 512, "nf4_asym", 4),
+    ([3, 800], 513, 5, 1, 7, "bfloat16", "float16", 512, "nf4", 3),
+    ([1500, 40], 777, 130, 2, 4, "float16", "bfloat16", 512, "nf4_asym", 3),
+    ([700] * 5, 2500, 2, 1, 16, "float32", "float32", 512, "nf4_asym", 4),
+    ([90], 500, 1, 1, 4, "bfloat16", "bfloat16", 512, "nf4_asym", 3),     # a prefix without blocks
+    ([90, 4], 1, 1, 1, 4, "bfloat16", "bfloat16", 512, "nf4_asym", 3),
+    ([300, 20], 1000, 3, 2, 6, "bfloat16", "bfloat16", 33, "nf4_asym", 3),
+    ([300] * 20, 900, 4, 1, 4, "float16", "float16", 100, "uniform", 4),
+    ([200, 700], 900, 2, 1, 4, "float32", "float32", 128, "polar", 4),
+    ([700, 3], 900, 1, 2, 4, "bfloat16", "bfloat16", 512, "polar", 3),
+    ([60] * 70, 1800, 1, 1, 2, "bfloat16", "float32", 512, "nf4_asym", 3),
+    ([600] * 3, 1111, 300, 1, 2, "bfloat16", "bfloat16", 512, "nf4_asym", 3),
+]
+
+
+def _build(torch, case, seed):
+    lens, prefix, t, h, hq, kv, qd, hot, keys, vb = case
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    ctx = _ctx(n_seqs=len(lens) + 1, n_kv_heads=h, n_q_heads=hq, kv_dtype=kv, hot_window=hot, key_mode=keys,
+               value_bits=vb, key_bits=vb if keys == "polar" else 4, outlier_frac=0.0 if keys == "polar" else 0.02)
+    _fill(torch, ctx, [prefix] + lens, gen)
+    q = torch.randn(len(lens), t, hq, 128, generator=gen, device="cuda").to(getattr(torch, qd))
+    return ctx, q, gen
+
+
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_matches_attention_in_64_bits(torch, case):
+    ctx, q, _ = _build(torch, case, 7)
+    b, t = q.shape[:2]
+    got = ctx.attend(0, q, prefix=0, seq_begin=1)
+    _check(torch, ctx, got, q, 0, seq_begin=1)
+    assert torch.equal(got, ctx.attend(0, q, prefix=0, seq_begin=1))
+    part = torch.tensor([(i * 7 + 3) % (t + 1) for i in range(b)], dtype=torch.int32, device="cuda")
+    got = ctx.attend(0, q, prefix=0, seq_begin=1, q_lens=part)
+    _check(torch, ctx, got, q, 0, part, seq_begin=1)
+    assert ctx.status() == 0
+
+
+def test_empty_prefix_and_empty_sequences(torch):
+    for hot in (512, 33):
+        ctx = _ctx(n_seqs=4, n_kv_heads=2, n_q_heads=4, kv_dtype="bfloat16", hot_window=hot)
+        gen = torch.Generator(device="cuda").manual_seed(1)
+        _fill(torch, ctx, [0, 600, 0, 9], gen)
+        q = torch.randn(3, 2, 4, 128, generator=gen, device="cuda").bfloat16()
+        got = ctx.attend(0, q, prefix=0, seq_begin=1)
+        oracle.check(got[0], oracle.attention(*ctx.dequant(0, 1, 0, 600), q[0], 2, None, 0))
+        assert not bool(got[1].any())
+        got = ctx.attend(0, q[:1], prefix=1, seq_begin=0)
+        assert not bool(got.any())
+
+
+def test_padding_that_is_no_number(torch):
+    for case in (CASES[0], CASES[5], CASES[9]):
+        ctx, q, _ = _build(torch, case, 2)
+        t = q.shape[1]
+        part = torch.tensor([t, max(t // 2, 0)], dtype=torch.int32, device="cuda")
+        q[1, int(part[1]):] = float("nan")
+        got = ctx.attend(0, q, prefix=0, seq_begin=1, q_lens=part)
+        _check(torch, ctx, got, torch.nan_to_num(q), 0, part, seq_begin=1)
+
+
+def test_large_and_small_values_in_the_prefix(torch):
+    # beyond what half precision holds, and infinities in the prefix's window: some heads go by the general form
+    for t in (1, 150):
+        gen = torch.Generator(device="cuda").manual_seed(3)
+        ctx = _ctx(n_seqs=3, n_kv_heads=2, n_q_heads=4, kv_dtype="float32", value_bits=3)
+        k, v = (torch.randn(1, 1500, 2, 128, generator=gen, device="cuda") for _ in range(2))
+        k[:, :, 1] *= 1e-3
+        v[:, 700:, 1] *= 1e9
+        ctx.append(0, k, v)
+        for s in (1, 2):
+            x = torch.randn(1, 200, 2, 128, generator=gen, device="cuda")
+            ctx.append(0, x, x, seq_begin=s)
+        q = torch.randn(2, t, 4, 128, generator=gen, device="cuda").bfloat16()
+        _check(torch, ctx, ctx.attend(0, q, prefix=0, seq_begin=1), q, 0, seq_begin=1)
+        w = torch.randn(1, 1, 2, 128, generator=gen, device="cuda")
+        ctx.append(0, w, torch.full_like(w, float("inf")))
+        got = ctx.attend(0, q, prefix=0, seq_begin=1)
+        assert bool(torch.isposinf(got).all())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("hot, keys, prefix, b, t", [(512, "nf4_asym", 2000, 20, 1), (100, "uniform", 1500, 9, 30),
+                                                     (512, "uniform", 2500, 3, 200), (512, "nf4_asym", 300, 2, 120)])
+def test_keys_with_a_large_constant_part(torch, dtype, hot, keys, prefix, b, t):
+    # other constants in the prefix than in each of the sequences: what a form takes off all scores of a part shows
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    ctx = _ctx(n_seqs=b + 1, n_kv_heads=2, n_q_heads=4, kv_dtype="float32" if dtype == "float32" else dtype, hot_window=hot,
+               key_mode=keys)
+    q = torch.randn(b, t, 4, 128, generator=gen, device="cuda").to(getattr(torch, dtype))
+    for s, n in enumerate([prefix] + [t + 130 * i for i in range(b)]):
+        constant = 0.5 * torch.randn(2, 128, generator=gen, device="cuda")
+        k = torch.randn(1, n, 2, 128, generator=gen, device="cuda") + constant
+        v = torch.randn(1, n, 2, 128, generator=gen, device="cuda")
+        ctx.append(0, k.to(ctx.kv_dtype), v.to(ctx.kv_dtype), seq_begin=s)
+    _check(torch, ctx, ctx.attend(0, q, prefix=0, seq_begin=1), q, 0, seq_begin=1)
+
+
+def test_orders_parts_of_the_batch_and_out(torch):
+    for case in (CASES[0], CASES[4], CASES[5], CASES[9]):
+        ctx, q, _ = _build(torch, case, 4)
+        want = ctx.attend(0, q, prefix=0, seq_begin=1)
+        b, t, hq, _ = q.shape
+        heads_first = q.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+        tokens_first = q.transpose(0, 1).contiguous().transpose(0, 1)
+        flat = torch.zeros(q.numel() + 3, dtype=q.dtype, device="cuda")
+        flat[3:] = q.flatten()
+        fused = torch.zeros(b, t, hq + 3, 128, dtype=q.dtype, device="cuda")
+        fused[:, :, 1:hq + 1] = q
+        for x in (heads_first, tokens_first, flat[3:].view(q.shape), fused[:, :, 1:hq + 1]):
+            assert torch.equal(ctx.attend(0, x, prefix=0, seq_begin=1), want)
+        out = torch.full((b + 1, t, hq, 128), 7.0, dtype=q.dtype, device="cuda")
+        ctx.attend(0, q, prefix=0, seq_begin=1, out=out[:b])
+        assert torch.equal(out[:b], want) and bool((out[b] == 7.0).all())
+        _check(torch, ctx, ctx.attend(0, q[1:], prefix=1, seq_begin=2), q[1:], 1, seq_begin=2)
+        _check(torch, ctx, ctx.attend(0, q[:1], prefix=2, seq_begin=0), q[:1], 2, seq_begin=0)
+
+
+def test_captured_calls_follow_the_lengths(torch):
+    for case in (([100, 700, 9], 600, 1, 2, 8, "bfloat16", "bfloat16", 512, "nf4_asym", 3),
+                 ([300] * 12, 600, 5, 1, 8, "bfloat16", "bfloat16", 512, "nf4_asym", 3)):
+        ctx, q, gen = _build(torch, case, 8)
+        ctx.attend(0, q, prefix=0, seq_begin=1)
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.graph(graph, stream=stream):
+            got = ctx.attend(0, q, prefix=0, seq_begin=1)
+        for n in (900, 1):
+            graph.replay()
+            _check(torch, ctx, got, q, 0, seq_begin=1)
+            for s in (0, 2):
+                k = torch.randn(1, n, ctx.n_kv_heads, 128, generator=gen, device="cuda").bfloat16()
+                ctx.append(0, k, oracle.values(n, ctx.n_kv_heads, gen, "cuda")[None].bfloat16(), seq_begin=s)
+        graph.replay()
+        _check(torch, ctx, got, q, 0, seq_begin=1)
+
+
+def test_two_calls_at_once(torch):
+    ctx, q, gen = _build(torch, CASES[3], 6)
+    qs = [q, torch.randn_like(q)]
+    want = [ctx.attend(0, x, prefix=0, seq_begin=1) for x in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for x, stream in zip(qs, streams):
+            with torch.cuda.stream(stream):
+                got.append(ctx.attend(0, x, prefix=0, seq_begin=1))
+    torch.cuda.synchronize()
+    for i, x in enumerate(got):
+        assert torch.equal(x, want[i % 2])
+
+
+def test_refusals(torch):
+    from turboquant_pro_b200._lib import TqError
+
+    ctx = _ctx(n_seqs=4, n_kv_heads=2, n_q_heads=4)
+    q = torch.zeros(2, 3, 4, 128, device="cuda")
+    for bad in (dict(prefix=1), dict(prefix=2), dict(prefix=-1), dict(prefix=4), dict(window=5), dict(sinks=1),
+                dict(blocks=torch.zeros(2, 3, 2, 1, dtype=torch.int32, device="cuda"))):
+        with pytest.raises(ValueError):
+            ctx.attend(**{"layer": 0, "q": q, "prefix": 0, "seq_begin": 1, **bad})
+    with pytest.raises(TypeError):
+        ctx.attend(0, q, prefix=0.5, seq_begin=1)
+    with pytest.raises(TqError, match="workspace"):
+        ctx.attend(0, q, prefix=0, seq_begin=1, max_workspace=1000)
+    assert ctx.attend(0, q[:, :0], prefix=0, seq_begin=1).shape == (2, 0, 4, 128)
+    assert ctx.attend(0, q[:0], prefix=0, seq_begin=1).shape == (0, 3, 4, 128)
+
+
+# ---- a layer's step with all of it ----------------------------------------------------------------------------
+def _freq(torch):
+    import numpy as np
+
+    return torch.tensor(1e6 ** (-np.arange(64) / 64), dtype=torch.float32, device="cuda")
+
+
+def test_a_step_on_a_shared_beginning(torch):
+    from turboquant_pro_b200 import norm_rope
+
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    ctx = _ctx(n_layers=2, n_seqs=4, n_kv_heads=2, n_q_heads=8, kv_dtype="bfloat16")
+    same = _ctx(n_seqs=3, n_kv_heads=2, n_q_heads=8, kv_dtype="bfloat16")
+    f = _freq(torch)
+
+    def tokens(b, t):
+        q, k, v = (torch.randn(b, t, h, 128, generator=gen, device="cuda").bfloat16() for h in (8, 2, 2))
+        return q, k, v
+
+    w = torch.rand(128, generator=gen, device="cuda").add_(0.5).bfloat16()
+    q, k, v = tokens(1, 1200)
+    ctx.step(1, q, k, v, f, q_weight=w, k_weight=w)
+    start = 1200
+    for t in (7, 1, 3):
+        q, k, v = tokens(3, t)
+        got = ctx.step(1, q, k, v, f, q_weight=w, k_weight=w, seq_begin=1, prefix=0)
+        at = start + torch.arange(t, device="cuda")
+        nq, nk = norm_rope(q, k, f, at, q_weight=w, k_weight=w)
+        same.append(0, nk, v)
+        start += t
+        pk, pv = ctx.dequant(1, 0, 0, 1200)
+        n = start - 1200
+        for s in range(3):
+            sk, sv = same.dequant(0, s, 0, n)
+            want = oracle.attention(torch.cat((pk, sk), 1), torch.cat((pv, sv), 1), nq[s], t, None, 0)
+            oracle.check(got[s], want)
+
+
+def test_a_step_on_selected_blocks_with_positions_of_several_axes(torch):
+    from turboquant_pro_b200 import norm_rope
+
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    a, b = (_ctx(n_seqs=2, n_kv_heads=2, n_q_heads=6, kv_dtype="float16") for _ in range(2))
+    f, axes = _freq(torch), torch.tensor([i % 3 for i in range(64)], dtype=torch.uint8, device="cuda")
+    start = 0
+    for t in (1500, 1, 1, 4):
+        q, k, v = (torch.randn(2, t, h, 128, generator=gen, device="cuda").half() for h in (6, 2, 2))
+        pos = start + torch.randint(0, 50, (3, 2, t), generator=gen, device="cuda")
+        got = a.step(0, q, k, v, f, positions=pos, axes=axes, top_blocks=3, first_blocks=1)
+        nq, nk = norm_rope(q, k, f, pos, axes=axes)
+        b.append(0, nk, v)
+        blocks = b.select_blocks(0, nq, 3, first=1)
+        assert torch.equal(got, b.attend(0, nq, blocks=blocks))
+        start += t
+
+
+def test_what_a_step_refuses_is_not_appended(torch):
+    ctx = _ctx(n_seqs=3, n_kv_heads=2, n_q_heads=4, kv_dtype="float16")
+    q, k = (torch.zeros(2, 1, h, 128, device="cuda").half() for h in (4, 2))
+    f = _freq(torch)
+    for bad in (dict(prefix=1), dict(prefix=3), dict(prefix=0, top_blocks=2), dict(prefix=0, window=4),
+                dict(top_blocks=2, sinks=3), dict(top_blocks=0), dict(top_blocks=2, first_blocks=-1),
+                dict(axes=torch.zeros(64, dtype=torch.uint8, device="cuda"))):
+        with pytest.raises(ValueError):
+            ctx.step(0, q, k, k, f, seq_begin=1, **bad)
+    assert [ctx.lengths(0, s)[0] for s in range(3)] == [0, 0, 0]

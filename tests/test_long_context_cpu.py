@@ -51,6 +51,8 @@ def test_null_arguments(lib):
     assert lib.tq_select_blocks(None, C.byref(TqSelectArgs()), None) == -1
     assert lib.tq_attend_blocks(None, C.byref(TqAttendArgs()), None, 1, None) == -1
     assert lib.tq_attend_blocks_workspace(None, C.byref(TqAttendArgs()), 1, None, C.byref(size)) == -1
+    assert lib.tq_attend_prefix(None, C.byref(TqAttendArgs()), 0, None) == -1
+    assert lib.tq_attend_prefix_workspace(None, C.byref(TqAttendArgs()), 0, None, C.byref(size)) == -1
     assert lib.tq_select_blocks_workspace(None, C.byref(TqSelectArgs()), None, C.byref(size)) == -1
 
 

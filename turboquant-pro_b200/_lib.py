@@ -112,6 +112,9 @@ SIGNATURES = {
     "tq_attend_blocks_workspace": (C.c_int32, [C.c_void_p, C.POINTER(TqAttendArgs), C.c_int32, C.c_void_p,
                                                C.POINTER(C.c_size_t)]),
     "tq_attend_blocks": (C.c_int32, [C.c_void_p, C.POINTER(TqAttendArgs), C.c_void_p, C.c_int32, C.c_void_p]),
+    "tq_attend_prefix_workspace": (C.c_int32, [C.c_void_p, C.POINTER(TqAttendArgs), C.c_int32, C.c_void_p,
+                                               C.POINTER(C.c_size_t)]),
+    "tq_attend_prefix": (C.c_int32, [C.c_void_p, C.POINTER(TqAttendArgs), C.c_int32, C.c_void_p]),
     "tq_select_blocks_workspace": (C.c_int32, [C.c_void_p, C.POINTER(TqSelectArgs), C.c_void_p,
                                                C.POINTER(C.c_size_t)]),
     "tq_select_blocks": (C.c_int32, [C.c_void_p, C.POINTER(TqSelectArgs), C.c_void_p]),

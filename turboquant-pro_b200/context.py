@@ -283,7 +283,8 @@ class KVContext:
         return out
 
     def attend(self, layer: int, q, window: int | None = None, sinks: int = 0, q_lens=None,
-               seq_begin: int = 0, out=None, max_workspace: int | None = None, blocks=None):
+               seq_begin: int = 0, out=None, max_workspace: int | None = None, blocks=None,
+               prefix: int | None = None):
         """Attention of one or many query tokens per sequence on the codes, with the causal mask, a
         sliding window and first tokens that stay visible.
 
@@ -306,6 +307,11 @@ class KVContext:
         blocks a query token then sees, for each KV head, those of the listed ones up to its own position, and the
         uncompressed window as ever.  A list ascends; it ends at the first entry that is not above the one before it, or
         no block of the sequence (``-1``).  It takes the place of ``window`` and ``sinks``.
+
+        ``prefix``: a sequence of the layer, none of the call's own, whose tokens stand before those of every sequence of the call:
+        an instruction or a document that they share, stored once and read once for all of them.  Every query token sees all of
+        it, and its own sequence's tokens as ever; rows without a token of their own sequence stay zeros.  Without
+        ``window``, ``sinks`` and ``blocks``.  (Positions: :meth:`norm_rope` with ``prefix``.)
         """
         # (a decode step's call is some microseconds on the GPU: the checks are kept short)
         torch = _torch()
@@ -324,6 +330,10 @@ class KVContext:
             raise ValueError(f"window must be at least 1 (or None), got {window}")
         if sinks < 0:
             raise ValueError(f"sinks must not be negative, got {sinks}")
+        if prefix is not None:
+            if window is not None or sinks or blocks is not None:
+                raise ValueError("a shared beginning goes without window, sinks and blocks")
+            prefix = self._check_prefix(prefix, seq_begin, shape[0])
         if blocks is not None:
             if window is not None or sinks:
                 raise ValueError("blocks take the place of a window: window and sinks must be left out")
@@ -350,7 +360,8 @@ class KVContext:
             s1 = 0
         if shape[2] == 1:
             s2 = 0
-        if (s3 != 1 or q.data_ptr() % 16 or s0 % step or s1 % step or s2 % step) and q.numel():
+        flat = prefix is None or s0 == shape[1] * s1 or shape[0] == 1 or shape[1] == 1
+        if (s3 != 1 or q.data_ptr() % 16 or s0 % step or s1 % step or s2 % step or not flat) and q.numel():
             # (not contiguous(), which gives back a tensor that begins off a 16-byte boundary as it is)
             q = torch.empty(shape, dtype=dtype, device=dev).copy_(q)
             s0, s1, s2, s3 = q.stride()
@@ -359,14 +370,18 @@ class KVContext:
                          min(sinks, 2**31 - 1))
         with self._here():
             stream, ref, size = self._stream(), C.byref(a), C.c_size_t()
-            if blocks is None:
+            if prefix is not None:
+                check(self._lib.tq_attend_prefix_workspace(self._h, ref, prefix, stream, C.byref(size)))
+            elif blocks is None:
                 check(self._lib.tq_attend_workspace(self._h, ref, stream, C.byref(size)))
             else:
                 check(self._lib.tq_attend_blocks_workspace(self._h, ref, blocks.shape[3], stream, C.byref(size)))
             n = size.value if max_workspace is None else min(size.value, max(max_workspace, 0))
             work = torch.empty(n, dtype=torch.uint8, device=dev)
             a.workspace, a.workspace_bytes = work.data_ptr(), n
-            if blocks is None:
+            if prefix is not None:
+                check(self._lib.tq_attend_prefix(self._h, ref, prefix, stream))
+            elif blocks is None:
                 check(self._lib.tq_attend(self._h, ref, stream))
             else:
                 check(self._lib.tq_attend_blocks(self._h, ref, blocks.data_ptr(), blocks.shape[3], stream))
@@ -454,21 +469,38 @@ class KVContext:
         return prefix
 
     def step(self, layer: int, q, k, v, inv_freq, *, q_weight=None, k_weight=None, eps: float = 1e-6,
-             window: int | None = None, sinks: int = 0, seq_begin: int = 0):
+             window: int | None = None, sinks: int = 0, seq_begin: int = 0, positions=None, axes=None,
+             top_blocks: int | None = None, first_blocks: int = 1, prefix: int | None = None):
         """One layer's attention for new tokens, from its projections to its output: :meth:`norm_rope`
-        at the positions that follow, :meth:`append`, :meth:`attend`.  ``q`` ``[n_seqs', T, n_q_heads,
-        D]``, ``k`` / ``v`` ``[n_seqs', T, n_kv_heads, D]``; prompts, chunks of them and single
-        tokens alike."""
+        at the positions that follow (or at ``positions``, of several ``axes`` where these are given), :meth:`append`,
+        :meth:`attend`.  ``q`` ``[n_seqs', T, n_q_heads, D]``, ``k`` / ``v`` ``[n_seqs', T, n_kv_heads, D]``; prompts,
+        chunks of them and single tokens alike.  ``top_blocks``: the query tokens attend so many blocks of
+        :meth:`select_blocks` (``first_blocks`` first ones among them) and the uncompressed window; ``prefix``: the sequences
+        go on from a shared one."""
         if v.dim() != 4 or v.shape != k.shape:
             raise ValueError(f"k and v differ in shape: {tuple(k.shape)} and {tuple(v.shape)}")
         # (what attend refuses is refused before anything is appended)
         window, sinks = None if window is None else operator.index(window), operator.index(sinks)
         if (window is not None and window < 1) or sinks < 0:
             raise ValueError(f"window must be at least 1 (or None) and sinks not negative, got {window}, {sinks}")
-        q, k = self.norm_rope(layer, q, k, inv_freq, q_weight=q_weight, k_weight=k_weight, eps=eps,
-                              seq_begin=seq_begin)
+        if (window is not None or sinks != 0) + (top_blocks is not None) + (prefix is not None) > 1:
+            raise ValueError("of a window, selected blocks and a shared beginning a layer has one")
+        if prefix is not None:
+            prefix = self._check_prefix(prefix, seq_begin, q.shape[0])
+        if top_blocks is not None:
+            top_blocks, first_blocks = operator.index(top_blocks), operator.index(first_blocks)
+            if not 1 <= top_blocks < 2**31 or not 0 <= first_blocks < 2**31:
+                raise ValueError(f"top_blocks must be at least 1 and first_blocks not negative, got {top_blocks}, "
+                                 f"{first_blocks}")
+            if self.key_mode == "polar":
+                raise NotImplementedError("blocks are selected by the keys' per-channel grids: polar keys have none")
+        q, k = self.norm_rope(layer, q, k, inv_freq, positions, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                              seq_begin=seq_begin, axes=axes, prefix=prefix if positions is None else None)
         self.append(layer, k, v, seq_begin)
-        return self.attend(layer, q, window, sinks, seq_begin=seq_begin)
+        blocks = None
+        if top_blocks is not None:
+            blocks = self.select_blocks(layer, q, top_blocks, first=first_blocks, seq_begin=seq_begin)
+        return self.attend(layer, q, window, sinks, seq_begin=seq_begin, blocks=blocks, prefix=prefix)
 
     def raise_on_timeout(self) -> int:
         """Reads the status word (synchronises); raises if a bounded wait of a kernel ran out since

@@ -30,11 +30,15 @@ struct Plan {
   size_t fixed_bytes, seq_bytes;  // workspace: of a launch, of a sequence
 };
 
-// A call: the caller's arguments, and the blocks on its lists (listed).
+// A call: the caller's arguments, the blocks on its lists (listed), and the parts of a call with a shared beginning (see
+// AttendArgs).
 struct Call : tq_attend_args {
   const int32_t* list;
   int32_t n_list;
-  bool listed;
+  bool listed, whole;
+  float* states;
+  const float* before;
+  int64_t before_rows;
 };
 Call plain_call(const tq_attend_args* r) {
   Call c = {};
@@ -51,6 +55,7 @@ Call part_of(const tq_ctx* ctx, const Call& r, int s, int n) {
   part.q = (const uint8_t*)r.q + (int64_t)s * r.q_seq_stride * (int64_t)esz;
   part.out = (uint8_t*)r.out + (size_t)s * r.n_tokens * g.n_q_heads * TQ_D * esz;
   part.q_lens = r.q_lens == nullptr ? nullptr : r.q_lens + s;
+  part.before = r.before == nullptr ? nullptr : r.before + (size_t)s * r.n_tokens * g.group * TQ_PART_STRIDE;
   part.list = r.list == nullptr ? nullptr : r.list + (size_t)s * r.n_tokens * g.n_kv_heads * r.n_list;
   return part;
 }
@@ -210,10 +215,11 @@ int run(tq_ctx* ctx, const Call* r, const Plan& p, cudaStream_t st) {
   a.wait_limit = ctx->wait_limit, a.withhold = ctx->withhold_tile;
   a.unit_stride = (int64_t)a.rows * (p.ns_cold + p.ns_hot) * TQ_PART_STRIDE;
   a.n_list = r->n_list, a.listed = r->listed;
+  a.whole = r->whole, a.states = r->states, a.before_rows = r->before_rows;
   for (int s = 0; s < r->seq_count; s += at_once) {
     const Call part = part_of(ctx, *r, s, std::min(at_once, r->seq_count - s));
     a.seq_begin = part.seq_begin, a.seq_count = part.seq_count;
-    a.q = part.q, a.out = part.out, a.q_lens = part.q_lens, a.list = part.list;
+    a.q = part.q, a.out = part.out, a.q_lens = part.q_lens, a.list = part.list, a.before = part.before;
     if (p.form == TILES) {
       const int rc = tq_launch_attend_tiles(a, r->workspace, p.cap, p.splits, st);
       if (rc != TQ_OK) return rc;
@@ -292,7 +298,70 @@ Call listed_call(const tq_attend_args* r, const int32_t* blocks, int32_t n_block
   return c;
 }
 
+// A call with a shared beginning, in two parts: the queries of all sequences as those of one, on the prefix, and the
+// sequences' own tokens.  The prefix's states stand before the workspace that the parts use one after the other.
+struct Shared {
+  Call prefix, own;
+  size_t states;  // bytes
+};
+int shared_call(tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, Shared* c) {
+  const tq_geom& g = ctx->g;
+  TQ_REQUIRE(r->window == 0 && r->sinks == 0, TQ_ERR_INVALID, "a window and a shared beginning do not go together");
+  TQ_REQUIRE(prefix >= 0 && prefix < g.n_seqs && (prefix < r->seq_begin || prefix >= r->seq_begin + r->seq_count),
+             TQ_ERR_INVALID, "prefix must be a sequence of the context that is none of the call's own");
+  const int64_t tokens = (int64_t)r->seq_count * r->n_tokens;
+  TQ_REQUIRE(tokens * g.group <= (1 << 30), TQ_ERR_INVALID, "too many query tokens in a call");
+  TQ_REQUIRE(r->seq_count <= 1 || r->n_tokens <= 1 || r->q_seq_stride == r->n_tokens * r->q_tok_stride, TQ_ERR_INVALID,
+             "with a shared beginning the queries of a sequence must follow those of the one before");
+  c->own = c->prefix = plain_call(r);
+  Call& p = c->prefix;
+  p.seq_begin = prefix, p.seq_count = 1, p.n_tokens = (int32_t)tokens;
+  if (r->n_tokens == 1) p.q_tok_stride = r->q_seq_stride;
+  p.q_lens = nullptr;
+  p.whole = true;
+  c->states = align_up((size_t)g.n_kv_heads * tokens * g.group * TQ_PART_STRIDE * 4, 256);
+  p.states = (float*)r->workspace;
+  c->own.before = (const float*)r->workspace;
+  c->own.before_rows = tokens * g.group;
+  for (Call* x : {&c->prefix, &c->own}) {
+    x->workspace = (uint8_t*)r->workspace + c->states;
+    x->workspace_bytes = r->workspace_bytes < c->states ? 0 : r->workspace_bytes - c->states;
+  }
+  return TQ_OK;
+}
+
 }  // namespace
+
+extern "C" int32_t tq_attend_prefix_workspace(tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, void* stream,
+                                              size_t* bytes) {
+  int rc = check_args(ctx, r);
+  if (rc != TQ_OK) return rc;
+  TQ_REQUIRE(bytes != nullptr, TQ_ERR_INVALID, "null argument");
+  Shared c;
+  rc = shared_call(ctx, r, prefix, &c);
+  size_t of_prefix = 0, of_own = 0;
+  if (rc == TQ_OK) rc = workspace_of(ctx, c.prefix, stream, &of_prefix);
+  if (rc == TQ_OK) rc = workspace_of(ctx, c.own, stream, &of_own);
+  if (rc == TQ_OK) *bytes = c.states + std::max(of_prefix, of_own);
+  return rc;
+}
+
+extern "C" int32_t tq_attend_prefix(tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, void* stream) {
+  int rc = check_args(ctx, r);
+  if (rc != TQ_OK) return rc;
+  Shared c;
+  rc = shared_call(ctx, r, prefix, &c);
+  if (rc != TQ_OK || r->seq_count == 0 || r->n_tokens == 0) return rc;
+  TQ_REQUIRE(r->workspace != nullptr && (uintptr_t)r->workspace % 256 == 0, TQ_ERR_INVALID,
+             "workspace must be a device pointer aligned to 256 bytes");
+  TQ_REQUIRE(r->workspace_bytes >= c.states, TQ_ERR_CAPACITY, "workspace smaller than the states of the shared beginning");
+  rc = attend(ctx, c.prefix, stream);
+  if (rc != TQ_OK) return rc;
+  const int launches = ctx->last_launches;
+  rc = attend(ctx, c.own, stream);
+  ctx->last_launches += launches;
+  return rc;
+}
 
 extern "C" int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* r, void* stream, size_t* bytes) {
   const int rc = check_args(ctx, r);

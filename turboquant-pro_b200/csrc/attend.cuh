@@ -46,6 +46,13 @@ struct AttendArgs {
   // listed: of the blocks a query token sees those on its list alone, [seq_count][n_tokens][n_kv_heads][n_list]
   const int32_t* list;
   int32_t n_list, listed;
+  // A shared beginning: the queries of all sequences are those of one, the prefix, and see all that it holds (whole); the merge
+  // leaves states (M, L, o[D]), o in the original basis, [unit][rows][2 + D].  The sequences' own part then takes them
+  // into its merge: row r of a unit of head h has the state [h][before_rows][2 + D] at s * rows + r.
+  int32_t whole;
+  float* states;
+  const float* before;
+  int64_t before_rows;
   int32_t wait_limit, withhold;  // test hook of the form for many rows (tq_debug_wait); 0 and -1 otherwise
 };
 
@@ -61,7 +68,7 @@ TQ_DEV AttendSeq attend_seq(const AttendArgs& a, int s) {
   r.n = a.seq_len[a.layer * a.g.n_seqs + a.seq_begin + s];
   r.cold = n_cold_blocks(r.n, a.g.hot_window, a.g.block_tokens) * a.g.block_tokens;
   r.q_n = a.q_lens == nullptr ? a.n_tokens : min(max(a.q_lens[s], 0), a.n_tokens);
-  r.first = r.n - r.q_n;
+  r.first = a.whole ? r.n : r.n - r.q_n;
   return r;
 }
 // position of a row's token; -1: the row sees nothing
@@ -110,6 +117,36 @@ TQ_DEV int attend_listed(const AttendArgs& a, const int32_t* list, int blocks) {
 
 TQ_DEV float* attend_partial(const AttendArgs& a, int unit, int row, int split) {
   return a.partials + (size_t)unit * a.unit_stride + ((size_t)row * (a.ns_cold + a.ns_hot) + split) * TQ_PART_STRIDE;
+}
+
+// The weight of a state in a merge whose maximum is `by`; a state without a sum takes no part, one whose sum is no number does.
+TQ_DEV float attend_weight(float m, float l, float by) { return l == 0.0f ? 0.0f : m > -INFINITY ? tq_exp2(m - by) : 1.0f; }
+// The state of a row's shared beginning, null where the row has no token of its own.
+TQ_DEV const float* attend_before(const AttendArgs& a, int s, int head, int row) {
+  if (a.before == nullptr || attend_position(a, attend_seq(a, s), row) < 0) return nullptr;
+  return a.before + ((size_t)head * a.before_rows + (size_t)s * a.rows + row) * TQ_PART_STRIDE;
+}
+// Channel e of a merged row (maximum M, sum of weights L, sum of weighted values o) as the call's result.
+TQ_DEV void attend_result(const AttendArgs& a, int s, int head, int row, int e, float M, float L, float o) {
+  const tq_geom& g = a.g;
+  if (a.states != nullptr) {
+    float* to = a.states + ((size_t)(s * g.n_kv_heads + head) * a.rows + row) * TQ_PART_STRIDE;
+    if (e == 0) *(float2*)to = make_float2(M, L);
+    to[2 + e] = o;
+    return;
+  }
+  if (const float* x = attend_before(a, s, head, row)) {
+    const float top = fmaxf(M, x[0]), by = top > -INFINITY ? top : 0.0f;
+    const float w = attend_weight(M, L, by), wx = attend_weight(x[0], x[1], by);
+    L = (w != 0.0f ? L * w : 0.0f) + (wx != 0.0f ? x[1] * wx : 0.0f);
+    o = (w != 0.0f ? o * w : 0.0f) + (wx != 0.0f ? x[2 + e] * wx : 0.0f);
+  }
+  const float v = L == 0.0f ? 0.0f : o / L;
+  const int G = g.group;
+  const size_t to = (((size_t)s * a.n_tokens + row / G) * g.n_q_heads + head * G + row % G) * TQ_D + e;
+  if (a.q_dtype == TQ_F32) ((float*)a.out)[to] = v;
+  else if (a.q_dtype == TQ_F16) ((__half*)a.out)[to] = __float2half_rn(v);
+  else ((__nv_bfloat16*)a.out)[to] = __float2bfloat16_rn(v);
 }
 
 TQ_DEV float attend_ld(const void* p, size_t i, int dt) {

@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(AG_THREADS) attend_left_kernel(AttendArgs a, i
 __global__ void __launch_bounds__(TQ_D) attend_combine_kernel(AttendArgs a) {
   const tq_geom& g = a.g;
   const int e = threadIdx.x, unit = blockIdx.x / a.rows, row = blockIdx.x % a.rows;
-  const int ns = a.ns_cold + a.ns_hot, H = g.n_kv_heads, G = g.group, s = unit / H, head = unit % H;
+  const int ns = a.ns_cold + a.ns_hot, H = g.n_kv_heads, s = unit / H, head = unit % H;
   __shared__ float cs[TQ_D];
   float M = -INFINITY, L = 0.0f, C = 0.0f, Y = 0.0f;
   const float* p = attend_partial(a, unit, row, 0);
@@ -411,11 +411,7 @@ __global__ void __launch_bounds__(TQ_D) attend_combine_kernel(AttendArgs a) {
     for (int d = 0; d < 16; ++d) z = fmaf(cs[d0 + d], a.tables->pi[(d0 + d) * TQ_D + e], z);
     y += z;
   }
-  const size_t at = (((size_t)s * a.n_tokens + row / G) * g.n_q_heads + head * G + row % G) * TQ_D + e;
-  const float x = L == 0.0f ? 0.0f : (y + Y) / L;
-  if (a.q_dtype == TQ_F32) ((float*)a.out)[at] = x;
-  else if (a.q_dtype == TQ_F16) ((__half*)a.out)[at] = __float2half_rn(x);
-  else ((__nv_bfloat16*)a.out)[at] = __float2bfloat16_rn(x);
+  attend_result(a, s, head, row, e, M, L, y + Y);
 }
 
 template <int RPT, bool LIST = false>

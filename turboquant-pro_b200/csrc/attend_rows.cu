@@ -216,7 +216,7 @@ template <bool LIST>
 TQ_DEV ArWork ar_work(const AttendArgs& a, int n, int q_n) {
   ArWork w;
   w.cold = n_cold_blocks(n, a.g.hot_window, AR_S) * AR_S;
-  const int p_lo = n - q_n, p_hi = q_n > 0 ? n - 1 : -1;
+  const int p_lo = a.whole ? n : n - q_n, p_hi = q_n > 0 ? (a.whole ? n + q_n : n) - 1 : -1;
   w.strip = LIST ? AttendTiles{0, 0, p_hi >= 0 ? min(a.n_list, w.cold / AR_S) * (AR_S / AR_STRIP) : 0}
                  : attend_tiles(a, 0, w.cold, AR_STRIP, p_lo, p_hi);
   w.hot = attend_tiles(a, w.cold, n, AR_HOT, p_lo, p_hi);
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
     }
   };
   auto start_row = [&]() {
-    const int n = sh.seq[s].x, q_n = sh.seq[s].y, first = n - q_n;
+    const int n = sh.seq[s].x, q_n = sh.seq[s].y, first = a.whole ? n : n - q_n;
     const int last = min(min(row0 + N, rows_end()), q_n * G) - 1;
     p_lo = first + row0 / G;
     p_hi = last >= row0 ? first + last / G : -1;
@@ -1277,7 +1277,7 @@ __global__ void __launch_bounds__(AC_THREADS, 2) attend_rows_combine_kernel(Atte
   const int64_t share = plan->share;
   for (int r0 = blockIdx.x * ROWS; r0 < total; r0 += gridDim.x * ROWS) {
     const int at = r0 + (ROWS == 4 ? h : 0);
-    float hot = 0.0f, L = 0.0f, x = 0.0f;
+    float hot = 0.0f, L = 0.0f, x = 0.0f, M = -INFINITY;
     int s = 0, head = 0, row = 0;
     if (at < total) {
       row = at % a.rows;
@@ -1292,7 +1292,6 @@ __global__ void __launch_bounds__(AC_THREADS, 2) attend_rows_combine_kernel(Atte
         const int nc = seq.x > 0 ? (int)(ar_div(middle - cost, share) - ar_div(begin, share)) + 1 : 0;
         const int nh = seq.y > 0 ? (int)(ar_div(middle + a.hot_cost * (seq.y - 1), share) - ar_div(middle, share)) + 1 : 0;
         const float* base = attend_partial(a, unit, row, 0);
-        float M = -INFINITY;
         constexpr int BATCH = 4, STEP = ROWS == 4 ? 1 : 4;
         for (int i0 = ROWS == 4 ? 0 : h; i0 < nc + nh; i0 += BATCH * STEP) {
           float m[BATCH], l[BATCH], v[BATCH];
@@ -1326,6 +1325,7 @@ __global__ void __launch_bounds__(AC_THREADS, 2) attend_rows_combine_kernel(Atte
           const float top = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), by = top > -INFINITY ? top : 0.0f;
           const float down = M > -INFINITY ? tq_exp2(M - by) : 1.0f;
           L *= down, x *= down, hot *= down;
+          M = top;
         }
       }
     }
@@ -1355,11 +1355,7 @@ __global__ void __launch_bounds__(AC_THREADS, 2) attend_rows_combine_kernel(Atte
       }
       const int k = ROWS == 4 ? h : 0;
       const float o = (ys[0][k][e] + ys[1][k][e]) + (ys[2][k][e] + ys[3][k][e]) + hot;
-      const float v = L == 0.0f ? 0.0f : o / L;
-      const size_t to = (((size_t)s * a.n_tokens + row / G) * g.n_q_heads + head * G + row % G) * TQ_D + e;
-      if (a.q_dtype == TQ_F32) ((float*)a.out)[to] = v;
-      else if (a.q_dtype == TQ_F16) ((__half*)a.out)[to] = __float2half_rn(v);
-      else ((__nv_bfloat16*)a.out)[to] = __float2bfloat16_rn(v);
+      attend_result(a, s, head, row, e, M, L, o);
     }
     if (ROWS == 1) __syncthreads();  // (the sums have been read)
   }

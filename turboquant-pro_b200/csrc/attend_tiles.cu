@@ -78,6 +78,14 @@ TQ_DEV AttendTiles unit_tiles(const AttendArgs& a, const AttendSeq& sq) {
   return attend_tiles(a, 0, sq.n, TI_T, sq.first, sq.q_n > 0 ? sq.n - 1 : -1);
 }
 
+// The vector that is taken off all keys of a (sequence, KV head): what its first block's channels are around.  (Uniform grids
+// count from their zero-point on: their middle.)
+TQ_DEV float ti_center(const tq_geom& g, const uint8_t* page, int d) {
+  float c = ((const float*)(page + g.mean_off))[d];
+  if (g.key_mode == TQ_KEYS_UNIFORM) c = fmaf(7.5f, ((const float*)(page + g.scale_off))[d], c);
+  return isfinite(c) ? c : 0.0f;
+}
+
 // 2^(top - floor(log2 x)), and the exponent of its inverse; what is below 2^-63, or 2^(least - 127), counts as that
 TQ_DEV float ti_lift(float x, int top, float& exponent, int least = 64) {
   const int e = min(max((int)(__float_as_uint(x) >> 23 & 255u), least), 254);
@@ -170,15 +178,7 @@ __global__ void __launch_bounds__(TS_THREADS, SPLIT ? 2 : 3) attend_stage_kernel
     sh.grid[tid] = a.tables->grid[tid];
     sh.cent[tid] = a.tables->centroids[tid];
   }
-  if (tid < TQ_D) {  // uniform grids count from their zero-point on: their middle
-    float c = 0.0f;
-    if (sq.cold > 0) {
-      c = ((const float*)(pages + g.mean_off))[tid];
-      if (g.key_mode == TQ_KEYS_UNIFORM) c = fmaf(7.5f, ((const float*)(pages + g.scale_off))[tid], c);
-      if (!isfinite(c)) c = 0.0f;
-    }
-    sh.center[tid] = c;
-  }
+  if (tid < TQ_D) sh.center[tid] = sq.cold > 0 ? ti_center(g, pages, tid) : 0.0f;
   bool odd = false;
   {  // ---- norms of the values: four threads a token
     const int row = tid >> 2, t = t0 + row;
@@ -733,7 +733,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       __syncwarp();
       ti_fence_after();
     };
-    float factor;
+    float factor, shift = 0.0f;
     {
       uint4 raw[16];
       const bool there = row < a.rows;
@@ -771,6 +771,22 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(enc_smem(&sh.q_ready[x]));
+      // What the keys' common vector took off this row's scores: a state that is merged with others' needs it again.
+      if ((a.states != nullptr || a.before != nullptr) && sq.cold > 0) {
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint8_t* page = a.pages + page_offset(g, a.layer, a.seq_begin + s, head, 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = pair(w[j]);
+            part[j] = fmaf(f.x, ti_center(g, page, 8 * i + 2 * j), part[j]);
+            part[j] = fmaf(f.y, ti_center(g, page, 8 * i + 2 * j + 1), part[j]);
+          }
+        }
+        shift = tq_scaled<true>((part[0] + part[1]) + (part[2] + part[3]));
+      }
     }
     const int p = row < a.rows ? attend_position(a, sq, row) : -1, w = attend_window(a, p);
     // whether all rows of this CTA see a tile goes by their earliest position and latest window
@@ -797,7 +813,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
       ti_wait_ld();
       ti_fence_before();
       mbar_arrive(enc_smem(&sh.s_read[x]));
-      const bool open = whole && t0 + TI_T - 1 <= p_lo && (t0 >= w_hi || t0 + TI_T <= a.sinks);
+      const bool open = whole && t0 + TI_T - 1 <= min(p_lo, sq.n - 1) && (t0 >= w_hi || t0 + TI_T <= a.sinks);
       if (!open) {
         const int hi = min(p, sq.n - 1) - t0, lo = w - t0, sk = a.sinks - t0;
 #pragma unroll
@@ -871,7 +887,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
     // the row's state: [channel][row], neighbouring threads side by side
     const size_t at = ((size_t)unit * ta.splits + split) * ta.row_tiles + rt;
     float* stats = ta.stats + at * 2 * TI_ROWS + 128 * x + r;
-    stats[0] = n > 0 ? m - TI_LIFT : -INFINITY;
+    stats[0] = n > 0 ? m - TI_LIFT + shift : -INFINITY;
     stats[TI_ROWS] = l;
     if (n > 0) {
       settled(&sh.o_done[x], (n - 1) & 1);
@@ -903,7 +919,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) attend_tiles_kernel(AttendArgs 
 constexpr int TC_ROWS = 64, TC_THREADS = 256;
 struct CombineShared {
   alignas(128) uint8_t ph[TQ_D * 256], pl[TQ_D * 256], hi[TC_ROWS * 256], lo[TC_ROWS * 256];
-  float top[TC_THREADS / 32][TC_ROWS], inv[TC_ROWS];
+  float top[TC_THREADS / 32][TC_ROWS], inv[TC_ROWS], of_before[TC_ROWS];
 };
 // Byte of eight neighbouring columns of a row: neither eight rows in a row nor every fourth of 32 share a bank.
 TQ_DEV int tc_at(int row, int c8) { return row * 256 + ((c8 ^ (row >> 2 & 7) ^ (row & 3) << 1) << 4); }
@@ -911,6 +927,8 @@ TQ_DEV void tc_ldmatrix(uint32_t (&r)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
+// SHARED: the merge leaves states, or takes those of a shared beginning in.
+template <bool SHARED>
 __global__ void __launch_bounds__(TC_THREADS, 2) attend_tiles_combine_kernel(AttendArgs a, TileArgs ta, int tiles, int total) {
   extern __shared__ __align__(128) uint8_t tc_smem[];
   CombineShared& sh = *(CombineShared*)tc_smem;
@@ -942,13 +960,16 @@ __global__ void __launch_bounds__(TC_THREADS, 2) attend_tiles_combine_kernel(Att
         const float* x = attend_partial(a, unit, row, 0);
         const float* y = x + TQ_PART_STRIDE;
         const float M = fmaxf(x[0], y[0]), by = M > -INFINITY ? M : 0.0f;
-        const float wx = x[1] == 0.0f ? 0.0f : x[0] > -INFINITY ? tq_exp2(x[0] - by) : 1.0f;
-        const float wy = y[1] == 0.0f ? 0.0f : y[0] > -INFINITY ? tq_exp2(y[0] - by) : 1.0f;
+        const float wx = attend_weight(x[0], x[1], by), wy = attend_weight(y[0], y[1], by);
         float o = 0.0f;
         if (wx != 0.0f)
           for (int d = 0; d < TQ_D; ++d) o = fmaf(x[2 + d] * wx, a.tables->pi[d * TQ_D + e], o);
         if (wy != 0.0f) o = fmaf(y[2 + e], wy, o);
         const float L = (wx != 0.0f ? x[1] * wx : 0.0f) + (wy != 0.0f ? y[1] * wy : 0.0f);
+        if (SHARED) {
+          attend_result(a, s, head, row, e, M, L, o);
+          continue;
+        }
         o = L == 0.0f ? 0.0f : o / L;
         if (a.q_dtype == TQ_F16) ((__half*)a.out)[out_at(row) + e] = __float2half_rn(o);
         else ((__nv_bfloat16*)a.out)[out_at(row) + e] = __float2bfloat16_rn(o);
@@ -1006,7 +1027,24 @@ __global__ void __launch_bounds__(TC_THREADS, 2) attend_tiles_combine_kernel(Att
 #pragma unroll
       for (int i = 0; i < TC_THREADS / 32; ++i) t = fmaxf(t, sh.top[i][r4 + j]);
       const float up = ti_lift(t, 13, exponent);
-      if (c8 == 0) sh.inv[r4 + j] = L[j] == 0.0f ? 0.0f : exp2f(exponent - 8.0f) / L[j];
+      if (c8 == 0) {
+        const int row = row0 + r4 + j;
+        const float lower = exp2f(exponent - 8.0f);
+        if (SHARED) sh.of_before[r4 + j] = 0.0f;
+        if (SHARED && a.states != nullptr) {
+          sh.inv[r4 + j] = lower;
+          if (row < a.rows)
+            *(float2*)(a.states + ((size_t)unit * a.rows + row) * TQ_PART_STRIDE) = make_float2(M[j], L[j]);
+        } else if (const float* x = SHARED && row < a.rows ? attend_before(a, s, head, row) : nullptr) {
+          const float top = fmaxf(M[j], x[0]), by = top > -INFINITY ? top : 0.0f;
+          const float w = attend_weight(M[j], L[j], by), wx = attend_weight(x[0], x[1], by);
+          const float all = (w != 0.0f ? L[j] * w : 0.0f) + (wx != 0.0f ? x[1] * wx : 0.0f);
+          sh.inv[r4 + j] = w == 0.0f ? 0.0f : lower * w / all;
+          sh.of_before[r4 + j] = wx == 0.0f ? 0.0f : wx / all;
+        } else {
+          sh.inv[r4 + j] = L[j] == 0.0f ? 0.0f : lower / L[j];
+        }
+      }
       uint32_t h[4], l[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -1046,10 +1084,27 @@ __global__ void __launch_bounds__(TC_THREADS, 2) attend_tiles_combine_kernel(Att
       for (int i = 0; i < 4; ++i) d[i] += d1[i] + d2[i];
       // channels q, q + 8 of the warp's sixteen; rows 2 c, 2 c + 1
       const float f0 = sh.inv[8 * nt + 2 * c], f1 = sh.inv[8 * nt + 2 * c + 1];
+      if (SHARED && a.states != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 8 * nt + 2 * c + (i & 1);
+          if (row < rows)
+            a.states[((size_t)unit * a.rows + row0 + row) * TQ_PART_STRIDE + 2 + 16 * warp + q + 8 * (i >> 1)] =
+                d[i] * (i & 1 ? f1 : f0);
+        }
+        continue;
+      }
       uint32_t w[2];
+      const float b0 = SHARED ? sh.of_before[8 * nt + 2 * c] : 0.0f, b1 = SHARED ? sh.of_before[8 * nt + 2 * c + 1] : 0.0f;
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const float u = d[2 * y] * f0, v = d[2 * y + 1] * f1;
+        float u = d[2 * y] * f0, v = d[2 * y + 1] * f1;
+        if (SHARED && (b0 != 0.0f || b1 != 0.0f)) {
+          const float* x = a.before + ((size_t)head * a.before_rows + (size_t)s * a.rows + row0 + 8 * nt + 2 * c) * TQ_PART_STRIDE + 2 +
+                           16 * warp + q + 8 * y;
+          if (b0 != 0.0f) u = fmaf(x[0], b0, u);
+          if (b1 != 0.0f) v = fmaf(x[TQ_PART_STRIDE], b1, v);
+        }
         if (a.q_dtype == TQ_F16) {
           w[y] = ti_pair(u, v);
         } else {
@@ -1139,10 +1194,12 @@ int tq_launch_attend_tiles(const AttendArgs& base, void* workspace, int cap, int
   if (rc != TQ_OK) return rc;
   rc = tq_launch_attend_general(a, st);
   if (rc != TQ_OK) return rc;
-  static bool combine_done[64];
-  rc = attend_shared(attend_tiles_combine_kernel, sizeof(CombineShared), a.device, combine_done);
+  const bool shared = a.states != nullptr || a.before != nullptr;
+  static bool combine_done[2][64];
+  const auto combine = shared ? attend_tiles_combine_kernel<true> : attend_tiles_combine_kernel<false>;
+  rc = attend_shared(combine, sizeof(CombineShared), a.device, combine_done[shared]);
   if (rc != TQ_OK) return rc;
-  attend_tiles_combine_kernel<<<std::min(units * tiles, 2 * a.sm_count), TC_THREADS, sizeof(CombineShared), st>>>(a, ta, tiles, units * tiles);
+  combine<<<std::min(units * tiles, 2 * a.sm_count), TC_THREADS, sizeof(CombineShared), st>>>(a, ta, tiles, units * tiles);
   TQ_CUDA(cudaGetLastError());
   return TQ_OK;
 }
