@@ -210,7 +210,8 @@ int32_t tq_attend(tq_ctx* ctx, const tq_attend_args* args, void* stream);
  * call's own, stand before those of each of them and are seen by all of their query tokens (the newest n of each
  * sequence's own tokens, as in tq_attend; rows that have no token of their sequence stay zeros).  They are read once for all
  * sequences.  `window` and `sinks` must be 0; with several sequences of several tokens q_seq_stride must be n_tokens *
- * q_tok_stride.  Positions for the rotation: tq_ctx_norm_rope_after. */
+ * q_tok_stride.  With less workspace than it asks for, down to what it asks for any one of the sequences, the call goes in
+ * rounds, each of which reads the shared tokens.  Positions for the rotation: tq_ctx_norm_rope_after. */
 int32_t tq_attend_prefix_workspace(tq_ctx* ctx, const tq_attend_args* args, int32_t prefix, void* stream, size_t* bytes);
 int32_t tq_attend_prefix(tq_ctx* ctx, const tq_attend_args* args, int32_t prefix, void* stream);
 

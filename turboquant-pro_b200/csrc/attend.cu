@@ -20,7 +20,7 @@ namespace {
 constexpr size_t AT_ONE_GO = (size_t)1 << 30;  // workspace that a call asks for at most, unless one
                                                // sequence needs more
 
-enum Form { GENERAL, ROWS, TILES };
+enum Form { GENERAL, ROWS, TILES, SHARED };
 struct Plan {
   Form form;
   int ns_cold, ns_hot;
@@ -101,6 +101,7 @@ Form choose(const tq_ctx* ctx, const Call* r, int n) {
   const bool channels = g.key_mode != TQ_KEYS_POLAR && !ctx->force_generic, blocks = g.block_tokens == 256;
   if (!channels) return GENERAL;
   if (r->listed) return blocks ? ROWS : GENERAL;
+  if (r->whole && blocks && r->q_dtype != TQ_F32) return SHARED;
   if (r->q_dtype == TQ_F32) return blocks && rows <= 48 ? ROWS : GENERAL;
   const double seen = r->window == 0 ? n : std::min((double)n, (double)r->window + r->n_tokens + r->sinks);
   const double w = seen * r->seq_count * g.n_kv_heads / 1000.0;
@@ -120,6 +121,17 @@ Plan make_plan(const tq_ctx* ctx, const Call* r, cudaStream_t st) {
   const int nb = n_cold_blocks(n, g.hot_window, g.block_tokens);
   p.form = choose(ctx, r, n);
   const int sm_count = ctx->sm_count;
+  if (p.form == SHARED) {
+    AttendArgs a = {};
+    a.g = g;
+    a.rows = rows;
+    a.q_dtype = r->q_dtype;
+    a.sm_count = sm_count;
+    tq_attend_shared_plan(a, n, &a.ns_cold, &a.ns_hot);
+    p.ns_cold = a.ns_cold, p.ns_hot = a.ns_hot;
+    p.seq_bytes = tq_attend_shared_bytes(a);
+    return p;
+  }
   if (p.form == TILES) {
     constexpr int TILE = TQ_ATTEND_TILE;
     const int64_t all = std::max<int64_t>((n + TILE - 1) / TILE, 1);
@@ -220,6 +232,12 @@ int run(tq_ctx* ctx, const Call* r, const Plan& p, cudaStream_t st) {
     const Call part = part_of(ctx, *r, s, std::min(at_once, r->seq_count - s));
     a.seq_begin = part.seq_begin, a.seq_count = part.seq_count;
     a.q = part.q, a.out = part.out, a.q_lens = part.q_lens, a.list = part.list, a.before = part.before;
+    if (p.form == SHARED) {
+      const int rc = tq_launch_attend_shared(a, r->workspace, st);
+      if (rc != TQ_OK) return rc;
+      ctx->last_launches += 3;
+      continue;
+    }
     if (p.form == TILES) {
       const int rc = tq_launch_attend_tiles(a, r->workspace, p.cap, p.splits, st);
       if (rc != TQ_OK) return rc;
@@ -304,30 +322,56 @@ struct Shared {
   Call prefix, own;
   size_t states;  // bytes
 };
-int shared_call(tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, Shared* c) {
-  const tq_geom& g = ctx->g;
+int check_shared(const tq_ctx* ctx, const tq_attend_args* r, int32_t prefix) {
   TQ_REQUIRE(r->window == 0 && r->sinks == 0, TQ_ERR_INVALID, "a window and a shared beginning do not go together");
-  TQ_REQUIRE(prefix >= 0 && prefix < g.n_seqs && (prefix < r->seq_begin || prefix >= r->seq_begin + r->seq_count),
+  TQ_REQUIRE(prefix >= 0 && prefix < ctx->g.n_seqs && (prefix < r->seq_begin || prefix >= r->seq_begin + r->seq_count),
              TQ_ERR_INVALID, "prefix must be a sequence of the context that is none of the call's own");
-  const int64_t tokens = (int64_t)r->seq_count * r->n_tokens;
-  TQ_REQUIRE(tokens * g.group <= (1 << 30), TQ_ERR_INVALID, "too many query tokens in a call");
+  TQ_REQUIRE((int64_t)r->seq_count * r->n_tokens * ctx->g.group <= (1 << 30), TQ_ERR_INVALID, "too many query tokens in a call");
   TQ_REQUIRE(r->seq_count <= 1 || r->n_tokens <= 1 || r->q_seq_stride == r->n_tokens * r->q_tok_stride, TQ_ERR_INVALID,
              "with a shared beginning the queries of a sequence must follow those of the one before");
-  c->own = c->prefix = plain_call(r);
-  Call& p = c->prefix;
-  p.seq_begin = prefix, p.seq_count = 1, p.n_tokens = (int32_t)tokens;
+  return TQ_OK;
+}
+// Sequences s .. s + n - 1 of the call
+Shared shared_part(const tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, int s, int n) {
+  const tq_geom& g = ctx->g;
+  Shared c;
+  c.own = c.prefix = part_of(ctx, plain_call(r), s, n);
+  const int tokens = n * r->n_tokens;
+  Call& p = c.prefix;
+  p.seq_begin = prefix, p.seq_count = 1, p.n_tokens = tokens;
   if (r->n_tokens == 1) p.q_tok_stride = r->q_seq_stride;
   p.q_lens = nullptr;
   p.whole = true;
-  c->states = align_up((size_t)g.n_kv_heads * tokens * g.group * TQ_PART_STRIDE * 4, 256);
+  c.states = align_up((size_t)g.n_kv_heads * tokens * g.group * TQ_PART_STRIDE * 4, 256);
   p.states = (float*)r->workspace;
-  c->own.before = (const float*)r->workspace;
-  c->own.before_rows = tokens * g.group;
-  for (Call* x : {&c->prefix, &c->own}) {
-    x->workspace = (uint8_t*)r->workspace + c->states;
-    x->workspace_bytes = r->workspace_bytes < c->states ? 0 : r->workspace_bytes - c->states;
+  c.own.before = (const float*)r->workspace;
+  c.own.before_rows = (int64_t)tokens * g.group;
+  for (Call* x : {&c.prefix, &c.own}) {
+    x->workspace = (uint8_t*)r->workspace + c.states;
+    x->workspace_bytes = r->workspace_bytes < c.states ? 0 : r->workspace_bytes - c.states;
+  }
+  return c;
+}
+// Bytes that the call needs in rounds of n sequences.
+int shared_bytes(tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, int n, cudaStream_t st, size_t* bytes) {
+  *bytes = 0;
+  for (int s = 0; s < r->seq_count; s += n) {
+    const Shared c = shared_part(ctx, r, prefix, s, std::min(n, r->seq_count - s));
+    size_t of_prefix = 0, of_own = 0;
+    int rc = workspace_of(ctx, c.prefix, st, &of_prefix);
+    if (rc == TQ_OK) rc = workspace_of(ctx, c.own, st, &of_own);
+    if (rc != TQ_OK) return rc;
+    *bytes = std::max(*bytes, c.states + std::max(of_prefix, of_own));
   }
   return TQ_OK;
+}
+// The most sequences a round for which `most` bytes do; one at least.
+int shared_rounds(tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, size_t most, cudaStream_t st, int* n, size_t* bytes) {
+  *n = std::max(r->seq_count, 1);
+  for (;; *n = (*n + 1) / 2) {
+    const int rc = shared_bytes(ctx, r, prefix, *n, st, bytes);
+    if (rc != TQ_OK || *bytes <= most || *n == 1) return rc;
+  }
 }
 
 }  // namespace
@@ -335,32 +379,35 @@ int shared_call(tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, Shared* c)
 extern "C" int32_t tq_attend_prefix_workspace(tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, void* stream,
                                               size_t* bytes) {
   int rc = check_args(ctx, r);
+  if (rc == TQ_OK) rc = check_shared(ctx, r, prefix);
   if (rc != TQ_OK) return rc;
   TQ_REQUIRE(bytes != nullptr, TQ_ERR_INVALID, "null argument");
-  Shared c;
-  rc = shared_call(ctx, r, prefix, &c);
-  size_t of_prefix = 0, of_own = 0;
-  if (rc == TQ_OK) rc = workspace_of(ctx, c.prefix, stream, &of_prefix);
-  if (rc == TQ_OK) rc = workspace_of(ctx, c.own, stream, &of_own);
-  if (rc == TQ_OK) *bytes = c.states + std::max(of_prefix, of_own);
-  return rc;
+  int n;
+  return shared_rounds(ctx, r, prefix, AT_ONE_GO, (cudaStream_t)stream, &n, bytes);
 }
 
 extern "C" int32_t tq_attend_prefix(tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, void* stream) {
   int rc = check_args(ctx, r);
-  if (rc != TQ_OK) return rc;
-  Shared c;
-  rc = shared_call(ctx, r, prefix, &c);
+  if (rc == TQ_OK) rc = check_shared(ctx, r, prefix);
   if (rc != TQ_OK || r->seq_count == 0 || r->n_tokens == 0) return rc;
   TQ_REQUIRE(r->workspace != nullptr && (uintptr_t)r->workspace % 256 == 0, TQ_ERR_INVALID,
              "workspace must be a device pointer aligned to 256 bytes");
-  TQ_REQUIRE(r->workspace_bytes >= c.states, TQ_ERR_CAPACITY, "workspace smaller than the states of the shared beginning");
-  rc = attend(ctx, c.prefix, stream);
+  int n;
+  size_t bytes;
+  rc = shared_rounds(ctx, r, prefix, r->workspace_bytes, (cudaStream_t)stream, &n, &bytes);
   if (rc != TQ_OK) return rc;
-  const int launches = ctx->last_launches;
-  rc = attend(ctx, c.own, stream);
-  ctx->last_launches += launches;
-  return rc;
+  TQ_REQUIRE(bytes <= r->workspace_bytes, TQ_ERR_CAPACITY, "workspace smaller than tq_attend_prefix_workspace asks for one sequence");
+  int launches = 0;
+  for (int s = 0; s < r->seq_count; s += n) {
+    const Shared c = shared_part(ctx, r, prefix, s, std::min(n, r->seq_count - s));
+    for (const Call* x : {&c.prefix, &c.own}) {
+      rc = attend(ctx, *x, stream);
+      if (rc != TQ_OK) return rc;
+      launches += ctx->last_launches;
+    }
+  }
+  ctx->last_launches = launches;
+  return TQ_OK;
 }
 
 extern "C" int32_t tq_attend_workspace(tq_ctx* ctx, const tq_attend_args* r, void* stream, size_t* bytes) {

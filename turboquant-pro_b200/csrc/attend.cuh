@@ -181,3 +181,7 @@ int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st);
 constexpr int TQ_ATTEND_TILE = 80;  // tokens of a tile
 size_t tq_attend_tiles_bytes(const AttendArgs& a, int units, int cap, int splits);
 int tq_launch_attend_tiles(const AttendArgs& a, void* workspace, int cap, int splits, cudaStream_t st);
+// A shared beginning: 16-bit queries, 256-token blocks of per-channel keys; the states
+void tq_attend_shared_plan(const AttendArgs& a, int tokens, int* ns_cold, int* ns_hot);
+size_t tq_attend_shared_bytes(const AttendArgs& a);
+int tq_launch_attend_shared(const AttendArgs& a, void* workspace, cudaStream_t st);
