@@ -72,6 +72,11 @@ CASES = [
     ([700, 3], 900, 1, 2, 4, "bfloat16", "bfloat16", 512, "polar", 3),
     ([60] * 70, 1800, 1, 1, 2, "bfloat16", "float32", 512, "nf4_asym", 3),
     ([600] * 3, 1111, 300, 1, 2, "bfloat16", "bfloat16", 512, "nf4_asym", 3),
+    # many tiles a CTA, pages that change within its part
+    ([9] * 40, 4096, 1, 16, 128, "bfloat16", "bfloat16", 512, "nf4_asym", 4),
+    ([30] * 50, 3900, 1, 32, 192, "bfloat16", "bfloat16", 512, "uniform", 3),
+    ([17] * 20, 4000, 1, 16, 128, "float16", "float16", 512, "nf4", 4),
+    ([40] * 70, 3333, 2, 8, 64, "float16", "float16", 512, "nf4_asym", 3),
 ]
 
 

@@ -10,6 +10,10 @@
 //               float32, outliers put over it.  c is one vector per head, the zero-point of the first block: it moves all
 //               scores of a row alike; what it takes off goes back into the state's maximum.
 //       values  in code space, norm * centroid[code] times a power of two per tile: two tokens of a channel a look-up.
+//     A row's error is that of its scores, and theirs comes from channels many times as wide as the others (half precision
+//     rounds a key of 60 by up to 0.016): the eight widest of a head's first page have a second part, a product step of
+//     its own.  The same 32768 tokens with three channels 20 times the others: 2.5e-3 -> 1.7e-3 off, rounding the exact
+//     result gives 1.65e-3.
 //     The uncompressed window is the work of CTAs of its own, whose sums are in the original basis.
 //     A page whose grid spans more than 2^20, an outlier that is 64 times its grid, window tokens below 2^-20 of their
 //     tile's largest, and what is no number set the flag of their head, which the general kernel then does.
@@ -24,12 +28,16 @@ constexpr int PX_T = 64;                     // tokens of a tile: a strip of a p
 constexpr int PX_S = 256;                    // tokens of a page
 constexpr int PX_IMAGE = PX_T * TQ_D * 2, PX_QIMAGE = 128 * TQ_D * 2;
 constexpr int PX_KLBO = PX_T * 16, PX_LBO = TQ_D * 16, PX_SBO = 128;  // from eight K to the next: keys; queries, values
-constexpr int PX_SOFTMAX = 256, PX_MAKERS = 256, PX_THREADS = PX_SOFTMAX + 64 + PX_MAKERS;
+// Warps: eight of softmax, two that issue products, two that put the outliers over the keys, eight that make operands.  A
+// thread's registers, 96 at launch, are divided anew by warpgroup: 120, 48 and 96 (two, one and two groups: 480 = 5 x 96).
+constexpr int PX_SOFTMAX = 256, PX_ISSUE = 128, PX_MAKERS = 256, PX_THREADS = PX_SOFTMAX + PX_ISSUE + PX_MAKERS;
+#define PX_REGISTERS(how, n) asm volatile("setmaxnreg." how ".sync.aligned.u32 " n ";")
 constexpr int PX_P = PX_T, PX_HALF = 128, PX_O = 256;  // tensor memory's columns, as in the form for many rows
-constexpr int PX_POLY = 2;                   // of eight pairs of exponentials, those on the multiply-add units
 constexpr int PX_STRIDE = 4 + TQ_D;          // floats of a state: M, L, -, -, o
 constexpr int PX_TOP = 8;                    // a page's largest key on the grid is lifted to 2^8 .. 2^9
-constexpr int PX_LIST = 3;                   // entries of a page's list that a thread holds
+constexpr int PX_LIST = 10;                  // entries of a page's list that a thread holds
+constexpr int PX_WIDE = 8;                   // channels whose keys are two parts
+constexpr int PX_WLBO = PX_T * 16, PX_WIMAGE = 2 * PX_WLBO, PX_QWLBO = 128 * 16, PX_QWIMAGE = 2 * PX_QWLBO;
 
 template <bool SPLIT>
 struct PxShape {
@@ -40,14 +48,20 @@ struct PxShape {
 template <bool SPLIT, int VB>
 struct PxShared {
   using Sh = PxShape<SPLIT>;
+  static constexpr int WIDE = SPLIT ? 0 : 1;
   static constexpr int ENTRY_K = 128, ENTRY_V = VB == 4 ? 64 : 128;  // bytes of a table's entry, copies and all
   alignas(128) uint8_t q[Sh::HALVES][PX_QIMAGE];
   alignas(128) uint8_t kv[Sh::STAGES][2 * Sh::PARTS][PX_IMAGE];
+  // the second parts of the wide channels (a step of 16 channels, the other eight of which stay zero), and their queries
+  alignas(128) uint8_t wide[Sh::STAGES][WIDE ? PX_WIMAGE : 128], q_wide[Sh::HALVES][WIDE ? PX_QWIMAGE : 128];
+  uint8_t wide_of[TQ_D];                     // a channel's place among the wide ones, or 255
+  int wide_at[PX_WIDE];
   alignas(128) uint8_t lut_k[256 * ENTRY_K], lut_v[(VB == 4 ? 256 : 64) * ENTRY_V];
-  alignas(16) float scale[2][TQ_D], mean[2][TQ_D], center[TQ_D];  // of a page, lifted
+  alignas(16) float center[TQ_D];
   float2 of_tile[Sh::STAGES];                // the values' exponent, the keys' factor
-  float part_top[2][4][PX_T], top[2][8];
-  unsigned long long k_full[Sh::STAGES], v_full[Sh::STAGES], empty[Sh::STAGES], q_ready[2], s_full[2], s_read[2], p_full[2],
+  float top[2][8];
+  float k_up;                                // the factor of the CTA's keys
+  unsigned long long on_grid[Sh::STAGES], k_full[Sh::STAGES], v_full[Sh::STAGES], empty[Sh::STAGES], q_ready[2], s_full[2], s_read[2], p_full[2],
       o_done[2], drained[2];
   uint32_t tmem;
 };
@@ -60,12 +74,12 @@ struct PrefixArgs {
 
 TQ_DEV uint64_t px_lds64(uint32_t at) {
   uint64_t v;
-  asm("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(at));
+  asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(at));  // (volatile, here and below: so that a batch stays one)
   return v;
 }
 TQ_DEV uint32_t px_lds32(uint32_t at) {
   uint32_t v;
-  asm("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
   return v;
 }
 TQ_DEV void px_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -95,12 +109,15 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
     for (int r = tid; r < min(ROWS, a.rows - row0); r += PX_THREADS) *(float2*)slot_of(row0 + r) = make_float2(-INFINITY, 0.0f);
     return;
   }
+  const bool listed = !hot && g.outlier_k > 0;  // two warps put the outliers over the keys
+  const int held = blockIdx.x == 0 ? a.withhold : -1;  // test hook: a tile whose keys are never handed over
   const int groups = Sh::HALVES == 2 && a.rows - row0 > 128 ? 2 : 1;  // halves of the rows that there are
   const uint8_t* const pages = a.pages + page_offset(g, a.layer, a.seq_begin, head, 0);
 
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(enc_smem(&sh.k_full[i]), PX_MAKERS / 32);
+      mbar_init(enc_smem(&sh.on_grid[i]), PX_MAKERS / 32);
+      mbar_init(enc_smem(&sh.k_full[i]), listed ? 2 : PX_MAKERS / 32);
       mbar_init(enc_smem(&sh.v_full[i]), PX_MAKERS / 32);
       mbar_init(enc_smem(&sh.empty[i]), groups);
     }
@@ -137,7 +154,24 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
       }
     }
   }
-  if (tid < TQ_D) sh.center[tid] = sq.cold > 0 ? ti_center(g, pages, tid) : 0.0f;
+  if (tid < TQ_D) {
+    sh.center[tid] = sq.cold > 0 ? ti_center(g, pages, tid) : 0.0f;
+    if (!SPLIT) {  // the widest channels, the lower of two equal ones first
+      const float* scales = (const float*)(pages + g.scale_off);
+      const float mine = sq.cold > 0 ? scales[tid] : 0.0f;
+      int place = 0;
+      for (int d = 0; d < TQ_D; ++d) {
+        const float x = sq.cold > 0 ? scales[d] : 0.0f;
+        place += x > mine || (x == mine && d < tid);
+      }
+      sh.wide_of[tid] = place < PX_WIDE ? place : 255;
+      if (place < PX_WIDE) sh.wide_at[place] = tid;
+    }
+  }
+  if (!SPLIT) {
+    for (int i = tid; i < STAGES * PX_WIMAGE / 16; i += PX_THREADS) ((uint4*)sh.wide)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = tid; i < Sh::HALVES * PX_QWIMAGE / 16; i += PX_THREADS) ((uint4*)sh.q_wide)[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
   ti_fence_before();
   __syncthreads();
   ti_fence_after();
@@ -157,80 +191,80 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
   };
   auto wait = [&](unsigned long long* bar, unsigned parity) { wait_for(bar, parity, limit); };
 
-  if (warp >= PX_SOFTMAX / 32 + 2) {
-    // ---- the makers of the operands
-    const int pt = tid - PX_SOFTMAX - 64, pw = pt >> 5;
-    const int token = pt & (PX_T - 1), quarter = pt / PX_T;  // keys: 32 channels of a token
-    const int held = blockIdx.x == 0 ? a.withhold : -1;      // test hook: a tile whose keys are never handed over
+  auto hand_over = [&](unsigned long long* bar) {  // operands, by a warp
+    px_fence();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(enc_smem(bar));
+  };
+
+  if (warp >= (PX_SOFTMAX + PX_ISSUE) / 32) {
+    // ---- the makers of the operands (96 registers, as at launch)
+    const int pt = tid - PX_SOFTMAX - PX_ISSUE, pw = pt >> 5;
+    const int token = pt & (PX_T - 1), quarter = pt / PX_T;  // of a token: 32 channels (window), two wide channels
     bool odd = false;
-    auto hand_over = [&](unsigned long long* bar) {
-      px_fence();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(enc_smem(bar));
-    };
-    auto put_key = [&](uint8_t* to, int chunk, const float (&x)[8]) {
+    auto put_key = [&](uint8_t* to, int chunk, int token, const float (&x)[8]) {  // eight channels of a token
       const uint4 hi = {ti_pair(x[0], x[1]), ti_pair(x[2], x[3]), ti_pair(x[4], x[5]), ti_pair(x[6], x[7])};
       *(uint4*)(to + chunk * PX_KLBO + token * 16) = hi;
       if (SPLIT)
         *(uint4*)(to + PX_IMAGE + chunk * PX_KLBO + token * 16) =
             make_uint4(ti_rest(x[0], x[1], hi.x), ti_rest(x[2], x[3], hi.y), ti_rest(x[4], x[5], hi.z), ti_rest(x[6], x[7], hi.w));
     };
+    const int wide0 = SPLIT ? 0 : sh.wide_at[2 * quarter], wide1 = SPLIT ? 0 : sh.wide_at[2 * quarter + 1];
+    auto put_wide = [&](int stage, float x, float y) {  // lifted keys of channels wide0 and wide1
+      *(uint32_t*)(sh.wide[stage] + token * 16 + 4 * quarter) = ti_rest(x, y, ti_pair(x, y));
+    };
     if (!hot) {
-      const size_t uix = unit_index(g, a.layer, a.seq_begin, head);
-      const uint32_t* const dec = a.pool_dec + uix * (size_t)g.pool_entries;
-      const uint16_t* const val = a.pool_val + uix * (size_t)g.pool_entries;
-      const PageMeta* const metas = a.page_meta + uix * g.max_blocks;
-      const bool listed = g.outlier_k > 0;
-      const float gridmost = g.key_mode == TQ_KEYS_UNIFORM ? 15.0f : 1.0f;
       // two warps expand the records of a group of 16 tokens; a lane: pairs 16 half .. + 15 of a record
       const int grp = pw >> 1, half = pw & 1, r = lane >> 2, c = lane & 3;
-      uint4 codes;
-      uint32_t rec[4];
-      float2 norm2[2];
-      float2 norm_of;  // of tokens 2 lane, 2 lane + 1 of the strip
-      PageMeta meta = {0, 0};
-      auto fetch = [&](int j) {  // strip j's, on their way
-        const uint8_t* page = pages + (size_t)(j >> 2) * g.page_bytes;
-        const int ts = (j & 3) * PX_T;
-        codes = *(const uint4*)(page + (ts + token) * (TQ_D / 2) + 16 * quarter);
-        const uint8_t* from = page + g.v_off + (size_t)((ts >> 4) + grp) * VGB;
+      // Keys: a thread has eight channels, whose scales and zero-points stay in registers, of four tokens; neighbouring lanes
+      // have neighbouring tokens, so that eight of them write 128 bytes in a row.
+      const int chunk = 4 * (pw & 3) + (lane >> 3), token0 = 32 * (pw >> 2) + (lane & 7);
+      // What a tile needs is on its way while the tile before it is made.  (Without conditions: a value that may or may not have
+      // been loaded is moved, and so waited for, at once.)
+      uint32_t codes[4], wide_codes[2] = {0u, 0u}, rec[4];
+      float2 norm2[2], norm_of;  // of the group; of tokens 2 lane, 2 lane + 1 of the strip
+      float4 scale4[2], mean4[2];
+      auto page_of = [&](int j) { return pages + (size_t)(j >> 2) * g.page_bytes; };
+      auto fetch_keys = [&](int j) {
+        const uint8_t* row = page_of(j) + (j & 3) * PX_T * (TQ_D / 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) codes[i] = *(const uint32_t*)(row + (token0 + 8 * i) * (TQ_D / 2) + 4 * chunk);
+        if (!SPLIT)
+          wide_codes[0] = row[token * (TQ_D / 2) + (wide0 >> 1)], wide_codes[1] = row[token * (TQ_D / 2) + (wide1 >> 1)];
+      };
+      auto fetch_norms = [&](int j) { norm_of = *(const float2*)(page_of(j) + g.norm_off + ((j & 3) * PX_T + 2 * lane) * 4); };
+      auto fetch_values = [&](int j) {
+        const uint8_t* from = page_of(j) + g.v_off + (size_t)((j & 3) * (PX_T / TQ_GROUP_TOK) + grp) * VGB;
         if (VB == 4) {
           const uint4 x = *(const uint4*)(from + half * 512 + lane * 16);
           rec[0] = x.x, rec[1] = x.y, rec[2] = x.z, rec[3] = x.w;
-        } else {  // the record's 24 bytes; these pairs are words 3 half .. + 2
-          const uint2 r0 = *(const uint2*)(from + (half ? 256 : 0) + lane * 8), r1 = *(const uint2*)(from + (half ? 512 : 256) + lane * 8);
-          rec[0] = half ? r0.y : r0.x, rec[1] = half ? r1.x : r0.y, rec[2] = half ? r1.y : r1.x, rec[3] = 0u;
+        } else {  // words 3 half .. + 2 of the record's six, two of which are side by side
+          const uint8_t* at = from + lane * 8;
+          rec[0] = *(const uint32_t*)(at + (half ? 256 + 4 : 0)), rec[1] = *(const uint32_t*)(at + (half ? 512 : 4));
+          rec[2] = *(const uint32_t*)(at + (half ? 512 + 4 : 256)), rec[3] = 0u;
         }
-        const float* norms = (const float*)(page + g.norm_off) + ts;
-        norm2[0] = *(const float2*)(norms + 16 * grp + 2 * c), norm2[1] = *(const float2*)(norms + 16 * grp + 8 + 2 * c);
-        norm_of = *(const float2*)(norms + 2 * lane);
+        const float* norms = (const float*)(page_of(j) + g.norm_off) + (j & 3) * PX_T + 16 * grp + 2 * c;
+        norm2[0] = *(const float2*)norms, norm2[1] = *(const float2*)(norms + 8);
       };
-      float k_up = 1.0f, k_factor = 1.0f;
-      uint32_t of_list[PX_LIST];
-      uint16_t of_val[PX_LIST];
-      if (listed) meta = metas[k_lo >> 2];
-      fetch(k_lo);
-      int turn = 0;  // of the page's place in shared memory
-#pragma unroll 1
-      for (int k = 0; k < n; ++k) {
-        const int j = k_lo + k, stage = k % STAGES;
-        const uint8_t* const page = pages + (size_t)(j >> 2) * g.page_bytes;
-        if (k == 0 || (j & 3) == 0) {
-          // ---- a page: its scales and zero-points, its list
-          turn ^= 1;
-          const float4 s4 = *(const float4*)(page + g.scale_off + lane * 16), m4 = *(const float4*)(page + g.mean_off + lane * 16);
-          if (listed) {
-            if (k > 0) meta = metas[j >> 2];
-#pragma unroll
-            for (int i = 0; i < PX_LIST; ++i) {
-              const uint32_t e = pt + PX_MAKERS * i;
-              of_list[i] = 0xffffffffu, of_val[i] = 0;
-              if (e < meta.cnt) of_list[i] = dec[meta.off + e], of_val[i] = val[meta.off + e];
-            }
-          }
-          const float4 z4 = *(const float4*)&sh.center[4 * lane];
+      auto fetch_page = [&](int j) {
+        const float* s = (const float*)(page_of(j) + g.scale_off) + 8 * chunk;
+        const float* m = (const float*)(page_of(j) + g.mean_off) + 8 * chunk;
+        scale4[0] = *(const float4*)s, scale4[1] = *(const float4*)(s + 4);
+        mean4[0] = *(const float4*)m, mean4[1] = *(const float4*)(m + 4);
+      };
+      fetch_page(k_lo);
+      fetch_keys(k_lo);
+      fetch_norms(k_lo);
+      fetch_values(k_lo);
+      // ---- the largest and the least that a channel of the CTA's pages may have
+      float k_up, k_factor;
+      {
+        float most = 0.0f, least = INFINITY;
+        const float gridmost = g.key_mode == TQ_KEYS_UNIFORM ? 15.0f : 1.0f;
+        const float4 z4 = *(const float4*)&sh.center[4 * lane];
+        for (int j = (k_lo & ~3) + 4 * pw; j < k_lo + n; j += 4 * (PX_MAKERS / 32)) {
+          const float4 s4 = *(const float4*)(page_of(j) + g.scale_off + lane * 16), m4 = *(const float4*)(page_of(j) + g.mean_off + lane * 16);
           const float s[4] = {s4.x, s4.y, s4.z, s4.w}, m[4] = {m4.x - z4.x, m4.y - z4.y, m4.z - z4.z, m4.w - z4.w};
-          float most = 0.0f, least = INFINITY;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float x = fmaf(fabsf(s[i]), gridmost, fabsf(m[i]));
@@ -238,16 +272,38 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
             most = fmaxf(most, x);
             if (x > 0.0f) least = fminf(least, x);
           }
-          most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
-          odd |= least < most * TI_LEAST;
-          float exponent;
-          k_up = ti_lift(most, PX_TOP, exponent, 97);
-          k_factor = exp2f(exponent);
-          if (pw == 0) {
-            *(float4*)&sh.scale[turn][4 * lane] = make_float4(s[0] * k_up, s[1] * k_up, s[2] * k_up, s[3] * k_up);
-            *(float4*)&sh.mean[turn][4 * lane] = make_float4(m[0] * k_up, m[1] * k_up, m[2] * k_up, m[3] * k_up);
+        }
+        most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+        least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least)));
+        if (lane == 0) sh.top[0][pw] = most, sh.top[1][pw] = least;
+        px_makers();
+#pragma unroll
+        for (int i = 0; i < PX_MAKERS / 32; ++i) most = fmaxf(most, sh.top[0][i]), least = fminf(least, sh.top[1][i]);
+        odd |= least < most * TI_LEAST;
+        float exponent;
+        k_up = ti_lift(most, PX_TOP, exponent, 97);
+        k_factor = exp2f(exponent);
+        if (pt == 0) sh.k_up = k_up;  // (the outliers' warps read it behind the first tile)
+      }
+      uint64_t s2[4], m2[4];
+      float of_wide[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // scale and zero-point of the wide channels
+#pragma unroll 1
+      for (int k = 0; k < n; ++k) {
+        const int j = k_lo + k, stage = k % STAGES, next = min(j + 1, k_lo + n - 1);
+        if (k == 0 || (j & 3) == 0) {
+          const float4 z0 = *(const float4*)&sh.center[8 * chunk], z1 = *(const float4*)&sh.center[8 * chunk + 4];
+          s2[0] = ti_f2(scale4[0].x * k_up, scale4[0].y * k_up), s2[1] = ti_f2(scale4[0].z * k_up, scale4[0].w * k_up);
+          s2[2] = ti_f2(scale4[1].x * k_up, scale4[1].y * k_up), s2[3] = ti_f2(scale4[1].z * k_up, scale4[1].w * k_up);
+          m2[0] = ti_f2((mean4[0].x - z0.x) * k_up, (mean4[0].y - z0.y) * k_up);
+          m2[1] = ti_f2((mean4[0].z - z0.z) * k_up, (mean4[0].w - z0.w) * k_up);
+          m2[2] = ti_f2((mean4[1].x - z1.x) * k_up, (mean4[1].y - z1.y) * k_up);
+          m2[3] = ti_f2((mean4[1].z - z1.z) * k_up, (mean4[1].w - z1.w) * k_up);
+          if (!SPLIT) {
+            const float* s = (const float*)(page_of(j) + g.scale_off);
+            const float* m = (const float*)(page_of(j) + g.mean_off);
+            of_wide[0] = s[wide0] * k_up, of_wide[1] = s[wide1] * k_up;
+            of_wide[2] = (m[wide0] - sh.center[wide0]) * k_up, of_wide[3] = (m[wide1] - sh.center[wide1]) * k_up;
           }
-          px_makers();
         }
         if (k >= STAGES) wait(&sh.empty[stage], (k / STAGES - 1) & 1);
         __syncwarp();
@@ -263,85 +319,84 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
           v_up = ti_lift(most, 14, exponent);
           if (pt == 0) sh.of_tile[stage] = make_float2(exponent, k_factor);
         }
+        fetch_norms(next);
         {  // ---- keys
           const uint32_t lut = enc_smem(sh.lut_k) + (lane & 15) * 8;
-          const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-          const uint32_t of_scale = enc_smem(&sh.scale[turn][32 * quarter]), of_mean = enc_smem(&sh.mean[turn][32 * quarter]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint64_t s[4], m[4];
+          for (int i0 = 0; i0 < 4; i0 += 2) {  // (two tokens' look-ups at once)
+            uint64_t y[2][4];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              asm("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(s[2 * e]), "=l"(s[2 * e + 1]) : "r"(of_scale + 32 * i + 16 * e));
-              asm("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(m[2 * e]), "=l"(m[2 * e + 1]) : "r"(of_mean + 32 * i + 16 * e));
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[i][e] = px_lds64(__byte_perm(codes[i0 + i], 0, 0x4440 + e) * 128 + lut);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = ti_floats(ti_fma2(y[i][e], s2[e], m2[e]));
+                x[2 * e] = f.x, x[2 * e + 1] = f.y;
+              }
+              put_key(ki, chunk, token0 + 8 * (i0 + i), x);
             }
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t off = (e == 0 ? w[i] << 7 : w[i] >> (8 * e - 7)) & 0x7f80u;
-              const float2 f = ti_floats(ti_fma2(px_lds64(lut + off), s[e], m[e]));
-              x[2 * e] = f.x, x[2 * e + 1] = f.y;
-            }
-            put_key(ki, 4 * quarter + i, x);
+          }
+          if (!SPLIT) {
+            const float x = __uint_as_float(px_lds32(lut + (wide_codes[0] >> (4 * (wide0 & 1)) & 15u) * 128));
+            const float y = __uint_as_float(px_lds32(lut + (wide_codes[1] >> (4 * (wide1 & 1)) & 15u) * 128));
+            put_wide(stage, fmaf(x, of_wide[0], of_wide[2]), fmaf(y, of_wide[1], of_wide[3]));
           }
         }
-        uint32_t vw[4] = {rec[0], rec[1], rec[2], rec[3]};
-        const float2 nv[2] = {norm2[0], norm2[1]};
-        if (k + 1 < n) fetch(j + 1);
-        if (listed) {
-          px_makers();  // (the grid's part is there)
-          auto put = [&](uint32_t e, uint16_t v) {
-            const int t = (int)(e >> 24), ch = (int)(e >> 16) & 127;
-            if (t >> 6 != (j & 3)) return;
-            const float x = (__half2float(__ushort_as_half(v)) - sh.center[ch]) * k_up;
-            odd |= !(fabsf(x) < 32768.0f);
-            const __half hi = __float2half_rn(x);
-            uint8_t* to = ki + (ch >> 3) * PX_KLBO + (t & (PX_T - 1)) * 16 + (ch & 7) * 2;
-            *(__half*)to = hi;
-            if (SPLIT) *(__half*)(to + PX_IMAGE) = __float2half_rn(x - __half2float(hi));
-          };
-#pragma unroll
-          for (int i = 0; i < PX_LIST; ++i)
-            if (pt + PX_MAKERS * i < meta.cnt) put(of_list[i], of_val[i]);
-          for (uint32_t e = pt + PX_MAKERS * PX_LIST; e < meta.cnt; e += PX_MAKERS) put(dec[meta.off + e], val[meta.off + e]);
-        }
-        if (k != held) hand_over(&sh.k_full[stage]);
+        if (listed) hand_over(&sh.on_grid[stage]);
+        else if (k != held) hand_over(&sh.k_full[stage]);
+        fetch_keys(next);
+        if ((next & 3) == 0) fetch_page(next);
         {  // ---- values
           const uint32_t lut = enc_smem(sh.lut_v) + (lane % (SPLIT ? Shared::ENTRY_V / 8 : Shared::ENTRY_V / 4)) * (SPLIT ? 8 : 4);
           uint32_t n2[2];
           uint64_t f2[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            n2[h] = ti_pair(nv[h].x * v_up, nv[h].y * v_up);
-            f2[h] = ti_f2(nv[h].x * v_up, nv[h].y * v_up);
+            n2[h] = ti_pair(norm2[h].x * v_up, norm2[h].y * v_up);
+            f2[h] = ti_f2(norm2[h].x * v_up, norm2[h].y * v_up);
           }
+          constexpr int AT_ONCE = SPLIT ? 4 : 8;
 #pragma unroll
-          for (int p = 0; p < 16; ++p) {
-            const int h = p & 1, d = r + 8 * (8 * half + (p >> 1));
-            uint32_t off;
-            if (VB == 4) off = ((p & 3) == 0 ? vw[p >> 2] << 6 : vw[p >> 2] >> (8 * (p & 3) - 6)) & 0x3fc0u;
-            else off = (__funnelshift_r(vw[6 * p >> 5], vw[min((6 * p >> 5) + 1, 3)], (6 * p) & 31) & 63u) * Shared::ENTRY_V;
-            uint8_t* const to = vi + (2 * grp + h) * PX_LBO + d * 16 + 4 * c;
-            if (SPLIT) {
-              const float2 f = ti_floats(ti_fma2(px_lds64(lut + off), f2[h], 0ull));
-              const uint32_t hi = ti_pair(f.x, f.y);
-              *(uint32_t*)to = hi;
-              *(uint32_t*)(to + PX_IMAGE) = ti_rest(f.x, f.y, hi);
-            } else {
-              const uint32_t y = px_lds32(lut + off);
-              const __half2 v = __hmul2(*(const __half2*)&y, *(const __half2*)&n2[h]);
-              *(uint32_t*)to = *(const uint32_t*)&v;
+          for (int p0 = 0; p0 < 16; p0 += AT_ONCE) {
+            uint64_t y[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+              const int p = p0 + i, at = 6 * p;
+              const uint32_t code = VB == 4 ? __byte_perm(rec[p >> 2], 0, 0x4440 + (p & 3))
+                                            : __funnelshift_r(rec[at >> 5], rec[min((at >> 5) + 1, 3)], at & 31) & 63u;
+              y[i] = SPLIT ? px_lds64(code * Shared::ENTRY_V + lut) : px_lds32(code * Shared::ENTRY_V + lut);
+            }
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+              const int p = p0 + i, h = p & 1, d = r + 8 * (8 * half + (p >> 1));
+              uint8_t* const to = vi + (2 * grp + h) * PX_LBO + d * 16 + 4 * c;
+              if (SPLIT) {
+                const float2 f = ti_floats(ti_fma2(y[i], f2[h], 0ull));
+                const uint32_t hi = ti_pair(f.x, f.y);
+                *(uint32_t*)to = hi;
+                *(uint32_t*)(to + PX_IMAGE) = ti_rest(f.x, f.y, hi);
+              } else {
+                const uint32_t w = (uint32_t)y[i];
+                const __half2 v = __hmul2(*(const __half2*)&w, *(const __half2*)&n2[h]);
+                *(uint32_t*)to = *(const uint32_t*)&v;
+              }
             }
           }
         }
+        fetch_values(next);
         hand_over(&sh.v_full[stage]);
       }
     } else {
       // ---- the uncompressed window: a thread has a quarter of a token's channels
       const size_t ring = hot_offset_elems(g, a.layer, a.seq_begin, head);
+      float(*const part_top)[4][PX_T] = (float(*)[4][PX_T])sh.lut_k;  // (the window has no use for the tables)
       // the largest of a tile; whether a token lies far below it, or something is no number
       auto largest = [&](float most, int which) {
-        sh.part_top[which][quarter][token] = most;
+        part_top[which][quarter][token] = most;
         const float mine = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
         if (lane == 0) sh.top[which][pw] = mine;
         px_makers();
@@ -349,7 +404,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, sh.top[which][i]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) of_token = fmaxf(of_token, sh.part_top[which][i][token]);
+        for (int i = 0; i < 4; ++i) of_token = fmaxf(of_token, part_top[which][i][token]);
         odd |= of_token > 0.0f && of_token < top * TI_LEAST;
         return top;
       };
@@ -360,14 +415,16 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
         __syncwarp();
         uint8_t* const ki = sh.kv[stage][0];
         uint8_t* const vi = sh.kv[stage][PARTS];
-        const size_t at = ring + (size_t)(t % g.hot_cap) * TQ_D + 32 * quarter;
-        float x[4][8], most = 0.0f, exponent, k_exponent;
+        const size_t row = ring + (size_t)(t % g.hot_cap) * TQ_D, at = row + 32 * quarter;
+        const bool there = t < sq.n;
+        float x[4][8], most = 0.0f, exponent, k_exponent, of_wide[2] = {0.0f, 0.0f};
+        if (!SPLIT && there) of_wide[0] = attend_ld(a.hot_k, row + wide0, g.kv_dtype), of_wide[1] = attend_ld(a.hot_k, row + wide1, g.kv_dtype);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (t < sq.n) ti_ld8(a.hot_k, at + 8 * i, g.kv_dtype, x[i]);
+          if (there) ti_ld8(a.hot_k, at + 8 * i, g.kv_dtype, x[i]);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            x[i][e] = t < sq.n ? x[i][e] - sh.center[32 * quarter + 8 * i + e] : 0.0f;
+            x[i][e] = there ? x[i][e] - sh.center[32 * quarter + 8 * i + e] : 0.0f;
             odd |= !(fabsf(x[i][e]) < TI_KEY_MOST);
             most = fmaxf(most, fabsf(x[i][e]));
           }
@@ -377,15 +434,17 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[i][e] *= k_up;
-          put_key(ki, 4 * quarter + i, x[i]);
+          put_key(ki, 4 * quarter + i, token, x[i]);
         }
+        if (!SPLIT)
+          put_wide(stage, there ? (of_wide[0] - sh.center[wide0]) * k_up : 0.0f, there ? (of_wide[1] - sh.center[wide1]) * k_up : 0.0f);
         most = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (t < sq.n) ti_ld8(a.hot_v, at + 8 * i, g.kv_dtype, x[i]);
+          if (there) ti_ld8(a.hot_v, at + 8 * i, g.kv_dtype, x[i]);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            x[i][e] = t < sq.n ? x[i][e] : 0.0f;
+            x[i][e] = there ? x[i][e] : 0.0f;
             odd |= !(fabsf(x[i][e]) < INFINITY);
             most = fmaxf(most, fabsf(x[i][e]));
           }
@@ -408,6 +467,57 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
     }
     if (odd) pa.left[head] = 1;
   } else if (warp >= PX_SOFTMAX / 32) {
+    // (the whole warpgroup, and where its paths part, not before: the compiler allocates by what it sees on a path)
+    PX_REGISTERS("dec", "48");
+    if (warp >= PX_SOFTMAX / 32 + 2) {
+    // ---- outliers: two warps hold a page's list, ordered by token, and put those of a tile over its keys
+    if (listed) {
+      const int at = tid - PX_SOFTMAX - 64;
+      const size_t uix = unit_index(g, a.layer, a.seq_begin, head);
+      const uint32_t* const dec = a.pool_dec + uix * (size_t)g.pool_entries;
+      const uint16_t* const val = a.pool_val + uix * (size_t)g.pool_entries;
+      PageMeta meta = {0, 0};
+      uint32_t of_list[PX_LIST];
+      uint16_t of_val[PX_LIST];
+      float k_up = 0.0f;
+      bool odd = false;
+#pragma unroll 1
+      for (int k = 0; k < n; ++k) {
+        const int j = k_lo + k, stage = k % STAGES;
+        if (k == 0 || (j & 3) == 0) {
+          meta = a.page_meta[uix * g.max_blocks + (j >> 2)];
+#pragma unroll
+          for (int i = 0; i < PX_LIST; ++i) {
+            const uint32_t e = at + 64 * i;
+            of_list[i] = 0u, of_val[i] = 0;
+            if (e < meta.cnt) of_list[i] = dec[meta.off + e], of_val[i] = val[meta.off + e];
+          }
+        }
+        wait(&sh.on_grid[stage], (k / STAGES) & 1);
+        __syncwarp();
+        if (k == 0) k_up = sh.k_up;
+        uint8_t* const ki = sh.kv[stage][0];
+        auto put = [&](uint32_t e, uint16_t v) {
+          const int t = (int)(e >> 24), ch = (int)(e >> 16) & 127;
+          if (t >> 6 != (j & 3)) return;
+          const float x = (__half2float(__ushort_as_half(v)) - sh.center[ch]) * k_up;
+          odd |= !(fabsf(x) < 32768.0f);
+          const __half hi = __float2half_rn(x);
+          uint8_t* to = ki + (ch >> 3) * PX_KLBO + (t & (PX_T - 1)) * 16 + (ch & 7) * 2;
+          *(__half*)to = hi;
+          if (SPLIT) *(__half*)(to + PX_IMAGE) = __float2half_rn(x - __half2float(hi));
+          else if (sh.wide_of[ch] < PX_WIDE)
+            *(__half*)(sh.wide[stage] + (t & (PX_T - 1)) * 16 + 2 * sh.wide_of[ch]) = __float2half_rn(x - __half2float(hi));
+        };
+#pragma unroll
+        for (int i = 0; i < PX_LIST; ++i)
+          if (at + 64 * i < meta.cnt) put(of_list[i], of_val[i]);
+        for (uint32_t e = at + 64 * PX_LIST; e < meta.cnt; e += 64) put(dec[meta.off + e], val[meta.off + e]);
+        if (k != held) hand_over(&sh.k_full[stage]);
+      }
+      if (odd) pa.left[head] = 1;
+    }
+    } else {
     // ---- products of half x: the whole warp runs this, one thread issues
     const int x = warp - PX_SOFTMAX / 32, n_u = __shfl_sync(0xffffffffu, x < groups ? n : 0, 0);
     if (n_u > 0) {
@@ -417,6 +527,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
       const uint64_t q = umma_desc_k_major(enc_smem(sh.q[0]), PX_LBO, PX_SBO) + (uint64_t)(x * (PX_QIMAGE >> 4));
       const uint64_t k0 = umma_desc_k_major(enc_smem(sh.kv[0][0]), PX_KLBO, PX_SBO);
       const uint64_t v0 = umma_desc_k_major(enc_smem(sh.kv[0][PARTS]), PX_LBO, PX_SBO);
+      const uint64_t q_wide = umma_desc_k_major(enc_smem(sh.q_wide[0]), PX_QWLBO, PX_SBO) + (uint64_t)(x * (PX_QWIMAGE >> 4));
+      const uint64_t k_wide = umma_desc_k_major(enc_smem(sh.wide[0]), PX_WLBO, PX_SBO);
       const uint32_t ds = tmem + PX_HALF * x, dp = tmem + PX_P + PX_HALF * x, d_o = tmem + PX_O + 128 * x;
       auto image = [&](int k, int part) { return (uint64_t)((uint32_t)(k % STAGES) * (2 * PARTS * PX_IMAGE >> 4) + part * (PX_IMAGE >> 4)); };
       auto wait_all = [&](unsigned long long* bar, unsigned parity) {  // (the warp stays together)
@@ -434,6 +546,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
           if (SPLIT)
 #pragma unroll
             for (int j = 0; j < 8; ++j) ti_mma<true>(ds, q + j * STEP, b[0] + j * KSTEP, s_desc);
+          else
+            ti_mma<true>(ds, q_wide, k_wide + (uint64_t)((uint32_t)(k % STAGES) * (PX_WIMAGE >> 4)), s_desc);
           umma_commit(enc_smem(&sh.s_full[x]));
         }
         __syncwarp();
@@ -480,7 +594,10 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
       gave_up = false;
       wait_for(&sh.drained[x], 0, TI_WAIT);
     }
-  } else if (warp < 4 * groups) {
+    }
+  } else {
+    PX_REGISTERS("inc", "120");
+    if (warp < 4 * groups) {
     // ---- a thread per row
     const int x = warp >> 2, r = tid & 127, row = row0 + 128 * x + r;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -529,6 +646,12 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
         }
         *(uint4*)(sh.q[x] + i * PX_LBO + r * 16) = make_uint4(h[0], h[1], h[2], h[3]);
       }
+      if (!SPLIT)
+#pragma unroll
+        for (int i = 0; i < PX_WIDE; ++i) {
+          const int d = sh.wide_at[i];
+          *(uint16_t*)(sh.q_wide[x] + r * 16 + 2 * i) = *(const uint16_t*)(sh.q[x] + (d >> 3) * PX_LBO + r * 16 + (d & 7) * 2);
+        }
       px_fence();
       mbar_arrive(enc_smem(&sh.q_ready[x]));
     }
@@ -587,15 +710,18 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
       const float off = TI_LIFT + e - (m > -INFINITY ? m : 0.0f);
       const uint64_t factor2 = ti_f2(by, by), off2 = ti_f2(off, off);
       uint64_t sum[2] = {0ull, 0ull};
-      uint32_t h[PX_T / 2];
 #pragma unroll
-      for (int j = 0; j < PX_T / 2; ++j) {
-        const uint64_t y = ti_fma2(ti_u2(v[2 * j], v[2 * j + 1]), factor2, off2);
-        const float2 z = j % 8 < PX_POLY ? ti_exp2_poly(y) : ti_exp2_unit(y);
-        sum[j & 1] = ti_add2(sum[j & 1], ti_f2(z.x, z.y));
-        h[j] = ti_pair(z.x, z.y);
+      for (int i = 0; i < PX_T / 2; i += 8) {
+        uint32_t h[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint64_t y = ti_fma2(ti_u2(v[2 * (i + j)], v[2 * (i + j) + 1]), factor2, off2);
+          const float2 z = ti_exp2_unit(y);
+          sum[j & 1] = ti_add2(sum[j & 1], ti_f2(z.x, z.y));
+          h[j] = ti_pair(z.x, z.y);
+        }
+        ti_st8(tp + i, h);
       }
-      ti_st32(tp, h);
       if (groups == 2 && (x == 0 || k + 1 < n)) asm volatile("bar.arrive %0, 256;" ::"r"(2 - x) : "memory");
       ti_wait_st();
       ti_fence_before();
@@ -614,6 +740,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
       if (row < a.rows)
 #pragma unroll
         for (int j = 0; j < 16; j += 4) *(uint4*)(slot + 4 + 16 * i + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+    }
     }
   }
   __syncwarp();
@@ -730,11 +857,11 @@ void tq_attend_shared_plan(const AttendArgs& a, int tokens, int* ns_cold, int* n
   const int64_t units = (int64_t)g.n_kv_heads * ((a.rows + rows_of_cta(a) - 1) / rows_of_cta(a));
   int64_t best = INT64_MAX;
   *ns_cold = *ns_hot = 1;
-  for (int64_t each = 1; each <= std::max(cold, hot); ++each) {  // tiles of a CTA
-    const int64_t nc = std::max<int64_t>((cold + each - 1) / each, 1), nh = std::max<int64_t>((hot + each - 1) / each, 1);
+  for (int64_t each = 1; each <= std::max<int64_t>(cold, 2 * hot); ++each) {  // tiles of a CTA; one of the window takes twice as long
+    const int64_t nc = std::max<int64_t>((cold + each - 1) / each, 1), nh = std::max<int64_t>((2 * hot + each - 1) / each, 1);
     if (nc + nh > 256) continue;
     const int64_t time = (units * (nc + nh) + a.sm_count - 1) / a.sm_count * (each + 6);
-    if (time < best) best = time, *ns_cold = (int)nc, *ns_hot = (int)nh;
+    if (time < best) best = time, *ns_cold = (int)nc, *ns_hot = (int)std::min(nh, hot);
   }
 }
 
