@@ -29,13 +29,13 @@ constexpr int PX_S = 256;                    // tokens of a page
 constexpr int PX_IMAGE = PX_T * TQ_D * 2, PX_QIMAGE = 128 * TQ_D * 2;
 constexpr int PX_KLBO = PX_T * 16, PX_LBO = TQ_D * 16, PX_SBO = 128;  // from eight K to the next: keys; queries, values
 // Warps: eight of softmax, two that issue products, two that put the outliers over the keys, eight that make operands.  A
-// thread's registers, 96 at launch, are divided anew by warpgroup: 120, 48 and 96 (two, one and two groups: 480 = 5 x 96).
+// thread's registers, 96 at launch, are divided anew by warpgroup: 120, 64 and 88 (two, one and two groups: 480 = 5 x 96).
 constexpr int PX_SOFTMAX = 256, PX_ISSUE = 128, PX_MAKERS = 256, PX_THREADS = PX_SOFTMAX + PX_ISSUE + PX_MAKERS;
 #define PX_REGISTERS(how, n) asm volatile("setmaxnreg." how ".sync.aligned.u32 " n ";")
 constexpr int PX_P = PX_T, PX_HALF = 128, PX_O = 256;  // tensor memory's columns, as in the form for many rows
 constexpr int PX_STRIDE = 4 + TQ_D;          // floats of a state: M, L, -, -, o
 constexpr int PX_TOP = 8;                    // a page's largest key on the grid is lifted to 2^8 .. 2^9
-constexpr int PX_LIST = 10;                  // entries of a page's list that a thread holds
+constexpr int PX_LIST = 7;                   // outliers of a tile that a lane holds (160 of a tile are usual)
 constexpr int PX_WIDE = 8;                   // channels whose keys are two parts
 constexpr int PX_WLBO = PX_T * 16, PX_WIMAGE = 2 * PX_WLBO, PX_QWLBO = 128 * 16, PX_QWIMAGE = 2 * PX_QWLBO;
 
@@ -54,7 +54,8 @@ struct PxShared {
   alignas(128) uint8_t kv[Sh::STAGES][2 * Sh::PARTS][PX_IMAGE];
   // the second parts of the wide channels (a step of 16 channels, the other eight of which stay zero), and their queries
   alignas(128) uint8_t wide[Sh::STAGES][WIDE ? PX_WIMAGE : 128], q_wide[Sh::HALVES][WIDE ? PX_QWIMAGE : 128];
-  uint8_t wide_of[TQ_D];                     // a channel's place among the wide ones, or 255
+  float levels[32];                          // of the keys' grid, of the values' codebook
+  uint8_t wide_of[TQ_D];                     // a channel's place among the wide ones, or 255: none
   int wide_at[PX_WIDE];
   alignas(128) uint8_t lut_k[256 * ENTRY_K], lut_v[(VB == 4 ? 256 : 64) * ENTRY_V];
   alignas(16) float center[TQ_D];
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(enc_smem(&sh.on_grid[i]), PX_MAKERS / 32);
-      mbar_init(enc_smem(&sh.k_full[i]), listed ? 2 : PX_MAKERS / 32);
+      mbar_init(enc_smem(&sh.k_full[i]), listed ? 1 : PX_MAKERS / 32);
       mbar_init(enc_smem(&sh.v_full[i]), PX_MAKERS / 32);
       mbar_init(enc_smem(&sh.empty[i]), groups);
     }
@@ -135,46 +136,105 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(enc_smem(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // ---- tables: an entry's copies side by side, so that the lanes of a look-up meet different banks
-  if (!hot) {
-    for (int e = tid; e < 256 * 8; e += PX_THREADS) {  // two copies at a time
-      const int b = e >> 3;
-      const float x = a.tables->grid[b & 15], y = a.tables->grid[b >> 4];
-      *(float4*)(sh.lut_k + e * 16) = make_float4(x, y, x, y);
-    }
-    constexpr int NV = VB == 4 ? 256 : 64, PER = Shared::ENTRY_V / 16;
-    for (int e = tid; e < NV * PER; e += PX_THREADS) {
-      const int b = e / PER;
-      const float x = a.tables->centroids[b & ((1 << VB) - 1)], y = a.tables->centroids[b >> VB];
-      if (SPLIT) {
-        *(float4*)(sh.lut_v + e * 16) = make_float4(x, y, x, y);
-      } else {
-        const uint32_t h = ti_pair(x, y);
-        *(uint4*)(sh.lut_v + e * 16) = make_uint4(h, h, h, h);
-      }
-    }
-  }
-  if (tid < TQ_D) {
-    sh.center[tid] = sq.cold > 0 ? ti_center(g, pages, tid) : 0.0f;
-    if (!SPLIT) {  // the widest channels, the lower of two equal ones first
-      const float* scales = (const float*)(pages + g.scale_off);
-      const float mine = sq.cold > 0 ? scales[tid] : 0.0f;
-      int place = 0;
-      for (int d = 0; d < TQ_D; ++d) {
-        const float x = sq.cold > 0 ? scales[d] : 0.0f;
-        place += x > mine || (x == mine && d < tid);
-      }
-      sh.wide_of[tid] = place < PX_WIDE ? place : 255;
-      if (place < PX_WIDE) sh.wide_at[place] = tid;
-    }
-  }
-  if (!SPLIT) {
-    for (int i = tid; i < STAGES * PX_WIMAGE / 16; i += PX_THREADS) ((uint4*)sh.wide)[i] = make_uint4(0u, 0u, 0u, 0u);
-    for (int i = tid; i < Sh::HALVES * PX_QWIMAGE / 16; i += PX_THREADS) ((uint4*)sh.q_wide)[i] = make_uint4(0u, 0u, 0u, 0u);
+  // ---- what the roles need, in two steps: from memory, and from what is then in shared memory.  (Loops, not unrolled: code that
+  // runs once is waited for from memory, 700 instructions for 10 000 cycles.)  Queries: a thread per row.
+  float factor = 0.0f, shift = 0.0f;  // of a row's scores; what the keys' common vector takes off them
+  if (warp < 4 * groups) {
+    const int row = row0 + tid;
+    const bool there = row < a.rows;
+    const uint16_t* q = (const uint16_t*)a.q;
+    if (there) q += (int64_t)(row / G) * a.q_tok + (int64_t)(head * G + row % G) * a.q_head;
+    const uint32_t to = enc_smem(sh.q[warp >> 2] + (tid & 127) * 16);
+#pragma unroll 2
+    for (int i = 0; i < 16; ++i)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * PX_LBO), "l"(q + 8 * i), "r"(there ? 16 : 0) : "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");  // (each thread its own row)
+  } else if (warp >= PX_SOFTMAX / 32 && warp < (PX_SOFTMAX + PX_ISSUE) / 32) {
+    const int d = tid - PX_SOFTMAX;
+    static_assert(PX_ISSUE == TQ_D, "a thread per channel");
+    sh.center[d] = sq.cold > 0 ? ti_center(g, pages, d) : 0.0f;
+    const float scale = sq.cold > 0 ? ((const float*)(pages + g.scale_off))[d] : 0.0f;
+    ((float*)sh.kv[0])[d] = scale < INFINITY ? scale : 0.0f;  // (numbers: places below are a permutation)
+  } else if (warp >= (PX_SOFTMAX + PX_ISSUE) / 32 && tid < PX_SOFTMAX + PX_ISSUE + 32) {
+    const int i = tid & 31;
+    sh.levels[i] = i < 16 ? a.tables->grid[i] : a.tables->centroids[i - 16];
   }
   ti_fence_before();
   __syncthreads();
   ti_fence_after();
+  if (warp < 4 * groups) {
+    uint8_t* const from = sh.q[warp >> 2] + (tid & 127) * 16;
+    auto pairs = [&](const uint4& w, float2 (&f)[4]) {
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        f[j] = SPLIT ? __half22float2(*(const __half2*)&u[j]) : make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u));
+    };
+    float top = 0.0f;
+    uint64_t part[2] = {0ull, 0ull};
+#pragma unroll 2
+    for (int i = 0; i < 16; ++i) {
+      float2 f[4];
+      pairs(*(const uint4*)(from + i * PX_LBO), f);
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        const float4 z = *(const float4*)&sh.center[8 * i + 2 * j];
+        top = ti_max3(ti_max3(top, fabsf(f[j].x), fabsf(f[j].y)), fabsf(f[j + 1].x), fabsf(f[j + 1].y));
+        part[0] = ti_fma2(ti_f2(f[j].x, f[j].y), ti_f2(z.x, z.y), part[0]);
+        part[1] = ti_fma2(ti_f2(f[j + 1].x, f[j + 1].y), ti_f2(z.z, z.w), part[1]);
+      }
+    }
+    const float2 of_center = ti_floats(ti_add2(part[0], part[1]));
+    shift = tq_scaled<true>(of_center.x + of_center.y);
+    float exponent;
+    const float up = ti_lift(top, 13, exponent);
+    factor = tq_scaled<true>(exp2f(exponent));
+#pragma unroll 2
+    for (int i = 0; i < 16; ++i) {
+      float2 f[4];
+      pairs(*(const uint4*)(from + i * PX_LBO), f);
+      *(uint4*)(from + i * PX_LBO) = make_uint4(ti_pair(f[0].x * up, f[0].y * up), ti_pair(f[1].x * up, f[1].y * up),
+                                                ti_pair(f[2].x * up, f[2].y * up), ti_pair(f[3].x * up, f[3].y * up));
+    }
+  } else if (warp >= (PX_SOFTMAX + PX_ISSUE) / 32) {
+    if (!hot) {  // tables: an entry's copies side by side, so that the lanes of a look-up meet different banks
+      const int pt = tid - PX_SOFTMAX - PX_ISSUE;
+      for (int e = pt; e < 256 * 8; e += PX_MAKERS) {  // two copies at a time
+        const int b = e >> 3;
+        const float x = sh.levels[b & 15], y = sh.levels[b >> 4];
+        *(float4*)(sh.lut_k + e * 16) = make_float4(x, y, x, y);
+      }
+      constexpr int NV = VB == 4 ? 256 : 64, PER = Shared::ENTRY_V / 16;
+      for (int e = pt; e < NV * PER; e += PX_MAKERS) {
+        const int b = e / PER;
+        const float x = sh.levels[16 + (b & ((1 << VB) - 1))], y = sh.levels[16 + (b >> VB)];
+        if (SPLIT) {
+          *(float4*)(sh.lut_v + e * 16) = make_float4(x, y, x, y);
+        } else {
+          const uint32_t h = ti_pair(x, y);
+          *(uint4*)(sh.lut_v + e * 16) = make_uint4(h, h, h, h);
+        }
+      }
+    }
+  } else if (!SPLIT && warp >= PX_SOFTMAX / 32) {
+    // the widest channels, the lower of two equal ones first
+    const int d = tid - PX_SOFTMAX;
+    const float* scales = (const float*)sh.kv[0];
+    const float mine = scales[d];
+    int place = 0;
+#pragma unroll 4
+    for (int i = 0; i < TQ_D; i += 4) {
+      const float4 x = *(const float4*)(scales + i);
+      place += (x.x > mine || (x.x == mine && i < d)) + (x.y > mine || (x.y == mine && i + 1 < d)) +
+               (x.z > mine || (x.z == mine && i + 2 < d)) + (x.w > mine || (x.w == mine && i + 3 < d));
+    }
+    sh.wide_of[d] = place < PX_WIDE ? place : 255;
+    if (place < PX_WIDE) sh.wide_at[place] = d;
+    for (int i = d; i < STAGES * PX_WIMAGE / 16; i += PX_ISSUE) ((uint4*)sh.wide)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = d; i < Sh::HALVES * PX_QWIMAGE / 16; i += PX_ISSUE) ((uint4*)sh.q_wide)[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  px_fence();
+  __syncthreads();
   constexpr uint32_t tmem = 0;  // (all 512 columns are this CTA's: they begin at the first)
 
   // Bounded waits: one that runs out sets the status bit, and the thread then waits for nothing more and starts no
@@ -198,7 +258,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
   };
 
   if (warp >= (PX_SOFTMAX + PX_ISSUE) / 32) {
-    // ---- the makers of the operands (96 registers, as at launch)
+    // ---- the makers of the operands
+    PX_REGISTERS("dec", "88");
     const int pt = tid - PX_SOFTMAX - PX_ISSUE, pw = pt >> 5;
     const int token = pt & (PX_T - 1), quarter = pt / PX_T;  // of a token: 32 channels (window), two wide channels
     bool odd = false;
@@ -468,52 +529,90 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
     if (odd) pa.left[head] = 1;
   } else if (warp >= PX_SOFTMAX / 32) {
     // (the whole warpgroup, and where its paths part, not before: the compiler allocates by what it sees on a path)
-    PX_REGISTERS("dec", "48");
+    PX_REGISTERS("dec", "64");
     if (warp >= PX_SOFTMAX / 32 + 2) {
-    // ---- outliers: two warps hold a page's list, ordered by token, and put those of a tile over its keys
+    // ---- outliers: two warps, a tile each in turn, put the entries of the page's list, which is ordered by token, over its keys
     if (listed) {
-      const int at = tid - PX_SOFTMAX - 64;
+      const int hw = warp - PX_SOFTMAX / 32 - 2;
       const size_t uix = unit_index(g, a.layer, a.seq_begin, head);
-      const uint32_t* const dec = a.pool_dec + uix * (size_t)g.pool_entries;
-      const uint16_t* const val = a.pool_val + uix * (size_t)g.pool_entries;
-      PageMeta meta = {0, 0};
-      uint32_t of_list[PX_LIST];
-      uint16_t of_val[PX_LIST];
       float k_up = 0.0f;
       bool odd = false;
+      wait(&sh.on_grid[0], 0);  // (the factor is there)
+      __syncwarp();
+      k_up = sh.k_up;
+      const PageMeta* const metas = a.page_meta + uix * g.max_blocks;
+      // Where a tile's entries begin: behind the last of 32 samples of the page's list that is before it.  (The samples are those of
+      // a page, and they are asked for ahead, as are its place and length: three loads that wait for one another otherwise.)
+      PageMeta meta = {0, 0}, meta_next = {0, 0};
+      int sample = 4;
+      auto open_page = [&]() {
+        const uint32_t e = lane * ((meta.cnt + 31) / 32);
+        sample = 4;
+        if (e < meta.cnt) sample = (int)(a.pool_dec[uix * (size_t)g.pool_entries + meta.off + e] >> 30);
+      };
+      if (hw < n) {
+        meta = metas[(k_lo + hw) >> 2];
+        open_page();
+      }
 #pragma unroll 1
-      for (int k = 0; k < n; ++k) {
-        const int j = k_lo + k, stage = k % STAGES;
-        if (k == 0 || (j & 3) == 0) {
-          meta = a.page_meta[uix * g.max_blocks + (j >> 2)];
+      for (int k = hw; k < n; k += 2) {
+        const int j = k_lo + k, stage = k % STAGES, strip = j & 3;
+        const uint32_t* const dec = a.pool_dec + uix * (size_t)g.pool_entries + meta.off;
+        const uint16_t* const val = a.pool_val + uix * (size_t)g.pool_entries + meta.off;
+        const int before = __popc(__ballot_sync(0xffffffffu, sample < strip));
+        const uint32_t first = before > 0 ? (before - 1) * ((meta.cnt + 31) / 32) : 0u;
+        uint32_t key[PX_LIST], rest[PX_LIST];
 #pragma unroll
-          for (int i = 0; i < PX_LIST; ++i) {
-            const uint32_t e = at + 64 * i;
-            of_list[i] = 0u, of_val[i] = 0;
-            if (e < meta.cnt) of_list[i] = dec[meta.off + e], of_val[i] = val[meta.off + e];
-          }
+        for (int i = 0; i < PX_LIST; ++i) {
+          key[i] = rest[i] = 0u;
+          const uint32_t at = first + 32 * i + lane;
+          if (at < meta.cnt) key[i] = dec[at], rest[i] = val[at];
         }
-        wait(&sh.on_grid[stage], (k / STAGES) & 1);
-        __syncwarp();
-        if (k == 0) k_up = sh.k_up;
+        const bool turn = k + 2 < n && (j + 2) >> 2 != j >> 2;
+        if (turn) meta_next = metas[(j + 2) >> 2];
+        // (whether the last entry held may be followed by more of the tile's)
+        const bool more = __shfl_sync(0xffffffffu, first + 32 * PX_LIST < meta.cnt && (int)(key[PX_LIST - 1] >> 30) <= strip, 31);
+        // An entry as it is put: its place in the tile's image | the key; the key's second part | the channel's place among the
+        // wide ones, or 256: none of the tile's.
+        auto prepare = [&](uint32_t& key, uint32_t& rest, bool there) {
+          const uint32_t t = key >> 24, ch = key >> 16 & 127u;
+          const float x = (__half2float(__ushort_as_half((unsigned short)rest)) - sh.center[ch]) * k_up;
+          there = there && t >> 6 == (uint32_t)strip;
+          odd |= there && !(fabsf(x) < 32768.0f);
+          const __half hi = __float2half_rn(x), lo = __float2half_rn(x - __half2float(hi));
+          key = (ch >> 3) * PX_KLBO + (t & (PX_T - 1)) * 16 + (ch & 7u) * 2 | (uint32_t)__half_as_ushort(hi) << 16;
+          rest = (uint32_t)__half_as_ushort(lo) << 16 | (there ? sh.wide_of[ch] : 256u);
+        };
+        static_assert(16 * PX_KLBO <= 65536 && PX_KLBO == 1024, "an entry's place");
         uint8_t* const ki = sh.kv[stage][0];
-        auto put = [&](uint32_t e, uint16_t v) {
-          const int t = (int)(e >> 24), ch = (int)(e >> 16) & 127;
-          if (t >> 6 != (j & 3)) return;
-          const float x = (__half2float(__ushort_as_half(v)) - sh.center[ch]) * k_up;
-          odd |= !(fabsf(x) < 32768.0f);
-          const __half hi = __float2half_rn(x);
-          uint8_t* to = ki + (ch >> 3) * PX_KLBO + (t & (PX_T - 1)) * 16 + (ch & 7) * 2;
-          *(__half*)to = hi;
-          if (SPLIT) *(__half*)(to + PX_IMAGE) = __float2half_rn(x - __half2float(hi));
-          else if (sh.wide_of[ch] < PX_WIDE)
-            *(__half*)(sh.wide[stage] + (t & (PX_T - 1)) * 16 + 2 * sh.wide_of[ch]) = __float2half_rn(x - __half2float(hi));
+        uint8_t* const wi = sh.wide[stage];
+        auto put = [&](uint32_t key, uint32_t rest) {
+          const uint32_t place = rest & 511u;
+          if (place < 256u) {
+            *(uint16_t*)(ki + (key & 0xffffu)) = (uint16_t)(key >> 16);
+            if (SPLIT) *(uint16_t*)(ki + PX_IMAGE + (key & 0xffffu)) = (uint16_t)(rest >> 16);
+          }
+          if (!SPLIT && place < PX_WIDE) *(uint16_t*)(wi + (key & 0x3f0u) + 2 * place) = (uint16_t)(rest >> 16);
         };
 #pragma unroll
-        for (int i = 0; i < PX_LIST; ++i)
-          if (at + 64 * i < meta.cnt) put(of_list[i], of_val[i]);
-        for (uint32_t e = at + 64 * PX_LIST; e < meta.cnt; e += 64) put(dec[meta.off + e], val[meta.off + e]);
+        for (int i = 0; i < PX_LIST; ++i) prepare(key[i], rest[i], first + 32 * i + lane < meta.cnt);
+        wait(&sh.on_grid[stage], (k / STAGES) & 1);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < PX_LIST; ++i) put(key[i], rest[i]);
+        if (more)
+          for (uint32_t at = first + 32 * PX_LIST + lane; at < meta.cnt; at += 32) {
+            uint32_t x = dec[at], y = val[at];
+            if ((int)(x >> 30) > strip) break;
+            prepare(x, y, true);
+            put(x, y);
+          }
+        __syncwarp();
         if (k != held) hand_over(&sh.k_full[stage]);
+        if (turn) {
+          meta = meta_next;
+          open_page();
+        }
       }
       if (odd) pa.left[head] = 1;
     }
@@ -608,44 +707,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
       __syncwarp();
       ti_fence_after();
     };
-    float factor, shift;
     {
-      uint4 raw[16];
-      const bool there = row < a.rows;
-      const uint16_t* q = (const uint16_t*)a.q + ((int64_t)(row / G) * a.q_tok + (int64_t)(head * G + row % G) * a.q_head);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) raw[i] = there ? *(const uint4*)(q + 8 * i) : make_uint4(0u, 0u, 0u, 0u);
-      auto pair = [&](uint32_t w) -> float2 {
-        if (SPLIT) return __half22float2(*(const __half2*)&w);
-        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-      };
-      float top = 0.0f, part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = pair(w[j]);
-          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-          // what the keys' common vector takes off this row's scores
-          part[j] = fmaf(f.x, sh.center[8 * i + 2 * j], fmaf(f.y, sh.center[8 * i + 2 * j + 1], part[j]));
-        }
-      }
-      shift = tq_scaled<true>((part[0] + part[1]) + (part[2] + part[3]));
-      float exponent;
-      const float up = ti_lift(top, 13, exponent);
-      factor = tq_scaled<true>(exp2f(exponent));
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-        uint32_t h[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = pair(w[j]);
-          h[j] = ti_pair(f.x * up, f.y * up);
-        }
-        *(uint4*)(sh.q[x] + i * PX_LBO + r * 16) = make_uint4(h[0], h[1], h[2], h[3]);
-      }
       if (!SPLIT)
 #pragma unroll
         for (int i = 0; i < PX_WIDE; ++i) {
@@ -730,16 +792,29 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
       l = fmaf(s2.x + s2.y, exp2f(-e), l * down);
     }
     settled(&sh.o_done[x], (n - 1) & 1);
-    float* const slot = slot_of(min(row, a.rows - 1));
-    if (row < a.rows) *(float2*)slot = make_float2(m - TI_LIFT + shift, l);
+    if (row < a.rows) *(float2*)slot_of(row) = make_float2(m - TI_LIFT + shift, l);
+    // The sums go through the queries' place, which the warp's rows have 64 columns at a time, so that half a warp writes 256
+    // bytes of a row in a row.  (The scores' products, which read it, are long done; the other half has a place of its own.)
+    uint8_t* const place = sh.q[x] + (warp & 3) * 8192;
+    auto at = [&](int r, int c4) { return (float4*)(place + r * 256 + ((c4 ^ (r & 15)) << 4)); };
 #pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-      uint32_t o[16];
-      ti_ld16(to + 16 * i, o);
-      ti_wait_ld();
-      if (row < a.rows)
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) *(uint4*)(slot + 4 + 16 * i + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+      for (int i = 0; i < 4; ++i) {
+        uint32_t o[16];
+        ti_ld16(to + 64 * half + 16 * i, o);
+        ti_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *at(lane, 4 * i + j) = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]),
+                                             __uint_as_float(o[4 * j + 3]));
+      }
+      __syncwarp();
+      const int first = row0 + 128 * x + 32 * (warp & 3) + (lane >> 4);
+#pragma unroll 4
+      for (int i = 0; i < 32; i += 2)
+        if (first + i < a.rows) *(float4*)(slot_of(first + i) + 4 + 64 * half + 4 * (lane & 15)) = *at(i + (lane >> 4), lane & 15);
+      __syncwarp();
     }
     }
   }
