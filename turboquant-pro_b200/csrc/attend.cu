@@ -39,6 +39,8 @@ struct Call : tq_attend_args {
   float* states;
   const float* before;
   int64_t before_rows;
+  SharedStates shared;  // the prefix's states, not merged
+  SharedStates* keep;   // of the prefix's part: they are to stay so
 };
 Call plain_call(const tq_attend_args* r) {
   Call c = {};
@@ -56,6 +58,11 @@ Call part_of(const tq_ctx* ctx, const Call& r, int s, int n) {
   part.out = (uint8_t*)r.out + (size_t)s * r.n_tokens * g.n_q_heads * TQ_D * esz;
   part.q_lens = r.q_lens == nullptr ? nullptr : r.q_lens + s;
   part.before = r.before == nullptr ? nullptr : r.before + (size_t)s * r.n_tokens * g.group * TQ_PART_STRIDE;
+  if (r.shared.slots != nullptr) {
+    const size_t row = (size_t)s * r.n_tokens * g.group;
+    part.shared.slots += row * r.shared.ns * TQ_SLOT_STRIDE;
+    part.shared.general += row * 2 * TQ_PART_STRIDE;
+  }
   part.list = r.list == nullptr ? nullptr : r.list + (size_t)s * r.n_tokens * g.n_kv_heads * r.n_list;
   return part;
 }
@@ -231,11 +238,13 @@ int run(tq_ctx* ctx, const Call* r, const Plan& p, cudaStream_t st) {
   for (int s = 0; s < r->seq_count; s += at_once) {
     const Call part = part_of(ctx, *r, s, std::min(at_once, r->seq_count - s));
     a.seq_begin = part.seq_begin, a.seq_count = part.seq_count;
-    a.q = part.q, a.out = part.out, a.q_lens = part.q_lens, a.list = part.list, a.before = part.before;
+    a.q = part.q, a.out = part.out, a.q_lens = part.q_lens, a.list = part.list, a.before = part.before, a.shared = part.shared;
     if (p.form == SHARED) {
-      const int rc = tq_launch_attend_shared(a, r->workspace, st);
+      SharedStates as;
+      const int rc = tq_launch_attend_shared(a, r->workspace, r->keep == nullptr, &as, st);
       if (rc != TQ_OK) return rc;
-      ctx->last_launches += 3;
+      if (r->keep != nullptr) *r->keep = as;
+      ctx->last_launches += r->keep != nullptr ? 2 : 3;
       continue;
     }
     if (p.form == TILES) {
@@ -317,10 +326,12 @@ Call listed_call(const tq_attend_args* r, const int32_t* blocks, int32_t n_block
 }
 
 // A call with a shared beginning, in two parts: the queries of all sequences as those of one, on the prefix, and the
-// sequences' own tokens.  The prefix's states stand before the workspace that the parts use one after the other.
+// sequences' own tokens, whose merge takes the prefix's states in: one a row, or, where both parts have the forms that can,
+// all of them as they are.
 struct Shared {
   Call prefix, own;
-  size_t states;  // bytes
+  size_t states, of_prefix, of_own;  // bytes
+  bool direct;                       // the states are not merged in between
 };
 int check_shared(const tq_ctx* ctx, const tq_attend_args* r, int32_t prefix) {
   TQ_REQUIRE(r->window == 0 && r->sinks == 0, TQ_ERR_INVALID, "a window and a shared beginning do not go together");
@@ -343,25 +354,35 @@ Shared shared_part(const tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, i
   p.q_lens = nullptr;
   p.whole = true;
   c.states = align_up((size_t)g.n_kv_heads * tokens * g.group * TQ_PART_STRIDE * 4, 256);
-  p.states = (float*)r->workspace;
-  c.own.before = (const float*)r->workspace;
   c.own.before_rows = (int64_t)tokens * g.group;
-  for (Call* x : {&c.prefix, &c.own}) {
-    x->workspace = (uint8_t*)r->workspace + c.states;
-    x->workspace_bytes = r->workspace_bytes < c.states ? 0 : r->workspace_bytes - c.states;
-  }
   return c;
+}
+// Bytes of a part's workspace; where it is, and how the parts go together.
+int shared_plan(tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st, Shared* c) {
+  int rc = workspace_of(ctx, c->prefix, st, &c->of_prefix);
+  if (rc == TQ_OK) rc = workspace_of(ctx, c->own, st, &c->of_own);
+  if (rc != TQ_OK) return rc;
+  const Plan own = make_plan(ctx, &c->own, st);
+  c->direct = make_plan(ctx, &c->prefix, st).form == SHARED && own.form == ROWS && c->of_own >= least_bytes(own);
+  uint8_t* w = (uint8_t*)r->workspace;
+  c->prefix.workspace = w, c->prefix.workspace_bytes = c->of_prefix;
+  c->own.workspace = w + c->of_prefix, c->own.workspace_bytes = c->of_own;
+  if (c->direct) {
+    c->states = 0;
+    return TQ_OK;
+  }
+  c->prefix.states = (float*)(w + c->of_prefix + c->of_own);
+  c->own.before = c->prefix.states;
+  return TQ_OK;
 }
 // Bytes that the call needs in rounds of n sequences.
 int shared_bytes(tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, int n, cudaStream_t st, size_t* bytes) {
   *bytes = 0;
   for (int s = 0; s < r->seq_count; s += n) {
-    const Shared c = shared_part(ctx, r, prefix, s, std::min(n, r->seq_count - s));
-    size_t of_prefix = 0, of_own = 0;
-    int rc = workspace_of(ctx, c.prefix, st, &of_prefix);
-    if (rc == TQ_OK) rc = workspace_of(ctx, c.own, st, &of_own);
+    Shared c = shared_part(ctx, r, prefix, s, std::min(n, r->seq_count - s));
+    const int rc = shared_plan(ctx, r, st, &c);
     if (rc != TQ_OK) return rc;
-    *bytes = std::max(*bytes, c.states + std::max(of_prefix, of_own));
+    *bytes = std::max(*bytes, c.of_prefix + c.of_own + c.states);
   }
   return TQ_OK;
 }
@@ -399,7 +420,10 @@ extern "C" int32_t tq_attend_prefix(tq_ctx* ctx, const tq_attend_args* r, int32_
   TQ_REQUIRE(bytes <= r->workspace_bytes, TQ_ERR_CAPACITY, "workspace smaller than tq_attend_prefix_workspace asks for one sequence");
   int launches = 0;
   for (int s = 0; s < r->seq_count; s += n) {
-    const Shared c = shared_part(ctx, r, prefix, s, std::min(n, r->seq_count - s));
+    Shared c = shared_part(ctx, r, prefix, s, std::min(n, r->seq_count - s));
+    rc = shared_plan(ctx, r, (cudaStream_t)stream, &c);
+    if (rc != TQ_OK) return rc;
+    if (c.direct) c.prefix.keep = &c.own.shared;
     for (const Call* x : {&c.prefix, &c.own}) {
       rc = attend(ctx, *x, stream);
       if (rc != TQ_OK) return rc;

@@ -17,6 +17,16 @@
 #include "common.cuh"
 #include "decode_generic.cuh"  // TQ_SCORE_LOG2, tq_exp2
 
+// The states of a shared beginning as its form leaves them: [head][rows][ns][TQ_SLOT_STRIDE], the first ns_cold of them in code
+// space; of a flagged head the general form's two, [head][rows][2][2 + D].
+struct SharedStates {
+  const float* slots;  // null: none
+  const int32_t* left;
+  const float* general;
+  int32_t ns_cold, ns;
+};
+constexpr int TQ_SLOT_STRIDE = 4 + TQ_D;  // M, L, -, -, o
+
 struct AttendArgs {
   tq_geom g;
   const uint8_t* pages;
@@ -53,6 +63,7 @@ struct AttendArgs {
   float* states;
   const float* before;
   int64_t before_rows;
+  SharedStates shared;  // or its states, unmerged
   int32_t wait_limit, withhold;  // test hook of the form for many rows (tq_debug_wait); 0 and -1 otherwise
 };
 
@@ -184,4 +195,5 @@ int tq_launch_attend_tiles(const AttendArgs& a, void* workspace, int cap, int sp
 // A shared beginning: 16-bit queries, 256-token blocks of per-channel keys; the states
 void tq_attend_shared_plan(const AttendArgs& a, int tokens, int* ns_cold, int* ns_hot);
 size_t tq_attend_shared_bytes(const AttendArgs& a);
-int tq_launch_attend_shared(const AttendArgs& a, void* workspace, cudaStream_t st);
+// `merged`: to a.states; else *as gets a.shared for those who merge it with theirs
+int tq_launch_attend_shared(const AttendArgs& a, void* workspace, bool merged, SharedStates* as, cudaStream_t st);

@@ -1361,6 +1361,136 @@ __global__ void __launch_bounds__(AC_THREADS, 2) attend_rows_combine_kernel(Atte
   }
 }
 
+// The same with the states of a shared beginning, of which there may be tens a row: eight rows at a time, two warps a row, a lane
+// four channels, and eight states of each on their way at once.  (Merged by a kernel of their own before, 64 x 8 x 8 rows cost 25 us
+// more, 32 x 8 x 4 rows 10.)
+constexpr int AM_THREADS = 512, AM_ROWS = 8;
+__global__ void __launch_bounds__(AM_THREADS, 1) attend_rows_merge_kernel(AttendArgs a, int tile, int total) {
+  __shared__ __align__(16) float cs[AM_ROWS][TQ_D], hs[AM_ROWS][TQ_D], ys[4][AM_ROWS][TQ_D];
+  __shared__ float ms[AM_ROWS], ls[AM_ROWS];
+  const tq_geom& g = a.g;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, e = tid % TQ_D, h = tid / TQ_D;
+  const int H = g.n_kv_heads, cost = ar_cost(a.q_dtype != TQ_BF16);
+  float pi[TQ_D / 4];
+#pragma unroll
+  for (int d = 0; d < TQ_D / 4; ++d) pi[d] = a.tables->pi[(32 * h + d) * TQ_D + e];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const ArPlan* plan = (const ArPlan*)a.plan;
+  const int64_t share = plan->share;
+  const int in = warp >> 1, half = warp & 1;
+  for (int r0 = blockIdx.x * AM_ROWS; r0 < total; r0 += gridDim.x * AM_ROWS) {
+    const int at = r0 + in;
+    float M = -INFINITY, L = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, hot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto weigh = [&](float top) {  // to the maximum `top`
+      const float by = top > -INFINITY ? top : 0.0f, down = M > -INFINITY ? tq_exp2(M - by) : 1.0f;
+      L *= down;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] *= down, hot[c] *= down;
+      M = top;
+      return by;
+    };
+    if (at < total) {
+      const int row = at % a.rows, unit = at / a.rows, s = unit / H, head = unit - s * H;
+      const int4 seq = plan->seq[s];
+      const int64_t before = plan->cum[s];
+      const float* of_prefix = nullptr;
+      int np = 0, np_cold = 0, stride = TQ_SLOT_STRIDE, skip = 4;
+      if (attend_position(a, attend_seq(a, s), row) >= 0) {
+        const size_t of = (size_t)head * a.before_rows + (size_t)s * a.rows + row;
+        const bool general = a.shared.left[head] != 0;
+        np = general ? 2 : a.shared.ns, np_cold = general ? 1 : a.shared.ns_cold;
+        if (general) stride = TQ_PART_STRIDE, skip = 2;
+        of_prefix = general ? a.shared.general + of * 2 * TQ_PART_STRIDE : a.shared.slots + of * np * TQ_SLOT_STRIDE;
+      }
+      int nc = 0, nh = 0;
+      if (row / tile < seq.z) {  // (slots as in the kernel above)
+        const int64_t begin = before + (int64_t)(head * seq.z + row / tile) * (cost * seq.x + a.hot_cost * seq.y);
+        const int64_t middle = begin + cost * seq.x;
+        nc = seq.x > 0 ? (int)(ar_div(middle - cost, share) - ar_div(begin, share)) + 1 : 0;
+        nh = seq.y > 0 ? (int)(ar_div(middle + a.hot_cost * (seq.y - 1), share) - ar_div(middle, share)) + 1 : 0;
+      }
+      const float* own = attend_partial(a, unit, row, 0);
+      constexpr int BATCH = 8;
+      for (int i0 = half; i0 < np + nc + nh; i0 += 2 * BATCH) {
+        float2 ml[BATCH], u[BATCH], v[BATCH];
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          ml[k] = make_float2(-INFINITY, 0.0f), u[k] = v[k] = make_float2(0.0f, 0.0f);
+          const int i = i0 + 2 * k, o = i - np;
+          if (o < nc + nh) {
+            const float* p = o < 0 ? of_prefix + (size_t)i * stride : own + (size_t)(o < nc ? o : a.ns_cold + o - nc) * TQ_PART_STRIDE;
+            ml[k] = *(const float2*)p;
+            p += (o < 0 ? skip : 2) + 4 * lane;
+            u[k] = *(const float2*)p, v[k] = *(const float2*)(p + 2);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) top = fmaxf(top, ml[k].x);
+        const float by = weigh(top);
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const float f = attend_weight(ml[k].x, ml[k].y, by);
+          if (f == 0.0f) continue;
+          const int i = i0 + 2 * k;
+          const float y[4] = {u[k].x, u[k].y, v[k].x, v[k].y};
+          L = fmaf(ml[k].y, f, L);
+          if (i < np ? i < np_cold : i - np < nc) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[c] = fmaf(y[c], f, x[c]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) hot[c] = fmaf(y[c], f, hot[c]);
+          }
+        }
+      }
+    }
+    // the second warp's to the first's
+    if (half == 1) {
+      *(float4*)&cs[in][4 * lane] = make_float4(x[0], x[1], x[2], x[3]);
+      *(float4*)&hs[in][4 * lane] = make_float4(hot[0], hot[1], hot[2], hot[3]);
+      if (lane == 0) ms[in] = M, ls[in] = L;
+    }
+    __syncthreads();
+    if (half == 0) {
+      const float m = ms[in], l = ls[in], by = weigh(fmaxf(M, m)), f = attend_weight(m, l, by);
+      const float4 u = *(const float4*)&cs[in][4 * lane], v = *(const float4*)&hs[in][4 * lane];
+      if (f != 0.0f) {
+        L = fmaf(l, f, L);
+        x[0] = fmaf(u.x, f, x[0]), x[1] = fmaf(u.y, f, x[1]), x[2] = fmaf(u.z, f, x[2]), x[3] = fmaf(u.w, f, x[3]);
+        hot[0] = fmaf(v.x, f, hot[0]), hot[1] = fmaf(v.y, f, hot[1]), hot[2] = fmaf(v.z, f, hot[2]), hot[3] = fmaf(v.w, f, hot[3]);
+      }
+      *(float4*)&cs[in][4 * lane] = make_float4(x[0], x[1], x[2], x[3]);
+      *(float4*)&hs[in][4 * lane] = make_float4(hot[0], hot[1], hot[2], hot[3]);
+      __syncwarp();
+      if (lane == 0) ms[in] = M, ls[in] = L;
+    }
+    __syncthreads();
+    float y[AM_ROWS];
+#pragma unroll
+    for (int k = 0; k < AM_ROWS; ++k) y[k] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < TQ_D / 4; d += 4)
+#pragma unroll
+      for (int k = 0; k < AM_ROWS; ++k) {
+        const float4 v = *(const float4*)&cs[k][32 * h + d];
+        y[k] = fmaf(v.x, pi[d], y[k]), y[k] = fmaf(v.y, pi[d + 1], y[k]);
+        y[k] = fmaf(v.z, pi[d + 2], y[k]), y[k] = fmaf(v.w, pi[d + 3], y[k]);
+      }
+#pragma unroll
+    for (int k = 0; k < AM_ROWS; ++k) ys[h][k][e] = y[k];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < AM_ROWS / 4; ++i) {
+      const int k = 4 * i + h;
+      if (r0 + k >= total) break;
+      const int row = (r0 + k) % a.rows, unit = (r0 + k) / a.rows, s = unit / H;
+      attend_result(a, s, unit - s * H, row, e, ms[k], ls[k], (ys[0][k][e] + ys[1][k][e]) + (ys[2][k][e] + ys[3][k][e]) + hs[k][e]);
+    }
+    __syncthreads();  // (the rows have been read)
+  }
+}
+
 template <bool SPLIT, int VB, bool LIST>
 int launch_rows(const AttendArgs& a, cudaStream_t st) {
   using Shared = ArShared<SPLIT, VB>;
@@ -1380,6 +1510,15 @@ int launch_rows(const AttendArgs& a, cudaStream_t st) {
   // calls, 4000 tokens: 32 rows 29 us against 47, 256 rows 36 against 50; 8 x 1000 tokens: 256 rows 25 against 30, 512
   // rows 30 and 30, 1024 rows 44 against 35.
   const bool few = all <= 2 * a.sm_count;
+  if (a.shared.slots != nullptr) {
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>((all + AM_ROWS - 1) / AM_ROWS, a.sm_count));
+    cfg.blockDim = dim3(AM_THREADS);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    TQ_CUDA(cudaLaunchKernelEx(&cfg, attend_rows_merge_kernel, a, 8 * NT, (int)all));
+    return TQ_OK;
+  }
   cfg.gridDim = dim3((unsigned)(few ? all : std::min<int64_t>((all + 3) / 4, 2 * a.sm_count)));
   cfg.blockDim = dim3(AC_THREADS);
   cfg.stream = st;

@@ -33,7 +33,7 @@ constexpr int PX_KLBO = PX_T * 16, PX_LBO = TQ_D * 16, PX_SBO = 128;  // from ei
 constexpr int PX_SOFTMAX = 256, PX_ISSUE = 128, PX_MAKERS = 256, PX_THREADS = PX_SOFTMAX + PX_ISSUE + PX_MAKERS;
 #define PX_REGISTERS(how, n) asm volatile("setmaxnreg." how ".sync.aligned.u32 " n ";")
 constexpr int PX_P = PX_T, PX_HALF = 128, PX_O = 256;  // tensor memory's columns, as in the form for many rows
-constexpr int PX_STRIDE = 4 + TQ_D;          // floats of a state: M, L, -, -, o
+constexpr int PX_STRIDE = TQ_SLOT_STRIDE;    // floats of a state
 constexpr int PX_TOP = 8;                    // a page's largest key on the grid is lifted to 2^8 .. 2^9
 constexpr int PX_LIST = 7;                   // outliers of a tile that a lane holds (160 of a tile are usual)
 constexpr int PX_WIDE = 8;                   // channels whose keys are two parts
@@ -923,26 +923,31 @@ int rows_of_cta(const AttendArgs& a) { return a.q_dtype == TQ_F16 ? PxShape<true
 
 }  // namespace
 
-// Splits of the blocks and of the window: as many as bring the rounds of CTAs nearest to even, with six tiles' time for what a
-// CTA does besides.
+// Splits of the blocks and of the window, one of whose tiles takes as long as two: of as many as fill the GPU once, twice .. those
+// with the least time, with six tiles' time for what a CTA does besides.
 void tq_attend_shared_plan(const AttendArgs& a, int tokens, int* ns_cold, int* ns_hot) {
   const tq_geom& g = a.g;
   const int64_t cold = (int64_t)n_cold_blocks(tokens, g.hot_window, PX_S) * (PX_S / PX_T);
-  const int64_t hot = (std::min(tokens, g.hot_window) + PX_T - 1) / PX_T;
+  const int64_t hot = std::max((std::min(tokens, g.hot_window) + PX_T - 1) / PX_T, 1);
   const int64_t units = (int64_t)g.n_kv_heads * ((a.rows + rows_of_cta(a) - 1) / rows_of_cta(a));
   int64_t best = INT64_MAX;
   *ns_cold = *ns_hot = 1;
-  for (int64_t each = 1; each <= std::max<int64_t>(cold, 2 * hot); ++each) {  // tiles of a CTA; one of the window takes twice as long
-    const int64_t nc = std::max<int64_t>((cold + each - 1) / each, 1), nh = std::max<int64_t>((2 * hot + each - 1) / each, 1);
-    if (nc + nh > 256) continue;
-    const int64_t time = (units * (nc + nh) + a.sm_count - 1) / a.sm_count * (each + 6);
-    if (time < best) best = time, *ns_cold = (int)nc, *ns_hot = (int)std::min(nh, hot);
+  for (int rounds = 1; rounds <= 8; ++rounds) {
+    const int64_t ctas = std::min<int64_t>(rounds * (int64_t)a.sm_count / std::max<int64_t>(units, 1), 256);  // of a unit
+    if (ctas < 2) continue;
+    int64_t each = std::max<int64_t>((cold + 2 * hot + ctas - 1) / ctas, 1), nc, nh;  // tiles of a CTA
+    for (;; ++each) {
+      nc = std::max<int64_t>((cold + each - 1) / each, 1), nh = std::min((2 * hot + each - 1) / each, hot);
+      if (nc + nh <= ctas) break;
+    }
+    if (rounds * (each + 6) < best) best = rounds * (each + 6), *ns_cold = (int)nc, *ns_hot = (int)nh;
   }
 }
 
 size_t tq_attend_shared_bytes(const AttendArgs& a) { return layout(a).total; }
 
-int tq_launch_attend_shared(const AttendArgs& base, void* workspace, cudaStream_t st) {
+int tq_launch_attend_shared(const AttendArgs& base, void* workspace, bool merged, SharedStates* as,
+                            cudaStream_t st) {
   AttendArgs a = base;
   const Layout l = layout(a);
   uint8_t* w = (uint8_t*)workspace;
@@ -963,6 +968,8 @@ int tq_launch_attend_shared(const AttendArgs& base, void* workspace, cudaStream_
   a.unit_stride = (int64_t)a.rows * 2 * TQ_PART_STRIDE;
   rc = tq_launch_attend_general(a, st);
   if (rc != TQ_OK) return rc;
+  *as = {pa.slots, pa.left, a.partials, pa.ns_cold, pa.ns_cold + pa.ns_hot};
+  if (!merged) return TQ_OK;
   const int64_t rows = (int64_t)a.g.n_kv_heads * a.rows;
   attend_shared_merge_kernel<<<(int)std::min<int64_t>((rows + 3) / 4, 2 * a.sm_count), PM_THREADS, 0, st>>>(a, pa);
   TQ_CUDA(cudaGetLastError());
