@@ -77,6 +77,10 @@ CASES = [
     ([30] * 50, 3900, 1, 32, 192, "bfloat16", "bfloat16", 512, "uniform", 3),
     ([17] * 20, 4000, 1, 16, 128, "float16", "float16", 512, "nf4", 4),
     ([40] * 70, 3333, 2, 8, 64, "float16", "float16", 512, "nf4_asym", 3),
+    # drafts on windows and blocks of their own, several tiles of rows
+    ([3, 800, 512, 513, 32, 33, 64], 700, 5, 1, 7, "bfloat16", "bfloat16", 512, "nf4_asym", 3),
+    ([300, 1, 2000], 300, 4, 2, 32, "float16", "float16", 512, "uniform", 4),
+    ([700] * 66, 600, 1, 1, 3, "float16", "float16", 512, "nf4_asym", 3),
 ]
 
 
@@ -161,6 +165,43 @@ def test_keys_with_a_large_constant_part(torch, dtype, hot, keys, prefix, b, t):
         v = torch.randn(1, n, 2, 128, generator=gen, device="cuda")
         ctx.append(0, k.to(ctx.kv_dtype), v.to(ctx.kv_dtype), seq_begin=s)
     _check(torch, ctx, ctx.attend(0, q, prefix=0, seq_begin=1), q, 0, seq_begin=1)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_values_that_are_no_numbers_in_the_sequences_windows(torch, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    ctx = _ctx(n_seqs=4, n_kv_heads=2, n_q_heads=6, kv_dtype=dtype)
+    _fill(torch, ctx, [900, 200, 300, 40], gen)
+    k, v = (torch.randn(3, 3, 2, 128, generator=gen, device="cuda") for _ in range(2))
+    v[0, 1, 0, 5], v[0, 1, 0, 6], v[1, 2, 1] = float("inf"), float("nan"), float("-inf")
+    k[2, 1, 0, 7] = float("inf")
+    ctx.append(0, k.to(ctx.kv_dtype), v.to(ctx.kv_dtype), seq_begin=1)
+    q = torch.randn(3, 3, 6, 128, generator=gen, device="cuda").to(ctx.kv_dtype)
+    q[..., 7] = -q[..., 7].abs() - 0.1  # (an infinite key then has a score of -inf, a weight of zero)
+    got = ctx.attend(0, q, prefix=0, seq_begin=1)
+    pk, pv = ctx.dequant(0, 0, 0, 900)
+    for s, n in enumerate((203, 303, 43)):
+        sk, sv = ctx.dequant(0, s + 1, 0, n)
+        kk, vv = torch.cat((pk, sk), 1), torch.cat((pv, sv), 1)
+        want = oracle.attention(torch.nan_to_num(kk, posinf=0.0), torch.nan_to_num(vv, 0.0, 0.0, 0.0), q[s], 3, None, 0)
+        spoilt = torch.zeros_like(want, dtype=torch.bool)
+        if s == 0:  # from the second token on, of the first KV head
+            spoilt[1:, :3, 5:7] = True
+            assert bool(torch.isposinf(got[s, 1:, :3, 5]).all()) and bool(torch.isnan(got[s, 1:, :3, 6]).all())
+        if s == 1:
+            spoilt[2:, 3:] = True
+            assert bool(torch.isneginf(got[s, 2, 3:]).all())
+        if s == 2:  # (the infinite key's token counts for nothing)
+            hidden = [slice(900 + 41, 900 + 42)]
+            first = oracle.attention(torch.nan_to_num(kk, posinf=0.0), vv, q[s], 3, None, 0, hidden)
+            want[:, :3] = first[:, :3]
+        x = torch.where(spoilt, want, got[s].double())
+        assert bool(torch.isfinite(x).all())
+        keep = ~spoilt.any(-1)
+        head, row = oracle.measures(got[s][keep][None], want[keep][None])
+        assert row <= oracle.limits(got.dtype)[1], row
+        rest = (x - want).norm(dim=-1) / want.norm(dim=-1)
+        assert float(rest.max()) <= oracle.limits(got.dtype)[1]
 
 
 def test_orders_parts_of_the_batch_and_out(torch):

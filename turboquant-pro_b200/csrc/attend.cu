@@ -20,7 +20,7 @@ namespace {
 constexpr size_t AT_ONE_GO = (size_t)1 << 30;  // workspace that a call asks for at most, unless one
                                                // sequence needs more
 
-enum Form { GENERAL, ROWS, TILES, SHARED };
+enum Form { GENERAL, ROWS, TILES, SHARED, WINDOW };
 struct Plan {
   Form form;
   int ns_cold, ns_hot;
@@ -35,7 +35,7 @@ struct Plan {
 struct Call : tq_attend_args {
   const int32_t* list;
   int32_t n_list;
-  bool listed, whole;
+  bool listed, whole, merges;  // merges: the sequences' own part of a call with a shared beginning, which merges the states
   float* states;
   const float* before;
   int64_t before_rows;
@@ -109,6 +109,8 @@ Form choose(const tq_ctx* ctx, const Call* r, int n) {
   if (!channels) return GENERAL;
   if (r->listed) return blocks ? ROWS : GENERAL;
   if (r->whole && blocks && r->q_dtype != TQ_F32) return SHARED;
+  // (and the merge of its states with few rows: a window of their type, and what blocks the sequences have by the rows form)
+  if (r->merges && blocks && rows <= 64 && r->q_dtype != TQ_F32 && r->q_dtype == g.kv_dtype) return WINDOW;
   if (r->q_dtype == TQ_F32) return blocks && rows <= 48 ? ROWS : GENERAL;
   const double seen = r->window == 0 ? n : std::min((double)n, (double)r->window + r->n_tokens + r->sinks);
   const double w = seen * r->seq_count * g.n_kv_heads / 1000.0;
@@ -163,8 +165,13 @@ Plan make_plan(const tq_ctx* ctx, const Call* r, cudaStream_t st) {
     p.seq_bytes = tq_attend_tiles_bytes(a, g.n_kv_heads, p.cap, p.splits);
     return p;
   }
-  if (p.form == ROWS) {
+  if (p.form == WINDOW && n <= g.hot_window) {  // no blocks
+    p.seq_bytes = 256;
+    return p;
+  }
+  if (p.form == ROWS || p.form == WINDOW) {
     AttendArgs a = {};
+    a.no_window = p.form == WINDOW;
     a.g = g;
     a.rows = rows;
     a.seq_count = r->seq_count;
@@ -239,6 +246,14 @@ int run(tq_ctx* ctx, const Call* r, const Plan& p, cudaStream_t st) {
     const Call part = part_of(ctx, *r, s, std::min(at_once, r->seq_count - s));
     a.seq_begin = part.seq_begin, a.seq_count = part.seq_count;
     a.q = part.q, a.out = part.out, a.q_lens = part.q_lens, a.list = part.list, a.before = part.before, a.shared = part.shared;
+    if (p.form == WINDOW) {
+      a.no_window = 1;
+      int rc = p.ns_cold > 0 ? tq_launch_attend_rows(a, st) : TQ_OK;
+      if (rc == TQ_OK) rc = tq_launch_attend_window(a, TQ_ROWS_TILE, st);
+      if (rc != TQ_OK) return rc;
+      ctx->last_launches += p.ns_cold > 0 ? 2 : 1;
+      continue;
+    }
     if (p.form == SHARED) {
       SharedStates as;
       const int rc = tq_launch_attend_shared(a, r->workspace, r->keep == nullptr, &as, st);
@@ -359,11 +374,12 @@ Shared shared_part(const tq_ctx* ctx, const tq_attend_args* r, int32_t prefix, i
 }
 // Bytes of a part's workspace; where it is, and how the parts go together.
 int shared_plan(tq_ctx* ctx, const tq_attend_args* r, cudaStream_t st, Shared* c) {
+  c->own.merges = make_plan(ctx, &c->prefix, st).form == SHARED;
   int rc = workspace_of(ctx, c->prefix, st, &c->of_prefix);
   if (rc == TQ_OK) rc = workspace_of(ctx, c->own, st, &c->of_own);
   if (rc != TQ_OK) return rc;
   const Plan own = make_plan(ctx, &c->own, st);
-  c->direct = make_plan(ctx, &c->prefix, st).form == SHARED && own.form == ROWS && c->of_own >= least_bytes(own);
+  c->direct = c->own.merges && (own.form == ROWS || own.form == WINDOW) && c->of_own >= least_bytes(own);
   uint8_t* w = (uint8_t*)r->workspace;
   c->prefix.workspace = w, c->prefix.workspace_bytes = c->of_prefix;
   c->own.workspace = w + c->of_prefix, c->own.workspace_bytes = c->of_own;

@@ -64,6 +64,7 @@ struct AttendArgs {
   const float* before;
   int64_t before_rows;
   SharedStates shared;  // or its states, unmerged
+  int32_t no_window;    // the rows form: the pages alone, and no merge
   int32_t wait_limit, withhold;  // test hook of the form for many rows (tq_debug_wait); 0 and -1 otherwise
 };
 
@@ -179,6 +180,20 @@ int attend_shared(K kernel, size_t bytes, int device, bool (&done)[64]) {
 int tq_most_tokens(const tq_ctx* ctx, int layer, int seq_begin, int seq_count, cudaStream_t st);
 int tq_launch_attend_general(const AttendArgs& a, cudaStream_t st);
 int tq_launch_attend_combine(const AttendArgs& a, cudaStream_t st);
+// ---- the rows form's division of its work
+constexpr int AR_SEQS = 64;        // sequences of a launch
+// How long a strip takes, by whether operands are pairs (the measurements are beside the kernel)
+TQ_HD constexpr int ar_cost(bool split) { return split ? 8 : 4; }
+TQ_DEV int64_t ar_div(int64_t x, int64_t y) {  // (mostly of numbers that fit 32 bits)
+  return (x | y) >> 32 == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+}
+// How a launch divides its work; the first CTA leaves it for the merge.
+struct ArPlan {
+  int64_t share;
+  int64_t cum[AR_SEQS + 1];
+  int4 seq[AR_SEQS];  // strips, window tiles and row tiles of a sequence
+};
+constexpr int TQ_ROWS_TILE = 8;  // query rows of a tile
 // Few rows, 256-token blocks of per-channel keys, queries on 16-byte boundaries; the merge too.
 struct AttendRowsPlan {
   int ns_cold, ns_hot;  // slots of a row's states
@@ -197,3 +212,5 @@ void tq_attend_shared_plan(const AttendArgs& a, int tokens, int* ns_cold, int* n
 size_t tq_attend_shared_bytes(const AttendArgs& a);
 // `merged`: to a.states; else *as gets a.shared for those who merge it with theirs
 int tq_launch_attend_shared(const AttendArgs& a, void* workspace, bool merged, SharedStates* as, cudaStream_t st);
+// The last part of such a call where the sequences' queries are few rows of the window's 16-bit type: window and merge
+int tq_launch_attend_window(const AttendArgs& a, int blocks_tile, cudaStream_t st);

@@ -369,6 +369,8 @@ __global__ void __launch_bounds__(AG_THREADS, 2) attend_general_kernel(AttendArg
 template <int RPT>
 __global__ void __launch_bounds__(AG_THREADS) attend_left_kernel(AttendArgs a, int row_tiles, int items) {
   extern __shared__ __align__(16) uint8_t ag_smem[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   bool any = false;
   for (int i = threadIdx.x; i < a.seq_count * a.g.n_kv_heads; i += AG_THREADS) any |= a.left[i] != 0;
   if (!__syncthreads_or(any)) return;
@@ -424,9 +426,18 @@ int launch_general(const AttendArgs& a, cudaStream_t st) {
   if (a.left != nullptr) {
     const int rc = attend_shared(attend_left_kernel<RPT>, sizeof(AgShared<RPT>), a.device, left_done);
     if (rc != TQ_OK) return rc;
-    attend_left_kernel<RPT><<<(int)std::min<int64_t>(grid, a.sm_count), AG_THREADS, sizeof(AgShared<RPT>), st>>>(
-        a, row_tiles, (int)grid);
-    TQ_CUDA(cudaGetLastError());
+    // (behind the form for shared beginnings it comes up under that one's last CTAs, and what follows it likewise)
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>(grid, a.sm_count));
+    cfg.blockDim = dim3(AG_THREADS);
+    cfg.dynamicSmemBytes = sizeof(AgShared<RPT>);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = a.whole ? 1 : 0;
+    TQ_CUDA(cudaLaunchKernelEx(&cfg, attend_left_kernel<RPT>, a, row_tiles, (int)grid));
     return TQ_OK;
   }
   const int rc = attend_shared(attend_general_kernel<RPT, LIST>, sizeof(AgShared<RPT>), a.device, done);

@@ -61,10 +61,8 @@ constexpr int AR_PITCH = TQ_D * 2 + 16, AR_PITCH32 = TQ_D * 4 + 16;  // bytes of
 //     tokens, 106, 90, 85, 84; 16 x 3000 float16 98, 88, 82, 89; 32 x 700 76, 70, 72, 80; 1 x 600 35, 35, 24, 24.  Half of
 //     that (HALF_HOT) where every warp then has one share of a strip's length, and would not otherwise: 1 x 2500 of 32 x 1,
 //     window 2000, 39, 43, 44, -.  (The kernel cannot choose: that took 1.5 to 4 us of its prologue.)
-TQ_HD constexpr int ar_cost(bool split) { return split ? 8 : 4; }
 inline int ar_hot_cost(int q_dtype, int kv_dtype) { return kv_dtype != TQ_F32 ? 3 : q_dtype == TQ_BF16 ? 4 : 8; }
 constexpr int HALF_HOT = 4;
-constexpr int AR_SEQS = 64;        // sequences of a launch
 constexpr int AR_LIST = 256;       // outliers of a strip that are copied ahead (160 is usual)
 
 template <bool SPLIT, int VB>
@@ -182,9 +180,6 @@ TQ_DEV uint2 ar_lut2(uint32_t addr) {
   asm("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
   return v;
 }
-TQ_DEV int64_t ar_div(int64_t x, int64_t y) {  // (mostly of numbers that fit 32 bits)
-  return (x | y) >> 32 == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
-}
 template <int N>
 struct ArTiles {
   static constexpr int value = N;
@@ -219,7 +214,7 @@ TQ_DEV ArWork ar_work(const AttendArgs& a, int n, int q_n) {
   const int p_lo = a.whole ? n : n - q_n, p_hi = q_n > 0 ? (a.whole ? n + q_n : n) - 1 : -1;
   w.strip = LIST ? AttendTiles{0, 0, p_hi >= 0 ? min(a.n_list, w.cold / AR_S) * (AR_S / AR_STRIP) : 0}
                  : attend_tiles(a, 0, w.cold, AR_STRIP, p_lo, p_hi);
-  w.hot = attend_tiles(a, w.cold, n, AR_HOT, p_lo, p_hi);
+  w.hot = a.no_window ? AttendTiles{0, 0, 0} : attend_tiles(a, w.cold, n, AR_HOT, p_lo, p_hi);
   return w;
 }
 // row tiles of a sequence that have query tokens
@@ -228,13 +223,6 @@ template <bool LIST>
 TQ_DEV int ar_tiles(const AttendArgs& a, int q_n, int n) {
   return LIST ? q_n * ((a.g.group + n - 1) / n) : (q_n * a.g.group + n - 1) / n;
 }
-
-// How a launch divides its work; the first CTA leaves it for the merge.
-struct ArPlan {
-  int64_t share;
-  int64_t cum[AR_SEQS + 1];
-  int4 seq[AR_SEQS];  // strips, window tiles and row tiles of a sequence
-};
 
 template <bool SPLIT, int VB, bool LIST>
 __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows_kernel(AttendArgs a) {
@@ -1502,6 +1490,7 @@ int launch_rows(const AttendArgs& a, cudaStream_t st) {
   if (rc != TQ_OK) return rc;
   attend_rows_kernel<SPLIT, VB, LIST><<<a.sm_count, 32 * ArShape<SPLIT, VB>::WARPS, sizeof(Shared), st>>>(a);
   TQ_CUDA(cudaGetLastError());
+  if (a.no_window) return TQ_OK;  // (the merge is another's)
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1542,7 +1531,7 @@ AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens) {
   const int64_t seen = a.window == INT_MAX ? in_blocks : std::min<int64_t>(in_blocks, (int64_t)a.window + a.n_tokens + 128);
   const int64_t strips = a.listed ? std::min<int64_t>(a.n_list, in_blocks / AR_S) * (AR_S / AR_STRIP)
                                   : (seen + AR_STRIP - 1) / AR_STRIP + (std::min<int64_t>(a.sinks, in_blocks) + AR_STRIP - 1) / AR_STRIP;
-  const int64_t hot = (std::min(tokens, g.hot_window) + AR_HOT - 1) / AR_HOT;
+  const int64_t hot = a.no_window ? 0 : (std::min(tokens, g.hot_window) + AR_HOT - 1) / AR_HOT;
   const int64_t tiles = a.listed ? (int64_t)a.n_tokens * ((g.group + 8 * NT - 1) / (8 * NT)) : (a.rows + 8 * NT - 1) / (8 * NT);
   const int64_t rows = (int64_t)std::min(a.seq_count, AR_SEQS) * g.n_kv_heads * tiles;
   const int64_t workers = (int64_t)a.sm_count * (a.q_dtype == TQ_BF16 ? ArShape<false, 3>::WARPS : ArShape<true, 3>::WARPS);

@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
   constexpr int VGB = TQ_GROUP_TOK * TQ_D * VB / 8;
   extern __shared__ __align__(128) uint8_t px_smem[];
   Shared& sh = *(Shared*)px_smem;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const tq_geom& g = a.g;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int ns = pa.ns_cold + pa.ns_hot;
