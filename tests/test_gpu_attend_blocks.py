@@ -91,6 +91,10 @@ CASES = [
     ([900, 100], 4, 1, 6, 4, "bfloat16", "bfloat16", 128, "polar", 4),
     ([1800], 1, 2, 4, 3, "float32", "float32", 512, "polar", 3),
     ([1300] * 70, 1, 1, 2, 2, "bfloat16", "bfloat16", 512, "nf4_asym", 3),
+    # many tokens on the same window: a kernel of its own
+    ([1700, 300, 600, 5, 0, 2000] * 3, 24, 3, 15, 3, "bfloat16", "bfloat16", 512, "nf4_asym", 3),
+    ([1000, 700], 60, 8, 80, 2, "float16", "float16", 512, "uniform", 4),
+    ([900], 900, 2, 16, 1, "bfloat16", "bfloat16", 512, "nf4", 3),
 ]
 
 

@@ -101,16 +101,23 @@ int check_args(tq_ctx* ctx, const tq_attend_args* r) {
 // float32 queries, which TILES would round: ROWS up to 48 rows, GENERAL above (ROWS against GENERAL, four
 // sequences of 8000, 8 KV heads: 32 rows 222 and 344, 48: 311 and 351, 64: 394 and 361, 128: 740 and 693; eight of 2000, 32
 // KV heads: 32 rows 527 and 666, 64: 1100 and 729).
-// Listed blocks differ from token to token: what is written for few rows, where the blocks are those it is written for.
+// Listed blocks differ from token to token: ROWS, where the blocks are those it is written for, tile of rows by tile.  The window is the
+// same for all tokens of a sequence: WINDOW takes it in tiles of 16 rows instead, for a kernel more, where ROWS would spend more
+// than 14 us on it by the above (27 x 8 heads of 5 x 8 rows, float16, 2 blocks: 210 us without, 141 with; 20 x 8 of 16 x 4 rows,
+// bfloat16: 98 and 48; 8 x 4 of 5 x 7 rows, 24 blocks: 70 and 74; 1 x 8 of 4 rows, 16 blocks: 28 and 43).
 Form choose(const tq_ctx* ctx, const Call* r, int n) {
   const tq_geom& g = ctx->g;
   const int rows = r->n_tokens * g.group;
   const bool channels = g.key_mode != TQ_KEYS_POLAR && !ctx->force_generic, blocks = g.block_tokens == 256;
   if (!channels) return GENERAL;
-  if (r->listed) return blocks ? ROWS : GENERAL;
+  const bool window = r->q_dtype != TQ_F32 && r->q_dtype == g.kv_dtype;
+  if (r->listed) {
+    const double w = (double)std::min(n, g.hot_window) * r->seq_count * g.n_kv_heads * r->n_tokens * ((g.group + 7) / 8) / 1000.0;
+    return !blocks ? GENERAL : window && (r->q_dtype == TQ_F16 ? 0.165 : 0.085) * w > 14.0 ? WINDOW : ROWS;
+  }
   if (r->whole && blocks && r->q_dtype != TQ_F32) return SHARED;
   // (and the merge of its states with few rows: a window of their type, and what blocks the sequences have by the rows form)
-  if (r->merges && blocks && rows <= 64 && r->q_dtype != TQ_F32 && r->q_dtype == g.kv_dtype) return WINDOW;
+  if (r->merges && blocks && rows <= 64 && window) return WINDOW;
   if (r->q_dtype == TQ_F32) return blocks && rows <= 48 ? ROWS : GENERAL;
   const double seen = r->window == 0 ? n : std::min((double)n, (double)r->window + r->n_tokens + r->sinks);
   const double w = seen * r->seq_count * g.n_kv_heads / 1000.0;

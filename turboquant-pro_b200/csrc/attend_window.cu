@@ -1,6 +1,7 @@
-// The last kernel of a call with a shared beginning: attention of a sequence's few query rows on its uncompressed window, which is
-// all that most sequences have behind a long beginning, and the merge with the states of the beginning and of the
-// sequence's own blocks, if it has any.  16-bit queries and a window of their type.
+// The last kernel of a call with a shared beginning or on listed blocks: attention of a sequence's query rows on its uncompressed
+// window (all that most sequences have behind a long beginning, and what all tokens share of calls whose blocks differ from
+// token to token), and the merge with the states of the beginning and of the sequence's own blocks, if it has any.
+// 16-bit queries and a window of their type.
 //
 // A CTA has 8 or 16 rows of a (sequence, KV head); its four warps take tiles of 32 tokens in turn and work alone: keys and values
 // come with cp.async, the next tile's keys while this one's values are summed and the other way round; S = Q K^T and O += P V on
@@ -260,8 +261,8 @@ __global__ void __launch_bounds__(AW_THREADS, 3) attend_window_kernel(AttendArgs
   // ---- the merge: a warp a row, a lane four channels, eight states of memory on their way at once
   float(*const xs)[TQ_D] = (float(*)[TQ_D])sh.kv[0][1];  // rows in code space, in the original basis
   float(*const hs)[TQ_D] = (float(*)[TQ_D])sh.kv[1][1];
-  const bool general = a.shared.left[head] != 0;  // (its two states)
-  const int np = general ? 2 : a.shared.ns, np_cold = general ? 1 : a.shared.ns_cold;
+  const bool behind = a.shared.slots != nullptr, general = behind && a.shared.left[head] != 0;  // (general: its two states)
+  const int np = general ? 2 : behind ? a.shared.ns : 0, np_cold = general ? 1 : a.shared.ns_cold;
   const int stride = general ? TQ_PART_STRIDE : TQ_SLOT_STRIDE, skip = general ? 2 : 4;
   const size_t of_unit = (size_t)head * a.before_rows + (size_t)s * a.rows;
   const float* const prefix = (general ? a.shared.general : a.shared.slots) + of_unit * np * stride;
@@ -288,10 +289,11 @@ __global__ void __launch_bounds__(AW_THREADS, 3) attend_window_kernel(AttendArgs
         if (a.ns_cold == 0) break;
         const ArPlan* plan = (const ArPlan*)a.plan;
         const int4 seq = plan->seq[s];
+        const int of_row = a.listed ? row / G * ((G + blocks_tile - 1) / blocks_tile) + row % G / blocks_tile : row / blocks_tile;
         n = 0;
-        if (seq.x > 0 && row / blocks_tile < seq.z) {
+        if (seq.x > 0 && of_row < seq.z) {
           const int cost = ar_cost(a.q_dtype != TQ_BF16);
-          const int64_t begin = plan->cum[s] + (int64_t)(head * seq.z + row / blocks_tile) * cost * seq.x;
+          const int64_t begin = plan->cum[s] + (int64_t)(head * seq.z + of_row) * cost * seq.x;
           n = (int)(ar_div(begin + cost * (seq.x - 1), plan->share) - ar_div(begin, plan->share)) + 1;
         }
         base = attend_partial(a, unit, row, 0), step = TQ_PART_STRIDE, head_of = 2, nc = n;
