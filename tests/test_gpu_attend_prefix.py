@@ -342,3 +342,27 @@ def test_what_a_step_refuses_is_not_appended(torch):
         with pytest.raises(ValueError):
             ctx.step(0, q, k, k, f, seq_begin=1, **bad)
     assert [ctx.lengths(0, s)[0] for s in range(3)] == [0, 0, 0]
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("tile", [0, 1, 5])
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(torch, dtype, tile):
+    """The test hook withholds the keys of a tile of the prefix and shortens the probe limit: the call returns, the status word
+    has bit 1, and nothing of it is left."""
+    from turboquant_pro_b200._lib import TqError
+
+    gen = torch.Generator(device="cuda").manual_seed(61)
+    # (enough heads that a CTA has a dozen tiles)
+    ctx = _ctx(n_seqs=21, n_kv_heads=37, n_q_heads=37 * 8, kv_dtype=dtype, hot_window=300, max_tokens_per_seq=4000)
+    _fill(torch, ctx, [40] * 20 + [3900], gen)
+    q = torch.randn(20, 1, 37 * 8, 128, generator=gen, device="cuda").to(getattr(torch, dtype))
+    good = ctx.attend(0, q, prefix=20)
+    assert ctx.status() == 0
+    ctx.debug_wait(wait_limit=64, withhold_tile=tile)
+    ctx.attend(0, q, prefix=20)
+    with pytest.raises(TqError, match="wait"):
+        ctx.raise_on_timeout()
+    assert ctx.status() == 0
+    ctx.debug_wait()
+    assert torch.equal(ctx.attend(0, q, prefix=20), good)
+    assert ctx.status() == 0
