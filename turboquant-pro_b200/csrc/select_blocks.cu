@@ -9,10 +9,15 @@
 // the order of a sum.
 //
 // A cluster of up to eight CTAs takes one (sequence, KV head) and up to eight query tokens: the CTAs divide the
-// blocks, eight lanes a block (a 128-byte line of scales, one of zero-points at a time, for all tokens), and leave the scores
-// in the shared memory of the CTA that chooses for the token (in the workspace where they do not fit).  The choice is
-// a radix selection from the highest bit in which the scores differ on: the threshold, eight bits at a time,
-// then the indices above it in order.
+// blocks, sixteen lanes two blocks and two tokens at a time, and leave the scores in the shared memory of the CTA that chooses
+// for the token (in the workspace where they do not fit).  Up to 128 blocks are counted, a thread a block; of more the choice is
+// a radix selection from the highest bit in which the scores differ on: the threshold, eight bits at a time, then
+// the indices above it in order.
+//
+// What bounds it is not its bytes (a 28th of a page) but its own steps one after the other, each from a cold cache: the launch of
+// a cluster, queries, blocks, choice.  8 heads of 31 blocks, one token: 7.3 us (2900 cycles to the queries' sums, 1800 for the
+// scores, 2000 for the choice); 128 units of 3 to 127 blocks: 11.5 us; 16 units of 512 blocks, five tokens: 17.5 us, 24.3 with
+// one block and one token at a time, where the sums were read from shared memory four times as often.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -25,8 +30,9 @@ namespace {
 
 constexpr int SB_THREADS = 256, SB_WARPS = SB_THREADS / 32;
 constexpr int SB_TOKENS = 8;                 // query tokens of a cluster
-constexpr int SB_LANES = 8;                  // lanes of a block
-constexpr int SB_SWEEP = SB_THREADS / SB_LANES;  // blocks of a CTA at once
+constexpr int SB_LANES = 16;                 // lanes of a block
+constexpr int SB_SWEEP = 2 * SB_THREADS / SB_LANES;  // blocks of a CTA at once, two a thread
+constexpr int SB_COUNTED = 128;              // blocks up to which the choice is by counting
 constexpr size_t SB_SHARED = 96 * 1024;      // most bytes of queries and scores in shared memory
 
 typedef unsigned long long u64;
@@ -49,11 +55,16 @@ TQ_DEV u64 sb_key(double x) {
   return x == x ? (b >> 63 ? ~b : b | 1ull << 63) : 0ull;
 }
 
+// a channel's place in a row of 128: lane l of a block's 16 has channels 4 l + 0 .. 3 and 64 + 4 l + 0 .. 3, and what the 16 read
+// at once is 256 bytes in a row
+TQ_DEV int sb_place(int d) { return (d & 64) | (d & 2) << 4 | (d & 60) >> 1 | (d & 1); }
+
 struct SelectShared {
   uint32_t hist[256];
   u64 most[SB_WARPS], least[SB_WARPS];
   uint32_t ties[SB_WARPS], taken[SB_WARPS];
   uint32_t digit, above, at;
+  int own[SB_TOKENS];  // block of a token's position, or -1
 };
 
 // The n highest of keys[0 .. m), ties to the lowest index, their indices in order to out[0 .. n), and -1 behind them.
@@ -61,6 +72,26 @@ TQ_DEV void sb_choose(const u64* keys, int m, int n, int always, int32_t* out, S
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (m <= n) {
     for (int i = tid; i < n; i += SB_THREADS) out[i] = i < m ? i : -1;
+    return;
+  }
+  if (m <= SB_COUNTED) {  // a thread a key: how many come before it
+    const u64 mine = tid < m ? keys[tid] : 0ull;
+    int before = 0;
+    if (32 * warp < m) {
+#pragma unroll 4
+      for (int j = 0; j < m; ++j) {
+        const u64 k = keys[j];
+        before += k > mine || (k == mine && j < tid);
+      }
+    }
+    const bool in = tid < m && before < n;
+    const uint32_t of_in = __ballot_sync(0xffffffffu, in);
+    __syncthreads();  // (the choice before has been read)
+    if (lane == 0) sh.taken[warp] = __popc(of_in);
+    __syncthreads();
+    int to = __popc(of_in & ((1u << lane) - 1u));
+    for (int w = 0; w < warp; ++w) to += sh.taken[w];
+    if (in) out[to] = tid;
     return;
   }
   // chosen: (key & mask) above `prefix`, and of those at it the first `need`
@@ -88,7 +119,7 @@ TQ_DEV void sb_choose(const u64* keys, int m, int n, int always, int32_t* out, S
     while (bits > 0) {
       const int shift = max(bits - 8, 0);
       const u64 field = (1ull << (bits - shift)) - 1ull;
-      sh.hist[tid] = 0u;
+      if (tid < 256) sh.hist[tid] = 0u;
       __syncthreads();
       for (int i = tid; i < m; i += SB_THREADS) {
         const u64 k = keys[i];
@@ -159,6 +190,7 @@ TQ_DEV void sb_choose(const u64* keys, int m, int n, int always, int32_t* out, S
   }
 }
 
+template <int DT>
 __global__ void __launch_bounds__(SB_THREADS, 2) select_blocks_kernel(SelectArgs a) {
   extern __shared__ __align__(16) uint8_t sb_smem[];
   __shared__ SelectShared sh;
@@ -171,6 +203,13 @@ __global__ void __launch_bounds__(SB_THREADS, 2) select_blocks_kernel(SelectArgs
   double* const of_mean = (double*)sb_smem;              // [tokens][128]: P + N
   double* const of_scale = of_mean + a.tokens * TQ_D;    // hi P + lo N
   u64* const mine = (u64*)(of_scale + a.tokens * TQ_D);  // scores of tokens rank, rank + cluster, ...
+  // all of the queries on their way at once (a thread waits for a few heads of one token at a time)
+  constexpr int LINES = TQ_D * (DT == TQ_F32 ? 4 : 2) / 64;
+  for (int i = tid; i < tokens * G * LINES; i += SB_THREADS) {
+    const int64_t at = (int64_t)s * r.q_seq_stride + (int64_t)(t0 + i / LINES / G) * r.q_tok_stride +
+                       (int64_t)(head * G + i / LINES % G) * r.q_head_stride + i % LINES * (TQ_D / LINES);
+    asm volatile("prefetch.global.L2 [%0];" ::"l"((const uint8_t*)r.q + at * (DT == TQ_F32 ? 4 : 2)));
+  }
   const int n = a.seq_len[(size_t)r.layer * g.n_seqs + r.seq_begin + s];
   const int q_n = r.q_lens == nullptr ? r.n_tokens : min(max(r.q_lens[s], 0), r.n_tokens);
   const int nb = min(n_cold_blocks(n, g.hot_window, S), a.cap);
@@ -181,56 +220,91 @@ __global__ void __launch_bounds__(SB_THREADS, 2) select_blocks_kernel(SelectArgs
     return p < 0 ? 0 : min(nb, p / S + 1);
   };
 
-  for (int i = tid; i < tokens * TQ_D; i += SB_THREADS) {
-    const int t = i / TQ_D, d = i % TQ_D;
+  cg::cluster_group cluster = cg::this_cluster();
+  auto there = cluster.barrier_arrive();  // (before another CTA's shared memory is written, it has to be there)
+  // the first blocks' lines, on their way while the queries are summed (pages that there may be, whatever the length)
+  const int sub = lane % SB_LANES;
+  const uint8_t* const pages = a.pages + page_offset(g, r.layer, r.seq_begin + s, head, 0);
+  float4 m4[2][2], s4[2][2];  // [block][channels]
+  auto fetch = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* page = pages + (size_t)min(b + i * (SB_SWEEP / 2), a.cap - 1) * g.page_bytes + 16 * sub;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        m4[i][j] = *(const float4*)(page + g.mean_off + 256 * j);
+        s4[i][j] = *(const float4*)(page + g.scale_off + 256 * j);
+      }
+    }
+  };
+  if (g.max_blocks > 0) fetch(rank * SB_SWEEP + tid / SB_LANES);
+  if (tid < tokens) sh.own[tid] = position(tid) < 0 ? -1 : position(tid) / S;
+  // (a half-warp has 16 channels and every second head of the group)
+#pragma unroll 2
+  for (int i = tid; i < tokens * 2 * TQ_D; i += SB_THREADS) {
+    const int t = i / (2 * TQ_D), d = i / 32 % 8 * 16 + lane % 16;
     const int64_t at = (int64_t)s * r.q_seq_stride + (int64_t)(t0 + t) * r.q_tok_stride +
                        (int64_t)(head * G) * r.q_head_stride + d;
     double up = 0.0, down = 0.0;
-    for (int k = 0; k < G; ++k) {
-      const float x = attend_ld(r.q, (size_t)(at + k * r.q_head_stride), r.q_dtype);
+#pragma unroll 4
+    for (int k = lane / 16; k < G; k += 2) {
+      const float x = attend_ld(r.q, (size_t)(at + k * r.q_head_stride), DT);
       up += x > 0.0f ? (double)x : 0.0;
       down += x > 0.0f ? 0.0 : (double)x;
     }
-    of_mean[i] = up + down;
-    of_scale[i] = a.hi * up + a.lo * down;
+    up += __shfl_xor_sync(0xffffffffu, up, 16), down += __shfl_xor_sync(0xffffffffu, down, 16);
+    const int to = t * TQ_D + sb_place(d);
+    if (lane < 16) of_mean[to] = up + down;
+    else of_scale[to] = a.hi * up + a.lo * down;
   }
-  cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();  // (every CTA of the cluster is there)
+  __syncthreads();
+  cluster.barrier_wait(std::move(there));
 
-  // ---- scores: eight lanes a block
+  // ---- scores: sixteen lanes two blocks
   auto scores_of = [&](int t) -> u64* {
     if (a.scores != nullptr) return a.scores + ((size_t)id * a.tokens + t) * a.cap;
-    return (u64*)cluster.map_shared_rank(mine, t % a.cluster) + (size_t)(t / a.cluster) * a.cap;
+    return (u64*)cluster.map_shared_rank(mine, t & (a.cluster - 1)) + (size_t)(t >> (31 - __clz(a.cluster))) * a.cap;
   };
   const int last = min(tokens, q_n - t0) - 1, most = last >= 0 ? candidates(last) : 0;
-  const int sub = lane % SB_LANES;
   for (int b0 = rank * SB_SWEEP; b0 < most; b0 += a.cluster * SB_SWEEP) {
     const int b = b0 + tid / SB_LANES;
-    const uint8_t* page = a.pages + page_offset(g, r.layer, r.seq_begin + s, head, min(b, nb - 1));
-    float4 m4[4], s4[4];
+    if (b0 != rank * SB_SWEEP) fetch(b);
+    double md[2][8], sd[2][8];  // (converted once, not for each token)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      m4[j] = *(const float4*)(page + g.mean_off + (32 * j + 4 * sub) * 4);
-      s4[j] = *(const float4*)(page + g.scale_off + (32 * j + 4 * sub) * 4);
-    }
-    for (int t = 0; t < tokens; ++t) {
-      double x = 0.0;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const double2* u = (const double2*)(of_mean + t * TQ_D + 32 * j + 4 * sub);
-        const double2* v = (const double2*)(of_scale + t * TQ_D + 32 * j + 4 * sub);
-        const double2 u0 = u[0], u1 = u[1], v0 = v[0], v1 = v[1];
-        x = fma(u0.x, (double)m4[j].x, x), x = fma(u0.y, (double)m4[j].y, x);
-        x = fma(u1.x, (double)m4[j].z, x), x = fma(u1.y, (double)m4[j].w, x);
-        x = fma(v0.x, (double)s4[j].x, x), x = fma(v0.y, (double)s4[j].y, x);
-        x = fma(v1.x, (double)s4[j].z, x), x = fma(v1.y, (double)s4[j].w, x);
+      for (int j = 0; j < 2; ++j) {
+        md[i][4 * j] = m4[i][j].x, md[i][4 * j + 1] = m4[i][j].y, md[i][4 * j + 2] = m4[i][j].z, md[i][4 * j + 3] = m4[i][j].w;
+        sd[i][4 * j] = s4[i][j].x, sd[i][4 * j + 1] = s4[i][j].y, sd[i][4 * j + 2] = s4[i][j].z, sd[i][4 * j + 3] = s4[i][j].w;
       }
+    // two tokens at a time: four sums, so that none waits for itself, from what is read of the queries once
+#pragma unroll 1
+    for (int t = 0; t < tokens; t += 2) {
+      double x[2][2] = {};  // [block][token]
 #pragma unroll
-      for (int o = 1; o < SB_LANES; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-      if (sub == 0 && b < nb) {
-        const int p = position(t);
-        scores_of(t)[b] = b < r.first || b == p / S ? SB_ALWAYS : sb_key(x);
-      }
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int at = (k == 0 ? t : min(t + 1, tokens - 1)) * TQ_D + 32 * j + 2 * sub;
+          const double2 u = *(const double2*)(of_mean + at), v = *(const double2*)(of_scale + at);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            x[i][k] = fma(u.x, md[i][2 * j], x[i][k]), x[i][k] = fma(u.y, md[i][2 * j + 1], x[i][k]);
+            x[i][k] = fma(v.x, sd[i][2 * j], x[i][k]), x[i][k] = fma(v.y, sd[i][2 * j + 1], x[i][k]);
+          }
+        }
+      // over the block's lanes; each half keeps a block, each quarter a token of it
+      const int of_block = sub >> 3, of_token = sub >> 2 & 1;
+      double y[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        y[k] = (of_block ? x[1][k] : x[0][k]) + __shfl_xor_sync(0xffffffffu, of_block ? x[0][k] : x[1][k], 8);
+      double z = (of_token ? y[1] : y[0]) + __shfl_xor_sync(0xffffffffu, of_token ? y[0] : y[1], 4);
+      z += __shfl_xor_sync(0xffffffffu, z, 2);
+      z += __shfl_xor_sync(0xffffffffu, z, 1);
+      const int at_t = t + of_token, at_b = b + of_block * (SB_SWEEP / 2);
+      if ((sub & 3) == 0 && at_t < tokens && at_b < nb)
+        scores_of(at_t)[at_b] = at_b < r.first || at_b == sh.own[at_t] ? SB_ALWAYS : sb_key(z);
     }
   }
   cluster.sync();
@@ -288,6 +362,25 @@ Plan make_plan(const tq_ctx* ctx, const tq_select_args* r, cudaStream_t st) {
   return p;
 }
 
+template <int DT>
+int launch(const tq_ctx* ctx, const SelectArgs& a, const Plan& p, int grid, cudaStream_t st) {
+  static bool done[64];
+  const int rc = attend_shared(select_blocks_kernel<DT>, SB_SHARED, ctx->device, done);
+  if (rc != TQ_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = p.cluster, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(SB_THREADS);
+  cfg.dynamicSmemBytes = p.shared_bytes;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  TQ_CUDA(cudaLaunchKernelEx(&cfg, select_blocks_kernel<DT>, a));
+  return TQ_OK;
+}
+
 }  // namespace
 
 extern "C" int32_t tq_select_blocks_workspace(tq_ctx* ctx, const tq_select_args* r, void* stream, size_t* bytes) {
@@ -312,9 +405,6 @@ extern "C" int32_t tq_select_blocks(tq_ctx* ctx, const tq_select_args* r, void* 
   const int64_t grid = (int64_t)r->seq_count * g.n_kv_heads * p.groups * p.cluster;
   TQ_REQUIRE(grid <= INT_MAX, TQ_ERR_UNSUPPORTED, "too many (sequence, head, query token) items in a call");
   TQ_CUDA(cudaSetDevice(ctx->device));
-  static bool done[64];
-  const int rc2 = attend_shared(select_blocks_kernel, SB_SHARED, ctx->device, done);
-  if (rc2 != TQ_OK) return rc2;
   SelectArgs a;
   a.g = g;
   a.pages = (const uint8_t*)ctx->b.pages;
@@ -323,17 +413,10 @@ extern "C" int32_t tq_select_blocks(tq_ctx* ctx, const tq_select_args* r, void* 
   a.lo = g.key_mode == TQ_KEYS_UNIFORM ? 0.0 : -1.0, a.hi = g.key_mode == TQ_KEYS_UNIFORM ? 15.0 : 1.0;
   a.scores = p.shared ? nullptr : (u64*)r->workspace;
   a.cap = p.cap, a.tokens = p.tokens, a.groups = p.groups, a.cluster = p.cluster;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = p.cluster, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(SB_THREADS);
-  cfg.dynamicSmemBytes = p.shared_bytes;
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  TQ_CUDA(cudaLaunchKernelEx(&cfg, select_blocks_kernel, a));
+  const int rc2 = r->q_dtype == TQ_F32 ? launch<TQ_F32>(ctx, a, p, (int)grid, st)
+                  : r->q_dtype == TQ_F16 ? launch<TQ_F16>(ctx, a, p, (int)grid, st)
+                                         : launch<TQ_BF16>(ctx, a, p, (int)grid, st);
+  if (rc2 != TQ_OK) return rc2;
   ctx->last_launches = 1;
   return TQ_OK;
 }
