@@ -224,6 +224,32 @@ def test_orders_parts_of_the_batch_and_out(torch):
         _check(torch, ctx, ctx.attend(0, q[:1], prefix=2, seq_begin=0), q[:1], 2, seq_begin=0)
 
 
+@pytest.mark.parametrize("case", [CASES[2], CASES[5], CASES[11], CASES[18]], ids=str)
+def test_rounds(torch, case):
+    import ctypes as C
+
+    from turboquant_pro_b200._lib import TqAttendArgs
+
+    ctx, q, _ = _build(torch, case, 9)
+    b, t = q.shape[:2]
+    a, size = TqAttendArgs(), C.c_size_t()
+    a.n_tokens, a.q_dtype, a.seq_begin, a.seq_count = t, {"float32": 0, "float16": 1, "bfloat16": 2}[case[6]], 1, b
+    a.q_seq_stride, a.q_tok_stride, a.q_head_stride = q.stride()[:3]
+    assert ctx._lib.tq_attend_prefix_workspace(ctx._h, C.byref(a), 0, None, C.byref(size)) == 0
+    whole, one = size.value, 0
+    a.seq_count = 1
+    for s in range(b):
+        a.seq_begin = 1 + s
+        assert ctx._lib.tq_attend_prefix_workspace(ctx._h, C.byref(a), 0, None, C.byref(size)) == 0
+        one = max(one, size.value)
+    want = ctx.attend(0, q, prefix=0, seq_begin=1)
+    assert torch.equal(ctx.attend(0, q, prefix=0, seq_begin=1, max_workspace=whole), want)
+    for most in (one, (one + whole) // 2, whole - 1):
+        if one <= most < whole:
+            _check(torch, ctx, ctx.attend(0, q, prefix=0, seq_begin=1, max_workspace=most), q, 0, seq_begin=1)
+    assert ctx.status() == 0
+
+
 def test_captured_calls_follow_the_lengths(torch):
     for case in (([100, 700, 9], 600, 1, 2, 8, "bfloat16", "bfloat16", 512, "nf4_asym", 3),
                  ([300] * 12, 600, 5, 1, 8, "bfloat16", "bfloat16", 512, "nf4_asym", 3)):

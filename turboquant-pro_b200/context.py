@@ -1008,8 +1008,8 @@ class KVContext:
         return {0: "none", 1: "tensor-core", 2: "general"}[int(self._lib.tq_last_kernel(self._h))]
 
     def debug_wait(self, wait_limit: int = 0, withhold_tile: int = -1) -> None:
-        """Test hook of the bounded waits of the decode kernel, of :meth:`attend` with many rows and of the
-        encoders: a shorter probe limit and a tile (a row) of the first CTA that is never started (see
+        """Test hook of the bounded waits of the decode kernel, of :meth:`attend` with many rows or a ``prefix`` and
+        of the encoders: a shorter probe limit and a tile (a row) of the first CTA that is never started (see
         ``tq_debug_wait``)."""
         check(self._lib.tq_debug_wait(self._h, int(wait_limit), int(withhold_tile)))
 

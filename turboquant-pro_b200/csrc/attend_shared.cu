@@ -6,7 +6,7 @@
 //     Eight warps turn codes into the two operands in shared memory (fp16, K-major core matrices of 8 rows x 16
 //     bytes); a warp per half of 128 rows issues S = Q K^T and O += P V; a thread per row makes the probabilities, which
 //     stay in tensor memory.  Codes are decoded where they are used: the operands, four times as large, never leave the SM.
-//       keys    (mean - c + scale * grid[code]) times a power of two per page, two channels a look-up and one multiply-add in
+//       keys    (mean - c + scale * grid[code]) times a power of two per CTA, two channels a look-up and one multiply-add in
 //               float32, outliers put over it.  c is one vector per head, the zero-point of the first block: it moves all
 //               scores of a row alike; what it takes off goes back into the state's maximum.
 //       values  in code space, norm * centroid[code] times a power of two per tile: two tokens of a channel a look-up.
@@ -15,9 +15,16 @@
 //     its own.  The same 32768 tokens with three channels 20 times the others: 2.5e-3 -> 1.7e-3 off, rounding the exact
 //     result gives 1.65e-3.
 //     The uncompressed window is the work of CTAs of its own, whose sums are in the original basis.
-//     A page whose grid spans more than 2^20, an outlier that is 64 times its grid, window tokens below 2^-20 of their
-//     tile's largest, and what is no number set the flag of their head, which the general kernel then does.
-// attend_shared_merge_kernel   merges a row's states in order, rotates what is in code space, and leaves one state a row.
+//     Pages whose grids span more than 2^20 in a CTA's part, an outlier that is 64 times its grid, window tokens below 2^-20 of
+//     their tile's largest, and what is no number set the flag of their head, which the general kernel then does.
+//     What bounds it: 64 tokens take 3000 cycles for 256 rows (32768 tokens, 8 heads of 512 rows: 130 us, 0.53 PFLOP/s; 8192 and 128
+//     rows 33 us; float16, 12345 tokens, 4 heads of 231 rows: 40).  The makers are busy for 2000 of them, the exponentials of
+//     the two halves for 1150 each, the products for 1090, and a ring of three stages, for which there is shared memory, ties
+//     them together; 48 % of the issue slots are used.  Exponentials of both halves at once, or more of them on the
+//     multiply-add units, measured the same.  Why 256 rows: codes are decoded once for all of a CTA's rows, and
+//     tensor memory holds two halves' scores, probabilities and sums.
+// attend_shared_merge_kernel   for other forms of the sequences' own tokens than few rows: merges a row's states in order,
+//     rotates what is in code space, and leaves one state a row.
 #include <algorithm>
 
 #include "attend_tc.cuh"
