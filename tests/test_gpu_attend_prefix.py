@@ -37,7 +37,7 @@ def _fill(torch, ctx, lens, gen, layer=0):
             ctx.append(layer, k.to(ctx.kv_dtype), v[None].to(ctx.kv_dtype), seq_begin=seq)
 
 
-def _check(torch, ctx, got, q, prefix, q_lens=None, seq_begin=0, layer=0):
+def _check(torch, ctx, got, q, prefix, q_lens=None, seq_begin=0, layer=0, by_head=1.0):
     assert got.shape == q.shape and got.dtype == q.dtype
     m = ctx.lengths(layer, prefix)[0]
     pk, pv = ctx.dequant(layer, prefix, 0, m)
@@ -52,7 +52,9 @@ def _check(torch, ctx, got, q, prefix, q_lens=None, seq_begin=0, layer=0):
         assert not bool(got[s, :skip].any()) and not bool(got[s, q_n:].any())
         if q_n > skip:
             want = oracle.attention(k, v, q[s, skip:q_n], q_n - skip, None, 0)
-            oracle.check(got[s, skip:q_n], want)
+            head, row = oracle.measures(got[s, skip:q_n], want)
+            most_head, most_row = oracle.limits(got.dtype)
+            assert head <= by_head * most_head and row <= most_row, (head / most_head, row / most_row)
 
 
 CASES = [
@@ -224,6 +226,14 @@ def test_orders_parts_of_the_batch_and_out(torch):
         _check(torch, ctx, ctx.attend(0, q[:1], prefix=2, seq_begin=0), q[:1], 2, seq_begin=0)
 
 
+# A head of few rows (two a sequence), float16.  The limit by head counts a probability's rounding as 0.42 of eps / 2, its mean square over
+# many.  A row's error is e = sum_j d_j p_j v_j with |d_j| <= eps / 2 (half a step, next to a power of two), and its output o = sum_j
+# p_j v_j: with v_j independent, of 128 channels and so nearly orthogonal, |e|^2 = sum d_j^2 p_j^2 |v_j|^2 <= (eps / 2)^2 |o|^2,
+# which a row comes to whose output is mostly that of one token (50 times as large as the others).  With the output's own rounding,
+# 0.42 as ever: sqrt(1 + 0.42^2) = 1.085.
+FEW_ROWS = 1.085
+
+
 @pytest.mark.parametrize("case", [CASES[2], CASES[5], CASES[11], CASES[18]], ids=str)
 def test_rounds(torch, case):
     import ctypes as C
@@ -246,7 +256,15 @@ def test_rounds(torch, case):
     assert torch.equal(ctx.attend(0, q, prefix=0, seq_begin=1, max_workspace=whole), want)
     for most in (one, (one + whole) // 2, whole - 1):
         if one <= most < whole:
-            _check(torch, ctx, ctx.attend(0, q, prefix=0, seq_begin=1, max_workspace=most), q, 0, seq_begin=1)
+            got = ctx.attend(0, q, prefix=0, seq_begin=1, max_workspace=most)
+            _check(torch, ctx, got, q, 0, seq_begin=1, by_head=FEW_ROWS if case[6] == "float16" else 1.0)
+            # the same as calls of so many sequences
+            n, same = b, False
+            while not same and n > 1:
+                n = (n + 1) // 2
+                parts = [ctx.attend(0, q[i:i + n], prefix=0, seq_begin=1 + i) for i in range(0, b, n)]
+                same = torch.equal(torch.cat(parts), got)
+            assert same
     assert ctx.status() == 0
 
 
