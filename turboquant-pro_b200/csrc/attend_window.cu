@@ -9,8 +9,10 @@
 // are merged in shared memory, with those of memory; what is in code space is rotated by Pi.
 //   An infinity or a NaN among the values spoils sums of rows that do not see it (0 * inf), and those of its low parts: a warp whose
 // sums are not all finite does its tiles again, term by term.
-//   (The form for few rows, whose kernel is made for blocks, took 27 us for the windows of 4 sequences and 45 for those of
-// 64, 8 KV heads, and its merge 10 and 28.)
+//   What bounds it: latencies of one thing after the other.  64 sequences with windows of up to 500 tokens, 8 KV heads of 8 rows, ten
+// states a row: 41 us, two waves of CTAs of 20 us each: lengths and queries 5900 cycles, window 11400, merge 10000, rotation 7800.
+// 32 x 8 heads of 4 rows 22 us, 4 x 8 12.5.  (The form for few rows, whose kernel is made for blocks, took 27 us for the windows
+// of 4 sequences and 45 for those of 64, 8 KV heads, and its merge 10 and 28.)  Rotating four rows at a time cost 4 us more of the 41.
 #include <algorithm>
 
 #include "attend.cuh"
@@ -258,7 +260,7 @@ __global__ void __launch_bounds__(AW_THREADS, 3) attend_window_kernel(AttendArgs
   __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  // ---- the merge: a warp a row, a lane four channels, eight states of memory on their way at once
+  // ---- the merge: a warp a row, a lane four channels, ten states of memory on their way at once
   float(*const xs)[TQ_D] = (float(*)[TQ_D])sh.kv[0][1];  // rows in code space, in the original basis
   float(*const hs)[TQ_D] = (float(*)[TQ_D])sh.kv[1][1];
   const bool behind = a.shared.slots != nullptr, general = behind && a.shared.left[head] != 0;  // (general: its two states)
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(AW_THREADS, 3) attend_window_kernel(AttendArgs
         }
         base = attend_partial(a, unit, row, 0), step = TQ_PART_STRIDE, head_of = 2, nc = n;
       }
-      constexpr int BATCH = 8;
+      constexpr int BATCH = 10;
 #pragma unroll 1
       for (int i0 = 0; i0 < n; i0 += BATCH) {
         float2 ml[BATCH], u[BATCH], v[BATCH];
@@ -340,18 +342,21 @@ __global__ void __launch_bounds__(AW_THREADS, 3) attend_window_kernel(AttendArgs
     if (lane == 0) sh.of_l[k] = L;
   }
   __syncthreads();
-  // ---- the rotation: a thread a channel, four rows at a time
+  // ---- the rotation: a thread a channel, eight rows at a time
   const int e = tid;
 #pragma unroll 1
-  for (int k0 = 0; k0 < rows; k0 += 4) {
-    uint64_t y[4] = {0ull, 0ull, 0ull, 0ull};  // (even and odd channels)
+  for (int k0 = 0; k0 < rows; k0 += 8) {
+    uint64_t y[8];  // (even and odd channels)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = 0ull;
 #pragma unroll 1
     for (int d = 0; d < TQ_D; d += 32) {
       uint64_t pi[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) pi[i] = aw_f2(a.tables->pi[(d + 2 * i) * TQ_D + e], a.tables->pi[(d + 2 * i + 1) * TQ_D + e]);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 8; ++k) {
+        if (k == 4 && rows - k0 <= 4) break;
         uint64_t z = 0ull;  // (32 at a time: a sum over all 128 in a row would be rounded at its full size 128 times)
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(AW_THREADS, 3) attend_window_kernel(AttendArgs
       }
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)  // (rows that there are not: of no use, and in place)
+    for (int k = 0; k < 8; ++k)  // (rows that there are not: of no use, and in place)
       hs[k0 + k][e] += __uint_as_float((uint32_t)y[k]) + __uint_as_float((uint32_t)(y[k] >> 32));
   }
   int i = row0 / G, gh = row0 - i * G;  // query token and head of the group
