@@ -138,16 +138,18 @@ TQ_DEV const float* attend_before(const AttendArgs& a, int s, int head, int row)
   if (a.before == nullptr || attend_position(a, attend_seq(a, s), row) < 0) return nullptr;
   return a.before + ((size_t)head * a.before_rows + (size_t)s * a.rows + row) * TQ_PART_STRIDE;
 }
-// Channel e of a merged row (maximum M, sum of weights L, sum of weighted values o) as the call's result.
+// Channel e of a merged row (maximum M, sum of weights L, sum of weighted values o) as the call's result.  PLAIN: no states of a
+// shared beginning, neither given nor wanted.
+template <bool PLAIN = false>
 TQ_DEV void attend_result(const AttendArgs& a, int s, int head, int row, int e, float M, float L, float o) {
   const tq_geom& g = a.g;
-  if (a.states != nullptr) {
+  if (!PLAIN && a.states != nullptr) {
     float* to = a.states + ((size_t)(s * g.n_kv_heads + head) * a.rows + row) * TQ_PART_STRIDE;
     if (e == 0) *(float2*)to = make_float2(M, L);
     to[2 + e] = o;
     return;
   }
-  if (const float* x = attend_before(a, s, head, row)) {
+  if (const float* x = PLAIN ? nullptr : attend_before(a, s, head, row)) {
     const float top = fmaxf(M, x[0]), by = top > -INFINITY ? top : 0.0f;
     const float w = attend_weight(M, L, by), wx = attend_weight(x[0], x[1], by);
     L = (w != 0.0f ? L * w : 0.0f) + (wx != 0.0f ? x[1] * wx : 0.0f);

@@ -183,7 +183,8 @@ TQ_DEV uint4 nr_head(const NrLane<DT>& n, const uint4& raw, bool normed, float e
   return nr_pack<DT>(y);
 }
 
-template <int DT, bool PAIRED, bool VEC>
+// MORE: several axes, or a prefix
+template <int DT, bool PAIRED, bool VEC, bool MORE>
 __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(RopeArgs a, int tokens, int per_cta) {
   using T = typename Elem<DT>::type;
   using Lane = NrLane<DT>;
@@ -232,10 +233,10 @@ __global__ void __launch_bounds__(NR_THREADS, 3) norm_rope_kernel(RopeArgs a, in
     int64_t p;
     if (a.seq_len != nullptr) {
       p = (int64_t)a.seq_len[us] + ut;
-      if (a.before != nullptr) p += *a.before;
+      if (MORE && a.before != nullptr) p += *a.before;
     } else {
       int64_t at = (int64_t)us * r.pos_seq_stride + (int64_t)ut * r.pos_tok_stride;
-      if (a.x.axes != nullptr) at += min((int)a.x.axes[f], a.x.n_axes - 1) * a.x.pos_axis_stride;
+      if (MORE && a.x.axes != nullptr) at += min((int)a.x.axes[f], a.x.n_axes - 1) * a.x.pos_axis_stride;
       p = r.pos_bits == 64 ? ((const int64_t*)r.positions)[at] : (int64_t)((const int32_t*)r.positions)[at];
     }
     const double turns = (double)p * ((double)r.inv_freq[f] * 0.15915494309189533577);
@@ -281,8 +282,10 @@ void start(const RopeArgs& a, int tokens, int sm_count, bool vec, cudaStream_t s
   int per_cta = 1;
   while (per_cta < NR_THREADS / 32 && tokens > per_cta * resident) per_cta *= 2;
   const int grid = (int)(((int64_t)tokens + per_cta - 1) / per_cta);
-  if (vec) norm_rope_kernel<DT, PAIRED, true><<<grid, NR_THREADS, 0, st>>>(a, tokens, per_cta);
-  else norm_rope_kernel<DT, PAIRED, false><<<grid, NR_THREADS, 0, st>>>(a, tokens, per_cta);
+  const bool more = a.before != nullptr || a.x.axes != nullptr;
+  const auto kernel = vec ? more ? norm_rope_kernel<DT, PAIRED, true, true> : norm_rope_kernel<DT, PAIRED, true, false>
+                          : more ? norm_rope_kernel<DT, PAIRED, false, true> : norm_rope_kernel<DT, PAIRED, false, false>;
+  kernel<<<grid, NR_THREADS, 0, st>>>(a, tokens, per_cta);
 }
 
 int check_rope(const tq_rope* r, bool stored) {
