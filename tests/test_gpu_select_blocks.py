@@ -75,6 +75,9 @@ CASES = [
     ([1200], 1, 1, 1, 7, 0, "float32", 512, "nf4"),
     ([900], 2, 1, 4, 1, 5, "bfloat16", 100, "nf4_asym"),
     ([6000], 1, 3, 9, 1, 0, "bfloat16", 100, "nf4_asym"),
+    # about as many blocks as a CTA has threads to count with, and as many as it has threads
+    ([126, 127, 128, 129, 130, 131, 132, 133], 3, 1, 2, 50, 1, "bfloat16", 2, "nf4_asym"),
+    ([255, 256, 257, 258, 259, 260], 9, 2, 6, 129, 3, "float16", 2, "uniform"),
     # more scores than a CTA's shared memory holds
     ([2000] + [0] * 73 + [30], 8, 2, 2, 40, 1, "float16", 2, "nf4_asym"),
 ]
