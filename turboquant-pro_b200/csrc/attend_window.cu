@@ -396,6 +396,10 @@ int tq_launch_attend_window(const AttendArgs& a, int blocks_tile, cudaStream_t s
   const bool bf = a.q_dtype == TQ_BF16;
   static bool done[2][64];
   const auto kernel = bf ? attend_window_kernel<true> : attend_window_kernel<false>;
+  // The kernel reads lengths, queries and windows before it waits for the one that it starts under.  So that has to be one of this
+  // call, whose first comes behind what is in the stream in full order.  Where there is none (lists, and no sequence with a block)
+  // what it would start under is another call's: a ring writer, say, that has not written yet.
+  const bool behind_own = a.ns_cold > 0 || a.shared.slots != nullptr;
   const int rc = attend_shared(kernel, sizeof(AwShared), a.device, done[bf]);
   if (rc != TQ_OK) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -407,7 +411,7 @@ int tq_launch_attend_window(const AttendArgs& a, int blocks_tile, cudaStream_t s
   cfg.dynamicSmemBytes = sizeof(AwShared);
   cfg.stream = st;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = behind_own ? 1 : 0;
   TQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, row_tiles, tile, blocks_tile));
   return TQ_OK;
 }
