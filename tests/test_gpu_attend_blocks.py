@@ -253,3 +253,26 @@ def test_refusals(torch):
             ctx.attend(**{"layer": 0, "q": q, "blocks": blocks, **bad})
     assert ctx.attend(0, q[:, :0], blocks=blocks[:, :0]).shape == (2, 0, 4, 128)
     assert ctx.attend(0, q[:0], blocks=blocks[:0]).shape == (0, 3, 4, 128)
+
+
+def test_workspace_of_calls_whose_window_has_a_kernel_of_its_own(torch):
+    # room for the states of the blocks alone: of one block, shared by many rows, at most three a row
+    import ctypes as C
+
+    from turboquant_pro_b200._lib import TqAttendArgs
+
+    b, t, h, hq = 64, 10, 8, 64
+    ctx, q, gen = _build(torch, ([700] * b, t, h, hq, 1, "bfloat16", "bfloat16", 512, "nf4_asym", 3), 8)
+    lists = _lists(torch, ctx, [700] * b, t, 1, gen)
+    want = ctx.attend(0, q, blocks=lists)
+    assert ctx.last_launches() == 2
+    _check(torch, ctx, want[:3], q[:3], lists[:3])
+    a, size = TqAttendArgs(), C.c_size_t()
+    a.seq_count, a.n_tokens, a.q_dtype = b, t, 2
+    assert ctx._lib.tq_attend_blocks_workspace(ctx._h, C.byref(a), 1, None, C.byref(size)) == 0
+    most = b * t * hq * 3 * (2 + 128) * 4 + 4096  # (and how the work is divided)
+    assert size.value <= most
+    assert torch.equal(ctx.attend(0, q, blocks=lists, max_workspace=most), want)
+    assert ctx.last_launches() == 2
+    ctx.attend(0, q, blocks=lists, max_workspace=most // 2)
+    assert ctx.last_launches() > 2

@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   const int64_t total = sh.cum[AR_SEQS];
   int64_t share = max((total + workers - 1) / workers, (int64_t)COST);
   share = max(share, (int64_t)((COST * sh.most[0] + a.ns_cold - 3) / (a.ns_cold - 2)));
-  share = max(share, (int64_t)((a.hot_cost * sh.most[1] + a.ns_hot - 3) / (a.ns_hot - 2)));
+  if (a.ns_hot > 0) share = max(share, (int64_t)((a.hot_cost * sh.most[1] + a.ns_hot - 3) / (a.ns_hot - 2)));
   if (blockIdx.x == 0) {
     ArPlan* plan = (ArPlan*)a.plan;
     if (tid == 0) plan->share = share;
@@ -1552,7 +1552,7 @@ AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens) {
   p.hot_cost = hot_cost;
   const int64_t share = std::max<int64_t>((cost * strips + hot_cost * hot) * ((rows + 1) / 2) / workers, cost);
   p.ns_cold = (int)std::min<int64_t>(cost * strips / share + 3, 1024);
-  p.ns_hot = (int)std::min<int64_t>(hot_cost * hot / share + 3, 64);
+  p.ns_hot = a.no_window ? 0 : (int)std::min<int64_t>(hot_cost * hot / share + 3, 64);
   return p;
 }
 
