@@ -268,8 +268,8 @@ int32_t tq_norm_rope(const tq_rope* rope, int32_t device, void* stream);
 /* The same for tokens that are about to be appended to sequences seq_begin .. of a layer: their positions
  * follow from the lengths on the device (rope->positions is not looked at). */
 int32_t tq_ctx_norm_rope(tq_ctx* ctx, int32_t layer, int32_t seq_begin, const tq_rope* rope, void* stream);
-/* The same where the sequences go on from sequence `prefix` of the layer: its length is added to their positions (see
- * tq_attend_prefix; -1: none). */
+/* The same where the sequences go on from sequence `prefix` of the layer, none of the call's own: its length is added to
+ * their positions (see tq_attend_prefix; -1: none). */
 int32_t tq_ctx_norm_rope_after(tq_ctx* ctx, int32_t layer, int32_t seq_begin, int32_t prefix, const tq_rope* rope,
                                void* stream);
 /* tq_norm_rope with positions of several axes (the time, height and width of images and video): frequency i turns by

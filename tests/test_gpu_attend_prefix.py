@@ -410,3 +410,20 @@ def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(torch, dtyp
     ctx.debug_wait()
     assert torch.equal(ctx.attend(0, q, prefix=20), good)
     assert ctx.status() == 0
+
+
+def test_a_prefix_among_the_callers_own_sequences_is_refused_below_python_too(torch):
+    import ctypes as C
+
+    from turboquant_pro_b200._lib import TqRope
+
+    ctx = _ctx(n_seqs=5, n_kv_heads=2, n_q_heads=4, kv_dtype="float16")
+    q, k = (torch.randn(2, 3, h, 128, device="cuda").half() for h in (4, 2))
+    out = [torch.empty_like(x) for x in (q, k)]
+    f = _freq(torch)
+    r = TqRope(q.data_ptr(), k.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), None, None, f.data_ptr(), None,
+               *q.stride()[:3], *k.stride()[:3], 0, 0, 2, 3, 4, 2, 1, 0, 64, 128, 1e-6)
+    stream = torch.cuda.current_stream().cuda_stream
+    for prefix, ok in ((-1, True), (0, True), (1, False), (2, False), (3, True), (4, True), (5, False), (-2, False)):
+        assert (ctx._lib.tq_ctx_norm_rope_after(ctx._h, 0, 1, prefix, C.byref(r), stream) == 0) == ok, prefix
+    assert b"prefix" in ctx._lib.tq_last_error()

@@ -366,7 +366,8 @@ extern "C" int32_t tq_ctx_norm_rope_after(tq_ctx* ctx, int32_t layer, int32_t se
              "head counts do not match the context");
   TQ_REQUIRE(seq_begin >= 0 && r->n_seqs >= 0 && (int64_t)seq_begin + r->n_seqs <= g.n_seqs, TQ_ERR_INVALID,
              "sequence range out of bounds");
-  TQ_REQUIRE(prefix >= -1 && prefix < g.n_seqs, TQ_ERR_INVALID, "prefix is no sequence of the context");
+  TQ_REQUIRE(prefix == -1 || (prefix >= 0 && prefix < g.n_seqs && (prefix < seq_begin || prefix >= seq_begin + r->n_seqs)),
+             TQ_ERR_INVALID, "prefix must be a sequence of the context that is none of the call's own");
   TQ_CUDA(cudaSetDevice(ctx->device));
   const int32_t* len = (const int32_t*)((const uint8_t*)ctx->b.state + state_len_off(g)) + (size_t)layer * g.n_seqs;
   return launch(r, len + seq_begin, prefix < 0 ? nullptr : len + prefix, tq_rope_axes{}, ctx->device,
