@@ -427,3 +427,23 @@ def test_a_prefix_among_the_callers_own_sequences_is_refused_below_python_too(to
     for prefix, ok in ((-1, True), (0, True), (1, False), (2, False), (3, True), (4, True), (5, False), (-2, False)):
         assert (ctx._lib.tq_ctx_norm_rope_after(ctx._h, 0, 1, prefix, C.byref(r), stream) == 0) == ok, prefix
     assert b"prefix" in ctx._lib.tq_last_error()
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_a_token_of_no_value_that_has_most_of_the_weight(torch, dtype):
+    """The first token of each window has a score 12 above the others' and a value of zero: the output is what tokens with
+    probabilities of some 1e-6 have, whose digits have to be there."""
+    b, n = 12, 300
+    ctx = _ctx(n_seqs=b + 1, n_kv_heads=2, n_q_heads=8, kv_dtype=dtype)
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    k, v = (torch.randn(b + 1, n, 2, 128, generator=gen, device="cuda") for _ in range(2))
+    q = torch.randn(b, 1, 8, 128, generator=gen, device="cuda")
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[1:, 0, :, 0], v[1:, 0] = 12.0 * 128**0.5 / 8.0, 0.0
+    v *= 2000.0  # (outputs are then some tenths, and keep their digits in float16)
+    k, v, q = (x.to(getattr(torch, dtype)) for x in (k, v, q))
+    ctx.append(0, k, v)
+    got = ctx.attend(0, q, prefix=0, seq_begin=1)
+    assert ctx.last_launches() == 3
+    assert float(got.abs().mean()) > 0.05
+    _check(torch, ctx, got, q, 0, seq_begin=1)

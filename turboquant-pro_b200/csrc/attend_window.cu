@@ -5,8 +5,9 @@
 //
 // A CTA has 8 or 16 rows of a (sequence, KV head); its four warps take tiles of 32 tokens in turn and work alone: keys and values
 // come with cp.async, the next tile's keys while this one's values are summed and the other way round; S = Q K^T and O += P V on
-// mma.sync (m16n8k16) with the rows as they are, so that products are exact; probabilities are pairs hi + lo.  The four states
-// are merged in shared memory, with those of memory; what is in code space is rotated by Pi.
+// mma.sync (m16n8k16) with the rows as they are, so that products are exact; probabilities are pairs hi + lo (float16: of 2^14
+// times their size; behind a first token that has no value and all but 1e-3 of the weight, results were 6.9e-4 off without that).
+// The four states are merged in shared memory, with those of memory; what is in code space is rotated by Pi.
 //   An infinity or a NaN among the values spoils sums of rows that do not see it (0 * inf), and those of its low parts: a warp whose
 // sums are not all finite does its tiles again, term by term.
 //   What bounds it: latencies of one thing after the other.  64 sequences with windows of up to 500 tokens, 8 KV heads of 8 rows, ten
@@ -77,6 +78,7 @@ TQ_DEV void aw_parts(float x, float y, uint32_t& hi, uint32_t& lo) {
 
 template <bool BF>
 __global__ void __launch_bounds__(AW_THREADS, 3) attend_window_kernel(AttendArgs a, int row_tiles, int tile, int blocks_tile) {
+  constexpr float LIFT = BF ? 0.0f : 14.0f;  // float16: probabilities are 2^14 at most, and small ones keep their digits
   extern __shared__ __align__(16) uint8_t aw_shared[];
   AwShared& sh = *(AwShared*)aw_shared;
   const tq_geom& g = a.g;
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(AW_THREADS, 3) attend_window_kernel(AttendArgs
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       top = fmaxf(top, m[x]);
-      const float by = top > -INFINITY ? top : 0.0f;
+      const float by = top > -INFINITY ? top : 0.0f, low = by - LIFT;
       down[x] = tq_exp2(m[x] - by);
       m[x] = top;
       l[x] *= down[x];
@@ -177,7 +179,7 @@ __global__ void __launch_bounds__(AW_THREADS, 3) attend_window_kernel(AttendArgs
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          const float p = tq_exp2(sc[i][2 * x + y] - by);
+          const float p = tq_exp2(sc[i][2 * x + y] - low);
           sc[i][2 * x + y] = p;
           l[x] += p;
         }
@@ -251,7 +253,7 @@ __global__ void __launch_bounds__(AW_THREADS, 3) attend_window_kernel(AttendArgs
     for (int x = 0; x < 2; ++x) {
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      if (c == 0) sh.m[warp][r + 8 * x] = m[x], sh.l[warp][r + 8 * x] = l[x];
+      if (c == 0) sh.m[warp][r + 8 * x] = m[x] - LIFT, sh.l[warp][r + 8 * x] = l[x];
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         *(float2*)&sums[(r + 8 * x) * (TQ_D + 4) + 8 * i + 2 * c] = make_float2(acc[i][2 * x], acc[i][2 * x + 1]);
