@@ -206,27 +206,33 @@ struct ArWork {
   TQ_DEV int items() const { return strip.count() + hot.count(); }
   TQ_DEV int cost(int of_strip, int of_hot) const { return of_strip * strip.count() + of_hot * hot.count(); }
 };
-// LIST: as many strips as a list can have, whether it has them or not, for every query token and head alike.
-template <bool LIST>
+// What a call is: AR_LISTS, blocks that differ by query token and KV head; AR_BEGINNING, either part of one with a shared beginning that
+// is not done as others are (queries behind all tokens, or the window done elsewhere).  Instances of their own: with what they take in
+// it the others' kernel spilled 72 bytes more, and 24 ragged float16 sequences took 82 us instead of 79.
+enum ArKind { AR_PLAIN, AR_LISTS, AR_BEGINNING };
+// AR_LISTS: as many strips as a list can have, whether it has them or not, for every query token and head alike.
+template <ArKind KIND>
 TQ_DEV ArWork ar_work(const AttendArgs& a, int n, int q_n) {
   ArWork w;
   w.cold = n_cold_blocks(n, a.g.hot_window, AR_S) * AR_S;
-  const int p_lo = a.whole ? n : n - q_n, p_hi = q_n > 0 ? (a.whole ? n + q_n : n) - 1 : -1;
-  w.strip = LIST ? AttendTiles{0, 0, p_hi >= 0 ? min(a.n_list, w.cold / AR_S) * (AR_S / AR_STRIP) : 0}
-                 : attend_tiles(a, 0, w.cold, AR_STRIP, p_lo, p_hi);
-  w.hot = a.no_window ? AttendTiles{0, 0, 0} : attend_tiles(a, w.cold, n, AR_HOT, p_lo, p_hi);
+  const bool whole = KIND == AR_BEGINNING && a.whole, no_window = KIND != AR_PLAIN && a.no_window;
+  const int p_lo = whole ? n : n - q_n, p_hi = q_n > 0 ? (whole ? n + q_n : n) - 1 : -1;
+  w.strip = KIND == AR_LISTS ? AttendTiles{0, 0, p_hi >= 0 ? min(a.n_list, w.cold / AR_S) * (AR_S / AR_STRIP) : 0}
+                             : attend_tiles(a, 0, w.cold, AR_STRIP, p_lo, p_hi);
+  w.hot = no_window ? AttendTiles{0, 0, 0} : attend_tiles(a, w.cold, n, AR_HOT, p_lo, p_hi);
   return w;
 }
 // row tiles of a sequence that have query tokens
-// (LIST: a tile has rows of one query token alone)
-template <bool LIST>
+// (AR_LISTS: a tile has rows of one query token alone)
+template <ArKind KIND>
 TQ_DEV int ar_tiles(const AttendArgs& a, int q_n, int n) {
-  return LIST ? q_n * ((a.g.group + n - 1) / n) : (q_n * a.g.group + n - 1) / n;
+  return KIND == AR_LISTS ? q_n * ((a.g.group + n - 1) / n) : (q_n * a.g.group + n - 1) / n;
 }
 
-template <bool SPLIT, int VB, bool LIST>
+template <bool SPLIT, int VB, ArKind KIND>
 __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows_kernel(AttendArgs a) {
   using Sh = ArShape<SPLIT, VB>;
+  constexpr bool LIST = KIND == AR_LISTS;
   constexpr int N = Sh::N, WARPS = Sh::WARPS, THREADS = 32 * WARPS, COST = ar_cost(SPLIT);
   constexpr int VGB = TQ_GROUP_TOK * TQ_D * VB / 8;
   extern __shared__ __align__(128) uint8_t ar_shared[];
@@ -254,8 +260,8 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
       if (s < a.seq_count) {
         const AttendSeq sq = attend_seq(a, s);
         sh.seq[s] = make_int2(sq.n, sq.q_n);
-        const ArWork w = ar_work<LIST>(a, sq.n, sq.q_n);
-        cost[i] = (int64_t)w.cost(COST, a.hot_cost) * (H * ar_tiles<LIST>(a, sq.q_n, N));
+        const ArWork w = ar_work<KIND>(a, sq.n, sq.q_n);
+        cost[i] = (int64_t)w.cost(COST, a.hot_cost) * (H * ar_tiles<KIND>(a, sq.q_n, N));
         most_strip = max(most_strip, w.strip.count());
         most_hot = max(most_hot, w.hot.count());
       }
@@ -286,14 +292,14 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   const int64_t total = sh.cum[AR_SEQS];
   int64_t share = max((total + workers - 1) / workers, (int64_t)COST);
   share = max(share, (int64_t)((COST * sh.most[0] + a.ns_cold - 3) / (a.ns_cold - 2)));
-  if (a.ns_hot > 0) share = max(share, (int64_t)((a.hot_cost * sh.most[1] + a.ns_hot - 3) / (a.ns_hot - 2)));
+  if (KIND == AR_PLAIN || a.ns_hot > 0) share = max(share, (int64_t)((a.hot_cost * sh.most[1] + a.ns_hot - 3) / (a.ns_hot - 2)));
   if (blockIdx.x == 0) {
     ArPlan* plan = (ArPlan*)a.plan;
     if (tid == 0) plan->share = share;
     for (int i = tid; i <= AR_SEQS; i += THREADS) plan->cum[i] = sh.cum[i];
     for (int i = tid; i < a.seq_count; i += THREADS) {
-      const ArWork w = ar_work<LIST>(a, sh.seq[i].x, sh.seq[i].y);
-      plan->seq[i] = make_int4(w.strip.count(), w.hot.count(), ar_tiles<LIST>(a, sh.seq[i].y, N), 0);
+      const ArWork w = ar_work<KIND>(a, sh.seq[i].x, sh.seq[i].y);
+      plan->seq[i] = make_int4(w.strip.count(), w.hot.count(), ar_tiles<KIND>(a, sh.seq[i].y, N), 0);
     }
   }
   // (neighbouring shares go to different SMs: where there are few, each has one to itself)
@@ -308,10 +314,10 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
   int s = 0, head = 0, rt = 0, it = 0, row_items = 0, row_strips = 0, row_tiles = 1;
   ArWork w;
   auto enter_seq = [&]() {
-    w = ar_work<LIST>(a, sh.seq[s].x, sh.seq[s].y);
+    w = ar_work<KIND>(a, sh.seq[s].x, sh.seq[s].y);
     row_strips = w.strip.count();
     row_items = w.items();
-    row_tiles = ar_tiles<LIST>(a, sh.seq[s].y, N);
+    row_tiles = ar_tiles<KIND>(a, sh.seq[s].y, N);
   };
   int64_t begin = 0;  // the cost of what is before this row
   if (more) {
@@ -460,7 +466,7 @@ __global__ void __launch_bounds__(32 * ArShape<SPLIT, VB>::WARPS, 1) attend_rows
     }
   };
   auto start_row = [&]() {
-    const int n = sh.seq[s].x, q_n = sh.seq[s].y, first = a.whole ? n : n - q_n;
+    const int n = sh.seq[s].x, q_n = sh.seq[s].y, first = KIND == AR_BEGINNING && a.whole ? n : n - q_n;
     const int last = min(min(row0 + N, rows_end()), q_n * G) - 1;
     p_lo = first + row0 / G;
     p_hi = last >= row0 ? first + last / G : -1;
@@ -1481,16 +1487,16 @@ __global__ void __launch_bounds__(AM_THREADS, 1) attend_rows_merge_kernel(Attend
   }
 }
 
-template <bool SPLIT, int VB, bool LIST>
+template <bool SPLIT, int VB, ArKind KIND>
 int launch_rows(const AttendArgs& a, cudaStream_t st) {
   using Shared = ArShared<SPLIT, VB>;
   static_assert(sizeof(Shared) <= 227 * 1024, "shared memory of one CTA");
   const int64_t all = (int64_t)a.seq_count * a.g.n_kv_heads * a.rows;
   TQ_REQUIRE(all <= INT_MAX - 4 * AC_THREADS, TQ_ERR_UNSUPPORTED, "too many query rows in a call");
   static bool done[64];
-  const int rc = attend_shared(attend_rows_kernel<SPLIT, VB, LIST>, sizeof(Shared), a.device, done);
+  const int rc = attend_shared(attend_rows_kernel<SPLIT, VB, KIND>, sizeof(Shared), a.device, done);
   if (rc != TQ_OK) return rc;
-  attend_rows_kernel<SPLIT, VB, LIST><<<a.sm_count, 32 * ArShape<SPLIT, VB>::WARPS, sizeof(Shared), st>>>(a);
+  attend_rows_kernel<SPLIT, VB, KIND><<<a.sm_count, 32 * ArShape<SPLIT, VB>::WARPS, sizeof(Shared), st>>>(a);
   TQ_CUDA(cudaGetLastError());
   if (a.no_window) return TQ_OK;  // (the merge is another's)
   cudaLaunchConfig_t cfg = {};
@@ -1556,12 +1562,12 @@ AttendRowsPlan tq_attend_rows_plan(const AttendArgs& a, int tokens) {
   return p;
 }
 
-template <bool LIST>
+template <ArKind KIND>
 static int launch_form(const AttendArgs& a, cudaStream_t st) {
-  if (a.q_dtype == TQ_BF16) return a.g.value_bits == 4 ? launch_rows<false, 4, LIST>(a, st) : launch_rows<false, 3, LIST>(a, st);
-  return a.g.value_bits == 4 ? launch_rows<true, 4, LIST>(a, st) : launch_rows<true, 3, LIST>(a, st);
+  if (a.q_dtype == TQ_BF16) return a.g.value_bits == 4 ? launch_rows<false, 4, KIND>(a, st) : launch_rows<false, 3, KIND>(a, st);
+  return a.g.value_bits == 4 ? launch_rows<true, 4, KIND>(a, st) : launch_rows<true, 3, KIND>(a, st);
 }
 
 int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st) {
-  return a.listed ? launch_form<true>(a, st) : launch_form<false>(a, st);
+  return a.listed ? launch_form<AR_LISTS>(a, st) : a.whole || a.no_window ? launch_form<AR_BEGINNING>(a, st) : launch_form<AR_PLAIN>(a, st);
 }
