@@ -115,6 +115,10 @@ Form choose(const tq_ctx* ctx, const Call* r, int n) {
     const double w = (double)std::min(n, g.hot_window) * r->seq_count * g.n_kv_heads * r->n_tokens * ((g.group + 7) / 8) / 1000.0;
     return !blocks ? GENERAL : window && (r->q_dtype == TQ_F16 ? 0.165 : 0.085) * w > 14.0 ? WINDOW : ROWS;
   }
+  // A shared beginning: SHARED, however many rows.  SHARED and TILES, the whole call, us, 8 KV heads of 4, by rows a head: bfloat16 on
+  // 8192 tokens 256 rows 53 and 129, 1280 145 and 208, 2048 243 and 237, 4096 526 and 383, 32768 2942 and 1673; on 2000 tokens 2048
+  // 120 and 170, 4096 297 and 273; on 32768 768 217 and 270, 2048 510 and 496, 4096 1080 and 848; float16 on 8192 512 119 and 173, 1280
+  // 269 and 253, 4096 858 and 470.  So prompts behind a beginning, from some 2000 rows a head on (float16: 1000), wait for a rule.
   if (r->whole && blocks && r->q_dtype != TQ_F32) return SHARED;
   // (and the merge of its states with few rows: a window of their type, and what blocks the sequences have by the rows form)
   if (r->merges && blocks && rows <= 64 && window) return WINDOW;

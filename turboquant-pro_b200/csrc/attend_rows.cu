@@ -22,8 +22,8 @@
 // SPLIT (float32 and float16 queries): the table's entries are hi + lo pairs too, hi * hi of 16 channels is added
 // up in float32 registers, and outliers count with their exact stored value: as exact as float32 arithmetic.
 // bfloat16 queries leave the table's lo part out (2^-11 of a level at worst, against the half step of their own type, 2^-8),
-// and take the outliers from the page's list by token, which holds their distance from the grid in fp16: 1.7 to 1.8e-3 off
-// (2-norms, 64 bits), where rounding the exact result gives 1.65e-3.
+// and take the outliers from the page's list by token, which holds their distance from the grid in fp16: 1.6 to 1.95e-3 off
+// (2-norms, 64 bits), a tenth more at most than rounding the exact result (1.57 to 1.75e-3: the spread is that of calls with few rows).
 //
 // The uncompressed window: 16-bit rows are the A operand as they are, in their own type (ldmatrix), so that only the
 // other operand is split: a query that is exact in that type has one part, others as many as they need;
@@ -33,10 +33,11 @@
 // whose scores are no numbers.
 //
 // Bound by look-ups, products and their latencies at twelve warps an SM: 44 % of the issue slots (29 % and 22 % with pairs, at
-// eight warps), a tenth of the waiting for instructions (a fifth for float32 windows: the code of all formats is
-// long); at one row tile the codes are read once.  Measured, 8 KV
-// heads, one token: 16 sequences of 8192 with a window of 4096 72.5 us, of these the merge's tail 10; 8 sequences of
-// 8000 and five tokens, three row tiles, 100 us; one sequence, window 1024, 19 us, a chain of latencies.
+// eight warps, on short windows; 46 % on 32 listed blocks a row tile, where a scheduler's two warps have 4.4 cycles between
+// instructions), a tenth of the waiting for instructions (a fifth for float32 windows: the code of all formats is long); at one
+// row tile the codes are read once.  Measured, 8 KV heads, one token: 16 sequences of 8192 with a window of 4096 72.5 us, of
+// these the merge's tail 10; 8 sequences of 8000 and five tokens, three row tiles, 100 us; one sequence, window 1024, 19 us, a
+// chain of latencies.
 #include <algorithm>
 
 #include "attend.cuh"
@@ -206,9 +207,9 @@ struct ArWork {
   TQ_DEV int items() const { return strip.count() + hot.count(); }
   TQ_DEV int cost(int of_strip, int of_hot) const { return of_strip * strip.count() + of_hot * hot.count(); }
 };
-// What a call is: AR_LISTS, blocks that differ by query token and KV head; AR_BEGINNING, either part of one with a shared beginning that
-// is not done as others are (queries behind all tokens, or the window done elsewhere).  Instances of their own: with what they take in
-// it the others' kernel spilled 72 bytes more, and 24 ragged float16 sequences took 82 us instead of 79.
+// What a call is: AR_LISTS, blocks that differ by query token and KV head; AR_BEGINNING, a part of one with a shared beginning that is
+// not done as others are (queries behind all tokens, or the window done elsewhere).  Instances of their own: with what these take
+// in it the kernel of plain calls spilled 72 bytes more, and 24 ragged float16 sequences took 82 us instead of 79.
 enum ArKind { AR_PLAIN, AR_LISTS, AR_BEGINNING };
 // AR_LISTS: as many strips as a list can have, whether it has them or not, for every query token and head alike.
 template <ArKind KIND>
@@ -1569,5 +1570,6 @@ static int launch_form(const AttendArgs& a, cudaStream_t st) {
 }
 
 int tq_launch_attend_rows(const AttendArgs& a, cudaStream_t st) {
-  return a.listed ? launch_form<AR_LISTS>(a, st) : a.whole || a.no_window ? launch_form<AR_BEGINNING>(a, st) : launch_form<AR_PLAIN>(a, st);
+  if (a.listed) return launch_form<AR_LISTS>(a, st);
+  return a.whole || a.no_window ? launch_form<AR_BEGINNING>(a, st) : launch_form<AR_PLAIN>(a, st);
 }

@@ -20,7 +20,7 @@
 //     What bounds it: 64 tokens take 3000 cycles for 256 rows (32768 tokens, 8 heads of 512 rows: 130 us, 0.53 PFLOP/s; 8192 and 128
 //     rows 33 us; float16, 12345 tokens, 4 heads of 231 rows: 40).  The makers are busy for 2000 of them, the exponentials of
 //     the two halves for 1150 each, the products for 1090, and a ring of three stages, for which there is shared memory, ties
-//     them together; 48 % of the issue slots are used.  Exponentials of both halves at once, or more of them on the
+//     them together; 49 % of the issue slots are used (58 % of those of cycles in which an SM has work).  Exponentials of both halves at once, or more of them on the
 //     multiply-add units, measured the same.  Why 256 rows: codes are decoded once for all of a CTA's rows, and
 //     tensor memory holds two halves' scores, probabilities and sums.
 // attend_shared_merge_kernel   for other forms of the sequences' own tokens than few rows: merges a row's states in order,
@@ -69,8 +69,8 @@ struct PxShared {
   float2 of_tile[Sh::STAGES];                // the values' exponent, the keys' factor
   float top[2][8];
   float k_up;                                // the factor of the CTA's keys
-  unsigned long long on_grid[Sh::STAGES], k_full[Sh::STAGES], v_full[Sh::STAGES], empty[Sh::STAGES], q_ready[2], s_full[2], s_read[2], p_full[2],
-      o_done[2], drained[2];
+  unsigned long long on_grid[Sh::STAGES], k_full[Sh::STAGES], v_full[Sh::STAGES], empty[Sh::STAGES];
+  unsigned long long q_ready[2], s_full[2], s_read[2], p_full[2], o_done[2], drained[2];
   uint32_t tmem;
 };
 
@@ -155,7 +155,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
     const uint32_t to = enc_smem(sh.q[warp >> 2] + (tid & 127) * 16);
 #pragma unroll 2
     for (int i = 0; i < 16; ++i)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * PX_LBO), "l"(q + 8 * i), "r"(there ? 16 : 0) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * PX_LBO), "l"(q + 8 * i), "r"(there ? 16 : 0)
+                   : "memory");
     asm volatile("cp.async.wait_all;" ::: "memory");  // (each thread its own row)
   } else if (warp >= PX_SOFTMAX / 32 && warp < (PX_SOFTMAX + PX_ISSUE) / 32) {
     const int d = tid - PX_SOFTMAX;
@@ -176,7 +177,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
       const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        f[j] = SPLIT ? __half22float2(*(const __half2*)&u[j]) : make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u));
+        f[j] = SPLIT ? __half22float2(*(const __half2*)&u[j])
+                     : make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u));
     };
     float top = 0.0f;
     uint64_t part[2] = {0ull, 0ull};
@@ -332,7 +334,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
         const float gridmost = g.key_mode == TQ_KEYS_UNIFORM ? 15.0f : 1.0f;
         const float4 z4 = *(const float4*)&sh.center[4 * lane];
         for (int j = (k_lo & ~3) + 4 * pw; j < k_lo + n; j += 4 * (PX_MAKERS / 32)) {
-          const float4 s4 = *(const float4*)(page_of(j) + g.scale_off + lane * 16), m4 = *(const float4*)(page_of(j) + g.mean_off + lane * 16);
+          const float4 s4 = *(const float4*)(page_of(j) + g.scale_off + lane * 16);
+          const float4 m4 = *(const float4*)(page_of(j) + g.mean_off + lane * 16);
           const float s[4] = {s4.x, s4.y, s4.z, s4.w}, m[4] = {m4.x - z4.x, m4.y - z4.y, m4.z - z4.z, m4.w - z4.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -487,7 +490,10 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
         const size_t row = ring + (size_t)(t % g.hot_cap) * TQ_D, at = row + 32 * quarter;
         const bool there = t < sq.n;
         float x[4][8], most = 0.0f, exponent, k_exponent, of_wide[2] = {0.0f, 0.0f};
-        if (!SPLIT && there) of_wide[0] = attend_ld(a.hot_k, row + wide0, g.kv_dtype), of_wide[1] = attend_ld(a.hot_k, row + wide1, g.kv_dtype);
+        if (!SPLIT && there) {
+          of_wide[0] = attend_ld(a.hot_k, row + wide0, g.kv_dtype);
+          of_wide[1] = attend_ld(a.hot_k, row + wide1, g.kv_dtype);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (there) ti_ld8(a.hot_k, at + 8 * i, g.kv_dtype, x[i]);
@@ -637,7 +643,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1) attend_shared_kernel(AttendArgs
       const uint64_t q_wide = umma_desc_k_major(enc_smem(sh.q_wide[0]), PX_QWLBO, PX_SBO) + (uint64_t)(x * (PX_QWIMAGE >> 4));
       const uint64_t k_wide = umma_desc_k_major(enc_smem(sh.wide[0]), PX_WLBO, PX_SBO);
       const uint32_t ds = tmem + PX_HALF * x, dp = tmem + PX_P + PX_HALF * x, d_o = tmem + PX_O + 128 * x;
-      auto image = [&](int k, int part) { return (uint64_t)((uint32_t)(k % STAGES) * (2 * PARTS * PX_IMAGE >> 4) + part * (PX_IMAGE >> 4)); };
+      auto image = [&](int k, int part) {
+        return (uint64_t)((uint32_t)(k % STAGES) * (2 * PARTS * PX_IMAGE >> 4) + part * (PX_IMAGE >> 4));
+      };
       auto wait_all = [&](unsigned long long* bar, unsigned parity) {  // (the warp stays together)
         wait(bar, parity);
         gave_up = __any_sync(0xffffffffu, gave_up);

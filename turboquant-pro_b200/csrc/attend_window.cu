@@ -120,7 +120,8 @@ __global__ void __launch_bounds__(AW_THREADS, 3) attend_window_kernel(AttendArgs
     const int row = row0 + r + 8 * x;
     const bool there = r + 8 * x < rows;
     pos[x] = there ? attend_position(a, sq, row) : -1;
-    q_at[x] = (const uint16_t*)a.q + (there ? (int64_t)s * a.q_seq + (int64_t)(row / G) * a.q_tok + (int64_t)(head * G + row % G) * a.q_head : 0);
+    q_at[x] = (const uint16_t*)a.q;
+    if (there) q_at[x] += (int64_t)s * a.q_seq + (int64_t)(row / G) * a.q_tok + (int64_t)(head * G + row % G) * a.q_head;
 #pragma unroll
     for (int k = 0; k < 8; ++k)
 #pragma unroll
@@ -233,7 +234,8 @@ __global__ void __launch_bounds__(AW_THREADS, 3) attend_window_kernel(AttendArgs
           float dot = 0.0f;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            dot = fmaf(attend_ld(a.q, (size_t)(at + lane + 32 * i), a.q_dtype), attend_ld(a.hot_k, from + lane + 32 * i, g.kv_dtype), dot);
+            dot = fmaf(attend_ld(a.q, (size_t)(at + lane + 32 * i), a.q_dtype),
+                       attend_ld(a.hot_k, from + lane + 32 * i, g.kv_dtype), dot);
 #pragma unroll
           for (int d = 16; d >= 1; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
           dot = tq_scaled<true>(dot);
